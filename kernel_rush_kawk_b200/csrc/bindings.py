@@ -20,28 +20,16 @@ from ctypes import c_float, c_int, c_longlong, c_uint, c_void_p
 import torch
 
 from .build import build_library
+from .cache_ops import BF16, F32, CacheOps, KernelError, _code, _load, _ptr  # noqa: F401
 
-F32, BF16 = 0, 1
 _P = c_void_p
-
-
-def _code(dtype: torch.dtype) -> int:
-    if dtype == torch.float32:
-        return F32
-    if dtype == torch.bfloat16:
-        return BF16
-    raise TypeError(f"kernels take float32 or bfloat16 tensors, got {dtype}")
-
-
-class KernelError(RuntimeError):
-    pass
 
 
 _SIGNATURES = {
     "krk_rmsnorm": [_P, _P, _P, _P, _P, c_int, c_int, c_int, c_float, c_int, _P],
     "krk_gather_rows": [_P, _P, _P, c_int, c_int, c_int, _P, c_int, _P],
     "krk_swiglu": [_P, _P, c_int, c_int, c_int, _P],
-    "krk_qk_norm_rope_write": [_P, _P, _P, c_int, _P, _P, _P, _P, _P, _P, c_int, _P, _P, c_int, c_int, c_int, c_int,
+    "krk_qk_norm_rope_write": [_P, _P, _P, c_int, _P, _P, _P, _P, _P, _P, _P, c_int, _P, _P, c_int, c_int, c_int, c_int,
                                c_int, c_float, c_int, _P, c_int, _P],
     "krk_gemm_nt": [_P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P, _P],
     "krk_selftest_wait_for_copies": [_P, _P, c_int, c_int, c_int, _P, c_int, _P],
@@ -158,26 +146,10 @@ _ATTN_SIGNATURES = {
 }
 
 
-def _load(path, signatures) -> ctypes.CDLL:
-    lib = ctypes.CDLL(str(path))
-    for name, args in signatures.items():
-        try:
-            fn = getattr(lib, name)
-        except AttributeError:
-            continue
-        fn.argtypes = args
-        fn.restype = c_int
-    return lib
-
-
-def _ptr(t) -> int | None:
-    return None if t is None else t.data_ptr()
-
-
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-class Kernels:
+class Kernels(CacheOps):
     """All kernels, for one device. ``head_dims``: the head sizes whose attention
     libraries are needed (compiled at first use)."""
 
@@ -191,6 +163,8 @@ class Kernels:
         self._mix = self._scan = self._moe = self._memory = None
         self.attn: dict[int, ctypes.CDLL] = {}
         self.latent: dict[tuple, ctypes.CDLL] = {}
+        self.parts: dict[int, ctypes.CDLL] = {}
+        self._cache_lib = None
         for d in head_dims:
             self._attn_lib(int(d))
         self.error = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -421,8 +395,8 @@ class Kernels:
         rot = self._rotated_width(cos, head_dim)
         self._ok(self.core.krk_qk_norm_rope_write(
             qkv.data_ptr(), _ptr(q_gain), _ptr(k_gain), int(gain is not None and gain.dtype == torch.float32),
-            _ptr(cos), _ptr(sin), batch.row_seq.data_ptr(), batch.row_pos.data_ptr(), batch.seq_slot.data_ptr(),
-            cache.table.data_ptr(), cache.width, cache.k.data_ptr() if kv_in_row else None,
+            _ptr(cos), _ptr(sin), batch.row_seq.data_ptr(), batch.row_pos.data_ptr(), _ptr(getattr(batch, "seq_shift", None)),
+            batch.seq_slot.data_ptr(), cache.table.data_ptr(), cache.width, cache.k.data_ptr() if kv_in_row else None,
             cache.v.data_ptr() if kv_in_row else None, qkv.shape[0], heads, kv_in_row, head_dim, rot, eps, n_pos,
             self.error.data_ptr(), _code(qkv.dtype), self._stream()), "q/k norm + rope + cache write")
 

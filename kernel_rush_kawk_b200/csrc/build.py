@@ -5,10 +5,11 @@ Kinds of library: ``core`` (kernels whose sizes are run-time arguments),
 ``-DKRK_HEAD_DIM=D``, so a model compiles only the head size it has), ``mix``
 (the kernels of models with a 32-bit residual stream, windowed attention with a
 sink or over latent rows), ``scan`` (recurrent state), ``memory`` (matrix states
-without a removal term) and ``moe`` (routed
-experts); each of the last four is compiled and loaded when a model first calls
+without a removal term), ``moe`` (routed
+experts) and ``cache`` (eviction); each of the last five is compiled and loaded when a model first calls
 one of its kernels, so a model compiles what it needs; ``latent_k<D>_v<P>`` (prompt
-attention over keys and values made from latent rows, per pair of sizes, likewise). A library
+attention over keys and values made from latent rows, per pair of sizes) and ``parts_d<D>`` (attention
+in parts: shared prefixes, weights per key) likewise. A library
 is rebuilt when a source or a flag changes (its name carries a hash of both) and
 is otherwise loaded as it is. Libraries live in ``csrc/_build`` inside the
 package when that is writable, else under ``$KRK_BUILD_DIR`` or a per-user
@@ -38,10 +39,12 @@ MIX_SOURCES = ["wide_rows.cu", "sink_attention.cu", "latent.cu", "hyper.cu", "mi
 SCAN_SOURCES = ["recurrent.cu", "recurrent_chunks.cu", "ssd.cu"]
 MEMORY_SOURCES = ["matrix_memory.cu", "matrix_memory_chunks.cu", "matrix_memory_step.cu"]
 MOE_SOURCES = ["routed.cu", "few_experts.cu", "grouped_gemm.cu"]
-SMALL_LIBRARIES = {"mix": MIX_SOURCES, "scan": SCAN_SOURCES, "memory": MEMORY_SOURCES, "moe": MOE_SOURCES}
+CACHE_SOURCES = ["evict.cu"]
+SMALL_LIBRARIES = {"mix": MIX_SOURCES, "scan": SCAN_SOURCES, "memory": MEMORY_SOURCES, "moe": MOE_SOURCES, "cache": CACHE_SOURCES}
+PARTS_SOURCES = ["partial_attention.cu"]
 LATENT_SOURCES = ["latent_prefill.cu"]
 ATTN_SOURCES = ["attention_simple.cu", "attention_mma.cu", "attention_tcgen05.cu"]
-HEADERS = ["common.cuh", "mma.cuh", "tcgen05.cuh", "attention_noalloc.h"]
+HEADERS = ["common.cuh", "mma.cuh", "tcgen05.cuh", "attention_noalloc.h", "partial_attention.cuh"]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
@@ -108,6 +111,9 @@ def library_path(kind: str, head_dim=None) -> tuple[Path, list, list]:
     elif kind in SMALL_LIBRARIES:
         sources, defines, stem = _existing(SMALL_LIBRARIES[kind]), [], f"libkrk_{kind}"
         return build_dir() / f"{stem}_{_key(sources, defines, [])}.so", sources, defines
+    elif kind == "parts":
+        sources, defines = _existing(PARTS_SOURCES), [f"-DKRK_HEAD_DIM={int(head_dim)}"]
+        return build_dir() / f"libkrk_parts_d{int(head_dim)}_{_key(sources, defines, [])}.so", sources, defines
     else:
         sources, defines, stem = _existing(ATTN_SOURCES), [f"-DKRK_HEAD_DIM={int(head_dim)}"], f"libkrk_attn_d{int(head_dim)}"
     return build_dir() / f"{stem}_{_key(sources, defines)}.so", sources, defines
@@ -174,11 +180,12 @@ def build_library(kind: str, head_dim=None, verbose: bool = True) -> Path:
 
 
 def build_all(head_dims=(16, 32, 64, 128), verbose: bool = True, latent_dims=((192, 128),)) -> list[Path]:
-    """Compile the core library, the attention library of every given head size and the latent library of every given
+    """Compile the core library, the two attention libraries of every given head size and the latent library of every given
     pair of sizes."""
     out = [build_library("core", verbose=verbose)] + [build_library(kind, verbose=verbose) for kind in SMALL_LIBRARIES]
     for d in head_dims:
         out.append(build_library("attn", d, verbose=verbose))
+        out.append(build_library("parts", d, verbose=verbose))
     for pair in latent_dims:
         out.append(build_library("latent", pair, verbose=verbose))
     return out

@@ -1,0 +1,239 @@
+"""Python bindings of the kernels that share and thin out the cache: attention behind a prefix that several sequences hold
+in the same pages, attention that adds up the weight which each cached key receives, and the eviction of the keys that
+received least. ``Kernels`` (bindings.py) takes them in.
+
+Scratch is drawn from torch's allocator for each call, so that calls on several streams, and captured steps beside
+others, never share any.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from ctypes import c_float, c_int, c_longlong, c_void_p
+
+import torch
+
+from .build import build_library
+
+F32, BF16 = 0, 1
+_P = c_void_p
+PAGE = 64
+
+
+def _code(dtype: torch.dtype) -> int:
+    if dtype == torch.float32:
+        return F32
+    if dtype == torch.bfloat16:
+        return BF16
+    raise TypeError(f"kernels take float32 or bfloat16 tensors, got {dtype}")
+
+
+class KernelError(RuntimeError):
+    pass
+
+
+def _load(path, signatures) -> ctypes.CDLL:
+    lib = ctypes.CDLL(str(path))
+    for name, args in signatures.items():
+        try:
+            fn = getattr(lib, name)
+        except AttributeError:
+            continue
+        fn.argtypes = args
+        fn.restype = c_int
+    return lib
+
+
+def _ptr(t) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+_SEGMENTS = [_P] * 7 + [c_int, c_int, _P, c_int]
+_PARTS_SIGNATURES = {
+    "krk_partial_attention": [_P, _P, c_int, c_int, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_float, c_int, _P],
+    "krk_join_parts": [_P, _P, _P, _P, c_int, c_int, c_int, c_int, _P],
+    "krk_key_weights": [_P, _P, _P, _P, c_int, _P, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, c_int, c_float, c_int, _P],
+}
+_CACHE_SIGNATURES = {
+    "krk_evict_max_seqs": [],
+    "krk_evict_keys": [_P, _P, c_longlong, c_longlong, c_int, c_int, c_int, c_int, _P, c_int, _P, _P, _P, _P, c_longlong, c_int, _P, _P, c_int,
+                       c_int, c_int, _P, _P, c_int, _P, _P, _P, _P],
+}
+
+
+class CacheOps:
+    """Mixed into ``Kernels``."""
+
+    EVICT_SCRATCH_BYTES = 64 << 20  # the lists of moves of one pair of launches; more sequences take several pairs
+
+    def _parts_lib(self, head_dim: int) -> ctypes.CDLL:
+        lib = self.parts.get(head_dim)
+        if lib is None:
+            if head_dim % 2 or head_dim > 256:
+                raise KernelError(f"attention kernels take an even head size up to 256, got {head_dim}")
+            lib = self.parts[head_dim] = _load(build_library("parts", head_dim), _PARTS_SIGNATURES)
+        return lib
+
+    @property
+    def cache_lib(self) -> ctypes.CDLL:
+        if self._cache_lib is None:
+            self._cache_lib = _load(build_library("cache"), _CACHE_SIGNATURES)
+        return self._cache_lib
+
+    # -- what both attentions ask of their arguments ---------------------------------
+    def _check_step(self, what, qkv, heads, kv_in_row, head_dim, batch, cache):
+        if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] != (heads + 2 * kv_in_row) * head_dim:
+            raise KernelError(f"{what}: rows of {(heads + 2 * kv_in_row) * head_dim} elements side by side are asked for, got {tuple(qkv.shape)}")
+        if heads % cache.kv_heads or cache.head_dim != head_dim or cache.v_dim != head_dim:
+            raise KernelError(f"{what}: {heads} heads of {head_dim} do not fit a cache of {cache.kv_heads} heads of {cache.head_dim} (values: {cache.v_dim})")
+        if cache.window is not None or cache.keep_pages:
+            raise KernelError(f"{what}: the cache keeps a window of keys; every key is asked for")
+        if cache.k.dtype != qkv.dtype or cache.v.dtype != qkv.dtype or not cache.k.is_contiguous() or not cache.v.is_contiguous():
+            raise KernelError(f"{what}: the cache's pages are contiguous and of the rows' dtype ({qkv.dtype}), got {cache.k.dtype}")
+        if qkv.shape[0] != batch.n_rows:
+            raise KernelError(f"{what}: {qkv.shape[0]} rows for a step of {batch.n_rows}")
+        if not qkv.device == cache.k.device == self.error.device:
+            raise KernelError(f"{what}: rows on {qkv.device}, pages on {cache.k.device}, kernels on {self.error.device}")
+
+    @staticmethod
+    def _segments(batch, cache, prefix):
+        groups = (None, None, None, batch.n_seqs, 0) if prefix is None else (
+            prefix.cu.data_ptr(), prefix.length.data_ptr(), prefix.group.data_ptr(), batch.n_seqs, prefix.n_groups)
+        return (batch.cu_q.data_ptr(), batch.seq_slot.data_ptr(), batch.seq_start.data_ptr(), batch.seq_qlen.data_ptr(), *groups,
+                cache.table.data_ptr(), cache.width)
+
+    @staticmethod
+    def _splits(blocks: int, most: int = 32) -> int:
+        """Parts that the keys of a unit of work are split into, so that the blocks fill the device three times over. By the numbers of rows
+        and heads, never by lengths: a captured step stays valid."""
+        return max(1, min(most, -(-444 // max(blocks, 1))))
+
+    def _attention_in_parts(self, qkv, heads, head_dim, batch, cache, scale, prefix, want_lse):
+        """(output, log2 of every row's sum of 2^score or None)."""
+        lib = self._parts_lib(head_dim)
+        rows, kv = qkv.shape[0], cache.kv_heads
+        out = torch.empty((rows, heads * head_dim), dtype=qkv.dtype, device=qkv.device)
+        lse = torch.empty((rows, heads), dtype=torch.float32, device=qkv.device) if want_lse else None
+        if rows == 0:
+            return out, lse
+        segments = self._segments(batch, cache, prefix)
+        code, stream, stride, per = _code(qkv.dtype), self._stream(), qkv.stride(0), heads // kv
+        tiles = lambda n: -(-n * per // 16)
+        own_splits = self._splits(tiles(batch.max_q_len) * kv * batch.n_seqs)
+        prefix_splits, group_rows = 0, 0
+        if prefix is not None and prefix.max_length:
+            group_rows = prefix.max_rows(batch)
+            prefix_splits = self._splits(tiles(group_rows) * kv * prefix.n_groups)
+        parts = prefix_splits + own_splits
+        o = torch.empty((parts, rows, heads, head_dim), dtype=torch.float32, device=qkv.device)
+        ml = torch.empty((parts, rows, heads, 2), dtype=torch.float32, device=qkv.device)
+        for own, first, n, most in ((0, 0, prefix_splits, group_rows), (1, prefix_splits, own_splits, batch.max_q_len)):
+            if n:
+                self._ok(lib.krk_partial_attention(o.data_ptr(), ml.data_ptr(), rows, first, n, own, qkv.data_ptr(), stride, heads, kv, *segments,
+                                                   cache.k.data_ptr(), cache.v.data_ptr(), most, scale, code, stream), "attention in parts")
+        self._ok(lib.krk_join_parts(out.data_ptr(), _ptr(lse), o.data_ptr(), ml.data_ptr(), rows, heads, parts, code, stream), "join of parts")
+        return out, lse
+
+    # -- a shared prefix -----------------------------------------------------------------
+    def shared_prefix_attention(self, qkv, heads, kv_in_row, head_dim, batch, cache, scale, prefix):
+        """``attention`` for a step whose sequences share prefixes: [rows, heads * head_dim], every row over all keys up to its own
+        position. ``prefix`` (cache.prefix.PrefixGroups) says which neighbouring sequences of the step hold the same first positions in the
+        same pages (``SequenceCache.fork`` makes such sequences); a group's keys and values are read once for all of its rows. The step's
+        own keys and values must be in the cache already, and its rows lie behind their group's prefix. Any number of tokens a
+        sequence, float32 or bfloat16; a captured step stays valid while the groups' number and sizes last, whatever the lengths become."""
+        self._check_step("shared prefix attention", qkv, heads, kv_in_row, head_dim, batch, cache)
+        prefix.check(batch, cache)
+        return self._attention_in_parts(qkv, heads, head_dim, batch, cache, float(scale), prefix, False)[0]
+
+    # -- weights per key -------------------------------------------------------------------
+    def _check_scores(self, what, scores, positions, cache, extra=()):
+        shape = (cache.table.shape[0], cache.kv_heads, cache.width * PAGE)
+        for name, t, dtype in (("scores", scores, torch.float32), ("positions", positions, torch.int32), *extra):
+            if t is not None and (tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous() or t.device != cache.k.device):
+                raise KernelError(f"{what}: {name} are contiguous {dtype} [slots, kv heads, rows of a slot] = {list(shape)} beside the cache, "
+                                  f"got {t.dtype} {list(t.shape)}")
+
+    def scored_attention(self, qkv, heads, kv_in_row, head_dim, batch, cache, scale, scores, positions=None, observe=None, out_scores=None):
+        """``attention`` that also adds up, for every cached row, the weight it receives: ``scores`` [slots, kv heads, rows] float32 grow by
+        the softmax weights of the step's queries, summed over the heads of a kv head and over the last ``observe`` queries of each sequence
+        (None: all). Rows that the step itself brings start from its own weights; rows behind a sequence's last stay as they are.
+        ``positions`` (int32, the same shape) take the step's rows' positions in the sequence, which lie ``batch.seq_shift`` behind their
+        rows where keys were evicted. ``out_scores`` takes the sums in place of ``scores``."""
+        self._check_step("scored attention", qkv, heads, kv_in_row, head_dim, batch, cache)
+        out_scores = scores if out_scores is None else out_scores
+        self._check_scores("scored attention", scores, positions, cache, (("out_scores", out_scores, torch.float32),))
+        if observe is not None and observe < 1:
+            raise KernelError(f"scored attention: at least one query a sequence is observed, got {observe}")
+        out, lse = self._attention_in_parts(qkv, heads, head_dim, batch, cache, float(scale), None, True)
+        if qkv.shape[0]:
+            kv = cache.kv_heads
+            blocks = max(1, min(cache.width, -(-888 // (kv * batch.n_seqs))))
+            self._ok(self._parts_lib(head_dim).krk_key_weights(
+                scores.data_ptr(), out_scores.data_ptr(), _ptr(positions), _ptr(getattr(batch, "seq_shift", None)), scores.shape[2], lse.data_ptr(),
+                int(observe or 0), qkv.data_ptr(), qkv.stride(0), heads, kv, *self._segments(batch, cache, None), cache.k.data_ptr(), blocks,
+                float(scale), _code(qkv.dtype), self._stream()), "weights of keys")
+        return out
+
+    # -- eviction ----------------------------------------------------------------------------
+    def evict_keys(self, k, v, table, slots, lengths, scores, positions, keep, recent, out_scores=None, out_positions=None, batch=None):
+        """Give up all but ``keep`` rows of every head of these cache slots (host lists ``slots`` and ``lengths``, the rows that each holds),
+        in every layer run at once: ``k`` and ``v`` [runs, pages, kv heads, 64, head size], ``table`` [slots, pages of a slot], ``scores`` and
+        ``positions`` [runs, slots, kv heads, rows]. The ``recent`` rows of highest position stay, of the others those of largest score
+        (ties: the lowest row; a NaN counts as the largest). What stays from row ``keep`` on moves, in place, into the rows below it that
+        are given up, in ascending order of both; scores and positions move along, or go to ``out_scores`` and ``out_positions`` (rows from
+        ``keep`` on are not written). A slot that holds no more than ``keep`` rows stays as it is. ``batch``: the description of a
+        single-token step of exactly these slots, whose rows and shifts follow on the device. Returns the rows held now, as a list."""
+        slots, lengths = [int(s) for s in slots], [int(n) for n in lengths]
+        keep, recent = int(keep), int(recent)
+        what = "eviction"
+        if k.dim() != 5 or v.dim() != 5 or k.shape[:4] != v.shape[:4] or k.shape[3] != PAGE or k.dtype != v.dtype:
+            raise KernelError(f"{what}: pages are [runs, pages, kv heads, {PAGE}, head size], got {list(k.shape)} and {list(v.shape)}")
+        _code(k.dtype)
+        if any(t.shape[0] and not t[0].is_contiguous() for t in (k, v)) or not table.is_contiguous() or table.dtype != torch.int32:
+            raise KernelError(f"{what}: every run's pages and the page table (int32) are contiguous")
+        out_scores = scores if out_scores is None else out_scores
+        out_positions = positions if out_positions is None else out_positions
+        shape = (k.shape[0], table.shape[0], k.shape[2], table.shape[1] * PAGE)
+        for name, t, dtype in (("scores", scores, torch.float32), ("positions", positions, torch.int32),
+                               ("out_scores", out_scores, torch.float32), ("out_positions", out_positions, torch.int32)):
+            if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
+                raise KernelError(f"{what}: {name} are contiguous {dtype} [runs, slots, kv heads, rows of a slot] = {list(shape)}, got {t.dtype} {list(t.shape)}")
+        if any(t.device != self.error.device for t in (k, v, table, scores, positions, out_scores, out_positions)):
+            raise KernelError(f"{what}: every tensor lies on the kernels' device, {self.error.device}")
+        if keep < 1 or not 0 <= recent <= keep:
+            raise KernelError(f"{what}: at least one row stays, and at most as many by their position as stay in all; got keep {keep}, recent {recent}")
+        if len(slots) != len(lengths) or len(set(slots)) != len(slots):
+            raise KernelError(f"{what}: every slot comes once, with its length")
+        for s, n in zip(slots, lengths):
+            if not 0 <= s < shape[1] or not 0 <= n <= shape[3]:
+                raise KernelError(f"{what}: slot {s} of {shape[1]} with {n} rows of {shape[3]}")
+        left = [min(n, keep) for n in lengths]
+        if not slots or k.numel() == 0:
+            return left
+        if batch is not None and (batch.n_seqs != len(slots) or batch.n_rows != len(slots) or getattr(batch, "seq_shift", None) is None):
+            raise KernelError(f"{what}: the step that follows has one token of each slot and keeps shifts")
+        runs, heads = shape[0], shape[2]
+        same = v.data_ptr() == k.data_ptr()
+        size = k.element_size()
+        most = int(self.cache_lib.krk_evict_max_seqs())
+        at = 0
+        while at < len(slots):
+            # as many sequences as the arguments and the scratch take
+            n, moves = 1, max(0, min(keep, lengths[at] - keep))
+            while n < most and at + n < len(slots):
+                m = max(moves, min(keep, lengths[at + n] - keep))
+                if runs * (n + 1) * heads * m * 8 > self.EVICT_SCRATCH_BYTES:
+                    break
+                n, moves = n + 1, m
+            lists = torch.empty(runs * n * heads * (2 * moves + 1), dtype=torch.int32, device=k.device)
+            counts = lists[runs * n * heads * 2 * moves:]
+            ints = c_int * n
+            follow = (None, None, None) if batch is None else tuple(t[at:].data_ptr() for t in (batch.seq_start, batch.row_pos, batch.seq_shift))
+            self._ok(self.cache_lib.krk_evict_keys(
+                k.data_ptr(), None if same else v.data_ptr(), k.stride(0) * size, v.stride(0) * size, k.shape[4] * size, v.shape[4] * size, heads, runs,
+                table.data_ptr(), table.shape[1], scores.data_ptr(), positions.data_ptr(), out_scores.data_ptr(), out_positions.data_ptr(),
+                scores.stride(0), shape[3], ints(*slots[at:at + n]), ints(*lengths[at:at + n]), n, keep, recent, lists.data_ptr(), counts.data_ptr(),
+                moves, *follow, self._stream()), what)
+            self.launches += int(moves > 0)
+            at += n
+        return left

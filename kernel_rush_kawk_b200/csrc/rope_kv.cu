@@ -20,7 +20,8 @@ template <typename T>
 __global__ void qk_norm_rope_write_kernel(T* __restrict__ qkv, const void* __restrict__ q_gain,
                                           const void* __restrict__ k_gain, int gain_f32, const T* __restrict__ cos_t,
                                           const T* __restrict__ sin_t, const int* __restrict__ row_seq,
-                                          const int* __restrict__ row_pos, const int* __restrict__ seq_slot,
+                                          const int* __restrict__ row_pos, const int* __restrict__ seq_shift,
+                                          const int* __restrict__ seq_slot,
                                           const int* __restrict__ table, int width, T* __restrict__ k_cache,
                                           T* __restrict__ v_cache, int rows, int HQ, int HKV, int D, int rot, float eps,
                                           int n_pos, int* error) {
@@ -33,7 +34,8 @@ __global__ void qk_norm_rope_write_kernel(T* __restrict__ qkv, const void* __res
   if (item >= (long long)rows * heads) return;
   const int row = (int)(item / heads);
   const int head = (int)(item % heads);
-  const int pos = row_pos[row];
+  const int place = row_pos[row];                                            // in the cache
+  const int pos = place + (seq_shift ? seq_shift[row_seq[row]] : 0);  // in the sequence
   const int half = D / 2;
   T* src = qkv + (size_t)row * heads * D + (size_t)head * D;
 
@@ -41,9 +43,9 @@ __global__ void qk_norm_rope_write_kernel(T* __restrict__ qkv, const void* __res
   if (head >= HQ) {
     const int kh = (head - HQ) % HKV;
     const int slot = seq_slot[row_seq[row]];
-    const int page = page_of(table, width, slot, pos);
+    const int page = page_of(table, width, slot, place);
     T* cache = head < HQ + HKV ? k_cache : v_cache;
-    dst = cache + (((size_t)page * HKV + kh) * KRK_PAGE + (pos % KRK_PAGE)) * D;
+    dst = cache + (((size_t)page * HKV + kh) * KRK_PAGE + (place % KRK_PAGE)) * D;
   }
   if (head >= HQ + HKV) {  // a value head: raw copy
     for (int i = lane; i < D; i += 32) dst[i] = src[i];
@@ -186,6 +188,7 @@ __global__ void qk_norm_rope_write_vec_kernel(bf16* __restrict__ qkv, const void
                                               const void* __restrict__ k_gain, int gain_f32,
                                               const bf16* __restrict__ cos_t, const bf16* __restrict__ sin_t,
                                               const int* __restrict__ row_seq, const int* __restrict__ row_pos,
+                                              const int* __restrict__ seq_shift,
                                               const int* __restrict__ seq_slot, const int* __restrict__ table, int width,
                                               bf16* __restrict__ k_cache, bf16* __restrict__ v_cache, int rows, int HQ,
                                               int HKV, int D, float eps, int n_pos, int* error) {
@@ -199,16 +202,17 @@ __global__ void qk_norm_rope_write_vec_kernel(bf16* __restrict__ qkv, const void
   const bool live = item < (long long)rows * heads;
   const int row = live ? (int)(item / heads) : 0;
   const int head = live ? (int)(item % heads) : 0;
-  const int raw_pos = row_pos[row];
-  const bool bad = raw_pos < 0 || raw_pos >= n_pos;  // flagged below; nothing is stored for such a row
-  const int pos = bad ? 0 : raw_pos;
+  const int raw_place = row_pos[row];                                                   // in the cache
+  const int raw_pos = raw_place + (seq_shift ? seq_shift[row_seq[row]] : 0);  // in the sequence
+  const bool bad = raw_place < 0 || raw_pos < 0 || raw_pos >= n_pos;  // flagged below; nothing is stored for such a row
+  const int pos = bad ? 0 : raw_pos, place = bad ? 0 : raw_place;
   bf16* src = qkv + (size_t)row * heads * D + (size_t)head * D + 8 * sub;
   bf16* dst = src;
   if (head >= HQ) {
     const int kh = (head - HQ) % HKV;
-    const int page = page_of(table, width, seq_slot[row_seq[row]], pos);
+    const int page = page_of(table, width, seq_slot[row_seq[row]], place);
     bf16* cache = head < HQ + HKV ? k_cache : v_cache;
-    dst = cache + (((size_t)page * HKV + kh) * KRK_PAGE + (pos % KRK_PAGE)) * D + 8 * sub;
+    dst = cache + (((size_t)page * HKV + kh) * KRK_PAGE + (place % KRK_PAGE)) * D + 8 * sub;
   }
   uint4 raw = make_uint4(0, 0, 0, 0);
   if (live) raw = *reinterpret_cast<const uint4*>(src);
@@ -228,7 +232,7 @@ __global__ void qk_norm_rope_write_vec_kernel(bf16* __restrict__ qkv, const void
 __global__ void __launch_bounds__(256)
 qk_norm_rope_write_row_kernel(bf16* __restrict__ qkv, const void* __restrict__ q_gain, const void* __restrict__ k_gain,
                               int gain_f32, const bf16* __restrict__ cos_t, const bf16* __restrict__ sin_t,
-                              const int* __restrict__ row_seq, const int* __restrict__ row_pos,
+                              const int* __restrict__ row_seq, const int* __restrict__ row_pos, const int* __restrict__ seq_shift,
                               const int* __restrict__ seq_slot, const int* __restrict__ table, int width,
                               bf16* __restrict__ k_cache, bf16* __restrict__ v_cache, int HQ, int HKV, int D, float eps,
                               int n_pos, int* error) {
@@ -241,14 +245,15 @@ qk_norm_rope_write_row_kernel(bf16* __restrict__ qkv, const void* __restrict__ q
   const int heads = HQ + 2 * HKV;
   const int row = blockIdx.x;
   bf16* src_row = qkv + (size_t)row * heads * D + 8 * sub;
-  const int raw_pos = row_pos[row];
-  const bool bad = raw_pos < 0 || raw_pos >= n_pos;  // flagged below; nothing is stored for such a row
-  const int pos = bad ? 0 : raw_pos;
+  const int raw_place = row_pos[row];                                                   // in the cache
+  const int raw_pos = raw_place + (seq_shift ? seq_shift[row_seq[row]] : 0);  // in the sequence
+  const bool bad = raw_place < 0 || raw_pos < 0 || raw_pos >= n_pos;  // flagged below; nothing is stored for such a row
+  const int pos = bad ? 0 : raw_pos, place = bad ? 0 : raw_place;
   if (bad && threadIdx.x == 0 && error) atomicExch(error, 2);
   size_t cache_row = 0;
   if (HKV > 0) {
-    const int page = page_of(table, width, seq_slot[row_seq[row]], pos);
-    cache_row = (size_t)page * HKV * KRK_PAGE + (pos % KRK_PAGE);
+    const int page = page_of(table, width, seq_slot[row_seq[row]], place);
+    cache_row = (size_t)page * HKV * KRK_PAGE + (place % KRK_PAGE);
   }
   RopeLane t;
   if (cos_t) t = rope_lane(cos_t, sin_t, pos, D, sub);
@@ -285,9 +290,10 @@ qk_norm_rope_write_row_kernel(bf16* __restrict__ qkv, const void* __restrict__ q
 constexpr int ROW_KERNEL_MIN_ROWS = 256;
 
 // gains may be null (no q/k norm); cos/sin may be null (no rotation); the cache
-// pointers are unused when HKV == 0. rot: the rotated width (even, <= D; the tables are [positions, rot/2]).
+// pointers are unused when HKV == 0. seq_shift (may be null): how much further each sequence's rows lie in the sequence than in the cache,
+// where keys were evicted from it. rot: the rotated width (even, <= D; the tables are [positions, rot/2]).
 KRK_API int krk_qk_norm_rope_write(void* qkv, const void* q_gain, const void* k_gain, int gain_f32, const void* cos_t,
-                                   const void* sin_t, const int* row_seq, const int* row_pos, const int* seq_slot,
+                                   const void* sin_t, const int* row_seq, const int* row_pos, const int* seq_shift, const int* seq_slot,
                                    const int* table, int width, void* k_cache, void* v_cache, int rows, int HQ, int HKV,
                                    int D, int rot, float eps, int n_pos, int* error, int dtype, cudaStream_t stream) {
   if (rows == 0) return 0;
@@ -299,14 +305,14 @@ KRK_API int krk_qk_norm_rope_write(void* qkv, const void* q_gain, const void* k_
   if (dtype == KRK_DTYPE_BF16 && gains_aligned && rot == D && (D == 16 || D == 32 || D == 64 || D == 128 || D == 256)) {
     if (rows >= ROW_KERNEL_MIN_ROWS)
       return (int)launch_pdl(qk_norm_rope_write_row_kernel, dim3((unsigned)rows), dim3(256), 0, stream, (bf16*)qkv, q_gain,
-                             k_gain, gain_f32, (const bf16*)cos_t, (const bf16*)sin_t, row_seq, row_pos, seq_slot, table,
+                             k_gain, gain_f32, (const bf16*)cos_t, (const bf16*)sin_t, row_seq, row_pos, seq_shift, seq_slot, table,
                              width, (bf16*)k_cache, (bf16*)v_cache, HQ, HKV, D, eps, n_pos, error);
     const int per_warp = 32 / (D / 8);
     const long long n_warps = (items + per_warp - 1) / per_warp;
     const long long n_blocks = (n_warps + 7) / 8;
     if (n_blocks > 0x7fffffffLL) return -3;
     return (int)launch_pdl(qk_norm_rope_write_vec_kernel, dim3((unsigned)n_blocks), dim3(256), 0, stream, (bf16*)qkv,
-                           q_gain, k_gain, gain_f32, (const bf16*)cos_t, (const bf16*)sin_t, row_seq, row_pos, seq_slot,
+                           q_gain, k_gain, gain_f32, (const bf16*)cos_t, (const bf16*)sin_t, row_seq, row_pos, seq_shift, seq_slot,
                            table, width, (bf16*)k_cache, (bf16*)v_cache, rows, HQ, HKV, D, eps, n_pos, error);
   }
   const int warps = 8;
@@ -314,9 +320,9 @@ KRK_API int krk_qk_norm_rope_write(void* qkv, const void* q_gain, const void* k_
   if (blocks > 0x7fffffffLL) return -3;
   if (dtype == KRK_DTYPE_F32)
     return (int)launch_pdl(qk_norm_rope_write_kernel<float>, dim3((unsigned)blocks), dim3(warps * 32), 0, stream,
-        (float*)qkv, q_gain, k_gain, gain_f32, (const float*)cos_t, (const float*)sin_t, row_seq, row_pos, seq_slot,
+        (float*)qkv, q_gain, k_gain, gain_f32, (const float*)cos_t, (const float*)sin_t, row_seq, row_pos, seq_shift, seq_slot,
         table, width, (float*)k_cache, (float*)v_cache, rows, HQ, HKV, D, rot, eps, n_pos, error);
   return (int)launch_pdl(qk_norm_rope_write_kernel<bf16>, dim3((unsigned)blocks), dim3(warps * 32), 0, stream,
-        (bf16*)qkv, q_gain, k_gain, gain_f32, (const bf16*)cos_t, (const bf16*)sin_t, row_seq, row_pos, seq_slot, table,
+        (bf16*)qkv, q_gain, k_gain, gain_f32, (const bf16*)cos_t, (const bf16*)sin_t, row_seq, row_pos, seq_shift, seq_slot, table,
         width, (bf16*)k_cache, (bf16*)v_cache, rows, HQ, HKV, D, rot, eps, n_pos, error);
 }
