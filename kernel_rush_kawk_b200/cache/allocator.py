@@ -63,7 +63,8 @@ class PageLedger:
     """Pages of one storage group: a pool and, per slot, the pages it holds in
     logical order. ``ring`` is None for a group that keeps every position, or the
     number of logical pages a slot holds at most for a group that keeps a window (the
-    pages of positions that are kept for good come first and count among them)."""
+    pages of positions that are kept for good come first and count among them).
+    A page may be held by several slots (``share``); it goes back to the pool with the last of them."""
 
     def __init__(self, n_pages: int, n_slots: int, width: int, page_size: int, ring: int | None):
         self.pool = FreeList(n_pages, "cache page")
@@ -71,6 +72,7 @@ class PageLedger:
         self.width = width
         self.page_size = page_size
         self.ring = ring
+        self.holders: dict[int, int] = {}  # page -> slots that hold it, where these are more than one
 
     def pages_for(self, length: int) -> int:
         need = -(-length // self.page_size)
@@ -97,15 +99,47 @@ class PageLedger:
             have.append(page)
         return new
 
+    def share(self, source: int, slot: int, n_pages: int) -> list[tuple[int, int]]:
+        """``slot``, which holds none yet, takes the first ``n_pages`` pages of ``source`` as its own first ones;
+        returns the (logical index, page) pairs."""
+        if self.ring is not None:
+            raise CacheError("pages that a window cycles through cannot be shared")
+        if self.pages[slot] or n_pages > len(self.pages[source]):
+            raise CacheError(f"a slot with {len(self.pages[slot])} pages cannot share {n_pages} of the {len(self.pages[source])} that another holds")
+        self.pages[slot] = self.pages[source][:n_pages]
+        for page in self.pages[slot]:
+            self.holders[page] = self.holders.get(page, 1) + 1
+        return list(enumerate(self.pages[slot]))
+
+    def _give(self, page: int) -> None:
+        n = self.holders.pop(page, 1) - 1
+        if n == 0:
+            self.pool.give(page)
+        elif n > 1:
+            self.holders[page] = n
+
+    def shrink(self, slot: int, length: int) -> None:
+        """Give back the pages behind those that ``length`` positions need."""
+        need = self.pages_for(length)
+        for page in self.pages[slot][need:]:
+            self._give(page)
+        del self.pages[slot][need:]
+
     def release(self, slot: int) -> None:
         for page in self.pages[slot]:
-            self.pool.give(page)
+            self._give(page)
         self.pages[slot] = []
 
     def check(self) -> None:
         self.pool.check()
-        held = [p for pages in self.pages for p in pages]
-        if len(held) != len(set(held)):
-            raise CacheError("a cache page is held by two slots")
-        if len(held) != self.pool.held:
-            raise CacheError(f"{self.pool.held} pages are handed out but slots hold {len(held)}")
+        count: dict[int, int] = {}
+        for pages in self.pages:
+            for p in pages:
+                count[p] = count.get(p, 0) + 1
+        for page, n in count.items():
+            if n != self.holders.get(page, 1):
+                raise CacheError(f"a cache page is held by two slots or more: by {n}, where {self.holders.get(page, 1)} share it")
+        if any(page not in count for page in self.holders):
+            raise CacheError("a shared cache page is held by no slot")
+        if len(count) != self.pool.held:
+            raise CacheError(f"{self.pool.held} pages are handed out but slots hold {len(count)}")

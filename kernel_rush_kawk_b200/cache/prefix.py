@@ -39,10 +39,14 @@ class PrefixGroups:
         n = self.n_groups
         self.cu, self.length, self.group = self.buffer[:n + 1], self.buffer[n + 1:2 * n + 1], self.buffer[2 * n + 1:]
 
+    @staticmethod
+    def shape_of(sizes, lengths) -> tuple:
+        """What a captured step of such groups depends on, beside their number of sequences."""
+        return (len(sizes), max(sizes), max(lengths) > 0)
+
     @property
     def shape(self) -> tuple:
-        """What a captured step of these groups depends on, beside their number of sequences."""
-        return (self.n_groups, self.max_seqs, self.max_length > 0)
+        return self.shape_of(self.sizes, self.lengths)
 
     def update(self, other: "PrefixGroups") -> None:
         """Take another object's sizes and lengths, in the same device buffer (a captured step goes on reading it)."""

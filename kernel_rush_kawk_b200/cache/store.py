@@ -17,6 +17,13 @@ zeroed when the slot is handed out.
 
 Pages are not cleared when a slot is given back: every read is bounded by the
 sequence's length, as in the reference, whose reset is ``pos.zero_()`` (:290).
+
+Sequences that begin alike may share the pages of their first positions (``fork``): full pages
+only, which nobody writes again. A step's attention reads them once for all neighbours in it.
+
+With a ``KeyEviction`` the cache counts, for every key, the attention weight that it has received, and ``evict`` gives
+up the keys that received least; a row's place in the cache and its position in the sequence then differ by what
+the sequence has given up (``evicted``).
 """
 
 from __future__ import annotations
@@ -28,6 +35,7 @@ import torch
 
 from ..parts.base import KVNeed, StateNeed
 from .allocator import CacheError, FreeList, PageLedger
+from .eviction import KeyEviction
 
 PAGE = 64  # positions per page; the attention kernels' key block
 
@@ -48,6 +56,11 @@ class KVView:
     #: cycle through the others: page index b = p // PAGE sits in entry b if b < keep_pages, else in entry
     #: keep_pages + (b - keep_pages) % (width - keep_pages)
     keep_pages: int = 0
+    #: where keys are evicted: the weight that each row has received (float32 [slots, kv_heads, width * PAGE]), its position in the
+    #: sequence (int32, the same shape), and how many of a step's last queries count (None: all)
+    scores: torch.Tensor | None = None
+    positions: torch.Tensor | None = None
+    observe: int | None = None
 
     def __post_init__(self):
         self.v_dim = self.v_dim or self.head_dim
@@ -60,7 +73,7 @@ class StateView:
 
 class _KVGroup:
     def __init__(self, need: KVNeed, runs: list[int], n_pages: int, n_slots: int, width: int, ring: int | None,
-                 device, dtype, keep_pages: int = 0):
+                 device, dtype, keep_pages: int = 0, eviction: KeyEviction | None = None):
         self.need = need
         self.runs = runs
         self.width = ring if ring is not None else width
@@ -73,10 +86,18 @@ class _KVGroup:
                                                            device=device)
         self.table_host = np.zeros((n_slots, self.width), dtype=np.int32)
         self.table = torch.zeros((n_slots, self.width), dtype=torch.int32, device=device)
+        self.scores = self.positions = None
+        if eviction is not None:
+            if need.window is not None or not need.values:
+                raise CacheError("keys can be evicted where a run keeps every key and a value for each")
+            counts = (len(runs), n_slots, need.kv_heads, self.width * PAGE)
+            self.scores = torch.zeros(counts, dtype=torch.float32, device=device)
+            self.positions = torch.zeros(counts, dtype=torch.int32, device=device)
         self.dirty: set[int] = set()
 
     def bytes(self) -> int:
-        return (self.k.numel() + (self.v.numel() if self.need.values else 0)) * self.k.element_size()
+        counts = 0 if self.scores is None else 8 * self.scores.numel()
+        return (self.k.numel() + (self.v.numel() if self.need.values else 0)) * self.k.element_size() + counts
 
 
 class _StateGroup:
@@ -95,10 +116,11 @@ class SequenceCache:
     max_tokens: positions all live sequences may hold together, each sequence's
     count rounded up to whole pages. max_slots: live sequences. max_context: the
     longest sequence. step_tokens: the most tokens one sequence brings in one step;
-    it sizes the rings of window groups."""
+    it sizes the rings of window groups. eviction: count the weight that keys receive, for ``evict``."""
 
     def __init__(self, needs: list, max_tokens: int, max_slots: int, max_context: int, device, dtype,
-                 step_tokens: int = 2048):
+                 step_tokens: int = 2048, eviction: KeyEviction | None = None):
+        self.eviction = eviction
         self.device = torch.device(device)
         self.dtype = dtype
         self.max_slots = int(max_slots)
@@ -107,7 +129,10 @@ class SequenceCache:
         self.n_pages = max(1, -(-int(max_tokens) // PAGE))
         self.width = max(1, -(-self.max_context // PAGE))
         self.slots = FreeList(self.max_slots, "cache slot")
-        self.length = [0] * self.max_slots
+        self.length = [0] * self.max_slots  # rows held
+        self.evicted = [0] * self.max_slots  # rows given up: the next row's position is length + evicted
+        self._family: list = [None] * self.max_slots  # (number, shared positions) of slots that share pages with others
+        self._families = 0
         self.h2d_bytes = 0  # page-table rows (and their indices) copied to the device so far
         self._kv_groups: list[_KVGroup] = []
         self._state_groups: list[_StateGroup] = []
@@ -134,7 +159,8 @@ class SequenceCache:
                     ring = min(self.width, keep_pages + -(-(need.window + self.step_tokens - 1) // PAGE) + 1)
                     keep_pages = min(keep_pages, ring - 1)  # a context this short never reaches the ring's turn
                     pages = min(self.n_pages, self.max_slots * ring)
-                group = _KVGroup(need, runs, pages, self.max_slots, self.width, ring, self.device, dtype, keep_pages)
+                group = _KVGroup(need, runs, pages, self.max_slots, self.width, ring, self.device, dtype, keep_pages,
+                                 eviction)
                 self._kv_groups.append(group)
             else:
                 group = _StateGroup(need, runs, self.max_slots, self.device, dtype)
@@ -154,7 +180,8 @@ class SequenceCache:
     # -- slots --------------------------------------------------------------
     def alloc(self) -> int:
         slot = self.slots.take()
-        self.length[slot] = 0
+        self.length[slot] = self.evicted[slot] = 0
+        self._family[slot] = None
         for g in self._state_groups:
             g.state[:, slot].zero_()
         return slot
@@ -163,13 +190,89 @@ class SequenceCache:
         self.slots.give(slot)  # raises on a slot that is not held
         for g in self._kv_groups:
             g.ledger.release(slot)
-        self.length[slot] = 0
+        self.length[slot] = self.evicted[slot] = 0
+        self._family[slot] = None
+
+    def can_share(self) -> bool:
+        """Whether sequences can share pages: no run keeps a window of keys, whose pages are written again, and no keys are evicted."""
+        return self.eviction is None and all(g.need.window is None for g in self._kv_groups)
+
+    def fork(self, slot: int, length: int) -> int:
+        """A new slot whose sequence begins with the first ``length`` positions of ``slot``'s: it holds the same pages, and copies of the
+        fixed-size state. ``length`` is a whole number of pages; where there is state, all that ``slot`` holds (the state of an earlier
+        position is gone). Single-token and longer steps read shared pages once for the sequences that stand side by side in them."""
+        if not self.slots.is_held(slot):
+            raise CacheError(f"cache slot {slot} is not held")
+        if not self.can_share():
+            raise CacheError("sequences share pages where every run keeps all keys and none are evicted")
+        if length < 0 or length % PAGE or length > self.length[slot]:
+            raise CacheError(f"a fork shares whole pages of {PAGE} positions that its source holds; got {length} of {self.length[slot]}")
+        if self._state_groups and length != self.length[slot]:
+            raise CacheError(f"the state behind position {length} is gone: the sequence is at {self.length[slot]}")
+        new = self.alloc()
+        for g in self._kv_groups:
+            for logical, page in g.ledger.share(slot, new, length // PAGE):
+                g.table_host[new, logical] = page
+            g.dirty.add(new)
+        for g in self._state_groups:
+            g.state[:, new].copy_(g.state[:, slot])
+        self.length[new] = length
+        if length:
+            if self._family[slot] is None:
+                self._families += 1
+                self._family[slot] = (self._families, length)
+            if length >= self._family[slot][1]:  # a fork of less than the family shares has none
+                self._family[new] = self._family[slot]
+        return new
+
+    @property
+    def has_forks(self) -> bool:
+        return self._families > 0
+
+    def shared_groups(self, slots) -> tuple[list, list]:
+        """(sizes, shared positions) of the neighbours among ``slots`` that share pages, in order; a slot alone shares 0."""
+        sizes, lengths, last = [], [], None
+        for s in slots:
+            family = self._family[s]
+            if family is not None and family == last:
+                sizes[-1] += 1
+                lengths[-1] = family[1]
+            else:
+                sizes.append(1)
+                lengths.append(0)
+            last = family
+        return sizes, lengths
+
+    # -- eviction -------------------------------------------------------------
+    def evict_due(self, slot: int) -> bool:
+        """Whether the slot holds so many rows that some go before its next step."""
+        return self.eviction is not None and self.length[slot] >= self.eviction.keep + self.eviction.every
+
+    def evict(self, ops, slots, batch=None) -> None:
+        """Give up all but ``eviction.keep`` rows of those of ``slots`` that are due. ``batch``: a single-token step of exactly these slots,
+        whose description follows on the device."""
+        keep = self.eviction.keep
+        due = [self.evict_due(s) for s in slots]
+        if not any(due):
+            return
+        if batch is None:
+            slots, due = [s for s, d in zip(slots, due) if d], [True] * sum(due)
+        lengths = [self.length[s] if d else min(self.length[s], keep) for s, d in zip(slots, due)]
+        for i, g in enumerate(self._kv_groups):
+            ops.evict_keys(g.k, g.v, g.table, slots, lengths, g.scores, g.positions, keep, self.eviction.recent, batch=None if i else batch)
+        for s, d in zip(slots, due):
+            if d:
+                self.evicted[s] += self.length[s] - keep
+                self.length[s] = keep
+                for g in self._kv_groups:
+                    g.ledger.shrink(s, keep)
 
     def reserve(self, slot: int, length: int) -> None:
         """Make room for ``slot`` to hold ``length`` positions."""
         if not self.slots.is_held(slot):
             raise CacheError(f"cache slot {slot} is not held")
-        if length > self.max_context:
+        if length + self.evicted[slot] > self.max_context:
+            length += self.evicted[slot]
             raise CacheError(f"a sequence of {length} tokens exceeds the longest the cache was built for ({self.max_context})")
         for g in self._kv_groups:
             if not g.ledger.can_grow(slot, length):
@@ -193,15 +296,19 @@ class SequenceCache:
             self.h2d_bytes += len(rows) * (8 + 4 * g.width)
             g.dirty.clear()
 
+    def _per_slot(self) -> list:
+        """What a second run of the same step would change: fixed-size state, and the weights that keys have received."""
+        return [g.state for g in self._state_groups] + [g.scores for g in self._kv_groups if g.scores is not None]
+
     def save_state(self, slots) -> list:
-        """Copies of the fixed-size state that these slots hold, one tensor per state group."""
+        """Copies of the fixed-size state that these slots hold, one tensor per state group (then of their keys' received weights)."""
         idx = torch.as_tensor(list(slots), dtype=torch.int64, device=self.device)
-        return [g.state.index_select(1, idx) for g in self._state_groups]
+        return [t.index_select(1, idx) for t in self._per_slot()]
 
     def restore_state(self, slots, saved: list) -> None:
         idx = torch.as_tensor(list(slots), dtype=torch.int64, device=self.device)
-        for g, s in zip(self._state_groups, saved):
-            g.state.index_copy_(1, idx, s)
+        for t, s in zip(self._per_slot(), saved):
+            t.index_copy_(1, idx, s)
 
     def per_sequence_step_limit(self) -> int | None:
         """The most tokens one sequence may bring in one pass, or None if any number will do. A group that
@@ -220,12 +327,14 @@ class SequenceCache:
             return tuple(self._view_of(group, line) for group, line in where)
         return self._view_of(*where)
 
-    @staticmethod
-    def _view_of(group, line):
+    def _view_of(self, group, line):
         if isinstance(group, _KVGroup):
-            return KVView(group.k[line], group.v[line], group.table, group.width, group.need.window,
+            view = KVView(group.k[line], group.v[line], group.table, group.width, group.need.window,
                           group.need.kv_heads, group.need.head_dim, group.need.v_dim or group.need.head_dim,
                           group.keep_pages)
+            if group.scores is not None:
+                view.scores, view.positions, view.observe = group.scores[line], group.positions[line], self.eviction.observe
+            return view
         return StateView(group.state[line])
 
     # -- accounting ---------------------------------------------------------

@@ -46,6 +46,11 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--max-context", type=int, default=None)
     g.add_argument("--max-batch", type=int, default=None, help="run the prompts as consecutive batches of this size")
 
+    g.add_argument("--share-prefix", action="store_true", help="run and hold what prompts begin with in common once")
+    g.add_argument("--keep-keys", type=int, default=None, metavar="N",
+                   help="hold about N keys a sequence: those that received least attention are given up")
+    g.add_argument("--keep-recent", type=int, default=None, metavar="N", help="of the keys kept, the newest N whatever they received (default: a quarter)")
+
     w = sub.add_parser("write-random", help="write a model folder with random weights")
     w.add_argument("--preset", required=True)
     w.add_argument("--seed", type=int, default=0)
@@ -84,7 +89,7 @@ def main(argv=None) -> int:
         folder = write_model_folder(args.out, preset_config(args.preset), args.seed, args.std)
         print(folder)
         return 0
-    from . import Engine
+    from . import Engine, KeyEviction
     prompts = list(args.prompt_ids)
     if args.prompt_file:
         prompts += [list(map(int, row)) for row in json.load(open(args.prompt_file))]
@@ -92,12 +97,20 @@ def main(argv=None) -> int:
         print("no prompts given (--prompt-ids or --prompt-file)", file=sys.stderr)
         return 2
     options = dict(dtype=args.dtype, max_slots=args.max_slots, max_context=args.max_context)
+    if args.keep_recent is not None and args.keep_keys is None:
+        parser.error("--keep-recent goes with --keep-keys")
+    if args.keep_keys is not None:
+        if args.share_prefix:
+            parser.error("--share-prefix and --keep-keys exclude each other: shared pages stay as they are")
+        recent = args.keep_keys // 4 if args.keep_recent is None else args.keep_recent
+        options["eviction"] = KeyEviction(keep=args.keep_keys, recent=recent)
     if args.model:
         engine = Engine(args.model, **options)
     else:
         engine = Engine.from_random(args.random, seed=args.weights_seed, **options)
     outs = engine.generate_all(prompts, args.max_new_tokens, temperature=args.temperature, seed=args.seed,
-                               stop_token_ids=args.stop_token_id or (), max_batch=args.max_batch)
+                               stop_token_ids=args.stop_token_id or (), max_batch=args.max_batch,
+                               share_prefix=args.share_prefix)
     for prompt, out in zip(prompts, outs):
         print(json.dumps({"prompt": prompt, "tokens": out}))
     return 0

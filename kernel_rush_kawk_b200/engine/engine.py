@@ -8,7 +8,9 @@ token (EOS is an ordinary id), exactly ``max_new_tokens`` yields. Keyword
 options add what the reference lacks: unequal prompt lengths need no option;
 ``temperature`` and ``seed`` sample; ``stop_token_ids`` end a sequence early (its
 place then holds None); ``dtype`` picks the bfloat16 serving path or the true
-float32 path. After a call ``Engine.last_stats`` holds the batch's times (the
+float32 path; ``share_prefix`` runs what prompts have in common once, in pages that their sequences share;
+``eviction`` (a ``KeyEviction``, at construction) bounds the keys that a sequence holds by giving up those that received
+least attention. After a call ``Engine.last_stats`` holds the batch's times (the
 reference logs the like: engine/engine.py:206,378); a kernel that flagged bad
 input or gave up on a wait makes the call raise ``KernelError``.
 
@@ -26,8 +28,10 @@ from pathlib import Path
 
 import torch
 
+from ..cache.eviction import KeyEviction
 from ..cache.store import PAGE, SequenceCache
 from ..config.registry import get_architecture, preset_config, read_config
+from ..parts.base import KVNeed, StateNeed
 from ..sampling.sampler import Sampler, SamplingParams
 from ..weights.loader import checkpoint_shapes, read_checkpoint
 from ..weights.random_init import random_tensors
@@ -65,7 +69,7 @@ def _default_ops(device: torch.device, head_dims):
 class Engine:
     def __init__(self, model_path=None, *, dtype="bfloat16", max_tokens: int | None = None, max_slots: int = 64,
                  max_context: int | None = None, use_cuda_graphs: bool = True, max_step_rows: int = 16384,
-                 step_tokens: int = 2048, device="cuda:0", ops=None, _config=None, _tensors=None):
+                 step_tokens: int = 2048, device="cuda:0", ops=None, eviction: KeyEviction | None = None, _config=None, _tensors=None):
         torch.backends.cuda.matmul.allow_tf32 = False
         torch.backends.cudnn.allow_tf32 = False
         torch.backends.cuda.matmul.allow_bf16_reduced_precision_reduction = False
@@ -105,6 +109,9 @@ class Engine:
         # the most tokens of one sequence in one pass where a layer keeps a window of keys: it sizes that
         # layer's ring of pages (window + step_tokens positions); longer steps are cut into passes
         self.step_tokens = int(step_tokens)
+        self.eviction = eviction
+        if eviction is not None:
+            self._check_eviction()
         self.cache = self.stepper = self.loop = None
         self.sampler = Sampler(self.ops, self.device)
         self.last_stats = None  # GenerationStats of the last batch that generate / generate_all ran
@@ -125,6 +132,18 @@ class Engine:
         tensors = random_tensors(expected, seed, std, device)
         return cls(None, _config=config, _tensors=tensors, **options)
 
+    def _check_eviction(self) -> None:
+        """Keys can be evicted where every run that keeps keys keeps all of them, reads its own, and counts what they receive."""
+        for entry, need in zip(self.plan.schedule, self.model.cache_needs()):
+            mixer = self.model.blocks[entry.layer].mixer
+            if entry.cache_from is not None:
+                raise ValueError("keys cannot be evicted from a cache that several layers read")
+            if isinstance(need, StateNeed) or need is None:
+                continue
+            if not isinstance(need, KVNeed) or need.window is not None or not getattr(mixer, "counts_weights", False):
+                raise ValueError(f"keys cannot be evicted in this model: a '{self.plan.layers[entry.layer].mixer.kind}' layer "
+                                 f"{'keeps a window of keys' if isinstance(need, KVNeed) and need.window is not None else 'does not count what its keys receive'}")
+
     def _build_cache(self, max_tokens: int, max_slots: int) -> None:
         if self.cache is not None and self.cache.live:
             raise RuntimeError(f"the cache cannot be rebuilt while {self.cache.live} sequences are live in it "
@@ -133,7 +152,7 @@ class Engine:
         if self.device.type == "cuda":
             torch.cuda.empty_cache()
         self.cache = SequenceCache(self.model.cache_needs(), max_tokens, max_slots, self.max_context, self.device,
-                                   self.dtype, step_tokens=self.step_tokens)
+                                   self.dtype, step_tokens=self.step_tokens, eviction=self.eviction)
         self.stepper = Stepper(self.model, self.cache, self.ops, self.max_step_rows, self.use_cuda_graphs)
         self.loop = GenerationLoop(self.stepper, self.cache, self.sampler)
 
@@ -149,9 +168,12 @@ class Engine:
 
     # -- the reference's entry ------------------------------------------------
     def generate(self, input_ids, max_new_tokens: int, *, temperature: float = 0.0, seed: int = 0,
-                 stop_token_ids=()):
+                 stop_token_ids=(), share_prefix: bool = False):
         """Yield, per step, one token id per sequence (None once a sequence has ended
         on a stop token). All sequences start together; their lengths may differ.
+
+        ``share_prefix``: what prompts begin with in common (whole pages of 64 tokens; a prompt given n times draws n samples of
+        it) is run and held once, and read once a step for all of its sequences.
 
         This is a generator: arguments are checked, and a cache without a fixed size is
         grown if the call needs more room, at the first ``next()``. One generation runs
@@ -166,13 +188,14 @@ class Engine:
                                  f"the context of {self.max_context}")
         self._ensure_cache([len(p) for p in prompts], max_new_tokens)
         try:
-            yield from self.loop.run_batch(prompts, max_new_tokens, SamplingParams(temperature, seed), stop_token_ids)
+            yield from self.loop.run_batch(prompts, max_new_tokens, SamplingParams(temperature, seed), stop_token_ids,
+                                           share_prefix=share_prefix)
         finally:
             self.last_stats = self.loop.stats
             log.info("generate: %s", self.last_stats.line())
 
     def generate_all(self, input_ids, max_new_tokens: int, *, temperature: float = 0.0, seed: int = 0,
-                     stop_token_ids=(), max_batch: int | None = None) -> list:
+                     stop_token_ids=(), max_batch: int | None = None, share_prefix: bool = False) -> list:
         """Any number of requests, run as consecutive batches; returns each request's tokens."""
         prompts = [list(map(int, row)) for row in input_ids]
         if not prompts or max_new_tokens < 1:
@@ -182,7 +205,7 @@ class Engine:
             self._ensure_cache(lens, max_new_tokens)
         try:
             return self.loop.run_requests(prompts, max_new_tokens, SamplingParams(temperature, seed), stop_token_ids,
-                                          max_batch)
+                                          max_batch, share_prefix)
         finally:
             self.last_stats = self.loop.stats
             log.info("generate_all, last batch: %s", self.last_stats.line())

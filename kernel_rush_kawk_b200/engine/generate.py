@@ -21,6 +21,10 @@ earlier step's tokens. When a read shows that a sequence has stopped, nothing mo
 is queued; the steps already queued still ran that sequence (into pages it gives
 back afterwards) and their tokens for it are dropped. The batch then goes on,
 smaller, from the host's tokens.
+
+With ``share_prefix`` the prompts stand in the order of their tokens, and neighbours that begin with the same whole
+pages form a group (``shared_prefixes``): the first of them runs those pages' tokens, the others' sequences are
+forked from it, and all bring the rest of their prompts in the next step.
 """
 
 from __future__ import annotations
@@ -96,6 +100,29 @@ def split_into_batches(prompt_lens: list, max_new_tokens: int, max_slots: int, m
     return batches
 
 
+def shared_prefixes(prompts: list) -> list:
+    """Groups of prompts that begin alike: (request indices, tokens shared) with the shared tokens whole pages, at least one token of
+    every prompt behind them, 0 for a prompt alone. Neighbours in the order of the prompts' tokens join a group while the pages that it
+    saves, (members - 1) * shared pages, do not get fewer."""
+    order = sorted(range(len(prompts)), key=lambda i: prompts[i])
+    groups: list = []
+    for i in order:
+        p = prompts[i]
+        if groups:
+            members, shared = groups[-1]
+            other = prompts[members[0]]
+            most = min(len(p) - 1, shared if len(members) > 1 else len(other) - 1)
+            n = 0
+            while n < most and p[n] == other[n]:
+                n += 1
+            n -= n % PAGE
+            if n > 0 and len(members) * n >= (len(members) - 1) * shared:
+                groups[-1] = (members + [i], n)
+                continue
+        groups.append(([i], 0))
+    return groups
+
+
 class GenerationLoop:
     RUN_AHEAD = 3  # single-token steps queued on the device while the host reads an earlier one
 
@@ -107,7 +134,7 @@ class GenerationLoop:
         self.stats = GenerationStats()  # of the last batch
 
     def run_batch(self, prompts: list, max_new_tokens: int, sampling: SamplingParams = SamplingParams(),
-                  stop_token_ids=(), first_request: int = 0):
+                  stop_token_ids=(), first_request: int = 0, share_prefix: bool = False):
         """Generator: yields, per step, a list with one entry per prompt: the new token
         id, or None for a sequence that ended at an earlier step."""
         if max_new_tokens < 1 or not prompts:
@@ -146,11 +173,16 @@ class GenerationLoop:
                     self.cache.free(s.slot)
                     s.slot = -1
 
+        if share_prefix and not self.cache.can_share():
+            raise ValueError("prompts cannot share their beginnings in this engine: a layer keeps a window of keys, or keys are evicted")
         try:
-            for s in seqs:
-                s.slot = self.cache.alloc()
-            live = list(seqs)
-            logits = self.stepper.step([StepEntry(s.slot, s.prompt, [len(s.prompt) - 1]) for s in live])
+            if share_prefix:
+                live, begun = self._start_shared(seqs)
+            else:
+                for s in seqs:
+                    s.slot = self.cache.alloc()
+                live, begun = list(seqs), [0] * len(seqs)
+            logits = self.stepper.step([StepEntry(s.slot, s.prompt[n:], [len(s.prompt) - 1 - n]) for s, n in zip(live, begun)])
             tokens = self.sampler.select(logits, sampling, [s.request for s in live], 0)
             t_first = time.perf_counter()
             stats.prefill_ms = (t_first - t_begin) * 1e3
@@ -198,8 +230,25 @@ class GenerationLoop:
                     self.cache.free(s.slot)
                     s.slot = -1
 
+    def _start_shared(self, seqs: list) -> tuple[list, list]:
+        """Run what the prompts share, once; (the sequences in the order of their groups, the tokens that each has had)."""
+        order, begun, first = [], [], []
+        groups = [([seqs[i] for i in members], shared) for members, shared in shared_prefixes([s.prompt for s in seqs])]
+        for members, shared in groups:
+            members[0].slot = self.cache.alloc()
+            if shared:
+                first.append(StepEntry(members[0].slot, members[0].prompt[:shared], []))
+        if first:
+            self.stepper.step(first)
+        for members, shared in groups:
+            for s in members[1:]:
+                s.slot = self.cache.fork(members[0].slot, shared)
+            order += members
+            begun += [shared] * len(members)
+        return order, begun
+
     def run_requests(self, prompts: list, max_new_tokens: int, sampling: SamplingParams = SamplingParams(),
-                     stop_token_ids=(), max_batch: int | None = None) -> list:
+                     stop_token_ids=(), max_batch: int | None = None, share_prefix: bool = False) -> list:
         """Run every request, batch after batch; returns each request's generated tokens."""
         max_slots = min(self.cache.max_slots, max_batch or self.cache.max_slots)
         batches = split_into_batches([len(p) for p in prompts], max_new_tokens, max_slots, self.cache.n_pages)
@@ -207,7 +256,7 @@ class GenerationLoop:
         for batch in batches:
             outs = [[] for _ in batch]
             for step_out in self.run_batch([prompts[i] for i in batch], max_new_tokens, sampling, stop_token_ids,
-                                           first_request=batch[0]):
+                                           first_request=batch[0], share_prefix=share_prefix):
                 for j, tok in enumerate(step_out):
                     if tok is not None:
                         outs[j].append(tok)

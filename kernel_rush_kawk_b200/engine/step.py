@@ -28,6 +28,7 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
+from ..cache.prefix import PrefixGroups
 from ..cache.store import SequenceCache
 
 
@@ -45,13 +46,20 @@ class BatchMeta:
     tokens[r], row_seq[r] (which sequence of the pass row r belongs to), row_pos[r]
     (its position in the sequence); seq_slot[s], seq_start[s] (cached length before
     the pass), seq_qlen[s], cu_q[s] (first row of sequence s; cu_q[n_seqs] = rows);
-    want[w] (rows whose logits are asked for)."""
+    want[w] (rows whose logits are asked for). Where keys are evicted (``shifts``), row_pos and seq_start count the rows
+    held, and seq_shift[s] how much further these lie in the sequence.
+
+    ``prefix`` (a PrefixGroups, or None) says which neighbouring sequences share pages."""
 
     FIELDS = ("tokens", "row_seq", "row_pos", "seq_slot", "seq_start", "seq_qlen", "cu_q", "want")
 
-    def __init__(self, n_rows: int, n_seqs: int, n_want: int, device):
+    def __init__(self, n_rows: int, n_seqs: int, n_want: int, device, shifts: bool = False):
         self.n_rows, self.n_seqs, self.n_want = n_rows, n_seqs, n_want
         sizes = (n_rows, n_rows, n_rows, n_seqs, n_seqs, n_seqs, n_seqs + 1, n_want)
+        fields = self.FIELDS
+        if shifts:
+            sizes, fields = sizes + (n_seqs,), fields + ("seq_shift",)
+        self.prefix = None
         # every array starts on a 16-byte boundary
         offsets, total = [], 0
         for s in sizes:
@@ -62,9 +70,9 @@ class BatchMeta:
         self.buffer = torch.zeros(self.total, dtype=torch.int32, device=device)
         self.host = torch.zeros(self.total, dtype=torch.int32, pin_memory=self.buffer.is_cuda)
         self.host_np = self.host.numpy()
-        self._host_views = {name: self.host_np[off:off + size] for name, off, size in zip(self.FIELDS, offsets, sizes)}
+        self._host_views = {name: self.host_np[off:off + size] for name, off, size in zip(fields, offsets, sizes)}
         self._single_token_shape = False  # the pinned buffer holds the constant arrays of a one-token-each pass
-        for name, off, size in zip(self.FIELDS, offsets, sizes):
+        for name, off, size in zip(fields, offsets, sizes):
             setattr(self, name, self.buffer[off:off + size])
         self.copied = torch.cuda.Event() if self.buffer.is_cuda else None
         # host-side facts, valid for the pass being built
@@ -79,7 +87,7 @@ class BatchMeta:
     def host_field(self, name: str) -> np.ndarray:
         return self._host_views[name]
 
-    def fill(self, slots, starts, token_lists, want_rows) -> None:
+    def fill(self, slots, starts, token_lists, want_rows, shifts=None) -> None:
         """Write one pass into the pinned buffer and start its copy to the device."""
         if self.copied is not None:
             self.copied.synchronize()  # the previous copy out of this pinned buffer is over
@@ -107,6 +115,8 @@ class BatchMeta:
         view["seq_slot"][:] = slots
         view["seq_start"][:] = starts
         view["want"][:] = want_rows
+        if "seq_shift" in view:
+            view["seq_shift"][:] = 0 if shifts is None else shifts
         self.upload()
         self.max_q_len = max(q_lens)
         self.max_kv_len = max(s + n for s, n in zip(starts, q_lens))
@@ -158,13 +168,15 @@ class DecodeRun:
         self.depth = max(1, depth)
         n = self.n = len(slots)
         cache, dev = stepper.cache, stepper.device
+        if cache.eviction is not None:
+            cache.evict(stepper.ops, slots)
         starts = [cache.length[s] for s in slots]
         for s, start in zip(slots, starts):
             cache.reserve(s, start + 1)
         cache.sync()
         token_lists = [[t] for t in tokens]
-        self.graph = stepper._graphs.get(n) or stepper._capture(n, slots, starts, token_lists)
-        self.graph.meta.fill(slots, starts, token_lists, list(range(n)))
+        self.graph = stepper._graph(slots, starts, token_lists)
+        self.graph.meta.fill(slots, starts, token_lists, list(range(n)), stepper._shifts(slots))
         stepper.h2d_bytes = self.graph.meta.bytes
         ring = stepper._run_rings.get((n, self.depth))
         if ring is None:
@@ -188,6 +200,8 @@ class DecodeRun:
             raise RuntimeError(f"{self.depth} steps are queued already; collect one first")
         st, cache, n = self.stepper, self.stepper.cache, self.n
         if self.launched:  # the first step's pages were reserved with the batch description
+            if cache.eviction is not None:
+                cache.evict(st.ops, self.slots, batch=self.graph.meta)
             for s in self.slots:
                 cache.reserve(s, cache.length[s] + 1)
             cache.sync()
@@ -224,7 +238,7 @@ class Stepper:
         self.device = cache.device
         self.use_graphs = bool(use_graphs) and self.device.type == "cuda" and model.graph_safe
         self.vocab = model.plan.vocab_size
-        self._graphs: dict[int, _DecodeGraph] = {}
+        self._graphs: dict = {}  # sequences, or (sequences, shape of their groups) -> _DecodeGraph
         self._metas: dict[tuple, list] = {}
         self.graph_launches: dict[int, int] = {}  # kernels of this package inside each captured step
         self.h2d_bytes = 0  # bytes of the last step's host-to-device copies
@@ -301,12 +315,32 @@ class Stepper:
         if ring is None:
             if len(self._metas) > 64:
                 self._metas.clear()
-            ring = self._metas[key] = [0, [BatchMeta(n_rows, n_seqs, n_want, self.device) for _ in range(2)]]
+            ring = self._metas[key] = [0, [BatchMeta(n_rows, n_seqs, n_want, self.device, self.cache.eviction is not None) for _ in range(2)]]
         ring[0] ^= 1
         return ring[1][ring[0]]
 
+    def _shifts(self, slots):
+        """How much further each sequence's rows lie in it than in the cache, where keys are evicted."""
+        return [self.cache.evicted[s] for s in slots] if self.cache.eviction is not None else None
+
+    #: keys that the steps of neighbours in shared pages do not read again, all kv heads together, from which on reading them once pays
+    SHARED_MIN = 1
+
+    def _prefix(self, slots):
+        """The groups of neighbours that share pages, or None where none do or too little. Float32 steps read shared pages row by row like
+        others: a row's logits are the same to the bit however steps are cut and batched."""
+        cache = self.cache
+        if not cache.has_forks or cache.dtype != torch.bfloat16:
+            return None
+        sizes, lengths = cache.shared_groups(slots)
+        if sum((size - 1) * length for size, length in zip(sizes, lengths)) < self.SHARED_MIN:
+            return None
+        return sizes, lengths
+
     def _pass(self, entries, chosen):
         cache = self.cache
+        if cache.eviction is not None:
+            cache.evict(self.ops, [entries[i].slot for i, _, _ in chosen])
         slots, starts, token_lists, want_rows, which = [], [], [], [], []
         row = 0
         for i, first, n in chosen:
@@ -328,7 +362,9 @@ class Stepper:
             logits = self._replay(slots, starts, token_lists, want_rows, n_seqs)
         else:
             meta = self._meta(n_rows, n_seqs, len(want_rows))
-            meta.fill(slots, starts, token_lists, want_rows)
+            meta.fill(slots, starts, token_lists, want_rows, self._shifts(slots))
+            groups = self._prefix(slots)
+            meta.prefix = None if groups is None else PrefixGroups(*groups, self.device)
             self.h2d_bytes += meta.bytes
             ctx = StepContext(self.ops, meta, cache)
             logits = self.model.forward(ctx, meta.want) if want_rows else self._forward_no_logits(ctx)
@@ -345,11 +381,22 @@ class Stepper:
         return None
 
     # -- decode from a captured graph ------------------------------------------
-    def _replay(self, slots, starts, token_lists, want_rows, n: int):
-        g = self._graphs.get(n)
+    def _graph(self, slots, starts, token_lists) -> _DecodeGraph:
+        """The captured step of these sequences: by their number and, where neighbours share pages, the number and size of the groups."""
+        n = len(slots)
+        groups = self._prefix(slots)
+        if groups is None:
+            return self._graphs.get(n) or self._capture(n, slots, starts, token_lists)
+        g = self._graphs.get((n, PrefixGroups.shape_of(*groups)))
         if g is None:
-            g = self._capture(n, slots, starts, token_lists)
-        g.meta.fill(slots, starts, token_lists, list(range(n)))
+            return self._capture(n, slots, starts, token_lists, PrefixGroups(*groups, self.device))
+        if (g.meta.prefix.sizes, g.meta.prefix.lengths) != tuple(map(tuple, groups)):
+            g.meta.prefix.update(PrefixGroups(*groups, self.device))
+        return g
+
+    def _replay(self, slots, starts, token_lists, want_rows, n: int):
+        g = self._graph(slots, starts, token_lists)
+        g.meta.fill(slots, starts, token_lists, list(range(n)), self._shifts(slots))
         self.h2d_bytes += g.meta.bytes
         g.graph.replay()
         if len(want_rows) == n:
@@ -367,30 +414,44 @@ class Stepper:
         are reserved before the first one."""
         n = len(slots)
         cache = self.cache
+        evicts = cache.eviction is not None
+        if evicts:  # as many rows as there are between two evictions: pages are reserved step by step
+            cache.evict(self.ops, slots)
         starts = [cache.length[s] for s in slots]
         for s in slots:
-            cache.reserve(s, cache.length[s] + n_steps)
+            cache.reserve(s, cache.length[s] + (1 if evicts else n_steps))
         cache.sync()
         token_lists = [[int(t)] for t in tokens]
         if self.use_graphs:
-            g = self._graphs.get(n) or self._capture(n, slots, starts, token_lists)
+            g = self._graph(slots, starts, token_lists)
             meta = g.meta
         else:
             g, meta = None, self._meta(n, n, n)
-        meta.fill(slots, starts, token_lists, list(range(n)))
+            groups = self._prefix(slots)
+            meta.prefix = None if groups is None else PrefixGroups(*groups, self.device)
+        meta.fill(slots, starts, token_lists, list(range(n)), self._shifts(slots))
         self.h2d_bytes = meta.bytes
         req = torch.tensor(list(requests) if requests is not None else list(range(n)), dtype=torch.int32).to(self.device)
         out = torch.empty((n_steps, n), dtype=torch.int32, device=self.device)
         ctx = StepContext(self.ops, meta, cache)
         for t in range(n_steps):
+            if evicts and t:
+                cache.evict(self.ops, slots, batch=meta)
+                for s in slots:
+                    cache.reserve(s, cache.length[s] + 1)
+                cache.sync()
             if g is not None:
                 g.graph.replay()
                 logits = g.logits
             else:
                 logits = self.model.forward(ctx, meta.want)
             self.ops.select_tokens(logits, temperature, seed, req, first_step + t, feed=meta, out=out[t])
-        for s in slots:
-            cache.advance(s, n_steps)
+            if evicts:
+                for s in slots:
+                    cache.advance(s, 1)
+        if not evicts:
+            for s in slots:
+                cache.advance(s, n_steps)
         self.passes += n_steps
         return out
 
@@ -401,14 +462,16 @@ class Stepper:
             return None
         return DecodeRun(self, list(slots), [int(t) for t in tokens], sampling, list(requests), int(first_step), int(depth))
 
-    def _capture(self, n: int, slots, starts, token_lists) -> _DecodeGraph:
-        meta = BatchMeta(n, n, n, self.device)
-        meta.fill(slots, starts, token_lists, list(range(n)))
+    def _capture(self, n: int, slots, starts, token_lists, prefix: PrefixGroups | None = None) -> _DecodeGraph:
+        meta = BatchMeta(n, n, n, self.device, self.cache.eviction is not None)
+        meta.fill(slots, starts, token_lists, list(range(n)), self._shifts(slots))
+        meta.prefix = prefix
+        key = n if prefix is None else (n, prefix.shape)
         ctx = StepContext(self.ops, meta, self.cache)
         # Run once outside a capture: everything that allocates or initialises lazily
         # does so now. The pass writes this step's keys and values; the replay of the
         # captured step writes the same values to the same places again. Fixed-size
-        # state is not like that (a second update is a different state), so the
+        # state (and the weights that keys have received) is not like that (a second update is a different state), so the
         # sequences' state is put back as it was before the trial run.
         saved = self.cache.save_state(slots)
         side = torch.cuda.Stream(device=self.device)
@@ -422,6 +485,6 @@ class Stepper:
         before = getattr(self.ops, "launches", 0)
         with torch.cuda.graph(graph):
             logits = self.model.forward(ctx, meta.want)
-        self.graph_launches[n] = getattr(self.ops, "launches", 0) - before
-        g = self._graphs[n] = _DecodeGraph(graph, meta, logits)
+        self.graph_launches[key] = getattr(self.ops, "launches", 0) - before
+        g = self._graphs[key] = _DecodeGraph(graph, meta, logits)
         return g

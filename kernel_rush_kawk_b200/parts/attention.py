@@ -10,6 +10,9 @@ softmax statistics in 32-bit, q head h reads kv head h // (heads / kv_heads)
 
 A run that reads another run's cache (``own_cache`` False) has no k/v
 projections: it projects, normalises and rotates queries only.
+
+Where neighbours of a step share pages, what they share is read once for all of them; where keys
+are evicted, the attention counts the weight that each key receives.
 """
 
 from __future__ import annotations
@@ -27,6 +30,7 @@ class GQAttention(Mixer):
     the model builder)."""
 
     graph_safe = True
+    counts_weights = True  # counts the weight that its keys receive where the cache asks for it
 
     def __init__(self, params):
         super().__init__(params)
@@ -87,8 +91,17 @@ class GQAttention(Mixer):
         qkv = ops.linear(h, self.w_qkv)
         tables = self.position.rotary_tables() if self.position is not None else None
         cos, sin = tables if tables is not None else (None, None)
-        attn = ops.rope_attention(qkv, self.heads, kv_in_row, self.head_dim, self.q_gain, self.k_gain, self.eps,
-                                  cos, sin, ctx.batch, cache, self.scale, self.window)
+        prefix = getattr(ctx.batch, "prefix", None)  # neighbours of the step that share pages
+        if cache.scores is not None or (prefix is not None and self.window is None):
+            ops.qk_norm_rope_write(qkv, self.heads, kv_in_row, self.head_dim, self.q_gain, self.k_gain, self.eps, cos, sin, ctx.batch, cache)
+            step = (qkv, self.heads, kv_in_row, self.head_dim, ctx.batch, cache, self.scale)
+            if cache.scores is not None:  # keys are evicted by the weight that they receive
+                attn = ops.scored_attention(*step, cache.scores, cache.positions, cache.observe)
+            else:
+                attn = ops.shared_prefix_attention(*step, prefix)
+        else:
+            attn = ops.rope_attention(qkv, self.heads, kv_in_row, self.head_dim, self.q_gain, self.k_gain, self.eps,
+                                      cos, sin, ctx.batch, cache, self.scale, self.window)
         return ops.linear(attn, self.w_o)
 
 
