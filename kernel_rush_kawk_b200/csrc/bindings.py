@@ -238,6 +238,7 @@ class Kernels(CacheOps):
                  4: "a tensor-core GEMM gave up waiting for a TMA load",
                  5: "a tensor-core GEMM gave up waiting for its accumulator",
                  24: "the delta rule's walk gave up waiting for its copies",
+                 25: "attention of few rows gave up waiting for a page of keys or values",
                  20: "a 32-bit product of few rows gave up waiting for its copies",
                  21: "the wait of the self-test kernel ran out (as it is meant to)"}
         if flag in known:

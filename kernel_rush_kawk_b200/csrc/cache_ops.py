@@ -54,6 +54,12 @@ _PARTS_SIGNATURES = {
     "krk_join_parts": [_P, _P, _P, _P, c_int, c_int, c_int, c_int, _P],
     "krk_key_weights": [_P, _P, _P, _P, c_int, _P, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, c_int, c_float, c_int, _P],
 }
+_PARTS_SIGNATURES.update({
+    "krk_prefix_few_rows": [_P, _P, c_int, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_int, c_float, _P, _P],
+    "krk_prefix_tcgen05": [_P, _P, c_int, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_int, c_float, _P, _P],
+    "krk_own_single": [_P, _P, _P, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_float, _P, _P],
+    "krk_scored_single": [_P, _P, _P, _P, _P, _P, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_float, _P, _P],
+})
 _CACHE_SIGNATURES = {
     "krk_evict_max_seqs": [],
     "krk_evict_keys": [_P, _P, c_longlong, c_longlong, c_int, c_int, c_int, c_int, _P, c_int, _P, _P, _P, _P, c_longlong, c_int, _P, _P, c_int,
@@ -64,6 +70,7 @@ _CACHE_SIGNATURES = {
 class CacheOps:
     """Mixed into ``Kernels``."""
 
+    PREFIX_TENSOR_ROWS = 33  # rows of a group from which on its prefix goes to the tcgen05 kernel
     EVICT_SCRATCH_BYTES = 64 << 20  # the lists of moves of one pair of launches; more sequences take several pairs
 
     def _parts_lib(self, head_dim: int) -> ctypes.CDLL:
@@ -108,6 +115,18 @@ class CacheOps:
         and heads, never by lengths: a captured step stays valid."""
         return max(1, min(most, -(-444 // max(blocks, 1))))
 
+    @staticmethod
+    def _tiles_take(qkv, cache, head_dim) -> bool:
+        """Whether the tensor-core kernels take these rows and pages: bfloat16, head sizes in steps of 16, rows from 4-byte, pages from 16-byte
+        boundaries on."""
+        return (qkv.dtype == torch.bfloat16 and head_dim % 16 == 0 and qkv.stride(0) % 2 == 0 and qkv.data_ptr() % 4 == 0
+                and (cache.k.data_ptr() | cache.v.data_ptr()) % 16 == 0)
+
+    @staticmethod
+    def _cluster_splits(items: int) -> int:
+        """Blocks of a cluster that share the keys of a sequence's token, by the number of (sequence, kv head, row tile) items."""
+        return 8 if items <= 37 else 4 if items <= 64 else 2 if items <= 148 else 1
+
     def _attention_in_parts(self, qkv, heads, head_dim, batch, cache, scale, prefix, want_lse):
         """(output, log2 of every row's sum of 2^score or None)."""
         lib = self._parts_lib(head_dim)
@@ -119,15 +138,35 @@ class CacheOps:
         segments = self._segments(batch, cache, prefix)
         code, stream, stride, per = _code(qkv.dtype), self._stream(), qkv.stride(0), heads // kv
         tiles = lambda n: -(-n * per // 16)
-        own_splits = self._splits(tiles(batch.max_q_len) * kv * batch.n_seqs)
-        prefix_splits, group_rows = 0, 0
+        fast = self._tiles_take(qkv, cache, head_dim)
+        single = fast and batch.is_decode and not want_lse
+        prefix_splits, group_rows, tensor = 0, 0, False
         if prefix is not None and prefix.max_length:
             group_rows = prefix.max_rows(batch)
             prefix_splits = self._splits(tiles(group_rows) * kv * prefix.n_groups)
-        parts = prefix_splits + own_splits
+            tensor = (fast and hasattr(lib, "krk_prefix_tcgen05") and stride % 8 == 0 and qkv.data_ptr() % 16 == 0
+                      and group_rows * per >= self.PREFIX_TENSOR_ROWS)
+            if tensor:
+                prefix_splits = max(1, min(32, 148 // (-(-group_rows * per // 256) * kv * prefix.n_groups)))
+        own_splits = self._cluster_splits(tiles(1) * kv * batch.n_seqs) if single else self._splits(tiles(batch.max_q_len) * kv * batch.n_seqs)
+        parts = prefix_splits + (0 if single else own_splits)
         o = torch.empty((parts, rows, heads, head_dim), dtype=torch.float32, device=qkv.device)
         ml = torch.empty((parts, rows, heads, 2), dtype=torch.float32, device=qkv.device)
-        for own, first, n, most in ((0, 0, prefix_splits, group_rows), (1, prefix_splits, own_splits, batch.max_q_len)):
+        tail = (qkv.data_ptr(), stride, heads, kv, *segments, cache.k.data_ptr(), cache.v.data_ptr(), cache.k.shape[0])
+        if prefix_splits and fast and tiles(group_rows) * kv <= 65535:
+            self._ok((lib.krk_prefix_tcgen05 if tensor else lib.krk_prefix_few_rows)(o.data_ptr(), ml.data_ptr(), rows, 0, prefix_splits, *tail, group_rows, scale, self.error.data_ptr(), stream),
+                     "prefix attention")
+            first_done = True
+        else:
+            first_done = False
+        if single:
+            if prefix_splits and not first_done:
+                self._ok(lib.krk_partial_attention(o.data_ptr(), ml.data_ptr(), rows, 0, prefix_splits, 0, *tail[:-1], group_rows, scale, code, stream),
+                         "attention in parts")
+            self._ok(lib.krk_own_single(out.data_ptr(), o.data_ptr(), ml.data_ptr(), prefix_splits, own_splits, *tail, scale, self.error.data_ptr(), stream),
+                     "attention over own keys")
+            return out, None
+        for own, first, n, most in ((0, 0, 0 if first_done else prefix_splits, group_rows), (1, prefix_splits, own_splits, batch.max_q_len)):
             if n:
                 self._ok(lib.krk_partial_attention(o.data_ptr(), ml.data_ptr(), rows, first, n, own, qkv.data_ptr(), stride, heads, kv, *segments,
                                                    cache.k.data_ptr(), cache.v.data_ptr(), most, scale, code, stream), "attention in parts")
@@ -164,9 +203,17 @@ class CacheOps:
         self._check_scores("scored attention", scores, positions, cache, (("out_scores", out_scores, torch.float32),))
         if observe is not None and observe < 1:
             raise KernelError(f"scored attention: at least one query a sequence is observed, got {observe}")
+        kv, rows = cache.kv_heads, qkv.shape[0]
+        if rows and batch.is_decode and heads // kv <= 16 and self._tiles_take(qkv, cache, head_dim):
+            out = torch.empty((rows, heads * head_dim), dtype=qkv.dtype, device=qkv.device)
+            raw = torch.empty((rows, heads, scores.shape[2]), dtype=torch.float32, device=qkv.device)
+            self._ok(self._parts_lib(head_dim).krk_scored_single(
+                out.data_ptr(), raw.data_ptr(), scores.data_ptr(), out_scores.data_ptr(), _ptr(positions), _ptr(getattr(batch, "seq_shift", None)),
+                scores.shape[2], self._cluster_splits(kv * rows), qkv.data_ptr(), qkv.stride(0), heads, kv, *self._segments(batch, cache, None),
+                cache.k.data_ptr(), cache.v.data_ptr(), cache.k.shape[0], float(scale), self.error.data_ptr(), self._stream()), "scored attention")
+            return out
         out, lse = self._attention_in_parts(qkv, heads, head_dim, batch, cache, float(scale), None, True)
-        if qkv.shape[0]:
-            kv = cache.kv_heads
+        if rows:
             blocks = max(1, min(cache.width, -(-888 // (kv * batch.n_seqs))))
             self._ok(self._parts_lib(head_dim).krk_key_weights(
                 scores.data_ptr(), out_scores.data_ptr(), _ptr(positions), _ptr(getattr(batch, "seq_shift", None)), scores.shape[2], lse.data_ptr(),

@@ -1,0 +1,448 @@
+// Attention in parts for few rows a unit, bfloat16, on the warp-level tensor cores (partial_attention.cuh says what the parts are):
+// a sequence's single token over its own keys, joined with the parts of the prefix that it shares and, where asked for, with
+// the weight of each key added up in the same launch; and the prefix parts themselves for groups of few rows.
+//
+// A block takes 16 rows (the heads of a kv head, or those of several sequences of a group) and a share of the unit's pages; its
+// four warps take 16 keys of every page each, with running statistics of their own that join in shared memory at the end. What
+// bounds it is the bytes in flight: a unit of work reads D * 256 bytes a page and kv head and multiplies little, so pages come by TMA
+// (a fifth warp asks for them, one unit a page of keys or of values, into a ring as deep as the shared memory that
+// the blocks of an SM have between them), or by cp.async where the head size is no multiple of 64.
+//
+// The splits of a sequence's keys form a cluster: their parts meet in the first block's shared memory, which also reads the prefix
+// parts of its rows and writes the output. That is the only place that waits for the kernel before, so a sequence's own
+// keys are read while the prefix kernel still runs.
+//
+// Weights per key: scaled scores (log2 units, float32) go to scratch as they come, four bytes beside the 4 D that a key costs; when the
+// row's sum is known every block of the cluster turns its own keys' scores into weights, sums them over the heads in order
+// and adds them to the keys' sums. A key belongs to one thread: no atomics, the same bits every time.
+//
+// P is rounded to bfloat16 before it meets the values, as everywhere on this path (half a step is 2^-9 of a weight, and errors
+// of the keys add up like their weights: far below the output's own rounding); scores, statistics and sums are float32.
+//
+// Compiled once per head size: -DKRK_HEAD_DIM=<D>.
+#include <cooperative_groups.h>
+
+#include "mma.cuh"
+#include "partial_attention.cuh"
+#include "tcgen05.cuh"
+
+#ifndef KRK_HEAD_DIM
+#error "compile with -DKRK_HEAD_DIM=<head size>"
+#endif
+
+#if KRK_HEAD_DIM % 16 == 0 && KRK_HEAD_DIM <= 256
+
+namespace {
+
+#include "attention_tiles.cuh"
+
+namespace cg = cooperative_groups;
+
+constexpr int UNIT_ELEMS = TMA_PAGES ? KRK_PAGE * D : TILE_ELEMS;  // one page of keys (or of values) of one kv head
+constexpr uint32_t UNIT_BYTES = UNIT_ELEMS * 2;
+constexpr int RP = D + 2;  // floats of a row's part in shared memory: o, m, l
+constexpr size_t RED_BYTES = (size_t)4 * 16 * RP * sizeof(float);
+constexpr int CP_STAGES = 2;  // page pairs, where pages come by cp.async
+
+__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 2, 128;" ::: "memory"); }
+
+struct KeySums {  // weights per key; see krk_scored_single
+  float* raw;     // [n_seqs][HQ][capacity]
+  const float* sums;
+  float* sums_out;
+  int* positions;
+  const int* seq_shift;
+  int capacity;
+};
+
+struct Layout {  // of the dynamic shared memory, from a 1024-byte boundary on
+  size_t ring, inbox, bars, total;
+  __host__ __device__ Layout(int units, int splits, int inbox_rows) {
+    ring = 0;
+    const size_t r = (size_t)units * UNIT_BYTES;
+    inbox = r > RED_BYTES ? r : RED_BYTES;
+    inbox = (inbox + 15) & ~(size_t)15;
+    bars = inbox + (size_t)(splits > 1 ? splits : 0) * inbox_rows * RP * sizeof(float);
+    bars = (bars + 15) & ~(size_t)15;
+    total = bars + (size_t)units * 16 + 16 * sizeof(float);
+  }
+};
+
+// PREFIX: unit = group, parts go to `parts` from part0 on. Otherwise: unit = sequence, one token; the parts 0 .. n_join - 1 of its row join.
+template <bool TMA, bool PREFIX, bool SUMS>
+__global__ void __launch_bounds__(TMA ? 160 : 128)
+few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, bf16* __restrict__ out, Parts parts, int part0,
+                int n_join, const bf16* __restrict__ q, int q_stride, int HQ, int HKV, Segments seg, const bf16* __restrict__ k_cache,
+                const bf16* __restrict__ v_cache, float scale_log2, int row_tiles, int units_in_ring, bool wait_first, KeySums ks, int* __restrict__ error) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* base = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int n_splits = gridDim.x, split = blockIdx.x;
+  const bool clustered = !PREFIX && n_splits > 1;
+  const int G = HQ / HKV, inbox_rows = min(16, G);
+  const Layout at(units_in_ring, clustered ? n_splits : 1, inbox_rows);
+  bf16* ring_s = reinterpret_cast<bf16*>(base);
+  float* red = reinterpret_cast<float*>(base);            // [4 warps][16 rows][RP], when the ring is done with
+  float* inbox = reinterpret_cast<float*>(base + at.inbox);  // [splits][inbox_rows][RP] in the first block
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(base + at.bars);
+  uint64_t* empty_bar = full_bar + units_in_ring;
+  float* lse_s = reinterpret_cast<float*>(empty_bar + units_in_ring);  // [16]
+
+  if (clustered) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // "I have started"
+  if (wait_first) grid_dependency_wait();
+  grid_launch_dependents();
+  const int kh = blockIdx.y / row_tiles, rt = blockIdx.y % row_tiles;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t4 = lane & 3;
+  const Unit u = PREFIX ? prefix_unit(seg, blockIdx.z) : own_unit(seg, blockIdx.z);
+  const int n_rows = u.n_tok * G;
+  const int q_rows = min(16, n_rows - rt * 16);
+  if (PREFIX && q_rows <= 0) return;  // a whole block, which has asked for nothing
+  int j_lo, j_hi;
+  split_pages(u.key_lo, u.key_hi, split, n_splits, j_lo, j_hi);
+  const int n_pages = j_hi - j_lo;
+
+  if (TMA) {
+    if (threadIdx.x == 0) {
+      for (int r = 0; r < units_in_ring; ++r) {
+        tc::mbar_init(full_bar + r, 1);
+        tc::mbar_init(empty_bar + r, 4);
+      }
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    if (warp == 4) {
+      // ---- the warp that asks for pages: keys and values of a page in turn ----
+      int page_here = 0;
+      int asked = 0;
+      bool ok = true;
+      for (int i = 0; i < n_pages && ok; ++i) {
+        if (i % 32 == 0) page_here = i + lane < n_pages ? seg.table[(size_t)u.slot * seg.width + j_lo + i + lane] : 0;
+        const int page = __shfl_sync(0xffffffffu, page_here, i % 32);
+        if (lane == 0) {
+          const int row = (page * HKV + kh) * KRK_PAGE;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int n = 2 * i + half, r = n % units_in_ring;
+            if (ok && n >= units_in_ring && !tc::mbar_wait(empty_bar + r, (uint32_t)((n / units_in_ring) - 1) & 1)) {
+              atomicExch(error, 25);
+              ok = false;
+            }
+            if (!ok) break;
+            tc::mbar_expect_tx(full_bar + r, UNIT_BYTES);
+            bf16* dst = ring_s + (size_t)r * UNIT_ELEMS;
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) tc::tma_load_2d(dst + h * SUB_ELEMS, half ? &map_v : &map_k, full_bar + r, h * 64, row);
+            asked = n + 1;
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+      }
+      if (lane == 0 && !ok) tc::wait_for_copies(full_bar, units_in_ring, asked);  // what was asked for lands before the block ends
+      __syncwarp();
+      if (clustered) {  // the cluster's barriers count every thread
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        cluster.sync();
+        if (SUMS) cluster.sync();
+      }
+      return;
+    }
+  }
+
+  // ---- warps 0..3 ----
+  const bf16* qp[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int R = rt * 16 + g + 8 * h;
+    qp[h] = R < n_rows ? q + (size_t)(u.row0 + R / G) * q_stride + (size_t)(kh * G + R % G) * D : nullptr;
+  }
+  uint32_t qf[KSTEPS][4];
+  load_q(qf, qp[0], qp[1], lane);
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float o[DTILES][4];
+#pragma unroll
+  for (int n = 0; n < DTILES; ++n)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[n][c] = 0.f;
+
+  const size_t page_stride = (size_t)HKV * KRK_PAGE * D, head_off = (size_t)kh * KRK_PAGE * D;
+  auto issue = [&](int i) {  // cp.async: page i of this block's share into its stage; one group per call
+    if (i < n_pages) {
+      const int page = seg.table[(size_t)u.slot * seg.width + j_lo + i];
+      bf16* dst = ring_s + (size_t)(i % CP_STAGES) * 2 * UNIT_ELEMS;
+      load_page(dst, k_cache + (size_t)page * page_stride + head_off);
+      load_page(dst + UNIT_ELEMS, v_cache + (size_t)page * page_stride + head_off);
+    }
+    cp_async_commit();
+  };
+  bool alive = true;  // false once a wait ran out: the flow stays the same for all warps, the results are void
+  auto arrived = [&](int n) {
+    if (alive && !tc::mbar_wait(full_bar + n % units_in_ring, (uint32_t)(n / units_in_ring) & 1)) {
+      alive = false;
+      if (lane == 0) atomicExch(error, 25);
+    }
+  };
+  auto hand_back = [&](int n) {
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(empty_bar + n % units_in_ring);
+  };
+  if (!TMA) issue(0);
+  for (int i = 0; i < n_pages; ++i) {
+    const int j = j_lo + i, nk = 2 * i, nv = nk + 1;
+    bf16 *ks_s, *vs_s;
+    if (TMA) {
+      ks_s = ring_s + (size_t)(nk % units_in_ring) * UNIT_ELEMS;
+      vs_s = ring_s + (size_t)(nv % units_in_ring) * UNIT_ELEMS;
+      arrived(nk);
+    } else {
+      ks_s = ring_s + (size_t)(i % CP_STAGES) * 2 * UNIT_ELEMS;
+      vs_s = ks_s + UNIT_ELEMS;
+      issue(i + 1);
+      cp_async_wait<1>();
+      __syncthreads();
+    }
+    const int key0 = warp * 16, count = u.key_hi - j * KRK_PAGE;  // keys of the page that count
+    float s[2][4];
+    qk_tile<2, TMA>(s, qf, ks_s, key0, lane);
+    if (TMA) hand_back(nk);
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[n][c] = key0 + n * 8 + 2 * t4 + (c & 1) < count ? s[n][c] * scale_log2 : -INFINITY;
+    if (SUMS) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (g + 8 * h < q_rows) {
+          float* dst = ks.raw + ((size_t)blockIdx.z * HQ + kh * G + g + 8 * h) * ks.capacity + j * KRK_PAGE + key0 + 2 * t4;
+#pragma unroll
+          for (int n = 0; n < 2; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(s[n][2 * h], s[n][2 * h + 1]);
+        }
+    }
+    softmax_update<2>(s, m, l, o);
+    if (TMA) arrived(nv);
+    if (count < KRK_PAGE) {  // values behind the sequence's last may be anything, and zero times infinity is not zero
+      for (int e = threadIdx.x; e < (KRK_PAGE - count) * (D / 8); e += 128)
+        *reinterpret_cast<uint4*>(vs_s + page_off<TMA>(count + e / (D / 8), e % (D / 8))) = make_uint4(0, 0, 0, 0);
+      consumer_sync();
+    }
+    pv_tile<2, TMA>(o, s, vs_s, key0, lane);
+    if (TMA) hand_back(nv);
+    else __syncthreads();
+  }
+  if (!TMA) cp_async_wait<0>();
+  else if (!alive) tc::wait_for_copies(full_bar, units_in_ring, 2 * n_pages);  // the ring's place is used again
+  consumer_sync();  // every warp is done with the ring: it now holds the warps' parts
+
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float* dst = red + ((size_t)warp * 16 + g + 8 * h) * RP;
+    if (t4 == 0) { dst[D] = m[h]; dst[D + 1] = l[h]; }
+#pragma unroll
+    for (int n = 0; n < DTILES; ++n) *reinterpret_cast<float2*>(dst + n * 8 + 2 * t4) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+  }
+  consumer_sync();
+  if (clustered) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every block of the cluster has started
+  if (!PREFIX && !clustered && !wait_first) grid_dependency_wait();                    // the prefix parts are there
+  float* inbox0 = clustered ? cluster.map_shared_rank(inbox, 0) : nullptr;
+  const size_t part_step = (size_t)parts.rows * parts.HQ;
+
+  // the prefix parts of a row join what the row has from its own keys, and the row is written; a warp's lanes hold its columns
+  auto finish = [&](int r, float big, float total, float (&acc)[(D + 31) / 32]) {
+    const int R = rt * 16 + r, head = kh * G + R % G;
+    const size_t item = (size_t)(u.row0 + R / G) * HQ + head;
+    if (n_join > 0) {
+      float mine = big;
+      for (int p = lane; p < n_join; p += 32) mine = fmaxf(mine, parts.ml[p * part_step + item].x);
+      const float all = warp_max(mine), safe = all == -INFINITY ? 0.f : all;
+      const float w = exp2f(big - safe);
+      total *= w;
+#pragma unroll
+      for (int i = 0; i < (D + 31) / 32; ++i) acc[i] *= w;
+#pragma unroll 4
+      for (int p = 0; p < n_join; ++p) {
+        const float2 ml = parts.ml[p * part_step + item];
+        if (ml.y == 0.f) continue;
+        const float wp = exp2f(ml.x - safe);
+        total += wp * ml.y;
+#pragma unroll
+        for (int i = 0; i < (D + 31) / 32; ++i) {
+          const int d = lane + 32 * i;
+          if (d < D) acc[i] += wp * parts.o[(p * part_step + item) * D + d];
+        }
+      }
+    }
+    const float inv = 1.f / total;
+#pragma unroll
+    for (int i = 0; i < (D + 31) / 32; ++i) {
+      const int d = lane + 32 * i;
+      if (d < D) out[item * D + d] = __float2bfloat16_rn(acc[i] * inv);
+    }
+  };
+
+  for (int r = warp; r < q_rows; r += 4) {  // the four warps' parts of a row, in warp order
+    float mw[4], big = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) { mw[w] = red[((size_t)w * 16 + r) * RP + D]; big = fmaxf(big, mw[w]); }
+    const float safe = big == -INFINITY ? 0.f : big;
+    float wgt[4], total = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) { wgt[w] = exp2f(mw[w] - safe); total += wgt[w] * red[((size_t)w * 16 + r) * RP + D + 1]; }
+    float acc[(D + 31) / 32];
+#pragma unroll
+    for (int i = 0; i < (D + 31) / 32; ++i) {
+      const int d = lane + 32 * i;
+      acc[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) acc[i] += d < D ? wgt[w] * red[((size_t)w * 16 + r) * RP + d] : 0.f;
+    }
+    if (PREFIX) {
+      const int R = rt * 16 + r;
+      const size_t to = parts.at(part0 + split, u.row0 + R / G, kh * G + R % G);
+      if (total != 0.f)
+#pragma unroll
+        for (int i = 0; i < (D + 31) / 32; ++i)
+          if (lane + 32 * i < D) parts.o[to * D + lane + 32 * i] = acc[i];
+      if (lane == 0) parts.ml[to] = make_float2(big, total);
+    } else if (clustered) {
+      float* dst = inbox0 + ((size_t)split * inbox_rows + r) * RP;
+#pragma unroll
+      for (int i = 0; i < (D + 31) / 32; ++i)
+        if (lane + 32 * i < D) dst[lane + 32 * i] = acc[i];
+      if (lane == 0) { dst[D] = big; dst[D + 1] = total; }
+    } else {
+      finish(r, big, total, acc);
+      if (SUMS && lane == 0) lse_s[r] = safe + log2f(total);
+    }
+  }
+  if (clustered) {
+    cluster.sync();  // every block's part has arrived in the first one
+    if (split == 0) {
+      if (!wait_first) grid_dependency_wait();
+      for (int r = warp; r < q_rows; r += 4) {  // the splits' parts of a row, in split order
+        const float* mine = inbox + (size_t)r * RP;
+        float big = -INFINITY;
+        for (int p = lane; p < n_splits; p += 32) big = fmaxf(big, mine[(size_t)p * inbox_rows * RP + D]);
+        big = warp_max(big);
+        const float safe = big == -INFINITY ? 0.f : big;
+        float total = 0.f, acc[(D + 31) / 32];
+#pragma unroll
+        for (int i = 0; i < (D + 31) / 32; ++i) acc[i] = 0.f;
+        for (int p = 0; p < n_splits; ++p) {
+          const float* from = mine + (size_t)p * inbox_rows * RP;
+          const float w = exp2f(from[D] - safe);
+          total += w * from[D + 1];
+#pragma unroll
+          for (int i = 0; i < (D + 31) / 32; ++i)
+            if (lane + 32 * i < D) acc[i] += w * from[lane + 32 * i];
+        }
+        finish(r, big, total, acc);
+        if (SUMS) {
+          const float lse = safe + log2f(total);
+          for (int p = lane; p < n_splits; p += 32) cluster.map_shared_rank(lse_s, p)[r] = lse;
+        }
+      }
+    }
+    if (SUMS) cluster.sync();
+  } else if (SUMS) {
+    consumer_sync();
+  }
+  if (SUMS) {
+    const int end = min(j_hi * KRK_PAGE, u.key_hi);
+    const float* raw = ks.raw + ((size_t)blockIdx.z * HQ + kh * G) * ks.capacity;
+    for (int key = j_lo * KRK_PAGE + threadIdx.x; key < end; key += 128) {
+      float w = 0.f;
+      for (int r = 0; r < q_rows; ++r) w += exp2f(raw[(size_t)r * ks.capacity + key] - lse_s[r]);
+      const size_t place = ((size_t)u.slot * HKV + kh) * ks.capacity + key;
+      ks.sums_out[place] = key < u.start ? ks.sums[place] + w : w;
+      if (ks.positions && key >= u.start) ks.positions[place] = key + (ks.seq_shift ? ks.seq_shift[blockIdx.z] : 0);
+    }
+  }
+}
+
+template <bool PREFIX, bool SUMS>
+int launch_few_rows(bf16* out, const Parts& parts, int part0, int n_join, const void* q, int q_stride, int HQ, int HKV, const Segments& seg,
+                    const void* k, const void* v, int n_pages, int max_rows, int n_splits, float scale, bool wait_first, const KeySums& ks, int* error,
+                    cudaStream_t stream) {
+  const int G = HQ / HKV;
+  const long long row_tiles = ((long long)max_rows * G + 15) / 16;
+  const int units = PREFIX ? seg.n_groups : seg.n_seqs;
+  if (row_tiles * HKV > 65535 || units > 65535) return -3;
+  const int splits_in_cluster = PREFIX ? 1 : n_splits, inbox_rows = G < 16 ? G : 16;
+  const long long blocks = row_tiles * HKV * units * n_splits;
+  CUtensorMap map_k = {}, map_v = {};
+  int in_ring;
+  if (TMA_PAGES) {
+    const long long rows = (long long)n_pages * HKV * KRK_PAGE;
+    int rc = tc::make_map_bf16(&map_k, k, rows, D, D, KRK_PAGE);
+    if (rc == 0) rc = tc::make_map_bf16(&map_v, v, rows, D, D, KRK_PAGE);
+    if (rc) return rc;
+    // as many units as the shared memory of an SM holds for the blocks that it gets
+    const int per_sm = blocks <= 148 ? 1 : blocks <= 296 ? 2 : 3;
+    const size_t room = 216 * 1024 / per_sm, fixed = Layout(0, splits_in_cluster, inbox_rows).total - Layout(0, 1, 0).total + 2048;
+    in_ring = (int)((room > fixed ? room - fixed : 0) / UNIT_BYTES);
+    in_ring = in_ring < 2 ? 2 : in_ring > 12 ? 12 : in_ring;
+  } else {
+    in_ring = 2 * CP_STAGES;
+  }
+  const size_t smem = Layout(in_ring, splits_in_cluster, inbox_rows).total + 1024;
+  if (smem > 227 * 1024) return -2;
+  auto kern = few_rows_kernel<TMA_PAGES, PREFIX, SUMS>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return (int)e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)n_splits, (unsigned)(row_tiles * HKV), (unsigned)units);
+  cfg.blockDim = dim3(TMA_PAGES ? 160 : 128);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = splits_in_cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return (int)cudaLaunchKernelEx(&cfg, kern, map_k, map_v, out, parts, part0, n_join, (const bf16*)q, q_stride, HQ, HKV, seg, (const bf16*)k,
+                                 (const bf16*)v, scale * LOG2E, (int)row_tiles, in_ring, wait_first, ks, error);
+}
+
+}  // namespace
+
+#define KRK_SEGMENTS                                                                                                                    \
+  const int *cu_q, const int *seq_slot, const int *seq_start, const int *seq_qlen, const int *group_cu, const int *group_len,             \
+      const int *seq_group, int n_seqs, int n_groups, const int *table, int width
+#define KRK_MAKE_SEGMENTS \
+  Segments { cu_q, seq_slot, seq_start, seq_qlen, group_cu, group_len, seq_group, n_seqs, n_groups, table, width }
+
+// Parts part0 .. part0 + n_splits - 1 of the groups' prefixes; max_rows: the most rows of the step that a group has.
+KRK_API int krk_prefix_few_rows(float* o, float* ml, int rows, int part0, int n_splits, const void* q, int q_stride, int HQ, int HKV, KRK_SEGMENTS,
+                                const void* k_cache, const void* v_cache, int n_pages, int max_rows, float scale, int* error, cudaStream_t stream) {
+  if (rows == 0 || n_groups == 0) return 0;
+  const Parts parts = {o, (float2*)ml, rows, HQ};
+  return launch_few_rows<true, false>(nullptr, parts, part0, 0, q, q_stride, HQ, HKV, KRK_MAKE_SEGMENTS, k_cache, v_cache, n_pages, max_rows, n_splits,
+                                      scale, true, KeySums{}, error, stream);
+}
+
+// One token a sequence: its own keys (all, without groups), joined with the prefix parts 0 .. n_join - 1, which the launch before this one
+// writes (n_join 0: none, and the launch before may write the rows and keys themselves). n_splits: at most 8, blocks of a cluster.
+KRK_API int krk_own_single(void* out, const float* o, const float* ml, int n_join, int n_splits, const void* q, int q_stride, int HQ, int HKV,
+                           KRK_SEGMENTS, const void* k_cache, const void* v_cache, int n_pages, float scale, int* error, cudaStream_t stream) {
+  if (n_seqs == 0) return 0;
+  const Parts parts = {const_cast<float*>(o), (float2*)const_cast<float*>(ml), n_seqs, HQ};
+  return launch_few_rows<false, false>((bf16*)out, parts, 0, n_join, q, q_stride, HQ, HKV, KRK_MAKE_SEGMENTS, k_cache, v_cache, n_pages, 1, n_splits,
+                                       scale, n_join == 0, KeySums{}, error, stream);
+}
+
+// One token a sequence over all of its keys, with the weight that each key receives added to its sum (see krk_key_weights). raw: scratch,
+// [n_seqs][HQ][capacity]. The heads of a kv head fit one tile: HQ / HKV <= 16 (-2 otherwise).
+KRK_API int krk_scored_single(void* out, float* raw, const float* sums, float* sums_out, int* positions, const int* seq_shift, int capacity,
+                              int n_splits, const void* q, int q_stride, int HQ, int HKV, KRK_SEGMENTS, const void* k_cache, const void* v_cache,
+                              int n_pages, float scale, int* error, cudaStream_t stream) {
+  if (n_seqs == 0) return 0;
+  if (HQ / HKV > 16) return -2;
+  return launch_few_rows<false, true>((bf16*)out, Parts{nullptr, nullptr, n_seqs, HQ}, 0, 0, q, q_stride, HQ, HKV, KRK_MAKE_SEGMENTS, k_cache, v_cache,
+                                      n_pages, 1, n_splits, scale, true, KeySums{raw, sums, sums_out, positions, seq_shift, capacity}, error, stream);
+}
+
+#endif  // head sizes served by these kernels

@@ -76,8 +76,8 @@ partial_attention_kernel(Parts parts, int part0, int n_splits, bool own, const T
                          const T* __restrict__ k_cache, const T* __restrict__ v_cache, float scale_log2) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Shared& sm = *reinterpret_cast<Shared*>(smem_raw);
-  grid_launch_dependents();
   grid_dependency_wait();
+  grid_launch_dependents();  // in this order: the kernel behind a prefix's parts reads rows and keys before it waits for these
   const int kh = blockIdx.y, G = HQ / HKV;
   const int split = blockIdx.x % n_splits, tile = blockIdx.x / n_splits;
   const Unit u = own ? own_unit(seg, blockIdx.z) : prefix_unit(seg, blockIdx.z);
