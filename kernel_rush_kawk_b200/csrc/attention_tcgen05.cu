@@ -74,7 +74,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int PAGE_IDS = 1024;         // page-table entries a block keeps in shared memory (64 K keys)
 constexpr float RESCALE_STEP = 8.f;    // in log2 units: the reference maximum moves when outgrown by 2^8
 
-enum Bar { K_FULL = 0, V_FULL = 2, K_FREE = 4, V_FREE = 6, S_FULL = 8, P_READY = 10, O_DONE = 12, Q_FULL = 14, N_BARS = 15 };
+enum Bar { K_FULL = 0, V_FULL = 2, K_FREE = 4, V_FREE = 6, S_FULL = 8, P_READY = 10, O_DONE = 12, Q_FULL = 14, LAST_V = 15, V_CLEAN = 16, N_BARS = 18 };
 
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
@@ -117,9 +117,10 @@ struct Extras {
   const bf16* gate;
   int gate_stride, gate_mode;  // 0: none, 1: a column per head, 2: a column per element
   int out_stride;
+  float* lse;  // LSE: [rows][HQ], log2 of the sum of the row's 2^score; there values behind the sequence's end, which may be anything, count as zero
 };
 
-template <bool WIDE, int SHAPE>
+template <bool WIDE, int SHAPE, bool LSE>
 __global__ void __launch_bounds__(THREADS, 1)
 attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                          const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_o, int q_by_tma, int rows, bf16* __restrict__ out, const bf16* __restrict__ qkv, int q_stride, int HQ, int HKV,
@@ -155,6 +156,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   const int j_lo = r0.lo;                                   // tile 0 exists and starts no later than tile 1
   const int j_hi = r1.lo <= r1.hi ? max(r0.hi, r1.hi) : r0.hi;
   const int n = j_hi - j_lo + 1;
+  // LSE: the places of the block's last keys that lie behind the sequence's end, from this one on (KEYS: none)
+  const int clean_from = LSE ? min(KEYS, start + q_len - j_hi * KEYS) : KEYS;
 
   // TMA loads: the first ones by the issuer (warp 8, lane 0) before the block's first barrier, the rest by the loader
   auto load_tile = [&](unsigned char* dst, const CUtensorMap* map, uint64_t* bar, int i) {
@@ -315,6 +318,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             if (!mbar_wait(bars + P_READY + t, (j - rng[t].lo) & 1)) { give_up(8); break; }
             if (!v_ready) {
               if (!mbar_wait(bars + V_FULL + b, (i >> 1) & 1)) { give_up(9); break; }
+              if (LSE && clean_from < KEYS && i == n - 1 && !mbar_wait(bars + V_CLEAN, 0)) { give_up(9); break; }
               v_ready = true;
             }
             tc_fence_after();
@@ -344,6 +348,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         if (i + 1 < n) {  // V of the next block goes where block i - 1's was
           if (i >= 1 && !mbar_wait(bars + V_FREE + ((i + 1) & 1), ((i - 1) >> 1) & 1)) { atomicExch(error, 7); break; }
           load_v(i + 1);
+          if (LSE && i + 2 == n) mbar_arrive(bars + LAST_V);
         }
         if (i + 2 < n) {  // K of block i + 2 goes where block i's was
           if (!mbar_wait(bars + K_FREE + (i & 1), (i >> 1) & 1)) { atomicExch(error, 11); break; }
@@ -351,6 +356,19 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         }
       }
     }
+    } else if (LSE && warp == 11 && clean_from < KEYS) {
+      // The last values behind the sequence's end: zero times infinity is not zero. The stage's earlier values have been read when its last ones
+      // are asked for, so that the wait below is for these.
+      const int i = n - 1;
+      if (__all_sync(0xffffffffu, (n == 1 || mbar_wait(bars + LAST_V, 0)) && mbar_wait(bars + V_FULL + (i & 1), (i >> 1) & 1))) {
+        unsigned char* v = v_s + (i & 1) * TILE_BYTES;
+        const int pieces = (KEYS - clean_from) * 8;
+        for (int p = lane; p < DB * pieces; p += 32)
+          *reinterpret_cast<uint4*>(v + (p / pieces) * SUB + (size_t)clean_from * 128 + (p % pieces) * 16) = make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + V_CLEAN);
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -529,6 +547,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         asm volatile("" : "+r"(row));  // its token and head are worked out again: they are not kept in registers through the walk
         const int tok = row / G, head = kh * G + row % G;
         float inv = valid ? (WIDE ? ex.out_scale : 1.0f) / (l2.x + l2.y) : 0.f;
+        if (LSE && valid) ex.lse[(size_t)(row0 + tok) * HQ + head] = m + log2f(l2.x + l2.y);
         if (WIDE && ex.gate_mode == 1 && valid)
           inv /= 1.0f + expf(-__bfloat162float(ex.gate[(size_t)(row0 + tok) * ex.gate_stride + head]));
         if (WIDE && ex.gate_mode == 2) {
@@ -613,7 +632,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
 
 constexpr size_t SMEM_BYTES = 6 * TILE_BYTES + 1024 + N_BARS * 8 + 64 + PAGE_IDS * sizeof(int) + 16;
 
-template <bool WIDE, int SHAPE>
+template <bool WIDE, int SHAPE, bool LSE = false>
 int launch_tcgen05(bf16* out, const bf16* q, int q_stride, int HQ, int HKV, const int* seq_slot, const int* seq_start,
                    const int* seq_qlen, const int* cu_q, const int* table, int width, const void* k_cache, const void* v_cache,
                    int n_pages, int n_seqs, int max_q_len, int total_rows, float scale, int window, int* error, const Extras& ex,
@@ -644,7 +663,7 @@ int launch_tcgen05(bf16* out, const bf16* q, int q_stride, int HQ, int HKV, cons
     if (rc) return rc;
   }
   if (scale == 0.f) scale = 1e-30f;  // weights of zero are made by scores of minus infinity: the scale must not be zero
-  auto kern = attention_tcgen05_kernel<WIDE, SHAPE>;
+  auto kern = attention_tcgen05_kernel<WIDE, SHAPE, LSE>;
   static bool configured = false;
   if (!configured) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
@@ -673,6 +692,21 @@ KRK_API int krk_attention_prefill_tcgen05(void* out, const void* qkv, int q_stri
   ex.out_stride = HQ * D;
   return launch_tcgen05<false, 0>((bf16*)out, (const bf16*)qkv, q_stride, HQ, HKV, seq_slot, seq_start, seq_qlen, cu_q, table, width,
                                       k_cache, v_cache, n_pages, n_seqs, max_q_len, total_rows, scale, window, error, ex, stream);
+}
+
+// The same over every key, with lse [rows][HQ] float32: log2 of the sum of each row's 2^(scaled score in log2 units), by which the weights of
+// its keys can be had again.
+KRK_API int krk_attention_prefill_lse(void* out, float* lse, const void* qkv, int q_stride, int HQ, int HKV, const int* seq_slot,
+                                      const int* seq_start, const int* seq_qlen, const int* cu_q, const int* table, int width,
+                                      const void* k_cache, const void* v_cache, int n_pages, int n_seqs, int max_q_len, int total_rows,
+                                      float scale, int* error, cudaStream_t stream) {
+  if (n_seqs == 0 || max_q_len == 0) return 0;
+  if ((q_stride % 8) || ((uintptr_t)qkv & 15) || ((uintptr_t)out & 15)) return -2;
+  Extras ex = {};
+  ex.out_stride = HQ * D;
+  ex.lse = lse;
+  return launch_tcgen05<false, 0, true>((bf16*)out, (const bf16*)qkv, q_stride, HQ, HKV, seq_slot, seq_start, seq_qlen, cu_q, table, width,
+                                        k_cache, v_cache, n_pages, n_seqs, max_q_len, total_rows, scale, 0, error, ex, stream);
 }
 
 // krk_sink_window_prefill (attention_mma.cu) on the 5th-generation tensor cores: the same arguments plus the cache's number of

@@ -127,6 +127,7 @@ _ATTN_SIGNATURES = {
     "krk_attention_head_dim": [],
     "krk_attention_prefill": [_P, _P, c_int, c_int, c_int, _P, _P, _P, _P, _P, c_int, _P, _P, c_int, c_int, c_float,
                               c_int, _P],
+    "krk_attention_prefill_lse": [_P, _P, _P, c_int, c_int, c_int, _P, _P, _P, _P, _P, c_int, _P, _P, c_int, c_int, c_int, c_int, c_float, _P, _P],
     "krk_sink_window_prefill": [_P, c_int, c_float, _P, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, c_int, _P, _P, c_int,
                                 c_int, c_float, c_int, c_int, c_int, _P, c_int, c_int, _P, c_float, _P],
     "krk_sink_prefill_tcgen05": [_P, c_int, c_float, _P, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, c_int, _P, _P, c_int, c_int,

@@ -41,7 +41,7 @@ MEMORY_SOURCES = ["matrix_memory.cu", "matrix_memory_chunks.cu", "matrix_memory_
 MOE_SOURCES = ["routed.cu", "few_experts.cu", "grouped_gemm.cu"]
 CACHE_SOURCES = ["evict.cu"]
 SMALL_LIBRARIES = {"mix": MIX_SOURCES, "scan": SCAN_SOURCES, "memory": MEMORY_SOURCES, "moe": MOE_SOURCES, "cache": CACHE_SOURCES}
-PARTS_SOURCES = ["partial_attention.cu", "few_rows_attention.cu", "prefix_tcgen05.cu"]
+PARTS_SOURCES = ["partial_attention.cu", "few_rows_attention.cu", "many_rows_attention.cu", "prefix_tcgen05.cu", "key_weights_tcgen05.cu"]
 LATENT_SOURCES = ["latent_prefill.cu"]
 ATTN_SOURCES = ["attention_simple.cu", "attention_mma.cu", "attention_tcgen05.cu"]
 HEADERS = ["common.cuh", "mma.cuh", "tcgen05.cuh", "attention_noalloc.h", "attention_tiles.cuh", "partial_attention.cuh"]

@@ -60,6 +60,10 @@ _PARTS_SIGNATURES.update({
     "krk_own_single": [_P, _P, _P, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_float, _P, _P],
     "krk_scored_single": [_P, _P, _P, _P, _P, _P, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_float, _P, _P],
 })
+_PARTS_SIGNATURES.update({
+    "krk_own_rows": [_P, _P, _P, _P, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_float, _P],
+    "krk_key_weights_tcgen05": [_P, _P, _P, _P, c_int, _P, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, c_int, c_int, c_int, c_float, _P, _P],
+})
 _CACHE_SIGNATURES = {
     "krk_evict_max_seqs": [],
     "krk_evict_keys": [_P, _P, c_longlong, c_longlong, c_int, c_int, c_int, c_int, _P, c_int, _P, _P, _P, _P, c_longlong, c_int, _P, _P, c_int,
@@ -116,62 +120,21 @@ class CacheOps:
         return max(1, min(most, -(-444 // max(blocks, 1))))
 
     @staticmethod
-    def _tiles_take(qkv, cache, head_dim) -> bool:
+    def _cluster_splits(items: int) -> int:
+        """Blocks of a cluster that share the keys of a sequence's token, by the number of (sequence, kv head, row tile) items."""
+        return 8 if items <= 37 else 4 if items <= 64 else 2 if items <= 148 else 1
+
+    @staticmethod
+    def _by_mma(qkv, cache, head_dim) -> bool:
         """Whether the tensor-core kernels take these rows and pages: bfloat16, head sizes in steps of 16, rows from 4-byte, pages from 16-byte
         boundaries on."""
         return (qkv.dtype == torch.bfloat16 and head_dim % 16 == 0 and qkv.stride(0) % 2 == 0 and qkv.data_ptr() % 4 == 0
                 and (cache.k.data_ptr() | cache.v.data_ptr()) % 16 == 0)
 
     @staticmethod
-    def _cluster_splits(items: int) -> int:
-        """Blocks of a cluster that share the keys of a sequence's token, by the number of (sequence, kv head, row tile) items."""
-        return 8 if items <= 37 else 4 if items <= 64 else 2 if items <= 148 else 1
-
-    def _attention_in_parts(self, qkv, heads, head_dim, batch, cache, scale, prefix, want_lse):
-        """(output, log2 of every row's sum of 2^score or None)."""
-        lib = self._parts_lib(head_dim)
-        rows, kv = qkv.shape[0], cache.kv_heads
-        out = torch.empty((rows, heads * head_dim), dtype=qkv.dtype, device=qkv.device)
-        lse = torch.empty((rows, heads), dtype=torch.float32, device=qkv.device) if want_lse else None
-        if rows == 0:
-            return out, lse
-        segments = self._segments(batch, cache, prefix)
-        code, stream, stride, per = _code(qkv.dtype), self._stream(), qkv.stride(0), heads // kv
-        tiles = lambda n: -(-n * per // 16)
-        fast = self._tiles_take(qkv, cache, head_dim)
-        single = fast and batch.is_decode and not want_lse
-        prefix_splits, group_rows, tensor = 0, 0, False
-        if prefix is not None and prefix.max_length:
-            group_rows = prefix.max_rows(batch)
-            prefix_splits = self._splits(tiles(group_rows) * kv * prefix.n_groups)
-            tensor = (fast and hasattr(lib, "krk_prefix_tcgen05") and stride % 8 == 0 and qkv.data_ptr() % 16 == 0
-                      and group_rows * per >= self.PREFIX_TENSOR_ROWS)
-            if tensor:
-                prefix_splits = max(1, min(32, 148 // (-(-group_rows * per // 256) * kv * prefix.n_groups)))
-        own_splits = self._cluster_splits(tiles(1) * kv * batch.n_seqs) if single else self._splits(tiles(batch.max_q_len) * kv * batch.n_seqs)
-        parts = prefix_splits + (0 if single else own_splits)
-        o = torch.empty((parts, rows, heads, head_dim), dtype=torch.float32, device=qkv.device)
-        ml = torch.empty((parts, rows, heads, 2), dtype=torch.float32, device=qkv.device)
-        tail = (qkv.data_ptr(), stride, heads, kv, *segments, cache.k.data_ptr(), cache.v.data_ptr(), cache.k.shape[0])
-        if prefix_splits and fast and tiles(group_rows) * kv <= 65535:
-            self._ok((lib.krk_prefix_tcgen05 if tensor else lib.krk_prefix_few_rows)(o.data_ptr(), ml.data_ptr(), rows, 0, prefix_splits, *tail, group_rows, scale, self.error.data_ptr(), stream),
-                     "prefix attention")
-            first_done = True
-        else:
-            first_done = False
-        if single:
-            if prefix_splits and not first_done:
-                self._ok(lib.krk_partial_attention(o.data_ptr(), ml.data_ptr(), rows, 0, prefix_splits, 0, *tail[:-1], group_rows, scale, code, stream),
-                         "attention in parts")
-            self._ok(lib.krk_own_single(out.data_ptr(), o.data_ptr(), ml.data_ptr(), prefix_splits, own_splits, *tail, scale, self.error.data_ptr(), stream),
-                     "attention over own keys")
-            return out, None
-        for own, first, n, most in ((0, 0, 0 if first_done else prefix_splits, group_rows), (1, prefix_splits, own_splits, batch.max_q_len)):
-            if n:
-                self._ok(lib.krk_partial_attention(o.data_ptr(), ml.data_ptr(), rows, first, n, own, qkv.data_ptr(), stride, heads, kv, *segments,
-                                                   cache.k.data_ptr(), cache.v.data_ptr(), most, scale, code, stream), "attention in parts")
-        self._ok(lib.krk_join_parts(out.data_ptr(), _ptr(lse), o.data_ptr(), ml.data_ptr(), rows, heads, parts, code, stream), "join of parts")
-        return out, lse
+    def _by_tcgen05(qkv, head_dim) -> bool:
+        """Whether the tcgen05 kernels take rows that ``_by_mma`` takes: heads of 64 or 128, rows from 16-byte boundaries on."""
+        return head_dim in (64, 128) and qkv.stride(0) % 8 == 0 and qkv.data_ptr() % 16 == 0
 
     # -- a shared prefix -----------------------------------------------------------------
     def shared_prefix_attention(self, qkv, heads, kv_in_row, head_dim, batch, cache, scale, prefix):
@@ -182,7 +145,45 @@ class CacheOps:
         sequence, float32 or bfloat16; a captured step stays valid while the groups' number and sizes last, whatever the lengths become."""
         self._check_step("shared prefix attention", qkv, heads, kv_in_row, head_dim, batch, cache)
         prefix.check(batch, cache)
-        return self._attention_in_parts(qkv, heads, head_dim, batch, cache, float(scale), prefix, False)[0]
+        lib, rows, kv, per, D = self._parts_lib(head_dim), qkv.shape[0], cache.kv_heads, heads // cache.kv_heads, head_dim
+        out = torch.empty((rows, heads * D), dtype=qkv.dtype, device=qkv.device)
+        if rows == 0:
+            return out
+        scale, stream, error = float(scale), self._stream(), self.error.data_ptr()
+        step = (qkv.data_ptr(), qkv.stride(0), heads, kv, *self._segments(batch, cache, prefix), cache.k.data_ptr(), cache.v.data_ptr())
+        by_mma = self._by_mma(qkv, cache, D)
+        # the prefixes' parts, then the own keys, which join them
+        splits, own_splits, group_rows, tensor = 0, 0, 0, False
+        if prefix.max_length:
+            group_rows = prefix.max_rows(batch)
+            tiles = -(-group_rows * per // 16) * kv
+            tensor = by_mma and group_rows * per >= self.PREFIX_TENSOR_ROWS and self._by_tcgen05(qkv, D)
+            if tensor:
+                splits = max(1, min(32, 148 // (-(-group_rows * per // 256) * kv * prefix.n_groups)))
+            else:
+                splits = self._splits(tiles * prefix.n_groups)
+        if not by_mma:
+            own_splits = self._splits(-(-batch.max_q_len * per // 16) * kv * batch.n_seqs)
+        parts = splits + own_splits
+        scratch = torch.empty(parts * rows * heads * (D + 2), dtype=torch.float32, device=qkv.device)
+        o = scratch.data_ptr()
+        ml = o + 4 * parts * rows * heads * D
+        if splits:
+            if tensor or (by_mma and tiles <= 65535):
+                self._ok((lib.krk_prefix_tcgen05 if tensor else lib.krk_prefix_few_rows)(o, ml, rows, 0, splits, *step, cache.k.shape[0], group_rows, scale,
+                                                                                         error, stream), "prefix attention")
+            else:
+                self._ok(lib.krk_partial_attention(o, ml, rows, 0, splits, 0, *step, group_rows, scale, _code(qkv.dtype), stream), "prefix attention")
+        if not by_mma:
+            self._ok(lib.krk_partial_attention(o, ml, rows, splits, own_splits, 1, *step, batch.max_q_len, scale, _code(qkv.dtype), stream),
+                     "attention over own keys")
+            self._ok(lib.krk_join_parts(out.data_ptr(), None, o, ml, rows, heads, parts, _code(qkv.dtype), stream), "join of parts")
+        elif batch.is_decode:
+            self._ok(lib.krk_own_single(out.data_ptr(), o, ml, splits, self._cluster_splits(-(-per // 16) * kv * batch.n_seqs), *step, cache.k.shape[0],
+                                        scale, error, stream), "attention over own keys")
+        else:
+            self._ok(lib.krk_own_rows(out.data_ptr(), None, o, ml, rows, splits, *step, batch.max_q_len, scale, stream), "attention over own keys")
+        return out
 
     # -- weights per key -------------------------------------------------------------------
     def _check_scores(self, what, scores, positions, cache, extra=()):
@@ -203,22 +204,46 @@ class CacheOps:
         self._check_scores("scored attention", scores, positions, cache, (("out_scores", out_scores, torch.float32),))
         if observe is not None and observe < 1:
             raise KernelError(f"scored attention: at least one query a sequence is observed, got {observe}")
-        kv, rows = cache.kv_heads, qkv.shape[0]
-        if rows and batch.is_decode and heads // kv <= 16 and self._tiles_take(qkv, cache, head_dim):
-            out = torch.empty((rows, heads * head_dim), dtype=qkv.dtype, device=qkv.device)
-            raw = torch.empty((rows, heads, scores.shape[2]), dtype=torch.float32, device=qkv.device)
-            self._ok(self._parts_lib(head_dim).krk_scored_single(
-                out.data_ptr(), raw.data_ptr(), scores.data_ptr(), out_scores.data_ptr(), _ptr(positions), _ptr(getattr(batch, "seq_shift", None)),
-                scores.shape[2], self._cluster_splits(kv * rows), qkv.data_ptr(), qkv.stride(0), heads, kv, *self._segments(batch, cache, None),
-                cache.k.data_ptr(), cache.v.data_ptr(), cache.k.shape[0], float(scale), self.error.data_ptr(), self._stream()), "scored attention")
+        lib, rows, kv, per, D = self._parts_lib(head_dim), qkv.shape[0], cache.kv_heads, heads // cache.kv_heads, head_dim
+        out = torch.empty((rows, heads * D), dtype=qkv.dtype, device=qkv.device)
+        if rows == 0:
             return out
-        out, lse = self._attention_in_parts(qkv, heads, head_dim, batch, cache, float(scale), None, True)
-        if rows:
+        scale, stream, error, capacity = float(scale), self._stream(), self.error.data_ptr(), scores.shape[2]
+        counts = (scores.data_ptr(), out_scores.data_ptr(), _ptr(positions), _ptr(getattr(batch, "seq_shift", None)), capacity)
+        segments = self._segments(batch, cache, None)
+        q = (qkv.data_ptr(), qkv.stride(0), heads, kv)
+        pages = (cache.k.data_ptr(), cache.v.data_ptr())
+        by_mma = self._by_mma(qkv, cache, D)
+        if by_mma and batch.is_decode and per <= 16:
+            raw = torch.empty(rows * heads * capacity, dtype=torch.float32, device=qkv.device)
+            self._ok(lib.krk_scored_single(out.data_ptr(), raw.data_ptr(), *counts, self._cluster_splits(kv * rows), *q, *segments, *pages,
+                                           cache.k.shape[0], scale, error, stream), "scored attention")
+            return out
+        # the output with every row's log sum, then the weights by these
+        lse = torch.empty(rows * heads, dtype=torch.float32, device=qkv.device)
+        by_tcgen05 = by_mma and self._by_tcgen05(qkv, D)
+        if by_tcgen05 and batch.max_q_len * per >= 128 and self.use_tcgen05_attention:
+            self._ok(self._attn_lib(D).krk_attention_prefill_lse(
+                out.data_ptr(), lse.data_ptr(), *q, batch.seq_slot.data_ptr(), batch.seq_start.data_ptr(), batch.seq_qlen.data_ptr(), batch.cu_q.data_ptr(),
+                cache.table.data_ptr(), cache.width, *pages, cache.k.shape[0], batch.n_seqs, batch.max_q_len, rows, scale, error, stream), "scored attention")
+        elif by_mma:
+            self._ok(lib.krk_own_rows(out.data_ptr(), lse.data_ptr(), None, None, rows, 0, *q, *segments, *pages, batch.max_q_len, scale, stream),
+                     "scored attention")
+        else:
+            parts = self._splits(-(-batch.max_q_len * per // 16) * kv * batch.n_seqs)
+            scratch = torch.empty(parts * rows * heads * (D + 2), dtype=torch.float32, device=qkv.device)
+            o = scratch.data_ptr()
+            ml = o + 4 * parts * rows * heads * D
+            self._ok(lib.krk_partial_attention(o, ml, rows, 0, parts, 1, *q, *segments, *pages, batch.max_q_len, scale, _code(qkv.dtype), stream),
+                     "scored attention")
+            self._ok(lib.krk_join_parts(out.data_ptr(), lse.data_ptr(), o, ml, rows, heads, parts, _code(qkv.dtype), stream), "join of parts")
+        if by_tcgen05 and not batch.is_decode and per <= 64:
+            self._ok(lib.krk_key_weights_tcgen05(*counts, lse.data_ptr(), int(observe or 0), *q, *segments, pages[0], cache.k.shape[0], rows,
+                                                 batch.max_kv_len, scale, error, stream), "weights of keys")
+        else:
             blocks = max(1, min(cache.width, -(-888 // (kv * batch.n_seqs))))
-            self._ok(self._parts_lib(head_dim).krk_key_weights(
-                scores.data_ptr(), out_scores.data_ptr(), _ptr(positions), _ptr(getattr(batch, "seq_shift", None)), scores.shape[2], lse.data_ptr(),
-                int(observe or 0), qkv.data_ptr(), qkv.stride(0), heads, kv, *self._segments(batch, cache, None), cache.k.data_ptr(), blocks,
-                float(scale), _code(qkv.dtype), self._stream()), "weights of keys")
+            self._ok(lib.krk_key_weights(*counts, lse.data_ptr(), int(observe or 0), *q, *segments, pages[0], blocks, scale, _code(qkv.dtype), stream),
+                     "weights of keys")
         return out
 
     # -- eviction ----------------------------------------------------------------------------

@@ -125,10 +125,11 @@ partial_attention_kernel(Parts parts, int part0, int n_splits, bool own, const T
       for (int o = 4; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       const float m_old = sm.m[r], m_new = fmaxf(m_old, mx), safe = m_new == -INFINITY ? 0.f : m_new;
       float sum = 0.f;
+      const int row_end = min(key_end, u.start + (tile * TILE + r) / G + 1) - j * KRK_PAGE;  // behind the last key of the page that the row sees
       for (int key = t; key < KRK_PAGE; key += 8) {
         const float p = exp2f(sm.s[key][r] - safe);
-        sm.s[key][r] = p;
-        sum += p;
+        sm.s[key][r] = key < row_end ? p : -1.f;  // no weight: what the value is does not count
+        if (key < row_end) sum += p;
       }
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -147,6 +148,7 @@ partial_attention_kernel(Parts parts, int part0, int n_splits, bool own, const T
 #pragma unroll
       for (int i = 0; i < PER_LANE; ++i) acc[r][i] *= a;
     }
+    const bool whole = j * KRK_PAGE + KRK_PAGE <= min(key_end, u.start + tile * TILE / G + 1);  // every row sees the page to its end
     for (int key = warp * 16; key < warp * 16 + 16; ++key) {
       float p[TILE];
 #pragma unroll
@@ -156,7 +158,8 @@ partial_attention_kernel(Parts parts, int part0, int n_splits, bool own, const T
         const int d = lane + 32 * i;
         const float v = d < DPAD ? sm.v[key][d] : 0.f;
 #pragma unroll
-        for (int r = 0; r < TILE; ++r) acc[r][i] = fmaf(p[r], v, acc[r][i]);
+        for (int r = 0; r < TILE; ++r)
+          if (whole || p[r] >= 0.f || p[r] != p[r]) acc[r][i] = fmaf(p[r], v, acc[r][i]);
       }
     }
   }

@@ -133,6 +133,26 @@ def test_shared_prefix_attention_in_a_captured_step(ops, dtype):
     assert torch.equal(out, eager)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [20, 48, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_shared_prefix_attention_beside_keys_that_are_no_numbers(ops, dtype, dim, bad):
+    """A token whose key and value are no numbers spoils the rows that see it, and no row before it nor any other sequence."""
+    heads, kv = 6, 2
+    held, brings = [128, 128 + 70], [40, 90]
+    qkv, batch, cache = make_step(DEVICE, dtype, heads, kv, dim, held, brings, 9, ([2], [128]))
+    call = lambda: ops.shared_prefix_attention(qkv, heads, kv, dim, batch, cache, 0.1, groups([2], [128]))
+    want = call()
+    at = held[1] + 33  # a token in the middle of the second sequence's
+    page = cache.table[batch.slots[1], at // PAGE]
+    cache.v[page, 1, at % PAGE, 3] = bad
+    cache.k[page, 0, at % PAGE] = bad
+    got = call()
+    first = brings[0] + 33
+    assert torch.equal(got[:first], want[:first]), "rows that do not see it"
+    assert not torch.isfinite(got[first:, heads * dim // 2 + 3]).any(), "rows that do"
+
+
 # -- weights per key -----------------------------------------------------------------------------------------
 SCORED = [
     ([0], [1], None), ([63], [1], None), ([64, 700, 5], [1, 1, 1], 4), ([0, 0, 0], [1, 64, 200], None), ([0, 0], [130, 65], 32),
