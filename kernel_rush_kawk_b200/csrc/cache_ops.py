@@ -62,7 +62,7 @@ _PARTS_SIGNATURES.update({
 })
 _PARTS_SIGNATURES.update({
     "krk_own_rows": [_P, _P, _P, _P, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_float, _P],
-    "krk_key_weights_tcgen05": [_P, _P, _P, _P, c_int, _P, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, c_int, c_int, c_int, c_float, _P, _P],
+    "krk_key_weights_tcgen05": [_P, _P, _P, _P, c_int, _P, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, c_int, c_int, c_int, c_int, c_float, _P, _P],
 })
 _CACHE_SIGNATURES = {
     "krk_evict_max_seqs": [],
@@ -114,15 +114,20 @@ class CacheOps:
                 cache.table.data_ptr(), cache.width)
 
     @staticmethod
-    def _splits(blocks: int, most: int = 32) -> int:
-        """Parts that the keys of a unit of work are split into, so that the blocks fill the device three times over. By the numbers of rows
+    def _splits(blocks: int, wanted: int = 444) -> int:
+        """Parts that the keys of a unit of work are split into, so that there are blocks enough for the device. By the numbers of rows
         and heads, never by lengths: a captured step stays valid."""
-        return max(1, min(most, -(-444 // max(blocks, 1))))
+        return max(1, min(32, -(-wanted // max(blocks, 1))))
 
     @staticmethod
-    def _cluster_splits(items: int) -> int:
-        """Blocks of a cluster that share the keys of a sequence's token, by the number of (sequence, kv head, row tile) items."""
-        return 8 if items <= 37 else 4 if items <= 64 else 2 if items <= 148 else 1
+    def _cluster_splits(items: int, all_keys: bool) -> int:
+        """Blocks of a cluster that share the keys of a sequence's token, by the number of (sequence, kv head, row tile) items. ``all_keys``: all
+        that the sequence holds, unequally many; else those behind a shared prefix, which are few. One sequence after 1,087 tokens in 1, 2, 4 and 8: 18.6,
+        14.4, 12.4 and 10.3 us; 32 sequences after 2,000 to 4,500: 101, 87.9, 88.5 and 95.9. Behind a prefix, eight sequences with up to
+        400 keys of their own: 20.6, 20.7, 22.7 and 25.2, 64 with up to 500: 42.7, 51.2, 60.3 and 80."""
+        if all_keys:
+            return 8 if items <= 64 else 4 if items <= 148 else 2 if items <= 592 else 1
+        return 4 if items <= 37 else 2 if items <= 148 else 1
 
     @staticmethod
     def _by_mma(qkv, cache, head_dim) -> bool:
@@ -161,7 +166,9 @@ class CacheOps:
             if tensor:
                 splits = max(1, min(32, 148 // (-(-group_rows * per // 256) * kv * prefix.n_groups)))
             else:
-                splits = self._splits(tiles * prefix.n_groups)
+                # eight sequences of four heads behind 1,024 positions: 16.5 us with one block an SM, 18.6 with two, 22.7 with three (the
+                # parts that the own keys' kernel has to join grow with them)
+                splits = self._splits(tiles * prefix.n_groups, 148 if by_mma else 444)
         if not by_mma:
             own_splits = self._splits(-(-batch.max_q_len * per // 16) * kv * batch.n_seqs)
         parts = splits + own_splits
@@ -179,7 +186,7 @@ class CacheOps:
                      "attention over own keys")
             self._ok(lib.krk_join_parts(out.data_ptr(), None, o, ml, rows, heads, parts, _code(qkv.dtype), stream), "join of parts")
         elif batch.is_decode:
-            self._ok(lib.krk_own_single(out.data_ptr(), o, ml, splits, self._cluster_splits(-(-per // 16) * kv * batch.n_seqs), *step, cache.k.shape[0],
+            self._ok(lib.krk_own_single(out.data_ptr(), o, ml, splits, self._cluster_splits(-(-per // 16) * kv * batch.n_seqs, False), *step, cache.k.shape[0],
                                         scale, error, stream), "attention over own keys")
         else:
             self._ok(lib.krk_own_rows(out.data_ptr(), None, o, ml, rows, splits, *step, batch.max_q_len, scale, stream), "attention over own keys")
@@ -216,7 +223,7 @@ class CacheOps:
         by_mma = self._by_mma(qkv, cache, D)
         if by_mma and batch.is_decode and per <= 16:
             raw = torch.empty(rows * heads * capacity, dtype=torch.float32, device=qkv.device)
-            self._ok(lib.krk_scored_single(out.data_ptr(), raw.data_ptr(), *counts, self._cluster_splits(kv * rows), *q, *segments, *pages,
+            self._ok(lib.krk_scored_single(out.data_ptr(), raw.data_ptr(), *counts, self._cluster_splits(kv * rows, True), *q, *segments, *pages,
                                            cache.k.shape[0], scale, error, stream), "scored attention")
             return out
         # the output with every row's log sum, then the weights by these
@@ -239,7 +246,8 @@ class CacheOps:
             self._ok(lib.krk_join_parts(out.data_ptr(), lse.data_ptr(), o, ml, rows, heads, parts, _code(qkv.dtype), stream), "join of parts")
         if by_tcgen05 and not batch.is_decode and per <= 64:
             self._ok(lib.krk_key_weights_tcgen05(*counts, lse.data_ptr(), int(observe or 0), *q, *segments, pages[0], cache.k.shape[0], rows,
-                                                 batch.max_kv_len, scale, error, stream), "weights of keys")
+                                                 min(batch.max_q_len, observe or batch.max_q_len), batch.max_kv_len, scale, error, stream),
+                     "weights of keys")
         else:
             blocks = max(1, min(cache.width, -(-888 // (kv * batch.n_seqs))))
             self._ok(lib.krk_key_weights(*counts, lse.data_ptr(), int(observe or 0), *q, *segments, pages[0], blocks, scale, _code(qkv.dtype), stream),

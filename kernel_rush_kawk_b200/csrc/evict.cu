@@ -6,8 +6,8 @@
 // keys in any order and keys are stored rotated, so a moved row is as good as before; its position moves with its sum. Sources lie
 // at or behind `keep` and destinations below it: the rows move in place, in any order, and no more of them than have to.
 //
-// Two launches: a block per head finds what stays (the n-th largest key of 32 bits by its digits, eight bits a pass, then the rows in
-// order), and blocks over all moves of all heads copy the rows.
+// A block per head finds what stays: a line through the positions and one through the other rows' sums, then the rows in order. It moves the
+// rows as well where there are heads enough; else blocks over all moves of all heads do, in a second launch.
 #include "common.cuh"
 
 namespace {
@@ -17,8 +17,6 @@ struct Sequences {
   int slot[MAX_SEQS], length[MAX_SEQS];
 };
 
-constexpr int THREADS = 512, WARPS = THREADS / 32;
-
 // Order of a sum as an unsigned number: a NaN counts as the largest, zeros are equal.
 __device__ __forceinline__ unsigned order_of(float x) {
   const unsigned u = __float_as_uint(x == 0.f ? 0.f : x);
@@ -26,203 +24,377 @@ __device__ __forceinline__ unsigned order_of(float x) {
 }
 __device__ __forceinline__ unsigned order_of(int p) { return (unsigned)p ^ 0x80000000u; }
 
+// Lists of a block of T threads; behind it, in dynamic shared memory, the rows' keys (STAGED) and a bit for each row that is kept.
+constexpr int MAX_CANDIDATES = 512, FEW = 64;
+template <int T, int BINS>
+struct Scratch {
+  static constexpr int COPIES = T > 128 ? 4 : 1;
+  int hist[BINS * COPIES];  // counters of a bin side by side, a lane's by its number: many rows of one warp fall into the same bins
+  unsigned cand_key[MAX_CANDIDATES];
+  int cand_row[MAX_CANDIDATES];
+  int part[2][32];
+  unsigned low, high;
+  int bin, want, n_cand, row;
+};
+
+// A line through the rows' keys: exactly the wanted number of rows lies above it.
 struct Line {
   unsigned value;
-  int row;  // of the rows of exactly `value`, those up to this one are above the line
+  int row;  // of the rows of exactly `value`, those up to this one
   __device__ __forceinline__ bool above(unsigned key, int r) const { return key > value || (key == value && r <= row); }
 };
 
-struct Scratch {
-  int hist[256];
-  int warp_sum[WARPS];
-  unsigned value;
-  int want, equal, row;
-};
-
-// Sum of `v` over the threads before this one (the block's total in `total`). All threads call it.
-__device__ __forceinline__ int scan_before(int v, Scratch& sc, int& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
+// The block's least and largest of the threads' (lo, hi).
+template <int T, int BINS>
+__device__ __forceinline__ void block_range(unsigned& lo, unsigned& hi, Scratch<T, BINS>& sc) {
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if (threadIdx.x == 0) { sc.low = 0xffffffffu; sc.high = 0; }
   __syncthreads();
-  if (lane == 31) sc.warp_sum[warp] = x;
+  if ((threadIdx.x & 31) == 0) { atomicMin(&sc.low, lo); atomicMax(&sc.high, hi); }
   __syncthreads();
-  int before = 0;
-  total = 0;
-  for (int w = 0; w < WARPS; ++w) {
-    if (w < warp) before += sc.warp_sum[w];
-    total += sc.warp_sum[w];
-  }
-  return before + x - v;
+  lo = sc.low;
+  hi = sc.high;
 }
 
-// The line above which exactly n of the rows 0 .. L - 1 lie that `key` gives a value for (its second result).
-template <typename Key>
-__device__ Line line_of(int n, int L, Scratch& sc, Key key) {
+// The line above which exactly n of the rows 0 .. L - 1 lie that `key` gives a value for (its second result), all of them from lo to hi; n
+// is at most their number. The range is cut into bins; the one that the line falls into holds few rows mostly, whose order is
+// counted out pair by pair, else it is the next range.
+// DENSE: numbers of which the n largest may be neighbours (positions), which one count shows.
+template <bool DENSE, int T, int BINS, typename Key>
+__device__ Line line_of(int n, int L, unsigned lo, unsigned hi, Scratch<T, BINS>& sc, Key key) {
   if (n <= 0) return Line{0xffffffffu, -1};
-  unsigned prefix = 0, mask = 0;
-  int want = n;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < 256; i += THREADS) sc.hist[i] = 0;
-    __syncthreads();
-    for (int r = threadIdx.x; r < L; r += THREADS) {
+  constexpr int BITS = BINS == 512 ? 9 : 11, EACH = BINS / T, COPIES = Scratch<T, BINS>::COPIES;
+  static_assert(1 << BITS == BINS && BINS % T == 0, "");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (DENSE && hi - lo >= (unsigned)n) {
+    int mine = 0;
+#pragma unroll 4
+    for (int r = threadIdx.x; r < L; r += T) {
       unsigned v;
-      if (key(r, v) && (v & mask) == prefix) atomicAdd(&sc.hist[(v >> shift) & 255], 1);
+      mine += key(r, v) && v > hi - n;
+    }
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if (lane == 0) sc.part[0][warp] = mine;
+    __syncthreads();
+    const int count = __reduce_add_sync(0xffffffffu, lane < T / 32 ? sc.part[0][lane] : 0);
+    if (count == n) return Line{hi - n + 1, 0x7fffffff};
+  }
+  int want = n;
+  for (;;) {
+    const int shift = max(0, 32 - __clz(hi - lo) - BITS);  // (a range of one value: shift 0)
+#pragma unroll
+    for (int i = 0; i < EACH * COPIES; ++i) sc.hist[threadIdx.x + i * T] = 0;
+    if (threadIdx.x == 0) sc.n_cand = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int r = threadIdx.x; r < L; r += T) {
+      unsigned v;
+      if (key(r, v) && v - lo <= hi - lo) atomicAdd(&sc.hist[((v - lo) >> shift) * COPIES + lane % COPIES], 1);
     }
     __syncthreads();
-    if (threadIdx.x < 32) {  // lane: eight digits from the top
-      int mine = 0;
-      for (int i = 0; i < 8; ++i) mine += sc.hist[255 - (threadIdx.x * 8 + i)];
-      int x = mine;
+    auto count_of = [&](int bin) {
+      int c = 0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if ((int)threadIdx.x >= o) x += y;
+      for (int e = 0; e < COPIES; ++e) c += sc.hist[bin * COPIES + e];
+      return c;
+    };
+    int mine = 0;  // of a thread's bins, from the top
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) mine += count_of(BINS - 1 - (threadIdx.x * EACH + i));
+    int x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) sc.part[1][warp] = x;
+    __syncthreads();
+    int above = x - mine + __reduce_add_sync(0xffffffffu, lane < warp ? sc.part[1][lane] : 0);
+    if (above < want && above + mine >= want)
+      for (int i = 0; i < EACH; ++i) {
+        const int at = BINS - 1 - (threadIdx.x * EACH + i), c = count_of(at);
+        if (above + c >= want) {
+          sc.bin = at;
+          sc.want = want - above;
+          break;
+        }
+        above += c;
       }
-      int above = x - mine;
-      if (above < want && x >= want) {
-        for (int i = 0; i < 8; ++i) {
-          const int digit = 255 - (threadIdx.x * 8 + i), c = sc.hist[digit];
-          if (above + c >= want) {
-            sc.value = prefix | ((unsigned)digit << shift);
-            sc.want = want - above;
-            sc.equal = c;
-            break;
-          }
-          above += c;
+    __syncthreads();
+    const int in_bin = count_of(sc.bin);
+    lo += (unsigned)sc.bin << shift;
+    hi = lo + min(hi - lo, (1u << shift) - 1);
+    want = sc.want;
+    if (in_bin == want) return Line{lo, 0x7fffffff};  // the bin as a whole (a key on its lower edge counts with all of its rows)
+    if (in_bin <= FEW || (shift == 0 && in_bin <= MAX_CANDIDATES)) {  // (of more, another cut leaves fewer, and costs less than their pairs)
+#pragma unroll 4
+      for (int r = threadIdx.x; r < L; r += T) {
+        unsigned v;
+        if (key(r, v) && v - lo <= hi - lo) {
+          const int c = atomicAdd(&sc.n_cand, 1);
+          sc.cand_key[c] = v;
+          sc.cand_row[c] = r;
         }
       }
+      __syncthreads();
+      for (int c = threadIdx.x; c < in_bin; c += T) {
+        const unsigned v = sc.cand_key[c];
+        const int r = sc.cand_row[c];
+        int before = 0;
+#pragma unroll 8
+        for (int e = 0; e < in_bin; ++e) before += sc.cand_key[e] > v || (sc.cand_key[e] == v && sc.cand_row[e] < r);
+        if (before == want - 1) { sc.low = v; sc.row = r; }
+      }
+      __syncthreads();
+      return Line{sc.low, sc.row};
     }
-    __syncthreads();
-    prefix = sc.value;
-    want = sc.want;
-    mask |= 255u << shift;
+    if (shift == 0) break;  // more rows of one value than the list holds
+    __syncthreads();        // the table is cleared for the next range
   }
-  Line line{prefix, 0x7fffffff};
-  if (sc.equal > want) {  // more rows of this value than are wanted: the first of them
-    if (threadIdx.x == 0) sc.row = -1;
-    int seen = 0;
-    for (int r0 = 0; r0 < L && seen < want; r0 += THREADS) {
-      const int r = r0 + threadIdx.x;
-      unsigned v;
-      const bool is = r < L && key(r, v) && v == prefix;
-      int total;
-      const int before = seen + scan_before(is, sc, total);
-      if (is && before == want - 1) sc.row = r;
-      seen += total;
-    }
-    __syncthreads();
-    line.row = sc.row;
-  }
-  return line;
-}
-
-__global__ void __launch_bounds__(THREADS)
-choose_rows_kernel(const float* scores, const int* positions, float* scores_out, int* positions_out, size_t run_stride, int HKV, int capacity,
-                   const Sequences seqs, int n_seqs, int keep, int recent, int* __restrict__ moves, int* __restrict__ n_moves, int max_moves,
-                   int* seq_start, int* row_pos, int* seq_shift) {
-  __shared__ Scratch sc;
-  grid_launch_dependents();
-  grid_dependency_wait();
-  const int kh = blockIdx.x % HKV, seq = blockIdx.x / HKV % n_seqs, run = blockIdx.x / HKV / n_seqs;
-  const int L = seqs.length[seq];
-  const size_t base = run * run_stride + ((size_t)seqs.slot[seq] * HKV + kh) * capacity;
-  const float* sum = scores + base;
-  const int* pos = positions + base;
-  float* sum_out = scores_out + base;
-  int* pos_out = positions_out + base;
-  const bool apart = sum != sum_out, pos_apart = pos != pos_out;
-  if (L <= keep) {
-    for (int r = threadIdx.x; r < L; r += THREADS) {
-      if (apart) sum_out[r] = sum[r];
-      if (pos_apart) pos_out[r] = pos[r];
-    }
-    if (threadIdx.x == 0) n_moves[blockIdx.x] = 0;
-    return;
-  }
-  if (seq_start && kh == 0 && run == 0 && threadIdx.x == 0) {  // the step's description follows
-    seq_start[seq] -= L - keep;
-    row_pos[seq] -= L - keep;
-    seq_shift[seq] += L - keep;
-  }
-  const Line newest = line_of(recent, L, sc, [&](int r, unsigned& v) { v = order_of(pos[r]); return true; });
-  const Line heavy = line_of(keep - recent, L, sc, [&](int r, unsigned& v) {
-    v = order_of(sum[r]);
-    return !newest.above(order_of(pos[r]), r);
-  });
-  // the rows in order: free ones below `keep`, kept ones from there on
-  int* to = moves + (size_t)blockIdx.x * 2 * max_moves;
-  int* from = to + max_moves;
-  int n_free = 0, n_kept = 0;
-  for (int r0 = 0; r0 < L; r0 += THREADS) {
+  // the first of the rows of this value
+  if (threadIdx.x == 0) sc.row = -1;
+  int seen = 0;
+  for (int r0 = 0; r0 < L && seen < want; r0 += T) {
     const int r = r0 + threadIdx.x;
-    bool kept = false;
-    if (r < L) kept = newest.above(order_of(pos[r]), r) || heavy.above(order_of(sum[r]), r);
-    const bool is_free = r < keep && !kept, moves_down = r >= keep && r < L && kept;
-    // a chunk of rows may lie on both sides of `keep`: both counts in one scan
-    int total;
-    const int before = scan_before((is_free ? 1 : 0) | (moves_down ? 1 << 16 : 0), sc, total);
-    if (is_free) to[n_free + (before & 0xffff)] = r;
-    if (moves_down) from[n_kept + (before >> 16)] = r;
-    if (r < keep && kept) {
-      if (apart) sum_out[r] = sum[r];
-      if (pos_apart) pos_out[r] = pos[r];
-    }
-    n_free += total & 0xffff;
-    n_kept += total >> 16;
+    unsigned v;
+    const bool is = r < L && key(r, v) && v == lo;
+    const unsigned votes = __ballot_sync(0xffffffffu, is);
+    __syncthreads();
+    if (lane == 0) sc.part[0][warp] = __popc(votes);
+    __syncthreads();
+    const int here = lane < T / 32 ? sc.part[0][lane] : 0;
+    const int before = seen + __reduce_add_sync(0xffffffffu, lane < warp ? here : 0) + __popc(votes & ((1u << lane) - 1));
+    if (is && before == want - 1) sc.row = r;
+    seen += __reduce_add_sync(0xffffffffu, here);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n_kept; i += THREADS) {
-    const int s = from[i], d = to[i];
-    sum_out[d] = sum[s];
-    pos_out[d] = pos[s];
-  }
-  if (threadIdx.x == 0) n_moves[blockIdx.x] = n_kept;
+  return Line{lo, sc.row};
 }
 
-// Piece: uint4, unsigned, unsigned short; a row is `pieces` of them.
-constexpr int MOVE_THREADS = 256;
+struct Pools {  // of keys and of values, as pieces of 16, 4 or 2 bytes; a row is `pieces` of them
+  void *k, *v;
+  size_t k_run, v_run;  // between runs, in pieces
+  int k_pieces, v_pieces;
+  const int* table;
+  int width, piece_bytes;
+};
+
+// Rows `from` to rows `to` of one head, this thread's share of n moves: `workers` threads share them, 32 or fewer lanes a move.
 template <typename Piece>
-__global__ void __launch_bounds__(MOVE_THREADS)
-move_rows_kernel(Piece* k, Piece* v, size_t k_run, size_t v_run, int k_pieces, int v_pieces, int HKV, const Sequences seqs, int n_seqs,
-                 const int* __restrict__ table, int width, const int* __restrict__ moves, const int* __restrict__ n_moves, int max_moves,
-                 int blocks_per_head) {
-  grid_launch_dependents();
-  grid_dependency_wait();
-  const int head = blockIdx.x / blocks_per_head, part = blockIdx.x % blocks_per_head;
-  const int n = n_moves[head];
-  const int kh = head % HKV, seq = head / HKV % n_seqs, run = head / HKV / n_seqs;
-  const int* to = moves + (size_t)head * 2 * max_moves;
-  const int* from = to + max_moves;
-  const int* row = table + (size_t)seqs.slot[seq] * width;
-  const int both = k_pieces + v_pieces;
-  constexpr int AHEAD = 4;
-  const long long total = (long long)n * both, step = (long long)blocks_per_head * MOVE_THREADS;
-  for (long long i0 = (long long)part * MOVE_THREADS + threadIdx.x; i0 < total; i0 += step * AHEAD) {
-    Piece got[AHEAD];
-    Piece* dst[AHEAD];
+__device__ __forceinline__ void move_rows(const Pools& p, const int* __restrict__ to, const int* __restrict__ from, int n, int run, int slot, int kh, int HKV,
+                                          int worker, int workers) {
+  const int both = p.k_pieces + p.v_pieces;
+  int lanes = 32;  // of a warp that share a move
+  while (lanes > 1 && lanes >= 2 * both) lanes >>= 1;
+  const int first = worker / lanes, step = workers / lanes, c0 = worker % lanes;
+  const int* row = p.table + (size_t)slot * p.width;
+  Piece* kp = reinterpret_cast<Piece*>(p.k) + run * p.k_run;
+  Piece* vp = reinterpret_cast<Piece*>(p.v) + run * p.v_run;
+  constexpr int AHEAD = 4;  // moves whose rows are on their way together
+  for (int m0 = first; m0 < n; m0 += step * AHEAD) {
+    int s[AHEAD], d[AHEAD];
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      const long long i = i0 + a * step;
-      dst[a] = nullptr;
-      if (i < total) {
-        const int move = (int)(i / both), c = (int)(i % both), s = from[move], d = to[move];
-        const bool key = c < k_pieces;
-        Piece* pool = key ? k + run * k_run : v + run * v_run;
-        const int pieces = key ? k_pieces : v_pieces, at = key ? c : c - k_pieces;
-        got[a] = pool[(((size_t)row[s / KRK_PAGE] * HKV + kh) * KRK_PAGE + s % KRK_PAGE) * pieces + at];
-        dst[a] = pool + (((size_t)row[d / KRK_PAGE] * HKV + kh) * KRK_PAGE + d % KRK_PAGE) * pieces + at;
-      }
+      const int m = m0 + a * step;
+      s[a] = m < n ? from[m] : -1;
+      d[a] = m < n ? to[m] : 0;
+    }
+    size_t sr[AHEAD], dr[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      sr[a] = s[a] < 0 ? 0 : ((size_t)row[s[a] / KRK_PAGE] * HKV + kh) * KRK_PAGE + s[a] % KRK_PAGE;
+      dr[a] = s[a] < 0 ? 0 : ((size_t)row[d[a] / KRK_PAGE] * HKV + kh) * KRK_PAGE + d[a] % KRK_PAGE;
+    }
+    for (int c = c0; c < both; c += lanes) {
+      const bool key = c < p.k_pieces;
+      Piece* pool = key ? kp : vp;
+      const int pieces = key ? p.k_pieces : p.v_pieces, at = key ? c : c - p.k_pieces;
+      Piece got[AHEAD];
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a)
+        if (s[a] >= 0) got[a] = pool[sr[a] * pieces + at];
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a)
+        if (s[a] >= 0) pool[dr[a] * pieces + at] = got[a];
+    }
+  }
+}
+
+__device__ __forceinline__ void move_rows(const Pools& p, const int* to, const int* from, int n, int run, int slot, int kh, int HKV, int worker, int workers) {
+  if (p.piece_bytes == 16) move_rows<uint4>(p, to, from, n, run, slot, kh, HKV, worker, workers);
+  else if (p.piece_bytes == 4) move_rows<unsigned>(p, to, from, n, run, slot, kh, HKV, worker, workers);
+  else move_rows<unsigned short>(p, to, from, n, run, slot, kh, HKV, worker, workers);
+}
+
+struct ChooseArgs {
+  const float* scores;
+  const int* positions;
+  float* scores_out;
+  int* positions_out;
+  size_t run_stride;
+  int HKV, capacity, n_seqs, keep, recent, max_moves;
+  int *moves, *n_moves;
+  int *seq_start, *row_pos, *seq_shift;
+  bool move_here;
+};
+
+// A block for a head: what stays, the moves, and, where there are heads enough to fill the device, the moving. STAGED: the rows' keys lie in
+// shared memory, each read once from the cache's tables; else every reading goes to memory again.
+template <int T, int BINS, bool STAGED>
+__global__ void __launch_bounds__(T)
+choose_rows_kernel(const ChooseArgs a, const Sequences seqs, const Pools pools, int staged_rows) {
+  __shared__ Scratch<T, BINS> sc;
+  extern __shared__ __align__(16) unsigned dynamic_s[];
+  unsigned *pos_s = dynamic_s, *sum_s = dynamic_s + staged_rows;  // order_of each; a sum that does not stand for election becomes 0, which no number has
+  unsigned* kept_s = dynamic_s + 2 * staged_rows;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int kh = blockIdx.x % a.HKV, seq = blockIdx.x / a.HKV % a.n_seqs, run = blockIdx.x / a.HKV / a.n_seqs;
+  const int L = seqs.length[seq], keep = a.keep;
+  const size_t base = run * a.run_stride + ((size_t)seqs.slot[seq] * a.HKV + kh) * a.capacity;
+  const float* sum = a.scores + base;
+  const int* pos = a.positions + base;
+  float* sum_out = a.scores_out + base;
+  int* pos_out = a.positions_out + base;
+  const bool apart = sum != sum_out, pos_apart = pos != pos_out;
+  if (L <= keep) {
+    for (int r = threadIdx.x; r < L; r += T) {
+      if (apart) sum_out[r] = sum[r];
+      if (pos_apart) pos_out[r] = pos[r];
+    }
+    if (threadIdx.x == 0) a.n_moves[blockIdx.x] = 0;
+    return;
+  }
+  if (a.seq_start && kh == 0 && run == 0 && threadIdx.x == 0) {  // the step's description follows
+    a.seq_start[seq] -= L - keep;
+    a.row_pos[seq] -= L - keep;
+    a.seq_shift[seq] += L - keep;
+  }
+  unsigned lo = 0xffffffffu, hi = 0;
+  constexpr int READS = 8;  // rows of a thread that are on their way together
+  for (int r0 = threadIdx.x; r0 < L; r0 += T * READS) {
+    int p[READS];
+    float x[READS];
+#pragma unroll
+    for (int e = 0; e < READS; ++e) {
+      const int r = min(r0 + e * T, L - 1);
+      p[e] = pos[r];
+      x[e] = STAGED ? sum[r] : 0.f;
     }
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a)
-      if (dst[a]) *dst[a] = got[a];
+    for (int e = 0; e < READS; ++e) {
+      const int r = min(r0 + e * T, L - 1);  // (the last row more than once)
+      const unsigned v = order_of(p[e]);
+      if (STAGED) {
+        pos_s[r] = v;
+        sum_s[r] = order_of(x[e]);
+      }
+      lo = min(lo, v);
+      hi = max(hi, v);
+    }
   }
+  block_range(lo, hi, sc);
+  const Line newest = line_of<true>(a.recent, L, lo, hi, sc, [&](int r, unsigned& v) { v = STAGED ? pos_s[r] : order_of(pos[r]); return true; });
+  auto key = [&](int r, unsigned& v) {
+    if (STAGED) {
+      v = sum_s[r];
+      return v != 0;
+    }
+    v = order_of(sum[r]);
+    return !newest.above(order_of(pos[r]), r);
+  };
+  lo = 0xffffffffu;
+  hi = 0;
+#pragma unroll 4
+  for (int r = threadIdx.x; r < L; r += T) {
+    unsigned v;
+    if (STAGED && newest.above(pos_s[r], r)) sum_s[r] = 0;
+    if (key(r, v)) { lo = min(lo, v); hi = max(hi, v); }
+  }
+  __syncthreads();
+  block_range(lo, hi, sc);
+  const Line heavy = line_of<false>(keep - a.recent, L, lo, hi, sc, key);
+  // the rows' bits; how many are free below `keep`, and kept from there on, in each warp's share of the words
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int WARPS = T / 32;
+  const int words = (L + 31) / 32, per = (words + WARPS - 1) / WARPS, w_lo = warp * per, w_hi = min(words, w_lo + per);
+  int n_free = 0, n_down = 0;
+  for (int w = w_lo; w < w_hi; ++w) {
+    const int r = 32 * w + lane;
+    unsigned v;
+    const bool stays = r < L && (!key(r, v) || heavy.above(v, r));
+    const unsigned bits = __ballot_sync(0xffffffffu, stays), below = __ballot_sync(0xffffffffu, r < keep);
+    if (lane == 0) kept_s[w] = bits;
+    n_free += __popc(~bits & below);
+    n_down += __popc(bits & ~below);
+  }
+  __syncthreads();
+  if (lane == 0) { sc.part[0][warp] = n_free; sc.part[1][warp] = n_down; }
+  __syncthreads();
+  int at_free = __reduce_add_sync(0xffffffffu, lane < warp ? sc.part[0][lane] : 0);
+  int at_down = __reduce_add_sync(0xffffffffu, lane < warp ? sc.part[1][lane] : 0);
+  const int n_moves = __reduce_add_sync(0xffffffffu, lane < WARPS ? sc.part[1][lane] : 0);
+  int* to = a.moves + (size_t)blockIdx.x * 2 * a.max_moves;
+  int* from = to + a.max_moves;
+  for (int w = w_lo; w < w_hi; ++w) {
+    const int r = 32 * w + lane;
+    const unsigned bits = kept_s[w], below = __ballot_sync(0xffffffffu, r < keep), before = (1u << lane) - 1;
+    if ((~bits & below) >> lane & 1) to[at_free + __popc(~bits & below & before)] = r;
+    if ((bits & ~below) >> lane & 1) from[at_down + __popc(bits & ~below & before)] = r;
+    at_free += __popc(~bits & below);
+    at_down += __popc(bits & ~below);
+  }
+  __syncthreads();
+  constexpr int AHEAD = 4;  // rows of a thread that are on their way together
+  if (apart || pos_apart)
+    for (int r0 = threadIdx.x; r0 < keep; r0 += T * AHEAD) {
+      float x[AHEAD];
+      int p[AHEAD];
+      bool stays[AHEAD];
+#pragma unroll
+      for (int e = 0; e < AHEAD; ++e) {
+        const int r = r0 + e * T;
+        stays[e] = r < keep && (kept_s[r / 32] >> (r % 32) & 1);
+        if (stays[e]) { x[e] = sum[r]; p[e] = pos[r]; }
+      }
+#pragma unroll
+      for (int e = 0; e < AHEAD; ++e)
+        if (stays[e]) {
+          if (apart) sum_out[r0 + e * T] = x[e];
+          if (pos_apart) pos_out[r0 + e * T] = p[e];
+        }
+    }
+  for (int i0 = threadIdx.x; i0 < n_moves; i0 += T * AHEAD) {
+    int s[AHEAD], d[AHEAD], p[AHEAD];
+    float x[AHEAD];
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e) {
+      const int i = i0 + e * T;
+      s[e] = i < n_moves ? from[i] : -1;
+      d[e] = i < n_moves ? to[i] : 0;
+    }
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e)
+      if (s[e] >= 0) { x[e] = sum[s[e]]; p[e] = pos[s[e]]; }
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e)
+      if (s[e] >= 0) { sum_out[d[e]] = x[e]; pos_out[d[e]] = p[e]; }
+  }
+  if (a.move_here) move_rows(pools, to, from, n_moves, run, seqs.slot[seq], kh, a.HKV, threadIdx.x, T);
+  else if (threadIdx.x == 0) a.n_moves[blockIdx.x] = n_moves;
+}
+
+constexpr int MOVE_THREADS = 256;
+__global__ void __launch_bounds__(MOVE_THREADS)
+move_rows_kernel(const Pools pools, int HKV, const Sequences seqs, int n_seqs, const int* __restrict__ moves, const int* __restrict__ n_moves, int max_moves,
+                 int blocks_per_head) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int head = blockIdx.x / blocks_per_head, part = blockIdx.x % blocks_per_head;
+  const int kh = head % HKV, seq = head / HKV % n_seqs, run = head / HKV / n_seqs;
+  const int* to = moves + (size_t)head * 2 * max_moves;
+  move_rows(pools, to, to + max_moves, n_moves[head], run, seqs.slot[seq], kh, HKV, part * MOVE_THREADS + threadIdx.x, blocks_per_head * MOVE_THREADS);
 }
 
 }  // namespace
@@ -242,24 +414,29 @@ KRK_API int krk_evict_keys(void* k, void* v, long long k_run_bytes, long long v_
   if (heads > 0x7fffffffLL) return -3;
   Sequences seqs = {};
   for (int i = 0; i < n_seqs; ++i) { seqs.slot[i] = slots[i]; seqs.length[i] = lengths[i]; }
-  cudaError_t e = launch_pdl(choose_rows_kernel, dim3((unsigned)heads), dim3(THREADS), 0, stream, scores, positions, scores_out, positions_out,
-                             (size_t)run_stride, HKV, capacity, seqs, n_seqs, keep, recent, moves, n_moves, max_moves, seq_start, row_pos, seq_shift);
-  if (e != cudaSuccess) return (int)e;
-  if (max_moves == 0) return 0;
   const long long align = k_row_bytes | (v ? v_row_bytes : 0) | k_run_bytes | (v ? v_run_bytes : 0) | (long long)(uintptr_t)k | (long long)(uintptr_t)v;
-  auto go = [&](auto piece) {
-    typedef decltype(piece) Piece;
-    const int size = (int)sizeof(Piece), kp = k_row_bytes / size, vp = v ? v_row_bytes / size : 0;
-    // enough blocks that a thread has one batch of pieces in flight, no more than fill the device a few times over
-    const long long wanted = ((long long)max_moves * (kp + vp) + 4 * MOVE_THREADS - 1) / (4 * MOVE_THREADS);
-    const long long room = (148 * 16 + heads - 1) / heads;
-    const int per_head = (int)(wanted < room ? wanted : room);
-    if (heads * per_head > 0x7fffffffLL) return -3;
-    return (int)launch_pdl(move_rows_kernel<Piece>, dim3((unsigned)(heads * per_head)), dim3(MOVE_THREADS), 0, stream, (Piece*)k, (Piece*)v,
-                           (size_t)(k_run_bytes / size), (size_t)(v_run_bytes / size), kp, vp, HKV, seqs, n_seqs, table, width, (const int*)moves,
-                           (const int*)n_moves, max_moves, per_head);
+  const int piece = align % 16 == 0 ? 16 : align % 4 == 0 ? 4 : 2;
+  const Pools pools = {k, v, (size_t)(k_run_bytes / piece), (size_t)(v_run_bytes / piece), k_row_bytes / piece, v ? v_row_bytes / piece : 0, table, width, piece};
+  // A head's block moves its rows itself where there are two heads an SM or more, or little to move.
+  const bool move_here = heads >= 296 || (long long)max_moves * (k_row_bytes + v_row_bytes) <= 32768;
+  const ChooseArgs args = {scores, positions, scores_out, positions_out, (size_t)run_stride, HKV, capacity, n_seqs, keep, recent, max_moves,
+                           moves, n_moves, seq_start, row_pos, seq_shift, move_here};
+  int longest = 0;
+  for (int i = 0; i < n_seqs; ++i) longest = lengths[i] > longest ? lengths[i] : longest;
+  // Few rows: few threads, whose sums and barriers cost more than the rows do. Rows whose keys do not fit shared memory are read again.
+  auto choose = [&](auto* kern, int threads, int staged) {
+    const size_t smem = (size_t)staged * 8 + ((size_t)longest + 31) / 32 * 4;
+    cudaError_t e = smem > 200 * 1024 ? cudaErrorInvalidValue : smem > 32 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
+    return e != cudaSuccess ? e : launch_pdl(kern, dim3((unsigned)heads), dim3(threads), smem, stream, args, seqs, pools, staged);
   };
-  if (align % 16 == 0) return go(uint4());
-  if (align % 4 == 0) return go(0u);
-  return go((unsigned short)0);
+  cudaError_t e = longest <= 2048    ? choose(choose_rows_kernel<128, 512, true>, 128, longest)
+                  : longest <= 24000 ? choose(choose_rows_kernel<512, 2048, true>, 512, longest)
+                                     : choose(choose_rows_kernel<1024, 2048, false>, 1024, 0);
+  if (e != cudaSuccess || max_moves == 0 || move_here) return (int)e;
+  // four moves in flight a warp's share, and no more blocks than fill the device a few times over
+  const long long wanted = ((long long)max_moves * 32 + 4 * MOVE_THREADS - 1) / (4 * MOVE_THREADS), room = (148 * 8 + heads - 1) / heads;
+  const int per_head = (int)(wanted < room ? wanted : room);
+  if (heads * per_head > 0x7fffffffLL) return -3;
+  return (int)launch_pdl(move_rows_kernel, dim3((unsigned)(heads * per_head)), dim3(MOVE_THREADS), 0, stream, pools, HKV, seqs, n_seqs, (const int*)moves,
+                         (const int*)n_moves, max_moves, per_head);
 }

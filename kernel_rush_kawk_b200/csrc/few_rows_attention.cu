@@ -8,6 +8,10 @@
 // (a fifth warp asks for them, one unit a page of keys or of values, into a ring as deep as the shared memory that
 // the blocks of an SM have between them), or by cp.async where the head size is no multiple of 64.
 //
+// Where a unit has at most eight rows (NARROW: the heads of a kv head mostly are), the products are taken the other way round: the page's
+// keys are the sixteen rows of an instruction and the queries its eight columns, S^T = K Q^T and O^T = V^T P^T, with P^T turned in
+// registers (movmatrix). Sixteen rows of which four are queries cost twice the instructions and registers: @@NARROW@@
+//
 // The splits of a sequence's keys form a cluster: their parts meet in the first block's shared memory, which also reads the prefix
 // parts of its rows and writes the output. That is the only place that waits for the kernel before, so a sequence's own
 // keys are read while the prefix kernel still runs.
@@ -46,6 +50,141 @@ constexpr int CP_STAGES = 2;  // page pairs, where pages come by cp.async
 
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 2, 128;" ::: "memory"); }
 
+// The 8 x 8 matrix of bfloat16 pairs that a warp holds, turned.
+__device__ __forceinline__ uint32_t turned(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// A warp's running softmax over 16 keys of each page, for 16 rows of queries: S in rows, as in the other kernels of this library.
+struct Wide {
+  static constexpr int TILE = 16;
+  uint32_t qf[KSTEPS][4];
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float o[DTILES][4], s[2][4];
+  __device__ __forceinline__ void begin(const bf16* const (&qp)[2], int lane) {
+    load_q(qf, qp[0], qp[1], lane);
+#pragma unroll
+    for (int n = 0; n < DTILES; ++n)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[n][c] = 0.f;
+  }
+  template <bool TMA> __device__ __forceinline__ void scores(const bf16* ks, int key0, int count, float scale_log2, int lane) {
+    qk_tile<2, TMA>(s, qf, ks, key0, lane);
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[n][c] = key0 + n * 8 + 2 * (lane & 3) + (c & 1) < count ? s[n][c] * scale_log2 : -INFINITY;
+  }
+  __device__ __forceinline__ void keep_scores(float* raw, size_t capacity, int q_rows, int lane) const {  // raw: of row 0, the warp's first key
+    const int g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (g + 8 * h < q_rows)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) *reinterpret_cast<float2*>(raw + (g + 8 * h) * capacity + n * 8 + 2 * t4) = make_float2(s[n][2 * h], s[n][2 * h + 1]);
+  }
+  __device__ __forceinline__ void update(int) { softmax_update<2>(s, m, l, o); }
+  template <bool TMA> __device__ __forceinline__ void values(const bf16* vs, int key0, int lane) { pv_tile<2, TMA>(o, s, vs, key0, lane); }
+  __device__ __forceinline__ void leave(float* red, int lane) {  // [16 rows][RP]
+    const int g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float* dst = red + (g + 8 * h) * RP;
+      if (t4 == 0) { dst[D] = m[h]; dst[D + 1] = l[h]; }
+#pragma unroll
+      for (int n = 0; n < DTILES; ++n) *reinterpret_cast<float2*>(dst + n * 8 + 2 * t4) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+    }
+  }
+};
+
+// The same for eight rows of queries, as the columns: a thread has keys g and g + 8 with rows 2 t4 and 2 t4 + 1. The reference maximum of
+// a row moves only when it has been outgrown by 2^8 (l and o are float32, P's bfloat16 is relative): then p <= 2^8, and most pages need
+// one vote of the warp instead of a maximum over its lanes.
+struct Narrow {
+  static constexpr int TILE = 8;
+  uint32_t qb[KSTEPS][2];
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // l: this thread's keys alone, until the end
+  float o[KSTEPS][4], s[4];
+  __device__ __forceinline__ void begin(const bf16* const (&qp)[2], int lane) {
+    const int t4 = lane & 3;
+#pragma unroll
+    for (int kk = 0; kk < KSTEPS; ++kk) {
+      qb[kk][0] = qp[0] ? *reinterpret_cast<const uint32_t*>(qp[0] + kk * 16 + 2 * t4) : 0u;
+      qb[kk][1] = qp[0] ? *reinterpret_cast<const uint32_t*>(qp[0] + kk * 16 + 2 * t4 + 8) : 0u;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[kk][c] = 0.f;
+    }
+  }
+  template <bool TMA> __device__ __forceinline__ void scores(const bf16* ks, int key0, int count, float scale_log2, int lane) {
+    float odd[4] = {0.f, 0.f, 0.f, 0.f};  // even and odd steps apart: two chains of dependent products
+#pragma unroll
+    for (int c = 0; c < 4; ++c) s[c] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < KSTEPS; ++kk) {
+      uint32_t a0, a1, a2, a3;
+      ldmatrix_x4(a0, a1, a2, a3, ks + page_off<TMA>(key0 + (lane & 15), kk * 2 + (lane >> 4)));
+      mma_bf16_16816(kk & 1 ? odd : s, a0, a1, a2, a3, qb[kk][0], qb[kk][1]);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) s[c] = key0 + (lane >> 2) + 8 * (c >> 1) < count ? (s[c] + odd[c]) * scale_log2 : -INFINITY;
+  }
+  __device__ __forceinline__ void keep_scores(float* raw, size_t capacity, int q_rows, int lane) const {
+    const int g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (2 * t4 + (c & 1) < q_rows) raw[(2 * t4 + (c & 1)) * capacity + g + 8 * (c >> 1)] = s[c];
+  }
+  __device__ __forceinline__ void update(int) {
+    // (a NaN outgrows nothing and goes through the sums; rows of infinities come out as they do with a running maximum)
+    const bool outgrown = s[0] > m[0] + 8.f || s[2] > m[0] + 8.f || s[1] > m[1] + 8.f || s[3] > m[1] + 8.f;
+    if (__any_sync(0xffffffffu, outgrown)) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float mx = fmaxf(s[j], s[2 + j]);
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+        const float m_new = fmaxf(m[j], mx), alpha = m[j] == m_new ? 1.f : fast_exp2(m[j] - m_new);
+        m[j] = m_new;
+        l[j] *= alpha;
+#pragma unroll
+        for (int kk = 0; kk < KSTEPS; ++kk) { o[kk][j] *= alpha; o[kk][2 + j] *= alpha; }
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float ref = m[c & 1];
+      s[c] = fast_exp2(s[c] - (ref == -INFINITY ? 0.f : ref));
+      l[c & 1] += s[c];
+    }
+  }
+  template <bool TMA> __device__ __forceinline__ void values(const bf16* vs, int key0, int lane) {
+    const uint32_t b0 = turned(pack_bf16x2(s[0], s[1])), b1 = turned(pack_bf16x2(s[2], s[3]));
+#pragma unroll
+    for (int kk = 0; kk < KSTEPS; ++kk) {
+      uint32_t a0, a1, a2, a3;
+      ldmatrix_x4_trans(a0, a1, a2, a3, vs + page_off<TMA>(key0 + (lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)));
+      mma_bf16_16816(o[kk], a0, a1, a2, a3, b0, b1);
+    }
+  }
+  __device__ __forceinline__ void leave(float* red, int lane) {
+    const int g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], x);
+      float* dst = red + (2 * t4 + j) * RP;
+      if (g == 0) { dst[D] = m[j]; dst[D + 1] = l[j]; }
+#pragma unroll
+      for (int kk = 0; kk < KSTEPS; ++kk) {
+        dst[kk * 16 + g] = o[kk][j];
+        dst[kk * 16 + g + 8] = o[kk][2 + j];
+      }
+    }
+  }
+};
+
 struct KeySums {  // weights per key; see krk_scored_single
   float* raw;     // [n_seqs][HQ][capacity]
   const float* sums;
@@ -69,7 +208,7 @@ struct Layout {  // of the dynamic shared memory, from a 1024-byte boundary on
 };
 
 // PREFIX: unit = group, parts go to `parts` from part0 on. Otherwise: unit = sequence, one token; the parts 0 .. n_join - 1 of its row join.
-template <bool TMA, bool PREFIX, bool SUMS>
+template <bool TMA, bool PREFIX, bool SUMS, typename Rows>
 __global__ void __launch_bounds__(TMA ? 160 : 128)
 few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, bf16* __restrict__ out, Parts parts, int part0,
                 int n_join, const bf16* __restrict__ q, int q_stride, int HQ, int HKV, Segments seg, const bf16* __restrict__ k_cache,
@@ -79,7 +218,8 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   cg::cluster_group cluster = cg::this_cluster();
   const int n_splits = gridDim.x, split = blockIdx.x;
   const bool clustered = !PREFIX && n_splits > 1;
-  const int G = HQ / HKV, inbox_rows = min(16, G);
+  constexpr int TILE = Rows::TILE;
+  const int G = HQ / HKV, inbox_rows = min(TILE, G);
   const Layout at(units_in_ring, clustered ? n_splits : 1, inbox_rows);
   bf16* ring_s = reinterpret_cast<bf16*>(base);
   float* red = reinterpret_cast<float*>(base);            // [4 warps][16 rows][RP], when the ring is done with
@@ -93,10 +233,10 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   grid_launch_dependents();
   const int kh = blockIdx.y / row_tiles, rt = blockIdx.y % row_tiles;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, t4 = lane & 3;
+  const int g = lane >> 2;
   const Unit u = PREFIX ? prefix_unit(seg, blockIdx.z) : own_unit(seg, blockIdx.z);
   const int n_rows = u.n_tok * G;
-  const int q_rows = min(16, n_rows - rt * 16);
+  const int q_rows = min(TILE, n_rows - rt * TILE);
   if (PREFIX && q_rows <= 0) return;  // a whole block, which has asked for nothing
   int j_lo, j_hi;
   split_pages(u.key_lo, u.key_hi, split, n_splits, j_lo, j_hi);
@@ -153,17 +293,11 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   const bf16* qp[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int R = rt * 16 + g + 8 * h;
-    qp[h] = R < n_rows ? q + (size_t)(u.row0 + R / G) * q_stride + (size_t)(kh * G + R % G) * D : nullptr;
+    const int R = rt * TILE + g + 8 * h;
+    qp[h] = g + 8 * h < TILE && R < n_rows ? q + (size_t)(u.row0 + R / G) * q_stride + (size_t)(kh * G + R % G) * D : nullptr;
   }
-  uint32_t qf[KSTEPS][4];
-  load_q(qf, qp[0], qp[1], lane);
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  float o[DTILES][4];
-#pragma unroll
-  for (int n = 0; n < DTILES; ++n)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) o[n][c] = 0.f;
+  Rows walk;
+  walk.begin(qp, lane);
 
   const size_t page_stride = (size_t)HKV * KRK_PAGE * D, head_off = (size_t)kh * KRK_PAGE * D;
   auto issue = [&](int i) {  // cp.async: page i of this block's share into its stage; one group per call
@@ -202,30 +336,17 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       __syncthreads();
     }
     const int key0 = warp * 16, count = u.key_hi - j * KRK_PAGE;  // keys of the page that count
-    float s[2][4];
-    qk_tile<2, TMA>(s, qf, ks_s, key0, lane);
+    walk.template scores<TMA>(ks_s, key0, count, scale_log2, lane);
     if (TMA) hand_back(nk);
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) s[n][c] = key0 + n * 8 + 2 * t4 + (c & 1) < count ? s[n][c] * scale_log2 : -INFINITY;
-    if (SUMS) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (g + 8 * h < q_rows) {
-          float* dst = ks.raw + ((size_t)blockIdx.z * HQ + kh * G + g + 8 * h) * ks.capacity + j * KRK_PAGE + key0 + 2 * t4;
-#pragma unroll
-          for (int n = 0; n < 2; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(s[n][2 * h], s[n][2 * h + 1]);
-        }
-    }
-    softmax_update<2>(s, m, l, o);
+    if (SUMS) walk.keep_scores(ks.raw + ((size_t)blockIdx.z * HQ + kh * G) * ks.capacity + j * KRK_PAGE + key0, ks.capacity, q_rows, lane);
+    walk.update(lane);
     if (TMA) arrived(nv);
     if (count < KRK_PAGE) {  // values behind the sequence's last may be anything, and zero times infinity is not zero
       for (int e = threadIdx.x; e < (KRK_PAGE - count) * (D / 8); e += 128)
         *reinterpret_cast<uint4*>(vs_s + page_off<TMA>(count + e / (D / 8), e % (D / 8))) = make_uint4(0, 0, 0, 0);
       consumer_sync();
     }
-    pv_tile<2, TMA>(o, s, vs_s, key0, lane);
+    walk.template values<TMA>(vs_s, key0, lane);
     if (TMA) hand_back(nv);
     else __syncthreads();
   }
@@ -233,13 +354,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   else if (!alive) tc::wait_for_copies(full_bar, units_in_ring, 2 * n_pages);  // the ring's place is used again
   consumer_sync();  // every warp is done with the ring: it now holds the warps' parts
 
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float* dst = red + ((size_t)warp * 16 + g + 8 * h) * RP;
-    if (t4 == 0) { dst[D] = m[h]; dst[D + 1] = l[h]; }
-#pragma unroll
-    for (int n = 0; n < DTILES; ++n) *reinterpret_cast<float2*>(dst + n * 8 + 2 * t4) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
-  }
+  walk.leave(red + (size_t)warp * 16 * RP, lane);
   consumer_sync();
   if (clustered) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every block of the cluster has started
   if (!PREFIX && !clustered && !wait_first) grid_dependency_wait();                    // the prefix parts are there
@@ -248,7 +363,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 
   // the prefix parts of a row join what the row has from its own keys, and the row is written; a warp's lanes hold its columns
   auto finish = [&](int r, float big, float total, float (&acc)[(D + 31) / 32]) {
-    const int R = rt * 16 + r, head = kh * G + R % G;
+    const int R = rt * TILE + r, head = kh * G + R % G;
     const size_t item = (size_t)(u.row0 + R / G) * HQ + head;
     if (n_join > 0) {
       float mine = big;
@@ -258,17 +373,24 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       total *= w;
 #pragma unroll
       for (int i = 0; i < (D + 31) / 32; ++i) acc[i] *= w;
-#pragma unroll 4
-      for (int p = 0; p < n_join; ++p) {
-        const float2 ml = parts.ml[p * part_step + item];
-        if (ml.y == 0.f) continue;
-        const float wp = exp2f(ml.x - safe);
-        total += wp * ml.y;
+      // eight parts at once: their loads are on their way together, and a part without a key has no weight and is not read
+      for (int p0 = 0; p0 < n_join; p0 += 8) {
+        float wp[8], v[8][(D + 31) / 32];
 #pragma unroll
-        for (int i = 0; i < (D + 31) / 32; ++i) {
-          const int d = lane + 32 * i;
-          if (d < D) acc[i] += wp * parts.o[(p * part_step + item) * D + d];
+        for (int e = 0; e < 8; ++e) {
+          const float2 ml = p0 + e < n_join ? parts.ml[(p0 + e) * part_step + item] : make_float2(0.f, 0.f);
+          wp[e] = ml.y == 0.f ? 0.f : exp2f(ml.x - safe);
+          total += ml.y == 0.f ? 0.f : wp[e] * ml.y;
+#pragma unroll
+          for (int i = 0; i < (D + 31) / 32; ++i) {
+            const int d = lane + 32 * i;
+            v[e][i] = ml.y != 0.f && d < D ? parts.o[((p0 + e) * part_step + item) * D + d] : 0.f;
+          }
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int i = 0; i < (D + 31) / 32; ++i) acc[i] += wp[e] * v[e][i];
       }
     }
     const float inv = 1.f / total;
@@ -296,7 +418,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       for (int w = 0; w < 4; ++w) acc[i] += d < D ? wgt[w] * red[((size_t)w * 16 + r) * RP + d] : 0.f;
     }
     if (PREFIX) {
-      const int R = rt * 16 + r;
+      const int R = rt * TILE + r;
       const size_t to = parts.at(part0 + split, u.row0 + R / G, kh * G + R % G);
       if (total != 0.f)
 #pragma unroll
@@ -349,25 +471,44 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   if (SUMS) {
     const int end = min(j_hi * KRK_PAGE, u.key_hi);
     const float* raw = ks.raw + ((size_t)blockIdx.z * HQ + kh * G) * ks.capacity;
-    for (int key = j_lo * KRK_PAGE + threadIdx.x; key < end; key += 128) {
-      float w = 0.f;
-      for (int r = 0; r < q_rows; ++r) w += exp2f(raw[(size_t)r * ks.capacity + key] - lse_s[r]);
-      const size_t place = ((size_t)u.slot * HKV + kh) * ks.capacity + key;
-      ks.sums_out[place] = key < u.start ? ks.sums[place] + w : w;
-      if (ks.positions && key >= u.start) ks.positions[place] = key + (ks.seq_shift ? ks.seq_shift[blockIdx.z] : 0);
+    const size_t place = ((size_t)u.slot * HKV + kh) * ks.capacity;
+    constexpr int AHEAD = 8;  // keys of a thread whose loads are on their way together
+    for (int key0 = j_lo * KRK_PAGE + threadIdx.x; key0 < end; key0 += 128 * AHEAD) {
+      float w[AHEAD], old[AHEAD];
+#pragma unroll
+      for (int e = 0; e < AHEAD; ++e) {
+        const int key = key0 + 128 * e;
+        w[e] = 0.f;
+        old[e] = key < min(end, u.start) ? ks.sums[place + key] : 0.f;
+      }
+      for (int r = 0; r < q_rows; ++r) {
+        const float* row = raw + (size_t)r * ks.capacity;
+        float s[AHEAD];
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) s[e] = key0 + 128 * e < end ? row[key0 + 128 * e] : -INFINITY;
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) w[e] += exp2f(s[e] - lse_s[r]);
+      }
+#pragma unroll
+      for (int e = 0; e < AHEAD; ++e) {
+        const int key = key0 + 128 * e;
+        if (key >= end) break;
+        ks.sums_out[place + key] = old[e] + w[e];
+        if (ks.positions && key >= u.start) ks.positions[place + key] = key + (ks.seq_shift ? ks.seq_shift[blockIdx.z] : 0);
+      }
     }
   }
 }
 
-template <bool PREFIX, bool SUMS>
+template <bool PREFIX, bool SUMS, typename Rows>
 int launch_few_rows(bf16* out, const Parts& parts, int part0, int n_join, const void* q, int q_stride, int HQ, int HKV, const Segments& seg,
                     const void* k, const void* v, int n_pages, int max_rows, int n_splits, float scale, bool wait_first, const KeySums& ks, int* error,
                     cudaStream_t stream) {
   const int G = HQ / HKV;
-  const long long row_tiles = ((long long)max_rows * G + 15) / 16;
+  const long long row_tiles = ((long long)max_rows * G + Rows::TILE - 1) / Rows::TILE;
   const int units = PREFIX ? seg.n_groups : seg.n_seqs;
   if (row_tiles * HKV > 65535 || units > 65535) return -3;
-  const int splits_in_cluster = PREFIX ? 1 : n_splits, inbox_rows = G < 16 ? G : 16;
+  const int splits_in_cluster = PREFIX ? 1 : n_splits, inbox_rows = G < Rows::TILE ? G : Rows::TILE;
   const long long blocks = row_tiles * HKV * units * n_splits;
   CUtensorMap map_k = {}, map_v = {};
   int in_ring;
@@ -377,7 +518,7 @@ int launch_few_rows(bf16* out, const Parts& parts, int part0, int n_join, const 
     if (rc == 0) rc = tc::make_map_bf16(&map_v, v, rows, D, D, KRK_PAGE);
     if (rc) return rc;
     // as many units as the shared memory of an SM holds for the blocks that it gets
-    const int per_sm = blocks <= 148 ? 1 : blocks <= 296 ? 2 : 3;
+    const int per_sm = blocks <= 148 ? 1 : blocks <= 296 ? 2 : blocks <= 444 || Rows::TILE == 16 ? 3 : 4;
     const size_t room = 216 * 1024 / per_sm, fixed = Layout(0, splits_in_cluster, inbox_rows).total - Layout(0, 1, 0).total + 2048;
     in_ring = (int)((room > fixed ? room - fixed : 0) / UNIT_BYTES);
     in_ring = in_ring < 2 ? 2 : in_ring > 12 ? 12 : in_ring;
@@ -386,7 +527,7 @@ int launch_few_rows(bf16* out, const Parts& parts, int part0, int n_join, const 
   }
   const size_t smem = Layout(in_ring, splits_in_cluster, inbox_rows).total + 1024;
   if (smem > 227 * 1024) return -2;
-  auto kern = few_rows_kernel<TMA_PAGES, PREFIX, SUMS>;
+  auto kern = few_rows_kernel<TMA_PAGES, PREFIX, SUMS, Rows>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg = {};
@@ -420,8 +561,9 @@ KRK_API int krk_prefix_few_rows(float* o, float* ml, int rows, int part0, int n_
                                 const void* k_cache, const void* v_cache, int n_pages, int max_rows, float scale, int* error, cudaStream_t stream) {
   if (rows == 0 || n_groups == 0) return 0;
   const Parts parts = {o, (float2*)ml, rows, HQ};
-  return launch_few_rows<true, false>(nullptr, parts, part0, 0, q, q_stride, HQ, HKV, KRK_MAKE_SEGMENTS, k_cache, v_cache, n_pages, max_rows, n_splits,
-                                      scale, true, KeySums{}, error, stream);
+  auto go = (long long)max_rows * (HQ / HKV) <= 8 ? launch_few_rows<true, false, Narrow> : launch_few_rows<true, false, Wide>;
+  return go(nullptr, parts, part0, 0, q, q_stride, HQ, HKV, KRK_MAKE_SEGMENTS, k_cache, v_cache, n_pages, max_rows, n_splits, scale, true, KeySums{}, error,
+            stream);
 }
 
 // One token a sequence: its own keys (all, without groups), joined with the prefix parts 0 .. n_join - 1, which the launch before this one
@@ -430,8 +572,9 @@ KRK_API int krk_own_single(void* out, const float* o, const float* ml, int n_joi
                            KRK_SEGMENTS, const void* k_cache, const void* v_cache, int n_pages, float scale, int* error, cudaStream_t stream) {
   if (n_seqs == 0) return 0;
   const Parts parts = {const_cast<float*>(o), (float2*)const_cast<float*>(ml), n_seqs, HQ};
-  return launch_few_rows<false, false>((bf16*)out, parts, 0, n_join, q, q_stride, HQ, HKV, KRK_MAKE_SEGMENTS, k_cache, v_cache, n_pages, 1, n_splits,
-                                       scale, n_join == 0, KeySums{}, error, stream);
+  auto go = HQ / HKV <= 8 ? launch_few_rows<false, false, Narrow> : launch_few_rows<false, false, Wide>;
+  return go((bf16*)out, parts, 0, n_join, q, q_stride, HQ, HKV, KRK_MAKE_SEGMENTS, k_cache, v_cache, n_pages, 1, n_splits, scale, n_join == 0, KeySums{},
+            error, stream);
 }
 
 // One token a sequence over all of its keys, with the weight that each key receives added to its sum (see krk_key_weights). raw: scratch,
@@ -441,8 +584,9 @@ KRK_API int krk_scored_single(void* out, float* raw, const float* sums, float* s
                               int n_pages, float scale, int* error, cudaStream_t stream) {
   if (n_seqs == 0) return 0;
   if (HQ / HKV > 16) return -2;
-  return launch_few_rows<false, true>((bf16*)out, Parts{nullptr, nullptr, n_seqs, HQ}, 0, 0, q, q_stride, HQ, HKV, KRK_MAKE_SEGMENTS, k_cache, v_cache,
-                                      n_pages, 1, n_splits, scale, true, KeySums{raw, sums, sums_out, positions, seq_shift, capacity}, error, stream);
+  auto go = HQ / HKV <= 8 ? launch_few_rows<false, true, Narrow> : launch_few_rows<false, true, Wide>;
+  return go((bf16*)out, Parts{nullptr, nullptr, n_seqs, HQ}, 0, 0, q, q_stride, HQ, HKV, KRK_MAKE_SEGMENTS, k_cache, v_cache, n_pages, 1, n_splits, scale, true,
+            KeySums{raw, sums, sums_out, positions, seq_shift, capacity}, error, stream);
 }
 
 #endif  // head sizes served by these kernels

@@ -6,7 +6,8 @@
 //
 // The rows that see the keys come by TMA in tiles of whole tokens, two in shared memory; S has two places in tensor memory (256 columns).
 // Warps 0..3 take the even tiles and warps 4..7 the odd ones; lane 0 of warp 8 issues the MMAs, lane 0 of warp 9 the loads. What bounds it
-// is the exponentials, one for every (query head, key): 16 a clock and SM.
+// is the exponentials, one for every (query head, key): 16 a clock and SM. Where the blocks are few for the device, and unequal (the first
+// keys are seen by every row), the tiles of a block's rows are dealt out to a cluster, whose sums meet in the first block, in order.
 //
 // Compiled once per head size, for head sizes 64 and 128: -DKRK_HEAD_DIM=<D>.
 #include "partial_attention.cuh"
@@ -30,6 +31,7 @@ constexpr int THREADS = 320;           // 8 warps that add up, the one that issu
 constexpr uint32_t SUB = 128 * 128;    // bytes of a [128 rows x 64 bf16] swizzled sub-tile
 constexpr uint32_t TILE_BYTES = DB * SUB;
 constexpr uint32_t TMEM_COLS = 256;
+constexpr int MAX_SHARE = 8;           // blocks of a cluster
 constexpr float LOG2E = 1.4426950408889634f;
 
 enum Bar { K_FULL = 0, Q_FULL = 1, Q_FREE = 3, S_FULL = 5, S_FREE = 7, N_BARS = 9 };
@@ -43,7 +45,7 @@ __device__ __forceinline__ float fast_exp2(float x) {
 __global__ void __launch_bounds__(THREADS, 2)
 key_weights_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_q, int rows, const float* sums, float* sums_out,
                            int* __restrict__ positions, const int* __restrict__ seq_shift, int capacity, const float* __restrict__ lse, int observe, int HQ,
-                           int HKV, Segments seg, float scale_log2, int* __restrict__ error) {
+                           int HKV, Segments seg, float scale_log2, int share, int* __restrict__ error) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   unsigned char* k_s = base;
@@ -52,16 +54,22 @@ key_weights_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS + 1);
   float* minus_lse = reinterpret_cast<float*>(tmem_slot + 4);  // [2][ROWS]
   float* other = minus_lse + 2 * ROWS;                         // [KEYS] the odd tiles' sums
+  float* inbox = other + KEYS;                                 // [share][KEYS] in the cluster's first block
 
+  if (share > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // "I have started"
   grid_dependency_wait();
   grid_launch_dependents();
-  const int kh = blockIdx.x % HKV, key0 = blockIdx.x / HKV * KEYS, seq = blockIdx.y, G = HQ / HKV;
+  const int rank = blockIdx.x % share, block = blockIdx.x / share;
+  const int kh = block % HKV, key0 = block / HKV * KEYS, seq = blockIdx.y, G = HQ / HKV;
   const Unit u = own_unit(seg, seq);
-  if (key0 >= u.key_hi) return;
+  if (key0 >= u.key_hi) {  // a cluster as a whole
+    if (share > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    return;
+  }
   const int seen = observe > 0 ? min(observe, u.n_tok) : u.n_tok, tok0 = u.n_tok - seen;
   const int start = u.start + tok0, row0 = u.row0 + tok0, n_rows = seen * G;  // of the rows that count
-  const int first = max(0, (key0 - start) * G) / rows;                         // the first tile with a row that sees a key of the block
-  const int n = max(0, (n_rows + rows - 1) / rows - first);
+  const int first = max(0, (key0 - start) * G) / rows + rank;                  // of the tiles with a row that sees a key, this block's first
+  const int n = max(0, ((n_rows + rows - 1) / rows - first + share - 1) / share);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool half = key0 + KRK_PAGE >= u.key_hi;  // one page only
 
@@ -128,7 +136,7 @@ key_weights_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
         mbar_expect_tx(bars + Q_FULL + b, DB * rows * 128);
 #pragma unroll
         for (int h = 0; h < DB; ++h)
-          tma_load_3d(q_s + b * TILE_BYTES + h * SUB, &map_q, bars + Q_FULL + b, h * 64, kh * G, row0 + (first + i) * rows / G);
+          tma_load_3d(q_s + b * TILE_BYTES + h * SUB, &map_q, bars + Q_FULL + b, h * 64, kh * G, row0 + (first + i * share) * rows / G);
         asked = i + 1;
       }
       // what was asked for lands before the block ends, whoever gave up
@@ -143,7 +151,7 @@ key_weights_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     float* mine = minus_lse + t * ROWS;
     bool alive = true;  // false once a wait ran out: the four warps go on to their barriers, the results are void
     for (int i = t; i < n; i += 2) {
-      const int tile0 = (first + i) * rows;  // the tile's first row, of those that count
+      const int tile0 = (first + i * share) * rows;  // the tile's first row, of those that count
       {
         const int R = tile0 + r;
         mine[r] = r < rows && R < n_rows ? -lse[(size_t)(row0 + R / G) * HQ + kh * G + R % G] : -INFINITY;
@@ -200,30 +208,45 @@ key_weights_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
   }
   const int key = key0 + threadIdx.x;
+  if (!dead && threadIdx.x < KEYS) total += other[threadIdx.x];
+  if (share > 1) {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every block of the cluster has started
+    if (threadIdx.x < KEYS)
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_address(inbox + rank * KEYS + threadIdx.x, 0)), "f"(total) : "memory");
+    cluster_sync();
+    if (rank != 0) return;
+    if (threadIdx.x < KEYS) {
+      total = 0.f;
+      for (int c = 0; c < share; ++c) total += inbox[c * KEYS + threadIdx.x];
+    }
+  }
   if (threadIdx.x < KEYS && key < u.key_hi) {
-    if (!dead) total += other[threadIdx.x];
     const size_t place = ((size_t)u.slot * HKV + kh) * capacity + key;
     sums_out[place] = key < u.start ? sums[place] + total : total;
     if (positions && key >= u.start) positions[place] = key + (seq_shift ? seq_shift[seq] : 0);
   }
 }
 
-constexpr size_t SMEM_BYTES = 3 * TILE_BYTES + 1024 + (N_BARS + 1) * 8 + 16 + (2 * ROWS + KEYS) * sizeof(float);
+constexpr size_t SMEM_BYTES = 3 * TILE_BYTES + 1024 + (N_BARS + 1) * 8 + 16 + (2 * ROWS + (1 + MAX_SHARE) * KEYS) * sizeof(float);
 
 }  // namespace
 
-// krk_key_weights on the tensor cores. max_kv_len: the most rows that a sequence holds after the step. -2: rows off 16-byte boundaries, or heads of
+// krk_key_weights on the tensor cores. max_seen: the most queries of a sequence that count; max_kv_len: the most rows that one holds after the step. -2: rows off 16-byte boundaries, or heads of
 // which whole tokens do not fill half a tile.
 KRK_API int krk_key_weights_tcgen05(const float* sums, float* sums_out, int* positions, const int* seq_shift, int capacity, const float* lse, int observe,
                                     const void* q, int q_stride, int HQ, int HKV, const int* cu_q, const int* seq_slot, const int* seq_start,
                                     const int* seq_qlen, const int* group_cu, const int* group_len, const int* seq_group, int n_seqs, int n_groups,
-                                    const int* table, int width, const void* k_cache, int n_pages, int rows, int max_kv_len, float scale, int* error,
-                                    cudaStream_t stream) {
+                                    const int* table, int width, const void* k_cache, int n_pages, int rows, int max_seen, int max_kv_len, float scale,
+                                    int* error, cudaStream_t stream) {
   if (n_seqs == 0 || rows == 0) return 0;
   const int G = HQ / HKV, tile_rows = G <= ROWS ? ROWS / G * G : 0;
   if (q_stride % 8 || ((uintptr_t)q & 15) || tile_rows < ROWS / 2) return -2;
   const long long blocks = ((long long)max_kv_len + KEYS - 1) / KEYS * HKV;
-  if (blocks > 0x7fffffffLL || n_seqs > 65535) return -3;
+  if (blocks * MAX_SHARE > 0x7fffffffLL || n_seqs > 65535) return -3;
+  // shares of four tiles or more, until the device has four blocks an SM to choose from
+  const long long tiles = ((long long)max_seen * G + tile_rows - 1) / tile_rows;
+  int share = 1;
+  while (share < MAX_SHARE && blocks * n_seqs * share < 4 * 148 && tiles >= 8 * share) share *= 2;
   CUtensorMap map_k, map_q;
   int rc = make_map_bf16(&map_k, k_cache, (long long)n_pages * HKV * KRK_PAGE, D, D, KRK_PAGE);
   if (rc == 0) rc = make_map_bf16_3d(&map_q, q, D, HQ, rows, D, q_stride, G, tile_rows / G);
@@ -231,8 +254,22 @@ KRK_API int krk_key_weights_tcgen05(const float* sums, float* sums_out, int* pos
   cudaError_t e = cudaFuncSetAttribute(key_weights_tcgen05_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
   if (e != cudaSuccess) return (int)e;
   const Segments seg = {cu_q, seq_slot, seq_start, seq_qlen, group_cu, group_len, seq_group, n_seqs, n_groups, table, width};
-  return (int)launch_pdl(key_weights_tcgen05_kernel, dim3((unsigned)blocks, n_seqs), dim3(THREADS), SMEM_BYTES, stream, map_k, map_q, tile_rows, sums, sums_out,
-                         positions, seq_shift, capacity, lse, observe, HQ, HKV, seg, scale * LOG2E, error);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(blocks * share), n_seqs);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = share;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return (int)cudaLaunchKernelEx(&cfg, key_weights_tcgen05_kernel, map_k, map_q, tile_rows, sums, sums_out, positions, seq_shift, capacity, lse, observe, HQ,
+                                 HKV, seg, scale * LOG2E, share, error);
 }
 
 #endif  // head sizes served by this kernel

@@ -45,6 +45,34 @@ __device__ __forceinline__ void load_queries(Shared& sm, const T* __restrict__ q
 // Keys (and values) `count` from the page's first on; the places behind them become zero, so that what they hold counts nowhere.
 template <typename T>
 __device__ __forceinline__ void load_page(Shared& sm, const T* __restrict__ k, const T* __restrict__ v, int count, bool values) {
+  constexpr int V = 16 / sizeof(T);  // elements of a 16-byte piece
+  if (D % V == 0 && (((uintptr_t)k | (values ? (uintptr_t)v : 0)) & 15) == 0) {
+    // a thread's pieces four at a time, so that their loads are on their way together
+    constexpr int PIECES = KRK_PAGE * (D / V), AHEAD = 4;
+    auto put = [&](float* to, uint4 x) {
+      const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+      for (int c = 0; c < V; c += 4) *reinterpret_cast<float4*>(to + c) = make_float4(to_float<T>(e[c]), to_float<T>(e[c + 1]), to_float<T>(e[c + 2]), to_float<T>(e[c + 3]));
+    };
+    for (int i0 = threadIdx.x; i0 < PIECES; i0 += THREADS * AHEAD) {
+      uint4 kp[AHEAD], vp[AHEAD];
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        const int i = i0 + a * THREADS;
+        const bool in = i < PIECES && i / (D / V) < count;
+        kp[a] = in ? *reinterpret_cast<const uint4*>(k + (size_t)i * V) : make_uint4(0, 0, 0, 0);
+        vp[a] = in && values ? *reinterpret_cast<const uint4*>(v + (size_t)i * V) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) {
+        const int i = i0 + a * THREADS, key = i / (D / V), d = i % (D / V) * V;
+        if (i >= PIECES) break;
+        put(&sm.k[key][d], kp[a]);
+        if (values) put(&sm.v[key][d], vp[a]);
+      }
+    }
+    return;
+  }
   for (int i = threadIdx.x; i < KRK_PAGE * DPAD; i += THREADS) {
     const int key = i / DPAD, d = i % DPAD;
     const bool in = key < count && d < D;
@@ -201,18 +229,27 @@ __global__ void __launch_bounds__(THREADS) join_parts_kernel(T* __restrict__ out
   float acc[PER_LANE];
 #pragma unroll
   for (int i = 0; i < PER_LANE; ++i) acc[i] = 0.f;
-  for (int p = 0; p < n_parts; ++p) big = fmaxf(big, parts.ml[p * step + item].x);
+  for (int p = lane; p < n_parts; p += 32) big = fmaxf(big, parts.ml[p * step + item].x);
+  big = warp_max(big);
   const float safe = big == -INFINITY ? 0.f : big;
-  for (int p = 0; p < n_parts; ++p) {
-    const float2 ml = parts.ml[p * step + item];
-    if (ml.y == 0.f) continue;
-    const float w = exp2f(ml.x - safe);
-    total += w * ml.y;
+  constexpr int AHEAD = PER_LANE <= 4 ? 8 : 4;  // parts whose loads are on their way together
+  for (int p0 = 0; p0 < n_parts; p0 += AHEAD) {
+    float w[AHEAD], v[AHEAD][PER_LANE];
 #pragma unroll
-    for (int i = 0; i < PER_LANE; ++i) {
-      const int d = lane + 32 * i;
-      if (d < D) acc[i] += w * parts.o[(p * step + item) * D + d];
+    for (int e = 0; e < AHEAD; ++e) {
+      const float2 ml = p0 + e < n_parts ? parts.ml[(p0 + e) * step + item] : make_float2(0.f, 0.f);
+      w[e] = ml.y == 0.f ? 0.f : exp2f(ml.x - safe);
+      total += ml.y == 0.f ? 0.f : w[e] * ml.y;
+#pragma unroll
+      for (int i = 0; i < PER_LANE; ++i) {
+        const int d = lane + 32 * i;
+        v[e][i] = ml.y != 0.f && d < D ? parts.o[((p0 + e) * step + item) * D + d] : 0.f;
+      }
     }
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e)
+#pragma unroll
+      for (int i = 0; i < PER_LANE; ++i) acc[i] += w[e] * v[e][i];
   }
   const float inv = 1.f / total;
 #pragma unroll

@@ -304,6 +304,23 @@ def test_evict_keys_of_many_rows_and_sequences(ops):
     ops.evict_keys(k, v, table, [1], [5700], scores, positions, 1100, 500)
     for got, ref in zip((k, v, scores, positions), want):
         assert torch.equal(got, ref)
+    # as long that the keys of a head do not fit shared memory; by torch's own sort
+    k, v, table, scores, positions = evict_case(F32, 1, 2, 4, 500, 10, n_slots=1, ties=True)
+    L, keep, recent = 31000, 9000, 700
+    rank = scores[0, 0, :, :L].clone()
+    rank.scatter_(-1, positions[0, 0, :, :L].argsort(dim=-1, descending=True)[:, :recent], float("inf"))
+    kept = rank.sort(dim=-1, descending=True, stable=True).indices[:, :keep].sort(dim=-1).values
+    before = [k.clone(), positions.clone()]
+    ops.evict_keys(k, v, table, [0], [L], scores, positions, keep, recent)
+    for h in range(2):
+        stay = set(kept[h].tolist())
+        src = list(range(keep))
+        for d, s in zip([r for r in range(keep) if r not in stay], [r for r in sorted(stay) if r >= keep]):
+            src[d] = s
+        src = torch.tensor(src, device=DEVICE)
+        assert torch.equal(positions[0, 0, h, :keep], before[1][0, 0, h, src])
+        page, old = table[0].long()[torch.arange(keep, device=DEVICE) // PAGE], table[0].long()[src // PAGE]
+        assert torch.equal(k[0, page, h, torch.arange(keep, device=DEVICE) % PAGE], before[0][0, old, h, src % PAGE])
     n = 150
     k, v, table, scores, positions = evict_case(BF16, 1, 1, 8, 2, 9, n_slots=n)
     slots, lengths = list(range(n - 1, -1, -1)), [70 + i % 59 for i in range(n)]
