@@ -57,7 +57,7 @@ _PARTS_SIGNATURES = {
 _PARTS_SIGNATURES.update({
     "krk_prefix_few_rows": [_P, _P, c_int, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_int, c_float, _P, _P],
     "krk_prefix_tcgen05": [_P, _P, c_int, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_int, c_float, _P, _P],
-    "krk_own_single": [_P, _P, _P, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_float, _P, _P],
+    "krk_shared_single": [_P, _P, _P, c_int, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_int, c_float, _P, _P],
     "krk_scored_single": [_P, _P, _P, _P, _P, _P, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_float, _P, _P],
 })
 _PARTS_SIGNATURES.update({
@@ -158,7 +158,7 @@ class CacheOps:
         step = (qkv.data_ptr(), qkv.stride(0), heads, kv, *self._segments(batch, cache, prefix), cache.k.data_ptr(), cache.v.data_ptr())
         by_mma = self._by_mma(qkv, cache, D)
         # the prefixes' parts, then the own keys, which join them
-        splits, own_splits, group_rows, tensor = 0, 0, 0, False
+        splits, own_splits, group_rows, tensor, tiles = 0, 0, 0, False, 0
         if prefix.max_length:
             group_rows = prefix.max_rows(batch)
             tiles = -(-group_rows * per // 16) * kv
@@ -175,28 +175,31 @@ class CacheOps:
         scratch = torch.empty(parts * rows * heads * (D + 2), dtype=torch.float32, device=qkv.device)
         o = scratch.data_ptr()
         ml = o + 4 * parts * rows * heads * D
+        if by_mma and batch.is_decode and (tensor or tiles <= 65535):
+            self.launches += splits > 0
+            self._ok(lib.krk_shared_single(out.data_ptr(), o, ml, splits, self._cluster_splits(-(-per // 16) * kv * batch.n_seqs, False), tensor, *step,
+                                           cache.k.shape[0], group_rows, scale, error, stream), "shared prefix attention")
+            return out
         if splits:
             if tensor or (by_mma and tiles <= 65535):
                 self._ok((lib.krk_prefix_tcgen05 if tensor else lib.krk_prefix_few_rows)(o, ml, rows, 0, splits, *step, cache.k.shape[0], group_rows, scale,
                                                                                          error, stream), "prefix attention")
             else:
                 self._ok(lib.krk_partial_attention(o, ml, rows, 0, splits, 0, *step, group_rows, scale, _code(qkv.dtype), stream), "prefix attention")
-        if not by_mma:
+        if by_mma:
+            self._ok(lib.krk_own_rows(out.data_ptr(), None, o, ml, rows, splits, *step, batch.max_q_len, scale, stream), "attention over own keys")
+        else:
             self._ok(lib.krk_partial_attention(o, ml, rows, splits, own_splits, 1, *step, batch.max_q_len, scale, _code(qkv.dtype), stream),
                      "attention over own keys")
             self._ok(lib.krk_join_parts(out.data_ptr(), None, o, ml, rows, heads, parts, _code(qkv.dtype), stream), "join of parts")
-        elif batch.is_decode:
-            self._ok(lib.krk_own_single(out.data_ptr(), o, ml, splits, self._cluster_splits(-(-per // 16) * kv * batch.n_seqs, False), *step, cache.k.shape[0],
-                                        scale, error, stream), "attention over own keys")
-        else:
-            self._ok(lib.krk_own_rows(out.data_ptr(), None, o, ml, rows, splits, *step, batch.max_q_len, scale, stream), "attention over own keys")
         return out
 
     # -- weights per key -------------------------------------------------------------------
-    def _check_scores(self, what, scores, positions, cache, extra=()):
+    @staticmethod
+    def _check_scores(what, cache, tables):
         shape = (cache.table.shape[0], cache.kv_heads, cache.width * PAGE)
-        for name, t, dtype in (("scores", scores, torch.float32), ("positions", positions, torch.int32), *extra):
-            if t is not None and (tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous() or t.device != cache.k.device):
+        for name, t, dtype in tables:
+            if t is not None and (t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.device != cache.k.device):
                 raise KernelError(f"{what}: {name} are contiguous {dtype} [slots, kv heads, rows of a slot] = {list(shape)} beside the cache, "
                                   f"got {t.dtype} {list(t.shape)}")
 
@@ -208,7 +211,8 @@ class CacheOps:
         rows where keys were evicted. ``out_scores`` takes the sums in place of ``scores``."""
         self._check_step("scored attention", qkv, heads, kv_in_row, head_dim, batch, cache)
         out_scores = scores if out_scores is None else out_scores
-        self._check_scores("scored attention", scores, positions, cache, (("out_scores", out_scores, torch.float32),))
+        self._check_scores("scored attention", cache, (("scores", scores, torch.float32), ("positions", positions, torch.int32),
+                                                       ("out_scores", out_scores, torch.float32)))
         if observe is not None and observe < 1:
             raise KernelError(f"scored attention: at least one query a sequence is observed, got {observe}")
         lib, rows, kv, per, D = self._parts_lib(head_dim), qkv.shape[0], cache.kv_heads, heads // cache.kv_heads, head_dim
@@ -263,57 +267,58 @@ class CacheOps:
         are given up, in ascending order of both; scores and positions move along, or go to ``out_scores`` and ``out_positions`` (rows from
         ``keep`` on are not written). A slot that holds no more than ``keep`` rows stays as it is. ``batch``: the description of a
         single-token step of exactly these slots, whose rows and shifts follow on the device. Returns the rows held now, as a list."""
-        slots, lengths = [int(s) for s in slots], [int(n) for n in lengths]
+        what, error = "eviction", self.error
         keep, recent = int(keep), int(recent)
-        what = "eviction"
-        if k.dim() != 5 or v.dim() != 5 or k.shape[:4] != v.shape[:4] or k.shape[3] != PAGE or k.dtype != v.dtype:
-            raise KernelError(f"{what}: pages are [runs, pages, kv heads, {PAGE}, head size], got {list(k.shape)} and {list(v.shape)}")
+        shape = k.shape
+        runs, n_pages, heads, page, dim = shape if len(shape) == 5 else (0, 0, 0, 0, 0)
+        if page != PAGE or v.dim() != 5 or v.shape[:4] != shape[:4] or k.dtype != v.dtype:
+            raise KernelError(f"{what}: pages are [runs, pages, kv heads, {PAGE}, head size], got {list(shape)} and {list(v.shape)}")
         _code(k.dtype)
-        if any(t.shape[0] and not t[0].is_contiguous() for t in (k, v)) or not table.is_contiguous() or table.dtype != torch.int32:
+        if (k.stride()[1:] != (heads * PAGE * dim, PAGE * dim, dim, 1) or v.stride()[1:] != (heads * PAGE * v.shape[4], PAGE * v.shape[4], v.shape[4], 1)
+                or not table.is_contiguous() or table.dtype != torch.int32):
             raise KernelError(f"{what}: every run's pages and the page table (int32) are contiguous")
         out_scores = scores if out_scores is None else out_scores
         out_positions = positions if out_positions is None else out_positions
-        shape = (k.shape[0], table.shape[0], k.shape[2], table.shape[1] * PAGE)
+        n_slots, width = table.shape
+        capacity = width * PAGE
+        counts = (runs, n_slots, heads, capacity)
         for name, t, dtype in (("scores", scores, torch.float32), ("positions", positions, torch.int32),
                                ("out_scores", out_scores, torch.float32), ("out_positions", out_positions, torch.int32)):
-            if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
-                raise KernelError(f"{what}: {name} are contiguous {dtype} [runs, slots, kv heads, rows of a slot] = {list(shape)}, got {t.dtype} {list(t.shape)}")
-        if any(t.device != self.error.device for t in (k, v, table, scores, positions, out_scores, out_positions)):
-            raise KernelError(f"{what}: every tensor lies on the kernels' device, {self.error.device}")
+            if t.shape != counts or t.dtype != dtype or not t.is_contiguous() or t.device != error.device:
+                raise KernelError(f"{what}: {name} are contiguous {dtype} [runs, slots, kv heads, rows of a slot] = {list(counts)} on {error.device}, "
+                                  f"got {t.dtype} {list(t.shape)} on {t.device}")
+        if k.device != error.device or v.device != error.device or table.device != error.device:
+            raise KernelError(f"{what}: every tensor lies on the kernels' device, {error.device}")
         if keep < 1 or not 0 <= recent <= keep:
             raise KernelError(f"{what}: at least one row stays, and at most as many by their position as stay in all; got keep {keep}, recent {recent}")
-        if len(slots) != len(lengths) or len(set(slots)) != len(slots):
+        n = len(slots)
+        if n != len(lengths) or len(set(slots)) != n:
             raise KernelError(f"{what}: every slot comes once, with its length")
-        for s, n in zip(slots, lengths):
-            if not 0 <= s < shape[1] or not 0 <= n <= shape[3]:
-                raise KernelError(f"{what}: slot {s} of {shape[1]} with {n} rows of {shape[3]}")
-        left = [min(n, keep) for n in lengths]
-        if not slots or k.numel() == 0:
-            return left
-        if batch is not None and (batch.n_seqs != len(slots) or batch.n_rows != len(slots) or getattr(batch, "seq_shift", None) is None):
+        if n == 0:
+            return []
+        longest = max(lengths)
+        if min(slots) < 0 or max(slots) >= n_slots or min(lengths) < 0 or longest > capacity:
+            raise KernelError(f"{what}: slots {list(slots)} of {n_slots} with {list(lengths)} rows of {capacity}")
+        if batch is not None and (batch.n_seqs != n or batch.n_rows != n or getattr(batch, "seq_shift", None) is None):
             raise KernelError(f"{what}: the step that follows has one token of each slot and keeps shifts")
-        runs, heads = shape[0], shape[2]
+        left = [keep if m > keep else m for m in lengths]
+        if k.numel() == 0:
+            return left
+        lib, stream, size = self.cache_lib, self._stream(), k.element_size()
         same = v.data_ptr() == k.data_ptr()
-        size = k.element_size()
-        most = int(self.cache_lib.krk_evict_max_seqs())
-        at = 0
-        while at < len(slots):
-            # as many sequences as the arguments and the scratch take
-            n, moves = 1, max(0, min(keep, lengths[at] - keep))
-            while n < most and at + n < len(slots):
-                m = max(moves, min(keep, lengths[at + n] - keep))
-                if runs * (n + 1) * heads * m * 8 > self.EVICT_SCRATCH_BYTES:
-                    break
-                n, moves = n + 1, m
-            lists = torch.empty(runs * n * heads * (2 * moves + 1), dtype=torch.int32, device=k.device)
-            counts = lists[runs * n * heads * 2 * moves:]
-            ints = c_int * n
-            follow = (None, None, None) if batch is None else tuple(t[at:].data_ptr() for t in (batch.seq_start, batch.row_pos, batch.seq_shift))
-            self._ok(self.cache_lib.krk_evict_keys(
-                k.data_ptr(), None if same else v.data_ptr(), k.stride(0) * size, v.stride(0) * size, k.shape[4] * size, v.shape[4] * size, heads, runs,
-                table.data_ptr(), table.shape[1], scores.data_ptr(), positions.data_ptr(), out_scores.data_ptr(), out_positions.data_ptr(),
-                scores.stride(0), shape[3], ints(*slots[at:at + n]), ints(*lengths[at:at + n]), n, keep, recent, lists.data_ptr(), counts.data_ptr(),
-                moves, *follow, self._stream()), what)
-            self.launches += int(moves > 0)
-            at += n
+        # as many sequences at once as the arguments and the scratch take
+        moves = max(0, min(keep, longest - keep))
+        most = max(1, min(lib.krk_evict_max_seqs(), n, self.EVICT_SCRATCH_BYTES // max(1, runs * heads * moves * 8)))
+        lists = torch.empty(runs * most * heads * (2 * moves + 1), dtype=torch.int32, device=k.device)
+        head = (k.data_ptr(), None if same else v.data_ptr(), k.stride(0) * size, v.stride(0) * size, dim * size, v.shape[4] * size, heads, runs,
+                table.data_ptr(), width, scores.data_ptr(), positions.data_ptr(), out_scores.data_ptr(), out_positions.data_ptr(), scores.stride(0), capacity)
+        moves_at = lists.data_ptr()
+        counts_at = moves_at + 8 * runs * most * heads * moves
+        for at in range(0, n, most):
+            part = slots[at:at + most]
+            ints = c_int * len(part)
+            follow = (None, None, None) if batch is None else (batch.seq_start.data_ptr() + 4 * at, batch.row_pos.data_ptr() + 4 * at,
+                                                               batch.seq_shift.data_ptr() + 4 * at)
+            self._ok(lib.krk_evict_keys(*head, ints(*part), ints(*lengths[at:at + most]), len(part), keep, recent, moves_at, counts_at, moves, *follow,
+                                        stream), what)
         return left

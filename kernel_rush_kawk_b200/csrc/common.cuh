@@ -84,6 +84,20 @@ __device__ __forceinline__ unsigned long long krk_now() {
 #define KRK_TRACE_MARKS_OUT(kind)
 #endif
 
+// Lets a kernel have up to `bytes` of dynamic shared memory, asked once a kernel and device (`allowed`: a static of the caller, one bit a device):
+// the most that its launches ever take, so that no call lowers what another is about to launch with.
+template <typename Kernel>
+inline cudaError_t allow_shared(Kernel kernel, size_t bytes, unsigned long long* allowed) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (device & 63);
+  if (__atomic_load_n(allowed, __ATOMIC_RELAXED) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) __atomic_fetch_or(allowed, bit, __ATOMIC_RELAXED);
+  return e;
+}
+
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                               Args... args) {

@@ -424,13 +424,15 @@ KRK_API int krk_evict_keys(void* k, void* v, long long k_run_bytes, long long v_
   int longest = 0;
   for (int i = 0; i < n_seqs; ++i) longest = lengths[i] > longest ? lengths[i] : longest;
   // Few rows: few threads, whose sums and barriers cost more than the rows do. Rows whose keys do not fit shared memory are read again.
+  static unsigned long long allowed[3] = {0, 0, 0};
+  constexpr size_t MOST = 190 * 1024;
   auto choose = [&](auto* kern, int threads, int staged) {
     const size_t smem = (size_t)staged * 8 + ((size_t)longest + 31) / 32 * 4;
-    cudaError_t e = smem > 200 * 1024 ? cudaErrorInvalidValue : smem > 32 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
+    const cudaError_t e = smem > MOST ? cudaErrorInvalidValue : allow_shared(kern, MOST, allowed + (threads > 128) + (threads > 512));
     return e != cudaSuccess ? e : launch_pdl(kern, dim3((unsigned)heads), dim3(threads), smem, stream, args, seqs, pools, staged);
   };
   cudaError_t e = longest <= 2048    ? choose(choose_rows_kernel<128, 512, true>, 128, longest)
-                  : longest <= 24000 ? choose(choose_rows_kernel<512, 2048, true>, 512, longest)
+                  : longest <= 23000 ? choose(choose_rows_kernel<512, 2048, true>, 512, longest)
                                      : choose(choose_rows_kernel<1024, 2048, false>, 1024, 0);
   if (e != cudaSuccess || max_moves == 0 || move_here) return (int)e;
   // four moves in flight a warp's share, and no more blocks than fill the device a few times over

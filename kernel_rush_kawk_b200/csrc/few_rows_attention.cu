@@ -528,7 +528,8 @@ int launch_few_rows(bf16* out, const Parts& parts, int part0, int n_join, const 
   const size_t smem = Layout(in_ring, splits_in_cluster, inbox_rows).total + 1024;
   if (smem > 227 * 1024) return -2;
   auto kern = few_rows_kernel<TMA_PAGES, PREFIX, SUMS, Rows>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static unsigned long long allowed = 0;
+  cudaError_t e = allow_shared(kern, 227 * 1024, &allowed);
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)n_splits, (unsigned)(row_tiles * HKV), (unsigned)units);
@@ -568,13 +569,37 @@ KRK_API int krk_prefix_few_rows(float* o, float* ml, int rows, int part0, int n_
 
 // One token a sequence: its own keys (all, without groups), joined with the prefix parts 0 .. n_join - 1, which the launch before this one
 // writes (n_join 0: none, and the launch before may write the rows and keys themselves). n_splits: at most 8, blocks of a cluster.
-KRK_API int krk_own_single(void* out, const float* o, const float* ml, int n_join, int n_splits, const void* q, int q_stride, int HQ, int HKV,
+static int krk_own_single(void* out, const float* o, const float* ml, int n_join, int n_splits, const void* q, int q_stride, int HQ, int HKV,
                            KRK_SEGMENTS, const void* k_cache, const void* v_cache, int n_pages, float scale, int* error, cudaStream_t stream) {
   if (n_seqs == 0) return 0;
   const Parts parts = {const_cast<float*>(o), (float2*)const_cast<float*>(ml), n_seqs, HQ};
   auto go = HQ / HKV <= 8 ? launch_few_rows<false, false, Narrow> : launch_few_rows<false, false, Wide>;
   return go((bf16*)out, parts, 0, n_join, q, q_stride, HQ, HKV, KRK_MAKE_SEGMENTS, k_cache, v_cache, n_pages, 1, n_splits, scale, n_join == 0, KeySums{},
             error, stream);
+}
+
+extern "C" int krk_prefix_tcgen05(float*, float*, int, int, int, const void*, int, int, int, const int*, const int*, const int*, const int*, const int*,
+                                  const int*, const int*, int, int, const int*, int, const void*, const void*, int, int, float, int*, cudaStream_t);
+
+// A single-token step behind shared prefixes, both launches: n_splits parts of the prefixes (none: 0; `tensor`: by the tcgen05 kernel), then the own
+// keys, shared by own_splits blocks a sequence, which join them. o, ml: scratch for the parts of n_seqs rows.
+KRK_API int krk_shared_single(void* out, float* o, float* ml, int n_splits, int own_splits, int tensor, const void* q, int q_stride, int HQ, int HKV,
+                              KRK_SEGMENTS, const void* k_cache, const void* v_cache, int n_pages, int max_rows, float scale, int* error,
+                              cudaStream_t stream) {
+  if (n_splits > 0) {
+    int rc;
+#if KRK_HEAD_DIM == 64 || KRK_HEAD_DIM == 128
+    if (tensor)
+      rc = krk_prefix_tcgen05(o, ml, n_seqs, 0, n_splits, q, q_stride, HQ, HKV, cu_q, seq_slot, seq_start, seq_qlen, group_cu, group_len, seq_group, n_seqs,
+                              n_groups, table, width, k_cache, v_cache, n_pages, max_rows, scale, error, stream);
+    else
+#endif
+      rc = krk_prefix_few_rows(o, ml, n_seqs, 0, n_splits, q, q_stride, HQ, HKV, cu_q, seq_slot, seq_start, seq_qlen, group_cu, group_len, seq_group, n_seqs,
+                               n_groups, table, width, k_cache, v_cache, n_pages, max_rows, scale, error, stream);
+    if (rc) return rc;
+  }
+  return krk_own_single(out, o, ml, n_splits, own_splits, q, q_stride, HQ, HKV, cu_q, seq_slot, seq_start, seq_qlen, group_cu, group_len, seq_group, n_seqs,
+                        n_groups, table, width, k_cache, v_cache, n_pages, scale, error, stream);
 }
 
 // One token a sequence over all of its keys, with the weight that each key receives added to its sum (see krk_key_weights). raw: scratch,

@@ -251,7 +251,8 @@ KRK_API int krk_key_weights_tcgen05(const float* sums, float* sums_out, int* pos
   int rc = make_map_bf16(&map_k, k_cache, (long long)n_pages * HKV * KRK_PAGE, D, D, KRK_PAGE);
   if (rc == 0) rc = make_map_bf16_3d(&map_q, q, D, HQ, rows, D, q_stride, G, tile_rows / G);
   if (rc) return rc;
-  cudaError_t e = cudaFuncSetAttribute(key_weights_tcgen05_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
+  static unsigned long long allowed = 0;
+  cudaError_t e = allow_shared(key_weights_tcgen05_kernel, SMEM_BYTES, &allowed);
   if (e != cudaSuccess) return (int)e;
   const Segments seg = {cu_q, seq_slot, seq_start, seq_qlen, group_cu, group_len, seq_group, n_seqs, n_groups, table, width};
   cudaLaunchConfig_t cfg = {};

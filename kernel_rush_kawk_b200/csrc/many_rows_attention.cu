@@ -196,7 +196,8 @@ KRK_API int krk_own_rows(void* out, float* lse, const float* o, const float* ml,
   const long long tiles = ((long long)max_q_len * (HQ / HKV) + 63) / 64;
   if (tiles > 0x7fffffffLL || HKV > 65535 || n_seqs > 65535) return -3;
   const size_t smem = PAGE_SMEM + WEIGHTS_BYTES;
-  cudaError_t e = cudaFuncSetAttribute(many_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static unsigned long long allowed = 0;
+  cudaError_t e = allow_shared(many_rows_kernel, smem, &allowed);
   if (e != cudaSuccess) return (int)e;
   const Parts parts = {const_cast<float*>(o), (float2*)const_cast<float*>(ml), rows, HQ};
   const Segments seg = {cu_q, seq_slot, seq_start, seq_qlen, group_cu, group_len, seq_group, n_seqs, n_groups, table, width};

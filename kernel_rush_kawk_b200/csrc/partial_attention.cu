@@ -321,7 +321,8 @@ int launch_partial(const Parts& parts, int part0, int n_splits, bool own, const 
   const int units = own ? seg.n_seqs : seg.n_groups;
   if (tiles * n_splits > 0x7fffffffLL || HKV > 65535 || units > 65535) return -3;
   auto kern = partial_attention_kernel<T>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
+  static unsigned long long allowed = 0;  // of this instance, one for each type
+  cudaError_t e = allow_shared(kern, SMEM_BYTES, &allowed);
   if (e != cudaSuccess) return (int)e;
   return (int)launch_pdl(kern, dim3((unsigned)(tiles * n_splits), HKV, units), dim3(THREADS), SMEM_BYTES, stream, parts, part0, n_splits, own, (const T*)q,
                          q_stride, HQ, HKV, seg, (const T*)k, (const T*)v, scale * LOG2E);
@@ -365,8 +366,9 @@ KRK_API int krk_key_weights(const float* sums, float* sums_out, int* positions, 
   if (n_seqs == 0) return 0;
   if (HKV > 65535 || n_seqs > 65535 || page_blocks < 1) return -3;
   const dim3 grid(page_blocks, HKV, n_seqs);
+  static unsigned long long allowed[2] = {0, 0};
   auto go = [&](auto* kern, auto* queries, auto* keys) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
+    cudaError_t e = allow_shared(kern, SMEM_BYTES, allowed + (dtype == KRK_DTYPE_F32));
     if (e != cudaSuccess) return (int)e;
     return (int)launch_pdl(kern, grid, dim3(THREADS), SMEM_BYTES, stream, sums, sums_out, positions, seq_shift, capacity, lse, observe, queries,
                            q_stride, HQ, HKV, seg, keys, scale * LOG2E);

@@ -344,7 +344,8 @@ KRK_API int krk_prefix_tcgen05(float* o, float* ml, int rows, int part0, int n_s
   CUtensorMap map_q = map_k;
   if (rc == 0 && q_by_tma) rc = make_map_bf16_3d(&map_q, q, D, HQ, rows, D, q_stride, G, tile_rows / G);
   if (rc) return rc;
-  cudaError_t e = cudaFuncSetAttribute(prefix_tcgen05_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES);
+  static unsigned long long allowed = 0;
+  cudaError_t e = allow_shared(prefix_tcgen05_kernel, SMEM_BYTES, &allowed);
   if (e != cudaSuccess) return (int)e;
   const Parts parts = {o, (float2*)ml, rows, HQ};
   const Segments seg = {cu_q, seq_slot, seq_start, seq_qlen, group_cu, group_len, seq_group, n_seqs, n_groups, table, width};
