@@ -56,7 +56,7 @@ _PARTS_SIGNATURES = {
 }
 _PARTS_SIGNATURES.update({
     "krk_prefix_few_rows": [_P, _P, c_int, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_int, c_float, _P, _P],
-    "krk_prefix_tcgen05": [_P, _P, c_int, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_int, c_float, _P, _P],
+    "krk_prefix_tcgen05": [_P, _P, c_int, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_int, c_int, c_float, _P, _P],
     "krk_shared_single": [_P, _P, _P, c_int, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_int, c_float, _P, _P],
     "krk_scored_single": [_P, _P, _P, _P, _P, _P, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_float, _P, _P],
 })
@@ -158,12 +158,12 @@ class CacheOps:
         step = (qkv.data_ptr(), qkv.stride(0), heads, kv, *self._segments(batch, cache, prefix), cache.k.data_ptr(), cache.v.data_ptr())
         by_mma = self._by_mma(qkv, cache, D)
         # the prefixes' parts, then the own keys, which join them
-        splits, own_splits, group_rows, tensor, tiles = 0, 0, 0, False, 0
+        splits, own_splits, group_rows, tensor, tiles = 0, 0, 0, 0, 0
         if prefix.max_length:
             group_rows = prefix.max_rows(batch)
             tiles = -(-group_rows * per // 16) * kv
-            tensor = by_mma and group_rows * per >= self.PREFIX_TENSOR_ROWS and self._by_tcgen05(qkv, D)
-            if tensor:
+            if by_mma and group_rows * per >= self.PREFIX_TENSOR_ROWS and self._by_tcgen05(qkv, D):
+                tensor = 2 if group_rows * per <= 112 else 1  # one tile: its halves take the pages in turn
                 splits = max(1, min(32, 148 // (-(-group_rows * per // 256) * kv * prefix.n_groups)))
             else:
                 # eight sequences of four heads behind 1,024 positions: 16.5 us with one block an SM, 18.6 with two, 22.7 with three (the
@@ -171,7 +171,7 @@ class CacheOps:
                 splits = self._splits(tiles * prefix.n_groups, 148 if by_mma else 444)
         if not by_mma:
             own_splits = self._splits(-(-batch.max_q_len * per // 16) * kv * batch.n_seqs)
-        parts = splits + own_splits
+        parts = splits * max(tensor, 1) + own_splits
         scratch = torch.empty(parts * rows * heads * (D + 2), dtype=torch.float32, device=qkv.device)
         o = scratch.data_ptr()
         ml = o + 4 * parts * rows * heads * D
@@ -181,9 +181,12 @@ class CacheOps:
                                            cache.k.shape[0], group_rows, scale, error, stream), "shared prefix attention")
             return out
         if splits:
-            if tensor or (by_mma and tiles <= 65535):
-                self._ok((lib.krk_prefix_tcgen05 if tensor else lib.krk_prefix_few_rows)(o, ml, rows, 0, splits, *step, cache.k.shape[0], group_rows, scale,
-                                                                                         error, stream), "prefix attention")
+            if tensor:
+                self._ok(lib.krk_prefix_tcgen05(o, ml, rows, 0, splits, *step, cache.k.shape[0], group_rows, tensor == 2, scale, error, stream),
+                         "prefix attention")
+                splits *= tensor
+            elif by_mma and tiles <= 65535:
+                self._ok(lib.krk_prefix_few_rows(o, ml, rows, 0, splits, *step, cache.k.shape[0], group_rows, scale, error, stream), "prefix attention")
             else:
                 self._ok(lib.krk_partial_attention(o, ml, rows, 0, splits, 0, *step, group_rows, scale, _code(qkv.dtype), stream), "prefix attention")
         if by_mma:

@@ -249,7 +249,7 @@ choose_rows_kernel(const ChooseArgs a, const Sequences seqs, const Pools pools, 
   unsigned *pos_s = dynamic_s, *sum_s = dynamic_s + staged_rows;  // order_of each; a sum that does not stand for election becomes 0, which no number has
   unsigned* kept_s = dynamic_s + 2 * staged_rows;
   grid_dependency_wait();
-  grid_launch_dependents();
+  if (!a.seq_start) grid_launch_dependents();  // kernels read a step's description before they wait for the one before: none overtakes its change
   const int kh = blockIdx.x % a.HKV, seq = blockIdx.x / a.HKV % a.n_seqs, run = blockIdx.x / a.HKV / a.n_seqs;
   const int L = seqs.length[seq], keep = a.keep;
   const size_t base = run * a.run_stride + ((size_t)seqs.slot[seq] * a.HKV + kh) * a.capacity;

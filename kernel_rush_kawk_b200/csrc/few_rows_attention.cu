@@ -579,10 +579,10 @@ static int krk_own_single(void* out, const float* o, const float* ml, int n_join
 }
 
 extern "C" int krk_prefix_tcgen05(float*, float*, int, int, int, const void*, int, int, int, const int*, const int*, const int*, const int*, const int*,
-                                  const int*, const int*, int, int, const int*, int, const void*, const void*, int, int, float, int*, cudaStream_t);
+                                  const int*, const int*, int, int, const int*, int, const void*, const void*, int, int, int, float, int*, cudaStream_t);
 
-// A single-token step behind shared prefixes, both launches: n_splits parts of the prefixes (none: 0; `tensor`: by the tcgen05 kernel), then the own
-// keys, shared by own_splits blocks a sequence, which join them. o, ml: scratch for the parts of n_seqs rows.
+// A single-token step behind shared prefixes, both launches: n_splits parts of the prefixes (none: 0; `tensor` 1: by the tcgen05 kernel, 2: by its
+// halves, n_splits each), then the own keys, shared by own_splits blocks a sequence, which join them. o, ml: scratch for the parts of n_seqs rows.
 KRK_API int krk_shared_single(void* out, float* o, float* ml, int n_splits, int own_splits, int tensor, const void* q, int q_stride, int HQ, int HKV,
                               KRK_SEGMENTS, const void* k_cache, const void* v_cache, int n_pages, int max_rows, float scale, int* error,
                               cudaStream_t stream) {
@@ -591,14 +591,14 @@ KRK_API int krk_shared_single(void* out, float* o, float* ml, int n_splits, int 
 #if KRK_HEAD_DIM == 64 || KRK_HEAD_DIM == 128
     if (tensor)
       rc = krk_prefix_tcgen05(o, ml, n_seqs, 0, n_splits, q, q_stride, HQ, HKV, cu_q, seq_slot, seq_start, seq_qlen, group_cu, group_len, seq_group, n_seqs,
-                              n_groups, table, width, k_cache, v_cache, n_pages, max_rows, scale, error, stream);
+                              n_groups, table, width, k_cache, v_cache, n_pages, max_rows, tensor == 2, scale, error, stream);
     else
 #endif
       rc = krk_prefix_few_rows(o, ml, n_seqs, 0, n_splits, q, q_stride, HQ, HKV, cu_q, seq_slot, seq_start, seq_qlen, group_cu, group_len, seq_group, n_seqs,
                                n_groups, table, width, k_cache, v_cache, n_pages, max_rows, scale, error, stream);
     if (rc) return rc;
   }
-  return krk_own_single(out, o, ml, n_splits, own_splits, q, q_stride, HQ, HKV, cu_q, seq_slot, seq_start, seq_qlen, group_cu, group_len, seq_group, n_seqs,
+  return krk_own_single(out, o, ml, tensor == 2 ? 2 * n_splits : n_splits, own_splits, q, q_stride, HQ, HKV, cu_q, seq_slot, seq_start, seq_qlen, group_cu, group_len, seq_group, n_seqs,
                         n_groups, table, width, k_cache, v_cache, n_pages, scale, error, stream);
 }
 
