@@ -149,7 +149,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   const int n_rows = q_len * G;
   const int pair_row = pair * 2 * rows;
   if (pair_row >= n_rows) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (the warp's number, and known to the compiler as such)
 
   const TileRange r0 = tile_range(pair_row, rows, n_rows, G, q_len, start, window);
   const TileRange r1 = tile_range(pair_row + rows, rows, n_rows, G, q_len, start, window);
@@ -247,40 +247,43 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   } else if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 8) {
-    if (lane == 0) {
-      // ---- issuer: TMA loads and MMAs ----
+      // ---- issuer of the MMAs, the whole warp ----
       // a negative scale: the products leave negated (the descriptor's bit for A), and the softmax takes the scale's size, so that maxima
       // before it are maxima after it and a score that is not seen is minus infinity
       const uint32_t idesc_s = (!WIDE && scale_log2 < 0.f ? 1u << 13 : 0u) | (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(KEYS >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
       constexpr uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
       bool ok = true;
-      auto give_up = [&](int code) { atomicExch(error, code); ok = false; };
+      auto give_up = [&](int code) { if (lane == 0) atomicExch(error, code); ok = false; };
+      auto wait = [&](int bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bars + bar, parity)); };
+      // Descriptors: what does not change is put together once, and an instruction's own differ from these by their address (in 16 bytes, in
+      // the low word, with no carry).
+      const uint64_t q_desc = umma_desc_sw128(q_s, 16, 1024), k_desc = umma_desc_sw128(k_s, 16, 1024), v_desc = umma_desc_sw128(v_s, SUB, 1024);
+      auto moved = [](uint64_t desc, uint32_t by) { return (desc & 0xffffffff00000000ull) | ((uint32_t)desc + by); };
       auto qk = [&](int t, int i) {  // S_t = Q_t K_i^T
-        const unsigned char* q = q_s + t * TILE_BYTES;
-        const unsigned char* k = k_s + (i & 1) * TILE_BYTES;
+        const uint64_t qd = moved(q_desc, t * (TILE_BYTES >> 4)), kd = moved(k_desc, (i & 1) * (TILE_BYTES >> 4));
 #pragma unroll
         for (int h = 0; h < DB; ++h)
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            umma_bf16(tmem + t * 128, umma_desc_sw128(q + h * SUB + kk * 32, 16, 1024),
-                      umma_desc_sw128(k + h * SUB + kk * 32, 16, 1024), idesc_s, (h > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(bars + S_FULL + t);
+            umma_bf16_warp(tmem + t * 128, moved(qd, h * (SUB >> 4) + kk * 2), moved(kd, h * (SUB >> 4) + kk * 2), idesc_s,
+                           (h > 0 || kk > 0) ? 1u : 0u);
+        umma_commit_warp(bars + S_FULL + t);
       };
       // WIDE: whether a tile's first block has a first page, and its last block a second one, that no row of it sees. Such a page
       // stays out of P V: its weights are zero, but its values may be anything (the second page of a sequence's last block
       // may belong to another sequence), and zero times infinity is not zero.
-      bool skip_first[2], skip_last[2];
+      bool skip_first[2] = {false, false}, skip_last[2] = {false, false};
       auto pv = [&](int t, int i, bool first, bool last) {  // O_t (+)= P_t V_i, 16 keys (8 columns of P) per instruction
-        const unsigned char* v = v_s + (i & 1) * TILE_BYTES;
+        const uint64_t vd = moved(v_desc, (i & 1) * (TILE_BYTES >> 4));
         if constexpr (WIDE) {
           const bool skip = first && skip_first[t];
           auto page = [&](int k0) {
 #pragma unroll
             for (int ks = k0; ks < k0 + KEYS / 32; ++ks) {
-              umma_bf16_tmem_a(tmem + TMEM_O + t * D, tmem + t * 128 + ks * 8, umma_desc_sw128(v + ks * 16 * 128, SUB, 1024),
+              umma_bf16_tmem_a_warp(tmem + TMEM_O + t * D, tmem + t * 128 + ks * 8, moved(vd, ks * (16 * 128 >> 4)),
                                idesc_o, (first && ks == 0) || (skip && ks == KEYS / 32) ? 0u : 1u);
               // the weights' low halves
-              umma_bf16_tmem_a(tmem + TMEM_O + t * D, tmem + t * 128 + 64 + ks * 8, umma_desc_sw128(v + ks * 16 * 128, SUB, 1024),
+              umma_bf16_tmem_a_warp(tmem + TMEM_O + t * D, tmem + t * 128 + 64 + ks * 8, moved(vd, ks * (16 * 128 >> 4)),
                                idesc_o, 1u);
             }
           };
@@ -289,18 +292,18 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         } else {
 #pragma unroll
           for (int ks = 0; ks < KEYS / 16; ++ks)
-            umma_bf16_tmem_a(tmem + TMEM_O + t * D, tmem + t * 128 + ks * 8, umma_desc_sw128(v + ks * 16 * 128, SUB, 1024),
+            umma_bf16_tmem_a_warp(tmem + TMEM_O + t * D, tmem + t * 128 + ks * 8, moved(vd, ks * (16 * 128 >> 4)),
                              idesc_o, (first && ks == 0) ? 0u : 1u);
         }
       };
       const TileRange rng[2] = {r0, r1};
-      if (q_by_tma && !mbar_wait(bars + Q_FULL, 0)) give_up(14);
-      if (ok && !mbar_wait(bars + K_FULL, 0)) give_up(6);
+      if (q_by_tma && !wait(Q_FULL, 0)) give_up(14);
+      if (ok && !wait(K_FULL, 0)) give_up(6);
       if (ok) {
         tc_fence_after();
         if (r0.has(j_lo)) qk(0, 0);
         if (r1.has(j_lo)) qk(1, 0);
-        umma_commit(bars + K_FREE);
+        umma_commit_warp(bars + K_FREE);
       }
       if constexpr (WIDE) {  // here, while the first scores are on their way
 #pragma unroll
@@ -315,31 +318,30 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (rng[t].has(j)) {
-            if (!mbar_wait(bars + P_READY + t, (j - rng[t].lo) & 1)) { give_up(8); break; }
+            if (!wait(P_READY + t, (j - rng[t].lo) & 1)) { give_up(8); break; }
             if (!v_ready) {
-              if (!mbar_wait(bars + V_FULL + b, (i >> 1) & 1)) { give_up(9); break; }
-              if (LSE && clean_from < KEYS && i == n - 1 && !mbar_wait(bars + V_CLEAN, 0)) { give_up(9); break; }
+              if (!wait(V_FULL + b, (i >> 1) & 1)) { give_up(9); break; }
+              if (LSE && clean_from < KEYS && i == n - 1 && !wait(V_CLEAN, 0)) { give_up(9); break; }
               v_ready = true;
             }
             tc_fence_after();
             pv(t, i, j == rng[t].lo, j == rng[t].hi);
-            if (j == rng[t].hi) umma_commit(bars + O_DONE + t);
+            if (j == rng[t].hi) umma_commit_warp(bars + O_DONE + t);
           }
-          if (t == 1) umma_commit(bars + V_FREE + b);
+          if (t == 1) umma_commit_warp(bars + V_FREE + b);
           if (i + 1 < n) {
             if (rng[t].has(j + 1)) {
               if (!k_ready) {
-                if (!mbar_wait(bars + K_FULL + ((i + 1) & 1), ((i + 1) >> 1) & 1)) { give_up(10); break; }
+                if (!wait(K_FULL + ((i + 1) & 1), ((i + 1) >> 1) & 1)) { give_up(10); break; }
                 k_ready = true;
               }
               tc_fence_after();
               qk(t, i + 1);
             }
-            if (t == 1) umma_commit(bars + K_FREE + ((i + 1) & 1));
+            if (t == 1) umma_commit_warp(bars + K_FREE + ((i + 1) & 1));
           }
         }
       }
-    }
     } else if (warp == 9) {
     if (lane == 0) {
       // ---- loader: the TMA loads after the first ones. A thread of its own: issuing a load takes the time of
@@ -362,7 +364,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
       const int i = n - 1;
       if (__all_sync(0xffffffffu, (n == 1 || mbar_wait(bars + LAST_V, 0)) && mbar_wait(bars + V_FULL + (i & 1), (i >> 1) & 1))) {
         unsigned char* v = v_s + (i & 1) * TILE_BYTES;
-        const int pieces = (KEYS - clean_from) * 8;
+        const int pieces = max(1, (KEYS - clean_from) * 8);
         for (int p = lane; p < DB * pieces; p += 32)
           *reinterpret_cast<uint4*>(v + (p / pieces) * SUB + (size_t)clean_from * 128 + (p % pieces) * 16) = make_uint4(0, 0, 0, 0);
         fence_async_smem();
