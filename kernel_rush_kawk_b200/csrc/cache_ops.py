@@ -50,7 +50,7 @@ def _ptr(t) -> int | None:
 
 _SEGMENTS = [_P] * 7 + [c_int, c_int, _P, c_int]
 _PARTS_SIGNATURES = {
-    "krk_partial_attention": [_P, _P, c_int, c_int, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_float, c_int, _P],
+    "krk_partial_attention": [_P, _P, c_int, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_int, c_float, c_int, _P],
     "krk_join_parts": [_P, _P, _P, _P, c_int, c_int, c_int, c_int, _P],
     "krk_key_weights": [_P, _P, _P, _P, c_int, _P, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, c_int, c_float, c_int, _P],
 }
@@ -114,7 +114,7 @@ class CacheOps:
                 cache.table.data_ptr(), cache.width)
 
     @staticmethod
-    def _splits(blocks: int, wanted: int = 444) -> int:
+    def _splits(blocks: int, wanted: int) -> int:
         """Parts that the keys of a unit of work are split into, so that there are blocks enough for the device. By the numbers of rows
         and heads, never by lengths: a captured step stays valid."""
         return max(1, min(32, -(-wanted // max(blocks, 1))))
@@ -156,45 +156,40 @@ class CacheOps:
             return out
         scale, stream, error = float(scale), self._stream(), self.error.data_ptr()
         step = (qkv.data_ptr(), qkv.stride(0), heads, kv, *self._segments(batch, cache, prefix), cache.k.data_ptr(), cache.v.data_ptr())
-        by_mma = self._by_mma(qkv, cache, D)
+        group_rows = prefix.max_rows(batch) if prefix.max_length else 0
+        tiles = -(-group_rows * per // 16) * kv
+        by_mma = self._by_mma(qkv, cache, D) and tiles <= 65535
         # the prefixes' parts, then the own keys, which join them
-        splits, own_splits, group_rows, tensor, tiles = 0, 0, 0, 0, 0
-        if prefix.max_length:
-            group_rows = prefix.max_rows(batch)
-            tiles = -(-group_rows * per // 16) * kv
-            if by_mma and group_rows * per >= self.PREFIX_TENSOR_ROWS and self._by_tcgen05(qkv, D):
-                tensor = 2 if group_rows * per <= 112 else 1  # one tile: its halves take the pages in turn
-                splits = max(1, min(32, 148 // (-(-group_rows * per // 256) * kv * prefix.n_groups)))
-            else:
-                # eight sequences of four heads behind 1,024 positions: 16.5 us with one block an SM, 18.6 with two, 22.7 with three (the
-                # parts that the own keys' kernel has to join grow with them)
-                splits = self._splits(tiles * prefix.n_groups, 148 if by_mma else 444)
+        own_splits, tensor = 0, 0
         if not by_mma:
-            own_splits = self._splits(-(-batch.max_q_len * per // 16) * kv * batch.n_seqs)
+            splits = self._splits(tiles * prefix.n_groups, 444) if group_rows else 0
+            own_splits = self._splits(-(-batch.max_q_len * per // 16) * kv * batch.n_seqs, 444)
+        elif group_rows * per >= self.PREFIX_TENSOR_ROWS and self._by_tcgen05(qkv, D):
+            tensor = 2 if group_rows * per <= 112 else 1  # one tile: its halves take the keys in turn
+            splits = max(1, min(32, 148 // (-(-group_rows * per // 256) * kv * prefix.n_groups)))
+        else:
+            # eight sequences of four heads behind 1,024 positions: 16.5 us with one block an SM, 18.6 with two, 22.7 with three (the
+            # parts that the own keys' kernel has to join grow with them)
+            splits = self._splits(tiles * prefix.n_groups, 148) if group_rows else 0
         parts = splits * max(tensor, 1) + own_splits
         scratch = torch.empty(parts * rows * heads * (D + 2), dtype=torch.float32, device=qkv.device)
         o = scratch.data_ptr()
         ml = o + 4 * parts * rows * heads * D
-        if by_mma and batch.is_decode and (tensor or tiles <= 65535):
+        if not by_mma:
+            code = _code(qkv.dtype)
+            self._ok(lib.krk_partial_attention(o, ml, rows, splits, own_splits, *step, group_rows, batch.max_q_len, scale, code, stream), "attention in parts")
+            self._ok(lib.krk_join_parts(out.data_ptr(), None, o, ml, rows, heads, parts, code, stream), "join of parts")
+        elif batch.is_decode:
             self.launches += splits > 0
             self._ok(lib.krk_shared_single(out.data_ptr(), o, ml, splits, self._cluster_splits(-(-per // 16) * kv * batch.n_seqs, False), tensor, *step,
                                            cache.k.shape[0], group_rows, scale, error, stream), "shared prefix attention")
-            return out
-        if splits:
+        else:
             if tensor:
                 self._ok(lib.krk_prefix_tcgen05(o, ml, rows, 0, splits, *step, cache.k.shape[0], group_rows, tensor == 2, scale, error, stream),
                          "prefix attention")
-                splits *= tensor
-            elif by_mma and tiles <= 65535:
+            elif splits:
                 self._ok(lib.krk_prefix_few_rows(o, ml, rows, 0, splits, *step, cache.k.shape[0], group_rows, scale, error, stream), "prefix attention")
-            else:
-                self._ok(lib.krk_partial_attention(o, ml, rows, 0, splits, 0, *step, group_rows, scale, _code(qkv.dtype), stream), "prefix attention")
-        if by_mma:
-            self._ok(lib.krk_own_rows(out.data_ptr(), None, o, ml, rows, splits, *step, batch.max_q_len, scale, stream), "attention over own keys")
-        else:
-            self._ok(lib.krk_partial_attention(o, ml, rows, splits, own_splits, 1, *step, batch.max_q_len, scale, _code(qkv.dtype), stream),
-                     "attention over own keys")
-            self._ok(lib.krk_join_parts(out.data_ptr(), None, o, ml, rows, heads, parts, _code(qkv.dtype), stream), "join of parts")
+            self._ok(lib.krk_own_rows(out.data_ptr(), None, o, ml, rows, parts, *step, batch.max_q_len, scale, stream), "attention over own keys")
         return out
 
     # -- weights per key -------------------------------------------------------------------
@@ -244,11 +239,11 @@ class CacheOps:
             self._ok(lib.krk_own_rows(out.data_ptr(), lse.data_ptr(), None, None, rows, 0, *q, *segments, *pages, batch.max_q_len, scale, stream),
                      "scored attention")
         else:
-            parts = self._splits(-(-batch.max_q_len * per // 16) * kv * batch.n_seqs)
+            parts = self._splits(-(-batch.max_q_len * per // 16) * kv * batch.n_seqs, 444)
             scratch = torch.empty(parts * rows * heads * (D + 2), dtype=torch.float32, device=qkv.device)
             o = scratch.data_ptr()
             ml = o + 4 * parts * rows * heads * D
-            self._ok(lib.krk_partial_attention(o, ml, rows, 0, parts, 1, *q, *segments, *pages, batch.max_q_len, scale, _code(qkv.dtype), stream),
+            self._ok(lib.krk_partial_attention(o, ml, rows, 0, parts, *q, *segments, *pages, 0, batch.max_q_len, scale, _code(qkv.dtype), stream),
                      "scored attention")
             self._ok(lib.krk_join_parts(out.data_ptr(), lse.data_ptr(), o, ml, rows, heads, parts, _code(qkv.dtype), stream), "join of parts")
         if by_tcgen05 and not batch.is_decode and per <= 64:

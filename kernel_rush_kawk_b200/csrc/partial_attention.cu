@@ -97,18 +97,22 @@ __device__ __forceinline__ void scores(const Shared& sm, float (&s)[8]) {
   }
 }
 
-// Block (tile x split, kv head, group or sequence); `own`: sequences.
+// Block (tile x split, kv head, group or sequence): the groups' prefixes first, in n_prefix parts, then the sequences' own keys in
+// n_own more.
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
-partial_attention_kernel(Parts parts, int part0, int n_splits, bool own, const T* __restrict__ q, int q_stride, int HQ, int HKV, Segments seg,
+partial_attention_kernel(Parts parts, int n_prefix, int n_own, const T* __restrict__ q, int q_stride, int HQ, int HKV, Segments seg,
                          const T* __restrict__ k_cache, const T* __restrict__ v_cache, float scale_log2) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Shared& sm = *reinterpret_cast<Shared*>(smem_raw);
   grid_dependency_wait();
   grid_launch_dependents();  // in this order: the kernel behind a prefix's parts reads rows and keys before it waits for these
   const int kh = blockIdx.y, G = HQ / HKV;
+  const int groups = n_prefix > 0 ? seg.n_groups : 0;
+  const bool own = (int)blockIdx.z >= groups;
+  const int n_splits = own ? n_own : n_prefix, part0 = own ? n_prefix : 0;
   const int split = blockIdx.x % n_splits, tile = blockIdx.x / n_splits;
-  const Unit u = own ? own_unit(seg, blockIdx.z) : prefix_unit(seg, blockIdx.z);
+  const Unit u = own ? own_unit(seg, blockIdx.z - groups) : prefix_unit(seg, blockIdx.z);
   const int n_rows = u.n_tok * G;
   if (tile * TILE >= n_rows) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -315,17 +319,18 @@ key_weights_kernel(const float* sums, float* sums_out, int* __restrict__ positio
 }
 
 template <typename T>
-int launch_partial(const Parts& parts, int part0, int n_splits, bool own, const void* q, int q_stride, int HQ, int HKV, const Segments& seg, const void* k,
-                   const void* v, int max_rows, float scale, cudaStream_t stream) {
-  const long long tiles = ((long long)max_rows * (HQ / HKV) + TILE - 1) / TILE;
-  const int units = own ? seg.n_seqs : seg.n_groups;
-  if (tiles * n_splits > 0x7fffffffLL || HKV > 65535 || units > 65535) return -3;
+int launch_partial(const Parts& parts, int n_prefix, int n_own, const void* q, int q_stride, int HQ, int HKV, const Segments& seg, const void* k,
+                   const void* v, int group_rows, int own_rows, float scale, cudaStream_t stream) {
+  auto blocks_of = [&](int rows, int splits) { return ((long long)rows * (HQ / HKV) + TILE - 1) / TILE * splits; };
+  const long long prefix_blocks = n_prefix > 0 ? blocks_of(group_rows, n_prefix) : 0, own_blocks = blocks_of(own_rows, n_own);
+  const long long blocks = prefix_blocks > own_blocks ? prefix_blocks : own_blocks;
+  const int units = seg.n_seqs + (n_prefix > 0 ? seg.n_groups : 0);
+  if (blocks > 0x7fffffffLL || HKV > 65535 || units > 65535) return -3;
   auto kern = partial_attention_kernel<T>;
   static unsigned long long allowed = 0;  // of this instance, one for each type
   cudaError_t e = allow_shared(kern, SMEM_BYTES, &allowed);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(kern, dim3((unsigned)(tiles * n_splits), HKV, units), dim3(THREADS), SMEM_BYTES, stream, parts, part0, n_splits, own, (const T*)q,
-                         q_stride, HQ, HKV, seg, (const T*)k, (const T*)v, scale * LOG2E);
+  return (int)launch_pdl(kern, dim3((unsigned)blocks, HKV, units), dim3(THREADS), SMEM_BYTES, stream, parts, n_prefix, n_own, (const T*)q, q_stride, HQ, HKV, seg, (const T*)k, (const T*)v, scale * LOG2E);
 }
 
 }  // namespace
@@ -336,16 +341,15 @@ int launch_partial(const Parts& parts, int part0, int n_splits, bool own, const 
 #define KRK_MAKE_SEGMENTS \
   Segments { cu_q, seq_slot, seq_start, seq_qlen, group_cu, group_len, seq_group, n_seqs, n_groups, table, width }
 
-// Parts part0 .. part0 + n_splits - 1: of the groups' prefixes (own = 0) or of the sequences' other keys (own = 1). max_rows: the most
-// rows of the step that a group (a sequence) has.
-KRK_API int krk_partial_attention(float* o, float* ml, int rows, int part0, int n_splits, int own, const void* q, int q_stride, int HQ, int HKV,
-                                  KRK_SEGMENTS, const void* k_cache, const void* v_cache, int max_rows, float scale, int dtype,
-                                  cudaStream_t stream) {
+// Parts 0 .. n_prefix - 1 of the groups' prefixes (none: 0) and the next n_own of the sequences' other keys. group_rows, own_rows: the most rows of the
+// step that a group and a sequence have.
+KRK_API int krk_partial_attention(float* o, float* ml, int rows, int n_prefix, int n_own, const void* q, int q_stride, int HQ, int HKV, KRK_SEGMENTS,
+                                  const void* k_cache, const void* v_cache, int group_rows, int own_rows, float scale, int dtype, cudaStream_t stream) {
   const Parts parts = {o, (float2*)ml, rows, HQ};
   const Segments seg = KRK_MAKE_SEGMENTS;
-  if (rows == 0 || max_rows == 0 || (own ? n_seqs : n_groups) == 0) return 0;
-  return dtype == KRK_DTYPE_F32 ? launch_partial<float>(parts, part0, n_splits, own != 0, q, q_stride, HQ, HKV, seg, k_cache, v_cache, max_rows, scale, stream)
-                                : launch_partial<bf16>(parts, part0, n_splits, own != 0, q, q_stride, HQ, HKV, seg, k_cache, v_cache, max_rows, scale, stream);
+  if (rows == 0 || own_rows == 0 || n_seqs == 0 || n_own < 1) return 0;
+  return dtype == KRK_DTYPE_F32 ? launch_partial<float>(parts, n_prefix, n_own, q, q_stride, HQ, HKV, seg, k_cache, v_cache, group_rows, own_rows, scale, stream)
+                                : launch_partial<bf16>(parts, n_prefix, n_own, q, q_stride, HQ, HKV, seg, k_cache, v_cache, group_rows, own_rows, scale, stream);
 }
 
 KRK_API int krk_join_parts(void* out, float* lse, const float* o, const float* ml, int rows, int HQ, int n_parts, int dtype, cudaStream_t stream) {
