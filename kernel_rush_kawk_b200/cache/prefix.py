@@ -12,6 +12,47 @@ from .allocator import CacheError
 from .store import PAGE
 
 
+# Where reading a prefix once pays. It takes a launch more, and parts of the softmax that have to join, so that what a step does not read again
+# has to be worth these.
+#
+# Single tokens, by the bytes of keys and values of one layer that are not read again: 8 MB a sequence, up to eight of them. A layer's attention with
+# rotation and cache write, us, each sequence by itself and shared, 32 heads over 8 of 128 with 100 keys of their own: 2 sequences behind 4,096 positions
+# (17 MB) 13.9 and 15.0, 8,192 22.8 and 16.9; 4 behind 2,048 (25 MB) 15.6 and 17.0, 4,096 22.1 and 18.7; 8 behind 2,048 (59 MB) 15.4 and 18.1,
+# 4,096 24.4 and 21.3; 16 behind 1,024 (63 MB) 16.2 and 18.9, 2,048 24.5 and 19.0; 64 behind 256 (66 MB) 22.9 and 21.6, 1,024 47.9 and 23.4, 8,192
+# 278.8 and 30.9. 16 heads over 4 of 64, a quarter of the bytes: 32 behind 1,024 (33 MB) 12.3 and 17.2, 2,048 18.9 and 18.0; 64 behind 1,024 (66 MB) 18.8 and
+# 17.5.
+SHARE_BYTES = 8 << 20
+# Several tokens a sequence: where the products bound the step, sharing saves whole rounds of the device alone (row tiles of short or ragged
+# sequences that share theirs, keys split over blocks that would stand idle), and costs the join. Counted in steps of 128 keys (about 2 us, of a pair of
+# row tiles; 1.75 times that in the kernel of steps of less than a tile): rounds * steps by themselves against rounds * steps + 8 + (rows * heads) / 4,096.
+# Measured behind 1,024 and 4,096 positions, us, by themselves and shared, 32 heads over 8 of 128: 2 sequences of 4 tokens 32.7 and 18.5, 116 and 25;
+# 4 of 16 31.8 and 36.4, 110 and 38.6; 32 of 4 45 and 26.2, 157 and 31.8; 4 of 60 24.7 and 25.3, 66 and 36.4; 16 of 60 26.4 and 40.9, 70 and 82; 16 of 45 to
+# 90 behind 4,096 129 and 94; 2 of 250 26.8 and 33.3, 69 and 55; 4 of 250 28 and 51, 71 and 92; 16 heads over 4 of 64, 16 of 60 23.6 and 22.1, 65
+# and 42, 32 of 60 24.2 and 30.7, 66 and 70.
+JOIN_STEPS = 8
+
+
+def single_tokens_share(sizes, lengths, row_bytes: int) -> bool:
+    """Whether a step of one token a sequence reads these groups' prefixes once. ``row_bytes``: of one position's keys and values in one layer."""
+    saved = sum((size - 1) * length for size, length in zip(sizes, lengths)) * row_bytes
+    return saved >= SHARE_BYTES * min(sum(sizes), 8)
+
+
+def longer_steps_share(sizes, lengths, q_lens, per: int, kv_heads: int) -> bool:
+    """Whether a step of several tokens a sequence reads these groups' prefixes once. ``per``: query heads of a kv head."""
+    steps = max(lengths) / 128
+    if 1.75 * steps < JOIN_STEPS:
+        return False
+    tile, factor = (256, 1.0) if max(q_lens) * per >= 128 else (64, 1.75)
+    alone = sum(-(-n * per // tile) for n in q_lens) * kv_heads
+    shared, at = 0, 0
+    for size in sizes:
+        shared += -(-sum(q_lens[at:at + size]) * per // 256) * kv_heads
+        at += size
+    rounds = -(-shared // 148) if shared >= 148 else shared / 148
+    return -(-alone // 148) * factor * steps >= rounds * steps + JOIN_STEPS + sum(q_lens) * per * kv_heads / 4096
+
+
 class PrefixGroups:
     """``sizes``: how many neighbouring sequences of the step form each group, in the step's order (one: a sequence alone).
     ``lengths``: the first positions that a group's sequences share, whole pages, 0 for none.

@@ -345,6 +345,10 @@ class SequenceCache:
     def free_pages(self) -> int:
         return min((len(g.ledger.pool) for g in self._kv_groups), default=0)
 
+    def row_bytes(self) -> int:
+        """Bytes of one position's keys and values in one layer (the largest)."""
+        return max((g.need.kv_heads * (g.need.head_dim + (g.need.v_dim or g.need.head_dim)) * g.k.element_size() for g in self._kv_groups), default=0)
+
     def bytes(self) -> int:
         return sum(g.bytes() for g in self._kv_groups) + sum(
             g.state.numel() * g.state.element_size() for g in self._state_groups)

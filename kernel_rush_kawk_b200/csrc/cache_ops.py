@@ -13,6 +13,7 @@ from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import torch
 
+from ..cache.prefix import longer_steps_share, single_tokens_share
 from .build import build_library
 
 F32, BF16 = 0, 1
@@ -145,7 +146,8 @@ class CacheOps:
     def shared_prefix_attention(self, qkv, heads, kv_in_row, head_dim, batch, cache, scale, prefix):
         """``attention`` for a step whose sequences share prefixes: [rows, heads * head_dim], every row over all keys up to its own
         position. ``prefix`` (cache.prefix.PrefixGroups) says which neighbouring sequences of the step hold the same first positions in the
-        same pages (``SequenceCache.fork`` makes such sequences); a group's keys and values are read once for all of its rows. The step's
+        same pages (``SequenceCache.fork`` makes such sequences); a group's keys and values are read once for all of its rows where that pays
+        (cache.prefix says when; elsewhere each sequence reads its own table's). The step's
         own keys and values must be in the cache already, and its rows lie behind their group's prefix. Any number of tokens a
         sequence, float32 or bfloat16; a captured step stays valid while the groups' number and sizes last, whatever the lengths become."""
         self._check_step("shared prefix attention", qkv, heads, kv_in_row, head_dim, batch, cache)
@@ -155,10 +157,15 @@ class CacheOps:
         if rows == 0:
             return out
         scale, stream, error = float(scale), self._stream(), self.error.data_ptr()
+        by_mma = self._by_mma(qkv, cache, D)
+        if by_mma and not (single_tokens_share(prefix.sizes, prefix.lengths, 4 * kv * D) if batch.is_decode else
+                           longer_steps_share(prefix.sizes, prefix.lengths, batch.q_lens, per, kv)):
+            self._whole_attention(out, None, qkv, heads, D, batch, cache, scale)  # each sequence by itself, through its own page table
+            return out
         step = (qkv.data_ptr(), qkv.stride(0), heads, kv, *self._segments(batch, cache, prefix), cache.k.data_ptr(), cache.v.data_ptr())
         group_rows = prefix.max_rows(batch) if prefix.max_length else 0
         tiles = -(-group_rows * per // 16) * kv
-        by_mma = self._by_mma(qkv, cache, D) and tiles <= 65535
+        by_mma = by_mma and tiles <= 65535
         # the prefixes' parts, then the own keys, which join them
         own_splits, tensor = 0, 0
         if not by_mma:
@@ -191,6 +198,26 @@ class CacheOps:
                 self._ok(lib.krk_prefix_few_rows(o, ml, rows, 0, splits, *step, cache.k.shape[0], group_rows, scale, error, stream), "prefix attention")
             self._ok(lib.krk_own_rows(out.data_ptr(), None, o, ml, rows, parts, *step, batch.max_q_len, scale, stream), "attention over own keys")
         return out
+
+    def _whole_attention(self, out, lse, qkv, heads, D, batch, cache, scale):
+        """Every row over all of its sequence's keys, for what ``_by_mma`` takes; ``lse`` (float32 [rows, heads] or None) takes the base-two
+        logarithm of each row's sum. Unlike ``attention``, whatever lies in pages and rows that no query sees."""
+        kv, rows, per = cache.kv_heads, qkv.shape[0], heads // cache.kv_heads
+        lib, error, stream = self._parts_lib(D), self.error.data_ptr(), self._stream()
+        q = (qkv.data_ptr(), qkv.stride(0), heads, kv)
+        pages = (cache.k.data_ptr(), cache.v.data_ptr())
+        if batch.is_decode and lse is None:
+            self._ok(lib.krk_shared_single(out.data_ptr(), None, None, 0, self._cluster_splits(-(-per // 16) * kv * batch.n_seqs, True), 0, *q,
+                                           *self._segments(batch, cache, None), *pages, cache.k.shape[0], 0, scale, error, stream), "single-token attention")
+        elif self._by_tcgen05(qkv, D) and batch.max_q_len * per >= 128 and self.use_tcgen05_attention:
+            if lse is None:
+                lse = torch.empty(rows * heads, dtype=torch.float32, device=qkv.device)
+            self._ok(self._attn_lib(D).krk_attention_prefill_lse(
+                out.data_ptr(), lse.data_ptr(), *q, batch.seq_slot.data_ptr(), batch.seq_start.data_ptr(), batch.seq_qlen.data_ptr(), batch.cu_q.data_ptr(),
+                cache.table.data_ptr(), cache.width, *pages, cache.k.shape[0], batch.n_seqs, batch.max_q_len, rows, scale, error, stream), "prompt attention")
+        else:
+            self._ok(lib.krk_own_rows(out.data_ptr(), _ptr(lse), None, None, rows, 0, *q, *self._segments(batch, cache, None), *pages, batch.max_q_len,
+                                      scale, stream), "prompt attention")
 
     # -- weights per key -------------------------------------------------------------------
     @staticmethod
@@ -230,14 +257,8 @@ class CacheOps:
             return out
         # the output with every row's log sum, then the weights by these
         lse = torch.empty(rows * heads, dtype=torch.float32, device=qkv.device)
-        by_tcgen05 = by_mma and self._by_tcgen05(qkv, D)
-        if by_tcgen05 and batch.max_q_len * per >= 128 and self.use_tcgen05_attention:
-            self._ok(self._attn_lib(D).krk_attention_prefill_lse(
-                out.data_ptr(), lse.data_ptr(), *q, batch.seq_slot.data_ptr(), batch.seq_start.data_ptr(), batch.seq_qlen.data_ptr(), batch.cu_q.data_ptr(),
-                cache.table.data_ptr(), cache.width, *pages, cache.k.shape[0], batch.n_seqs, batch.max_q_len, rows, scale, error, stream), "scored attention")
-        elif by_mma:
-            self._ok(lib.krk_own_rows(out.data_ptr(), lse.data_ptr(), None, None, rows, 0, *q, *segments, *pages, batch.max_q_len, scale, stream),
-                     "scored attention")
+        if by_mma:
+            self._whole_attention(out, lse, qkv, heads, D, batch, cache, scale)
         else:
             parts = self._splits(-(-batch.max_q_len * per // 16) * kv * batch.n_seqs, 444)
             scratch = torch.empty(parts * rows * heads * (D + 2), dtype=torch.float32, device=qkv.device)
@@ -246,7 +267,7 @@ class CacheOps:
             self._ok(lib.krk_partial_attention(o, ml, rows, 0, parts, *q, *segments, *pages, 0, batch.max_q_len, scale, _code(qkv.dtype), stream),
                      "scored attention")
             self._ok(lib.krk_join_parts(out.data_ptr(), lse.data_ptr(), o, ml, rows, heads, parts, _code(qkv.dtype), stream), "join of parts")
-        if by_tcgen05 and not batch.is_decode and per <= 64:
+        if by_mma and self._by_tcgen05(qkv, D) and not batch.is_decode and per <= 64:
             self._ok(lib.krk_key_weights_tcgen05(*counts, lse.data_ptr(), int(observe or 0), *q, *segments, pages[0], cache.k.shape[0], rows,
                                                  min(batch.max_q_len, observe or batch.max_q_len), batch.max_kv_len, scale, error, stream),
                      "weights of keys")

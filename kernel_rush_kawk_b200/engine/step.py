@@ -28,7 +28,7 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
-from ..cache.prefix import PrefixGroups
+from ..cache.prefix import PrefixGroups, single_tokens_share
 from ..cache.store import SequenceCache
 
 
@@ -323,18 +323,15 @@ class Stepper:
         """How much further each sequence's rows lie in it than in the cache, where keys are evicted."""
         return [self.cache.evicted[s] for s in slots] if self.cache.eviction is not None else None
 
-    #: keys that the steps of neighbours in shared pages do not read again, all kv heads together, from which on reading them once pays
-    SHARED_MIN = 1
-
-    def _prefix(self, slots):
-        """The groups of neighbours that share pages, or None where none do or too little. Float32 steps read shared pages row by row like
-        others: a row's logits are the same to the bit however steps are cut and batched."""
+    def _prefix(self, slots, single: bool = True):
+        """The groups of neighbours that share pages, or None where none do or where reading them once does not pay. Float32 steps read
+        shared pages row by row like others: a row's logits are the same to the bit however steps are cut and batched."""
         cache = self.cache
         if not cache.has_forks or cache.dtype != torch.bfloat16:
             return None
         sizes, lengths = cache.shared_groups(slots)
-        if sum((size - 1) * length for size, length in zip(sizes, lengths)) < self.SHARED_MIN:
-            return None
+        if max(lengths) == 0 or (single and not single_tokens_share(sizes, lengths, cache.row_bytes())):
+            return None  # (of longer steps the attention itself sees the row tiles that it has)
         return sizes, lengths
 
     def _pass(self, entries, chosen):
@@ -363,7 +360,7 @@ class Stepper:
         else:
             meta = self._meta(n_rows, n_seqs, len(want_rows))
             meta.fill(slots, starts, token_lists, want_rows, self._shifts(slots))
-            groups = self._prefix(slots)
+            groups = self._prefix(slots, decode)
             meta.prefix = None if groups is None else PrefixGroups(*groups, self.device)
             self.h2d_bytes += meta.bytes
             ctx = StepContext(self.ops, meta, cache)

@@ -22,6 +22,15 @@ def ops():
     return load_kernels(())
 
 
+@pytest.fixture(autouse=True)
+def always_shared(monkeypatch):
+    """Small cases take the kernels that large ones do."""
+    from kernel_rush_kawk_b200.cache import prefix
+
+    monkeypatch.setattr(prefix, "SHARE_BYTES", 0)
+    monkeypatch.setattr(prefix, "JOIN_STEPS", -1e9)
+
+
 def groups(sizes, lengths):
     from kernel_rush_kawk_b200.cache.prefix import PrefixGroups
 
@@ -151,6 +160,18 @@ def test_shared_prefix_attention_beside_keys_that_are_no_numbers(ops, dtype, dim
     first = brings[0] + 33
     assert torch.equal(got[:first], want[:first]), "rows that do not see it"
     assert not torch.isfinite(got[first:, heads * dim // 2 + 3]).any(), "rows that do"
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", [(5, 1, 48), (16, 4, 64), (32, 8, 128), (40, 2, 128)])
+@pytest.mark.parametrize("case", range(len(GROUPS)))
+def test_each_sequence_by_itself(ops, dtype, shape, case, monkeypatch):
+    """Groups that do not pay: the same definition through each sequence's own table."""
+    from kernel_rush_kawk_b200.cache import prefix
+
+    monkeypatch.setattr(prefix, "SHARE_BYTES", 1 << 60)
+    monkeypatch.setattr(prefix, "JOIN_STEPS", 1e9)
+    test_shared_prefix_attention(ops, dtype, shape, case)
 
 
 # -- weights per key -----------------------------------------------------------------------------------------

@@ -14,6 +14,15 @@ from kernel_rush_kawk_b200.engine.generate import shared_prefixes
 from kernel_rush_kawk_b200.parts.base import KVNeed, StateNeed
 
 
+@pytest.fixture(autouse=True)
+def always_shared(monkeypatch):
+    """Tiny models take the paths that large ones do."""
+    from kernel_rush_kawk_b200.cache import prefix
+
+    monkeypatch.setattr(prefix, "SHARE_BYTES", 0)
+    monkeypatch.setattr(prefix, "JOIN_STEPS", -1e9)
+
+
 def cpu_engine(folders, name, dtype="float32", **kw):
     from kernel_rush_kawk_b200 import Engine
 
@@ -324,3 +333,17 @@ def test_the_command_line_takes_the_options():
     for bad in ("--keep-recent 5", "--keep-keys 64 --share-prefix"):
         with pytest.raises(SystemExit):
             main(f"generate --random tiny_a --prompt-ids 1 {bad}".split())
+
+
+def test_the_lines_between_shared_and_alone(monkeypatch):
+    """Both sides of the measured lines, at sizes that were measured."""
+    from kernel_rush_kawk_b200.cache import prefix
+
+    monkeypatch.undo()
+    single = lambda n, p, row=4096: prefix.single_tokens_share([n], [p], row)
+    assert [single(2, 2048), single(2, 8192), single(8, 1024), single(8, 4096), single(64, 64), single(64, 8192)] == [False, True, False, True, False, True]
+    assert not single(1, 1 << 20) and not prefix.single_tokens_share([1, 1], [0, 0], 4096)
+    longer = lambda n, t, p, per=4, kv=8: prefix.longer_steps_share([n], [p], [t] * n, per, kv)
+    assert [longer(2, 4, 4096), longer(4, 60, 4096), longer(2, 250, 4096)] == [True] * 3
+    assert [longer(16, 60, 4096), longer(4, 250, 4096), longer(32, 60, 4096), longer(16, 16, 256)] == [False] * 4
+    assert prefix.longer_steps_share([16], [4096], [90 - 90 * i // 32 for i in range(16)], 4, 8)

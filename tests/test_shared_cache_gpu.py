@@ -12,6 +12,15 @@ pytestmark = pytest.mark.gpu
 NAMES = ["tiny_a", "tiny_b"]
 
 
+@pytest.fixture(autouse=True)
+def always_shared(monkeypatch):
+    """Tiny models take the paths that large ones do."""
+    from kernel_rush_kawk_b200.cache import prefix
+
+    monkeypatch.setattr(prefix, "SHARE_BYTES", 0)
+    monkeypatch.setattr(prefix, "JOIN_STEPS", -1e9)
+
+
 def engine_of(folders, name, **kw):
     from kernel_rush_kawk_b200 import Engine
 
