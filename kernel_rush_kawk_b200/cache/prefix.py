@@ -71,7 +71,7 @@ class PrefixGroups:
                 raise CacheError(f"sequences share whole pages of {PAGE} positions, got {length}")
         self.sizes, self.lengths = tuple(sizes), tuple(lengths)
         self.n_groups, self.n_seqs = len(sizes), sum(sizes)
-        self.max_seqs, self.max_length = max(sizes), max(lengths)
+        self.max_length = max(lengths)
         cu = [0]
         for size in sizes:
             cu.append(cu[-1] + size)
@@ -82,8 +82,9 @@ class PrefixGroups:
 
     @staticmethod
     def shape_of(sizes, lengths) -> tuple:
-        """What a captured step of such groups depends on, beside their number of sequences."""
-        return (len(sizes), max(sizes), max(lengths) > 0)
+        """What a captured step of such groups depends on, beside their number of sequences: how many there are, the power of two
+        that none has more sequences than, and whether any shares."""
+        return (len(sizes), 1 << (max(sizes) - 1).bit_length(), max(lengths) > 0)
 
     @property
     def shape(self) -> tuple:
@@ -97,9 +98,9 @@ class PrefixGroups:
         self.sizes, self.lengths, self.max_length = other.sizes, other.lengths, other.max_length
 
     def max_rows(self, batch) -> int:
-        """The most rows of a step that one group has."""
+        """No fewer rows of a step than one group has; of single tokens the same number as long as a captured step lasts."""
         if batch.max_q_len == 1:
-            return self.max_seqs
+            return self.shape[1]
         at, most = 0, 0
         for size in self.sizes:
             most = max(most, sum(batch.q_lens[at:at + size]))

@@ -116,10 +116,11 @@ class SequenceCache:
     max_tokens: positions all live sequences may hold together, each sequence's
     count rounded up to whole pages. max_slots: live sequences. max_context: the
     longest sequence. step_tokens: the most tokens one sequence brings in one step;
-    it sizes the rings of window groups. eviction: count the weight that keys receive, for ``evict``."""
+    it sizes the rings of window groups. eviction: count the weight that keys receive, for ``evict``; a slot then has room for
+    what it may hold when a pass of ``pass_tokens`` new tokens has come (None: for the longest sequence)."""
 
     def __init__(self, needs: list, max_tokens: int, max_slots: int, max_context: int, device, dtype,
-                 step_tokens: int = 2048, eviction: KeyEviction | None = None):
+                 step_tokens: int = 2048, eviction: KeyEviction | None = None, pass_tokens: int | None = None):
         self.eviction = eviction
         self.device = torch.device(device)
         self.dtype = dtype
@@ -127,7 +128,10 @@ class SequenceCache:
         self.max_context = int(max_context)
         self.step_tokens = int(step_tokens)
         self.n_pages = max(1, -(-int(max_tokens) // PAGE))
-        self.width = max(1, -(-self.max_context // PAGE))
+        rows = self.max_context
+        if eviction is not None and pass_tokens is not None:
+            rows = min(rows, eviction.keep + eviction.every - 1 + int(pass_tokens))
+        self.width = max(1, -(-rows // PAGE))
         self.slots = FreeList(self.max_slots, "cache slot")
         self.length = [0] * self.max_slots  # rows held
         self.evicted = [0] * self.max_slots  # rows given up: the next row's position is length + evicted

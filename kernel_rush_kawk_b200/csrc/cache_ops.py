@@ -51,8 +51,8 @@ def _ptr(t) -> int | None:
 
 _SEGMENTS = [_P] * 7 + [c_int, c_int, _P, c_int]
 _PARTS_SIGNATURES = {
-    "krk_partial_attention": [_P, _P, c_int, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_int, c_float, c_int, _P],
-    "krk_join_parts": [_P, _P, _P, _P, c_int, c_int, c_int, c_int, _P],
+    "krk_attention_in_parts": [_P, _P, _P, _P, c_int, c_int, c_int, _P, _P, _P, _P, c_int, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int,
+                               c_int, c_float, c_int, _P],
     "krk_key_weights": [_P, _P, _P, _P, c_int, _P, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, c_int, c_float, c_int, _P],
 }
 _PARTS_SIGNATURES.update({
@@ -102,10 +102,20 @@ class CacheOps:
             raise KernelError(f"{what}: the cache keeps a window of keys; every key is asked for")
         if cache.k.dtype != qkv.dtype or cache.v.dtype != qkv.dtype or not cache.k.is_contiguous() or not cache.v.is_contiguous():
             raise KernelError(f"{what}: the cache's pages are contiguous and of the rows' dtype ({qkv.dtype}), got {cache.k.dtype}")
-        if qkv.shape[0] != batch.n_rows:
-            raise KernelError(f"{what}: {qkv.shape[0]} rows for a step of {batch.n_rows}")
-        if not qkv.device == cache.k.device == self.error.device:
-            raise KernelError(f"{what}: rows on {qkv.device}, pages on {cache.k.device}, kernels on {self.error.device}")
+        if qkv.shape[0] != batch.n_rows or batch.max_kv_len > cache.width * PAGE:
+            raise KernelError(f"{what}: {qkv.shape[0]} rows for a step of {batch.n_rows} with up to {batch.max_kv_len} keys, in slots of {cache.width * PAGE}")
+        if qkv.shape[0] > 1 and qkv.stride(0) < qkv.shape[1]:
+            raise KernelError(f"{what}: rows that overlap (a stride of {qkv.stride(0)})")
+        self._check_device(what, qkv.device, cache.k.device)
+
+    def _check_device(self, what, *devices):
+        mine = self.error.device
+        if any(d != mine for d in devices) or torch.cuda.current_device() != mine.index:
+            raise KernelError(f"{what}: tensors on {', '.join(map(str, devices))}, device {torch.cuda.current_device()} current, kernels on {mine}")
+
+    @staticmethod
+    def _row_stride(qkv) -> int:
+        return qkv.stride(0) if qkv.shape[0] > 1 else qkv.shape[1]  # a single row has none that means anything
 
     @staticmethod
     def _segments(batch, cache, prefix):
@@ -130,17 +140,17 @@ class CacheOps:
             return 8 if items <= 64 else 4 if items <= 148 else 2 if items <= 592 else 1
         return 4 if items <= 37 else 2 if items <= 148 else 1
 
-    @staticmethod
-    def _by_mma(qkv, cache, head_dim) -> bool:
+    @classmethod
+    def _by_mma(cls, qkv, cache, head_dim) -> bool:
         """Whether the tensor-core kernels take these rows and pages: bfloat16, head sizes in steps of 16, rows from 4-byte, pages from 16-byte
         boundaries on."""
-        return (qkv.dtype == torch.bfloat16 and head_dim % 16 == 0 and qkv.stride(0) % 2 == 0 and qkv.data_ptr() % 4 == 0
+        return (qkv.dtype == torch.bfloat16 and head_dim % 16 == 0 and cls._row_stride(qkv) % 2 == 0 and qkv.data_ptr() % 4 == 0
                 and (cache.k.data_ptr() | cache.v.data_ptr()) % 16 == 0)
 
-    @staticmethod
-    def _by_tcgen05(qkv, head_dim) -> bool:
+    @classmethod
+    def _by_tcgen05(cls, qkv, head_dim) -> bool:
         """Whether the tcgen05 kernels take rows that ``_by_mma`` takes: heads of 64 or 128, rows from 16-byte boundaries on."""
-        return head_dim in (64, 128) and qkv.stride(0) % 8 == 0 and qkv.data_ptr() % 16 == 0
+        return head_dim in (64, 128) and cls._row_stride(qkv) % 8 == 0 and qkv.data_ptr() % 16 == 0
 
     # -- a shared prefix -----------------------------------------------------------------
     def shared_prefix_attention(self, qkv, heads, kv_in_row, head_dim, batch, cache, scale, prefix):
@@ -162,7 +172,7 @@ class CacheOps:
                            longer_steps_share(prefix.sizes, prefix.lengths, batch.q_lens, per, kv)):
             self._whole_attention(out, None, qkv, heads, D, batch, cache, scale)  # each sequence by itself, through its own page table
             return out
-        step = (qkv.data_ptr(), qkv.stride(0), heads, kv, *self._segments(batch, cache, prefix), cache.k.data_ptr(), cache.v.data_ptr())
+        step = (qkv.data_ptr(), self._row_stride(qkv), heads, kv, *self._segments(batch, cache, prefix), cache.k.data_ptr(), cache.v.data_ptr())
         group_rows = prefix.max_rows(batch) if prefix.max_length else 0
         tiles = -(-group_rows * per // 16) * kv
         by_mma = by_mma and tiles <= 65535
@@ -183,9 +193,9 @@ class CacheOps:
         o = scratch.data_ptr()
         ml = o + 4 * parts * rows * heads * D
         if not by_mma:
-            code = _code(qkv.dtype)
-            self._ok(lib.krk_partial_attention(o, ml, rows, splits, own_splits, *step, group_rows, batch.max_q_len, scale, code, stream), "attention in parts")
-            self._ok(lib.krk_join_parts(out.data_ptr(), None, o, ml, rows, heads, parts, code, stream), "join of parts")
+            self.launches += 1
+            self._ok(lib.krk_attention_in_parts(out.data_ptr(), None, o, ml, rows, splits, own_splits, None, None, None, None, 0, 0, 1, *step, group_rows,
+                                                batch.max_q_len, scale, _code(qkv.dtype), stream), "shared prefix attention")
         elif batch.is_decode:
             self.launches += splits > 0
             self._ok(lib.krk_shared_single(out.data_ptr(), o, ml, splits, self._cluster_splits(-(-per // 16) * kv * batch.n_seqs, False), tensor, *step,
@@ -204,7 +214,7 @@ class CacheOps:
         logarithm of each row's sum. Unlike ``attention``, whatever lies in pages and rows that no query sees."""
         kv, rows, per = cache.kv_heads, qkv.shape[0], heads // cache.kv_heads
         lib, error, stream = self._parts_lib(D), self.error.data_ptr(), self._stream()
-        q = (qkv.data_ptr(), qkv.stride(0), heads, kv)
+        q = (qkv.data_ptr(), self._row_stride(qkv), heads, kv)
         pages = (cache.k.data_ptr(), cache.v.data_ptr())
         if batch.is_decode and lse is None:
             self._ok(lib.krk_shared_single(out.data_ptr(), None, None, 0, self._cluster_splits(-(-per // 16) * kv * batch.n_seqs, True), 0, *q,
@@ -247,7 +257,7 @@ class CacheOps:
         scale, stream, error, capacity = float(scale), self._stream(), self.error.data_ptr(), scores.shape[2]
         counts = (scores.data_ptr(), out_scores.data_ptr(), _ptr(positions), _ptr(getattr(batch, "seq_shift", None)), capacity)
         segments = self._segments(batch, cache, None)
-        q = (qkv.data_ptr(), qkv.stride(0), heads, kv)
+        q = (qkv.data_ptr(), self._row_stride(qkv), heads, kv)
         pages = (cache.k.data_ptr(), cache.v.data_ptr())
         by_mma = self._by_mma(qkv, cache, D)
         if by_mma and batch.is_decode and per <= 16:
@@ -257,23 +267,22 @@ class CacheOps:
             return out
         # the output with every row's log sum, then the weights by these
         lse = torch.empty(rows * heads, dtype=torch.float32, device=qkv.device)
-        if by_mma:
-            self._whole_attention(out, lse, qkv, heads, D, batch, cache, scale)
-        else:
+        page_blocks = max(1, min(cache.width, -(-888 // (kv * batch.n_seqs))))
+        if not by_mma:
             parts = self._splits(-(-batch.max_q_len * per // 16) * kv * batch.n_seqs, 444)
             scratch = torch.empty(parts * rows * heads * (D + 2), dtype=torch.float32, device=qkv.device)
             o = scratch.data_ptr()
-            ml = o + 4 * parts * rows * heads * D
-            self._ok(lib.krk_partial_attention(o, ml, rows, 0, parts, *q, *segments, *pages, 0, batch.max_q_len, scale, _code(qkv.dtype), stream),
-                     "scored attention")
-            self._ok(lib.krk_join_parts(out.data_ptr(), lse.data_ptr(), o, ml, rows, heads, parts, _code(qkv.dtype), stream), "join of parts")
-        if by_mma and self._by_tcgen05(qkv, D) and not batch.is_decode and per <= 64:
+            self.launches += 2
+            self._ok(lib.krk_attention_in_parts(out.data_ptr(), lse.data_ptr(), o, o + 4 * parts * rows * heads * D, rows, 0, parts, *counts, int(observe or 0),
+                                                page_blocks, *q, *segments, *pages, 0, batch.max_q_len, scale, _code(qkv.dtype), stream), "scored attention")
+            return out
+        self._whole_attention(out, lse, qkv, heads, D, batch, cache, scale)
+        if self._by_tcgen05(qkv, D) and not batch.is_decode and per <= 64:
             self._ok(lib.krk_key_weights_tcgen05(*counts, lse.data_ptr(), int(observe or 0), *q, *segments, pages[0], cache.k.shape[0], rows,
                                                  min(batch.max_q_len, observe or batch.max_q_len), batch.max_kv_len, scale, error, stream),
                      "weights of keys")
         else:
-            blocks = max(1, min(cache.width, -(-888 // (kv * batch.n_seqs))))
-            self._ok(lib.krk_key_weights(*counts, lse.data_ptr(), int(observe or 0), *q, *segments, pages[0], blocks, scale, _code(qkv.dtype), stream),
+            self._ok(lib.krk_key_weights(*counts, lse.data_ptr(), int(observe or 0), *q, *segments, pages[0], page_blocks, scale, _code(qkv.dtype), stream),
                      "weights of keys")
         return out
 
@@ -306,8 +315,7 @@ class CacheOps:
             if t.shape != counts or t.dtype != dtype or not t.is_contiguous() or t.device != error.device:
                 raise KernelError(f"{what}: {name} are contiguous {dtype} [runs, slots, kv heads, rows of a slot] = {list(counts)} on {error.device}, "
                                   f"got {t.dtype} {list(t.shape)} on {t.device}")
-        if k.device != error.device or v.device != error.device or table.device != error.device:
-            raise KernelError(f"{what}: every tensor lies on the kernels' device, {error.device}")
+        self._check_device(what, k.device, v.device, table.device)
         if keep < 1 or not 0 <= recent <= keep:
             raise KernelError(f"{what}: at least one row stays, and at most as many by their position as stay in all; got keep {keep}, recent {recent}")
         n = len(slots)

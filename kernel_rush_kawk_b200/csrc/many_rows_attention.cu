@@ -25,17 +25,17 @@ namespace {
 
 #include "attention_tiles.cuh"
 
-constexpr int P_PITCH = KRK_PAGE + 2;  // floats between rows of weights in shared memory
-constexpr size_t WEIGHTS_BYTES = (size_t)64 * P_PITCH * sizeof(float);
+// The weights of a page with values that are no numbers, [64 rows][64 keys], lie where its keys were, or behind the pages where keys are too small.
+constexpr bool WEIGHTS_IN_KEYS = TILE_ELEMS >= 64 * KRK_PAGE;
+constexpr size_t WEIGHTS_BYTES = WEIGHTS_IN_KEYS ? 0 : (size_t)64 * KRK_PAGE * sizeof(bf16);
 
 __device__ __forceinline__ bool not_finite(uint32_t two) { return (two & 0x7f80u) == 0x7f80u || (two & 0x7f800000u) == 0x7f800000u; }
 
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, D <= 128 ? 3 : 1)
 many_rows_kernel(bf16* __restrict__ out, float* __restrict__ lse, Parts parts, int n_join, const bf16* __restrict__ q, int q_stride, int HQ, int HKV,
                  Segments seg, const bf16* __restrict__ k_cache, const bf16* __restrict__ v_cache, float scale_log2, bool wait_first) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   bf16* smem = reinterpret_cast<bf16*>(smem_raw);                          // [2 stages][K, V][64][pitch]
-  float* weights = reinterpret_cast<float*>(smem_raw + PAGE_SMEM);  // [64][P_PITCH], for pages with values that are no numbers
   if (wait_first) grid_dependency_wait();
   grid_launch_dependents();
   const int kh = blockIdx.y, G = HQ / HKV;
@@ -64,7 +64,7 @@ many_rows_kernel(bf16* __restrict__ out, float* __restrict__ lse, Parts parts, i
   const int tile_min_pos = u.start + tile * 64 / G;  // the least position of the tile's rows
 
   const int last_tok = min(u.n_tok - 1, (tile * 64 + 63) / G);
-  const int j_lo = u.key_lo / KRK_PAGE, j_hi = (u.start + last_tok) / KRK_PAGE;
+  const int j_lo = u.key_lo / KRK_PAGE, j_hi = min(u.start + last_tok, u.key_hi - 1) / KRK_PAGE;
   const size_t page_stride = (size_t)HKV * KRK_PAGE * D, head_off = (size_t)kh * KRK_PAGE * D;
   auto issue = [&](int j, int stage) {
     const int page = seg.table[(size_t)u.slot * seg.width + j];
@@ -81,7 +81,7 @@ many_rows_kernel(bf16* __restrict__ out, float* __restrict__ lse, Parts parts, i
 #pragma unroll
     for (int c = 0; c < 4; ++c) o[n][c] = 0.f;
 
-  issue(j_lo, 0);
+  if (j_lo <= j_hi) issue(j_lo, 0);
   for (int j = j_lo; j <= j_hi; ++j) {
     const int stage = (j - j_lo) & 1, key_base = j * KRK_PAGE;
     if (j + 1 <= j_hi) {
@@ -122,20 +122,19 @@ many_rows_kernel(bf16* __restrict__ out, float* __restrict__ lse, Parts parts, i
     if (!one_by_one) {
       pv_tile<8>(o, s, vs, 0, lane);
     } else {
+      bf16* weights = WEIGHTS_IN_KEYS ? ks : reinterpret_cast<bf16*>(smem_raw + PAGE_SMEM);
+      __syncthreads();  // every warp has its scores
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          float* to = weights + (warp * 16 + g + 8 * h) * P_PITCH + n * 8 + 2 * t4;
-          to[0] = round_to<bf16>(s[n][2 * h]);
-          to[1] = round_to<bf16>(s[n][2 * h + 1]);
-        }
+        for (int n = 0; n < 8; ++n)
+          *reinterpret_cast<uint32_t*>(weights + (warp * 16 + g + 8 * h) * KRK_PAGE + n * 8 + 2 * t4) = pack_bf16x2(s[n][2 * h], s[n][2 * h + 1]);
       __syncwarp();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float* row = weights + (warp * 16 + g + 8 * h) * P_PITCH;
+        const bf16* row = weights + (warp * 16 + g + 8 * h) * KRK_PAGE;
         for (int key = 0; key < KRK_PAGE && key_base + key <= pos[h]; ++key) {
-          const float p = row[key];
+          const float p = __bfloat162float(row[key]);
 #pragma unroll
           for (int n = 0; n < DTILES; ++n) {
             const bf16* v = vs + kv_off(key, n) + 2 * t4;

@@ -343,7 +343,7 @@ int launch_partial(const Parts& parts, int n_prefix, int n_own, const void* q, i
 
 // Parts 0 .. n_prefix - 1 of the groups' prefixes (none: 0) and the next n_own of the sequences' other keys. group_rows, own_rows: the most rows of the
 // step that a group and a sequence have.
-KRK_API int krk_partial_attention(float* o, float* ml, int rows, int n_prefix, int n_own, const void* q, int q_stride, int HQ, int HKV, KRK_SEGMENTS,
+static int krk_partial_attention(float* o, float* ml, int rows, int n_prefix, int n_own, const void* q, int q_stride, int HQ, int HKV, KRK_SEGMENTS,
                                   const void* k_cache, const void* v_cache, int group_rows, int own_rows, float scale, int dtype, cudaStream_t stream) {
   const Parts parts = {o, (float2*)ml, rows, HQ};
   const Segments seg = KRK_MAKE_SEGMENTS;
@@ -352,7 +352,7 @@ KRK_API int krk_partial_attention(float* o, float* ml, int rows, int n_prefix, i
                                 : launch_partial<bf16>(parts, n_prefix, n_own, q, q_stride, HQ, HKV, seg, k_cache, v_cache, group_rows, own_rows, scale, stream);
 }
 
-KRK_API int krk_join_parts(void* out, float* lse, const float* o, const float* ml, int rows, int HQ, int n_parts, int dtype, cudaStream_t stream) {
+static int krk_join_parts(void* out, float* lse, const float* o, const float* ml, int rows, int HQ, int n_parts, int dtype, cudaStream_t stream) {
   const Parts parts = {const_cast<float*>(o), (float2*)const_cast<float*>(ml), rows, HQ};
   const long long blocks = ((long long)rows * HQ + THREADS / 32 - 1) / (THREADS / 32);
   if (blocks == 0) return 0;
@@ -379,4 +379,19 @@ KRK_API int krk_key_weights(const float* sums, float* sums_out, int* positions, 
   };
   if (dtype == KRK_DTYPE_F32) return go(key_weights_kernel<float>, (const float*)q, (const float*)k_cache);
   return go(key_weights_kernel<bf16>, (const bf16*)q, (const bf16*)k_cache);
+}
+
+// Attention in parts and their join (out; lse may be null) and, where sums_out is given, the weights of the keys, with lse as their logarithms: krk_partial_attention,
+// krk_join_parts and krk_key_weights in one call. o, ml: scratch for n_prefix + n_own parts.
+KRK_API int krk_attention_in_parts(void* out, float* lse, float* o, float* ml, int rows, int n_prefix, int n_own, const float* sums, float* sums_out,
+                                   int* positions, const int* seq_shift, int capacity, int observe, int page_blocks, const void* q, int q_stride, int HQ,
+                                   int HKV, KRK_SEGMENTS, const void* k_cache, const void* v_cache, int group_rows, int own_rows, float scale, int dtype,
+                                   cudaStream_t stream) {
+  int rc = krk_partial_attention(o, ml, rows, n_prefix, n_own, q, q_stride, HQ, HKV, cu_q, seq_slot, seq_start, seq_qlen, group_cu, group_len, seq_group,
+                                 n_seqs, n_groups, table, width, k_cache, v_cache, group_rows, own_rows, scale, dtype, stream);
+  if (rc == 0) rc = krk_join_parts(out, lse, o, ml, rows, HQ, n_prefix + n_own, dtype, stream);
+  if (rc == 0 && sums_out)
+    rc = krk_key_weights(sums, sums_out, positions, seq_shift, capacity, lse, observe, q, q_stride, HQ, HKV, cu_q, seq_slot, seq_start, seq_qlen, group_cu,
+                         group_len, seq_group, n_seqs, n_groups, table, width, k_cache, page_blocks, scale, dtype, stream);
+  return rc;
 }

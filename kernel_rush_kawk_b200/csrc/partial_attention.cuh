@@ -32,7 +32,7 @@ __device__ __forceinline__ Unit prefix_unit(const Segments& s, int group) {
   u.row0 = s.cu_q[first];
   u.n_tok = s.cu_q[last] - u.row0;
   u.key_lo = 0;
-  u.key_hi = s.group_len[group];
+  u.key_hi = min(s.group_len[group], s.width * KRK_PAGE);  // no page beyond a slot's
   u.slot = s.seq_slot[first];
   u.start = 0x3fffffff;  // every key of the prefix lies before every row
   return u;
@@ -44,7 +44,7 @@ __device__ __forceinline__ Unit own_unit(const Segments& s, int seq) {
   u.n_tok = s.seq_qlen[seq];
   u.start = s.seq_start[seq];
   u.key_lo = s.n_groups > 0 ? s.group_len[s.seq_group[seq]] : 0;
-  u.key_hi = u.start + u.n_tok;
+  u.key_hi = min(u.start + u.n_tok, s.width * KRK_PAGE);  // no page beyond a slot's
   u.slot = s.seq_slot[seq];
   return u;
 }

@@ -152,7 +152,7 @@ class Engine:
         if self.device.type == "cuda":
             torch.cuda.empty_cache()
         self.cache = SequenceCache(self.model.cache_needs(), max_tokens, max_slots, self.max_context, self.device,
-                                   self.dtype, step_tokens=self.step_tokens, eviction=self.eviction)
+                                   self.dtype, step_tokens=self.step_tokens, eviction=self.eviction, pass_tokens=self.max_step_rows)
         self.stepper = Stepper(self.model, self.cache, self.ops, self.max_step_rows, self.use_cuda_graphs)
         self.loop = GenerationLoop(self.stepper, self.cache, self.sampler)
 
