@@ -98,9 +98,11 @@ class PrefixGroups:
         self.sizes, self.lengths, self.max_length = other.sizes, other.lengths, other.max_length
 
     def max_rows(self, batch) -> int:
-        """No fewer rows of a step than one group has; of single tokens the same number as long as a captured step lasts."""
+        """No fewer rows of a step than one group has; where it is captured, for as long as ``update`` takes other groups."""
         if batch.max_q_len == 1:
             return self.shape[1]
+        if self.buffer.is_cuda and torch.cuda.is_current_stream_capturing():
+            return min(batch.n_rows, self.shape[1] * batch.max_q_len)
         at, most = 0, 0
         for size in self.sizes:
             most = max(most, sum(batch.q_lens[at:at + size]))

@@ -278,9 +278,9 @@ class CacheOps:
             return out
         self._whole_attention(out, lse, qkv, heads, D, batch, cache, scale)
         if self._by_tcgen05(qkv, D) and not batch.is_decode and per <= 64:
+            longest = cache.width * PAGE if torch.cuda.is_current_stream_capturing() else batch.max_kv_len  # a captured step's sequences grow
             self._ok(lib.krk_key_weights_tcgen05(*counts, lse.data_ptr(), int(observe or 0), *q, *segments, pages[0], cache.k.shape[0], rows,
-                                                 min(batch.max_q_len, observe or batch.max_q_len), batch.max_kv_len, scale, error, stream),
-                     "weights of keys")
+                                                 min(batch.max_q_len, observe or batch.max_q_len), longest, scale, error, stream), "weights of keys")
         else:
             self._ok(lib.krk_key_weights(*counts, lse.data_ptr(), int(observe or 0), *q, *segments, pages[0], page_blocks, scale, _code(qkv.dtype), stream),
                      "weights of keys")

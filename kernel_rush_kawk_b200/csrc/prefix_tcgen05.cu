@@ -372,6 +372,7 @@ KRK_API int krk_prefix_tcgen05(float* o, float* ml, int rows, int part0, int n_s
   CUtensorMap map_q = map_k;
   if (rc == 0 && q_by_tma) rc = make_map_bf16_3d(&map_q, q, D, HQ, rows, D, q_stride, G, tile_rows / G);
   if (rc) return rc;
+  if (scale == 0.f) scale = 1e-30f;  // a key that is not there has no weight by a score of minus infinity: the scale must not be zero
   static unsigned long long allowed = 0;
   cudaError_t e = allow_shared(prefix_tcgen05_kernel, SMEM_BYTES, &allowed);
   if (e != cudaSuccess) return (int)e;

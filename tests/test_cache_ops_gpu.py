@@ -86,6 +86,37 @@ def test_shared_prefix_attention_of_other_scales(ops, dtype, scale, dim):
     within(got, want, off, f"scale {scale}")
 
 
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 2.0])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n_seqs,length", [(10, 320), (40, 192)])
+def test_shared_prefix_attention_of_many_rows_and_other_scales(ops, n_seqs, length, dim, scale):
+    """Rows that fill a tile in part, or two, and an odd number of pages."""
+    qkv, batch, cache = make_step(DEVICE, BF16, 8, 2, dim, [length + i for i in range(n_seqs)], [1] * n_seqs, 5, ([n_seqs], [length]))
+    got = ops.shared_prefix_attention(qkv, 8, 2, dim, batch, cache, scale, groups([n_seqs], [length]))
+    want, off, _, _ = exact_attention(qkv, 8, 2, dim, batch, cache, scale)
+    within(got, want, off, f"scale {scale}")
+
+
+@pytest.mark.parametrize("dtype,dim", [(F32, 48), (BF16, 48), (BF16, 128)])
+def test_shared_prefix_attention_of_captured_pieces(ops, dtype, dim):
+    """A captured step of several tokens a sequence, replayed for a group with more sequences than the step was captured for."""
+    heads, kv, n, each = 8, 2, 5, 9
+    qkv, batch, cache = make_step(DEVICE, dtype, heads, kv, dim, [256 + 3 * i for i in range(n)], [each] * n, 6, ([n], [256]))
+    prefix = groups([3, 2], [128, 64])
+    call = lambda: ops.shared_prefix_attention(qkv, heads, kv, dim, batch, cache, 0.2, prefix)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    want, off, _, _ = exact_attention(qkv, heads, kv, dim, batch, cache, 0.2)
+    for sizes, lengths in (([3, 2], [128, 64]), ([4, 1], [256, 0]), ([1, 4], [64, 192])):
+        prefix.update(groups(sizes, lengths))
+        out.fill_(float("nan"))
+        graph.replay()
+        within(out, want, off, f"replayed for {sizes}")
+
+
 @pytest.mark.parametrize("n_seqs,length,dim", [(64, 2048, 128), (70, 1088, 64), (33, 4032, 128), (5, 16384, 128)])
 def test_shared_prefix_attention_of_many_rows(ops, n_seqs, length, dim):
     """More rows than several tiles, long prefixes, odd numbers of pages: the sizes of a server."""
@@ -259,6 +290,31 @@ def test_scored_attention_in_a_captured_step(ops):
     within(scores, want, allowed, "sums over replays")
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_scored_attention_of_captured_pieces(ops, dtype):
+    """A captured step of several tokens a sequence, replayed for sequences that have grown over pages that the captured one did not see."""
+    heads, kv, dim, each, later = 8, 2, 128, 5, 500
+    held = [40, 0]
+    qkv, batch, cache = make_step(DEVICE, dtype, heads, kv, dim, [h + later for h in held], [each] * 2, 4)
+    batch = make_batch(DEVICE, batch.slots, held, [each] * 2)
+    scores = torch.zeros((cache.table.shape[0], kv, cache.width * PAGE), device=DEVICE)
+    call = lambda: ops.scored_attention(qkv, heads, kv, dim, batch, cache, 0.1, scores)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    batch.starts = [s + later for s in batch.starts]
+    batch.seq_start += later
+    batch.row_pos += later
+    scores.zero_()
+    graph.replay()
+    want, off, weights, weights_off = exact_attention(qkv, heads, kv, dim, batch, cache, 0.1)
+    within(out, want, off, "output")
+    for i, (slot, start) in enumerate(zip(batch.slots, batch.starts)):
+        within(scores[slot, :, :start + each], weights[i], weights_off[i], f"weights of sequence {i}")
+
+
 # -- eviction ---------------------------------------------------------------------------------------------------
 def evict_case(dtype, runs, kv, dim, width, seed, n_slots=5, ties=True):
     g = torch.Generator(DEVICE).manual_seed(seed)
@@ -426,6 +482,9 @@ def test_refusals(ops):
     for error, change in [(KernelError, dict(qkv=qkv[:, :-1])), (KernelError, dict(qkv=qkv.float())), (KernelError, dict(heads=3)),
                           (KernelError, dict(cache=SimpleNamespace(**{**vars(cache), "window": 64}))), (KernelError, dict(qkv=qkv[:1])),
                           (KernelError, dict(qkv=qkv.t().contiguous().t())), (CacheError, dict(prefix=groups([3], [64]))),
+                          (KernelError, dict(qkv=qkv.as_strided(qkv.shape, (qkv.shape[1] - 64, 1)))),
+                          (KernelError, dict(batch=SimpleNamespace(**{**vars(batch), "max_kv_len": cache.width * PAGE + 1}))),
+                          (KernelError, dict(cache=SimpleNamespace(**{**vars(cache), "k": cache.k[:, :1]}))),
                           (CacheError, dict(prefix=groups([2], [128]))), (CacheError, dict(prefix=groups([1, 1], [64, 640])))]:
         with pytest.raises(error):
             shared(**change)
@@ -445,6 +504,16 @@ def test_refusals(ops):
         for a, b in zip(before, (k, v, scores, positions)):
             assert torch.equal(a, b)
     assert ops.evict_keys(k, v, table, [], [], scores, positions, 10, 3) == []
+
+
+@pytest.mark.parametrize("dim", [64, 48])
+def test_a_single_row_has_no_stride(ops, dim):
+    """A step of one row from a view whose stride is odd: the row alone decides which kernel takes it."""
+    qkv, batch, cache = make_step(DEVICE, BF16, 4, 2, dim, [130], [1], 1)
+    odd = torch.empty((2, qkv.shape[1] + 1), dtype=BF16, device=DEVICE)[:1, :-1]
+    odd.copy_(qkv)
+    want = ops.shared_prefix_attention(qkv, 4, 2, dim, batch, cache, 0.1, groups([1], [128]))
+    assert torch.equal(ops.shared_prefix_attention(odd, 4, 2, dim, batch, cache, 0.1, groups([1], [128])), want)
 
 
 def test_steps_without_rows(ops):
