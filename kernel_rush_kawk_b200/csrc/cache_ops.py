@@ -94,24 +94,31 @@ class CacheOps:
 
     # -- what both attentions ask of their arguments ---------------------------------
     def _check_step(self, what, qkv, heads, kv_in_row, head_dim, batch, cache):
-        if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] != (heads + 2 * kv_in_row) * head_dim:
-            raise KernelError(f"{what}: rows of {(heads + 2 * kv_in_row) * head_dim} elements side by side are asked for, got {tuple(qkv.shape)}")
+        shape, dtype, k, v = qkv.shape, qkv.dtype, cache.k, cache.v
+        if len(shape) != 2 or qkv.stride(1) != 1 or shape[1] != (heads + 2 * kv_in_row) * head_dim:
+            raise KernelError(f"{what}: rows of {(heads + 2 * kv_in_row) * head_dim} elements side by side are asked for, got {tuple(shape)}")
         if heads % cache.kv_heads or cache.head_dim != head_dim or cache.v_dim != head_dim:
             raise KernelError(f"{what}: {heads} heads of {head_dim} do not fit a cache of {cache.kv_heads} heads of {cache.head_dim} (values: {cache.v_dim})")
         if cache.window is not None or cache.keep_pages:
             raise KernelError(f"{what}: the cache keeps a window of keys; every key is asked for")
-        if cache.k.dtype != qkv.dtype or cache.v.dtype != qkv.dtype or not cache.k.is_contiguous() or not cache.v.is_contiguous():
-            raise KernelError(f"{what}: the cache's pages are contiguous and of the rows' dtype ({qkv.dtype}), got {cache.k.dtype}")
-        if qkv.shape[0] != batch.n_rows or batch.max_kv_len > cache.width * PAGE:
-            raise KernelError(f"{what}: {qkv.shape[0]} rows for a step of {batch.n_rows} with up to {batch.max_kv_len} keys, in slots of {cache.width * PAGE}")
-        if qkv.shape[0] > 1 and qkv.stride(0) < qkv.shape[1]:
+        if k.dtype != dtype or v.dtype != dtype or not k.is_contiguous() or not v.is_contiguous():
+            raise KernelError(f"{what}: the cache's pages are contiguous and of the rows' dtype ({dtype}), got {k.dtype}")
+        if shape[0] != batch.n_rows or batch.max_kv_len > cache.width * PAGE:
+            raise KernelError(f"{what}: {shape[0]} rows for a step of {batch.n_rows} with up to {batch.max_kv_len} keys, in slots of {cache.width * PAGE}")
+        if shape[0] > 1 and qkv.stride(0) < shape[1]:
             raise KernelError(f"{what}: rows that overlap (a stride of {qkv.stride(0)})")
-        self._check_device(what, qkv.device, cache.k.device)
+        self._check_device(what, qkv, k)
 
-    def _check_device(self, what, *devices):
-        mine = self.error.device
-        if any(d != mine for d in devices) or torch.cuda.current_device() != mine.index:
-            raise KernelError(f"{what}: tensors on {', '.join(map(str, devices))}, device {torch.cuda.current_device()} current, kernels on {mine}")
+    def _check_device(self, what, *tensors):
+        mine = self.error.get_device()
+        for t in tensors:
+            if t.get_device() != mine:
+                break
+        else:
+            if torch.cuda.current_device() == mine:
+                return
+        raise KernelError(f"{what}: tensors on {', '.join(str(t.device) for t in tensors)}, device {torch.cuda.current_device()} current, "
+                          f"kernels on {self.error.device}")
 
     @staticmethod
     def _row_stride(qkv) -> int:
@@ -233,8 +240,9 @@ class CacheOps:
     @staticmethod
     def _check_scores(what, cache, tables):
         shape = (cache.table.shape[0], cache.kv_heads, cache.width * PAGE)
+        device = cache.k.get_device()
         for name, t, dtype in tables:
-            if t is not None and (t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.device != cache.k.device):
+            if t is not None and (t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.get_device() != device):
                 raise KernelError(f"{what}: {name} are contiguous {dtype} [slots, kv heads, rows of a slot] = {list(shape)} beside the cache, "
                                   f"got {t.dtype} {list(t.shape)}")
 
@@ -247,7 +255,7 @@ class CacheOps:
         self._check_step("scored attention", qkv, heads, kv_in_row, head_dim, batch, cache)
         out_scores = scores if out_scores is None else out_scores
         self._check_scores("scored attention", cache, (("scores", scores, torch.float32), ("positions", positions, torch.int32),
-                                                       ("out_scores", out_scores, torch.float32)))
+                                                       ("out_scores", None if out_scores is scores else out_scores, torch.float32)))
         if observe is not None and observe < 1:
             raise KernelError(f"scored attention: at least one query a sequence is observed, got {observe}")
         lib, rows, kv, per, D = self._parts_lib(head_dim), qkv.shape[0], cache.kv_heads, heads // cache.kv_heads, head_dim
@@ -315,7 +323,7 @@ class CacheOps:
             if t.shape != counts or t.dtype != dtype or not t.is_contiguous() or t.device != error.device:
                 raise KernelError(f"{what}: {name} are contiguous {dtype} [runs, slots, kv heads, rows of a slot] = {list(counts)} on {error.device}, "
                                   f"got {t.dtype} {list(t.shape)} on {t.device}")
-        self._check_device(what, k.device, v.device, table.device)
+        self._check_device(what, k, v, table)
         if keep < 1 or not 0 <= recent <= keep:
             raise KernelError(f"{what}: at least one row stays, and at most as many by their position as stay in all; got keep {keep}, recent {recent}")
         n = len(slots)

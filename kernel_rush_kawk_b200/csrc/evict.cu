@@ -8,6 +8,11 @@
 //
 // A block per head finds what stays: a line through the positions and one through the other rows' sums, then the rows in order. It moves the
 // rows as well where there are heads enough; else blocks over all moves of all heads do, in a second launch.
+//
+// What bounds it is the finding: passes of one block over a head's rows in shared memory, with barriers between. The lines by bins of the numbers'
+// range (two passes mostly) instead of a bisection of their bits: 58.8 to 26 us. 16 sequences of 1,088 rows to 1,024, 8 layers of 8 heads
+// of 128 (1,024 heads, 82 MB): 27 us, of which the bytes would take 12.5. One prompt of 16,300 rows to 2,048 (64 heads, 129 MB): 26 us for the lines and
+// 27 for the moves.
 #include "common.cuh"
 
 namespace {

@@ -10,7 +10,10 @@
 //
 // Where a unit has at most eight rows (NARROW: the heads of a kv head mostly are), the products are taken the other way round: the page's
 // keys are the sixteen rows of an instruction and the queries its eight columns, S^T = K Q^T and O^T = V^T P^T, with P^T turned in
-// registers (movmatrix). Sixteen rows of which four are queries cost twice the instructions and registers: @@NARROW@@
+// registers (movmatrix). Sixteen rows of which four are queries cost twice the instructions and registers:
+// 64 sequences' own keys (up to 500 each, 8 kv heads of 128) take 43 us a pass in columns and 59.6 in rows, with 96 registers a thread instead of 158 to
+// 168. 32 sequences of 2,000 to 4,500 keys with their weights, 8 kv heads of 128: 85 us for 434 MB, 5.1 TB/s, beside 1,631 in the kernel for every type; one
+// sequence of 1,087 keys: 10.4 us, the latency of two launches' worth of dependent steps (page table, pages, statistics, join, weights).
 //
 // The splits of a sequence's keys form a cluster: their parts meet in the first block's shared memory, which also reads the prefix
 // parts of its rows and writes the output. That is the only place that waits for the kernel before, so a sequence's own

@@ -4,7 +4,7 @@
 //
 // A block takes 64 (token, head) rows of one kv head, 16 a warp, and walks the pages that the tile sees, two in shared memory (cp.async).
 // The keys behind a shared prefix are few beside it, which is where the time goes (prefix_tcgen05.cu): this kernel's share of
-// sixteen questions of up to 90 tokens behind 4,096 positions is a tenth.
+// sixteen questions of up to 90 tokens behind 4,096 positions is a sixth, 16 of 92 us, most of it the join's reading of the parts (47 MB).
 //
 // Values that a row does not see may be anything, and zero times infinity is not zero: values behind the sequence's end count
 // as zero, and a page that some row sees in part and that holds an infinity or a NaN goes through the multiplications one by one.

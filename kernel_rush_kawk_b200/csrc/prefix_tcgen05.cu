@@ -11,8 +11,13 @@
 // Warps 0..3 run the softmax of tile 0 and warps 4..7 that of tile 1 (thread = row = tensor-memory lane, all 128 keys of a step); warp 8 issues the
 // MMAs, lane 0 of warp 9 the TMA loads. While one tile's rows are in the softmax the tensor core works for the other.
 //
-// What bounds it was the issuing of the products (@@ISSUE@@). S of 64 keys in two places a tile, two steps ahead of the softmax, was slower: a product of 64 columns
-// takes the tensor core as long as one of 128.
+// What bounds it: for one pair of tiles what comes before its few steps (tables, first pages, first softmax) and behind them, else the chain of a tile's step, as in the kernel for prompts. The MMAs are
+// issued by a whole warp that elects a lane for each: their descriptors then stay in registers that the warp shares. From one
+// lane's branch an MMA took 113 clocks to issue, where the tensor core needs 65 to 70, and that was the bound. 64 sequences behind 8,192 positions,
+// 32 heads over 8 of 128 (34 MB, 8.6 GFLOP; a pair of tiles a block, three or four steps each): 19.7 us (23.0 from one lane); sixteen questions of up to 90
+// tokens behind 4,096 positions (73 GFLOP): 75 us, 977 TFLOP/s (93 from one lane). S of 64 keys in two places a tile, two steps ahead of the softmax, was
+// slower: a product of 64 columns takes the tensor core as long as one of 128. Asking for the sequences' own pages ahead into L2 from here gained
+// nothing: this kernel slowed down by as much as the next one gained.
 //
 // A group of no more than one tile (HALVES): both halves of the block have the same rows and take the steps in turn, as parts of their own.
 // No row masks a key: only the last step of a share may have a single page, whose missing half takes part in nothing.
