@@ -23,7 +23,7 @@
 // row's sum is known every block of the cluster turns its own keys' scores into weights, sums them over the heads in order
 // and adds them to the keys' sums. A key belongs to one thread: no atomics, the same bits every time.
 //
-// P is rounded to bfloat16 before it meets the values, as everywhere on this path (half a step is 2^-9 of a weight, and errors
+// P is rounded to bfloat16 before it meets the values, as everywhere on this path (half a step is 2^-8 of a weight, and errors
 // of the keys add up like their weights: far below the output's own rounding); scores, statistics and sums are float32.
 //
 // Compiled once per head size: -DKRK_HEAD_DIM=<D>.

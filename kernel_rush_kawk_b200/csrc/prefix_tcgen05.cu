@@ -24,7 +24,7 @@
 //
 // The reference maximum m of a row moves only when the row's maximum has grown by more than 2^8 since it was set (its row of O is then
 // rescaled in tensor memory); until then p <= 2^8. The part that leaves is (m, sum, O) in float32, with
-// whichever m. P in bfloat16 is off by half a step, 2^-9 of a weight.
+// whichever m. P in bfloat16 is off by half a step, 2^-8 of a weight.
 //
 // Compiled once per head size, for head sizes 64 and 128: -DKRK_HEAD_DIM=<D>.
 #include "partial_attention.cuh"
