@@ -51,9 +51,9 @@ def _ptr(t) -> int | None:
 
 _SEGMENTS = [_P] * 7 + [c_int, c_int, _P, c_int]
 _PARTS_SIGNATURES = {
-    "krk_attention_in_parts": [_P, _P, _P, _P, c_int, c_int, c_int, _P, _P, _P, _P, c_int, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int,
+    "krk_attention_in_parts": [_P, _P, _P, _P, c_int, c_int, c_int, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int,
                                c_int, c_float, c_int, _P],
-    "krk_key_weights": [_P, _P, _P, _P, c_int, _P, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, c_int, c_float, c_int, _P],
+    "krk_key_weights": [_P, _P, _P, _P, c_int, _P, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, c_int, c_int, c_float, c_int, _P],
 }
 _PARTS_SIGNATURES.update({
     "krk_prefix_few_rows": [_P, _P, c_int, c_int, c_int, _P, c_int, c_int, c_int, *_SEGMENTS, _P, _P, c_int, c_int, c_float, _P, _P],
@@ -186,8 +186,8 @@ class CacheOps:
         # the prefixes' parts, then the own keys, which join them
         own_splits, tensor = 0, 0
         if not by_mma:
-            splits = self._splits(tiles * prefix.n_groups, 444) if group_rows else 0
-            own_splits = self._splits(-(-batch.max_q_len * per // 16) * kv * batch.n_seqs, 444)
+            splits = self._splits(-(-group_rows * per // 64) * kv * prefix.n_groups, 444) if group_rows else 0
+            own_splits = self._splits(-(-batch.max_q_len * per // 64) * kv * batch.n_seqs, 444)
         elif group_rows * per >= self.PREFIX_TENSOR_ROWS and self._by_tcgen05(qkv, D):
             tensor = 2 if group_rows * per <= 112 else 1  # one tile: its halves take the keys in turn
             splits = max(1, min(32, 148 // (-(-group_rows * per // 256) * kv * prefix.n_groups)))
@@ -201,7 +201,7 @@ class CacheOps:
         ml = o + 4 * parts * rows * heads * D
         if not by_mma:
             self.launches += 1
-            self._ok(lib.krk_attention_in_parts(out.data_ptr(), None, o, ml, rows, splits, own_splits, None, None, None, None, 0, 0, 1, *step, group_rows,
+            self._ok(lib.krk_attention_in_parts(out.data_ptr(), None, o, ml, rows, splits, own_splits, None, None, None, None, 0, 0, 1, 1, *step, group_rows,
                                                 batch.max_q_len, scale, _code(qkv.dtype), stream), "shared prefix attention")
         elif batch.is_decode:
             self.launches += splits > 0
@@ -276,22 +276,23 @@ class CacheOps:
         # the output with every row's log sum, then the weights by these
         lse = torch.empty(rows * heads, dtype=torch.float32, device=qkv.device)
         page_blocks = max(1, min(cache.width, -(-888 // (kv * batch.n_seqs))))
+        seen = min(batch.max_q_len, observe or batch.max_q_len)
         if not by_mma:
-            parts = self._splits(-(-batch.max_q_len * per // 16) * kv * batch.n_seqs, 444)
+            parts = self._splits(-(-batch.max_q_len * per // 64) * kv * batch.n_seqs, 444)
             scratch = torch.empty(parts * rows * heads * (D + 2), dtype=torch.float32, device=qkv.device)
             o = scratch.data_ptr()
             self.launches += 2
             self._ok(lib.krk_attention_in_parts(out.data_ptr(), lse.data_ptr(), o, o + 4 * parts * rows * heads * D, rows, 0, parts, *counts, int(observe or 0),
-                                                page_blocks, *q, *segments, *pages, 0, batch.max_q_len, scale, _code(qkv.dtype), stream), "scored attention")
+                                                page_blocks, seen, *q, *segments, *pages, 0, batch.max_q_len, scale, _code(qkv.dtype), stream), "scored attention")
             return out
         self._whole_attention(out, lse, qkv, heads, D, batch, cache, scale)
         if self._by_tcgen05(qkv, D) and not batch.is_decode and per <= 64:
             longest = cache.width * PAGE if torch.cuda.is_current_stream_capturing() else batch.max_kv_len  # a captured step's sequences grow
-            self._ok(lib.krk_key_weights_tcgen05(*counts, lse.data_ptr(), int(observe or 0), *q, *segments, pages[0], cache.k.shape[0], rows,
-                                                 min(batch.max_q_len, observe or batch.max_q_len), longest, scale, error, stream), "weights of keys")
+            self._ok(lib.krk_key_weights_tcgen05(*counts, lse.data_ptr(), int(observe or 0), *q, *segments, pages[0], cache.k.shape[0], rows, seen, longest,
+                                                 scale, error, stream), "weights of keys")
         else:
-            self._ok(lib.krk_key_weights(*counts, lse.data_ptr(), int(observe or 0), *q, *segments, pages[0], page_blocks, scale, _code(qkv.dtype), stream),
-                     "weights of keys")
+            self._ok(lib.krk_key_weights(*counts, lse.data_ptr(), int(observe or 0), *q, *segments, pages[0], page_blocks, seen, scale, _code(qkv.dtype),
+                                         stream), "weights of keys")
         return out
 
     # -- eviction ----------------------------------------------------------------------------

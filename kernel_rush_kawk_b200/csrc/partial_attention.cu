@@ -2,14 +2,14 @@
 // prefix and of a sequence's own keys, their join, and the weight that each key received. See partial_attention.cuh for what
 // the parts are.
 //
-// A block takes TILE (token, head) rows of one kv head and walks pages of 64 keys, brought to shared memory as float32:
-// S = Q K^T with a key and half the rows a thread, running maximum and sum of a row by eight threads, O += P V with a warp per
-// 16 keys of the page and a lane per column; the four warps' sums of O join at the end. Weights stay float32. All rows of a tile
-// share one read of K and V: with 16 rows the products take 3 shared-memory wavefronts per 8 multiply-adds a warp, two thirds
-// of the multiply-add rate.
+// A block takes TILE (token, head) rows of one kv head and walks pages of 64 keys, brought to shared memory as float32. Thread (ty, tx) of
+// 16 x 16 has rows ty + 16 i and keys tx + 16 j of S = Q K^T, four by four in registers, and columns 4 tx + 64 c of the same rows of O: a row's
+// statistics and its weights stay within half a warp. Weights stay float32. A product of 64 multiply-adds a thread reads 8 pieces of 16 bytes,
+// 12 shared-memory wavefronts a warp in the 16 clocks that the multiply-adds take. Tiles of fewer rows skip the places behind them by sixteens.
 //
 // Compiled once per head size: -DKRK_HEAD_DIM=<D>.
 #include "partial_attention.cuh"
+#include "tcgen05.cuh"
 
 #ifndef KRK_HEAD_DIM
 #error "compile with -DKRK_HEAD_DIM=<head size>"
@@ -19,80 +19,92 @@ namespace {
 
 constexpr int D = KRK_HEAD_DIM;
 constexpr int DPAD = (D + 3) / 4 * 4;  // columns in shared memory; those behind D are zero
-constexpr int PITCH = DPAD + 4;        // floats between rows of keys: eight neighbouring keys' pieces fall into different banks
-constexpr int TILE = 16;               // rows of a block
-constexpr int THREADS = 128;
+constexpr int PITCH = DPAD / 4 % 2 ? DPAD : DPAD + 4;  // floats between rows of queries and keys: eight neighbouring rows' pieces fall into different banks
+constexpr int P_PITCH = KRK_PAGE + 4;
+constexpr int TILE = 64;               // rows of a block
+constexpr int THREADS = 256;
+constexpr int JOIN_THREADS = 128;
+constexpr int MAX_SHARE = 8;           // blocks of a cluster that share a page's row tiles
+constexpr int CHUNKS = (DPAD + 63) / 64;  // of columns: a thread has four of each
 constexpr int PER_LANE = (D + 31) / 32;
 constexpr float LOG2E = 1.4426950408889634f;
+// Where the head is large the weights lie where the keys were, so that two blocks fit an SM; it costs a barrier a page.
+constexpr bool OVER_KEYS = D > 64;
 
 struct Shared {
-  float q[TILE][DPAD];
-  float k[KRK_PAGE][PITCH];
-  float v[KRK_PAGE][DPAD];
-  float s[KRK_PAGE][TILE + 4];  // scores, then weights, by key
-  float alpha[TILE], m[TILE], l[TILE];
+  float q[TILE * PITCH];
+  float k[KRK_PAGE * PITCH];
+  float v[KRK_PAGE * DPAD];
+  float p[OVER_KEYS ? 4 : TILE * P_PITCH];  // weights, [row][key]
 };
+static_assert(!OVER_KEYS || PITCH >= P_PITCH, "");
 constexpr size_t SMEM_BYTES = sizeof(Shared);
 
-template <typename T>
-__device__ __forceinline__ void load_queries(Shared& sm, const T* __restrict__ q, int q_stride, int row0, int n_rows, int tile, int G, int kh) {
-  for (int i = threadIdx.x; i < TILE * DPAD; i += THREADS) {
-    const int r = i / DPAD, d = i % DPAD, R = tile * TILE + r;
-    sm.q[r][d] = R < n_rows && d < D ? to_float<T>(q[(size_t)(row0 + R / G) * q_stride + (size_t)(kh * G + R % G) * D + d]) : 0.f;
-  }
-}
-
-// Keys (and values) `count` from the page's first on; the places behind them become zero, so that what they hold counts nowhere.
-template <typename T>
-__device__ __forceinline__ void load_page(Shared& sm, const T* __restrict__ k, const T* __restrict__ v, int count, bool values) {
+// 64 rows of D elements, row r from row(r) on, as float32; rows from `count` on become zero, so that what they hold counts nowhere. `pieces`: every row starts
+// on a 16-byte boundary.
+template <typename T, int STRIDE, typename Row>
+__device__ __forceinline__ void load_tile(float* dst, int count, bool pieces, Row row) {
   constexpr int V = 16 / sizeof(T);  // elements of a 16-byte piece
-  if (D % V == 0 && (((uintptr_t)k | (values ? (uintptr_t)v : 0)) & 15) == 0) {
-    // a thread's pieces four at a time, so that their loads are on their way together
-    constexpr int PIECES = KRK_PAGE * (D / V), AHEAD = 4;
-    auto put = [&](float* to, uint4 x) {
-      const T* e = reinterpret_cast<const T*>(&x);
-#pragma unroll
-      for (int c = 0; c < V; c += 4) *reinterpret_cast<float4*>(to + c) = make_float4(to_float<T>(e[c]), to_float<T>(e[c + 1]), to_float<T>(e[c + 2]), to_float<T>(e[c + 3]));
-    };
-    for (int i0 = threadIdx.x; i0 < PIECES; i0 += THREADS * AHEAD) {
-      uint4 kp[AHEAD], vp[AHEAD];
+  if (D % V == 0 && pieces) {
+    constexpr int ALL = 64 * (D / V), AHEAD = 4;  // a thread's pieces four at a time, so that their loads are on their way together
+    for (int i0 = threadIdx.x; i0 < ALL; i0 += THREADS * AHEAD) {
+      uint4 x[AHEAD];
 #pragma unroll
       for (int a = 0; a < AHEAD; ++a) {
-        const int i = i0 + a * THREADS;
-        const bool in = i < PIECES && i / (D / V) < count;
-        kp[a] = in ? *reinterpret_cast<const uint4*>(k + (size_t)i * V) : make_uint4(0, 0, 0, 0);
-        vp[a] = in && values ? *reinterpret_cast<const uint4*>(v + (size_t)i * V) : make_uint4(0, 0, 0, 0);
+        const int i = i0 + a * THREADS, r = i / (D / V);
+        x[a] = i < ALL && r < count ? *reinterpret_cast<const uint4*>(row(r) + i % (D / V) * V) : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
       for (int a = 0; a < AHEAD; ++a) {
-        const int i = i0 + a * THREADS, key = i / (D / V), d = i % (D / V) * V;
-        if (i >= PIECES) break;
-        put(&sm.k[key][d], kp[a]);
-        if (values) put(&sm.v[key][d], vp[a]);
+        const int i = i0 + a * THREADS;
+        if (i >= ALL) break;
+        const T* e = reinterpret_cast<const T*>(x + a);
+        float* to = dst + i / (D / V) * STRIDE + i % (D / V) * V;
+#pragma unroll
+        for (int c = 0; c < V; c += 4) *reinterpret_cast<float4*>(to + c) = make_float4(to_float<T>(e[c]), to_float<T>(e[c + 1]), to_float<T>(e[c + 2]), to_float<T>(e[c + 3]));
       }
     }
     return;
   }
-  for (int i = threadIdx.x; i < KRK_PAGE * DPAD; i += THREADS) {
-    const int key = i / DPAD, d = i % DPAD;
-    const bool in = key < count && d < D;
-    sm.k[key][d] = in ? to_float<T>(k[key * D + d]) : 0.f;
-    if (values) sm.v[key][d] = in ? to_float<T>(v[key * D + d]) : 0.f;
+  for (int i = threadIdx.x; i < 64 * DPAD; i += THREADS) {
+    const int r = i / DPAD, d = i % DPAD;
+    dst[r * STRIDE + d] = r < count && d < D ? to_float<T>(row(r)[d]) : 0.f;
   }
 }
 
-// Scores of key threadIdx.x % 64 with eight of the tile's rows, from row 8 * (threadIdx.x / 64) on.
-__device__ __forceinline__ void scores(const Shared& sm, float (&s)[8]) {
-  const int key = threadIdx.x % KRK_PAGE, r0 = threadIdx.x / KRK_PAGE * 8;
+// Rows `tile` of one kv head's n_rows (token, head) rows from row0 on.
+template <typename T>
+__device__ __forceinline__ void load_queries(Shared& sm, const T* __restrict__ q, int q_stride, int row0, int n_rows, int tile, int G, int kh) {
+  const bool pieces = (((uintptr_t)q | (q_stride * sizeof(T)) | (D * sizeof(T))) & 15) == 0;
+  load_tile<T, PITCH>(sm.q, n_rows - tile * TILE, pieces, [&](int r) {
+    const int R = tile * TILE + r;
+    return q + (size_t)(row0 + R / G) * q_stride + (size_t)(kh * G + R % G) * D;
+  });
+}
+
+template <typename T, int STRIDE>
+__device__ __forceinline__ void load_page(float* dst, const T* __restrict__ page, int count) {
+  load_tile<T, STRIDE>(dst, count, ((uintptr_t)page & 15) == 0, [&](int r) { return page + r * D; });
+}
+
+// Scores of rows ty + 16 i (i below `live`) with keys tx + 16 j.
+__device__ __forceinline__ void scores(const Shared& sm, int live, float (&s)[4][4]) {
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
 #pragma unroll
-  for (int r = 0; r < 8; ++r) s[r] = 0.f;
-#pragma unroll 4
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll 2
   for (int d = 0; d < DPAD; d += 4) {
-    const float4 kv = *reinterpret_cast<const float4*>(&sm.k[key][d]);
+    float4 k[4];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      const float4 qv = *reinterpret_cast<const float4*>(&sm.q[r0 + r][d]);
-      s[r] = fmaf(kv.x, qv.x, fmaf(kv.y, qv.y, fmaf(kv.z, qv.z, fmaf(kv.w, qv.w, s[r]))));
+    for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const float4*>(sm.k + (tx + 16 * j) * PITCH + d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i >= live) break;
+      const float4 q = *reinterpret_cast<const float4*>(sm.q + (ty + 16 * i) * PITCH + d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[i][j] = fmaf(k[j].x, q.x, fmaf(k[j].y, q.y, fmaf(k[j].z, q.z, fmaf(k[j].w, q.w, s[i][j]))));
     }
   }
 }
@@ -100,7 +112,7 @@ __device__ __forceinline__ void scores(const Shared& sm, float (&s)[8]) {
 // Block (tile x split, kv head, group or sequence): the groups' prefixes first, in n_prefix parts, then the sequences' own keys in
 // n_own more.
 template <typename T>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1)
 partial_attention_kernel(Parts parts, int n_prefix, int n_own, const T* __restrict__ q, int q_stride, int HQ, int HKV, Segments seg,
                          const T* __restrict__ k_cache, const T* __restrict__ v_cache, float scale_log2) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -115,117 +127,139 @@ partial_attention_kernel(Parts parts, int n_prefix, int n_own, const T* __restri
   const Unit u = own ? own_unit(seg, blockIdx.z - groups) : prefix_unit(seg, blockIdx.z);
   const int n_rows = u.n_tok * G;
   if (tile * TILE >= n_rows) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  const int live = min(4, (n_rows - tile * TILE + 15) / 16);
   const int last_tok = min(u.n_tok - 1, (tile * TILE + TILE - 1) / G);
   const int key_end = own ? min(u.key_hi, u.start + last_tok + 1) : u.key_hi;  // behind the last key that the tile sees
   int j_lo, j_hi;
   split_pages(u.key_lo, key_end, split, n_splits, j_lo, j_hi);
 
   load_queries(sm, q, q_stride, u.row0, n_rows, tile, G, kh);
-  if (threadIdx.x < TILE) {
-    sm.m[threadIdx.x] = -INFINITY;
-    sm.l[threadIdx.x] = 0.f;
+  float m[4], l[4], acc[4][CHUNKS][4];  // l: of this thread's keys alone, until the end
+  int row_end[4];                       // behind the last key that the row sees
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+    row_end[i] = min(key_end, u.start + (tile * TILE + ty + 16 * i) / G + 1);
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][c][e] = 0.f;
   }
-  float acc[TILE][PER_LANE];
-#pragma unroll
-  for (int r = 0; r < TILE; ++r)
-#pragma unroll
-    for (int i = 0; i < PER_LANE; ++i) acc[r][i] = 0.f;
+  float* p_s = OVER_KEYS ? sm.k : sm.p;
 
   for (int j = j_lo; j < j_hi; ++j) {
-    const int page = seg.table[(size_t)u.slot * seg.width + j];
+    const int page = seg.table[(size_t)u.slot * seg.width + j], key0 = j * KRK_PAGE, count = min(KRK_PAGE, key_end - key0);
     const size_t base = ((size_t)page * HKV + kh) * KRK_PAGE * D;
     __syncthreads();  // the page before this one has been read
-    load_page(sm, k_cache + base, v_cache + base, min(KRK_PAGE, key_end - j * KRK_PAGE), true);
+    load_page<T, PITCH>(sm.k, k_cache + base, count);
+    load_page<T, DPAD>(sm.v, v_cache + base, count);
     __syncthreads();
-    {
-      float s[8];
-      scores(sm, s);
-      const int key = threadIdx.x % KRK_PAGE, r0 = threadIdx.x / KRK_PAGE * 8;
+    float s[4][4];
+    scores(sm, live, s);
+    if (OVER_KEYS) __syncthreads();  // every thread has its scores
+    const bool whole = key0 + KRK_PAGE <= min(key_end, u.start + tile * TILE / G + 1);  // every row sees the page to its end
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        const int tok = (tile * TILE + r0 + r) / G;
-        sm.s[key][r0 + r] = j * KRK_PAGE + key < min(key_end, u.start + tok + 1) ? s[r] * scale_log2 : -INFINITY;
-      }
-    }
-    __syncthreads();
-    {
-      const int r = threadIdx.x / 8, t = threadIdx.x % 8;  // eight threads a row, neighbours in a warp
+    for (int i = 0; i < 4; ++i) {
+      if (i >= live) break;
+      const int seen = row_end[i] - key0;  // keys of the page that the row sees
       float mx = -INFINITY;
-      for (int key = t; key < KRK_PAGE; key += 8) mx = fmaxf(mx, sm.s[key][r]);
 #pragma unroll
-      for (int o = 4; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      const float m_old = sm.m[r], m_new = fmaxf(m_old, mx), safe = m_new == -INFINITY ? 0.f : m_new;
+      for (int e = 0; e < 4; ++e) {
+        s[i][e] = tx + 16 * e < seen ? s[i][e] * scale_log2 : -INFINITY;
+        mx = fmaxf(mx, s[i][e]);
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float m_new = fmaxf(m[i], mx), safe = m_new == -INFINITY ? 0.f : m_new, alpha = exp2f(m[i] - safe);
+      m[i] = m_new;
       float sum = 0.f;
-      const int row_end = min(key_end, u.start + (tile * TILE + r) / G + 1) - j * KRK_PAGE;  // behind the last key of the page that the row sees
-      for (int key = t; key < KRK_PAGE; key += 8) {
-        const float p = exp2f(sm.s[key][r] - safe);
-        sm.s[key][r] = key < row_end ? p : -1.f;  // no weight: what the value is does not count
-        if (key < row_end) sum += p;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = exp2f(s[i][e] - safe);
+        if (tx + 16 * e < seen) sum += p;
+        p_s[(ty + 16 * i) * P_PITCH + tx + 16 * e] = tx + 16 * e < seen ? p : -1.f;  // no weight: what the value is does not count
       }
+      l[i] = l[i] * alpha + sum;
 #pragma unroll
-      for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      __syncwarp();
-      if (t == 0) {
-        const float a = exp2f(m_old - safe);
-        sm.alpha[r] = a;
-        sm.l[r] = sm.l[r] * a + sum;
-        sm.m[r] = m_new;
-      }
+      for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][c][e] *= alpha;
     }
-    __syncthreads();
+    __syncwarp();  // a row's weights come from the half warp that reads them
+    if (whole) {
+#pragma unroll 2
+      for (int key = 0; key < KRK_PAGE; key += 4) {
+        float4 p[4];
 #pragma unroll
-    for (int r = 0; r < TILE; ++r) {
-      const float a = sm.alpha[r];
+        for (int i = 0; i < 4; ++i)
+          if (i < live) p[i] = *reinterpret_cast<const float4*>(p_s + (ty + 16 * i) * P_PITCH + key);
 #pragma unroll
-      for (int i = 0; i < PER_LANE; ++i) acc[r][i] *= a;
-    }
-    const bool whole = j * KRK_PAGE + KRK_PAGE <= min(key_end, u.start + tile * TILE / G + 1);  // every row sees the page to its end
-    for (int key = warp * 16; key < warp * 16 + 16; ++key) {
-      float p[TILE];
+        for (int c = 0; c < CHUNKS; ++c) {
+          const int d = 4 * tx + 64 * c;
+          if (DPAD % 64 && d >= DPAD) break;
 #pragma unroll
-      for (int r = 0; r < TILE; r += 4) *reinterpret_cast<float4*>(p + r) = *reinterpret_cast<const float4*>(&sm.s[key][r]);
+          for (int e = 0; e < 4; ++e) {
+            const float4 v = *reinterpret_cast<const float4*>(sm.v + (key + e) * DPAD + d);
 #pragma unroll
-      for (int i = 0; i < PER_LANE; ++i) {
-        const int d = lane + 32 * i;
-        const float v = d < DPAD ? sm.v[key][d] : 0.f;
-#pragma unroll
-        for (int r = 0; r < TILE; ++r)
-          if (whole || p[r] >= 0.f || p[r] != p[r]) acc[r][i] = fmaf(p[r], v, acc[r][i]);
-      }
-    }
-  }
-  // the four warps' sums, in warp order, through the place of the keys
-  __syncthreads();
-  float* sum = &sm.k[0][0];  // [TILE][D]
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (warp == w) {
-#pragma unroll
-      for (int r = 0; r < TILE; ++r)
-#pragma unroll
-        for (int i = 0; i < PER_LANE; ++i) {
-          const int d = lane + 32 * i;
-          if (d < D) sum[r * D + d] = (w ? sum[r * D + d] : 0.f) + acc[r][i];
+            for (int i = 0; i < 4; ++i) {
+              if (i >= live) break;
+              const float w = e == 0 ? p[i].x : e == 1 ? p[i].y : e == 2 ? p[i].z : p[i].w;
+              acc[i][c][0] = fmaf(w, v.x, acc[i][c][0]);
+              acc[i][c][1] = fmaf(w, v.y, acc[i][c][1]);
+              acc[i][c][2] = fmaf(w, v.z, acc[i][c][2]);
+              acc[i][c][3] = fmaf(w, v.w, acc[i][c][3]);
+            }
+          }
         }
+      }
+    } else {
+      for (int key = 0; key < count; ++key) {
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = i < live ? p_s[(ty + 16 * i) * P_PITCH + key] : -1.f;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+          const int d = 4 * tx + 64 * c;
+          if (DPAD % 64 && d >= DPAD) break;
+          const float4 v = *reinterpret_cast<const float4*>(sm.v + key * DPAD + d);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (p[i] >= 0.f || p[i] != p[i]) {
+              acc[i][c][0] = fmaf(p[i], v.x, acc[i][c][0]);
+              acc[i][c][1] = fmaf(p[i], v.y, acc[i][c][1]);
+              acc[i][c][2] = fmaf(p[i], v.z, acc[i][c][2]);
+              acc[i][c][3] = fmaf(p[i], v.w, acc[i][c][3]);
+            }
+        }
+      }
     }
-    __syncthreads();
   }
-  for (int r = 0; r < TILE; ++r) {
-    const int R = tile * TILE + r;
-    if (R >= n_rows) break;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i >= live) break;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+    const int R = tile * TILE + ty + 16 * i;
+    if (R >= n_rows) continue;
     const size_t at = parts.at(part0 + split, u.row0 + R / G, kh * G + R % G);
-    if (sm.l[r] > 0.f || sm.l[r] != sm.l[r])
-      for (int d = threadIdx.x; d < D; d += THREADS) parts.o[at * D + d] = sum[r * D + d];
-    if (threadIdx.x == 0) parts.ml[at] = make_float2(sm.m[r], sm.l[r]);
+    if (l[i] != 0.f)  // (a NaN is none)
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * tx + 64 * c + e < D) parts.o[at * D + 4 * tx + 64 * c + e] = acc[i][c][e];
+    if (tx == 0) parts.ml[at] = make_float2(m[i], l[i]);
   }
 }
 
 // One warp per (row, head): the parts' join. lse (may be null): log2 of the sum of the row's 2^s, for the weights of its keys.
 template <typename T>
-__global__ void __launch_bounds__(THREADS) join_parts_kernel(T* __restrict__ out, float* __restrict__ lse, Parts parts, int n_parts) {
+__global__ void __launch_bounds__(JOIN_THREADS) join_parts_kernel(T* __restrict__ out, float* __restrict__ lse, Parts parts, int n_parts) {
   grid_launch_dependents();
   grid_dependency_wait();
-  const long long item = (long long)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
+  const long long item = (long long)blockIdx.x * (JOIN_THREADS / 32) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (item >= (long long)parts.rows * parts.HQ) return;
   const size_t step = (size_t)parts.rows * parts.HQ;
@@ -266,55 +300,77 @@ __global__ void __launch_bounds__(THREADS) join_parts_kernel(T* __restrict__ out
 
 // The weight that each key of a sequence receives from the step's last `observe` queries (all of them where it is 0), added up
 // over the heads of its kv head: sums_out = sums + weight for keys held before the step, the weight alone for the step's
-// own. Block (pages x, x + gridDim.x, ..., kv head, sequence); a key's sum is one thread pair's, in the order of the rows.
+// own. Block (pages x, x + gridDim.x / share, ..., kv head, sequence); a cluster's `share` blocks take the row tiles of a page in turn, and the first adds
+// their sums up in order.
 template <typename T>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, D <= 128 ? 2 : 1)
 key_weights_kernel(const float* sums, float* sums_out, int* __restrict__ positions, const int* __restrict__ seq_shift, int capacity,
                    const float* __restrict__ lse, int observe, const T* __restrict__ q, int q_stride, int HQ, int HKV, Segments seg,
-                   const T* __restrict__ k_cache, float scale_log2) {
+                   const T* __restrict__ k_cache, float scale_log2, int share) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Shared& sm = *reinterpret_cast<Shared*>(smem_raw);
+  __shared__ float minus_lse[TILE], warp_sums[THREADS / 32][KRK_PAGE], inbox[MAX_SHARE][KRK_PAGE];
+  if (share > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // "I have started"
   grid_launch_dependents();
   grid_dependency_wait();
-  const int kh = blockIdx.y, seq = blockIdx.z, G = HQ / HKV;
+  if (share > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const int rank = blockIdx.x % share, kh = blockIdx.y, seq = blockIdx.z, G = HQ / HKV;
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Unit u = own_unit(seg, seq);
   const int seen = observe > 0 ? min(observe, u.n_tok) : u.n_tok, tok0 = u.n_tok - seen;
-  const int n_rows = seen * G, row0 = u.row0 + tok0;
-  const int key = threadIdx.x % KRK_PAGE, half = threadIdx.x / KRK_PAGE;
-  for (int j = blockIdx.x; j * KRK_PAGE < u.key_hi; j += gridDim.x) {
-    const int page = seg.table[(size_t)u.slot * seg.width + j];
+  const int n_rows = seen * G, row0 = u.row0 + tok0, start = u.start + tok0;
+  for (int j = blockIdx.x / share; j * KRK_PAGE < u.key_hi; j += gridDim.x / share) {
+    const int page = seg.table[(size_t)u.slot * seg.width + j], key0 = j * KRK_PAGE;
     const size_t base = ((size_t)page * HKV + kh) * KRK_PAGE * D;
-    const int at = j * KRK_PAGE + key;
     __syncthreads();
-    load_page<T>(sm, k_cache + base, nullptr, min(KRK_PAGE, u.key_hi - j * KRK_PAGE), false);
-    float sum = 0.f;
-    for (int tile = 0; tile * TILE < n_rows; ++tile) {
-      if (u.start + tok0 + min(seen - 1, (tile * TILE + TILE - 1) / G) < j * KRK_PAGE) continue;  // none of its rows sees the page
+    load_page<T, PITCH>(sm.k, k_cache + base, min(KRK_PAGE, u.key_hi - key0));
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    // the first tile that has a row that sees the page's first key
+    for (int tile = max(0, key0 - start) * G / TILE + rank; tile * TILE < n_rows; tile += share) {
+      const int live = min(4, (n_rows - tile * TILE + 15) / 16);
       __syncthreads();
       load_queries(sm, q, q_stride, row0, n_rows, tile, G, kh);
       if (threadIdx.x < TILE) {
         const int R = tile * TILE + threadIdx.x;
-        sm.l[threadIdx.x] = R < n_rows ? lse[(size_t)(row0 + R / G) * HQ + kh * G + R % G] : 0.f;
+        minus_lse[threadIdx.x] = R < n_rows ? -lse[(size_t)(row0 + R / G) * HQ + kh * G + R % G] : 0.f;
       }
       __syncthreads();
-      float s[8], part = 0.f;
-      scores(sm, s);
+      float s[4][4];
+      scores(sm, live, s);
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        const int R = tile * TILE + half * 8 + r;
-        if (R < n_rows && at <= u.start + tok0 + R / G) part += exp2f(fmaf(s[r], scale_log2, -sm.l[half * 8 + r]));
+      for (int i = 0; i < 4; ++i) {
+        if (i >= live) break;
+        const int R = tile * TILE + ty + 16 * i, end = R < n_rows ? start + R / G + 1 - key0 : 0;  // behind the last key of the page that the row sees
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (tx + 16 * e < end) sum[e] += exp2f(fmaf(s[i][e], scale_log2, minus_lse[ty + 16 * i]));
       }
-      sum += part;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 16);
+      if (lane < 16) warp_sums[warp][tx + 16 * e] = sum[e];
     }
     __syncthreads();
-    if (half == 1) sm.s[key][0] = sum;
-    __syncthreads();
-    if (half == 0 && at < u.key_hi) {
-      sum += sm.s[key][0];
+    float total = 0.f;
+    if (threadIdx.x < KRK_PAGE)
+#pragma unroll
+      for (int w = 0; w < THREADS / 32; ++w) total += warp_sums[w][threadIdx.x];
+    if (share > 1) {
+      if (threadIdx.x < KRK_PAGE)
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(tc::cluster_address(&inbox[rank][threadIdx.x], 0)), "f"(total) : "memory");
+      tc::cluster_sync();
+      total = 0.f;
+      if (rank == 0 && threadIdx.x < KRK_PAGE)
+        for (int c = 0; c < share; ++c) total += inbox[c][threadIdx.x];
+    }
+    const int at = key0 + threadIdx.x;
+    if (rank == 0 && threadIdx.x < KRK_PAGE && at < u.key_hi) {
       const size_t place = ((size_t)u.slot * HKV + kh) * capacity + at;
-      sums_out[place] = at < u.start ? sums[place] + sum : sum;
+      sums_out[place] = at < u.start ? sums[place] + total : total;
       if (positions && at >= u.start) positions[place] = at + (seq_shift ? seq_shift[seq] : 0);
     }
+    if (share > 1) tc::cluster_sync();  // the first block has read what the others sent
   }
 }
 
@@ -354,28 +410,45 @@ static int krk_partial_attention(float* o, float* ml, int rows, int n_prefix, in
 
 static int krk_join_parts(void* out, float* lse, const float* o, const float* ml, int rows, int HQ, int n_parts, int dtype, cudaStream_t stream) {
   const Parts parts = {const_cast<float*>(o), (float2*)const_cast<float*>(ml), rows, HQ};
-  const long long blocks = ((long long)rows * HQ + THREADS / 32 - 1) / (THREADS / 32);
+  const long long blocks = ((long long)rows * HQ + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32);
   if (blocks == 0) return 0;
   if (blocks > 0x7fffffffLL) return -3;
   if (dtype == KRK_DTYPE_F32)
-    return (int)launch_pdl(join_parts_kernel<float>, dim3((unsigned)blocks), dim3(THREADS), 0, stream, (float*)out, lse, parts, n_parts);
-  return (int)launch_pdl(join_parts_kernel<bf16>, dim3((unsigned)blocks), dim3(THREADS), 0, stream, (bf16*)out, lse, parts, n_parts);
+    return (int)launch_pdl(join_parts_kernel<float>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, stream, (float*)out, lse, parts, n_parts);
+  return (int)launch_pdl(join_parts_kernel<bf16>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, stream, (bf16*)out, lse, parts, n_parts);
 }
 
-// page_blocks: blocks that share a sequence's pages; any number is right.
+// page_blocks: blocks, or clusters, that share a sequence's pages; any number is right. max_seen: the most queries of a sequence that count.
 KRK_API int krk_key_weights(const float* sums, float* sums_out, int* positions, const int* seq_shift, int capacity, const float* lse, int observe,
-                            const void* q, int q_stride, int HQ, int HKV, KRK_SEGMENTS, const void* k_cache, int page_blocks, float scale, int dtype,
-                            cudaStream_t stream) {
+                            const void* q, int q_stride, int HQ, int HKV, KRK_SEGMENTS, const void* k_cache, int page_blocks, int max_seen, float scale,
+                            int dtype, cudaStream_t stream) {
   const Segments seg = KRK_MAKE_SEGMENTS;
   if (n_seqs == 0) return 0;
   if (HKV > 65535 || n_seqs > 65535 || page_blocks < 1) return -3;
-  const dim3 grid(page_blocks, HKV, n_seqs);
+  // a page's row tiles are shared out while blocks are few for the device and each has two tiles or more
+  const long long tiles = ((long long)max_seen * (HQ / HKV) + TILE - 1) / TILE, blocks = (long long)page_blocks * HKV * n_seqs;
+  int share = 1;
+  while (share < MAX_SHARE && blocks * share < 296 && tiles >= 4 * share) share *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)page_blocks * share, HKV, n_seqs);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = share;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
   static unsigned long long allowed[2] = {0, 0};
   auto go = [&](auto* kern, auto* queries, auto* keys) {
     cudaError_t e = allow_shared(kern, SMEM_BYTES, allowed + (dtype == KRK_DTYPE_F32));
     if (e != cudaSuccess) return (int)e;
-    return (int)launch_pdl(kern, grid, dim3(THREADS), SMEM_BYTES, stream, sums, sums_out, positions, seq_shift, capacity, lse, observe, queries,
-                           q_stride, HQ, HKV, seg, keys, scale * LOG2E);
+    return (int)cudaLaunchKernelEx(&cfg, kern, sums, sums_out, positions, seq_shift, capacity, lse, observe, queries, q_stride, HQ, HKV, seg, keys,
+                                   scale * LOG2E, share);
   };
   if (dtype == KRK_DTYPE_F32) return go(key_weights_kernel<float>, (const float*)q, (const float*)k_cache);
   return go(key_weights_kernel<bf16>, (const bf16*)q, (const bf16*)k_cache);
@@ -384,7 +457,7 @@ KRK_API int krk_key_weights(const float* sums, float* sums_out, int* positions, 
 // Attention in parts and their join (out; lse may be null) and, where sums_out is given, the weights of the keys, with lse as their logarithms: krk_partial_attention,
 // krk_join_parts and krk_key_weights in one call. o, ml: scratch for n_prefix + n_own parts.
 KRK_API int krk_attention_in_parts(void* out, float* lse, float* o, float* ml, int rows, int n_prefix, int n_own, const float* sums, float* sums_out,
-                                   int* positions, const int* seq_shift, int capacity, int observe, int page_blocks, const void* q, int q_stride, int HQ,
+                                   int* positions, const int* seq_shift, int capacity, int observe, int page_blocks, int max_seen, const void* q, int q_stride, int HQ,
                                    int HKV, KRK_SEGMENTS, const void* k_cache, const void* v_cache, int group_rows, int own_rows, float scale, int dtype,
                                    cudaStream_t stream) {
   int rc = krk_partial_attention(o, ml, rows, n_prefix, n_own, q, q_stride, HQ, HKV, cu_q, seq_slot, seq_start, seq_qlen, group_cu, group_len, seq_group,
@@ -392,6 +465,6 @@ KRK_API int krk_attention_in_parts(void* out, float* lse, float* o, float* ml, i
   if (rc == 0) rc = krk_join_parts(out, lse, o, ml, rows, HQ, n_prefix + n_own, dtype, stream);
   if (rc == 0 && sums_out)
     rc = krk_key_weights(sums, sums_out, positions, seq_shift, capacity, lse, observe, q, q_stride, HQ, HKV, cu_q, seq_slot, seq_start, seq_qlen, group_cu,
-                         group_len, seq_group, n_seqs, n_groups, table, width, k_cache, page_blocks, scale, dtype, stream);
+                         group_len, seq_group, n_seqs, n_groups, table, width, k_cache, page_blocks, max_seen, scale, dtype, stream);
   return rc;
 }
