@@ -8,6 +8,7 @@
 // 12 shared-memory wavefronts a warp in the 16 clocks that the multiply-adds take. Tiles of fewer rows skip the places behind them by sixteens.
 //
 // Compiled once per head size: -DKRK_HEAD_DIM=<D>.
+#include "mma.cuh"
 #include "partial_attention.cuh"
 #include "tcgen05.cuh"
 
@@ -34,17 +35,27 @@ constexpr bool OVER_KEYS = D > 64;
 struct Shared {
   float q[TILE * PITCH];
   float k[KRK_PAGE * PITCH];
-  float v[KRK_PAGE * DPAD];
+  float v[KRK_PAGE * PITCH];  // [key][DPAD]; of the weights' kernel a second tile of queries
   float p[OVER_KEYS ? 4 : TILE * P_PITCH];  // weights, [row][key]
 };
 static_assert(!OVER_KEYS || PITCH >= P_PITCH, "");
 constexpr size_t SMEM_BYTES = sizeof(Shared);
 
-// 64 rows of D elements, row r from row(r) on, as float32; rows from `count` on become zero, so that what they hold counts nowhere. `pieces`: every row starts
-// on a 16-byte boundary.
+// 64 rows of D elements, row r from row(r) on, as float32; rows from `count` (1 or more) on become zero, so that what they hold counts nowhere. `pieces`: every row
+// starts on a 16-byte boundary. Rows of float32 are on their way when the call returns (cp.async; a group of its own), others are there.
 template <typename T, int STRIDE, typename Row>
 __device__ __forceinline__ void load_tile(float* dst, int count, bool pieces, Row row) {
   constexpr int V = 16 / sizeof(T);  // elements of a 16-byte piece
+  if (sizeof(T) == 4 && D % V == 0 && pieces) {
+    for (int i = threadIdx.x; i < 64 * (D / V); i += THREADS) {
+      const int r = i / (D / V), c = i % (D / V) * V;
+      const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst + r * STRIDE + c);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(row(min(r, count - 1)) + c), "r"(r < count ? 16 : 0) : "memory");
+    }
+    cp_async_commit();
+    return;
+  }
+  cp_async_commit();  // (an empty group: the waits count groups)
   if (D % V == 0 && pieces) {
     constexpr int ALL = 64 * (D / V), AHEAD = 4;  // a thread's pieces four at a time, so that their loads are on their way together
     for (int i0 = threadIdx.x; i0 < ALL; i0 += THREADS * AHEAD) {
@@ -74,9 +85,9 @@ __device__ __forceinline__ void load_tile(float* dst, int count, bool pieces, Ro
 
 // Rows `tile` of one kv head's n_rows (token, head) rows from row0 on.
 template <typename T>
-__device__ __forceinline__ void load_queries(Shared& sm, const T* __restrict__ q, int q_stride, int row0, int n_rows, int tile, int G, int kh) {
+__device__ __forceinline__ void load_queries(float* dst, const T* __restrict__ q, int q_stride, int row0, int n_rows, int tile, int G, int kh) {
   const bool pieces = (((uintptr_t)q | (q_stride * sizeof(T)) | (D * sizeof(T))) & 15) == 0;
-  load_tile<T, PITCH>(sm.q, n_rows - tile * TILE, pieces, [&](int r) {
+  load_tile<T, PITCH>(dst, n_rows - tile * TILE, pieces, [&](int r) {
     const int R = tile * TILE + r;
     return q + (size_t)(row0 + R / G) * q_stride + (size_t)(kh * G + R % G) * D;
   });
@@ -88,7 +99,7 @@ __device__ __forceinline__ void load_page(float* dst, const T* __restrict__ page
 }
 
 // Scores of rows ty + 16 i (i below `live`) with keys tx + 16 j.
-__device__ __forceinline__ void scores(const Shared& sm, int live, float (&s)[4][4]) {
+__device__ __forceinline__ void scores(const float* q_s, const float* k_s, int live, float (&s)[4][4]) {
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -98,11 +109,11 @@ __device__ __forceinline__ void scores(const Shared& sm, int live, float (&s)[4]
   for (int d = 0; d < DPAD; d += 4) {
     float4 k[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const float4*>(sm.k + (tx + 16 * j) * PITCH + d);
+    for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const float4*>(k_s + (tx + 16 * j) * PITCH + d);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (i >= live) break;
-      const float4 q = *reinterpret_cast<const float4*>(sm.q + (ty + 16 * i) * PITCH + d);
+      const float4 q = *reinterpret_cast<const float4*>(q_s + (ty + 16 * i) * PITCH + d);
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[i][j] = fmaf(k[j].x, q.x, fmaf(k[j].y, q.y, fmaf(k[j].z, q.z, fmaf(k[j].w, q.w, s[i][j]))));
     }
@@ -134,7 +145,19 @@ partial_attention_kernel(Parts parts, int n_prefix, int n_own, const T* __restri
   int j_lo, j_hi;
   split_pages(u.key_lo, key_end, split, n_splits, j_lo, j_hi);
 
-  load_queries(sm, q, q_stride, u.row0, n_rows, tile, G, kh);
+  auto load_k = [&](int j) {
+    const size_t page = (size_t)seg.table[(size_t)u.slot * seg.width + j] * HKV + kh;
+    load_page<T, PITCH>(sm.k, k_cache + page * KRK_PAGE * D, min(KRK_PAGE, key_end - j * KRK_PAGE));
+  };
+  auto load_v = [&](int j) {
+    const size_t page = (size_t)seg.table[(size_t)u.slot * seg.width + j] * HKV + kh;
+    load_page<T, DPAD>(sm.v, v_cache + page * KRK_PAGE * D, min(KRK_PAGE, key_end - j * KRK_PAGE));
+  };
+  if (j_lo < j_hi) {
+    load_queries(sm.q, q, q_stride, u.row0, n_rows, tile, G, kh);
+    load_k(j_lo);
+    load_v(j_lo);
+  }
   float m[4], l[4], acc[4][CHUNKS][4];  // l: of this thread's keys alone, until the end
   int row_end[4];                       // behind the last key that the row sees
 #pragma unroll
@@ -150,15 +173,14 @@ partial_attention_kernel(Parts parts, int n_prefix, int n_own, const T* __restri
   float* p_s = OVER_KEYS ? sm.k : sm.p;
 
   for (int j = j_lo; j < j_hi; ++j) {
-    const int page = seg.table[(size_t)u.slot * seg.width + j], key0 = j * KRK_PAGE, count = min(KRK_PAGE, key_end - key0);
-    const size_t base = ((size_t)page * HKV + kh) * KRK_PAGE * D;
-    __syncthreads();  // the page before this one has been read
-    load_page<T, PITCH>(sm.k, k_cache + base, count);
-    load_page<T, DPAD>(sm.v, v_cache + base, count);
-    __syncthreads();
+    const int key0 = j * KRK_PAGE, count = min(KRK_PAGE, key_end - key0);
+    cp_async_wait<1>();
+    __syncthreads();  // the keys are here
     float s[4][4];
-    scores(sm, live, s);
-    if (OVER_KEYS) __syncthreads();  // every thread has its scores
+    scores(sm.q, sm.k, live, s);
+    cp_async_wait<0>();
+    __syncthreads();  // the values are here, and the keys' place is free
+    if (!OVER_KEYS && j + 1 < j_hi) load_k(j + 1);
     const bool whole = key0 + KRK_PAGE <= min(key_end, u.start + tile * TILE / G + 1);  // every row sees the page to its end
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -235,6 +257,11 @@ partial_attention_kernel(Parts parts, int n_prefix, int n_own, const T* __restri
         }
       }
     }
+    if (j + 1 < j_hi) {
+      __syncthreads();  // the values have been read
+      if (OVER_KEYS) load_k(j + 1);
+      load_v(j + 1);
+    }
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -309,7 +336,7 @@ key_weights_kernel(const float* sums, float* sums_out, int* __restrict__ positio
                    const T* __restrict__ k_cache, float scale_log2, int share) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Shared& sm = *reinterpret_cast<Shared*>(smem_raw);
-  __shared__ float minus_lse[TILE], warp_sums[THREADS / 32][KRK_PAGE], inbox[MAX_SHARE][KRK_PAGE];
+  __shared__ float minus_lse[2][TILE], warp_sums[THREADS / 32][KRK_PAGE], inbox[MAX_SHARE][KRK_PAGE];
   if (share > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // "I have started"
   grid_launch_dependents();
   grid_dependency_wait();
@@ -322,30 +349,40 @@ key_weights_kernel(const float* sums, float* sums_out, int* __restrict__ positio
   for (int j = blockIdx.x / share; j * KRK_PAGE < u.key_hi; j += gridDim.x / share) {
     const int page = seg.table[(size_t)u.slot * seg.width + j], key0 = j * KRK_PAGE;
     const size_t base = ((size_t)page * HKV + kh) * KRK_PAGE * D;
-    __syncthreads();
+    __syncthreads();  // the sums of the page before have been read
     load_page<T, PITCH>(sm.k, k_cache + base, min(KRK_PAGE, u.key_hi - key0));
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    // the first tile that has a row that sees the page's first key
-    for (int tile = max(0, key0 - start) * G / TILE + rank; tile * TILE < n_rows; tile += share) {
-      const int live = min(4, (n_rows - tile * TILE + 15) / 16);
-      __syncthreads();
-      load_queries(sm, q, q_stride, row0, n_rows, tile, G, kh);
+    const int first = max(0, key0 - start) * G / TILE + rank;  // of the tiles with a row that sees the page's first key, this block's first
+    auto load = [&](int tile, int place) {
+      load_queries(place ? sm.v : sm.q, q, q_stride, row0, n_rows, tile, G, kh);
       if (threadIdx.x < TILE) {
         const int R = tile * TILE + threadIdx.x;
-        minus_lse[threadIdx.x] = R < n_rows ? -lse[(size_t)(row0 + R / G) * HQ + kh * G + R % G] : 0.f;
+        minus_lse[place][threadIdx.x] = R < n_rows ? -lse[(size_t)(row0 + R / G) * HQ + kh * G + R % G] : 0.f;
+      }
+    };
+    if (first * TILE < n_rows) load(first, 0);
+    for (int tile = first, place = 0; tile * TILE < n_rows; tile += share, place ^= 1) {
+      const int live = min(4, (n_rows - tile * TILE + 15) / 16);
+      if ((tile + share) * TILE < n_rows) {
+        load(tile + share, place ^ 1);
+        cp_async_wait<1>();
+      } else {
+        cp_async_wait<0>();
       }
       __syncthreads();
       float s[4][4];
-      scores(sm, live, s);
+      scores(place ? sm.v : sm.q, sm.k, live, s);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (i >= live) break;
         const int R = tile * TILE + ty + 16 * i, end = R < n_rows ? start + R / G + 1 - key0 : 0;  // behind the last key of the page that the row sees
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (tx + 16 * e < end) sum[e] += exp2f(fmaf(s[i][e], scale_log2, minus_lse[ty + 16 * i]));
+          if (tx + 16 * e < end) sum[e] += exp2f(fmaf(s[i][e], scale_log2, minus_lse[place][ty + 16 * i]));
       }
+      __syncthreads();  // the tile has been read
     }
+    cp_async_wait<0>();  // of a page that no tile of this block's sees the keys are still on their way
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 16);
