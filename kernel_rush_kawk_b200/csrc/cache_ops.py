@@ -138,6 +138,13 @@ class CacheOps:
         return max(1, min(32, -(-wanted // max(blocks, 1))))
 
     @staticmethod
+    def _places(blocks: int, head_dim: int) -> int:
+        """Parts of a prefix, whose blocks have equal work, for the kernel of every type: of its blocks an SM has two, or one of large heads, and as many
+        come as run at once (four sequences of 30 tokens behind 1,024 positions, 32 heads over 8 of 128 in float32: 103 us, 128 with half a round more). Own
+        keys are unequally many, and come in more: a prompt of 600 tokens, 16 heads over 4 of 64, 115 us in three parts a tile and 150 in one."""
+        return max(1, min(32, 148 * (2 if head_dim <= 128 else 1) // max(blocks, 1)))
+
+    @staticmethod
     def _cluster_splits(items: int, all_keys: bool) -> int:
         """Blocks of a cluster that share the keys of a sequence's token, by the number of (sequence, kv head, row tile) items. ``all_keys``: all
         that the sequence holds, unequally many; else those behind a shared prefix, which are few. One sequence after 1,087 tokens in 1, 2, 4 and 8: 18.6,
@@ -186,7 +193,7 @@ class CacheOps:
         # the prefixes' parts, then the own keys, which join them
         own_splits, tensor = 0, 0
         if not by_mma:
-            splits = self._splits(-(-group_rows * per // 64) * kv * prefix.n_groups, 444) if group_rows else 0
+            splits = self._places(-(-group_rows * per // 64) * kv * prefix.n_groups, D) if group_rows else 0
             own_splits = self._splits(-(-batch.max_q_len * per // 64) * kv * batch.n_seqs, 444)
         elif group_rows * per >= self.PREFIX_TENSOR_ROWS and self._by_tcgen05(qkv, D):
             tensor = 2 if group_rows * per <= 112 else 1  # one tile: its halves take the keys in turn

@@ -7,6 +7,11 @@
 // statistics and its weights stay within half a warp. Weights stay float32. A product of 64 multiply-adds a thread reads 8 pieces of 16 bytes,
 // 12 shared-memory wavefronts a warp in the 16 clocks that the multiply-adds take. Tiles of fewer rows skip the places behind them by sixteens.
 //
+// What bounds it, float32: of single tokens the dependent steps of two or three launches (six sequences behind 960 positions, 16 heads over 4 of 64: 11.3 us for
+// the parts; 15 in tiles of 16 rows by 128 threads, the form before this one); of many rows issue slots and latencies at 16 warps an SM: two sequences of 300
+// tokens behind 512 positions, 32 heads over 8 of 128: 269 us, 23 TFLOP/s of 72 (430 in tiles of 16). Eight rows a thread by 128 threads
+// (fewer reads, fewer warps) took 335, three blocks an SM in 80 registers spilled and gained nothing.
+//
 // Compiled once per head size: -DKRK_HEAD_DIM=<D>.
 #include "mma.cuh"
 #include "partial_attention.cuh"
