@@ -94,8 +94,10 @@ class CacheOps:
 
     # -- what both attentions ask of their arguments ---------------------------------
     def _check_step(self, what, qkv, heads, kv_in_row, head_dim, batch, cache):
+        """Raise unless the step can be taken; (address of the rows, elements between them, addresses of the pages of keys and of values)."""
         shape, dtype, k, v = qkv.shape, qkv.dtype, cache.k, cache.v
-        if len(shape) != 2 or qkv.stride(1) != 1 or shape[1] != (heads + 2 * kv_in_row) * head_dim:
+        strides = qkv.stride()
+        if len(shape) != 2 or strides[1] != 1 or shape[1] != (heads + 2 * kv_in_row) * head_dim:
             raise KernelError(f"{what}: rows of {(heads + 2 * kv_in_row) * head_dim} elements side by side are asked for, got {tuple(shape)}")
         if heads % cache.kv_heads or cache.head_dim != head_dim or cache.v_dim != head_dim:
             raise KernelError(f"{what}: {heads} heads of {head_dim} do not fit a cache of {cache.kv_heads} heads of {cache.head_dim} (values: {cache.v_dim})")
@@ -105,9 +107,11 @@ class CacheOps:
             raise KernelError(f"{what}: the cache's pages are contiguous and of the rows' dtype ({dtype}), got {k.dtype}")
         if shape[0] != batch.n_rows or batch.max_kv_len > cache.width * PAGE:
             raise KernelError(f"{what}: {shape[0]} rows for a step of {batch.n_rows} with up to {batch.max_kv_len} keys, in slots of {cache.width * PAGE}")
-        if shape[0] > 1 and qkv.stride(0) < shape[1]:
-            raise KernelError(f"{what}: rows that overlap (a stride of {qkv.stride(0)})")
+        if shape[0] > 1 and strides[0] < shape[1]:
+            raise KernelError(f"{what}: rows that overlap (a stride of {strides[0]})")
         self._check_device(what, qkv, k)
+        # (a single row has no stride that means anything)
+        return qkv.data_ptr(), strides[0] if shape[0] > 1 else shape[1], k.data_ptr(), v.data_ptr()
 
     def _check_device(self, what, *tensors):
         mine = self.error.get_device()
@@ -119,10 +123,6 @@ class CacheOps:
                 return
         raise KernelError(f"{what}: tensors on {', '.join(str(t.device) for t in tensors)}, device {torch.cuda.current_device()} current, "
                           f"kernels on {self.error.device}")
-
-    @staticmethod
-    def _row_stride(qkv) -> int:
-        return qkv.stride(0) if qkv.shape[0] > 1 else qkv.shape[1]  # a single row has none that means anything
 
     @staticmethod
     def _segments(batch, cache, prefix):
@@ -154,17 +154,16 @@ class CacheOps:
             return 8 if items <= 64 else 4 if items <= 148 else 2 if items <= 592 else 1
         return 4 if items <= 37 else 2 if items <= 148 else 1
 
-    @classmethod
-    def _by_mma(cls, qkv, cache, head_dim) -> bool:
+    @staticmethod
+    def _by_mma(dtype, head_dim, q, stride, k, v) -> bool:
         """Whether the tensor-core kernels take these rows and pages: bfloat16, head sizes in steps of 16, rows from 4-byte, pages from 16-byte
         boundaries on."""
-        return (qkv.dtype == torch.bfloat16 and head_dim % 16 == 0 and cls._row_stride(qkv) % 2 == 0 and qkv.data_ptr() % 4 == 0
-                and (cache.k.data_ptr() | cache.v.data_ptr()) % 16 == 0)
+        return dtype == torch.bfloat16 and head_dim % 16 == 0 and stride % 2 == 0 and q % 4 == 0 and (k | v) % 16 == 0
 
-    @classmethod
-    def _by_tcgen05(cls, qkv, head_dim) -> bool:
+    @staticmethod
+    def _by_tcgen05(head_dim, q, stride) -> bool:
         """Whether the tcgen05 kernels take rows that ``_by_mma`` takes: heads of 64 or 128, rows from 16-byte boundaries on."""
-        return head_dim in (64, 128) and cls._row_stride(qkv) % 8 == 0 and qkv.data_ptr() % 16 == 0
+        return head_dim in (64, 128) and stride % 8 == 0 and q % 16 == 0
 
     # -- a shared prefix -----------------------------------------------------------------
     def shared_prefix_attention(self, qkv, heads, kv_in_row, head_dim, batch, cache, scale, prefix):
@@ -174,19 +173,19 @@ class CacheOps:
         (cache.prefix says when; elsewhere each sequence reads its own table's). The step's
         own keys and values must be in the cache already, and its rows lie behind their group's prefix. Any number of tokens a
         sequence, float32 or bfloat16; a captured step stays valid while the groups' number and sizes last, whatever the lengths become."""
-        self._check_step("shared prefix attention", qkv, heads, kv_in_row, head_dim, batch, cache)
+        q, stride, k, v = self._check_step("shared prefix attention", qkv, heads, kv_in_row, head_dim, batch, cache)
         prefix.check(batch, cache)
-        lib, rows, kv, per, D = self._parts_lib(head_dim), qkv.shape[0], cache.kv_heads, heads // cache.kv_heads, head_dim
-        out = torch.empty((rows, heads * D), dtype=qkv.dtype, device=qkv.device)
+        lib, rows, kv, per, D = self._parts_lib(head_dim), batch.n_rows, cache.kv_heads, heads // cache.kv_heads, head_dim
+        out = qkv.new_empty((rows, heads * D))
         if rows == 0:
             return out
         scale, stream, error = float(scale), self._stream(), self.error.data_ptr()
-        by_mma = self._by_mma(qkv, cache, D)
+        by_mma = self._by_mma(qkv.dtype, D, q, stride, k, v)
         if by_mma and not (single_tokens_share(prefix.sizes, prefix.lengths, 4 * kv * D) if batch.is_decode else
                            longer_steps_share(prefix.sizes, prefix.lengths, batch.q_lens, per, kv)):
-            self._whole_attention(out, None, qkv, heads, D, batch, cache, scale)  # each sequence by itself, through its own page table
+            self._whole_attention(out, None, (q, stride, heads, kv), D, batch, cache, (k, v), scale)  # each sequence by itself, through its own page table
             return out
-        step = (qkv.data_ptr(), self._row_stride(qkv), heads, kv, *self._segments(batch, cache, prefix), cache.k.data_ptr(), cache.v.data_ptr())
+        step = (q, stride, heads, kv, *self._segments(batch, cache, prefix), k, v)
         group_rows = prefix.max_rows(batch) if prefix.max_length else 0
         tiles = -(-group_rows * per // 16) * kv
         by_mma = by_mma and tiles <= 65535
@@ -195,7 +194,7 @@ class CacheOps:
         if not by_mma:
             splits = self._places(-(-group_rows * per // 64) * kv * prefix.n_groups, D) if group_rows else 0
             own_splits = self._splits(-(-batch.max_q_len * per // 64) * kv * batch.n_seqs, 444)
-        elif group_rows * per >= self.PREFIX_TENSOR_ROWS and self._by_tcgen05(qkv, D):
+        elif group_rows * per >= self.PREFIX_TENSOR_ROWS and self._by_tcgen05(D, q, stride):
             tensor = 2 if group_rows * per <= 112 else 1  # one tile: its halves take the keys in turn
             splits = max(1, min(32, 148 // (-(-group_rows * per // 256) * kv * prefix.n_groups)))
         else:
@@ -203,7 +202,7 @@ class CacheOps:
             # parts that the own keys' kernel has to join grow with them)
             splits = self._splits(tiles * prefix.n_groups, 148) if group_rows else 0
         parts = splits * max(tensor, 1) + own_splits
-        scratch = torch.empty(parts * rows * heads * (D + 2), dtype=torch.float32, device=qkv.device)
+        scratch = self._scratch(parts * rows * heads * (D + 2))
         o = scratch.data_ptr()
         ml = o + 4 * parts * rows * heads * D
         if not by_mma:
@@ -223,19 +222,22 @@ class CacheOps:
             self._ok(lib.krk_own_rows(out.data_ptr(), None, o, ml, rows, parts, *step, batch.max_q_len, scale, stream), "attention over own keys")
         return out
 
-    def _whole_attention(self, out, lse, qkv, heads, D, batch, cache, scale):
+    def _scratch(self, n: int):
+        """n places of 32 bits, of this call alone; the caller holds them until its launches are queued."""
+        return self.error.new_empty(n)
+
+    def _whole_attention(self, out, lse, q, D, batch, cache, pages, scale):
         """Every row over all of its sequence's keys, for what ``_by_mma`` takes; ``lse`` (float32 [rows, heads] or None) takes the base-two
         logarithm of each row's sum. Unlike ``attention``, whatever lies in pages and rows that no query sees."""
-        kv, rows, per = cache.kv_heads, qkv.shape[0], heads // cache.kv_heads
+        address, stride, heads, kv = q
+        rows, per = batch.n_rows, heads // kv
         lib, error, stream = self._parts_lib(D), self.error.data_ptr(), self._stream()
-        q = (qkv.data_ptr(), self._row_stride(qkv), heads, kv)
-        pages = (cache.k.data_ptr(), cache.v.data_ptr())
         if batch.is_decode and lse is None:
             self._ok(lib.krk_shared_single(out.data_ptr(), None, None, 0, self._cluster_splits(-(-per // 16) * kv * batch.n_seqs, True), 0, *q,
                                            *self._segments(batch, cache, None), *pages, cache.k.shape[0], 0, scale, error, stream), "single-token attention")
-        elif self._by_tcgen05(qkv, D) and batch.max_q_len * per >= 128 and self.use_tcgen05_attention:
+        elif self._by_tcgen05(D, address, stride) and batch.max_q_len * per >= 128 and self.use_tcgen05_attention:
             if lse is None:
-                lse = torch.empty(rows * heads, dtype=torch.float32, device=qkv.device)
+                lse = self._scratch(rows * heads)
             self._ok(self._attn_lib(D).krk_attention_prefill_lse(
                 out.data_ptr(), lse.data_ptr(), *q, batch.seq_slot.data_ptr(), batch.seq_start.data_ptr(), batch.seq_qlen.data_ptr(), batch.cu_q.data_ptr(),
                 cache.table.data_ptr(), cache.width, *pages, cache.k.shape[0], batch.n_seqs, batch.max_q_len, rows, scale, error, stream), "prompt attention")
@@ -259,41 +261,40 @@ class CacheOps:
         (None: all). Rows that the step itself brings start from its own weights; rows behind a sequence's last stay as they are.
         ``positions`` (int32, the same shape) take the step's rows' positions in the sequence, which lie ``batch.seq_shift`` behind their
         rows where keys were evicted. ``out_scores`` takes the sums in place of ``scores``."""
-        self._check_step("scored attention", qkv, heads, kv_in_row, head_dim, batch, cache)
+        address, stride, k, v = self._check_step("scored attention", qkv, heads, kv_in_row, head_dim, batch, cache)
         out_scores = scores if out_scores is None else out_scores
         self._check_scores("scored attention", cache, (("scores", scores, torch.float32), ("positions", positions, torch.int32),
                                                        ("out_scores", None if out_scores is scores else out_scores, torch.float32)))
         if observe is not None and observe < 1:
             raise KernelError(f"scored attention: at least one query a sequence is observed, got {observe}")
-        lib, rows, kv, per, D = self._parts_lib(head_dim), qkv.shape[0], cache.kv_heads, heads // cache.kv_heads, head_dim
-        out = torch.empty((rows, heads * D), dtype=qkv.dtype, device=qkv.device)
+        lib, rows, kv, per, D = self._parts_lib(head_dim), batch.n_rows, cache.kv_heads, heads // cache.kv_heads, head_dim
+        out = qkv.new_empty((rows, heads * D))
         if rows == 0:
             return out
         scale, stream, error, capacity = float(scale), self._stream(), self.error.data_ptr(), scores.shape[2]
         counts = (scores.data_ptr(), out_scores.data_ptr(), _ptr(positions), _ptr(getattr(batch, "seq_shift", None)), capacity)
         segments = self._segments(batch, cache, None)
-        q = (qkv.data_ptr(), self._row_stride(qkv), heads, kv)
-        pages = (cache.k.data_ptr(), cache.v.data_ptr())
-        by_mma = self._by_mma(qkv, cache, D)
+        q, pages = (address, stride, heads, kv), (k, v)
+        by_mma = self._by_mma(qkv.dtype, D, address, stride, k, v)
         if by_mma and batch.is_decode and per <= 16:
-            raw = torch.empty(rows * heads * capacity, dtype=torch.float32, device=qkv.device)
+            raw = self._scratch(rows * heads * capacity)
             self._ok(lib.krk_scored_single(out.data_ptr(), raw.data_ptr(), *counts, self._cluster_splits(kv * rows, True), *q, *segments, *pages,
                                            cache.k.shape[0], scale, error, stream), "scored attention")
             return out
         # the output with every row's log sum, then the weights by these
-        lse = torch.empty(rows * heads, dtype=torch.float32, device=qkv.device)
+        lse = self._scratch(rows * heads)
         page_blocks = max(1, min(cache.width, -(-888 // (kv * batch.n_seqs))))
         seen = min(batch.max_q_len, observe or batch.max_q_len)
         if not by_mma:
             parts = self._splits(-(-batch.max_q_len * per // 64) * kv * batch.n_seqs, 444)
-            scratch = torch.empty(parts * rows * heads * (D + 2), dtype=torch.float32, device=qkv.device)
+            scratch = self._scratch(parts * rows * heads * (D + 2))
             o = scratch.data_ptr()
             self.launches += 2
             self._ok(lib.krk_attention_in_parts(out.data_ptr(), lse.data_ptr(), o, o + 4 * parts * rows * heads * D, rows, 0, parts, *counts, int(observe or 0),
                                                 page_blocks, seen, *q, *segments, *pages, 0, batch.max_q_len, scale, _code(qkv.dtype), stream), "scored attention")
             return out
-        self._whole_attention(out, lse, qkv, heads, D, batch, cache, scale)
-        if self._by_tcgen05(qkv, D) and not batch.is_decode and per <= 64:
+        self._whole_attention(out, lse, q, D, batch, cache, pages, scale)
+        if self._by_tcgen05(D, address, stride) and not batch.is_decode and per <= 64:
             longest = cache.width * PAGE if torch.cuda.is_current_stream_capturing() else batch.max_kv_len  # a captured step's sequences grow
             self._ok(lib.krk_key_weights_tcgen05(*counts, lse.data_ptr(), int(observe or 0), *q, *segments, pages[0], cache.k.shape[0], rows, seen, longest,
                                                  scale, error, stream), "weights of keys")
@@ -352,7 +353,7 @@ class CacheOps:
         # as many sequences at once as the arguments and the scratch take
         moves = max(0, min(keep, longest - keep))
         most = max(1, min(lib.krk_evict_max_seqs(), n, self.EVICT_SCRATCH_BYTES // max(1, runs * heads * moves * 8)))
-        lists = torch.empty(runs * most * heads * (2 * moves + 1), dtype=torch.int32, device=k.device)
+        lists = self._scratch(runs * most * heads * (2 * moves + 1))
         head = (k.data_ptr(), None if same else v.data_ptr(), k.stride(0) * size, v.stride(0) * size, dim * size, v.shape[4] * size, heads, runs,
                 table.data_ptr(), width, scores.data_ptr(), positions.data_ptr(), out_scores.data_ptr(), out_positions.data_ptr(), scores.stride(0), capacity)
         moves_at = lists.data_ptr()
