@@ -11,7 +11,7 @@
 //
 // What bounds it is the finding: passes of one block over a head's rows in shared memory, with barriers between. The lines by bins of the numbers'
 // range (two passes mostly) instead of a bisection of their bits: 58.8 to 26 us. 16 sequences of 1,088 rows to 1,024, 8 layers of 8 heads
-// of 128 (1,024 heads, 82 MB): 27 us, of which the bytes would take 12.5. One prompt of 16,300 rows to 2,048 (64 heads, 129 MB): 26 us for the lines and
+// of 128 (1,024 heads, 82 MB): 27 us, of which the bytes would take 12.5. One prompt of 16,300 rows to 2,048 (64 heads, 129 MB): 22 us for the lines and
 // 27 for the moves.
 #include "common.cuh"
 
@@ -428,15 +428,18 @@ KRK_API int krk_evict_keys(void* k, void* v, long long k_run_bytes, long long v_
                            moves, n_moves, seq_start, row_pos, seq_shift, move_here};
   int longest = 0;
   for (int i = 0; i < n_seqs; ++i) longest = lengths[i] > longest ? lengths[i] : longest;
-  // Few rows: few threads, whose sums and barriers cost more than the rows do. Rows whose keys do not fit shared memory are read again.
-  static unsigned long long allowed[3] = {0, 0, 0};
+  // Few rows: few threads, whose sums and barriers cost more than the rows do. Many rows of few heads: as many threads as a block has (64 heads of 16,300 rows
+  // 58.4 us by 512 threads and 54.3 by 1,024, 128 of 8,000 54.3 and 50.2; 256 of 8,000 85.0 and 89.1). Rows whose keys do not fit shared memory are
+  // read again.
+  static unsigned long long allowed[4] = {0, 0, 0, 0};
   constexpr size_t MOST = 190 * 1024;
   auto choose = [&](auto* kern, int threads, int staged) {
     const size_t smem = (size_t)staged * 8 + ((size_t)longest + 31) / 32 * 4;
-    const cudaError_t e = smem > MOST ? cudaErrorInvalidValue : allow_shared(kern, MOST, allowed + (threads > 128) + (threads > 512));
+    const cudaError_t e = smem > MOST ? cudaErrorInvalidValue : allow_shared(kern, MOST, allowed + (threads > 128) + (threads > 512) + (threads > 512 && staged));
     return e != cudaSuccess ? e : launch_pdl(kern, dim3((unsigned)heads), dim3(threads), smem, stream, args, seqs, pools, staged);
   };
   cudaError_t e = longest <= 2048    ? choose(choose_rows_kernel<128, 512, true>, 128, longest)
+                  : heads <= 148 && longest > 6000 && longest <= 23000 ? choose(choose_rows_kernel<1024, 2048, true>, 1024, longest)
                   : longest <= 23000 ? choose(choose_rows_kernel<512, 2048, true>, 512, longest)
                                      : choose(choose_rows_kernel<1024, 2048, false>, 1024, 0);
   if (e != cudaSuccess || max_moves == 0 || move_here) return (int)e;

@@ -411,6 +411,16 @@ def test_evict_keys_of_many_rows_and_sequences(ops):
     assert torch.equal(k, want[0]) and torch.equal(scores, want[2]) and torch.equal(positions, want[3])
 
 
+@pytest.mark.parametrize("L,keep,recent", [(6001, 40, 7), (9000, 5000, 1), (23000, 2048, 2048), (23001, 64, 3)])
+def test_evict_keys_of_few_long_heads(ops, L, keep, recent):
+    """On both sides of the lengths at which the blocks change."""
+    k, v, table, scores, positions = evict_case(BF16, 1, 2, 4, -(-L // PAGE), L, n_slots=1, ties=False)
+    want = exact_evict(k, v, table, [0], [L], scores, positions, keep, recent)
+    assert ops.evict_keys(k, v, table, [0], [L], scores, positions, keep, recent) == [keep]
+    for got, ref in zip((k, v, scores, positions), want):
+        assert torch.equal(got, ref)
+
+
 def test_evict_keys_moves_the_step_on(ops):
     """A single-token step of the evicted slots: rows fall back, shifts take what was given up."""
     k, v, table, scores, positions = evict_case(BF16, 1, 2, 16, 4, 3)
