@@ -248,7 +248,8 @@ def test_scored_attention(ops, dtype, shape, case):
     ops.check()
 
 
-@pytest.mark.parametrize("held,brings,observe", [([3000, 4090, 2], [1, 1, 1], None), ([0], [2100], None), ([0, 0], [1300, 700], 64), ([900], [1100], 200)])
+@pytest.mark.parametrize("held,brings,observe", [([3000, 4090, 2], [1, 1, 1], None), ([0], [2100], None), ([0, 0], [1300, 700], 64), ([900], [1100], 200),
+                                               ([0, 0, 0], [1300, 40, 1100], None), ([0, 100], [1900, 130], None)])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_scored_attention_of_long_sequences(ops, held, brings, observe, dim):
     heads, kv = 12, 4
