@@ -34,8 +34,10 @@ JOIN_STEPS = 8
 
 def single_tokens_share(sizes, lengths, row_bytes: int) -> bool:
     """Whether a step of one token a sequence reads these groups' prefixes once. ``row_bytes``: of one position's keys and values in one layer."""
-    saved = sum((size - 1) * length for size, length in zip(sizes, lengths)) * row_bytes
-    return saved >= SHARE_BYTES * min(sum(sizes), 8)
+    saved = 0
+    for size, length in zip(sizes, lengths):
+        saved += (size - 1) * length
+    return saved * row_bytes >= SHARE_BYTES * min(sum(sizes), 8)
 
 
 def longer_steps_share(sizes, lengths, q_lens, per: int, kv_heads: int) -> bool:

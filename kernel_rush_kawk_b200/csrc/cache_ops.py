@@ -19,6 +19,7 @@ from .build import build_library
 F32, BF16 = 0, 1
 _P = c_void_p
 PAGE = 64
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # (the function around it costs as much again)
 
 
 def _code(dtype: torch.dtype) -> int:
@@ -119,7 +120,7 @@ class CacheOps:
             if t.get_device() != mine:
                 break
         else:
-            if torch.cuda.current_device() == mine:
+            if _current_device() == mine:
                 return
         raise KernelError(f"{what}: tensors on {', '.join(str(t.device) for t in tensors)}, device {torch.cuda.current_device()} current, "
                           f"kernels on {self.error.device}")
@@ -306,7 +307,7 @@ class CacheOps:
     # -- eviction ----------------------------------------------------------------------------
     def evict_keys(self, k, v, table, slots, lengths, scores, positions, keep, recent, out_scores=None, out_positions=None, batch=None):
         """Give up all but ``keep`` rows of every head of these cache slots (host lists ``slots`` and ``lengths``, the rows that each holds),
-        in every layer run at once: ``k`` and ``v`` [runs, pages, kv heads, 64, head size], ``table`` [slots, pages of a slot], ``scores`` and
+        in every layer run at once (no two of the slots share a page): ``k`` and ``v`` [runs, pages, kv heads, 64, head size], ``table`` [slots, pages of a slot], ``scores`` and
         ``positions`` [runs, slots, kv heads, rows]. The ``recent`` rows of highest position stay, of the others those of largest score
         (ties: the lowest row; a NaN counts as the largest). What stays from row ``keep`` on moves, in place, into the rows below it that
         are given up, in ascending order of both; scores and positions move along, or go to ``out_scores`` and ``out_positions`` (rows from
