@@ -11,8 +11,8 @@ from .allocator import CacheError
 class KeyEviction:
     """Every kv head of every layer holds at most ``keep + every`` keys of a sequence between its steps: a sequence that holds so many
     falls back to ``keep`` before its next step, to its ``recent`` newest keys and those that received most weight. A step may bring any
-    number of tokens, and its queries see all keys that were held before it (one that is cut into passes falls back between them, too). ``observe``: of a step's queries of a sequence, the last
-    so many count (None: all)."""
+    number of tokens, and its queries see all keys that were held before it (one that is cut into passes falls back between them, too).
+    ``observe``: of a step's queries of a sequence, the last so many count (None: all)."""
 
     keep: int
     recent: int = 0

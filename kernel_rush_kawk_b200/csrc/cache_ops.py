@@ -307,8 +307,8 @@ class CacheOps:
     # -- eviction ----------------------------------------------------------------------------
     def evict_keys(self, k, v, table, slots, lengths, scores, positions, keep, recent, out_scores=None, out_positions=None, batch=None):
         """Give up all but ``keep`` rows of every head of these cache slots (host lists ``slots`` and ``lengths``, the rows that each holds),
-        in every layer run at once (no two of the slots share a page): ``k`` and ``v`` [runs, pages, kv heads, 64, head size], ``table`` [slots, pages of a slot], ``scores`` and
-        ``positions`` [runs, slots, kv heads, rows]. The ``recent`` rows of highest position stay, of the others those of largest score
+        in every layer run at once (no two of the slots share a page): ``k`` and ``v`` [runs, pages, kv heads, 64, head size], ``table``
+        [slots, pages of a slot], ``scores`` and ``positions`` [runs, slots, kv heads, rows]. The ``recent`` rows of highest position stay, of the others those of largest score
         (ties: the lowest row; a NaN counts as the largest). What stays from row ``keep`` on moves, in place, into the rows below it that
         are given up, in ascending order of both; scores and positions move along, or go to ``out_scores`` and ``out_positions`` (rows from
         ``keep`` on are not written). A slot that holds no more than ``keep`` rows stays as it is. ``batch``: the description of a

@@ -21,7 +21,7 @@ struct Segments {
 };
 
 // The rows and keys of one unit of work: rows row0 .. row0 + n_tok - 1 of the step (times the G heads of a kv head), keys
-// key_lo .. key_hi - 1 of slot `slot`; token t sees keys up to start + t (all of them where `causal` is off).
+// key_lo .. key_hi - 1 of slot `slot`; token t sees keys up to start + t (of a prefix all: its start lies behind every key).
 struct Unit {
   int row0, n_tok, key_lo, key_hi, slot, start;
 };
