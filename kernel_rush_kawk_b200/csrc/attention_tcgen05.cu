@@ -67,7 +67,7 @@ constexpr int D = KRK_HEAD_DIM;
 constexpr int ROWS = 128;              // query rows per tile
 constexpr int KEYS = 128;              // keys per block iteration: two pages
 constexpr int DB = D / 64;             // 64-wide blocks of the head dimension
-constexpr int THREADS = 384;           // 8 softmax warps, the warps that issue the MMAs, load and allocate, one idle
+constexpr int THREADS = 384;           // 8 softmax warps, the warps that issue the MMAs, load and allocate, one idle (LSE: two that look at values)
 constexpr uint32_t SUB = 128 * 128;    // bytes of a [128 rows x 64 bf16] swizzled sub-tile
 constexpr uint32_t TILE_BYTES = DB * SUB;  // a Q, K or V tile
 constexpr uint32_t TMEM_COLS = 512;
@@ -76,7 +76,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int PAGE_IDS = 1024;         // page-table entries a block keeps in shared memory (64 K keys)
 constexpr float RESCALE_STEP = 8.f;    // in log2 units: the reference maximum moves when outgrown by 2^8
 
-enum Bar { K_FULL = 0, V_FULL = 2, K_FREE = 4, V_FREE = 6, S_FULL = 8, P_READY = 10, O_DONE = 12, Q_FULL = 14, LAST_V = 15, V_CLEAN = 16, N_BARS = 18 };
+enum Bar { K_FULL = 0, V_FULL = 2, K_FREE = 4, V_FREE = 6, S_FULL = 8, P_READY = 10, O_DONE = 12, Q_FULL = 14, V_RAW = 15, V_HALF = 17, N_BARS = 19 };
 
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
@@ -119,8 +119,54 @@ struct Extras {
   const bf16* gate;
   int gate_stride, gate_mode;  // 0: none, 1: a column per head, 2: a column per element
   int out_stride;
-  float* lse;  // LSE: [rows][HQ], log2 of the sum of the row's 2^score; there values behind the sequence's end, which may be anything, count as zero
+  // LSE: [rows][HQ], log2 of the sum of the row's 2^score. There values that a row does not see may be anything (zero times infinity is not
+  // zero): those behind the sequence's end count as zero, and of the blocks of keys that some row sees in part those that are no
+  // numbers are taken out before P V and added to the rows that do see them when these are written.
+  float* lse;
+  const bf16* v;  // LSE: the pages of values, for these
 };
+
+// The halves of a word that hold an infinity or a NaN, by their highest bits: an exponent of ones carries into the sign's place.
+__device__ __forceinline__ uint32_t not_finite(uint32_t two) { return ((two & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+
+// LSE: the values that were taken out, to the rows of this block that see them, which have been written (a weight is above zero, and so is a sum of
+// weights: what such a value is, the sum is). `odd`: the blocks that held some. What the block is about is asked for again here: kept
+// through the walk it cost the softmax registers.
+__device__ __forceinline__ void add_odd_values(bf16* __restrict__ out, int rows, int HQ, int HKV, const int* seq_slot, const int* seq_start, const int* seq_qlen,
+                                               const int* cu_q, const int* table, int width, const bf16* v_cache, int odd) {
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // a thread that stored a tile: it is there
+  __syncthreads();
+  int seq = blockIdx.y, block = blockIdx.x;
+  asm volatile("" : "+r"(seq), "+r"(block));
+  const int G = HQ / HKV, kh = block % HKV, pair_row = ((int)gridDim.x / HKV - 1 - block / HKV) * 2 * rows;
+  const int start = seq_start[seq], slot = seq_slot[seq], row0 = cu_q[seq], n_rows = min(seq_qlen[seq] * G - pair_row, 2 * rows);
+  const int key0 = (start + pair_row / G + 1) / KEYS * KEYS;
+#pragma unroll 1
+  for (int x = threadIdx.x; x < n_rows * (D / 8); x += THREADS) {
+    const int R = pair_row + x / (D / 8), c = x % (D / 8) * 8;
+    bool any = false;
+    float add[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int key = key0; key <= start + R / G; ++key) {
+      if (!(odd >> ((key - key0) / KEYS) & 1)) continue;
+      const size_t page = table[(size_t)slot * width + key / KRK_PAGE];
+      const uint4 piece = *reinterpret_cast<const uint4*>(v_cache + ((page * HKV + kh) * KRK_PAGE + key % KRK_PAGE) * D + c);
+      const uint32_t two[4] = {piece.x, piece.y, piece.z, piece.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t f = not_finite(two[e]);
+        any |= f != 0;
+        if (f & 0x8000u) add[2 * e] += __uint_as_float(two[e] << 16);
+        if (f >> 31) add[2 * e + 1] += __uint_as_float(two[e] & 0xffff0000u);
+      }
+    }
+    if (!any) continue;
+    bf16* to = out + (size_t)(row0 + R / G) * HQ * D + (size_t)(kh * G + R % G) * D + c;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (add[e] != 0.f) to[e] = __float2bfloat16_rn(__bfloat162float(to[e]) + add[e]);
+  }
+}
 
 template <bool WIDE, int SHAPE, bool LSE>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -139,6 +185,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
   int* pages_s = reinterpret_cast<int*>(tmem_slot + 2);  // [PAGE_IDS] the block's page-table entries, from page 2 * j_lo on
   volatile int* gave_up = pages_s + PAGE_IDS;  // [2] per tile
+  int* odd_blocks = pages_s + PAGE_IDS + 2;    // LSE: a bit for each block from `look` on that held values that are no numbers
 
   // blockIdx.x counts (row pair, kv head) with the pair as the slow index, descending: blocks start in
   // launch order, so the pairs with the most key blocks, of every kv head, run first and the short ones
@@ -158,8 +205,9 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   const int j_lo = r0.lo;                                   // tile 0 exists and starts no later than tile 1
   const int j_hi = r1.lo <= r1.hi ? max(r0.hi, r1.hi) : r0.hi;
   const int n = j_hi - j_lo + 1;
-  // LSE: the places of the block's last keys that lie behind the sequence's end, from this one on (KEYS: none)
-  const int clean_from = LSE ? min(KEYS, start + q_len - j_hi * KEYS) : KEYS;
+  // LSE: the blocks from this one on hold keys that some row does not see, three at most (a tile has at most KEYS tokens); their
+  // values arrive at barriers of their own, and V_FULL is completed by the warps that have looked at them
+  const int look = LSE ? max(0, (start + pair_row / G + 1) / KEYS - j_lo) : n;
 
   // TMA loads: the first ones by the issuer (warp 8, lane 0) before the block's first barrier, the rest by the loader
   auto load_tile = [&](unsigned char* dst, const CUtensorMap* map, uint64_t* bar, int i) {
@@ -175,7 +223,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     }
   };
   auto load_k = [&](int i) { load_tile(k_s + (i & 1) * TILE_BYTES, &map_k, bars + K_FULL + (i & 1), i); };
-  auto load_v = [&](int i) { load_tile(v_s + (i & 1) * TILE_BYTES, &map_v, bars + V_FULL + (i & 1), i); };
+  auto load_v = [&](int i) { load_tile(v_s + (i & 1) * TILE_BYTES, &map_v, bars + (LSE && i >= look ? V_RAW : V_FULL) + (i & 1), i); };
 
   if (warp == 9 && lane < 4) {
     const CUtensorMap* map = lane == 0 ? &map_k : lane == 1 ? &map_v : lane == 2 ? &map_q : &map_o;
@@ -197,6 +245,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
       for (int i = 0; i < N_BARS; ++i) mbar_init(bars + i, (i == P_READY || i == P_READY + 1) ? ROWS / 32 : 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       gave_up[0] = gave_up[1] = 0;
+      if (LSE) odd_blocks[0] = 0;
       if (q_by_tma) {
         // a query tile is a box of whole tokens x G heads x 64 dims per 64-wide block of the head: its rows land in
         // (token, group member) order, which is the tile's row order
@@ -323,7 +372,6 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             if (!wait(P_READY + t, (j - rng[t].lo) & 1)) { give_up(8); break; }
             if (!v_ready) {
               if (!wait(V_FULL + b, (i >> 1) & 1)) { give_up(9); break; }
-              if (LSE && clean_from < KEYS && i == n - 1 && !wait(V_CLEAN, 0)) { give_up(9); break; }
               v_ready = true;
             }
             tc_fence_after();
@@ -352,7 +400,6 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         if (i + 1 < n) {  // V of the next block goes where block i - 1's was
           if (i >= 1 && !mbar_wait(bars + V_FREE + ((i + 1) & 1), ((i - 1) >> 1) & 1)) { atomicExch(error, 7); break; }
           load_v(i + 1);
-          if (LSE && i + 2 == n) mbar_arrive(bars + LAST_V);
         }
         if (i + 2 < n) {  // K of block i + 2 goes where block i's was
           if (!mbar_wait(bars + K_FREE + (i & 1), (i >> 1) & 1)) { atomicExch(error, 11); break; }
@@ -360,18 +407,49 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         }
       }
     }
-    } else if (LSE && warp == 11 && clean_from < KEYS) {
-      // The last values behind the sequence's end: zero times infinity is not zero. The stage's earlier values have been read when its last ones
-      // are asked for, so that the wait below is for these.
-      const int i = n - 1;
-      if (__all_sync(0xffffffffu, (n == 1 || mbar_wait(bars + LAST_V, 0)) && mbar_wait(bars + V_FULL + (i & 1), (i >> 1) & 1))) {
-        unsigned char* v = v_s + (i & 1) * TILE_BYTES;
-        const int pieces = max(1, (KEYS - clean_from) * 8);
-        for (int p = lane; p < DB * pieces; p += 32)
-          *reinterpret_cast<uint4*>(v + (p / pieces) * SUB + (size_t)clean_from * 128 + (p % pieces) * 16) = make_uint4(0, 0, 0, 0);
+    } else if (LSE) {
+      // ---- warps 10 and 11: the values of blocks that some row sees in part (see Extras), half of them each, while their scores are on their way ----
+      // The issuer waits for V_FULL either way: a wait of its own for these blocks, though never taken, cost it 2 us of a prompt of 4,001 tokens (32 heads over
+      // 8 of 128; 133.4 us like this, as without the look).
+      const int me = (warp - 10) * 32 + lane;
+      for (int i = look; i < n; ++i) {
+        const int b = i & 1;
+        if (!__all_sync(0xffffffffu, mbar_wait(bars + V_RAW + b, ((i - look) >> 1) & 1))) break;
+        uint4* v = reinterpret_cast<uint4*>(v_s + b * TILE_BYTES);  // eight pieces a key and 64-wide block of the head
+        const int held = min(KEYS, start + q_len - (j_lo + i) * KEYS);  // keys of the block that are the sequence's
+        // what is no number leaves a NaN in a sum of zeros
+        const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
+        __nv_bfloat162 sums[4] = {zero, zero, zero, zero};
+#pragma unroll
+        for (int h = 0; h < DB; ++h) {
+#pragma unroll 8
+          for (int p = me; p < held * 8; p += 64) {
+            const uint4 x = v[h * KEYS * 8 + p];
+            const __nv_bfloat162* two = reinterpret_cast<const __nv_bfloat162*>(&x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sums[e] = __hfma2(two[e], zero, sums[e]);
+          }
+          for (int p = held * 8 + me; p < KEYS * 8; p += 64) v[h * KEYS * 8 + p] = make_uint4(0, 0, 0, 0);
+        }
+        const __nv_bfloat162 all = __hadd2(__hadd2(sums[0], sums[1]), __hadd2(sums[2], sums[3]));
+        if (__any_sync(0xffffffffu, __hisnan(__low2bfloat16(all)) || __hisnan(__high2bfloat16(all)))) {
+          auto taken_out = [](uint32_t two) { return two & ~((not_finite(two) >> 15) * 0xffffu); };  // (one bit of a half, times all of its bits)
+#pragma unroll 1
+          for (int h = 0; h < DB; ++h)
+#pragma unroll 1
+            for (int p = me; p < held * 8; p += 64) {
+              const uint4 x = v[h * KEYS * 8 + p];
+              v[h * KEYS * 8 + p] = make_uint4(taken_out(x.x), taken_out(x.y), taken_out(x.z), taken_out(x.w));
+            }
+          if (lane == 0) atomicOr(odd_blocks, 1 << (i - look));
+        }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bars + V_CLEAN);
+        if (warp == 10 && lane == 0) mbar_arrive(bars + V_HALF + b);
+        if (warp == 11) {  // when both halves are done
+          if (!__all_sync(0xffffffffu, mbar_wait(bars + V_HALF + b, ((i - look) >> 1) & 1))) break;
+          if (lane == 0) mbar_arrive(bars + V_FULL + b);
+        }
       }
     }
   } else {
@@ -628,6 +706,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (LSE)
+    if (odd_blocks[0]) add_odd_values(out, rows, HQ, HKV, seq_slot, seq_start, seq_qlen, cu_q, table, width, ex.v, odd_blocks[0]);
   if (warp == 8) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
@@ -709,6 +789,7 @@ KRK_API int krk_attention_prefill_lse(void* out, float* lse, const void* qkv, in
   Extras ex = {};
   ex.out_stride = HQ * D;
   ex.lse = lse;
+  ex.v = (const bf16*)v_cache;
   return launch_tcgen05<false, 0, true>((bf16*)out, (const bf16*)qkv, q_stride, HQ, HKV, seq_slot, seq_start, seq_qlen, cu_q, table, width,
                                         k_cache, v_cache, n_pages, n_seqs, max_q_len, total_rows, scale, 0, error, ex, stream);
 }

@@ -1,0 +1,68 @@
+"""The cache's operators where their paths meet (cache_ops_helpers.py has the definitions in 64 bits): values that are no numbers in the prompt
+attention with log sums."""
+
+import pytest
+import torch
+
+from cache_ops_helpers import PAGE, exact_attention, make_step
+from test_cache_ops_gpu import BF16, DEVICE, F32, groups, ops, within  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def scores_of(cache, kv):
+    return torch.zeros((cache.table.shape[0], kv, cache.width * PAGE), device=DEVICE)
+
+
+@pytest.mark.parametrize("dtype,shape", [(F32, (6, 2, 64)), (BF16, (6, 2, 48)), (BF16, (6, 2, 64)), (BF16, (6, 2, 128)), (BF16, (2, 2, 128)), (BF16, (40, 2, 64)),
+                                         (BF16, (66, 2, 128))])
+@pytest.mark.parametrize("held", [0, 70, 191])
+@pytest.mark.parametrize("operator", ["alone", "scored"])
+def test_rows_before_values_that_are_no_numbers(ops, dtype, shape, held, operator):
+    """Prompts whose sequences are read each by itself, and counted ones: a value that is no number reaches the rows that see it, in its column, and
+    changes nothing else; a key that is none reaches the rows that see it. At the edges of pages, of blocks of 128 keys and of tiles."""
+    heads, kv, dim = shape
+    starts, brings = [5, held], [130, 400]
+    qkv, batch, cache = make_step(DEVICE, dtype, heads, kv, dim, starts, brings, 3 * held + dim)
+    assert brings[0] * (heads // kv) >= 128
+
+    def call():
+        if operator == "alone":
+            return ops.shared_prefix_attention(qkv, heads, kv, dim, batch, cache, 0.1, groups([2], [0])), None
+        scores = scores_of(cache, kv)
+        return ops.scored_attention(qkv, heads, kv, dim, batch, cache, 0.1, scores), scores
+
+    exact, off, _, _ = exact_attention(qkv, heads, kv, dim, batch, cache, 0.1)
+    clean, sums = call()
+    within(clean, exact, off, "without them")
+    inf, nan = float("inf"), float("nan")
+    clean_v, clean_k = cache.v.clone(), cache.k.clone()
+    column = heads * dim // 2 + 3  # of the second kv head's first query head
+    per_half = heads // 2 * dim
+    for plant in [((33, inf),), ((0, nan),), ((399, -inf),), ((127, inf), (128, -inf)), ((200, inf), (370, nan)), ((63, -inf), (64, -inf))]:
+        for token, bad in plant:
+            at = held + token
+            cache.v[cache.table[batch.slots[1], at // PAGE], 1, at % PAGE, 3] = bad
+        got, got_sums = call()
+        want = clean.clone()
+        # a finite column that holds what is no number from the token on, for every query head of the second kv head
+        columns = torch.arange(column, heads * dim, dim, device=DEVICE)
+        for token, bad in plant:
+            want[brings[0] + token:, columns] += bad
+        where = torch.isfinite(want)
+        within(got[where], exact[where], off[where], f"{plant}: what does not see them")
+        assert torch.equal(torch.isnan(got[~where]), torch.isnan(want[~where])), f"{plant}: what does"
+        infinite = torch.isinf(want)
+        assert torch.equal(got[infinite], want[infinite]), f"{plant}: infinities keep their signs"
+        if sums is not None:
+            assert torch.equal(got_sums, sums), f"{plant}: weights depend on no value"
+        cache.v.copy_(clean_v)
+    for token, bad in [(33, nan), (128, inf), (399, -inf)]:
+        at = held + token
+        cache.k[cache.table[batch.slots[1], at // PAGE], 0, at % PAGE] = bad
+        got, _ = call()
+        first = brings[0] + token
+        within(got[:first], exact[:first], off[:first], "rows before the key")
+        within(got[first:, per_half:], exact[first:, per_half:], off[first:, per_half:], "the other kv head")
+        cache.k.copy_(clean_k)
+    ops.check()
