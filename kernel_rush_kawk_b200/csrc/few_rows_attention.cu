@@ -511,7 +511,13 @@ int launch_few_rows(bf16* out, const Parts& parts, int part0, int n_join, const 
   const long long row_tiles = ((long long)max_rows * G + Rows::TILE - 1) / Rows::TILE;
   const int units = PREFIX ? seg.n_groups : seg.n_seqs;
   if (row_tiles * HKV > 65535 || units > 65535) return -3;
-  const int splits_in_cluster = PREFIX ? 1 : n_splits, inbox_rows = G < Rows::TILE ? G : Rows::TILE;
+  const int inbox_rows = G < Rows::TILE ? G : Rows::TILE;
+  // A cluster's parts meet beside the ring of pages: of large heads fewer, where not all fit (pages by cp.async, which take four places: heads of 240 and
+  // 14 or more of them a kv head in eight parts would take 236 KB or more).
+  constexpr size_t MOST = 227 * 1024;
+  if (!PREFIX)
+    while (n_splits > 1 && Layout(TMA_PAGES ? 2 : 2 * CP_STAGES, n_splits, inbox_rows).total + 1024 > MOST) n_splits /= 2;
+  const int splits_in_cluster = PREFIX ? 1 : n_splits;
   const long long blocks = row_tiles * HKV * units * n_splits;
   CUtensorMap map_k = {}, map_v = {};
   int in_ring;
@@ -529,10 +535,10 @@ int launch_few_rows(bf16* out, const Parts& parts, int part0, int n_join, const 
     in_ring = 2 * CP_STAGES;
   }
   const size_t smem = Layout(in_ring, splits_in_cluster, inbox_rows).total + 1024;
-  if (smem > 227 * 1024) return -2;
+  if (smem > MOST) return -2;
   auto kern = few_rows_kernel<TMA_PAGES, PREFIX, SUMS, Rows>;
   static unsigned long long allowed = 0;
-  cudaError_t e = allow_shared(kern, 227 * 1024, &allowed);
+  cudaError_t e = allow_shared(kern, MOST, &allowed);
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)n_splits, (unsigned)(row_tiles * HKV), (unsigned)units);

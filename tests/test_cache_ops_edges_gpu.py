@@ -1,5 +1,7 @@
 """The cache's operators where their paths meet (cache_ops_helpers.py has the definitions in 64 bits): values that are no numbers in the prompt
-attention with log sums."""
+attention with log sums, head sizes whose splits fill shared memory."""
+
+import math
 
 import pytest
 import torch
@@ -65,4 +67,25 @@ def test_rows_before_values_that_are_no_numbers(ops, dtype, shape, held, operato
         within(got[:first], exact[:first], off[:first], "rows before the key")
         within(got[first:, per_half:], exact[first:, per_half:], off[first:, per_half:], "the other kv head")
         cache.k.copy_(clean_k)
+    ops.check()
+
+
+@pytest.mark.parametrize("shape", [(16, 1, 224), (16, 1, 240), (24, 1, 240), (28, 2, 240)])
+@pytest.mark.parametrize("n_seqs", [1, 5, 70])
+def test_single_tokens_of_many_large_heads(ops, shape, n_seqs, monkeypatch):
+    """Where a cluster's parts and a block's pages would not fit shared memory together, fewer blocks share a sequence's keys."""
+    from kernel_rush_kawk_b200.cache import prefix
+
+    heads, kv, dim = shape
+    held = [130 + 7 * i for i in range(n_seqs)]
+    qkv, batch, cache = make_step(DEVICE, BF16, heads, kv, dim, held, [1] * n_seqs, n_seqs)
+    scale = 1 / math.sqrt(dim)
+    want, off, weights, weights_off = exact_attention(qkv, heads, kv, dim, batch, cache, scale)
+    scores = scores_of(cache, kv)
+    within(ops.scored_attention(qkv, heads, kv, dim, batch, cache, scale, scores), want, off, "counted")
+    for i, (slot, n) in enumerate(zip(batch.slots, held)):
+        within(scores[slot, :, :n + 1], weights[i], weights_off[i], f"weights of sequence {i}")
+    within(ops.shared_prefix_attention(qkv, heads, kv, dim, batch, cache, scale, groups([n_seqs], [0])), want, off, "no prefix, shared")
+    monkeypatch.setattr(prefix, "SHARE_BYTES", 1 << 60)
+    within(ops.shared_prefix_attention(qkv, heads, kv, dim, batch, cache, scale, groups([n_seqs], [0])), want, off, "each sequence by itself")
     ops.check()
