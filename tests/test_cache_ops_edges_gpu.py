@@ -1,5 +1,5 @@
 """The cache's operators where their paths meet (cache_ops_helpers.py has the definitions in 64 bits): values that are no numbers in the prompt
-attention with log sums, head sizes whose splits fill shared memory."""
+attention with log sums, head sizes whose splits fill shared memory, shares of more pages than the loading warp reads at once."""
 
 import math
 
@@ -88,4 +88,24 @@ def test_single_tokens_of_many_large_heads(ops, shape, n_seqs, monkeypatch):
     within(ops.shared_prefix_attention(qkv, heads, kv, dim, batch, cache, scale, groups([n_seqs], [0])), want, off, "no prefix, shared")
     monkeypatch.setattr(prefix, "SHARE_BYTES", 1 << 60)
     within(ops.shared_prefix_attention(qkv, heads, kv, dim, batch, cache, scale, groups([n_seqs], [0])), want, off, "each sequence by itself")
+    ops.check()
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(16, 8, 128), (32, 8, 64)])
+def test_shares_of_more_pages_than_the_loading_warp_reads_at_once(ops, heads, kv, dim, monkeypatch):
+    """Page numbers come 32 at a time: single tokens whose blocks have 31 to 36 pages each, of two blocks a sequence."""
+    from kernel_rush_kawk_b200.cache import prefix
+
+    lengths = [31 * 128, 32 * 128, 33 * 128, 4500, 63, 4095, 64 * 64 + 1, 70 * 64]
+    held = [lengths[i % len(lengths)] - 1 for i in range(24)]
+    assert ops._cluster_splits(kv * len(held), True) == 2
+    qkv, batch, cache = make_step(DEVICE, BF16, heads, kv, dim, held, [1] * len(held), 12)
+    scale = 1 / math.sqrt(dim)
+    want, off, weights, weights_off = exact_attention(qkv, heads, kv, dim, batch, cache, scale)
+    scores = scores_of(cache, kv)
+    within(ops.scored_attention(qkv, heads, kv, dim, batch, cache, scale, scores), want, off, "counted")
+    for i, (slot, n) in enumerate(zip(batch.slots, held)):
+        within(scores[slot, :, :n + 1], weights[i], weights_off[i], f"weights of sequence {i}")
+    monkeypatch.setattr(prefix, "SHARE_BYTES", 1 << 60)
+    within(ops.shared_prefix_attention(qkv, heads, kv, dim, batch, cache, scale, groups([len(held)], [0])), want, off, "each sequence by itself")
     ops.check()
