@@ -159,7 +159,7 @@ class Engine:
     def _ensure_cache(self, prompt_lens, max_new_tokens: int) -> None:
         """Without a fixed ``max_tokens`` the cache grows to what a call needs, as the
         reference rebuilds its plan for a new shape (engine/engine.py:562-588)."""
-        pages = sum(pages_needed(n, max_new_tokens) for n in prompt_lens)
+        pages = sum(pages_needed(n, max_new_tokens, self.eviction, self.max_step_rows) for n in prompt_lens)
         slots = max(self.max_slots, min(len(prompt_lens), 1024))
         if self.cache is not None and (self.max_tokens is not None or (
                 self.cache.n_pages >= pages and self.cache.max_slots >= min(len(prompt_lens), slots))):

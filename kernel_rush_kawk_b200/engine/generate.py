@@ -32,6 +32,7 @@ from __future__ import annotations
 import time
 from dataclasses import dataclass, field
 
+from ..cache.eviction import KeyEviction
 from ..cache.store import PAGE
 from ..sampling.sampler import SamplingParams
 from .step import StepEntry
@@ -77,17 +78,28 @@ class GenerationStats:
                 f"{self.decode_ms_per_step:.3f} ms ({self.decode_tokens_per_s:.0f} tokens/s)")
 
 
-def pages_needed(prompt_len: int, max_new_tokens: int) -> int:
-    """Pages a sequence may come to hold: the last generated token is never fed back."""
-    return -(-(prompt_len + max(max_new_tokens - 1, 0)) // PAGE)
+def rows_held(prompt_len: int, max_new_tokens: int, eviction: KeyEviction | None = None, pass_tokens: int | None = None) -> int:
+    """The most rows of the cache that a sequence comes to hold: the last generated token is never fed back. Where keys are evicted, it holds fewer than
+    ``keep + every`` before a step, and what the step brings beside them: a piece of its prompt, of ``pass_tokens`` at most, or one token."""
+    rows = prompt_len + max(max_new_tokens - 1, 0)
+    if eviction is None:
+        return rows
+    full = eviction.keep + eviction.every
+    return min(rows, max(full, prompt_len if pass_tokens is None else min(prompt_len, full - 1 + pass_tokens)))
 
 
-def split_into_batches(prompt_lens: list, max_new_tokens: int, max_slots: int, max_pages: int) -> list:
+def pages_needed(prompt_len: int, max_new_tokens: int, eviction: KeyEviction | None = None, pass_tokens: int | None = None) -> int:
+    """Pages that these rows take."""
+    return -(-rows_held(prompt_len, max_new_tokens, eviction, pass_tokens) // PAGE)
+
+
+def split_into_batches(prompt_lens: list, max_new_tokens: int, max_slots: int, max_pages: int, eviction: KeyEviction | None = None,
+                       pass_tokens: int | None = None) -> list:
     """Consecutive requests are grouped while slots and pages last. Returns lists of
     request indices. A request that cannot fit even alone raises ValueError."""
     batches, current, pages = [], [], 0
     for i, n in enumerate(prompt_lens):
-        need = pages_needed(n, max_new_tokens)
+        need = pages_needed(n, max_new_tokens, eviction, pass_tokens)
         if need > max_pages:
             raise ValueError(f"request {i} needs {need * PAGE} cached tokens; the cache holds {max_pages * PAGE}")
         if current and (len(current) >= max_slots or pages + need > max_pages):
@@ -251,7 +263,8 @@ class GenerationLoop:
                      stop_token_ids=(), max_batch: int | None = None, share_prefix: bool = False) -> list:
         """Run every request, batch after batch; returns each request's generated tokens."""
         max_slots = min(self.cache.max_slots, max_batch or self.cache.max_slots)
-        batches = split_into_batches([len(p) for p in prompts], max_new_tokens, max_slots, self.cache.n_pages)
+        batches = split_into_batches([len(p) for p in prompts], max_new_tokens, max_slots, self.cache.n_pages, self.cache.eviction,
+                                     getattr(self.stepper, "max_step_rows", None))
         results: list = [None] * len(prompts)
         for batch in batches:
             outs = [[] for _ in batch]
