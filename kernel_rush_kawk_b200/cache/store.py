@@ -117,7 +117,8 @@ class SequenceCache:
     count rounded up to whole pages. max_slots: live sequences. max_context: the
     longest sequence. step_tokens: the most tokens one sequence brings in one step;
     it sizes the rings of window groups. eviction: count the weight that keys receive, for ``evict``; a slot then has room for
-    what it may hold when a pass of ``pass_tokens`` new tokens has come (None: for the longest sequence)."""
+    what it may hold when a pass of ``pass_tokens`` new tokens has come (None: for the longest sequence), within the pool. Sums and positions
+    take eight bytes for each row of that room, slot and kv head: a smaller pass makes them smaller."""
 
     def __init__(self, needs: list, max_tokens: int, max_slots: int, max_context: int, device, dtype,
                  step_tokens: int = 2048, eviction: KeyEviction | None = None, pass_tokens: int | None = None):
@@ -129,8 +130,10 @@ class SequenceCache:
         self.step_tokens = int(step_tokens)
         self.n_pages = max(1, -(-int(max_tokens) // PAGE))
         rows = self.max_context
-        if eviction is not None and pass_tokens is not None:
-            rows = min(rows, eviction.keep + eviction.every - 1 + int(pass_tokens))
+        if eviction is not None:  # every row of a slot has a sum and a position beside it: no more rows than the pool has
+            rows = min(rows, self.n_pages * PAGE)
+            if pass_tokens is not None:
+                rows = min(rows, eviction.keep + eviction.every - 1 + int(pass_tokens))
         self.width = max(1, -(-rows // PAGE))
         self.slots = FreeList(self.max_slots, "cache slot")
         self.length = [0] * self.max_slots  # rows held

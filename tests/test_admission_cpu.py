@@ -77,3 +77,14 @@ def test_pools_are_as_large_as_what_the_sequences_hold(folders, rows):
     plenty = cpu_engine(folders, name, eviction=eviction, max_step_rows=rows, max_tokens=64 * 40)
     assert list(plenty.generate(prompts, 60)) == want
     assert cpu_engine(folders, name, eviction=eviction, max_step_rows=rows).generate_all(prompts, 60) == [[s[i] for s in want] for i in range(3)]
+
+
+def test_sums_and_positions_are_no_wider_than_the_pool(folders):
+    """A slot never holds more rows than the pool has pages for; a pass bounds it where that is less."""
+    prompts = prompts_for("tiny_a", [30, 20], 3)
+    engine = cpu_engine(folders, "tiny_a", eviction=KeyEviction(keep=50, recent=10, every=9))
+    list(engine.generate(prompts, 50))
+    assert engine.cache.n_pages == 2, "59 rows each at most"
+    assert engine.cache.view(0).scores.shape == engine.cache.view(0).positions.shape == (8, 2, 2 * PAGE)
+    engine = cpu_engine(folders, "tiny_a", eviction=KeyEviction(keep=50, recent=10, every=9), max_step_rows=60, max_tokens=64 * 40)
+    assert engine.cache.width == 2, "50 + 9 - 1 rows before a pass, and the pass"
