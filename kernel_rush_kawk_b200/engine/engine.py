@@ -35,7 +35,7 @@ from ..parts.base import KVNeed, StateNeed
 from ..sampling.sampler import Sampler, SamplingParams
 from ..weights.loader import checkpoint_shapes, read_checkpoint
 from ..weights.random_init import random_tensors
-from .generate import GenerationLoop, pages_needed
+from .generate import GenerationLoop, pages_needed, shared_pages
 from .model import Model, PartTree, Runtime
 from .step import StepEntry, Stepper
 
@@ -156,10 +156,11 @@ class Engine:
         self.stepper = Stepper(self.model, self.cache, self.ops, self.max_step_rows, self.use_cuda_graphs)
         self.loop = GenerationLoop(self.stepper, self.cache, self.sampler)
 
-    def _ensure_cache(self, prompt_lens, max_new_tokens: int) -> None:
+    def _ensure_cache(self, prompt_lens, max_new_tokens: int, pages: int | None = None) -> None:
         """Without a fixed ``max_tokens`` the cache grows to what a call needs, as the
-        reference rebuilds its plan for a new shape (engine/engine.py:562-588)."""
-        pages = sum(pages_needed(n, max_new_tokens, self.eviction, self.max_step_rows) for n in prompt_lens)
+        reference rebuilds its plan for a new shape (engine/engine.py:562-588). ``pages``: where that is not each prompt's own."""
+        if pages is None:
+            pages = sum(pages_needed(n, max_new_tokens, self.eviction, self.max_step_rows) for n in prompt_lens)
         slots = max(self.max_slots, min(len(prompt_lens), 1024))
         if self.cache is not None and (self.max_tokens is not None or (
                 self.cache.n_pages >= pages and self.cache.max_slots >= min(len(prompt_lens), slots))):
@@ -186,7 +187,8 @@ class Engine:
             if len(row) + max_new_tokens - 1 > self.max_context:
                 raise ValueError(f"a prompt of {len(row)} tokens plus {max_new_tokens} new ones exceeds "
                                  f"the context of {self.max_context}")
-        self._ensure_cache([len(p) for p in prompts], max_new_tokens)
+        self._ensure_cache([len(p) for p in prompts], max_new_tokens,
+                           shared_pages(prompts, max_new_tokens) if share_prefix else None)
         try:
             yield from self.loop.run_batch(prompts, max_new_tokens, SamplingParams(temperature, seed), stop_token_ids,
                                            share_prefix=share_prefix)
@@ -201,8 +203,10 @@ class Engine:
         if not prompts or max_new_tokens < 1:
             return [[] for _ in prompts]
         if self.max_tokens is None:  # no fixed size: room for the largest batch these requests can form
-            lens = sorted((len(p) for p in prompts), reverse=True)[:max_batch or self.max_slots]
-            self._ensure_cache(lens, max_new_tokens)
+            size = max_batch or self.max_slots
+            lens = sorted((len(p) for p in prompts), reverse=True)[:size]
+            self._ensure_cache(lens, max_new_tokens, max(shared_pages(prompts[i:i + size], max_new_tokens)
+                                                         for i in range(0, len(prompts), size)) if share_prefix else None)
         try:
             return self.loop.run_requests(prompts, max_new_tokens, SamplingParams(temperature, seed), stop_token_ids,
                                           max_batch, share_prefix)

@@ -93,25 +93,6 @@ def pages_needed(prompt_len: int, max_new_tokens: int, eviction: KeyEviction | N
     return -(-rows_held(prompt_len, max_new_tokens, eviction, pass_tokens) // PAGE)
 
 
-def split_into_batches(prompt_lens: list, max_new_tokens: int, max_slots: int, max_pages: int, eviction: KeyEviction | None = None,
-                       pass_tokens: int | None = None) -> list:
-    """Consecutive requests are grouped while slots and pages last. Returns lists of
-    request indices. A request that cannot fit even alone raises ValueError."""
-    batches, current, pages = [], [], 0
-    for i, n in enumerate(prompt_lens):
-        need = pages_needed(n, max_new_tokens, eviction, pass_tokens)
-        if need > max_pages:
-            raise ValueError(f"request {i} needs {need * PAGE} cached tokens; the cache holds {max_pages * PAGE}")
-        if current and (len(current) >= max_slots or pages + need > max_pages):
-            batches.append(current)
-            current, pages = [], 0
-        current.append(i)
-        pages += need
-    if current:
-        batches.append(current)
-    return batches
-
-
 def shared_prefixes(prompts: list) -> list:
     """Groups of prompts that begin alike: (request indices, tokens shared) with the shared tokens whole pages, at least one token of
     every prompt behind them, 0 for a prompt alone. Neighbours in the order of the prompts' tokens join a group while the pages that it
@@ -133,6 +114,39 @@ def shared_prefixes(prompts: list) -> list:
                 continue
         groups.append(([i], 0))
     return groups
+
+
+def shared_pages(prompts: list, max_new_tokens: int) -> int:
+    """Pages that a batch of prompts comes to hold which share what they begin with: a group's shared ones count once."""
+    pages = sum(pages_needed(len(p), max_new_tokens) for p in prompts)
+    return pages - sum((len(members) - 1) * (shared // PAGE) for members, shared in shared_prefixes(prompts))
+
+
+def split_into_batches(prompt_lens: list, max_new_tokens: int, max_slots: int, max_pages: int, eviction: KeyEviction | None = None,
+                       pass_tokens: int | None = None, prompts: list | None = None) -> list:
+    """Consecutive requests are grouped while slots and pages last. Returns lists of
+    request indices. A request that cannot fit even alone raises ValueError. ``prompts``: theirs, where a batch shares what they begin with."""
+    needs = [pages_needed(n, max_new_tokens, eviction, pass_tokens) for n in prompt_lens]
+    for i, need in enumerate(needs):
+        if need > max_pages:
+            raise ValueError(f"request {i} needs {need * PAGE} cached tokens; the cache holds {max_pages * PAGE}")
+    batches, first, n = [], 0, len(needs)
+    while first < n:
+        most = min(n - first, max(max_slots, 1))
+        size, pages = 1, needs[first]
+        while size < most and pages + needs[first + size] <= max_pages:
+            pages += needs[first + size]
+            size += 1
+        if prompts is not None and size < most:  # more fit where pages are shared: all that there are slots for, or as many as halving finds
+            low, high = size, most + 1
+            while high - low > 1:
+                middle = most if high > most else (low + high) // 2
+                fits = shared_pages(prompts[first:first + middle], max_new_tokens) <= max_pages
+                low, high = (middle, high) if fits else (low, middle)
+            size = low
+        batches.append(list(range(first, first + size)))
+        first += size
+    return batches
 
 
 class GenerationLoop:
@@ -264,7 +278,7 @@ class GenerationLoop:
         """Run every request, batch after batch; returns each request's generated tokens."""
         max_slots = min(self.cache.max_slots, max_batch or self.cache.max_slots)
         batches = split_into_batches([len(p) for p in prompts], max_new_tokens, max_slots, self.cache.n_pages, self.cache.eviction,
-                                     getattr(self.stepper, "max_step_rows", None))
+                                     getattr(self.stepper, "max_step_rows", None), prompts if share_prefix else None)
         results: list = [None] * len(prompts)
         for batch in batches:
             outs = [[] for _ in batch]

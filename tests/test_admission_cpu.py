@@ -10,7 +10,8 @@ from cache_engine_helpers import CacheTorchOps
 from helpers import prompts_for
 from kernel_rush_kawk_b200 import Engine, KeyEviction
 from kernel_rush_kawk_b200.cache import PAGE
-from kernel_rush_kawk_b200.engine.generate import pages_needed, rows_held, split_into_batches
+from kernel_rush_kawk_b200.engine.generate import pages_needed, rows_held, shared_pages, split_into_batches
+from test_generate_loop import make
 
 
 def cpu_engine(folders, name, **kw):
@@ -88,3 +89,69 @@ def test_sums_and_positions_are_no_wider_than_the_pool(folders):
     assert engine.cache.view(0).scores.shape == engine.cache.view(0).positions.shape == (8, 2, 2 * PAGE)
     engine = cpu_engine(folders, "tiny_a", eviction=KeyEviction(keep=50, recent=10, every=9), max_step_rows=60, max_tokens=64 * 40)
     assert engine.cache.width == 2, "50 + 9 - 1 rows before a pass, and the pass"
+
+
+# -- beginnings that are shared -----------------------------------------------------------------------------
+def test_shared_pages_are_counted_once():
+    """What a batch is counted to need is what it comes to hold, to the page, and a pool of that size runs it."""
+    rng = random.Random(5)
+    for _ in range(120):
+        stems = [[rng.randint(0, 1) for _ in range(rng.randint(1, 300))] for _ in range(2)]
+        prompts = [rng.choice(stems)[:rng.randint(1, 300)] + [rng.randint(0, 1) for _ in range(rng.randint(0, 70))] for _ in range(rng.randint(1, 7))]
+        new = rng.randint(1, 80)
+        pages = shared_pages(prompts, new)
+        assert pages <= sum(pages_needed(len(p), new) for p in prompts)
+        script = {i: [3] * new for i in range(len(prompts))}
+        loop, cache, stepper, _ = make(script, max_tokens=pages * PAGE, max_slots=8)
+        step, held = stepper.step, []
+        stepper.step = lambda entries: (step(entries), held.append(cache.n_pages - cache.free_pages()))[0]
+        assert len(list(loop.run_batch(prompts, new, share_prefix=True))) == new
+        assert max(held) == pages
+        cache.check()
+        assert loop.run_requests(prompts, new, share_prefix=True) == [script[i] for i in range(len(prompts))]
+    doc = list(range(320))
+    prompts = [doc + [i] * 3 for i in range(8)]
+    assert sum(pages_needed(len(p), 2) for p in prompts) == 48 and shared_pages(prompts, 2) == 5 + 8
+
+
+def test_batches_of_requests_that_share():
+    """As many neighbours as slots and pages take, the shared pages counted once; each batch of those that are tried fits."""
+    doc = list(range(320))
+    prompts = [doc + [i] * 3 for i in range(8)]
+    lens = [len(p) for p in prompts]
+    split = lambda slots, pages, ps=prompts: split_into_batches([len(p) for p in ps], 2, slots, pages, prompts=ps)
+    assert split(8, 13) == [list(range(8))] and split(8, 14) == [list(range(8))]
+    assert split(3, 13) == [[0, 1, 2], [3, 4, 5], [6, 7]]
+    assert split(8, 10) == [[0, 1, 2, 3, 4], [5, 6, 7]]
+    assert split_into_batches(lens, 2, 8, 14) == [[0, 1], [2, 3], [4, 5], [6, 7]], "not shared: six pages each"
+    with pytest.raises(ValueError, match="request 2 needs 640"):
+        split(8, 8, prompts[:2] + [list(range(600))])
+    rng = random.Random(6)
+    for _ in range(200):
+        stems = [[rng.randint(0, 1) for _ in range(200)] for _ in range(2)]
+        some = [rng.choice(stems)[:rng.randint(1, 200)] + [rng.randint(0, 1)] for _ in range(rng.randint(1, 12))]
+        slots, pages = rng.randint(1, 12), rng.randint(4, 20)
+        batches = split(slots, pages, some)
+        assert [i for b in batches for i in b] == list(range(len(some)))
+        assert all(1 <= len(b) <= slots and shared_pages([some[i] for i in b], 2) <= pages for b in batches)
+        plain = split_into_batches([len(p) for p in some], 2, slots, pages)
+        assert len(batches) <= len(plain), "sharing costs no batch"
+
+
+def test_a_pool_that_the_shared_pages_fit_runs_all_at_once(folders):
+    name = "tiny_a"
+    doc = prompts_for(name, [200], 5)[0]
+    prompts = [doc + t for t in prompts_for(name, [3, 9, 1, 30, 2, 5, 4, 60], 6)]
+    want = [list(s) for s in zip(*cpu_engine(folders, name, max_tokens=64 * 60).generate(prompts, 4))]
+    engine = cpu_engine(folders, name, max_tokens=14 * PAGE)
+    before = engine.loop.steps
+    assert engine.generate_all(prompts, 4, share_prefix=True) == want
+    assert engine.loop.steps - before == 4, "one batch"
+    pool = cpu_engine(folders, name)
+    assert [list(s) for s in zip(*pool.generate(prompts, 4, share_prefix=True))] == want
+    assert pool.cache.n_pages == 3 + 8 + 1, "three pages of the document, one of each prompt's own, a second of the longest's"
+    pool = cpu_engine(folders, name)
+    assert pool.generate_all(prompts, 4, share_prefix=True) == want and pool.cache.n_pages == 12
+    assert pool.generate_all(prompts, 4) == want and pool.cache.n_pages == sum(pages_needed(len(p), 4) for p in prompts), "the pool grows when it must"
+    pool = cpu_engine(folders, name)
+    assert pool.generate_all(prompts, 4, share_prefix=True, max_batch=3) == want and pool.cache.n_pages < 12
