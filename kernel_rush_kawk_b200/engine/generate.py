@@ -54,6 +54,7 @@ class GenerationStats:
     the like per plan (``GraphPlan.stats`` and its log lines, engine/engine.py:87,206,378)."""
     sequences: int = 0
     prompt_tokens: int = 0
+    shared_tokens: int = 0         # of these, the ones that did not run because another prompt's had
     prefill_ms: float = 0.0        # from the call to the first tokens on the host
     decode_steps: int = 0          # single-token steps whose tokens were read
     decode_ms: float = 0.0         # from the first tokens to the last ones
@@ -70,10 +71,11 @@ class GenerationStats:
 
     @property
     def prefill_tokens_per_s(self) -> float:
-        return self.prompt_tokens * 1000.0 / self.prefill_ms if self.prefill_ms > 0 else 0.0
+        return (self.prompt_tokens - self.shared_tokens) * 1000.0 / self.prefill_ms if self.prefill_ms > 0 else 0.0
 
     def line(self) -> str:
-        return (f"{self.sequences} sequences, {self.prompt_tokens} prompt tokens in {self.prefill_ms:.1f} ms "
+        shared = f" ({self.shared_tokens} shared)" if self.shared_tokens else ""
+        return (f"{self.sequences} sequences, {self.prompt_tokens} prompt tokens{shared} in {self.prefill_ms:.1f} ms "
                 f"({self.prefill_tokens_per_s:.0f} tokens/s); {self.decode_steps} decode steps at "
                 f"{self.decode_ms_per_step:.3f} ms ({self.decode_tokens_per_s:.0f} tokens/s)")
 
@@ -203,7 +205,7 @@ class GenerationLoop:
             raise ValueError("prompts cannot share their beginnings in this engine: a layer keeps a window of keys, or keys are evicted")
         try:
             if share_prefix:
-                live, begun = self._start_shared(seqs)
+                live, begun, stats.shared_tokens = self._start_shared(seqs)
             else:
                 for s in seqs:
                     s.slot = self.cache.alloc()
@@ -256,8 +258,9 @@ class GenerationLoop:
                     self.cache.free(s.slot)
                     s.slot = -1
 
-    def _start_shared(self, seqs: list) -> tuple[list, list]:
-        """Run what the prompts share, once; (the sequences in the order of their groups, the tokens that each has had)."""
+    def _start_shared(self, seqs: list) -> tuple[list, list, int]:
+        """Run what the prompts share, once; (the sequences in the order of their groups, the tokens that each has had, how many of these in all did
+        not run again)."""
         order, begun, first = [], [], []
         groups = [([seqs[i] for i in members], shared) for members, shared in shared_prefixes([s.prompt for s in seqs])]
         for members, shared in groups:
@@ -271,7 +274,7 @@ class GenerationLoop:
                 s.slot = self.cache.fork(members[0].slot, shared)
             order += members
             begun += [shared] * len(members)
-        return order, begun
+        return order, begun, sum((len(members) - 1) * shared for members, shared in groups)
 
     def run_requests(self, prompts: list, max_new_tokens: int, sampling: SamplingParams = SamplingParams(),
                      stop_token_ids=(), max_batch: int | None = None, share_prefix: bool = False) -> list:

@@ -155,3 +155,20 @@ def test_a_pool_that_the_shared_pages_fit_runs_all_at_once(folders):
     assert pool.generate_all(prompts, 4) == want and pool.cache.n_pages == sum(pages_needed(len(p), 4) for p in prompts), "the pool grows when it must"
     pool = cpu_engine(folders, name)
     assert pool.generate_all(prompts, 4, share_prefix=True, max_batch=3) == want and pool.cache.n_pages < 12
+
+
+def test_speeds_count_the_tokens_that_ran():
+    """A batch's prompt tokens are all of them; its speed is by those that went through the model."""
+    doc = list(range(320))
+    prompts = [doc + [i] * 3 for i in range(8)] + [[7, 8]]
+    loop, _, stepper, _ = make({i: [3] for i in range(9)}, max_slots=9)
+    list(loop.run_batch(prompts, 1, share_prefix=True))
+    ran = sum(len(tokens) for call in stepper.calls for _, tokens, _ in call)
+    assert ran == 320 + 8 * 3 + 2
+    stats = loop.stats
+    assert stats.prompt_tokens == 8 * 323 + 2 and stats.shared_tokens == 7 * 320
+    assert stats.prefill_tokens_per_s == pytest.approx(ran * 1000 / stats.prefill_ms) and "(2240 shared)" in stats.line()
+    loop, _, _, _ = make({i: [3] for i in range(9)}, max_tokens=64 * 60, max_slots=9)
+    list(loop.run_batch(prompts, 1))
+    assert loop.stats.shared_tokens == 0 and loop.stats.prefill_tokens_per_s == pytest.approx(2586 * 1000 / loop.stats.prefill_ms)
+    assert "shared" not in loop.stats.line()
