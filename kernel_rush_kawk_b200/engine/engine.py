@@ -31,7 +31,7 @@ import torch
 from ..cache.eviction import KeyEviction
 from ..cache.store import PAGE, SequenceCache
 from ..config.registry import get_architecture, preset_config, read_config
-from ..parts.base import KVNeed, StateNeed
+from ..parts.base import KVNeed
 from ..sampling.sampler import Sampler, SamplingParams
 from ..weights.loader import checkpoint_shapes, read_checkpoint
 from ..weights.random_init import random_tensors
@@ -133,16 +133,17 @@ class Engine:
         return cls(None, _config=config, _tensors=tensors, **options)
 
     def _check_eviction(self) -> None:
-        """Keys can be evicted where every run that keeps keys keeps all of them, reads its own, and counts what they receive."""
+        """Keys can be evicted where every layer that keeps anything keeps all of its keys, reads them alone, and counts what they receive."""
         for entry, need in zip(self.plan.schedule, self.model.cache_needs()):
-            mixer = self.model.blocks[entry.layer].mixer
+            mixer, kind = self.model.blocks[entry.layer].mixer, self.plan.layers[entry.layer].mixer.kind
             if entry.cache_from is not None:
                 raise ValueError("keys cannot be evicted from a cache that several layers read")
-            if isinstance(need, StateNeed) or need is None:
+            if need is None:
                 continue
-            if not isinstance(need, KVNeed) or need.window is not None or not getattr(mixer, "counts_weights", False):
-                raise ValueError(f"keys cannot be evicted in this model: a '{self.plan.layers[entry.layer].mixer.kind}' layer "
-                                 f"{'keeps a window of keys' if isinstance(need, KVNeed) and need.window is not None else 'does not count what its keys receive'}")
+            why = ("keeps other things than keys" if not isinstance(need, KVNeed) else "keeps a window of keys" if need.window is not None else
+                   None if getattr(mixer, "counts_weights", False) else "does not count what its keys receive")
+            if why is not None:
+                raise ValueError(f"keys cannot be evicted in this model: a '{kind}' layer {why}")
 
     def _build_cache(self, max_tokens: int, max_slots: int) -> None:
         if self.cache is not None and self.cache.live:

@@ -172,3 +172,10 @@ def test_speeds_count_the_tokens_that_ran():
     list(loop.run_batch(prompts, 1))
     assert loop.stats.shared_tokens == 0 and loop.stats.prefill_tokens_per_s == pytest.approx(2586 * 1000 / loop.stats.prefill_ms)
     assert "shared" not in loop.stats.line()
+
+
+@pytest.mark.parametrize("preset,why", [("zadunex_tiny", "'mamba2' layer keeps other things than keys"), ("taredra_tiny", "'parallel' layer keeps what is no key"),
+                                        ("disorax_tiny", "keeps a window of keys"), ("zefapel_tiny", "'gla' layer keeps other things than keys")])
+def test_models_whose_layers_keep_other_things_evict_no_keys(preset, why):
+    with pytest.raises(ValueError, match=why):
+        Engine.from_random(preset, dtype="float32", device="cpu", ops=CacheTorchOps(torch.float32), eviction=KeyEviction(64))
