@@ -174,7 +174,7 @@ def test_speeds_count_the_tokens_that_ran():
     assert "shared" not in loop.stats.line()
 
 
-@pytest.mark.parametrize("preset,why", [("zadunex_tiny", "'mamba2' layer keeps other things than keys"), ("taredra_tiny", "'parallel' layer keeps what is no key"),
+@pytest.mark.parametrize("preset,why", [("zadunex_tiny", "'mamba2' layer keeps other things than keys"), ("taredra_tiny", "'parallel' layer keeps other things than keys"),
                                         ("disorax_tiny", "keeps a window of keys"), ("zefapel_tiny", "'gla' layer keeps other things than keys")])
 def test_models_whose_layers_keep_other_things_evict_no_keys(preset, why):
     with pytest.raises(ValueError, match=why):
