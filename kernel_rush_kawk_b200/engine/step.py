@@ -230,6 +230,10 @@ class DecodeRun:
 
 
 class Stepper:
+    # Captured steps of sequences that share pages, of which there may be as many as numbers of sequences, of groups, and powers of two: the ones
+    # used last stay (each holds its activations and logits, 40 MB and more for 64 sequences of the 4B shape)
+    MAX_GROUP_GRAPHS = 64
+
     def __init__(self, model, cache: SequenceCache, ops, max_step_rows: int = 16384, use_graphs: bool = True):
         self.model = model
         self.cache = cache
@@ -384,12 +388,24 @@ class Stepper:
         groups = self._prefix(slots)
         if groups is None:
             return self._graphs.get(n) or self._capture(n, slots, starts, token_lists)
-        g = self._graphs.get((n, PrefixGroups.shape_of(*groups)))
+        key = (n, PrefixGroups.shape_of(*groups))
+        g = self._graphs.pop(key, None)
         if g is None:
+            self._drop_group_graphs(self.MAX_GROUP_GRAPHS - 1)
             return self._capture(n, slots, starts, token_lists, PrefixGroups(*groups, self.device))
+        self._graphs[key] = g  # the last one used
         if (g.meta.prefix.sizes, g.meta.prefix.lengths) != tuple(map(tuple, groups)):
             g.meta.prefix.update(PrefixGroups(*groups, self.device))
         return g
+
+    def _drop_group_graphs(self, keep: int) -> None:
+        """Let go of all but the ``keep`` captured steps of groups that were used last."""
+        old = [key for key in self._graphs if isinstance(key, tuple)]
+        old = old[:max(0, len(old) - keep)]
+        if old:
+            torch.cuda.synchronize(self.device)  # none is running
+            for key in old:
+                del self._graphs[key]
 
     def _replay(self, slots, starts, token_lists, want_rows, n: int):
         g = self._graph(slots, starts, token_lists)
