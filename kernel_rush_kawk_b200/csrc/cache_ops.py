@@ -148,12 +148,19 @@ class CacheOps:
     @staticmethod
     def _cluster_splits(items: int, all_keys: bool) -> int:
         """Blocks of a cluster that share the keys of a sequence's token, by the number of (sequence, kv head, row tile) items. ``all_keys``: all
-        that the sequence holds, unequally many; else those behind a shared prefix, which are few. One sequence after 1,087 tokens in 1, 2, 4 and 8: 18.6,
-        14.4, 12.4 and 10.3 us; 32 sequences after 2,000 to 4,500: 101, 87.9, 88.5 and 95.9. Behind a prefix, eight sequences with up to
-        400 keys of their own: 20.6, 20.7, 22.7 and 25.2, 64 with up to 500: 42.7, 51.2, 60.3 and 80."""
+        that the sequence holds, unequally many; else those behind a shared prefix, which are few.
+
+        As many as run at once, four blocks an SM: 60 clusters of eight, 132 of four, 296 of two. Counted tokens of 32 heads over 8 of 128 or of 4 over one, us
+        after 300, 1,500 and 8,000 keys, from keys in memory: 48 items in eight 9.6, 14.1 and 39, in four 9.2, 14.0 and 44; 66 in eight 12.5, 18.4 and
+        52, in four 9.7, 15.9 and 56; 128 in four 11.2, 23.5 and 92, in two 11.1, 24.5 and 104; 144 in four 17.9, 35.9 and 137, in two
+        11.3, 26.4 and 111; 296 in two 15.2, 45.2 and 208, in one 13.6, 46.4 and 228; 297 in two 22.4, 59 and 264, in one 14.3, 48 and 234. One sequence, eight
+        items, after 1,500 keys in 1, 2, 4 and 8: 23.5, 15.5, 11.3 and 9.4.
+
+        Behind a prefix of 4,096, with 100, 500 and 2,000 keys of their own (the prefix's kernel among it): 16 items in two 14.1, 12.7 and 20.9, in one 11.6,
+        13.9 and 30.6; 24 in two 15.7, 17.6 and 21.4, in one 13.5, 14.0 and 31.0; 64 in two 20.1, 22.2 and 30.5, in one 16.2, 16.4 and 30.4."""
         if all_keys:
-            return 8 if items <= 64 else 4 if items <= 148 else 2 if items <= 592 else 1
-        return 4 if items <= 37 else 2 if items <= 148 else 1
+            return 8 if items <= 60 else 4 if items <= 132 else 2 if items <= 296 else 1
+        return 2 if items <= 16 else 1
 
     @staticmethod
     def _by_mma(dtype, head_dim, q, stride, k, v) -> bool:

@@ -11,9 +11,9 @@
 // Where a unit has at most eight rows (NARROW: the heads of a kv head mostly are), the products are taken the other way round: the page's
 // keys are the sixteen rows of an instruction and the queries its eight columns, S^T = K Q^T and O^T = V^T P^T, with P^T turned in
 // registers (movmatrix). Sixteen rows of which four are queries cost twice the instructions and registers:
-// 64 sequences' own keys (up to 500 each, 8 kv heads of 128) take 43 us a pass in columns and 59.6 in rows, with 96 registers a thread instead of 158 to
-// 168. 32 sequences of 2,000 to 4,500 keys with their weights, 8 kv heads of 128: 85 us for 434 MB, 5.1 TB/s, beside 1,631 in the kernel for every type; one
-// sequence of 1,087 keys: 10.4 us, the latency of two launches' worth of dependent steps (page table, pages, statistics, join, weights).
+// 64 sequences' own keys (up to 500 each, 8 kv heads of 128, 70 MB) take 17.2 us in columns and 25.0 in rows, with 96 registers a thread instead of 158 to
+// 168. 32 sequences of 2,000 to 4,500 keys with their weights, 8 kv heads of 128: 83 us for 434 MB, 5.2 TB/s, beside 1,631 in the kernel for every type; one
+// sequence of 1,087 keys: 8.0 us, the latency of two launches' worth of dependent steps (page table, pages, statistics, join, weights).
 //
 // The splits of a sequence's keys form a cluster: their parts meet in the first block's shared memory, which also reads the prefix
 // parts of its rows and writes the output. That is the only place that waits for the kernel before, so a sequence's own
@@ -526,8 +526,11 @@ int launch_few_rows(bf16* out, const Parts& parts, int part0, int n_join, const 
     int rc = tc::make_map_bf16(&map_k, k, rows, D, D, KRK_PAGE);
     if (rc == 0) rc = tc::make_map_bf16(&map_v, v, rows, D, D, KRK_PAGE);
     if (rc) return rc;
-    // as many units as the shared memory of an SM holds for the blocks that it gets
-    const int per_sm = blocks <= 148 ? 1 : blocks <= 296 ? 2 : blocks <= 444 || Rows::TILE == 16 ? 3 : 4;
+    // As many units as the shared memory of an SM holds for the blocks that it gets. Clusters of four or eight do not fill every SM: 33 and 15 of them
+    // run at once with a block an SM, and more wait for a second
+    // round: 16 sequences' kv heads in clusters of eight after 1,500 keys 17.5 us by the device's 148 and 10.0 by 120, 36 in clusters of four 21.9 and 12.9.
+    const int fit = splits_in_cluster >= 8 ? 120 : splits_in_cluster >= 4 ? 132 : 148;
+    const int per_sm = blocks <= fit ? 1 : blocks <= 2 * fit ? 2 : blocks <= 3 * fit || Rows::TILE == 16 ? 3 : 4;
     const size_t room = 216 * 1024 / per_sm, fixed = Layout(0, splits_in_cluster, inbox_rows).total - Layout(0, 1, 0).total + 2048;
     in_ring = (int)((room > fixed ? room - fixed : 0) / UNIT_BYTES);
     in_ring = in_ring < 2 ? 2 : in_ring > 12 ? 12 : in_ring;
