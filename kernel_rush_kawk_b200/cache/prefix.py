@@ -15,21 +15,24 @@ from .store import PAGE
 # Where reading a prefix once pays. It takes a launch more, and parts of the softmax that have to join, so that what a step does not read again
 # has to be worth these.
 #
-# Single tokens, by the bytes of keys and values of one layer that are not read again: 8 MB a sequence, up to eight of them. A layer's attention with
-# rotation and cache write, us, each sequence by itself and shared, 32 heads over 8 of 128 with 100 keys of their own: 2 sequences behind 4,096 positions
-# (17 MB) 13.9 and 15.0, 8,192 22.8 and 16.9; 4 behind 2,048 (25 MB) 15.6 and 17.0, 4,096 22.1 and 18.7; 8 behind 2,048 (59 MB) 15.4 and 18.1,
-# 4,096 24.4 and 21.3; 16 behind 1,024 (63 MB) 16.2 and 18.9, 2,048 24.5 and 19.0; 64 behind 256 (66 MB) 22.9 and 21.6, 1,024 47.9 and 23.4, 8,192
-# 278.8 and 30.9. 16 heads over 4 of 64, a quarter of the bytes: 32 behind 1,024 (33 MB) 12.3 and 17.2, 2,048 18.9 and 18.0; 64 behind 1,024 (66 MB) 18.8 and
-# 17.5.
-SHARE_BYTES = 8 << 20
+# Single tokens, by the bytes of keys and values of one layer that are not read again: 9 MB a sequence, up to eight of them. A layer's attention with
+# rotation and cache write in replayed steps, us, each sequence by itself and shared, 32 heads over 8 of 128 with 100 keys of their own: 2 sequences behind 4,096
+# positions (17 MB) 14.3 and 17.4, 8,192 23.0 and 20.1; 4 behind 2,048 (25 MB) 15.8 and 15.5, 4,096 21.7 and 17.4; 8 behind 2,048 (59 MB) 15.5 and 16.7,
+# 4,096 24.3 and 19.8; 16 behind 1,024 (63 MB) 16.4 and 19.2, 2,048 24.8 and 19.8; 64 behind 256 (66 MB) 23.3 and 23.4, 1,024 48.0 and 26.4, 8,192
+# 279 and 33. 16 heads over 4 of 64, a quarter of the bytes: 32 behind 2,048 (65 MB) 19.0 and 18.2; 64 behind 1,024 (66 MB) 19.0 and 19.8.
+SHARE_BYTES = 9 << 20
 # Several tokens a sequence: where the products bound the step, sharing saves whole rounds of the device alone (row tiles of short or ragged
 # sequences that share theirs, keys split over blocks that would stand idle), and costs the join. Counted in steps of 128 keys (about 2 us, of a pair of
-# row tiles; 1.75 times that in the kernel of steps of less than a tile): rounds * steps by themselves against rounds * steps + 8 + (rows * heads) / 4,096.
-# Measured behind 1,024 and 4,096 positions, us, by themselves and shared, 32 heads over 8 of 128: 2 sequences of 4 tokens 32.7 and 18.5, 116 and 25;
-# 4 of 16 31.8 and 36.4, 110 and 38.6; 32 of 4 45 and 26.2, 157 and 31.8; 4 of 60 24.7 and 25.3, 66 and 36.4; 16 of 60 26.4 and 40.9, 70 and 82; 16 of 45 to
-# 90 behind 4,096 129 and 94; 2 of 250 26.8 and 33.3, 69 and 55; 4 of 250 28 and 51, 71 and 92; 16 heads over 4 of 64, 16 of 60 23.6 and 22.1, 65
-# and 42, 32 of 60 24.2 and 30.7, 66 and 70.
-JOIN_STEPS = 8
+# row tiles; 1.75 times that in the kernel of steps of less than a tile): rounds * steps by themselves against rounds * steps and, for the join, 7 steps
+# (half of them where a group's few rows go without tcgen05), 0.3 for each part of a row's prefix that is not empty (twice where a block has more than
+# eight rows, which a thread joins one after the other), and (rows * heads) / 4,096.
+# Behind 512, 1,024, 2,048 and 4,096 positions, us, by themselves and shared, 32 heads over 8 of 128: 2 sequences of 4 tokens 18.5 and 18.4, 31.5 and 19.1, 57 and
+# 21, 109 and 26; 4 of 4 18.6 and 29.8, 31.8 and 36.9, 58 and 37, 110 and 51; 4 of 16 19.5 and 32.0, 32.5 and 43.5, 59 and 44, 111 and 46; 8 of 2 18.0 and 18.7, 31.1
+# and 23.8, 57 and 24, 109 and 32; 8 of 30 19.6 and 26.6, 32.8 and 28.5, 59 and 32, 111 and 40; 32 of 8 32.6 and 24.1, 57 and 26, 104 and 30, 200 and 37. Behind
+# 1,024 and 4,096: 4 of 60 24.6 and 28.9, 66 and 40; 16 of 60 26.9 and 41.1, 69 and 83; 2 of 250 26.8 and 38.3, 68 and 60; 4 of 250 28.4 and 49.0, 70 and
+# 91; 16 of 45 to 90 behind 4,096 126 and 87. 16 heads over 4 of 64: 16 of 60 23.5 and 21.8, 66 and 41, 32 of 60 24.4 and 30.5, 67 and 70.
+JOIN_STEPS = 7
+PART_STEPS = 0.3
 
 
 def single_tokens_share(sizes, lengths, row_bytes: int) -> bool:
@@ -42,17 +45,23 @@ def single_tokens_share(sizes, lengths, row_bytes: int) -> bool:
 
 def longer_steps_share(sizes, lengths, q_lens, per: int, kv_heads: int) -> bool:
     """Whether a step of several tokens a sequence reads these groups' prefixes once. ``per``: query heads of a kv head."""
-    steps = max(lengths) / 128
+    steps, pages = max(lengths) / 128, max(lengths) // PAGE
     if 1.75 * steps < JOIN_STEPS:
         return False
-    tile, factor = (256, 1.0) if max(q_lens) * per >= 128 else (64, 1.75)
+    most = max(q_lens) * per  # rows of a sequence, for each kv head
+    tile, factor = (256, 1.0) if most >= 128 else (64, 1.75)
     alone = sum(-(-n * per // tile) for n in q_lens) * kv_heads
-    shared, at = 0, 0
+    group_rows, at = [], 0
     for size in sizes:
-        shared += -(-sum(q_lens[at:at + size]) * per // 256) * kv_heads
+        group_rows.append(sum(q_lens[at:at + size]) * per)
         at += size
+    few = max(group_rows) <= 32
+    shared = sum(-(-rows // (16 if few else 256)) for rows in group_rows) * kv_heads
+    splits = max(1, min(32, -(-148 // shared) if few else 148 // shared))
+    parts = -(-pages // -(-pages // splits))
     rounds = -(-shared // 148) if shared >= 148 else shared / 148
-    return -(-alone // 148) * factor * steps >= rounds * steps + JOIN_STEPS + sum(q_lens) * per * kv_heads / 4096
+    join = JOIN_STEPS * (0.5 if few else 1) + PART_STEPS * parts * (2 if most > 8 else 1) + sum(q_lens) * per * kv_heads / 4096
+    return -(-alone // 148) * factor * steps >= rounds * steps + join
 
 
 class PrefixGroups:
