@@ -114,6 +114,12 @@ class CacheOps:
         # (a single row has no stride that means anything)
         return qkv.data_ptr(), strides[0] if shape[0] > 1 else shape[1], k.data_ptr(), v.data_ptr()
 
+    @staticmethod
+    def _one_each(batch) -> bool:
+        """Whether every sequence brings one token: what the single-token kernels, which take a sequence's number for its row, need. (Steps in which some
+        bring none are longer ones to them.)"""
+        return batch.is_decode and batch.n_rows == batch.n_seqs
+
     def _check_device(self, what, *tensors):
         mine = self.error.get_device()
         for t in tensors:
@@ -188,8 +194,8 @@ class CacheOps:
         if rows == 0:
             return out
         scale, stream, error = float(scale), self._stream(), self.error.data_ptr()
-        by_mma = self._by_mma(qkv.dtype, D, q, stride, k, v)
-        if by_mma and not (single_tokens_share(prefix.sizes, prefix.lengths, 4 * kv * D) if batch.is_decode else
+        by_mma, one_each = self._by_mma(qkv.dtype, D, q, stride, k, v), self._one_each(batch)
+        if by_mma and not (single_tokens_share(prefix.sizes, prefix.lengths, 4 * kv * D) if one_each else
                            longer_steps_share(prefix.sizes, prefix.lengths, batch.q_lens, per, kv)):
             self._whole_attention(out, None, (q, stride, heads, kv), D, batch, cache, (k, v), scale)  # each sequence by itself, through its own page table
             return out
@@ -217,7 +223,7 @@ class CacheOps:
             self.launches += 1
             self._ok(lib.krk_attention_in_parts(out.data_ptr(), None, o, ml, rows, splits, own_splits, None, None, None, None, 0, 0, 1, 1, *step, group_rows,
                                                 batch.max_q_len, scale, _code(qkv.dtype), stream), "shared prefix attention")
-        elif batch.is_decode:
+        elif one_each:
             self.launches += splits > 0
             self._ok(lib.krk_shared_single(out.data_ptr(), o, ml, splits, self._cluster_splits(-(-per // 16) * kv * batch.n_seqs, False), tensor, *step,
                                            cache.k.shape[0], group_rows, scale, error, stream), "shared prefix attention")
@@ -240,7 +246,7 @@ class CacheOps:
         address, stride, heads, kv = q
         rows, per = batch.n_rows, heads // kv
         lib, error, stream = self._parts_lib(D), self.error.data_ptr(), self._stream()
-        if batch.is_decode and lse is None:
+        if lse is None and self._one_each(batch):
             self._ok(lib.krk_shared_single(out.data_ptr(), None, None, 0, self._cluster_splits(-(-per // 16) * kv * batch.n_seqs, True), 0, *q,
                                            *self._segments(batch, cache, None), *pages, cache.k.shape[0], 0, scale, error, stream), "single-token attention")
         elif self._by_tcgen05(D, address, stride) and batch.max_q_len * per >= 128 and self.use_tcgen05_attention:
@@ -284,7 +290,7 @@ class CacheOps:
         segments = self._segments(batch, cache, None)
         q, pages = (address, stride, heads, kv), (k, v)
         by_mma = self._by_mma(qkv.dtype, D, address, stride, k, v)
-        if by_mma and batch.is_decode and per <= 16:
+        if by_mma and per <= 16 and self._one_each(batch):
             raw = self._scratch(rows * heads * capacity)
             self._ok(lib.krk_scored_single(out.data_ptr(), raw.data_ptr(), *counts, self._cluster_splits(kv * rows, True), *q, *segments, *pages,
                                            cache.k.shape[0], scale, error, stream), "scored attention")

@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from cache_ops_helpers import PAGE, exact_attention, make_step
+from cache_ops_helpers import PAGE, exact_attention, make_batch, make_step
 from test_cache_ops_gpu import BF16, DEVICE, F32, groups, ops, within  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -108,4 +108,35 @@ def test_shares_of_more_pages_than_the_loading_warp_reads_at_once(ops, heads, kv
         within(scores[slot, :, :n + 1], weights[i], weights_off[i], f"weights of sequence {i}")
     monkeypatch.setattr(prefix, "SHARE_BYTES", 1 << 60)
     within(ops.shared_prefix_attention(qkv, heads, kv, dim, batch, cache, scale, groups([len(held)], [0])), want, off, "each sequence by itself")
+    ops.check()
+
+
+@pytest.mark.parametrize("dtype,shape", [(F32, (8, 2, 64)), (BF16, (8, 2, 48)), (BF16, (8, 2, 128)), (BF16, (40, 2, 64)), (BF16, (5, 1, 20))])
+@pytest.mark.parametrize("sizes,lengths,own,brings", [([2, 1], [64, 0], [3, 0, 70], [0, 1, 1]), ([3], [128], [0, 70, 5], [1, 0, 1]), ([2, 2], [64, 192], [1, 90, 0, 200], [0, 70, 0, 5]),
+                                                     ([1, 2], [0, 0], [0, 64, 9], [0, 0, 150]), ([1, 1], [64, 0], [0, 5], [0, 1])])
+@pytest.mark.parametrize("together", [True, False])
+def test_sequences_that_bring_nothing(ops, dtype, shape, sizes, lengths, own, brings, together, monkeypatch):
+    """Beside others that bring one token or more: these come out as without them, and of the idle ones nothing changes."""
+    from kernel_rush_kawk_b200.cache import prefix
+
+    if not together:
+        monkeypatch.setattr(prefix, "SHARE_BYTES", 1 << 60)
+        monkeypatch.setattr(prefix, "JOIN_STEPS", 1e9)
+    heads, kv, dim = shape
+    held = [p + o for p, o in zip([p for s, p in zip(sizes, lengths) for _ in range(s)], own)]
+    qkv, batch, cache = make_step(DEVICE, dtype, heads, kv, dim, held, brings, 21, (sizes, lengths))
+    busy = [i for i, t in enumerate(brings) if t]
+    some = make_batch(DEVICE, [batch.slots[i] for i in busy], [held[i] for i in busy], [brings[i] for i in busy])
+    want, off, weights, weights_off = exact_attention(qkv, heads, kv, dim, some, cache, 0.1)
+    within(ops.shared_prefix_attention(qkv, heads, kv, dim, batch, cache, 0.1, groups(sizes, lengths)), want, off, "behind prefixes")
+    scores = torch.rand((cache.table.shape[0], kv, cache.width * PAGE), device=DEVICE)
+    before = scores.clone()
+    within(ops.scored_attention(qkv, heads, kv, dim, batch, cache, 0.1, scores), want, off, "counted")
+    for j, i in enumerate(busy):
+        slot, n, t = batch.slots[i], held[i], brings[i]
+        sums = weights[j].clone()
+        sums[:, :n] += before[slot, :, :n].double()
+        within(scores[slot, :, :n + t], sums, weights_off[j] + sums * 2.0 ** -24, f"weights of sequence {i}")
+        before[slot, :, :n + t] = scores[slot, :, :n + t]
+    assert torch.equal(scores, before), "other slots"
     ops.check()
