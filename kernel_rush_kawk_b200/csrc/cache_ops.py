@@ -104,13 +104,20 @@ class CacheOps:
             raise KernelError(f"{what}: {heads} heads of {head_dim} do not fit a cache of {cache.kv_heads} heads of {cache.head_dim} (values: {cache.v_dim})")
         if cache.window is not None or cache.keep_pages:
             raise KernelError(f"{what}: the cache keeps a window of keys; every key is asked for")
-        if k.dtype != dtype or v.dtype != dtype or not k.is_contiguous() or not v.is_contiguous():
-            raise KernelError(f"{what}: the cache's pages are contiguous and of the rows' dtype ({dtype}), got {k.dtype}")
+        pages = k.shape
+        if k.dtype != dtype or v.dtype != dtype or not k.is_contiguous() or not v.is_contiguous() or v.shape != pages or pages[1:] != (cache.kv_heads, PAGE, head_dim):
+            raise KernelError(f"{what}: the cache's pages are contiguous [pages, kv heads, {PAGE}, head size] of the rows' dtype ({dtype}), "
+                              f"got {k.dtype} {list(pages)} and {v.dtype} {list(v.shape)}")
+        table = cache.table
+        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[1] != cache.width or not table.is_contiguous():
+            raise KernelError(f"{what}: the page table is contiguous int32 [slots, {cache.width}], got {table.dtype} {list(table.shape)}")
         if shape[0] != batch.n_rows or batch.max_kv_len > cache.width * PAGE:
             raise KernelError(f"{what}: {shape[0]} rows for a step of {batch.n_rows} with up to {batch.max_kv_len} keys, in slots of {cache.width * PAGE}")
+        if batch.slots and (min(batch.slots) < 0 or max(batch.slots) >= table.shape[0]):
+            raise KernelError(f"{what}: slots {list(batch.slots)} of {table.shape[0]}")
         if shape[0] > 1 and strides[0] < shape[1]:
             raise KernelError(f"{what}: rows that overlap (a stride of {strides[0]})")
-        self._check_device(what, qkv, k)
+        self._check_device(what, qkv, k, v, table, batch.cu_q)
         # (a single row has no stride that means anything)
         return qkv.data_ptr(), strides[0] if shape[0] > 1 else shape[1], k.data_ptr(), v.data_ptr()
 
@@ -189,6 +196,7 @@ class CacheOps:
         sequence, float32 or bfloat16; a captured step stays valid while the groups' number and sizes last, whatever the lengths become."""
         q, stride, k, v = self._check_step("shared prefix attention", qkv, heads, kv_in_row, head_dim, batch, cache)
         prefix.check(batch, cache)
+        self._check_device("shared prefix attention", prefix.buffer)
         lib, rows, kv, per, D = self._parts_lib(head_dim), batch.n_rows, cache.kv_heads, heads // cache.kv_heads, head_dim
         out = qkv.new_empty((rows, heads * D))
         if rows == 0:
@@ -277,6 +285,9 @@ class CacheOps:
         rows where keys were evicted. ``out_scores`` takes the sums in place of ``scores``."""
         address, stride, k, v = self._check_step("scored attention", qkv, heads, kv_in_row, head_dim, batch, cache)
         out_scores = scores if out_scores is None else out_scores
+        shift = getattr(batch, "seq_shift", None)
+        if shift is not None:
+            self._check_device("scored attention", shift)
         self._check_scores("scored attention", cache, (("scores", scores, torch.float32), ("positions", positions, torch.int32),
                                                        ("out_scores", None if out_scores is scores else out_scores, torch.float32)))
         if observe is not None and observe < 1:
@@ -286,7 +297,7 @@ class CacheOps:
         if rows == 0:
             return out
         scale, stream, error, capacity = float(scale), self._stream(), self.error.data_ptr(), scores.shape[2]
-        counts = (scores.data_ptr(), out_scores.data_ptr(), _ptr(positions), _ptr(getattr(batch, "seq_shift", None)), capacity)
+        counts = (scores.data_ptr(), out_scores.data_ptr(), _ptr(positions), _ptr(shift), capacity)
         segments = self._segments(batch, cache, None)
         q, pages = (address, stride, heads, kv), (k, v)
         by_mma = self._by_mma(qkv.dtype, D, address, stride, k, v)
@@ -334,8 +345,9 @@ class CacheOps:
             raise KernelError(f"{what}: pages are [runs, pages, kv heads, {PAGE}, head size], got {list(shape)} and {list(v.shape)}")
         _code(k.dtype)
         if (k.stride()[1:] != (heads * PAGE * dim, PAGE * dim, dim, 1) or v.stride()[1:] != (heads * PAGE * v.shape[4], PAGE * v.shape[4], v.shape[4], 1)
-                or not table.is_contiguous() or table.dtype != torch.int32):
-            raise KernelError(f"{what}: every run's pages and the page table (int32) are contiguous")
+                or (runs > 1 and (k.stride(0) < n_pages * k.stride(1) or v.stride(0) < n_pages * v.stride(1)))
+                or not table.is_contiguous() or table.dtype != torch.int32 or table.dim() != 2):
+            raise KernelError(f"{what}: every run's pages and the page table (int32 [slots, pages of a slot]) are contiguous, and runs lie apart")
         out_scores = scores if out_scores is None else out_scores
         out_positions = positions if out_positions is None else out_positions
         n_slots, width = table.shape
@@ -359,6 +371,8 @@ class CacheOps:
             raise KernelError(f"{what}: slots {list(slots)} of {n_slots} with {list(lengths)} rows of {capacity}")
         if batch is not None and (batch.n_seqs != n or batch.n_rows != n or getattr(batch, "seq_shift", None) is None):
             raise KernelError(f"{what}: the step that follows has one token of each slot and keeps shifts")
+        if batch is not None:
+            self._check_device(what, batch.seq_start, batch.seq_shift)
         left = [keep if m > keep else m for m in lengths]
         if k.numel() == 0:
             return left
