@@ -90,6 +90,7 @@ def main(argv=None) -> int:
         print(folder)
         return 0
     from . import Engine, KeyEviction
+    from .cache import CacheError
     prompts = list(args.prompt_ids)
     if args.prompt_file:
         prompts += [list(map(int, row)) for row in json.load(open(args.prompt_file))]
@@ -103,7 +104,10 @@ def main(argv=None) -> int:
         if args.share_prefix:
             parser.error("--share-prefix and --keep-keys exclude each other: shared pages stay as they are")
         recent = args.keep_keys // 4 if args.keep_recent is None else args.keep_recent
-        options["eviction"] = KeyEviction(keep=args.keep_keys, recent=recent)
+        try:
+            options["eviction"] = KeyEviction(keep=args.keep_keys, recent=recent)
+        except CacheError as e:
+            parser.error(str(e))
     if args.model:
         engine = Engine(args.model, **options)
     else:

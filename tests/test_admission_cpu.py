@@ -179,3 +179,12 @@ def test_speeds_count_the_tokens_that_ran():
 def test_models_whose_layers_keep_other_things_evict_no_keys(preset, why):
     with pytest.raises(ValueError, match=why):
         Engine.from_random(preset, dtype="float32", device="cpu", ops=CacheTorchOps(torch.float32), eviction=KeyEviction(64))
+
+
+@pytest.mark.parametrize("options", ["--keep-keys 0", "--keep-keys 10 --keep-recent 11", "--keep-keys 10 --keep-recent -1"])
+def test_the_command_line_says_what_keeps_nothing(options, capsys):
+    from kernel_rush_kawk_b200.cli import main
+
+    with pytest.raises(SystemExit):
+        main(f"generate --random tiny_a --prompt-ids 1 {options}".split())
+    assert "at least one key stays" in capsys.readouterr().err
