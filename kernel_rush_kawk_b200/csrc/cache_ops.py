@@ -292,6 +292,8 @@ class CacheOps:
                                                        ("out_scores", None if out_scores is scores else out_scores, torch.float32)))
         if observe is not None and observe < 1:
             raise KernelError(f"scored attention: at least one query a sequence is observed, got {observe}")
+        if len(set(batch.slots)) != len(batch.slots):
+            raise KernelError(f"scored attention: every slot comes once, its sums are one call's; got {list(batch.slots)}")
         lib, rows, kv, per, D = self._parts_lib(head_dim), batch.n_rows, cache.kv_heads, heads // cache.kv_heads, head_dim
         out = qkv.new_empty((rows, heads * D))
         if rows == 0:
@@ -310,21 +312,22 @@ class CacheOps:
         lse = self._scratch(rows * heads)
         page_blocks = max(1, min(cache.width, -(-888 // (kv * batch.n_seqs))))
         seen = min(batch.max_q_len, observe or batch.max_q_len)
+        last = seen if observe else 0  # (0: all; no sequence of the step has more than seen either way)
         if not by_mma:
             parts = self._splits(-(-batch.max_q_len * per // 64) * kv * batch.n_seqs, 444)
             scratch = self._scratch(parts * rows * heads * (D + 2))
             o = scratch.data_ptr()
             self.launches += 2
-            self._ok(lib.krk_attention_in_parts(out.data_ptr(), lse.data_ptr(), o, o + 4 * parts * rows * heads * D, rows, 0, parts, *counts, int(observe or 0),
+            self._ok(lib.krk_attention_in_parts(out.data_ptr(), lse.data_ptr(), o, o + 4 * parts * rows * heads * D, rows, 0, parts, *counts, last,
                                                 page_blocks, seen, *q, *segments, *pages, 0, batch.max_q_len, scale, _code(qkv.dtype), stream), "scored attention")
             return out
         self._whole_attention(out, lse, q, D, batch, cache, pages, scale)
         if self._by_tcgen05(D, address, stride) and not batch.is_decode and per <= 64:
             longest = cache.width * PAGE if torch.cuda.is_current_stream_capturing() else batch.max_kv_len  # a captured step's sequences grow
-            self._ok(lib.krk_key_weights_tcgen05(*counts, lse.data_ptr(), int(observe or 0), *q, *segments, pages[0], cache.k.shape[0], rows, seen, longest,
+            self._ok(lib.krk_key_weights_tcgen05(*counts, lse.data_ptr(), last, *q, *segments, pages[0], cache.k.shape[0], rows, seen, longest,
                                                  scale, error, stream), "weights of keys")
         else:
-            self._ok(lib.krk_key_weights(*counts, lse.data_ptr(), int(observe or 0), *q, *segments, pages[0], page_blocks, seen, scale, _code(qkv.dtype),
+            self._ok(lib.krk_key_weights(*counts, lse.data_ptr(), last, *q, *segments, pages[0], page_blocks, seen, scale, _code(qkv.dtype),
                                          stream), "weights of keys")
         return out
 

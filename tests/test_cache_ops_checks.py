@@ -74,3 +74,10 @@ def test_evictions_that_do_not_fit():
                dict(batch=step(seq_shift=elsewhere(scores))), dict(batch=step(seq_start=elsewhere(scores))), dict(batch=step(n_rows=2)), dict(v=elsewhere(k)), dict(table=elsewhere(table))]:
         with pytest.raises(KernelError):
             evict(**kw)
+
+
+def test_a_slot_whose_sums_two_sequences_would_add_to():
+    qkv, batch, cache = step()
+    batch.slots = [1, 1]
+    with pytest.raises(KernelError, match="every slot comes once"):
+        Checks().scored_attention(qkv, 4, 2, 32, batch, cache, 0.1, torch.zeros((cache.table.shape[0], 2, cache.width * 64)))

@@ -140,3 +140,14 @@ def test_sequences_that_bring_nothing(ops, dtype, shape, sizes, lengths, own, br
         before[slot, :, :n + t] = scores[slot, :, :n + t]
     assert torch.equal(scores, before), "other slots"
     ops.check()
+
+
+@pytest.mark.parametrize("dtype,dim", [(F32, 64), (BF16, 48), (BF16, 128)])
+@pytest.mark.parametrize("observe", [2 ** 32 + 5, 2 ** 31, 10 ** 30])
+def test_more_observed_queries_than_there_are(ops, dtype, dim, observe):
+    """A number beyond 32 bits is as good as all."""
+    qkv, batch, cache = make_step(DEVICE, dtype, 8, 2, dim, [60, 0], [9, 40], 4)
+    all_of_them, some = scores_of(cache, 2), scores_of(cache, 2)
+    ops.scored_attention(qkv, 8, 2, dim, batch, cache, 0.1, all_of_them)
+    ops.scored_attention(qkv, 8, 2, dim, batch, cache, 0.1, some, observe=observe)
+    assert torch.equal(all_of_them, some)
