@@ -17,6 +17,7 @@ from ..cache.prefix import longer_steps_share, single_tokens_share
 from .build import build_library
 
 F32, BF16 = 0, 1
+_F32, _I32 = torch.float32, torch.int32
 _P = c_void_p
 PAGE = 64
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # (the function around it costs as much again)
@@ -94,32 +95,36 @@ class CacheOps:
         return self._cache_lib
 
     # -- what both attentions ask of their arguments ---------------------------------
-    def _check_step(self, what, qkv, heads, kv_in_row, head_dim, batch, cache):
-        """Raise unless the step can be taken; (address of the rows, elements between them, addresses of the pages of keys and of values)."""
-        shape, dtype, k, v = qkv.shape, qkv.dtype, cache.k, cache.v
-        strides = qkv.stride()
+    def _check_step(self, what, qkv, heads, kv_in_row, head_dim, batch, cache, also=None):
+        """Raise unless the step can be taken; (address of the rows, elements between them, addresses of the pages of keys and of values).
+        ``also``: one more tensor (or None) that the call reads on the device."""
+        shape, dtype, k, v, table, kv, width = qkv.shape, qkv.dtype, cache.k, cache.v, cache.table, cache.kv_heads, cache.width
+        strides, pages, slots, held = qkv.stride(), k.shape, batch.slots, table.shape
         if len(shape) != 2 or strides[1] != 1 or shape[1] != (heads + 2 * kv_in_row) * head_dim:
             raise KernelError(f"{what}: rows of {(heads + 2 * kv_in_row) * head_dim} elements side by side are asked for, got {tuple(shape)}")
-        if heads % cache.kv_heads or cache.head_dim != head_dim or cache.v_dim != head_dim:
-            raise KernelError(f"{what}: {heads} heads of {head_dim} do not fit a cache of {cache.kv_heads} heads of {cache.head_dim} (values: {cache.v_dim})")
+        if heads % kv or cache.head_dim != head_dim or cache.v_dim != head_dim:
+            raise KernelError(f"{what}: {heads} heads of {head_dim} do not fit a cache of {kv} heads of {cache.head_dim} (values: {cache.v_dim})")
         if cache.window is not None or cache.keep_pages:
             raise KernelError(f"{what}: the cache keeps a window of keys; every key is asked for")
-        pages = k.shape
-        if k.dtype != dtype or v.dtype != dtype or not k.is_contiguous() or not v.is_contiguous() or v.shape != pages or pages[1:] != (cache.kv_heads, PAGE, head_dim):
+        if (k.dtype is not dtype or v.dtype is not dtype or not k.is_contiguous() or not v.is_contiguous() or v.shape != pages
+                or pages != (pages[0], kv, PAGE, head_dim)):
             raise KernelError(f"{what}: the cache's pages are contiguous [pages, kv heads, {PAGE}, head size] of the rows' dtype ({dtype}), "
                               f"got {k.dtype} {list(pages)} and {v.dtype} {list(v.shape)}")
-        table = cache.table
-        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[1] != cache.width or not table.is_contiguous():
-            raise KernelError(f"{what}: the page table is contiguous int32 [slots, {cache.width}], got {table.dtype} {list(table.shape)}")
-        if shape[0] != batch.n_rows or batch.max_kv_len > cache.width * PAGE:
-            raise KernelError(f"{what}: {shape[0]} rows for a step of {batch.n_rows} with up to {batch.max_kv_len} keys, in slots of {cache.width * PAGE}")
-        if batch.slots and (min(batch.slots) < 0 or max(batch.slots) >= table.shape[0]):
-            raise KernelError(f"{what}: slots {list(batch.slots)} of {table.shape[0]}")
-        if shape[0] > 1 and strides[0] < shape[1]:
+        if held != (held[0], width) or table.dtype is not _I32 or not table.is_contiguous():
+            raise KernelError(f"{what}: the page table is contiguous int32 [slots, {width}], got {table.dtype} {list(held)}")
+        rows = shape[0]
+        if rows != batch.n_rows or batch.max_kv_len > width * PAGE:
+            raise KernelError(f"{what}: {rows} rows for a step of {batch.n_rows} with up to {batch.max_kv_len} keys, in slots of {width * PAGE}")
+        if slots and (min(slots) < 0 or max(slots) >= held[0]):
+            raise KernelError(f"{what}: slots {list(slots)} of {held[0]}")
+        if rows > 1 and strides[0] < shape[1]:
             raise KernelError(f"{what}: rows that overlap (a stride of {strides[0]})")
-        self._check_device(what, qkv, k, v, table, batch.cu_q)
+        here, cu = self.error.get_device(), batch.cu_q
+        if not (here == qkv.get_device() == k.get_device() == v.get_device() == table.get_device() == cu.get_device() == _current_device()
+                and (also is None or also.get_device() == here)):
+            self._check_device(what, qkv, k, v, table, cu, *(() if also is None else (also,)))
         # (a single row has no stride that means anything)
-        return qkv.data_ptr(), strides[0] if shape[0] > 1 else shape[1], k.data_ptr(), v.data_ptr()
+        return qkv.data_ptr(), strides[0] if rows > 1 else shape[1], k.data_ptr(), v.data_ptr()
 
     @staticmethod
     def _one_each(batch) -> bool:
@@ -194,11 +199,10 @@ class CacheOps:
         (cache.prefix says when; elsewhere each sequence reads its own table's). The step's
         own keys and values must be in the cache already, and its rows lie behind their group's prefix. Any number of tokens a
         sequence, float32 or bfloat16; a captured step stays valid while the groups' number and sizes last, whatever the lengths become."""
-        q, stride, k, v = self._check_step("shared prefix attention", qkv, heads, kv_in_row, head_dim, batch, cache)
+        q, stride, k, v = self._check_step("shared prefix attention", qkv, heads, kv_in_row, head_dim, batch, cache, prefix.buffer)
         prefix.check(batch, cache)
-        self._check_device("shared prefix attention", prefix.buffer)
         lib, rows, kv, per, D = self._parts_lib(head_dim), batch.n_rows, cache.kv_heads, heads // cache.kv_heads, head_dim
-        out = qkv.new_empty((rows, heads * D))
+        out = qkv.new_empty(rows, heads * D)
         if rows == 0:
             return out
         scale, stream, error = float(scale), self._stream(), self.error.data_ptr()
@@ -269,11 +273,11 @@ class CacheOps:
 
     # -- weights per key -------------------------------------------------------------------
     @staticmethod
-    def _check_scores(what, cache, tables):
-        shape = (cache.table.shape[0], cache.kv_heads, cache.width * PAGE)
-        device = cache.k.get_device()
-        for name, t, dtype in tables:
-            if t is not None and (t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.get_device() != device):
+    def _check_scores(what, cache, scores, positions, out_scores):
+        shape, device = (cache.table.shape[0], cache.kv_heads, cache.width * PAGE), cache.k.get_device()
+        for t, dtype in ((scores, _F32), (positions, _I32), (None if out_scores is scores else out_scores, _F32)):
+            if t is not None and (t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or t.get_device() != device):
+                name = "scores" if t is scores else "positions" if t is positions else "out_scores"
                 raise KernelError(f"{what}: {name} are contiguous {dtype} [slots, kv heads, rows of a slot] = {list(shape)} beside the cache, "
                                   f"got {t.dtype} {list(t.shape)}")
 
@@ -283,22 +287,19 @@ class CacheOps:
         (None: all). Rows that the step itself brings start from its own weights; rows behind a sequence's last stay as they are.
         ``positions`` (int32, the same shape) take the step's rows' positions in the sequence, which lie ``batch.seq_shift`` behind their
         rows where keys were evicted. ``out_scores`` takes the sums in place of ``scores``."""
-        address, stride, k, v = self._check_step("scored attention", qkv, heads, kv_in_row, head_dim, batch, cache)
-        out_scores = scores if out_scores is None else out_scores
         shift = getattr(batch, "seq_shift", None)
-        if shift is not None:
-            self._check_device("scored attention", shift)
-        self._check_scores("scored attention", cache, (("scores", scores, torch.float32), ("positions", positions, torch.int32),
-                                                       ("out_scores", None if out_scores is scores else out_scores, torch.float32)))
+        address, stride, k, v = self._check_step("scored attention", qkv, heads, kv_in_row, head_dim, batch, cache, shift)
+        out_scores = scores if out_scores is None else out_scores
+        self._check_scores("scored attention", cache, scores, positions, out_scores)
         if observe is not None and observe < 1:
             raise KernelError(f"scored attention: at least one query a sequence is observed, got {observe}")
         if len(set(batch.slots)) != len(batch.slots):
             raise KernelError(f"scored attention: every slot comes once, its sums are one call's; got {list(batch.slots)}")
         lib, rows, kv, per, D = self._parts_lib(head_dim), batch.n_rows, cache.kv_heads, heads // cache.kv_heads, head_dim
-        out = qkv.new_empty((rows, heads * D))
+        out = qkv.new_empty(rows, heads * D)
         if rows == 0:
             return out
-        scale, stream, error, capacity = float(scale), self._stream(), self.error.data_ptr(), scores.shape[2]
+        scale, stream, error, capacity = float(scale), self._stream(), self.error.data_ptr(), cache.width * PAGE
         counts = (scores.data_ptr(), out_scores.data_ptr(), _ptr(positions), _ptr(shift), capacity)
         segments = self._segments(batch, cache, None)
         q, pages = (address, stride, heads, kv), (k, v)
