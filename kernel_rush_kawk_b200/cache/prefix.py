@@ -56,9 +56,9 @@ def longer_steps_share(sizes, lengths, q_lens, per: int, kv_heads: int) -> bool:
         group_rows.append(sum(q_lens[at:at + size]) * per)
         at += size
     few = max(group_rows) <= 32
-    shared = sum(-(-rows // (16 if few else 256)) for rows in group_rows) * kv_heads
+    shared = max(1, sum(-(-rows // (16 if few else 256)) for rows in group_rows) * kv_heads)
     splits = max(1, min(32, -(-148 // shared) if few else 148 // shared))
-    parts = -(-pages // -(-pages // splits))
+    parts = -(-pages // max(1, -(-pages // splits)))  # that are not empty
     rounds = -(-shared // 148) if shared >= 148 else shared / 148
     join = JOIN_STEPS * (0.5 if few else 1) + PART_STEPS * parts * (2 if most > 8 else 1) + sum(q_lens) * per * kv_heads / 4096
     return -(-alone // 148) * factor * steps >= rounds * steps + join

@@ -18,3 +18,19 @@ def test_single_tokens(n, length, shares):
 def test_longer_steps(n, tokens, length, shares):
     """32 heads over 8: what a block joins one part after the other weighs against short prefixes."""
     assert longer_steps_share([n], [length], [tokens] * n, 4, 8) is shares
+
+
+def test_nothing_to_share():
+    for sizes, lengths, tokens in (([3], [0], [1, 5, 0]), ([1, 1], [64, 64], [700, 0]), ([1], [4096], [0])):
+        assert longer_steps_share(sizes, lengths, tokens, 4, 8) is False
+        assert single_tokens_share(sizes, [0] * len(sizes), 4096) is False
+
+
+def test_lines_that_are_moved_out_of_the_way(monkeypatch):
+    """As the tests of small cases do."""
+    from kernel_rush_kawk_b200.cache import prefix
+
+    monkeypatch.setattr(prefix, "JOIN_STEPS", -1e9)
+    assert longer_steps_share([3], [0], [1, 5, 0], 4, 8) is True
+    monkeypatch.setattr(prefix, "JOIN_STEPS", 1e9)
+    assert longer_steps_share([64], [8192], [4] * 64, 4, 8) is False
