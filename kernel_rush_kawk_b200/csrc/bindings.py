@@ -19,6 +19,7 @@ from ctypes import c_float, c_int, c_longlong, c_uint, c_void_p
 
 import torch
 
+from .adapter_ops import AdapterOps
 from .build import build_library
 from .cache_ops import BF16, F32, CacheOps, KernelError, _code, _load, _ptr  # noqa: F401
 
@@ -150,7 +151,7 @@ _ATTN_SIGNATURES = {
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-class Kernels(CacheOps):
+class Kernels(CacheOps, AdapterOps):
     """All kernels, for one device. ``head_dims``: the head sizes whose attention
     libraries are needed (compiled at first use)."""
 
@@ -165,7 +166,7 @@ class Kernels(CacheOps):
         self.attn: dict[int, ctypes.CDLL] = {}
         self.latent: dict[tuple, ctypes.CDLL] = {}
         self.parts: dict[int, ctypes.CDLL] = {}
-        self._cache_lib = None
+        self._cache_lib = self._adapt = None
         for d in head_dims:
             self._attn_lib(int(d))
         self.error = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -240,6 +241,8 @@ class Kernels(CacheOps):
                  5: "a tensor-core GEMM gave up waiting for its accumulator",
                  24: "the delta rule's walk gave up waiting for its copies",
                  25: "attention of few rows gave up waiting for a page of keys or values",
+                 26: "a row has an adapter that the bank does not hold",
+                 27: "lengths, slots or pages that do not fit a step reached its maps",
                  20: "a 32-bit product of few rows gave up waiting for its copies",
                  21: "the wait of the self-test kernel ran out (as it is meant to)"}
         if flag in known:

@@ -6,7 +6,7 @@ Kinds of library: ``core`` (kernels whose sizes are run-time arguments),
 (the kernels of models with a 32-bit residual stream, windowed attention with a
 sink or over latent rows), ``scan`` (recurrent state), ``memory`` (matrix states
 without a removal term), ``moe`` (routed
-experts) and ``cache`` (eviction); each of the last five is compiled and loaded when a model first calls
+experts), ``cache`` (eviction) and ``adapt`` (maps of a step, low-rank adapters); each of the last six is compiled and loaded when a model first calls
 one of its kernels, so a model compiles what it needs; ``latent_k<D>_v<P>`` (prompt
 attention over keys and values made from latent rows, per pair of sizes) and ``parts_d<D>`` (attention
 in parts: shared prefixes, weights per key) likewise. A library
@@ -40,11 +40,14 @@ SCAN_SOURCES = ["recurrent.cu", "recurrent_chunks.cu", "ssd.cu"]
 MEMORY_SOURCES = ["matrix_memory.cu", "matrix_memory_chunks.cu", "matrix_memory_step.cu"]
 MOE_SOURCES = ["routed.cu", "few_experts.cu", "grouped_gemm.cu"]
 CACHE_SOURCES = ["evict.cu"]
-SMALL_LIBRARIES = {"mix": MIX_SOURCES, "scan": SCAN_SOURCES, "memory": MEMORY_SOURCES, "moe": MOE_SOURCES, "cache": CACHE_SOURCES}
+ADAPT_SOURCES = ["adapters.cu"]
+SMALL_LIBRARIES = {"mix": MIX_SOURCES, "scan": SCAN_SOURCES, "memory": MEMORY_SOURCES, "moe": MOE_SOURCES, "cache": CACHE_SOURCES,
+                   "adapt": ADAPT_SOURCES}
 PARTS_SOURCES = ["partial_attention.cu", "few_rows_attention.cu", "many_rows_attention.cu", "prefix_tcgen05.cu", "key_weights_tcgen05.cu"]
 LATENT_SOURCES = ["latent_prefill.cu"]
 ATTN_SOURCES = ["attention_simple.cu", "attention_mma.cu", "attention_tcgen05.cu"]
 HEADERS = ["common.cuh", "mma.cuh", "tcgen05.cuh", "attention_noalloc.h", "attention_tiles.cuh", "partial_attention.cuh"]
+ADAPT_HEADERS = ["adapters.cuh"]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
@@ -110,7 +113,8 @@ def library_path(kind: str, head_dim=None) -> tuple[Path, list, list]:
         sources, defines, stem = _existing(CORE_SOURCES), [], "libkrk_core"
     elif kind in SMALL_LIBRARIES:
         sources, defines, stem = _existing(SMALL_LIBRARIES[kind]), [], f"libkrk_{kind}"
-        return build_dir() / f"{stem}_{_key(sources, defines, [])}.so", sources, defines
+        headers = _existing(ADAPT_HEADERS) if kind == "adapt" else []
+        return build_dir() / f"{stem}_{_key(sources + headers, defines, [])}.so", sources, defines
     elif kind == "parts":
         sources, defines = _existing(PARTS_SOURCES), [f"-DKRK_HEAD_DIM={int(head_dim)}"]
         return build_dir() / f"libkrk_parts_d{int(head_dim)}_{_key(sources, defines, [])}.so", sources, defines
