@@ -28,6 +28,7 @@ _BANK = POINTER(_Bank)
 _ADAPT_SIGNATURES = {
     "krk_step_maps": [_P, _P, _P, _P, c_int, c_int, _P, c_int, c_int, _P, c_int, _P, _P, _P, _P, _P, POINTER(_P), POINTER(_P), POINTER(c_int), c_int, _P, _P],
     "krk_adapter_first": [_P, _P, c_longlong, c_int, c_int, _BANK, _P, _P, c_int, _P],
+    "krk_adapted_gemm": [_P, _P, c_longlong, _P, c_longlong, c_int, c_int, c_int, _BANK, _P, _P, _P, c_int, c_int, _P, _P, c_int, c_int, _P, _P],
     "krk_adapter_second": [_P, _P, _P, c_int, c_int, _BANK, _P, c_int, c_int, _P],
 }
 
@@ -158,6 +159,15 @@ class AdapterOps:
             raise KernelError(f"adapted gate and up: a bank of two parts of {intermediate} outputs is asked for, got {list(bank.outs)}")
         return self._adapted("adapted gate and up", self._resolve(x), w_gate_up, bank, rows, intermediate)
 
+    @staticmethod
+    def _height(rows, N: int) -> int:
+        """Which of the rows' tile heights: the one whose tiles are done first, in rounds of the 74 pairs of SMs."""
+        if len(rows.heights) == 1:
+            return 0
+        cols = -(-N // 256)
+        costs = [-(-(-(-rows.n_rows // h) * cols) // 74) * (h + 8) for h in rows.heights]
+        return min(range(len(costs)), key=costs.__getitem__)
+
     def _adapted(self, what, x, w, bank, rows, gated):
         self._check_adapted(what, x, w, bank, rows)
         (M, K), N = x.shape, w.shape[0]
@@ -165,6 +175,22 @@ class AdapterOps:
         if M == 0:
             return out
         described, dtype, error = self._bank(bank), _code(w.dtype), self.error.data_ptr()
+        ldx, ldw, x_at, w_at = x.stride(0) if M > 1 else K, w.stride(0) if N > 1 else K, x.data_ptr(), w.data_ptr()
+        if w.dtype is torch.bfloat16 and K >= 64 and not (K | ldx | ldw | (gated or N)) & 7 and not (x_at | w_at) & 15:
+            import os
+            shares = M <= 256 and not os.environ.get("NOSHARES")
+            which = self._height(rows, N)
+            height, tiles = rows.heights[which], -(-N // 256)
+            slots = -(-M // height) + rows.n_seqs
+            scratch = slots * height * bank.parts * (-(-bank.rank // 16) * 8)
+            t = self.error.new_empty(scratch + (M * N * (-(-74 // tiles) + 1) if shares else 0))
+            t_at = t.data_ptr()
+            spread = min(rows.n_seqs, bank.capacity, 64) if M <= 256 else min(8, 1 + rows.n_seqs // (M // height))
+            self.launches += 2 if shares else 1
+            self._ok(self.adapt.krk_adapted_gemm(
+                out.data_ptr(), x_at, ldx, w_at, ldw, M, N, K, described, rows.row_adapter.data_ptr(), rows.info[which], rows.list[which], height, slots,
+                t_at, t_at + 4 * scratch if shares else None, int(gated > 0), spread, error, self._stream()), what)
+            return out
         t = self.error.new_empty(M * bank.parts * (-(-bank.rank // 16) * 16))
         if not x.is_contiguous():
             x = x.contiguous()

@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(MAP_THREADS) step_maps_kernel(const Maps m) {
 //
 // A sum's order depends on K alone, so a row gives the same bits whatever stands beside it.
 template <typename T>
-__global__ void __launch_bounds__(256) first_factor_kernel(float* __restrict__ t, const T* __restrict__ x, long long ldx, int K, AdapterBank bank,
+__global__ void __launch_bounds__(256) first_factor_kernel(float* __restrict__ t, const T* __restrict__ x, long long ldx, int K, const __grid_constant__ AdapterBank bank,
                                                            const int* __restrict__ row_adapter, int rows, int* __restrict__ error) {
   grid_launch_dependents();
   grid_dependency_wait();
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(256) first_factor_kernel(float* __restrict__ t
   for (int r = blockIdx.y; r < rows; r += gridDim.y) {
     const int a = row_adapter[r];
     if (a < 0 || a >= bank.capacity) {
-      if ((a < -1 || a >= bank.capacity) && threadIdx.x == 0) atomicExch(error, KRK_ERROR_ADAPTER);
+      if (a >= bank.capacity && threadIdx.x == 0) atomicExch(error, KRK_ERROR_ADAPTER);
       continue;
     }
     for (int i = blockIdx.x * 8 + warp; i < per_row; i += gridDim.x * 8) {
@@ -226,7 +226,7 @@ __device__ __forceinline__ float second_factor(const AdapterBank& bank, const fl
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) second_factor_kernel(T* __restrict__ out, const float* __restrict__ y, const float* __restrict__ t, AdapterBank bank,
+__global__ void __launch_bounds__(256) second_factor_kernel(T* __restrict__ out, const float* __restrict__ y, const float* __restrict__ t, const __grid_constant__ AdapterBank bank,
                                                             const int* __restrict__ row_adapter, int rows, int N, int gated) {
   grid_launch_dependents();
   grid_dependency_wait();

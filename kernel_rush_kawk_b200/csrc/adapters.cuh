@@ -4,7 +4,7 @@
 // begin[p] <= n < begin[p + 1]. A bank holds for adapter `a` the first factors A [parts * rank, K], the second factors B [N, rank] and for
 // each part the rank in use (0: the adapter leaves the part as it is) and the scale:
 //   y[r, n] = sum_k x[r, k] W[n, k] + scale[a, p] sum_j B[a, n, j] (sum_k x[r, k] A[a, p * rank + j, k])      a = row_adapter[r], p of n
-// Rows whose adapter is -1 have none. An adapter that the bank does not hold sets the error word and counts as none.
+// Rows whose adapter is negative have none. An adapter that the bank does not hold sets the error word and counts as none.
 #pragma once
 
 #include "common.cuh"

@@ -40,7 +40,7 @@ SCAN_SOURCES = ["recurrent.cu", "recurrent_chunks.cu", "ssd.cu"]
 MEMORY_SOURCES = ["matrix_memory.cu", "matrix_memory_chunks.cu", "matrix_memory_step.cu"]
 MOE_SOURCES = ["routed.cu", "few_experts.cu", "grouped_gemm.cu"]
 CACHE_SOURCES = ["evict.cu"]
-ADAPT_SOURCES = ["adapters.cu"]
+ADAPT_SOURCES = ["adapters.cu", "adapted_gemm.cu"]
 SMALL_LIBRARIES = {"mix": MIX_SOURCES, "scan": SCAN_SOURCES, "memory": MEMORY_SOURCES, "moe": MOE_SOURCES, "cache": CACHE_SOURCES,
                    "adapt": ADAPT_SOURCES}
 PARTS_SOURCES = ["partial_attention.cu", "few_rows_attention.cu", "many_rows_attention.cu", "prefix_tcgen05.cu", "key_weights_tcgen05.cu"]
