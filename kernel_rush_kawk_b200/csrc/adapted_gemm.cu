@@ -4,19 +4,21 @@
 // for rows that have another. Gated: W and B hold gate rows and then up rows, and C = silu(g) u.
 //
 // first_factor_tiles_kernel makes t = scale (x A^T), rounded to bfloat16 (half a step of 2^-8 of a sum that is itself a part of the result, which is
-// rounded the same way), by mma.sync: 16 rows and 16 ranks a block, K dealt to its eight warps.
+// rounded the same way).
 //
 // adapted_gemm_kernel works in pairs of blocks (cta_group::2): 256 rows of W are the product's M, half of them in each block's shared memory, and a
 // tile's rows, 32 to 256, its N. So a product costs what it has rows, in steps of 32, and W passes once for up to 256 of them. Pairs stay
 // and walk the tiles; an accumulator is half of tensor memory, so that one tile is read back while the next is multiplied.
 //   Whole tiles: every pair takes tiles in turn, the row tiles of 256 columns side by side, and writes C.
-//   Shares: for few rows, where W's bytes are the cost and there are fewer tiles than pairs. The blocks of k of all tiles are
-//   dealt to the pairs in equal runs; what a pair has of a tile goes to scratch in 32 bits, and finish_kernel adds a tile's shares in order.
+//   Shares: the blocks of k of the tiles that make no whole round of the pairs (for few rows, where W's bytes are the cost, of all tiles) are dealt to the
+//   pairs in equal runs; what a pair has of a tile goes to scratch in 32 bits, and finish_kernel adds a tile's shares in order.
 //
 // Warp 0 of either block drives TMA (64 elements of k a stage, 128-byte swizzle) and counts on the first block's barriers; warp 1 of the first
 // block issues tcgen05.mma for both; warps 2 to 9 read accumulators back: a lane is a column of C there and what it holds are rows, so a warp turns
 // 32 x 32 of them through a patch of shared memory. Gate and up rows alternate in the tile, so that neighbouring lanes hold a column's
 // two sums. Every wait is bounded: one that runs out sets the error word, and the blocks leave after freeing their tensor memory.
+#include <cooperative_groups.h>
+
 #include "adapters.cuh"
 #include "mma.cuh"
 #include "tcgen05.cuh"
@@ -29,74 +31,150 @@ using namespace tc;
 // The first factor
 // ---------------------------------------------------------------------------------------------------------------------
 
-// t of the row tiles' adapters, [slot of the list][tile_rows][parts * wide]: zeros where a row has another adapter. Blocks of 16 rows (x), of
-// the tile's adapters in turn (y), of 16 ranks of a part (z). A warp has every eighth block of 32 k; inside one, lane t's 16 bytes are elements 8 t
-// and after for rows and ranks alike, which a sum over k does not mind.
-__global__ void __launch_bounds__(256) first_factor_tiles_kernel(bf16* __restrict__ t, const bf16* __restrict__ x, long long ldx, int K, const __grid_constant__ AdapterBank bank,
-                                                                 const __grid_constant__ AdapterTiles tiles, int* __restrict__ error) {
-  __shared__ float red[8][256];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-  const int r0 = blockIdx.x * 16, tile = r0 / tiles.tile_rows;
-  const int chunks = (bank.rank + 15) / 16, part = blockIdx.z / chunks, j0 = blockIdx.z % chunks * 16;
-  grid_launch_dependents();
+// t of every slot, [slot][tile_rows][parts * wide]: zeros where a row has another adapter than the slot's. A cluster has 128 rows of a slot's tile (y), 64 of the
+// adapter's ranks, all parts' side by side (z), and its `ways` blocks share k. A block multiplies its part of k on the tensor cores (128 rows by 64
+// ranks, fed by TMA in blocks of 64 k); the blocks' sums meet in 32 bits through distributed shared memory, each block adding and writing its share of
+// the rows, in the blocks' order.
+//
+// The product's blocks come in while these run, once what came before is over, and wait for t where they need it; so a block's ring is no larger than
+// fits beside theirs.
+constexpr int FIRST_RANKS = 64, FIRST_STAGES = 3, FIRST_THREADS = 192, FIRST_PITCH = FIRST_RANKS + 4;
+constexpr uint32_t FIRST_X = 128 * 64 * 2, FIRST_STAGE = FIRST_X + FIRST_RANKS * 64 * 2;
+constexpr size_t FIRST_SMEM = 1024 + FIRST_STAGES * FIRST_STAGE;
+static_assert(128 * FIRST_PITCH * 4 <= FIRST_STAGES * FIRST_STAGE, "the sums take the ring's place");
+
+__global__ void __launch_bounds__(FIRST_THREADS) first_factor_tiles_kernel(bf16* __restrict__ t, const __grid_constant__ CUtensorMap map_x,
+                                                                           const __grid_constant__ CUtensorMap map_a, int K,
+                                                                           const __grid_constant__ AdapterBank bank, const __grid_constant__ AdapterTiles tiles,
+                                                                           int ways, int* __restrict__ error) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  float* sums = reinterpret_cast<float*>(ring);  // [128][FIRST_PITCH], when the ring has done its work
+  __shared__ uint64_t full_bar[FIRST_STAGES], empty_bar[FIRST_STAGES], acc_bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int asked_for;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = blockIdx.x % ways, slot = blockIdx.x / ways;
   grid_dependency_wait();
-  const int first = tiles.info[2 * tile], count = tiles.info[2 * tile + 1];
-  const int mine = lane < 16 && r0 + lane < tiles.rows ? tiles.row_adapter[r0 + lane] : -1;
-  const int width = bank.parts * bank.wide;
-  for (int i = blockIdx.y; i < count; i += gridDim.y) {
-    const int a = tiles.list[first + i];
-    if (a >= bank.capacity) {
-      if (threadIdx.x == 0) atomicExch(error, KRK_ERROR_ADAPTER);
-      continue;
+  grid_launch_dependents();  // (the product reads what earlier kernels wrote before it waits)
+  const int2 is = *reinterpret_cast<const int2*>(tiles.slots + 2 * slot);
+  const int a = is.x, r0 = is.y * tiles.tile_rows + blockIdx.y * 128;
+  if (a < 0 || a >= bank.capacity) {  // the whole cluster
+    if (a >= 0 && threadIdx.x == 0) atomicExch(error, KRK_ERROR_ADAPTER);
+    return;
+  }
+  const int here = min(128, min(tiles.tile_rows - (int)blockIdx.y * 128, tiles.rows - r0));  // rows
+  if (here <= 0) return;
+  bool has = false;
+  for (int r = threadIdx.x; r < here; r += FIRST_THREADS) has |= tiles.row_adapter[r0 + r] == a;
+  const int k_blocks = (K + 63) / 64, each = (k_blocks + ways - 1) / ways, b0 = min(way * each, k_blocks), b1 = min(b0 + each, k_blocks);
+  const int n0 = blockIdx.z * FIRST_RANKS, per_adapter = bank.parts * bank.rank;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < FIRST_STAGES; ++s) {
+      mbar_init(full_bar + s, 1);
+      mbar_init(empty_bar + s, 1);
     }
-    const int rank = bank.ranks[a * bank.parts + part];
-    if (j0 >= rank) continue;
-    const unsigned has = __ballot_sync(0xffffffffu, mine == a);
-    bf16* to = t + ((size_t)(first + i) * tiles.tile_rows + (r0 - tile * tiles.tile_rows)) * width + part * bank.wide + j0;
-    if (has == 0) {  // columns come in steps of 16, rows of a multiple of 32 bytes
-      if (threadIdx.x < 32) *reinterpret_cast<uint4*>(to + (size_t)(threadIdx.x >> 1) * width + (threadIdx.x & 1) * 8) = make_uint4(0, 0, 0, 0);
-      continue;
+    mbar_init(&acc_bar, 1);
+    asked_for = -1;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  has = __syncthreads_or(has);
+  if (has) {  // the same for the whole cluster
+    if (warp == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(FIRST_RANKS) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    const bf16* x0 = x + (size_t)min(r0 + g, tiles.rows - 1) * ldx + 8 * q;
-    const bf16* x1 = x + (size_t)min(r0 + g + 8, tiles.rows - 1) * ldx + 8 * q;
-    const bool row0 = has >> g & 1, row1 = has >> (g + 8) & 1, rank0 = j0 + g < rank, rank1 = j0 + 8 + g < rank;
-    const bf16* a0 = reinterpret_cast<const bf16*>(bank.a) + ((size_t)a * bank.parts * bank.rank + part * bank.rank + min(j0 + g, rank - 1)) * K + 8 * q;
-    const bf16* a1 = reinterpret_cast<const bf16*>(bank.a) + ((size_t)a * bank.parts * bank.rank + part * bank.rank + min(j0 + 8 + g, rank - 1)) * K + 8 * q;
-    float acc[2][4] = {};
-    constexpr int DEEP = 5;
-    for (int c = warp * 32; c < K; c += 8 * 32 * DEEP) {
-      uint4 xv[DEEP][2], av[DEEP][2];
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t acc = tmem_slot;
+    if (warp == 0) {
+      for (int b = b0; b < b1; ++b) {
+        const int i = b - b0, s = i % FIRST_STAGES;
+        if (i >= FIRST_STAGES && !__all_sync(0xffffffffu, mbar_wait(empty_bar + s, (i / FIRST_STAGES - 1) & 1))) {
+          if (lane == 0) {
+            atomicExch(error, 3);
+            asked_for = i;
+          }
+          break;
+        }
+        if (lane == 0) {
+          mbar_expect_tx(full_bar + s, FIRST_STAGE);
+          tma_load_2d(ring + s * FIRST_STAGE, &map_x, full_bar + s, b * 64, r0);
+          tma_load_2d(ring + s * FIRST_STAGE + FIRST_X, &map_a, full_bar + s, b * 64, a * per_adapter + n0);
+        }
+        __syncwarp();
+      }
+    } else if (warp == 1) {
+      constexpr uint32_t idesc = umma_idesc(128, FIRST_RANKS);
+      for (int b = b0; b < b1; ++b) {
+        const int i = b - b0, s = i % FIRST_STAGES;
+        if (!__all_sync(0xffffffffu, mbar_wait(full_bar + s, (i / FIRST_STAGES) & 1))) {
+          if (lane == 0) atomicExch(error, 4);
+          break;
+        }
+        tc_fence_after();
+        const uint64_t x_desc = umma_desc(ring + s * FIRST_STAGE), a_desc = umma_desc(ring + s * FIRST_STAGE + FIRST_X);
 #pragma unroll
-      for (int d = 0; d < DEEP; ++d) {
-        const int k = c + d * 256;
-        const bool in = k + 8 * q < K;  // K is a multiple of 8
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        av[d][0] = in && rank0 ? ld_stream_16(a0 + k) : zero;
-        av[d][1] = in && rank1 ? ld_stream_16(a1 + k) : zero;
-        xv[d][0] = in && row0 ? *reinterpret_cast<const uint4*>(x0 + k) : zero;
-        xv[d][1] = in && row1 ? *reinterpret_cast<const uint4*>(x1 + k) : zero;
+        for (int k = 0; k < 4; ++k) umma_bf16_warp(acc, x_desc + k * 2, a_desc + k * 2, idesc, (b > b0 || k > 0) ? 1u : 0u);
+        umma_commit_warp(empty_bar + s);
+      }
+      umma_commit_warp(&acc_bar);  // arrives even after a failed wait, so that all move on
+    }
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(&acc_bar, 0));
+    if (!ok && lane == 0) atomicExch(error, 5);
+    __syncthreads();  // the ring has been read by the products that the barrier stands for
+    if (threadIdx.x == 0 && asked_for >= 0)  // copies on their way end before the ring is written
+      for (int i = max(0, asked_for - FIRST_STAGES); i < asked_for; ++i) mbar_wait(full_bar + i % FIRST_STAGES, (uint32_t)(i / FIRST_STAGES) & 1u, WAIT_LIMIT_NS / 20);
+    __syncthreads();
+    if (warp >= 2) {
+      const int row = (warp & 3) * 32 + lane;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < FIRST_RANKS; c += 32) {
+        uint32_t v[32];
+        tmem_ld_32x32(acc + ((uint32_t)((warp & 3) * 32) << 16) + c, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+          *reinterpret_cast<float4*>(sums + row * FIRST_PITCH + c + j) =
+              b1 > b0 ? make_float4(__uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 1) {
+      tc_fence_after();
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(acc), "r"(FIRST_RANKS) : "memory");
+    }
+    if (ways > 1) cluster_sync();
+  }
+  // eight ranks of a row a thread
+  namespace cg = cooperative_groups;
+  const int share = (here + ways - 1) / ways, first_row = way * share, rows = min(share, here - first_row);
+  const int width = bank.parts * bank.wide;
+  for (int o = threadIdx.x; o < rows * (FIRST_RANKS / 8); o += FIRST_THREADS) {
+    const int row = first_row + o / (FIRST_RANKS / 8), c = o % (FIRST_RANKS / 8) * 8, part = (n0 + c) / bank.rank, j = (n0 + c) % bank.rank;
+    if (part >= bank.parts) continue;
+    bf16* to = t + ((size_t)slot * tiles.tile_rows + blockIdx.y * 128 + row) * width + part * bank.wide + j;
+    uint4 pack = make_uint4(0, 0, 0, 0);
+    if (tiles.row_adapter[r0 + row] == a) {
+      const int rank = bank.ranks[a * bank.parts + part];
+      const float scale = bank.scale[a * bank.parts + part];
+      float v[8] = {};
+      for (int w = 0; w < ways; ++w) {
+        const float* from = (ways > 1 ? cg::this_cluster().map_shared_rank(sums, w) : sums) + row * FIRST_PITCH + c;
+        const float4 lo = *reinterpret_cast<const float4*>(from), hi = *reinterpret_cast<const float4*>(from + 4);
+        v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
+        v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
       }
 #pragma unroll
-      for (int d = 0; d < DEEP; ++d)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          mma_bf16_16816(acc[h], xv[d][0].x, xv[d][1].x, xv[d][0].y, xv[d][1].y, av[d][h].x, av[d][h].y);
-          mma_bf16_16816(acc[h], xv[d][0].z, xv[d][1].z, xv[d][0].w, xv[d][1].w, av[d][h].z, av[d][h].w);
-        }
+      for (int i = 0; i < 8; ++i) v[i] = j + i < rank ? v[i] * scale : 0.f;
+      pack = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) red[warp][(g + (c >> 1) * 8) * 16 + h * 8 + 2 * q + (c & 1)] = acc[h][c];
-    __syncthreads();
-    const int row = threadIdx.x >> 4, j = threadIdx.x & 15;
-    float sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) sum += red[w][threadIdx.x];
-    const bool live = (has >> row & 1) && j0 + j < rank;
-    to[(size_t)row * width + j] = from_float<bf16>(live ? sum * bank.scale[a * bank.parts + part] : 0.f);
-    __syncthreads();
+    *reinterpret_cast<uint4*>(to) = pack;
+    if (j + 8 == bank.rank && bank.wide > bank.rank) *reinterpret_cast<uint4*>(to + 8) = make_uint4(0, 0, 0, 0);  // the product takes whole steps of sixteen
   }
+  if (has && ways > 1) cluster_sync();  // no block leaves while another reads its sums
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -111,17 +189,47 @@ constexpr uint32_t W_BYTES = 128 * BK * 2;  // a block's half of the pair's weig
 constexpr int BUF_COLS = 256;               // tensor memory of an accumulator; there are two
 constexpr int PATCH_PITCH = 80;             // bytes of a row of a warp's patch for the transpose: 16-byte reads of 32 rows meet no bank twice
 constexpr int PATCH_BYTES = 32 * PATCH_PITCH;
-constexpr int RING_BYTES = 196 * 1024, MOST_STAGES = 10;
-constexpr size_t SMEM_BYTES = 1024 + (size_t)RING_BYTES + READERS * PATCH_BYTES + (2 * MOST_STAGES + 5) * 8 + (MOST_STAGES + 4) * 4;
+constexpr int RING_BYTES = 128 * 1024, MOST_STAGES = 7;  // (beside it an SM has room for a block of the first factor's)
+constexpr size_t SMEM_BYTES = 1024 + (size_t)RING_BYTES + READERS * PATCH_BYTES + (2 * MOST_STAGES + 6) * 8 + (MOST_STAGES + 4) * 4;
 
 struct Maps {
   CUtensorMap x, w, t, b[KRK_MAX_PARTS];
 };
 
-__device__ __forceinline__ void tma_load_4d_pair(void* smem_dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y, int z, int u) {
+// Asked for by a whole warp, one lane of which does it (see umma_bf16_warp). With the rest of the producer's loop in a single lane's branch a block of k took
+// some 1,000 clocks, twice what its products take, whatever was loaded.
+__device__ __forceinline__ void tma_load_2d_pair_warp(uint32_t smem_dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-      ::"r"(smem_u32(smem_dst)), "l"(map), "r"(cluster_bar), "r"(x), "r"(y), "r"(z), "r"(u)
+      "{\n.reg .pred q;\n"
+      "elect.sync _|q, 0xffffffff;\n"
+      "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n}"
+      ::"r"(smem_dst), "l"(map), "r"(cluster_bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair_warp(uint32_t smem_dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y, int z) {
+  asm volatile(
+      "{\n.reg .pred q;\n"
+      "elect.sync _|q, 0xffffffff;\n"
+      "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n}"
+      ::"r"(smem_dst), "l"(map), "r"(cluster_bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d_pair_warp(uint32_t smem_dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y, int z, int u) {
+  asm volatile(
+      "{\n.reg .pred q;\n"
+      "elect.sync _|q, 0xffffffff;\n"
+      "@q cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n}"
+      ::"r"(smem_dst), "l"(map), "r"(cluster_bar), "r"(x), "r"(y), "r"(z), "r"(u)
+      : "memory");
+}
+// Leaves a word for who waits on the barrier, and says how many bytes it waits for.
+__device__ __forceinline__ void expect_with_word_warp(uint32_t bar, uint32_t bytes, uint32_t word_at, int word) {
+  asm volatile(
+      "{\n.reg .pred q;\n"
+      "elect.sync _|q, 0xffffffff;\n"
+      "@q st.shared.u32 [%2], %3;\n"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}"
+      ::"r"(bar), "r"(bytes), "r"(word_at), "r"(word)
       : "memory");
 }
 __device__ __forceinline__ void umma_bf16_pair_warp(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -142,21 +250,40 @@ __device__ __forceinline__ void umma_commit_pair_warp(uint64_t* bar) {
       : "memory");
 }
 
-// The work of a pair. Whole tiles: tiles pair, pair + pairs, ... . Shares: of the units of all tiles (a tile's blocks of k, then its adapters, each
-// one unit) in order, `run` from pair * run on.
+// The work of a pair: of the tiles before `shared`, tiles pair, pair + pairs, ... as a whole; of the units of the tiles from there on, in order, `run` from
+// pair * run on. A tile's units are its blocks of k and, where there is a single row tile, its adapters (else they go to who has the last k).
 struct Walk {
-  int units, run, at, end;  // units a tile; the next unit and the last (shares)
-  __device__ Walk(int pair, int units_, int tiles, int pairs) : units(units_) {
-    const long long all = (long long)units * tiles;
-    run = (int)((all + pairs - 1) / pairs);
+  int shared, units, run, at, end, whole, pairs;
+  __device__ Walk(int pair, int pairs_, int tiles, int shared_, int units_) : shared(shared_), units(units_), whole(pair), pairs(pairs_) {
+    const long long all = (long long)units * (tiles - shared);
+    run = max(1, (int)((all + pairs - 1) / pairs));
     at = (int)min((long long)pair * run, all);
     end = (int)min((long long)at + run, all);
   }
+  // tile t, of which units u0 to u1
+  __device__ bool next(int& t, int& u0, int& u1) {
+    if (whole < shared) {
+      t = whole;
+      whole += pairs;
+      u0 = 0;
+      u1 = units;
+      return true;
+    }
+    if (at >= end) return false;
+    t = at / units;
+    u0 = at - t * units;
+    u1 = min(units, u0 + end - at);
+    at += u1 - u0;
+    t += shared;
+    return true;
+  }
+  __device__ int first_pair(int t) const { return (int)((long long)(t - shared) * units / run); }
+  __device__ int count(int t) const { return (int)(((long long)(t - shared + 1) * units - 1) / run) - first_pair(t) + 1; }
 };
 
-template <bool GATED, bool SHARES>
+template <bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS)
-adapted_gemm_kernel(const __grid_constant__ Maps maps, void* __restrict__ out, int N, int K, const __grid_constant__ AdapterBank bank,
+adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, float* __restrict__ shares, int shared, int most_shares, int N, int K, const __grid_constant__ AdapterBank bank,
                     const __grid_constant__ AdapterTiles tiles, int* __restrict__ error) {
   constexpr int BC = GATED ? 64 : 128;  // columns of C a block makes of a tile; the pair twice as many
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -167,7 +294,8 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, void* __restrict__ out, i
   uint64_t* acc_full = empty_bar + MOST_STAGES;   // either block's
   uint64_t* acc_empty = acc_full + 2;             // the first block's: the reading warps of both are through
   uint64_t* drain_bar = acc_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  uint64_t* ready_bar = drain_bar + 1;            // the first block's: the second has its tensor memory
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ready_bar + 1);
   int* issued = reinterpret_cast<int*>(tmem_slot + 1);  // blocks of k that were asked for, where a wait ran out; else -1
   volatile int* steps = issued + 1;  // [stages] of 16 k in the stage; 256 more: the tile's last
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -183,64 +311,61 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, void* __restrict__ out, i
       mbar_init(acc_empty + b, 2 * READERS);
     }
     mbar_init(drain_bar, 1);
+    mbar_init(ready_bar, 1);
     *issued = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  __syncthreads();
+  cluster_sync();  // the other block's barriers exist
+  grid_launch_dependents();
+  // Tensor memory may be held by a block of the first factor's: only those who need it wait for it, while the ring fills.
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * BUF_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    if (rank == 1 && lane == 0) mbar_arrive_cluster(cluster_address(ready_bar, 0));
   }
-  tc_fence_before();
-  __syncthreads();
-  cluster_sync();  // the other block's barriers exist
+  if (warp >= 1) asm volatile("bar.sync 1, %0;" ::"n"(THREADS - 32) : "memory");
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-  grid_launch_dependents();
-  grid_dependency_wait();
+  const uint32_t tmem_base = warp >= 1 ? *tmem_slot : 0;
   const int half = tiles.tile_rows / 2;  // rows that each block of the pair brings
   const uint32_t stage_bytes = W_BYTES + (uint32_t)half * BK * 2;
   const int stages = min(MOST_STAGES, (int)(RING_BYTES / stage_bytes));
   const int k_blocks = (K + BK - 1) / BK, row_tiles = (tiles.rows + tiles.tile_rows - 1) / tiles.tile_rows;
   const int all_tiles = row_tiles * ((N + 2 * BC - 1) / (2 * BC));
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  Walk walk(pair, k_blocks + (SHARES ? tiles.info[1] : 0), all_tiles, pairs);  // (shares have a single row tile)
-  // the tiles of this pair, in order: t, and for shares its units from u0 to u1
-  auto next_tile = [&](int& t, int& u0, int& u1) {
-    if (SHARES) {
-      if (walk.at >= walk.end) return false;
-      t = walk.at / walk.units;
-      u0 = walk.at - t * walk.units;
-      u1 = min(walk.units, u0 + walk.end - walk.at);
-      walk.at += u1 - u0;
-      return true;
-    }
-    t = t < 0 ? pair : t + pairs;
-    u0 = 0;
-    u1 = INT_MAX;
-    return t < all_tiles;
-  };
-  int t = -1, u0, u1;
+  const bool extras = row_tiles == 1;
+  Walk walk(pair, pairs, all_tiles, shared, k_blocks + (extras ? tiles.info[1] : 0));
+  int t, u0, u1;
 
   if (warp == 0) {
     int s = 0, asked = 0;
     uint32_t parity = 1;  // of the round before: a first round finds its stages empty
     bool ok = true;
-    const uint32_t bytes = 2 * stage_bytes;
-    // a stage to fill, by one lane
+    const uint32_t bytes = 2 * stage_bytes, ring_at = smem_u32(ring), steps_at = smem_u32(const_cast<int*>(steps)), own_full = smem_u32(full_bar);
+    const uint32_t first_full = cluster_address(full_bar, 0);
+    uint32_t stage, bar;
+    // a stage to fill
     auto enter = [&](int what) {
-      if (!mbar_wait(empty_bar + s, parity)) {
-        atomicExch(error, 3);
-        *issued = asked;
-        return false;
+      if (!__all_sync(0xffffffffu, mbar_wait(empty_bar + s, parity))) {
+        if (lane == 0) {
+          atomicExch(error, 3);
+          *issued = asked;
+        }
+        return ok = false;
       }
-      if (rank == 0) {
-        steps[s] = what;
-        mbar_expect_tx(full_bar + s, bytes);
-      }
+      if (rank == 0) expect_with_word_warp(own_full + 8 * s, bytes, steps_at + 4 * s, what);
+      stage = ring_at + s * stage_bytes;
+      bar = first_full + 8 * s;
       ++asked;
+      if (++s == stages) { s = 0; parity ^= 1; }
       return true;
     };
-    while (ok && next_tile(t, u0, u1)) {
+    auto shared_block = [&](int kb, int f0, int m0) {
+      if (GATED) tma_load_3d_pair_warp(stage, &maps.w, bar, kb * BK, 0, f0);
+      else tma_load_2d_pair_warp(stage, &maps.w, bar, kb * BK, f0);
+      tma_load_2d_pair_warp(stage + W_BYTES, &maps.x, bar, kb * BK, m0);
+    };
+    while (ok && walk.next(t, u0, u1)) {
       const int rt = t % row_tiles, wt = t / row_tiles, f0 = (wt * 2 + (int)rank) * BC, m0 = rt * tiles.tile_rows + (int)rank * half;
       const int first = tiles.info[2 * rt], count = tiles.info[2 * rt + 1];
       // which parts the pair's columns reach into (gated: both)
@@ -249,12 +374,12 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, void* __restrict__ out, i
         p0 = part_of(bank, wt * 2 * BC);
         p1 = part_of(bank, min(N, (wt + 1) * 2 * BC) - 1) + 1;
       }
-      const int e0 = max(0, u0 - k_blocks), e1 = min(count, u1 - k_blocks);  // adapters of the list
+      const int e0 = extras ? max(0, u0 - k_blocks) : 0, e1 = extras ? u1 - k_blocks : u1 == k_blocks ? count : 0;  // of the tile's adapters
       // a lane's adapter of the list, and its parts' ranks in steps of 16, a byte each
       int a = -1;
       uint32_t ranks = 0;
       auto look = [&](int i) {
-        a = i + lane < e1 ? tiles.list[first + i + lane] : -1;
+        a = i + lane < e1 ? tiles.slots[2 * (first + i + lane)] : -1;
         ranks = 0;
         if (a >= 0 && a < bank.capacity)
           for (int p = p0; p < p1; ++p) ranks |= (uint32_t)((bank.ranks[a * bank.parts + p] + 15) / 16) << 8 * p;
@@ -267,51 +392,34 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, void* __restrict__ out, i
         left += __reduce_add_sync(0xffffffffu, n);
       }
       const int k1 = min(k_blocks, u1);
-      if (lane == 0) {
-        for (int kb = u0; kb < k1 && ok; ++kb) {
-          if (!(ok = enter(4 | (kb + 1 == k1 && left == 0 ? 256 : 0)))) break;
-          unsigned char* stage = ring + s * stage_bytes;
-          const uint32_t bar = cluster_address(full_bar + s, 0);
-          if (GATED) tma_load_3d_pair(stage, &maps.w, bar, kb * BK, 0, f0);
-          else tma_load_2d_pair(stage, &maps.w, bar, kb * BK, f0);
-          tma_load_2d_pair(stage + W_BYTES, &maps.x, bar, kb * BK, m0);
-          if (++s == stages) { s = 0; parity ^= 1; }
-        }
-        if (SHARES && ok && u0 >= k1 && left == 0) {  // a share of adapters that leave these columns as they are: zeros from behind the last k
-          if ((ok = enter(1 | 256))) {
-            unsigned char* stage = ring + s * stage_bytes;
-            const uint32_t bar = cluster_address(full_bar + s, 0);
-            if (GATED) tma_load_3d_pair(stage, &maps.w, bar, k_blocks * BK, 0, f0);
-            else tma_load_2d_pair(stage, &maps.w, bar, k_blocks * BK, f0);
-            tma_load_2d_pair(stage + W_BYTES, &maps.x, bar, k_blocks * BK, m0);
-            if (++s == stages) { s = 0; parity ^= 1; }
-          }
-        }
+      for (int kb = u0; kb < k1; ++kb) {
+        if (!enter(4 | (kb + 1 == k1 && left == 0 ? 256 : 0))) break;
+        shared_block(kb, f0, m0);
       }
-      for (int i = e0; i < e1; ++i) {
+      // a share of adapters that leave these columns as they are: zeros from behind the last k
+      if (ok && u0 >= k1 && left == 0 && enter(1 | 256)) shared_block(k_blocks, f0, m0);
+      for (int i = e0; i < e1 && ok; ++i) {
         if ((i - e0) % 32 == 0) look(i);
+        grid_dependency_wait();  // t
         const int ai = __shfl_sync(0xffffffffu, a, (i - e0) % 32);
         const uint32_t of = __shfl_sync(0xffffffffu, ranks, (i - e0) % 32);
-        if (lane == 0 && ok)
-          for (int p = p0; p < p1 && ok; ++p)
-            for (int r = of >> 8 * p & 255, kb = 0; r > 0; r -= 4, ++kb) {
-              --left;
-              if (!(ok = enter(min(r, 4) | (left == 0 ? 256 : 0)))) break;
-              unsigned char* stage = ring + s * stage_bytes;
-              const uint32_t bar = cluster_address(full_bar + s, 0);
-              if (GATED) tma_load_4d_pair(stage, &maps.b[p], bar, kb * BK, -p, f0, ai);
-              else tma_load_3d_pair(stage, &maps.b[p], bar, kb * BK, f0 - bank.begin[p], ai);
-              tma_load_2d_pair(stage + W_BYTES, &maps.t, bar, p * bank.wide + kb * BK, (first + i) * tiles.tile_rows + (int)rank * half);
-              if (++s == stages) { s = 0; parity ^= 1; }
-            }
+        for (int p = p0; p < p1 && ok; ++p)
+          for (int r = of >> 8 * p & 255, kb = 0; r > 0; r -= 4, ++kb) {
+            --left;
+            if (!enter(min(r, 4) | (left == 0 ? 256 : 0))) break;
+            if (GATED) tma_load_4d_pair_warp(stage, &maps.b[p], bar, kb * BK, -p, f0, ai);
+            else tma_load_3d_pair_warp(stage, &maps.b[p], bar, kb * BK, f0 - bank.begin[p], ai);
+            tma_load_2d_pair_warp(stage + W_BYTES, &maps.t, bar, p * bank.wide + kb * BK, (first + i) * tiles.tile_rows + (int)rank * half);
+          }
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
     }
-    if (lane == 0 && ok)  // the last stages' releases, too, have arrived before the block leaves
+    if (ok)  // the last stages' releases, too, have arrived before the block leaves
       for (int i = 0; i < stages; ++i) {
-        if (!mbar_wait(empty_bar + s, parity)) {
-          atomicExch(error, 3);
-          *issued = asked;
+        if (!__all_sync(0xffffffffu, mbar_wait(empty_bar + s, parity))) {
+          if (lane == 0) {
+            atomicExch(error, 3);
+            *issued = asked;
+          }
           break;
         }
         if (++s == stages) { s = 0; parity ^= 1; }
@@ -319,9 +427,10 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, void* __restrict__ out, i
   } else if (warp == 1) {
     int s = 0, buf = 0;
     uint32_t parity = 0, acc_parity = 1;
-    bool ok = rank == 0;
+    bool ok = rank == 0 && __all_sync(0xffffffffu, mbar_wait(ready_bar, 0));
+    if (rank == 0 && !ok && lane == 0) atomicExch(error, 4);
     const uint32_t idesc = umma_idesc(256, tiles.tile_rows);
-    while (ok && next_tile(t, u0, u1)) {
+    while (ok && walk.next(t, u0, u1)) {
       const uint32_t acc = tmem_base + (uint32_t)buf * BUF_COLS;
       ok = mbar_wait(acc_empty + buf, acc_parity);  // both blocks have read what was there
       ok = __all_sync(0xffffffffu, ok);
@@ -367,7 +476,7 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, void* __restrict__ out, i
     unsigned char* patch = patches + (warp - 2) * PATCH_BYTES;
     int buf = 0;
     uint32_t parity = 0;
-    while (next_tile(t, u0, u1)) {
+    while (walk.next(t, u0, u1)) {
       if (!__all_sync(0xffffffffu, mbar_wait(acc_full + buf, parity))) {
         if (lane == 0) atomicExch(error, 5);
         break;
@@ -376,20 +485,16 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, void* __restrict__ out, i
       const int rt = t % row_tiles, wt = t / row_tiles, m0 = rt * tiles.tile_rows;
       const int live_rows = min(tiles.tile_rows, tiles.rows - m0);
       const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)buf * BUF_COLS;
-      if (SHARES) {
-        // [share of the tile][row][column of W, gate and up in turn where gated]: a lane's column, 32 of them side by side
-        const int first_pair = (int)((long long)t * walk.units / walk.run);
-        const int column = (wt * 2 + (int)rank) * 128 + quarter * 32 + lane, columns = GATED ? 2 * N : N;
-        float* dst = reinterpret_cast<float*>(out) + (size_t)(pair - first_pair) * tiles.rows * columns + column;
+      if (t >= shared) {
+        // [tile][share][row][256 rows of W, gate and up in turn where gated]: a lane's column, 32 of them side by side
+        float* dst = shares + ((size_t)((t - shared) * most_shares + pair - walk.first_pair(t)) * tiles.tile_rows) * 256 + rank * 128 + quarter * 32 + lane;
         for (int c0 = (warp - 2) / 4 * 32; c0 < live_rows; c0 += 32 * (READERS / 4)) {
           uint32_t v[32];
           tmem_ld_32x32(acc + (uint32_t)c0, v);
           tmem_wait_ld();
-          if (column < columns) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (c0 + j < live_rows) dst[(size_t)(c0 + j) * columns] = __uint_as_float(v[j]);
-          }
+          for (int j = 0; j < 32; ++j)
+            if (c0 + j < live_rows) dst[(size_t)(c0 + j) * 256] = __uint_as_float(v[j]);
         }
       } else {
         constexpr int MINE = BC / 4;  // columns of this warp
@@ -415,12 +520,15 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, void* __restrict__ out, i
               for (int j = 0; j < 32; ++j) *reinterpret_cast<bf16*>(patch + j * PATCH_PITCH + lane * 2) = from_float<bf16>(__uint_as_float(v[j]));
             }
             __syncwarp();
-            if (c0 + lane < live_rows) {
-              bf16* dst = reinterpret_cast<bf16*>(out) + (size_t)(m0 + c0 + lane) * N + f0;
+            // neighbouring lanes have a row's 16 bytes each: whole sectors at once (N is a multiple of 8)
+            constexpr int PER = MINE / 8, STEP = 32 / PER;
+            const int j = lane % PER * 8;
+            if (f0 + j < N)
 #pragma unroll
-              for (int j = 0; j < MINE; j += 8)  // N is a multiple of 8
-                if (f0 + j < N) *reinterpret_cast<uint4*>(dst + j) = *reinterpret_cast<const uint4*>(patch + lane * PATCH_PITCH + j * 2);
-            }
+              for (int r = lane / PER; r < 32; r += STEP)
+                if (c0 + r < live_rows)
+                  *reinterpret_cast<uint4*>(out + (size_t)(m0 + c0 + r) * N + f0 + j) =
+                      *reinterpret_cast<const uint4*>(patch + r * PATCH_PITCH + j * 2);
             __syncwarp();
           }
         }
@@ -433,6 +541,7 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, void* __restrict__ out, i
     }
   }
   __syncwarp();
+  grid_dependency_wait();  // who waits for this kernel waits for the first factor's as well
   tc_fence_before();
   __syncthreads();
   if (rank == 0 && threadIdx.x == 0 && *issued >= 0)  // copies on their way end before shared memory is given up
@@ -445,30 +554,31 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, void* __restrict__ out, i
   }
 }
 
-// The shares of a tile's columns, added in the pairs' order. A block has a tile's 256 columns of W and four rows.
+// The shares of a tile, added in the pairs' order. A block has a tile's 256 columns (x) of four rows (y).
 template <bool GATED>
-__global__ void __launch_bounds__(256) finish_kernel(bf16* __restrict__ out, const float* __restrict__ shares, int rows, int columns, int k_blocks, int pairs,
-                                                     const int* __restrict__ info) {
+__global__ void __launch_bounds__(256) finish_kernel(bf16* __restrict__ out, const float* __restrict__ shares, int shared, int most_shares, int N, int k_blocks,
+                                                     int pairs, const __grid_constant__ AdapterTiles tiles) {
   grid_launch_dependents();
   grid_dependency_wait();
-  const Walk walk(0, k_blocks + info[1], gridDim.x, pairs);
-  const int tile = blockIdx.x, r = blockIdx.y * 4 + threadIdx.x / 64, column = tile * 256 + threadIdx.x % 64 * 4;
-  const int count = (int)((((long long)tile + 1) * walk.units - 1) / walk.run - (long long)tile * walk.units / walk.run) + 1;
-  if (r >= rows || column >= columns) return;
-  const float* from = shares + (size_t)r * columns + column;
+  const int row_tiles = (tiles.rows + tiles.tile_rows - 1) / tiles.tile_rows, all_tiles = shared + gridDim.x;
+  const Walk walk(0, pairs, all_tiles, shared, k_blocks + (row_tiles == 1 ? tiles.info[1] : 0));
+  const int t = shared + blockIdx.x, rt = t % row_tiles, wt = t / row_tiles, r = blockIdx.y * 4 + threadIdx.x / 64, column = threadIdx.x % 64 * 4;
+  const int row = rt * tiles.tile_rows + r, n = GATED ? wt * 128 + column / 2 : wt * 256 + column;
+  if (r >= tiles.tile_rows || row >= tiles.rows || n >= N) return;
+  const int count = walk.count(t);
+  const float* from = shares + ((size_t)blockIdx.x * most_shares * tiles.tile_rows + r) * 256 + column;
   float4 sum = *reinterpret_cast<const float4*>(from);
   for (int i = 1; i < count; ++i) {
-    const float4 more = *reinterpret_cast<const float4*>(from + (size_t)i * rows * columns);
+    const float4 more = *reinterpret_cast<const float4*>(from + (size_t)i * tiles.tile_rows * 256);
     sum.x += more.x;
     sum.y += more.y;
     sum.z += more.z;
     sum.w += more.w;
   }
   if (GATED) {
-    *reinterpret_cast<uint32_t*>(out + (size_t)r * (columns / 2) + column / 2) =
-        pack_bf16x2(sum.x / (1.0f + expf(-sum.x)) * sum.y, sum.z / (1.0f + expf(-sum.z)) * sum.w);
+    *reinterpret_cast<uint32_t*>(out + (size_t)row * N + n) = pack_bf16x2(sum.x / (1.0f + expf(-sum.x)) * sum.y, sum.z / (1.0f + expf(-sum.z)) * sum.w);
   } else {
-    *reinterpret_cast<uint2*>(out + (size_t)r * columns + column) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
+    *reinterpret_cast<uint2*>(out + (size_t)row * N + n) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
   }
 }
 
@@ -496,53 +606,86 @@ int make_map_b(CUtensorMap* map, const AdapterBank& bank, int part, int N, bool 
   return make_map(map, base, 3, size, stride, box);
 }
 
-template <bool GATED, bool SHARES>
-int launch_gemm(const Maps& maps, void* out, int N, int K, const AdapterBank& bank, const AdapterTiles& tiles, int pairs, int* error, cudaStream_t stream) {
+int launch_first(bf16* t, const CUtensorMap& map_x, const CUtensorMap& map_a, int K, const AdapterBank& bank, const AdapterTiles& tiles, int* error, cudaStream_t stream) {
+  // an SM gives its memory to L1 or to blocks anew only when it is empty: split as the product's blocks need it, they come in beside these
+  static unsigned long long told = 0, allowed = 0;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && !(__atomic_load_n(&told, __ATOMIC_RELAXED) >> (device & 63) & 1)) {
+    e = cudaFuncSetAttribute(first_factor_tiles_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess) __atomic_fetch_or(&told, 1ull << (device & 63), __ATOMIC_RELAXED);
+  }
+  if (e == cudaSuccess) e = allow_shared(first_factor_tiles_kernel, FIRST_SMEM, &allowed);
+  if (e != cudaSuccess) return (int)e;
+  const int parts = (min(tiles.tile_rows, tiles.rows) + 127) / 128, chunks = (bank.parts * bank.rank + FIRST_RANKS - 1) / FIRST_RANKS;
+  const long long blocks = (long long)tiles.n_slots * parts * chunks;
+  int ways = 1;
+  while (ways < 8 && ways * blocks <= 2 * PAIRS && K >= 64 * 2 * ways) ways *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(tiles.n_slots * ways, parts, chunks);
+  cfg.blockDim = dim3(FIRST_THREADS);
+  cfg.dynamicSmemBytes = FIRST_SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ways;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  static const bool plain = getenv("KRK_NO_PDL") != nullptr;
+  cfg.attrs = attr;
+  cfg.numAttrs = plain ? 1 : 2;
+  return (int)cudaLaunchKernelEx(&cfg, first_factor_tiles_kernel, t, map_x, map_a, K, bank, tiles, ways, error);
+}
+
+template <bool GATED>
+int launch_gemm(const Maps& maps, bf16* out, float* shares, int shared, int most_shares, int N, int K, const AdapterBank& bank, const AdapterTiles& tiles, int pairs,
+                int* error, cudaStream_t stream) {
   static unsigned long long allowed = 0;
-  auto kern = adapted_gemm_kernel<GATED, SHARES>;
+  auto kern = adapted_gemm_kernel<GATED>;
   const cudaError_t e = allow_shared(kern, SMEM_BYTES, &allowed);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(kern, dim3(2 * pairs), dim3(THREADS), SMEM_BYTES, stream, maps, out, N, K, bank, tiles, error);
+  return (int)launch_pdl(kern, dim3(2 * pairs), dim3(THREADS), SMEM_BYTES, stream, maps, out, shares, shared, most_shares, N, K, bank, tiles, error);
 }
 
 }  // namespace
 
-// out [rows, N] (gated: [rows, N / 2]) bfloat16 from x [rows, K] (row stride ldx) and w [N, K] (row stride ldw), by tiles of tile_rows rows. t: scratch of
-// `slots` * tile_rows * parts * wide bfloat16, as many slots as the lists have (tiles and sequences together). shares: float32 scratch of
-// (74 / tiles of 256 columns, rounded up, and one more) * rows * N, or null for whole tiles; shares take one row tile. spread: how many of a tile's
-// adapters are taken side by side by the first factor.
+// out [rows, N] (gated: [rows, N / 2]) bfloat16 from x [rows, K] (row stride ldx) and w [N, K] (row stride ldw), by tiles of tile_rows rows and 256 rows of w, the
+// first `shared` of them as whole ones (a multiple of 74, or all). t: scratch of n_slots * tile_rows * parts * wide bfloat16. shares: float32 scratch of the
+// other tiles' number times (74 / their number, rounded up, and one more) * tile_rows * 256, or null where there are none.
 KRK_API int krk_adapted_gemm(void* out, const void* x, long long ldx, const void* w, long long ldw, int rows, int N, int K, const AdapterBank* bank,
-                             const int* row_adapter, const int* info, const int* list, int tile_rows, int slots, void* t, float* shares, int gated, int spread,
+                             const int* row_adapter, const int* info, const int* slots, int n_slots, int tile_rows, void* t, float* shares, int shared, int gated,
                              int* error, cudaStream_t stream) {
   if (rows == 0 || N == 0) return 0;
   const int width = gated ? N / 2 : N;
-  if (K < 64 || K % 8 || width % 8 || ldx % 8 || ldw % 8 || tile_rows % 32 || tile_rows < 32 || tile_rows > 256 || (shares && rows > tile_rows) || spread < 1 ||
+  if (K < 64 || K % 8 || width % 8 || ldx % 8 || ldw % 8 || tile_rows % 32 || tile_rows < 32 || tile_rows > 256 || n_slots < 1 ||
       (((uintptr_t)x | (uintptr_t)w | (uintptr_t)out | (uintptr_t)bank->a | (uintptr_t)bank->b | (uintptr_t)t | (uintptr_t)shares) & 15))
     return -2;
-  const AdapterTiles tiles = {row_adapter, info, list, rows, tile_rows};
+  const AdapterTiles tiles = {row_adapter, info, slots, rows, tile_rows, n_slots};
   const long long all = (long long)((rows + tile_rows - 1) / tile_rows) * ((N + 255) / 256);
-  if (all * (K / 64 + 1 + slots) > 0x7fffffffLL || (long long)slots * tile_rows > 0x7fffffffLL) return -3;
+  const int k_blocks = (K + BK - 1) / BK, per_adapter = bank->parts * bank->rank;
+  if (all * (k_blocks + n_slots) > 0x7fffffffLL || (long long)n_slots * tile_rows > 0x7fffffffLL || (long long)n_slots * 8 > 0x7fffffffLL ||
+      (long long)bank->capacity * per_adapter > 0x7fffffffLL)
+    return -3;
+  if (shared < 0 || shared > all || (shared < all && (shared % PAIRS || !shares))) return -2;
   Maps maps;
+  CUtensorMap map_x, map_a;
   int rc = make_map_bf16(&maps.x, x, rows, K, ldx, tile_rows / 2);
   if (rc) return rc;
   rc = gated ? make_map_bf16_3d(&maps.w, w, K, 2, width, (long long)width * ldw, ldw, 2, 64) : make_map_bf16(&maps.w, w, N, K, ldw, 128);
-  if (rc) return rc;
-  rc = make_map_bf16(&maps.t, t, (long long)slots * tile_rows, bank->parts * bank->wide, bank->parts * bank->wide, tile_rows / 2);
+  if (!rc) rc = make_map_bf16(&maps.t, t, (long long)n_slots * tile_rows, bank->parts * bank->wide, bank->parts * bank->wide, tile_rows / 2);
   for (int p = 0; p < bank->parts && !rc; ++p) rc = make_map_b(&maps.b[p], *bank, p, N, gated);
+  if (!rc) rc = make_map_bf16(&map_x, x, rows, K, ldx, 128);
+  if (!rc) rc = make_map_bf16(&map_a, bank->a, (long long)bank->capacity * per_adapter, K, K, FIRST_RANKS);
+  if (!rc) rc = launch_first((bf16*)t, map_x, map_a, K, *bank, tiles, error, stream);
   if (rc) return rc;
-  const dim3 grid((rows + 15) / 16, spread, bank->parts * ((bank->rank + 15) / 16));
-  rc = (int)launch_pdl(first_factor_tiles_kernel, grid, dim3(256), 0, stream, (bf16*)t, (const bf16*)x, ldx, K, *bank, tiles, error);
-  if (rc) return rc;
-  const int k_blocks = (K + BK - 1) / BK;
-  if (!shares) {
-    const int pairs = all < PAIRS ? (int)all : PAIRS;
-    return gated ? launch_gemm<true, false>(maps, out, width, K, *bank, tiles, pairs, error, stream)
-                 : launch_gemm<false, false>(maps, out, width, K, *bank, tiles, pairs, error, stream);
-  }
-  rc = gated ? launch_gemm<true, true>(maps, shares, width, K, *bank, tiles, PAIRS, error, stream)
-             : launch_gemm<false, true>(maps, shares, width, K, *bank, tiles, PAIRS, error, stream);
-  if (rc) return rc;
-  const dim3 blocks((N + 255) / 256, (rows + 3) / 4);
-  return gated ? (int)launch_pdl(finish_kernel<true>, blocks, dim3(256), 0, stream, (bf16*)out, (const float*)shares, rows, N, k_blocks, PAIRS, info)
-               : (int)launch_pdl(finish_kernel<false>, blocks, dim3(256), 0, stream, (bf16*)out, (const float*)shares, rows, N, k_blocks, PAIRS, info);
+  const int rest = (int)(all - shared), most_shares = rest ? (PAIRS + rest - 1) / rest + 1 : 0;
+  const int pairs = rest || all > PAIRS ? PAIRS : (int)all;
+  rc = gated ? launch_gemm<true>(maps, (bf16*)out, shares, shared, most_shares, width, K, *bank, tiles, pairs, error, stream)
+             : launch_gemm<false>(maps, (bf16*)out, shares, shared, most_shares, width, K, *bank, tiles, pairs, error, stream);
+  if (rc || !rest) return rc;
+  const dim3 blocks(rest, (min(rows, tile_rows) + 3) / 4);
+  return gated ? (int)launch_pdl(finish_kernel<true>, blocks, dim3(256), 0, stream, (bf16*)out, (const float*)shares, shared, most_shares, width, k_blocks, PAIRS, tiles)
+               : (int)launch_pdl(finish_kernel<false>, blocks, dim3(256), 0, stream, (bf16*)out, (const float*)shares, shared, most_shares, width, k_blocks, PAIRS, tiles);
 }

@@ -8,6 +8,7 @@ others, never share any.
 from __future__ import annotations
 
 import ctypes
+import os
 from ctypes import POINTER, Structure, byref, c_float, c_int, c_longlong, c_void_p
 
 import torch
@@ -43,14 +44,16 @@ class AdapterRows:
         self.n_rows, self.n_seqs = n_rows, n_seqs
         self.heights = self.HEIGHTS if n_rows > 256 else (max(32, -(-n_rows // 32) * 32),)
         tiles = [-(-n_rows // h) for h in self.heights]
-        self.buffer = torch.empty(n_rows + sum(3 * t + n_seqs for t in tiles), dtype=_I32, device=device)
+        self.n_slots = [t + n_seqs for t in tiles]
+        at = n_rows + n_rows % 2  # pairs of words lie on boundaries of theirs
+        self.buffer = torch.empty(at + sum(2 * t + 2 * s for t, s in zip(tiles, self.n_slots)), dtype=_I32, device=device)
         self.row_adapter = self.buffer[:n_rows]
-        at, address = n_rows, self.buffer.data_ptr()
-        self.info, self.list = [], []  # addresses
-        for t in tiles:
+        address = self.buffer.data_ptr()
+        self.info, self.slots = [], []  # addresses
+        for t, s in zip(tiles, self.n_slots):
             self.info.append(address + 4 * at)
-            self.list.append(address + 4 * (at + 2 * t))
-            at += 3 * t + n_seqs
+            self.slots.append(address + 4 * (at + 2 * t))
+            at += 2 * t + 2 * s
 
 
 class StepMaps:
@@ -115,7 +118,7 @@ class AdapterOps:
             count = 0
         else:
             count = len(rows.heights)
-            info, lists, heights = (_P * count)(*rows.info), (_P * count)(*rows.list), (c_int * count)(*rows.heights)
+            info, lists, heights = (_P * count)(*rows.info), (_P * count)(*rows.slots), (c_int * count)(*rows.heights)
         self._ok(self.adapt.krk_step_maps(
             slots.data_ptr(), starts.data_ptr(), lengths.data_ptr(), _ptr(adapters), n, n_rows, _ptr(table), width, n_slots, _ptr(pages), n_pages,
             out.cu_q.data_ptr(), out.row_seq.data_ptr(), out.row_pos.data_ptr(), None if rows is None else rows.row_adapter.data_ptr(),
@@ -159,14 +162,25 @@ class AdapterOps:
             raise KernelError(f"adapted gate and up: a bank of two parts of {intermediate} outputs is asked for, got {list(bank.outs)}")
         return self._adapted("adapted gate and up", self._resolve(x), w_gate_up, bank, rows, intermediate)
 
-    @staticmethod
-    def _height(rows, N: int) -> int:
-        """Which of the rows' tile heights: the one whose tiles are done first, in rounds of the 74 pairs of SMs."""
+    PAIRS = 74  # of SMs
+
+    def _tiling(self, rows, M: int, K: int, N: int) -> tuple[int, int]:
+        """(which of the rows' tile heights, the first tile that the pairs share): by the time of whole rounds of the pairs, or of whole rounds
+        and shares of what is left, in clocks."""
         if len(rows.heights) == 1:
-            return 0
-        cols = -(-N // 256)
-        costs = [-(-(-(-rows.n_rows // h) * cols) // 74) * (h + 8) for h in rows.heights]
-        return min(range(len(costs)), key=costs.__getitem__)
+            return 0, 0
+        if os.environ.get('TR'):
+            h = int(os.environ['TR']); i = rows.heights.index(h); tiles = -(-M // h) * -(-N // 256)
+            return i, (tiles if os.environ.get('NOSH') else tiles // 74 * 74)
+        best = None
+        for i, h in enumerate(rows.heights):
+            tiles = -(-M // h) * -(-N // 256)
+            tile = -(-K // 64) * (176 + 1.3125 * h)
+            whole, rest = divmod(tiles, self.PAIRS)
+            for cost, shared in (((whole + (rest > 0)) * tile, tiles), (whole * tile + rest / self.PAIRS * tile + 6000 + (self.PAIRS + rest) * h / 2, tiles - rest)):
+                if best is None or cost < best[0]:
+                    best = cost, i, shared
+        return best[1], best[2]
 
     def _adapted(self, what, x, w, bank, rows, gated):
         self._check_adapted(what, x, w, bank, rows)
@@ -177,19 +191,17 @@ class AdapterOps:
         described, dtype, error = self._bank(bank), _code(w.dtype), self.error.data_ptr()
         ldx, ldw, x_at, w_at = x.stride(0) if M > 1 else K, w.stride(0) if N > 1 else K, x.data_ptr(), w.data_ptr()
         if w.dtype is torch.bfloat16 and K >= 64 and not (K | ldx | ldw | (gated or N)) & 7 and not (x_at | w_at) & 15:
-            import os
-            shares = M <= 256 and not os.environ.get("NOSHARES")
-            which = self._height(rows, N)
-            height, tiles = rows.heights[which], -(-N // 256)
-            slots = -(-M // height) + rows.n_seqs
-            scratch = slots * height * bank.parts * (-(-bank.rank // 16) * 8)
-            t = self.error.new_empty(scratch + (M * N * (-(-74 // tiles) + 1) if shares else 0))
+            which, shared = self._tiling(rows, M, K, N)
+            height = rows.heights[which]
+            n_slots, tiles = rows.n_slots[which], -(-M // height) * -(-N // 256)
+            t_words = n_slots * height * bank.parts * (-(-bank.rank // 16) * 8)
+            rest = tiles - shared
+            t = self.error.new_empty(t_words + (rest * (-(-self.PAIRS // rest) + 1) * height * 256 if rest else 0))
             t_at = t.data_ptr()
-            spread = min(rows.n_seqs, bank.capacity, 64) if M <= 256 else min(8, 1 + rows.n_seqs // (M // height))
-            self.launches += 2 if shares else 1
+            self.launches += 2 if rest else 1
             self._ok(self.adapt.krk_adapted_gemm(
-                out.data_ptr(), x_at, ldx, w_at, ldw, M, N, K, described, rows.row_adapter.data_ptr(), rows.info[which], rows.list[which], height, slots,
-                t_at, t_at + 4 * scratch if shares else None, int(gated > 0), spread, error, self._stream()), what)
+                out.data_ptr(), x_at, ldx, w_at, ldw, M, N, K, described, rows.row_adapter.data_ptr(), rows.info[which], rows.slots[which], n_slots, height,
+                t_at, t_at + 4 * t_words if rest else None, shared, int(gated > 0), error, self._stream()), what)
             return out
         t = self.error.new_empty(M * bank.parts * (-(-bank.rank // 16) * 16))
         if not x.is_contiguous():

@@ -12,8 +12,8 @@ namespace {
 // One launch, whose blocks do not wait on one another: each adds up all sequences' lengths and new pages for itself (a thousand sequences
 // are 8 KB out of L2) and takes 768 rows, which are whole tiles of 128, 192 and 256. A row finds its sequence by bisection. The row at the
 // first position of a new page writes the table's entry; places of other rows on that page come from the list of pages, not from the table.
-// A tile's list begins at (tile + sequence of its first row): every earlier tile had no more adapters than sequences, and a sequence is
-// counted once more for each tile that it goes on into, so lists never meet, and no block needs another's count.
+// A tile's slots begin at (tile + sequence of its first row): every earlier tile had no more adapters than sequences, and a sequence is
+// counted once more for each tile that it goes on into, so tiles never meet in them, and no block needs another's count.
 constexpr int MAP_ROWS = 768, MAP_THREADS = 256;
 
 struct Maps {
@@ -153,9 +153,13 @@ __global__ void __launch_bounds__(MAP_THREADS) step_maps_kernel(const Maps m) {
     const int tile_rows = m.tile_rows[l];
     for (int r0 = first + warp * tile_rows; r0 < last; r0 += MAP_THREADS / 32 * tile_rows) {
       const int tile = r0 / tile_rows;
-      int count = 0, lo = 0;
+      const int tiles = (m.n_rows + tile_rows - 1) / tile_rows;
+      // where the slots of a tile begin: the first tile's at 0; behind the last sequence, as if there were one more
+      auto begin_of = [&](int i) { return i == 0 ? 0 : i == tiles ? tiles + m.n_seqs : i + (i * tile_rows < covered ? seq_of(i * tile_rows) : m.n_seqs); };
+      const int begin = begin_of(tile), end = begin_of(tile + 1);
+      int count = 0;
       if (r0 < covered) {
-        lo = seq_of(r0);
+        const int lo = seq_of(r0);
         const int hi = seq_of(min(min(r0 + tile_rows, m.n_rows), covered) - 1);
         for (int s = lo; s <= hi; s += 32) {
           const int mine = s + lane;
@@ -168,16 +172,14 @@ __global__ void __launch_bounds__(MAP_THREADS) step_maps_kernel(const Maps m) {
           const int at = count + __popc(all & ((1u << lane) - 1));
           if (is_new) {
             found[warp][at] = a;
-            m.list[l][tile + lo + at] = a;
+            *reinterpret_cast<int2*>(m.list[l] + 2 * (begin + at)) = make_int2(a, tile);
           }
           count += __popc(all);
           __syncwarp();
         }
       }
-      if (lane == 0) {
-        m.info[l][2 * tile] = tile + lo;
-        m.info[l][2 * tile + 1] = count;
-      }
+      if (lane == 0) *reinterpret_cast<int2*>(m.info[l] + 2 * tile) = make_int2(begin, count);
+      for (int i = begin + count + lane; i < end; i += 32) *reinterpret_cast<int2*>(m.list[l] + 2 * i) = make_int2(-1, tile);
       __syncwarp();
     }
   }

@@ -23,12 +23,13 @@ struct AdapterBank {
   int wide;            // columns of t for a part: rank, up to the next multiple of 16
 };
 
-// The rows in tiles, and the adapters that a tile's rows have: tile i has info[2 * i + 1] of them, at list[info[2 * i]] and after.
+// The rows in tiles, and the adapters that a tile's rows have: tile i has info[2 * i + 1] of them, in the slots from info[2 * i] on. A slot has an adapter
+// and its tile; -1 for a slot that is not used.
 struct AdapterTiles {
   const int* row_adapter;  // [rows]
   const int* info;         // [tiles, 2]
-  const int* list;
-  int rows, tile_rows;
+  const int* slots;        // [n_slots, 2]
+  int rows, tile_rows, n_slots;
 };
 
 __device__ __forceinline__ int part_of(const AdapterBank& bank, int n) {

@@ -108,11 +108,11 @@ def test_too_many_sequences():
 def test_lists_have_room_for_every_tile():
     for n_rows, n_seqs in ((1, 1), (256, 256), (257, 3), (5000, 40)):
         rows = AdapterRows(n_rows, n_seqs, "cpu")
-        at = rows.buffer.data_ptr() + 4 * n_rows
-        for h, info, lists in zip(rows.heights, rows.info, rows.list):
+        at = rows.buffer.data_ptr() + 4 * (n_rows + n_rows % 2)
+        for h, info, slots, n_slots in zip(rows.heights, rows.info, rows.slots, rows.n_slots):
             tiles = -(-n_rows // h)
-            assert info == at and lists == at + 8 * tiles
-            at += 4 * (3 * tiles + n_seqs)
+            assert info == at and slots == at + 8 * tiles and n_slots == tiles + n_seqs and info % 8 == 0
+            at = slots + 8 * n_slots
         assert at == rows.buffer.data_ptr() + 4 * rows.buffer.numel()
         assert n_rows > 256 or rows.heights[0] >= n_rows
 

@@ -228,19 +228,22 @@ def ints(values):
 
 
 def check_lists(rows, per_sequence, lengths):
-    """Every tile's list holds the adapters of its rows, each once."""
+    """The slots of every tile hold the adapters of its rows, each once, and nothing else; no two tiles have a slot in common, and all slots are said to be."""
     words = rows.buffer.cpu().tolist()
     of = per_row(lengths, per_sequence)
     base = rows.buffer.data_ptr()
-    for height, info, lists in zip(rows.heights, rows.info, rows.list):
-        spans = []
+    for height, info, slots, n_slots in zip(rows.heights, rows.info, rows.slots, rows.n_slots):
+        at = (slots - base) // 4
+        pairs = list(zip(words[at:at + 2 * n_slots:2], words[at + 1:at + 2 * n_slots:2]))
+        used, last = set(), 0
         for tile in range(-(-rows.n_rows // height)):
             first, count = words[(info - base) // 4 + 2 * tile:(info - base) // 4 + 2 * tile + 2]
-            got = words[(lists - base) // 4 + first:(lists - base) // 4 + first + count]
-            assert sorted(got) == sorted({a for a in of[tile * height:(tile + 1) * height] if a >= 0})
-            spans.append((first, first + count))
-        assert all(b <= c for (_, b), (c, _) in zip(spans, spans[1:]))
-        assert not spans or spans[-1][1] <= -(-rows.n_rows // height) + rows.n_seqs
+            assert first >= last
+            last = first + count
+            assert all(t == tile for _, t in pairs[first:last])
+            assert sorted(a for a, _ in pairs[first:last]) == sorted({a for a in of[tile * height:(tile + 1) * height] if a >= 0})
+            used.update(range(first, last))
+        assert last <= n_slots and (rows.n_rows == 0 or all(a == -1 for i, (a, _) in enumerate(pairs) if i not in used))
 
 
 @pytest.mark.parametrize("starts, lengths", [
