@@ -11,7 +11,8 @@
 // and walk the tiles; an accumulator is half of tensor memory, so that one tile is read back while the next is multiplied.
 //   Whole tiles: every pair takes tiles in turn, the row tiles of 256 columns side by side, and writes C.
 //   Shares: the blocks of k of the tiles that make no whole round of the pairs (for few rows, where W's bytes are the cost, of all tiles) are dealt to the
-//   pairs in equal runs; what a pair has of a tile goes to scratch in 32 bits, and finish_kernel adds a tile's shares in order.
+//   pairs in equal runs; what a pair has of a tile goes to scratch in 32 bits, and who brings a tile's last share adds them
+//   in order.
 //
 // Warp 0 of either block drives TMA (64 elements of k a stage, 128-byte swizzle) and counts on the first block's barriers; warp 1 of the first
 // block issues tcgen05.mma for both; warps 2 to 9 read accumulators back: a lane is a column of C there and what it holds are rows, so a warp turns
@@ -27,6 +28,59 @@ namespace {
 
 using namespace tc;
 
+// Asked for by a whole warp, one lane of which does it (see umma_bf16_warp). In a single lane's branch a block of k of the first factor took some
+// 700 clocks, whatever was loaded.
+__device__ __forceinline__ void tma_load_2d_pair_warp(uint32_t smem_dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y) {
+  asm volatile(
+      "{\n.reg .pred q;\n"
+      "elect.sync _|q, 0xffffffff;\n"
+      "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n}"
+      ::"r"(smem_dst), "l"(map), "r"(cluster_bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair_warp(uint32_t smem_dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y, int z) {
+  asm volatile(
+      "{\n.reg .pred q;\n"
+      "elect.sync _|q, 0xffffffff;\n"
+      "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n}"
+      ::"r"(smem_dst), "l"(map), "r"(cluster_bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d_pair_warp(uint32_t smem_dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y, int z, int u) {
+  asm volatile(
+      "{\n.reg .pred q;\n"
+      "elect.sync _|q, 0xffffffff;\n"
+      "@q cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n}"
+      ::"r"(smem_dst), "l"(map), "r"(cluster_bar), "r"(x), "r"(y), "r"(z), "r"(u)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_warp(uint32_t smem_dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "{\n.reg .pred q;\n"
+      "elect.sync _|q, 0xffffffff;\n"
+      "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n}"
+      ::"r"(smem_dst), "l"(map), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx_warp(uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n.reg .pred q;\n"
+      "elect.sync _|q, 0xffffffff;\n"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}"
+      ::"r"(bar), "r"(bytes)
+      : "memory");
+}
+// Leaves a word for who waits on the barrier, and says how many bytes it waits for.
+__device__ __forceinline__ void expect_with_word_warp(uint32_t bar, uint32_t bytes, uint32_t word_at, int word) {
+  asm volatile(
+      "{\n.reg .pred q;\n"
+      "elect.sync _|q, 0xffffffff;\n"
+      "@q st.shared.u32 [%2], %3;\n"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}"
+      ::"r"(bar), "r"(bytes), "r"(word_at), "r"(word)
+      : "memory");
+}
+
 // ---------------------------------------------------------------------------------------------------------------------
 // The first factor
 // ---------------------------------------------------------------------------------------------------------------------
@@ -36,17 +90,17 @@ using namespace tc;
 // ranks, fed by TMA in blocks of 64 k); the blocks' sums meet in 32 bits through distributed shared memory, each block adding and writing its share of
 // the rows, in the blocks' order.
 //
-// The product's blocks come in while these run, once what came before is over, and wait for t where they need it; so a block's ring is no larger than
-// fits beside theirs.
-constexpr int FIRST_RANKS = 64, FIRST_STAGES = 3, FIRST_THREADS = 192, FIRST_PITCH = FIRST_RANKS + 4;
-constexpr uint32_t FIRST_X = 128 * 64 * 2, FIRST_STAGE = FIRST_X + FIRST_RANKS * 64 * 2;
-constexpr size_t FIRST_SMEM = 1024 + FIRST_STAGES * FIRST_STAGE;
-static_assert(128 * FIRST_PITCH * 4 <= FIRST_STAGES * FIRST_STAGE, "the sums take the ring's place");
+// The product's blocks come in while these run, once what came before is over, and wait for t where they need it; so a ring of few blocks of k is no
+// larger than fits beside theirs.
+constexpr int FIRST_RANKS = 64, FIRST_STAGES = 8, FIRST_THREADS = 192, FIRST_PITCH = FIRST_RANKS + 4;
+constexpr int FIRST_BYTES = 100 * 1024, FIRST_DEEP_BYTES = 160 * 1024;  // of the ring
+constexpr int FIRST_BLOCKS = 148;  // as many as are worth sharing k among
+static_assert(128 * FIRST_PITCH * 4 <= FIRST_BYTES, "the sums take the ring's place");
 
-__global__ void __launch_bounds__(FIRST_THREADS) first_factor_tiles_kernel(bf16* __restrict__ t, const __grid_constant__ CUtensorMap map_x,
+__global__ void __launch_bounds__(FIRST_THREADS) first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_done, const __grid_constant__ CUtensorMap map_x,
                                                                            const __grid_constant__ CUtensorMap map_a, int K,
                                                                            const __grid_constant__ AdapterBank bank, const __grid_constant__ AdapterTiles tiles,
-                                                                           int ways, int* __restrict__ error) {
+                                                                           int ways, int stages, int box_rows, int box_ranks, int* __restrict__ error) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   float* sums = reinterpret_cast<float*>(ring);  // [128][FIRST_PITCH], when the ring has done its work
@@ -56,12 +110,11 @@ __global__ void __launch_bounds__(FIRST_THREADS) first_factor_tiles_kernel(bf16*
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = blockIdx.x % ways, slot = blockIdx.x / ways;
   grid_dependency_wait();
   grid_launch_dependents();  // (the product reads what earlier kernels wrote before it waits)
+  if (blockIdx.x + blockIdx.y + blockIdx.z == 0)
+    for (int i = threadIdx.x; i < n_done; i += FIRST_THREADS) done[i] = 0;  // the product's counts of shares
   const int2 is = *reinterpret_cast<const int2*>(tiles.slots + 2 * slot);
   const int a = is.x, r0 = is.y * tiles.tile_rows + blockIdx.y * 128;
-  if (a < 0 || a >= bank.capacity) {  // the whole cluster
-    if (a >= 0 && threadIdx.x == 0) atomicExch(error, KRK_ERROR_ADAPTER);
-    return;
-  }
+  if (a < 0 || a >= bank.capacity) return;  // the whole cluster (the product says so)
   const int here = min(128, min(tiles.tile_rows - (int)blockIdx.y * 128, tiles.rows - r0));  // rows
   if (here <= 0) return;
   bool has = false;
@@ -69,7 +122,7 @@ __global__ void __launch_bounds__(FIRST_THREADS) first_factor_tiles_kernel(bf16*
   const int k_blocks = (K + 63) / 64, each = (k_blocks + ways - 1) / ways, b0 = min(way * each, k_blocks), b1 = min(b0 + each, k_blocks);
   const int n0 = blockIdx.z * FIRST_RANKS, per_adapter = bank.parts * bank.rank;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < FIRST_STAGES; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(full_bar + s, 1);
       mbar_init(empty_bar + s, 1);
     }
@@ -86,51 +139,49 @@ __global__ void __launch_bounds__(FIRST_THREADS) first_factor_tiles_kernel(bf16*
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t acc = tmem_slot;
+    const uint32_t acc = tmem_slot, bytes = (uint32_t)(box_rows + box_ranks) * 128;
     if (warp == 0) {
       for (int b = b0; b < b1; ++b) {
-        const int i = b - b0, s = i % FIRST_STAGES;
-        if (i >= FIRST_STAGES && !__all_sync(0xffffffffu, mbar_wait(empty_bar + s, (i / FIRST_STAGES - 1) & 1))) {
+        const int i = b - b0, s = i % stages;
+        if (i >= stages && !__all_sync(0xffffffffu, mbar_wait(empty_bar + s, (i / stages - 1) & 1))) {
           if (lane == 0) {
             atomicExch(error, 3);
             asked_for = i;
           }
           break;
         }
-        if (lane == 0) {
-          mbar_expect_tx(full_bar + s, FIRST_STAGE);
-          tma_load_2d(ring + s * FIRST_STAGE, &map_x, full_bar + s, b * 64, r0);
-          tma_load_2d(ring + s * FIRST_STAGE + FIRST_X, &map_a, full_bar + s, b * 64, a * per_adapter + n0);
-        }
-        __syncwarp();
+        const uint32_t stage = smem_u32(ring) + s * bytes, bar = smem_u32(full_bar + s);
+        mbar_expect_tx_warp(bar, bytes);
+        tma_load_2d_warp(stage, &map_x, bar, b * 64, r0);
+        tma_load_2d_warp(stage + box_rows * 128, &map_a, bar, b * 64, a * per_adapter + n0);
       }
     } else if (warp == 1) {
-      constexpr uint32_t idesc = umma_idesc(128, FIRST_RANKS);
+      const uint32_t idesc = umma_idesc(128, box_ranks);  // (rows beyond the copies' give rows that nobody reads)
       for (int b = b0; b < b1; ++b) {
-        const int i = b - b0, s = i % FIRST_STAGES;
-        if (!__all_sync(0xffffffffu, mbar_wait(full_bar + s, (i / FIRST_STAGES) & 1))) {
+        const int i = b - b0, s = i % stages;
+        if (!__all_sync(0xffffffffu, mbar_wait(full_bar + s, (i / stages) & 1))) {
           if (lane == 0) atomicExch(error, 4);
           break;
         }
         tc_fence_after();
-        const uint64_t x_desc = umma_desc(ring + s * FIRST_STAGE), a_desc = umma_desc(ring + s * FIRST_STAGE + FIRST_X);
+        const uint64_t x_desc = umma_desc(ring + s * bytes), a_desc = umma_desc(ring + s * bytes + box_rows * 128);
 #pragma unroll
         for (int k = 0; k < 4; ++k) umma_bf16_warp(acc, x_desc + k * 2, a_desc + k * 2, idesc, (b > b0 || k > 0) ? 1u : 0u);
         umma_commit_warp(empty_bar + s);
       }
       umma_commit_warp(&acc_bar);  // arrives even after a failed wait, so that all move on
     }
-    const bool ok = __all_sync(0xffffffffu, mbar_wait(&acc_bar, 0));
-    if (!ok && lane == 0) atomicExch(error, 5);
+    if (!__all_sync(0xffffffffu, mbar_wait(&acc_bar, 0)) && lane == 0) atomicExch(error, 5);
     __syncthreads();  // the ring has been read by the products that the barrier stands for
     if (threadIdx.x == 0 && asked_for >= 0)  // copies on their way end before the ring is written
-      for (int i = max(0, asked_for - FIRST_STAGES); i < asked_for; ++i) mbar_wait(full_bar + i % FIRST_STAGES, (uint32_t)(i / FIRST_STAGES) & 1u, WAIT_LIMIT_NS / 20);
+      for (int i = max(0, asked_for - stages); i < asked_for; ++i) mbar_wait(full_bar + i % stages, (uint32_t)(i / stages) & 1u, WAIT_LIMIT_NS / 20);
     __syncthreads();
-    if (warp >= 2) {
+    if (warp >= 2 && (warp & 3) * 32 < here) {
       const int row = (warp & 3) * 32 + lane;
       tc_fence_after();
 #pragma unroll
       for (int c = 0; c < FIRST_RANKS; c += 32) {
+        if (c >= box_ranks) break;
         uint32_t v[32];
         tmem_ld_32x32(acc + ((uint32_t)((warp & 3) * 32) << 16) + c, v);
         tmem_wait_ld();
@@ -186,52 +237,16 @@ constexpr int PAIRS = 74;
 constexpr int READERS = 8;  // warps that read accumulators: two to a quarter of tensor memory's lanes
 constexpr int THREADS = 64 + 32 * READERS;
 constexpr uint32_t W_BYTES = 128 * BK * 2;  // a block's half of the pair's weights
-constexpr int BUF_COLS = 256;               // tensor memory of an accumulator; there are two
-constexpr int PATCH_PITCH = 80;             // bytes of a row of a warp's patch for the transpose: 16-byte reads of 32 rows meet no bank twice
-constexpr int PATCH_BYTES = 32 * PATCH_PITCH;
-constexpr int RING_BYTES = 128 * 1024, MOST_STAGES = 7;  // (beside it an SM has room for a block of the first factor's)
-constexpr size_t SMEM_BYTES = 1024 + (size_t)RING_BYTES + READERS * PATCH_BYTES + (2 * MOST_STAGES + 6) * 8 + (MOST_STAGES + 4) * 4;
+constexpr int PATCH_PITCH = 36;             // words of two rows in a warp's patch for the transpose
+constexpr int PATCH_BYTES = 16 * PATCH_PITCH * 4;
+constexpr int MOST_STAGES = 7;
+constexpr int RING_BYTES = 96 * 1024, DEEP_RING_BYTES = 192 * 1024;  // beside the smaller an SM has room for a block of the first factor's
+constexpr size_t BESIDE_BYTES = 1024 + READERS * PATCH_BYTES + (2 * MOST_STAGES + 6) * 8 + (MOST_STAGES + 5) * 4;
 
 struct Maps {
   CUtensorMap x, w, t, b[KRK_MAX_PARTS];
 };
 
-// Asked for by a whole warp, one lane of which does it (see umma_bf16_warp). With the rest of the producer's loop in a single lane's branch a block of k took
-// some 1,000 clocks, twice what its products take, whatever was loaded.
-__device__ __forceinline__ void tma_load_2d_pair_warp(uint32_t smem_dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y) {
-  asm volatile(
-      "{\n.reg .pred q;\n"
-      "elect.sync _|q, 0xffffffff;\n"
-      "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n}"
-      ::"r"(smem_dst), "l"(map), "r"(cluster_bar), "r"(x), "r"(y)
-      : "memory");
-}
-__device__ __forceinline__ void tma_load_3d_pair_warp(uint32_t smem_dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y, int z) {
-  asm volatile(
-      "{\n.reg .pred q;\n"
-      "elect.sync _|q, 0xffffffff;\n"
-      "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n}"
-      ::"r"(smem_dst), "l"(map), "r"(cluster_bar), "r"(x), "r"(y), "r"(z)
-      : "memory");
-}
-__device__ __forceinline__ void tma_load_4d_pair_warp(uint32_t smem_dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y, int z, int u) {
-  asm volatile(
-      "{\n.reg .pred q;\n"
-      "elect.sync _|q, 0xffffffff;\n"
-      "@q cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n}"
-      ::"r"(smem_dst), "l"(map), "r"(cluster_bar), "r"(x), "r"(y), "r"(z), "r"(u)
-      : "memory");
-}
-// Leaves a word for who waits on the barrier, and says how many bytes it waits for.
-__device__ __forceinline__ void expect_with_word_warp(uint32_t bar, uint32_t bytes, uint32_t word_at, int word) {
-  asm volatile(
-      "{\n.reg .pred q;\n"
-      "elect.sync _|q, 0xffffffff;\n"
-      "@q st.shared.u32 [%2], %3;\n"
-      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}"
-      ::"r"(bar), "r"(bytes), "r"(word_at), "r"(word)
-      : "memory");
-}
 __device__ __forceinline__ void umma_bf16_pair_warp(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n.reg .pred p, q;\n"
@@ -250,15 +265,34 @@ __device__ __forceinline__ void umma_commit_pair_warp(uint64_t* bar) {
       : "memory");
 }
 
-// The work of a pair: of the tiles before `shared`, tiles pair, pair + pairs, ... as a whole; of the units of the tiles from there on, in order, `run` from
-// pair * run on. A tile's units are its blocks of k and, where there is a single row tile, its adapters (else they go to who has the last k).
+// The wait for a load of tensor memory, after which what it loaded may be used and not before.
+__device__ __forceinline__ void tmem_wait_ld_of(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+// The work of a pair: of the tiles before `shared`, tiles pair, pair + pairs, ... as a whole; of the tiles from there on a share. A tile's units are its blocks of k
+// and, where there is a single row tile, its adapters (else they go to who has the last k). With `aligned` a tile is dealt to so many pairs
+// in equal parts; else the units of all tiles, in order, to all pairs, `run` from pair * run on.
 struct Walk {
-  int shared, units, run, at, end, whole, pairs;
-  __device__ Walk(int pair, int pairs_, int tiles, int shared_, int units_) : shared(shared_), units(units_), whole(pair), pairs(pairs_) {
-    const long long all = (long long)units * (tiles - shared);
-    run = max(1, (int)((all + pairs - 1) / pairs));
-    at = (int)min((long long)pair * run, all);
-    end = (int)min((long long)at + run, all);
+  int shared, units, run, aligned, at, end, whole, pairs;
+  __device__ Walk(int pair, int pairs_, int tiles, int shared_, int units_, int aligned_) : shared(shared_), units(units_), aligned(aligned_), whole(pair), pairs(pairs_) {
+    const int all = units * (tiles - shared);
+    if (aligned) {
+      run = (units + aligned - 1) / aligned;
+      const int t = pair / aligned, first = pair % aligned * run;
+      at = min(t * units + first, all);
+      end = t >= tiles - shared ? at : max(at, t * units + min(units, first + run));
+    } else {
+      run = max(1, (int)(((long long)all + pairs - 1) / pairs));
+      at = (int)min((long long)pair * run, (long long)all);
+      end = (int)min((long long)at + run, (long long)all);
+    }
   }
   // tile t, of which units u0 to u1
   __device__ bool next(int& t, int& u0, int& u1) {
@@ -269,26 +303,29 @@ struct Walk {
       u1 = units;
       return true;
     }
+    // from behind: a run begins with what it has of its last tile, whose t it does not need, and waits for t where nothing is left to load but that
     if (at >= end) return false;
-    t = at / units;
-    u0 = at - t * units;
-    u1 = min(units, u0 + end - at);
-    at += u1 - u0;
+    t = (end - 1) / units;
+    u1 = end - t * units;
+    u0 = max(0, at - t * units);
+    end -= u1 - u0;
     t += shared;
     return true;
   }
-  __device__ int first_pair(int t) const { return (int)((long long)(t - shared) * units / run); }
-  __device__ int count(int t) const { return (int)(((long long)(t - shared + 1) * units - 1) / run) - first_pair(t) + 1; }
+  __device__ int first_pair(int t) const { return aligned ? (t - shared) * aligned : (int)((long long)(t - shared) * units / run); }
+  __device__ int count(int t) const {
+    return aligned ? (units + run - 1) / run : (int)(((long long)(t - shared + 1) * units - 1) / run) - first_pair(t) + 1;
+  }
 };
 
 template <bool GATED>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS)
-adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, float* __restrict__ shares, int shared, int most_shares, int N, int K, const __grid_constant__ AdapterBank bank,
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(512)  // (of 320: 128 registers a thread leave room for a block of the first factor's)
+adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, float* __restrict__ shares, int* __restrict__ done, int shared, int most_shares, int aligned, int ring_bytes, int N, int K, const __grid_constant__ AdapterBank bank,
                     const __grid_constant__ AdapterTiles tiles, int* __restrict__ error) {
   constexpr int BC = GATED ? 64 : 128;  // columns of C a block makes of a tile; the pair twice as many
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  unsigned char* patches = ring + RING_BYTES;
+  unsigned char* patches = ring + ring_bytes;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(patches + READERS * PATCH_BYTES);  // the first block's: copies of both have landed
   uint64_t* empty_bar = full_bar + MOST_STAGES;   // either block's: the products have read a stage
   uint64_t* acc_full = empty_bar + MOST_STAGES;   // either block's
@@ -297,7 +334,8 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
   uint64_t* ready_bar = drain_bar + 1;            // the first block's: the second has its tensor memory
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ready_bar + 1);
   int* issued = reinterpret_cast<int*>(tmem_slot + 1);  // blocks of k that were asked for, where a wait ran out; else -1
-  volatile int* steps = issued + 1;  // [stages] of 16 k in the stage; 256 more: the tile's last
+  volatile int* last = issued + 1;   // whether this block has brought a tile's last share
+  volatile int* steps = issued + 2;  // [stages] of 16 k in the stage; 256 more: the tile's last
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
 
@@ -318,9 +356,11 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
   __syncthreads();
   cluster_sync();  // the other block's barriers exist
   grid_launch_dependents();
-  // Tensor memory may be held by a block of the first factor's: only those who need it wait for it, while the ring fills.
+  // Two accumulators of a power of two of columns, no fewer than the tile's rows. With tiles of more than 128 rows that is all there is, and a block of the first
+  // factor's may hold some yet: only those who need it wait for it, while the ring fills.
+  const int buf_cols = tiles.tile_rows <= 32 ? 32 : 1 << (32 - __clz(tiles.tile_rows - 1));
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * BUF_COLS) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * buf_cols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     if (rank == 1 && lane == 0) mbar_arrive_cluster(cluster_address(ready_bar, 0));
   }
@@ -329,12 +369,12 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
   const uint32_t tmem_base = warp >= 1 ? *tmem_slot : 0;
   const int half = tiles.tile_rows / 2;  // rows that each block of the pair brings
   const uint32_t stage_bytes = W_BYTES + (uint32_t)half * BK * 2;
-  const int stages = min(MOST_STAGES, (int)(RING_BYTES / stage_bytes));
+  const int stages = min(MOST_STAGES, (int)(ring_bytes / stage_bytes));
   const int k_blocks = (K + BK - 1) / BK, row_tiles = (tiles.rows + tiles.tile_rows - 1) / tiles.tile_rows;
   const int all_tiles = row_tiles * ((N + 2 * BC - 1) / (2 * BC));
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const bool extras = row_tiles == 1;
-  Walk walk(pair, pairs, all_tiles, shared, k_blocks + (extras ? tiles.info[1] : 0));
+  Walk walk(pair, pairs, all_tiles, shared, k_blocks + (extras ? tiles.info[1] : 0), aligned);
   int t, u0, u1;
 
   if (warp == 0) {
@@ -381,7 +421,8 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
       auto look = [&](int i) {
         a = i + lane < e1 ? tiles.slots[2 * (first + i + lane)] : -1;
         ranks = 0;
-        if (a >= 0 && a < bank.capacity)
+        if (a >= bank.capacity) atomicExch(error, KRK_ERROR_ADAPTER);
+        else if (a >= 0)
           for (int p = p0; p < p1; ++p) ranks |= (uint32_t)((bank.ranks[a * bank.parts + p] + 15) / 16) << 8 * p;
       };
       int left = 0;  // blocks of k that the adapters make
@@ -431,7 +472,7 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
     if (rank == 0 && !ok && lane == 0) atomicExch(error, 4);
     const uint32_t idesc = umma_idesc(256, tiles.tile_rows);
     while (ok && walk.next(t, u0, u1)) {
-      const uint32_t acc = tmem_base + (uint32_t)buf * BUF_COLS;
+      const uint32_t acc = tmem_base + (uint32_t)(buf * buf_cols);
       ok = mbar_wait(acc_empty + buf, acc_parity);  // both blocks have read what was there
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
@@ -484,58 +525,124 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
       tc_fence_after();
       const int rt = t % row_tiles, wt = t / row_tiles, m0 = rt * tiles.tile_rows;
       const int live_rows = min(tiles.tile_rows, tiles.rows - m0);
-      const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)buf * BUF_COLS;
-      if (t >= shared) {
+      const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * buf_cols);
+      const int c_first = (warp - 2) / 4 * 32;
+      constexpr int C_STEP = 32 * (READERS / 4);
+      const int parts = t >= shared ? walk.count(t) : 1;
+      // 32 columns of tensor memory at a time, the next ones on their way
+      uint32_t v[2][32];
+      auto each = [&](auto use) {
+        if (c_first < live_rows) tmem_ld_32x32(acc + (uint32_t)c_first, v[0]);
+        for (int c0 = c_first; c0 < live_rows; c0 += 2 * C_STEP)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int c = c0 + h * C_STEP;
+            if (c >= live_rows) break;
+            tmem_wait_ld_of(v[h]);
+            if (c + C_STEP < live_rows) tmem_ld_32x32(acc + (uint32_t)(c + C_STEP), v[h ^ 1]);
+            use(c, v[h]);
+          }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(cluster_address(acc_empty + buf, 0));
+      };
+      if (parts > 1) {
         // [tile][share][row][256 rows of W, gate and up in turn where gated]: a lane's column, 32 of them side by side
-        float* dst = shares + ((size_t)((t - shared) * most_shares + pair - walk.first_pair(t)) * tiles.tile_rows) * 256 + rank * 128 + quarter * 32 + lane;
-        for (int c0 = (warp - 2) / 4 * 32; c0 < live_rows; c0 += 32 * (READERS / 4)) {
-          uint32_t v[32];
-          tmem_ld_32x32(acc + (uint32_t)c0, v);
-          tmem_wait_ld();
+        const size_t share = (size_t)tiles.tile_rows * 256;
+        float* mine = shares + (size_t)(t - shared) * most_shares * share + rank * 128;
+        float* dst = mine + (pair - walk.first_pair(t)) * share + quarter * 32 + lane;
+        each([&](int c, const uint32_t (&w)[32]) {
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            if (c0 + j < live_rows) dst[(size_t)(c0 + j) * 256] = __uint_as_float(v[j]);
+            if (c + j < live_rows) dst[(size_t)(c + j) * 256] = __uint_as_float(w[j]);
+        });
+        // The block that brings a tile's last share adds them all, in the pairs' order. (The first factor's kernel has set the counts to zero.)
+        grid_dependency_wait();
+        __threadfence();
+        asm volatile("bar.sync 2, %0;" ::"n"(32 * READERS) : "memory");
+        if (threadIdx.x == 64) *last = atomicAdd(done + (t - shared) * 2 + rank, 1) == parts - 1;
+        asm volatile("bar.sync 2, %0;" ::"n"(32 * READERS) : "memory");
+        if (*last) {
+          __threadfence();
+          constexpr int ROWS = 4, DEEP = 3;  // of the shares of so many rows at once, for a warp
+          const int column = lane * 4, n = GATED ? (wt * 2 + (int)rank) * BC + column / 2 : (wt * 2 + (int)rank) * BC + column;
+          for (int r0 = (warp - 2) * ROWS; r0 < live_rows; r0 += READERS * ROWS) {
+            float4 sum[ROWS];
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int p = 0; p < parts; p += DEEP) {
+              float4 more[DEEP][ROWS];
+              // (a row or share too many is read again from the last one, and not added)
+#pragma unroll
+              for (int d = 0; d < DEEP; ++d)
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i)
+                  more[d][i] = __ldcg(reinterpret_cast<const float4*>(mine + min(p + d, parts - 1) * share + (size_t)min(r0 + i, live_rows - 1) * 256 + column));
+#pragma unroll
+              for (int d = 0; d < DEEP; ++d)
+                if (p + d < parts)
+#pragma unroll
+                  for (int i = 0; i < ROWS; ++i) {
+                    sum[i].x += more[d][i].x;
+                    sum[i].y += more[d][i].y;
+                    sum[i].z += more[d][i].z;
+                    sum[i].w += more[d][i].w;
+                  }
+            }
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i)
+              if (r0 + i < live_rows && n < N) {  // N is a multiple of 8
+                bf16* to = out + (size_t)(m0 + r0 + i) * N + n;
+                const float4 s = sum[i];
+                if (GATED) *reinterpret_cast<uint32_t*>(to) = pack_bf16x2(s.x / (1.0f + expf(-s.x)) * s.y, s.z / (1.0f + expf(-s.z)) * s.w);
+                else *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+              }
+          }
         }
       } else {
         constexpr int MINE = BC / 4;  // columns of this warp
         const int f0 = (wt * 2 + (int)rank) * BC + quarter * MINE;
-        if (f0 < N) {
-          for (int c0 = (warp - 2) / 4 * 32; c0 < live_rows; c0 += 32 * (READERS / 4)) {
-            uint32_t v[32];
-            tmem_ld_32x32(acc + (uint32_t)c0, v);
-            tmem_wait_ld();
-            if constexpr (GATED) {
-              // an even lane has a column's gate and the odd one after it the same column's up: they share the rows, the even ones to the even lane
-              const bool odd = lane & 1;
+        uint32_t* words = reinterpret_cast<uint32_t*>(patch);
+        each([&](int c, const uint32_t (&w)[32]) {
+          // The patch has a word for two rows of a column.
+          if constexpr (GATED) {
+            // an even lane has a column's gate and the odd one after it the same column's up: they share the rows, the even lane takes the first two of four
+            const bool odd = lane & 1;
 #pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const float a = __uint_as_float(v[2 * j]), b = __uint_as_float(v[2 * j + 1]);
+            for (int j = 0; j < 32; j += 4) {
+              float z[2];
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const float a = __uint_as_float(w[j + i]), b = __uint_as_float(w[j + 2 + i]);
                 const float got = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
                 const float gate = odd ? got : a, up = odd ? b : got;
-                *reinterpret_cast<bf16*>(patch + (2 * j + (odd ? 1 : 0)) * PATCH_PITCH + (lane >> 1) * 2) =
-                    from_float<bf16>(__fdividef(gate, 1.0f + __expf(-gate)) * up);
+                z[i] = __fdividef(gate, 1.0f + __expf(-gate)) * up;
               }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) *reinterpret_cast<bf16*>(patch + j * PATCH_PITCH + lane * 2) = from_float<bf16>(__uint_as_float(v[j]));
+              words[(j / 2 + (odd ? 1 : 0)) * PATCH_PITCH + (lane >> 1)] = pack_bf16x2(z[0], z[1]);
             }
-            __syncwarp();
-            // neighbouring lanes have a row's 16 bytes each: whole sectors at once (N is a multiple of 8)
-            constexpr int PER = MINE / 8, STEP = 32 / PER;
-            const int j = lane % PER * 8;
-            if (f0 + j < N)
+          } else {
 #pragma unroll
-              for (int r = lane / PER; r < 32; r += STEP)
-                if (c0 + r < live_rows)
-                  *reinterpret_cast<uint4*>(out + (size_t)(m0 + c0 + r) * N + f0 + j) =
-                      *reinterpret_cast<const uint4*>(patch + r * PATCH_PITCH + j * 2);
-            __syncwarp();
+            for (int j = 0; j < 32; j += 2) words[j / 2 * PATCH_PITCH + lane] = pack_bf16x2(__uint_as_float(w[j]), __uint_as_float(w[j + 1]));
           }
-        }
+          __syncwarp();
+          // neighbouring lanes take eight columns of two rows each: whole sectors at once (N is a multiple of 8)
+          constexpr int PER = MINE / 8, STEP = 32 / PER;
+          const int j = lane % PER * 8;
+          if (f0 + j < N)
+#pragma unroll
+            for (int r = lane / PER; r < 16; r += STEP) {
+              const uint4 lo = *reinterpret_cast<const uint4*>(words + r * PATCH_PITCH + j), hi = *reinterpret_cast<const uint4*>(words + r * PATCH_PITCH + j + 4);
+              bf16* to = out + (size_t)(m0 + c + 2 * r) * N + f0 + j;
+              if (c + 2 * r < live_rows)
+                *reinterpret_cast<uint4*>(to) = make_uint4(__byte_perm(lo.x, lo.y, 0x5410), __byte_perm(lo.z, lo.w, 0x5410), __byte_perm(hi.x, hi.y, 0x5410),
+                                                           __byte_perm(hi.z, hi.w, 0x5410));
+              if (c + 2 * r + 1 < live_rows)
+                *reinterpret_cast<uint4*>(to + N) = make_uint4(__byte_perm(lo.x, lo.y, 0x7632), __byte_perm(lo.z, lo.w, 0x7632), __byte_perm(hi.x, hi.y, 0x7632),
+                                                               __byte_perm(hi.z, hi.w, 0x7632));
+            }
+          __syncwarp();
+        });
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(cluster_address(acc_empty + buf, 0));
       buf ^= 1;
       parity ^= buf == 0;
     }
@@ -550,35 +657,7 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
   cluster_sync();  // neither block's barriers are signalled any more
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * BUF_COLS) : "memory");
-  }
-}
-
-// The shares of a tile, added in the pairs' order. A block has a tile's 256 columns (x) of four rows (y).
-template <bool GATED>
-__global__ void __launch_bounds__(256) finish_kernel(bf16* __restrict__ out, const float* __restrict__ shares, int shared, int most_shares, int N, int k_blocks,
-                                                     int pairs, const __grid_constant__ AdapterTiles tiles) {
-  grid_launch_dependents();
-  grid_dependency_wait();
-  const int row_tiles = (tiles.rows + tiles.tile_rows - 1) / tiles.tile_rows, all_tiles = shared + gridDim.x;
-  const Walk walk(0, pairs, all_tiles, shared, k_blocks + (row_tiles == 1 ? tiles.info[1] : 0));
-  const int t = shared + blockIdx.x, rt = t % row_tiles, wt = t / row_tiles, r = blockIdx.y * 4 + threadIdx.x / 64, column = threadIdx.x % 64 * 4;
-  const int row = rt * tiles.tile_rows + r, n = GATED ? wt * 128 + column / 2 : wt * 256 + column;
-  if (r >= tiles.tile_rows || row >= tiles.rows || n >= N) return;
-  const int count = walk.count(t);
-  const float* from = shares + ((size_t)blockIdx.x * most_shares * tiles.tile_rows + r) * 256 + column;
-  float4 sum = *reinterpret_cast<const float4*>(from);
-  for (int i = 1; i < count; ++i) {
-    const float4 more = *reinterpret_cast<const float4*>(from + (size_t)i * tiles.tile_rows * 256);
-    sum.x += more.x;
-    sum.y += more.y;
-    sum.z += more.z;
-    sum.w += more.w;
-  }
-  if (GATED) {
-    *reinterpret_cast<uint32_t*>(out + (size_t)row * N + n) = pack_bf16x2(sum.x / (1.0f + expf(-sum.x)) * sum.y, sum.z / (1.0f + expf(-sum.z)) * sum.w);
-  } else {
-    *reinterpret_cast<uint2*>(out + (size_t)row * N + n) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * buf_cols) : "memory");
   }
 }
 
@@ -606,7 +685,11 @@ int make_map_b(CUtensorMap* map, const AdapterBank& bank, int part, int N, bool 
   return make_map(map, base, 3, size, stride, box);
 }
 
-int launch_first(bf16* t, const CUtensorMap& map_x, const CUtensorMap& map_a, int K, const AdapterBank& bank, const AdapterTiles& tiles, int* error, cudaStream_t stream) {
+// rows and ranks of a copy of the first factor's: as many as there are
+int first_rows(const AdapterTiles& tiles) { return min(128, (min(tiles.rows, tiles.tile_rows) + 7) / 8 * 8); }
+int first_ranks(const AdapterBank& bank) { return min(FIRST_RANKS, (bank.parts * bank.rank + 15) / 16 * 16); }
+
+int launch_first(bf16* t, int* done, int n_done, const CUtensorMap& map_x, const CUtensorMap& map_a, int K, const AdapterBank& bank, const AdapterTiles& tiles, int* error, cudaStream_t stream) {
   // an SM gives its memory to L1 or to blocks anew only when it is empty: split as the product's blocks need it, they come in beside these
   static unsigned long long told = 0, allowed = 0;
   int device = 0;
@@ -615,16 +698,24 @@ int launch_first(bf16* t, const CUtensorMap& map_x, const CUtensorMap& map_a, in
     e = cudaFuncSetAttribute(first_factor_tiles_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e == cudaSuccess) __atomic_fetch_or(&told, 1ull << (device & 63), __ATOMIC_RELAXED);
   }
-  if (e == cudaSuccess) e = allow_shared(first_factor_tiles_kernel, FIRST_SMEM, &allowed);
+  if (e == cudaSuccess) e = allow_shared(first_factor_tiles_kernel, 1024 + FIRST_DEEP_BYTES, &allowed);
   if (e != cudaSuccess) return (int)e;
-  const int parts = (min(tiles.tile_rows, tiles.rows) + 127) / 128, chunks = (bank.parts * bank.rank + FIRST_RANKS - 1) / FIRST_RANKS;
-  const long long blocks = (long long)tiles.n_slots * parts * chunks;
+  const int row_tiles = (tiles.rows + tiles.tile_rows - 1) / tiles.tile_rows, ranks = bank.parts * bank.rank;
+  const int parts = (min(tiles.tile_rows, tiles.rows) + 127) / 128, chunks = (ranks + FIRST_RANKS - 1) / FIRST_RANKS;
+  // a single tile's adapters are in the first slots; of several tiles' some half are used
+  const int slots = row_tiles == 1 ? min(tiles.n_slots, bank.capacity) : tiles.n_slots;
+  const long long blocks = (long long)slots * parts * chunks * (row_tiles == 1 ? 2 : 1);
   int ways = 1;
-  while (ways < 8 && ways * blocks <= 2 * PAIRS && K >= 64 * 2 * ways) ways *= 2;
+  while (ways < 8 && ways * blocks <= FIRST_BLOCKS && K >= 64 * 2 * ways) ways *= 2;
+  // Where the product's blocks leave tensor memory for these, they run side by side; else these have the larger ring. Products read 128 rows, so that
+  // the last stage has them behind it.
+  const int stage = (first_rows(tiles) + first_ranks(bank)) * 128, behind = (128 - first_rows(tiles)) * 128;
+  const int stages = min(FIRST_STAGES, ((tiles.tile_rows > 128 ? FIRST_DEEP_BYTES : FIRST_BYTES) - behind) / stage);
+  const int bytes = 1024 + max(stages * stage + behind, 128 * FIRST_PITCH * 4);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tiles.n_slots * ways, parts, chunks);
+  cfg.gridDim = dim3(slots * ways, parts, chunks);
   cfg.blockDim = dim3(FIRST_THREADS);
-  cfg.dynamicSmemBytes = FIRST_SMEM;
+  cfg.dynamicSmemBytes = bytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -636,24 +727,26 @@ int launch_first(bf16* t, const CUtensorMap& map_x, const CUtensorMap& map_a, in
   static const bool plain = getenv("KRK_NO_PDL") != nullptr;
   cfg.attrs = attr;
   cfg.numAttrs = plain ? 1 : 2;
-  return (int)cudaLaunchKernelEx(&cfg, first_factor_tiles_kernel, t, map_x, map_a, K, bank, tiles, ways, error);
+  return (int)cudaLaunchKernelEx(&cfg, first_factor_tiles_kernel, t, done, n_done, map_x, map_a, K, bank, tiles, ways, stages, first_rows(tiles), first_ranks(bank), error);
 }
 
 template <bool GATED>
-int launch_gemm(const Maps& maps, bf16* out, float* shares, int shared, int most_shares, int N, int K, const AdapterBank& bank, const AdapterTiles& tiles, int pairs,
-                int* error, cudaStream_t stream) {
+int launch_gemm(const Maps& maps, bf16* out, float* shares, int* done, int shared, int most_shares, int aligned, int N, int K, const AdapterBank& bank, const AdapterTiles& tiles,
+                int pairs, int* error, cudaStream_t stream) {
   static unsigned long long allowed = 0;
   auto kern = adapted_gemm_kernel<GATED>;
-  const cudaError_t e = allow_shared(kern, SMEM_BYTES, &allowed);
+  const cudaError_t e = allow_shared(kern, BESIDE_BYTES + DEEP_RING_BYTES, &allowed);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(kern, dim3(2 * pairs), dim3(THREADS), SMEM_BYTES, stream, maps, out, shares, shared, most_shares, N, K, bank, tiles, error);
+  const int ring = tiles.tile_rows <= 128 ? RING_BYTES : DEEP_RING_BYTES;
+  return (int)launch_pdl(kern, dim3(2 * pairs), dim3(THREADS), BESIDE_BYTES + ring, stream, maps, out, shares, done, shared, most_shares, aligned, ring, N, K, bank,
+                         tiles, error);
 }
 
 }  // namespace
 
 // out [rows, N] (gated: [rows, N / 2]) bfloat16 from x [rows, K] (row stride ldx) and w [N, K] (row stride ldw), by tiles of tile_rows rows and 256 rows of w, the
 // first `shared` of them as whole ones (a multiple of 74, or all). t: scratch of n_slots * tile_rows * parts * wide bfloat16. shares: float32 scratch of the
-// other tiles' number times (74 / their number, rounded up, and one more) * tile_rows * 256, or null where there are none.
+// other tiles' number times (74 / their number, rounded up, and one more) * tile_rows * 256, and two words a tile behind that, or null where there are none.
 KRK_API int krk_adapted_gemm(void* out, const void* x, long long ldx, const void* w, long long ldw, int rows, int N, int K, const AdapterBank* bank,
                              const int* row_adapter, const int* info, const int* slots, int n_slots, int tile_rows, void* t, float* shares, int shared, int gated,
                              int* error, cudaStream_t stream) {
@@ -676,16 +769,15 @@ KRK_API int krk_adapted_gemm(void* out, const void* x, long long ldx, const void
   rc = gated ? make_map_bf16_3d(&maps.w, w, K, 2, width, (long long)width * ldw, ldw, 2, 64) : make_map_bf16(&maps.w, w, N, K, ldw, 128);
   if (!rc) rc = make_map_bf16(&maps.t, t, (long long)n_slots * tile_rows, bank->parts * bank->wide, bank->parts * bank->wide, tile_rows / 2);
   for (int p = 0; p < bank->parts && !rc; ++p) rc = make_map_b(&maps.b[p], *bank, p, N, gated);
-  if (!rc) rc = make_map_bf16(&map_x, x, rows, K, ldx, 128);
-  if (!rc) rc = make_map_bf16(&map_a, bank->a, (long long)bank->capacity * per_adapter, K, K, FIRST_RANKS);
-  if (!rc) rc = launch_first((bf16*)t, map_x, map_a, K, *bank, tiles, error, stream);
-  if (rc) return rc;
+  if (!rc) rc = make_map_bf16(&map_x, x, rows, K, ldx, first_rows(tiles));
+  if (!rc) rc = make_map_bf16(&map_a, bank->a, (long long)bank->capacity * per_adapter, K, K, first_ranks(*bank));
   const int rest = (int)(all - shared), most_shares = rest ? (PAIRS + rest - 1) / rest + 1 : 0;
+  int* done = rest ? reinterpret_cast<int*>(shares + (size_t)rest * most_shares * tile_rows * 256) : nullptr;
+  if (!rc) rc = launch_first((bf16*)t, done, 2 * rest, map_x, map_a, K, *bank, tiles, error, stream);
+  if (rc) return rc;
   const int pairs = rest || all > PAIRS ? PAIRS : (int)all;
-  rc = gated ? launch_gemm<true>(maps, (bf16*)out, shares, shared, most_shares, width, K, *bank, tiles, pairs, error, stream)
-             : launch_gemm<false>(maps, (bf16*)out, shares, shared, most_shares, width, K, *bank, tiles, pairs, error, stream);
-  if (rc || !rest) return rc;
-  const dim3 blocks(rest, (min(rows, tile_rows) + 3) / 4);
-  return gated ? (int)launch_pdl(finish_kernel<true>, blocks, dim3(256), 0, stream, (bf16*)out, (const float*)shares, shared, most_shares, width, k_blocks, PAIRS, tiles)
-               : (int)launch_pdl(finish_kernel<false>, blocks, dim3(256), 0, stream, (bf16*)out, (const float*)shares, shared, most_shares, width, k_blocks, PAIRS, tiles);
+  // as many pairs a tile, where that leaves few of them idle: fewer shares, and no pair has two
+  const int aligned = rest && rest * (PAIRS / rest) * 10 >= PAIRS * 9 ? PAIRS / rest : 0;
+  return gated ? launch_gemm<true>(maps, (bf16*)out, shares, done, shared, most_shares, aligned, width, K, *bank, tiles, pairs, error, stream)
+               : launch_gemm<false>(maps, (bf16*)out, shares, done, shared, most_shares, aligned, width, K, *bank, tiles, pairs, error, stream);
 }

@@ -196,9 +196,9 @@ class AdapterOps:
             n_slots, tiles = rows.n_slots[which], -(-M // height) * -(-N // 256)
             t_words = n_slots * height * bank.parts * (-(-bank.rank // 16) * 8)
             rest = tiles - shared
-            t = self.error.new_empty(t_words + (rest * (-(-self.PAIRS // rest) + 1) * height * 256 if rest else 0))
+            t = self.error.new_empty(t_words + (rest * ((-(-self.PAIRS // rest) + 1) * height * 256 + 2) if rest else 0))
             t_at = t.data_ptr()
-            self.launches += 2 if rest else 1
+            self.launches += 1
             self._ok(self.adapt.krk_adapted_gemm(
                 out.data_ptr(), x_at, ldx, w_at, ldw, M, N, K, described, rows.row_adapter.data_ptr(), rows.info[which], rows.slots[which], n_slots, height,
                 t_at, t_at + 4 * t_words if rest else None, shared, int(gated > 0), error, self._stream()), what)
