@@ -3,7 +3,7 @@
 // are further blocks of k: behind W's columns come, for every adapter a that a tile of rows has, B's rows of a beside the rows' t, which are zero
 // for rows that have another. Gated: W and B hold gate rows and then up rows, and C = silu(g) u.
 //
-// first_factor_tiles_kernel makes t = scale (x A^T), rounded to bfloat16 (half a step of 2^-8 of a sum that is itself a part of the result, which is
+// The first factor's kernel (first_factor.cu) makes t, rounded to bfloat16 (half a step of 2^-8 of a sum that is itself a part of the result, which is
 // rounded the same way).
 //
 // adapted_gemm_kernel works in pairs of blocks (cta_group::2): 256 rows of W are the product's M, half of them in each block's shared memory, and a
@@ -18,230 +18,28 @@
 // block issues tcgen05.mma for both; warps 2 to 9 read accumulators back: a lane is a column of C there and what it holds are rows, so a warp turns
 // 32 x 32 of them through a patch of shared memory. Gate and up rows alternate in the tile, so that neighbouring lanes hold a column's
 // two sums. Every wait is bounded: one that runs out sets the error word, and the blocks leave after freeing their tensor memory.
-#include <cooperative_groups.h>
-
 #include "adapters.cuh"
 #include "mma.cuh"
-#include "tcgen05.cuh"
+#include "warp_copies.cuh"
 
 namespace {
 
 using namespace tc;
-
-// Asked for by a whole warp, one lane of which does it (see umma_bf16_warp). In a single lane's branch a block of k of the first factor took some
-// 700 clocks, whatever was loaded.
-__device__ __forceinline__ void tma_load_2d_pair_warp(uint32_t smem_dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y) {
-  asm volatile(
-      "{\n.reg .pred q;\n"
-      "elect.sync _|q, 0xffffffff;\n"
-      "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n}"
-      ::"r"(smem_dst), "l"(map), "r"(cluster_bar), "r"(x), "r"(y)
-      : "memory");
-}
-__device__ __forceinline__ void tma_load_3d_pair_warp(uint32_t smem_dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y, int z) {
-  asm volatile(
-      "{\n.reg .pred q;\n"
-      "elect.sync _|q, 0xffffffff;\n"
-      "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n}"
-      ::"r"(smem_dst), "l"(map), "r"(cluster_bar), "r"(x), "r"(y), "r"(z)
-      : "memory");
-}
-__device__ __forceinline__ void tma_load_4d_pair_warp(uint32_t smem_dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y, int z, int u) {
-  asm volatile(
-      "{\n.reg .pred q;\n"
-      "elect.sync _|q, 0xffffffff;\n"
-      "@q cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n}"
-      ::"r"(smem_dst), "l"(map), "r"(cluster_bar), "r"(x), "r"(y), "r"(z), "r"(u)
-      : "memory");
-}
-__device__ __forceinline__ void tma_load_2d_warp(uint32_t smem_dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
-  asm volatile(
-      "{\n.reg .pred q;\n"
-      "elect.sync _|q, 0xffffffff;\n"
-      "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n}"
-      ::"r"(smem_dst), "l"(map), "r"(bar), "r"(x), "r"(y)
-      : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx_warp(uint32_t bar, uint32_t bytes) {
-  asm volatile(
-      "{\n.reg .pred q;\n"
-      "elect.sync _|q, 0xffffffff;\n"
-      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}"
-      ::"r"(bar), "r"(bytes)
-      : "memory");
-}
-// Leaves a word for who waits on the barrier, and says how many bytes it waits for.
-__device__ __forceinline__ void expect_with_word_warp(uint32_t bar, uint32_t bytes, uint32_t word_at, int word) {
-  asm volatile(
-      "{\n.reg .pred q;\n"
-      "elect.sync _|q, 0xffffffff;\n"
-      "@q st.shared.u32 [%2], %3;\n"
-      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}"
-      ::"r"(bar), "r"(bytes), "r"(word_at), "r"(word)
-      : "memory");
-}
-
-// ---------------------------------------------------------------------------------------------------------------------
-// The first factor
-// ---------------------------------------------------------------------------------------------------------------------
-
-// t of every slot, [slot][tile_rows][parts * wide]: zeros where a row has another adapter than the slot's. A cluster has 128 rows of a slot's tile (y), 64 of the
-// adapter's ranks, all parts' side by side (z), and its `ways` blocks share k. A block multiplies its part of k on the tensor cores (128 rows by 64
-// ranks, fed by TMA in blocks of 64 k); the blocks' sums meet in 32 bits through distributed shared memory, each block adding and writing its share of
-// the rows, in the blocks' order.
-//
-// The product's blocks come in while these run, once what came before is over, and wait for t where they need it; so a ring of few blocks of k is no
-// larger than fits beside theirs.
-constexpr int FIRST_RANKS = 64, FIRST_STAGES = 8, FIRST_THREADS = 192, FIRST_PITCH = FIRST_RANKS + 4;
-constexpr int FIRST_BYTES = 100 * 1024, FIRST_DEEP_BYTES = 160 * 1024;  // of the ring
-constexpr int FIRST_BLOCKS = 148;  // as many as are worth sharing k among
-static_assert(128 * FIRST_PITCH * 4 <= FIRST_BYTES, "the sums take the ring's place");
-
-__global__ void __launch_bounds__(FIRST_THREADS) first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_done, const __grid_constant__ CUtensorMap map_x,
-                                                                           const __grid_constant__ CUtensorMap map_a, int K,
-                                                                           const __grid_constant__ AdapterBank bank, const __grid_constant__ AdapterTiles tiles,
-                                                                           int ways, int stages, int box_rows, int box_ranks, int* __restrict__ error) {
-  extern __shared__ __align__(1024) unsigned char smem_raw[];
-  unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  float* sums = reinterpret_cast<float*>(ring);  // [128][FIRST_PITCH], when the ring has done its work
-  __shared__ uint64_t full_bar[FIRST_STAGES], empty_bar[FIRST_STAGES], acc_bar;
-  __shared__ uint32_t tmem_slot;
-  __shared__ int asked_for;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = blockIdx.x % ways, slot = blockIdx.x / ways;
-  grid_dependency_wait();
-  grid_launch_dependents();  // (the product reads what earlier kernels wrote before it waits)
-  if (blockIdx.x + blockIdx.y + blockIdx.z == 0)
-    for (int i = threadIdx.x; i < n_done; i += FIRST_THREADS) done[i] = 0;  // the product's counts of shares
-  const int2 is = *reinterpret_cast<const int2*>(tiles.slots + 2 * slot);
-  const int a = is.x, r0 = is.y * tiles.tile_rows + blockIdx.y * 128;
-  if (a < 0 || a >= bank.capacity) return;  // the whole cluster (the product says so)
-  const int here = min(128, min(tiles.tile_rows - (int)blockIdx.y * 128, tiles.rows - r0));  // rows
-  if (here <= 0) return;
-  bool has = false;
-  for (int r = threadIdx.x; r < here; r += FIRST_THREADS) has |= tiles.row_adapter[r0 + r] == a;
-  const int k_blocks = (K + 63) / 64, each = (k_blocks + ways - 1) / ways, b0 = min(way * each, k_blocks), b1 = min(b0 + each, k_blocks);
-  const int n0 = blockIdx.z * FIRST_RANKS, per_adapter = bank.parts * bank.rank;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < stages; ++s) {
-      mbar_init(full_bar + s, 1);
-      mbar_init(empty_bar + s, 1);
-    }
-    mbar_init(&acc_bar, 1);
-    asked_for = -1;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  has = __syncthreads_or(has);
-  if (has) {  // the same for the whole cluster
-    if (warp == 1) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(FIRST_RANKS) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t acc = tmem_slot, bytes = (uint32_t)(box_rows + box_ranks) * 128;
-    if (warp == 0) {
-      for (int b = b0; b < b1; ++b) {
-        const int i = b - b0, s = i % stages;
-        if (i >= stages && !__all_sync(0xffffffffu, mbar_wait(empty_bar + s, (i / stages - 1) & 1))) {
-          if (lane == 0) {
-            atomicExch(error, 3);
-            asked_for = i;
-          }
-          break;
-        }
-        const uint32_t stage = smem_u32(ring) + s * bytes, bar = smem_u32(full_bar + s);
-        mbar_expect_tx_warp(bar, bytes);
-        tma_load_2d_warp(stage, &map_x, bar, b * 64, r0);
-        tma_load_2d_warp(stage + box_rows * 128, &map_a, bar, b * 64, a * per_adapter + n0);
-      }
-    } else if (warp == 1) {
-      const uint32_t idesc = umma_idesc(128, box_ranks);  // (rows beyond the copies' give rows that nobody reads)
-      for (int b = b0; b < b1; ++b) {
-        const int i = b - b0, s = i % stages;
-        if (!__all_sync(0xffffffffu, mbar_wait(full_bar + s, (i / stages) & 1))) {
-          if (lane == 0) atomicExch(error, 4);
-          break;
-        }
-        tc_fence_after();
-        const uint64_t x_desc = umma_desc(ring + s * bytes), a_desc = umma_desc(ring + s * bytes + box_rows * 128);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) umma_bf16_warp(acc, x_desc + k * 2, a_desc + k * 2, idesc, (b > b0 || k > 0) ? 1u : 0u);
-        umma_commit_warp(empty_bar + s);
-      }
-      umma_commit_warp(&acc_bar);  // arrives even after a failed wait, so that all move on
-    }
-    if (!__all_sync(0xffffffffu, mbar_wait(&acc_bar, 0)) && lane == 0) atomicExch(error, 5);
-    __syncthreads();  // the ring has been read by the products that the barrier stands for
-    if (threadIdx.x == 0 && asked_for >= 0)  // copies on their way end before the ring is written
-      for (int i = max(0, asked_for - stages); i < asked_for; ++i) mbar_wait(full_bar + i % stages, (uint32_t)(i / stages) & 1u, WAIT_LIMIT_NS / 20);
-    __syncthreads();
-    if (warp >= 2 && (warp & 3) * 32 < here) {
-      const int row = (warp & 3) * 32 + lane;
-      tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < FIRST_RANKS; c += 32) {
-        if (c >= box_ranks) break;
-        uint32_t v[32];
-        tmem_ld_32x32(acc + ((uint32_t)((warp & 3) * 32) << 16) + c, v);
-        tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 32; j += 4)
-          *reinterpret_cast<float4*>(sums + row * FIRST_PITCH + c + j) =
-              b1 > b0 ? make_float4(__uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      tc_fence_before();
-    }
-    __syncthreads();
-    if (warp == 1) {
-      tc_fence_after();
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(acc), "r"(FIRST_RANKS) : "memory");
-    }
-    if (ways > 1) cluster_sync();
-  }
-  // eight ranks of a row a thread
-  namespace cg = cooperative_groups;
-  const int share = (here + ways - 1) / ways, first_row = way * share, rows = min(share, here - first_row);
-  const int width = bank.parts * bank.wide;
-  for (int o = threadIdx.x; o < rows * (FIRST_RANKS / 8); o += FIRST_THREADS) {
-    const int row = first_row + o / (FIRST_RANKS / 8), c = o % (FIRST_RANKS / 8) * 8, part = (n0 + c) / bank.rank, j = (n0 + c) % bank.rank;
-    if (part >= bank.parts) continue;
-    bf16* to = t + ((size_t)slot * tiles.tile_rows + blockIdx.y * 128 + row) * width + part * bank.wide + j;
-    uint4 pack = make_uint4(0, 0, 0, 0);
-    if (tiles.row_adapter[r0 + row] == a) {
-      const int rank = bank.ranks[a * bank.parts + part];
-      const float scale = bank.scale[a * bank.parts + part];
-      float v[8] = {};
-      for (int w = 0; w < ways; ++w) {
-        const float* from = (ways > 1 ? cg::this_cluster().map_shared_rank(sums, w) : sums) + row * FIRST_PITCH + c;
-        const float4 lo = *reinterpret_cast<const float4*>(from), hi = *reinterpret_cast<const float4*>(from + 4);
-        v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
-        v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = j + i < rank ? v[i] * scale : 0.f;
-      pack = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-    }
-    *reinterpret_cast<uint4*>(to) = pack;
-    if (j + 8 == bank.rank && bank.wide > bank.rank) *reinterpret_cast<uint4*>(to + 8) = make_uint4(0, 0, 0, 0);  // the product takes whole steps of sixteen
-  }
-  if (has && ways > 1) cluster_sync();  // no block leaves while another reads its sums
-}
 
 // ---------------------------------------------------------------------------------------------------------------------
 // The product
 // ---------------------------------------------------------------------------------------------------------------------
 
 constexpr int BK = 64, UMMA_K = 16;
-constexpr int PAIRS = 74;
+constexpr int PAIRS = 74;  // of SMs
 constexpr int READERS = 8;  // warps that read accumulators: two to a quarter of tensor memory's lanes
 constexpr int THREADS = 64 + 32 * READERS;
 constexpr uint32_t W_BYTES = 128 * BK * 2;  // a block's half of the pair's weights
 constexpr int PATCH_PITCH = 36;             // words of two rows in a warp's patch for the transpose
 constexpr int PATCH_BYTES = 16 * PATCH_PITCH * 4;
 constexpr int MOST_STAGES = 7;
-constexpr int RING_BYTES = 96 * 1024, DEEP_RING_BYTES = 192 * 1024;  // beside the smaller an SM has room for a block of the first factor's
-constexpr size_t BESIDE_BYTES = 1024 + READERS * PATCH_BYTES + (2 * MOST_STAGES + 6) * 8 + (MOST_STAGES + 5) * 4;
+constexpr int RING_BYTES = 96 * 1024, LARGE_RING_BYTES = 128 * 1024;  // an SM has room for a block of the first factor's beside it
+constexpr size_t BESIDE_BYTES = 1024 + READERS * PATCH_BYTES + (2 * MOST_STAGES + 8) * 8 + (MOST_STAGES + 6) * 4;
 
 struct Maps {
   CUtensorMap x, w, t, b[KRK_MAX_PARTS];
@@ -331,9 +129,10 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
   uint64_t* acc_full = empty_bar + MOST_STAGES;   // either block's
   uint64_t* acc_empty = acc_full + 2;             // the first block's: the reading warps of both are through
   uint64_t* drain_bar = acc_empty + 2;
-  uint64_t* ready_bar = drain_bar + 1;            // the first block's: the second has its tensor memory
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ready_bar + 1);
-  int* issued = reinterpret_cast<int*>(tmem_slot + 1);  // blocks of k that were asked for, where a wait ran out; else -1
+  uint64_t* ready_bar = drain_bar + 1;            // [2] the first block's: the second has its accumulators
+  uint64_t* grown_bar = ready_bar + 2;            // either block's: the second accumulator is there
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(grown_bar + 1);  // [2]
+  int* issued = reinterpret_cast<int*>(tmem_slot + 2);  // blocks of k that were asked for, where a wait ran out; else -1
   volatile int* last = issued + 1;   // whether this block has brought a tile's last share
   volatile int* steps = issued + 2;  // [stages] of 16 k in the stage; 256 more: the tile's last
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -350,23 +149,32 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
     }
     mbar_init(drain_bar, 1);
     mbar_init(ready_bar, 1);
+    mbar_init(ready_bar + 1, 1);
+    mbar_init(grown_bar, 1);
     *issued = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
   cluster_sync();  // the other block's barriers exist
-  grid_launch_dependents();
-  // Two accumulators of a power of two of columns, no fewer than the tile's rows. With tiles of more than 128 rows that is all there is, and a block of the first
-  // factor's may hold some yet: only those who need it wait for it, while the ring fills.
+  // Two accumulators of a power of two of columns, no fewer than the tile's rows. With tiles of more than 128 rows they are all of tensor memory, and a block of
+  // the first factor's may hold some of it yet: the second one is taken when the first tile's products are on their way. Until then no later kernel's
+  // blocks are let in, which might take it and wait for this kernel's end.
   const int buf_cols = tiles.tile_rows <= 32 ? 32 : 1 << (32 - __clz(tiles.tile_rows - 1));
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * buf_cols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    if (rank == 1 && lane == 0) mbar_arrive_cluster(cluster_address(ready_bar, 0));
-  }
+  auto take = [&](int buf) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot + buf)), "r"(buf_cols) : "memory");
+    __syncwarp();
+    if (buf == 1) {
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+      grid_launch_dependents();
+      tc_fence_before();
+      if (lane == 0) mbar_arrive(grown_bar);
+    }
+    if (rank == 1 && lane == 0) mbar_arrive_cluster(cluster_address(ready_bar + buf, 0));
+  };
+  if (warp == 1) take(0);
   if (warp >= 1) asm volatile("bar.sync 1, %0;" ::"n"(THREADS - 32) : "memory");
   tc_fence_after();
-  const uint32_t tmem_base = warp >= 1 ? *tmem_slot : 0;
+  uint32_t tmem[2] = {warp >= 1 ? tmem_slot[0] : 0, 0};
   const int half = tiles.tile_rows / 2;  // rows that each block of the pair brings
   const uint32_t stage_bytes = W_BYTES + (uint32_t)half * BK * 2;
   const int stages = min(MOST_STAGES, (int)(ring_bytes / stage_bytes));
@@ -470,9 +278,23 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
     uint32_t parity = 0, acc_parity = 1;
     bool ok = rank == 0 && __all_sync(0xffffffffu, mbar_wait(ready_bar, 0));
     if (rank == 0 && !ok && lane == 0) atomicExch(error, 4);
+    bool grown = false;
+    auto grow = [&] {
+      if (grown) return;
+      grown = true;
+      take(1);
+      tmem[1] = tmem_slot[1];
+      if (rank == 0 && !__all_sync(0xffffffffu, mbar_wait(ready_bar + 1, 0))) {
+        ok = false;
+        if (lane == 0) atomicExch(error, 4);
+      }
+    };
+    if (buf_cols <= 128) grow();
     const uint32_t idesc = umma_idesc(256, tiles.tile_rows);
     while (ok && walk.next(t, u0, u1)) {
-      const uint32_t acc = tmem_base + (uint32_t)(buf * buf_cols);
+      if (buf == 1) grow();
+      if (!ok) break;
+      const uint32_t acc = buf ? tmem[1] : tmem[0];
       ok = mbar_wait(acc_empty + buf, acc_parity);  // both blocks have read what was there
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
@@ -512,6 +334,7 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
       buf ^= 1;
       acc_parity ^= buf == 0;
     }
+    grow();
   } else {
     const int quarter = warp & 3;
     unsigned char* patch = patches + (warp - 2) * PATCH_BYTES;
@@ -525,7 +348,15 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
       tc_fence_after();
       const int rt = t % row_tiles, wt = t / row_tiles, m0 = rt * tiles.tile_rows;
       const int live_rows = min(tiles.tile_rows, tiles.rows - m0);
-      const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * buf_cols);
+      if (buf == 1 && tmem[1] == 0) {  // (the first accumulator is not at 0 where the second is: asked again, to no harm)
+        if (!__all_sync(0xffffffffu, mbar_wait(grown_bar, 0))) {
+          if (lane == 0) atomicExch(error, 5);
+          break;
+        }
+        tmem[1] = *reinterpret_cast<volatile uint32_t*>(tmem_slot + 1);
+        tc_fence_after();
+      }
+      const uint32_t acc = (buf ? tmem[1] : tmem[0]) + ((uint32_t)(quarter * 32) << 16);
       const int c_first = (warp - 2) / 4 * 32;
       constexpr int C_STEP = 32 * (READERS / 4);
       const int parts = t >= shared ? walk.count(t) : 1;
@@ -657,7 +488,7 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
   cluster_sync();  // neither block's barriers are signalled any more
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * buf_cols) : "memory");
+    for (int b = 0; b < 2; ++b) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem[b]), "r"(buf_cols) : "memory");
   }
 }
 
@@ -685,59 +516,14 @@ int make_map_b(CUtensorMap* map, const AdapterBank& bank, int part, int N, bool 
   return make_map(map, base, 3, size, stride, box);
 }
 
-// rows and ranks of a copy of the first factor's: as many as there are
-int first_rows(const AdapterTiles& tiles) { return min(128, (min(tiles.rows, tiles.tile_rows) + 7) / 8 * 8); }
-int first_ranks(const AdapterBank& bank) { return min(FIRST_RANKS, (bank.parts * bank.rank + 15) / 16 * 16); }
-
-int launch_first(bf16* t, int* done, int n_done, const CUtensorMap& map_x, const CUtensorMap& map_a, int K, const AdapterBank& bank, const AdapterTiles& tiles, int* error, cudaStream_t stream) {
-  // an SM gives its memory to L1 or to blocks anew only when it is empty: split as the product's blocks need it, they come in beside these
-  static unsigned long long told = 0, allowed = 0;
-  int device = 0;
-  cudaError_t e = cudaGetDevice(&device);
-  if (e == cudaSuccess && !(__atomic_load_n(&told, __ATOMIC_RELAXED) >> (device & 63) & 1)) {
-    e = cudaFuncSetAttribute(first_factor_tiles_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-    if (e == cudaSuccess) __atomic_fetch_or(&told, 1ull << (device & 63), __ATOMIC_RELAXED);
-  }
-  if (e == cudaSuccess) e = allow_shared(first_factor_tiles_kernel, 1024 + FIRST_DEEP_BYTES, &allowed);
-  if (e != cudaSuccess) return (int)e;
-  const int row_tiles = (tiles.rows + tiles.tile_rows - 1) / tiles.tile_rows, ranks = bank.parts * bank.rank;
-  const int parts = (min(tiles.tile_rows, tiles.rows) + 127) / 128, chunks = (ranks + FIRST_RANKS - 1) / FIRST_RANKS;
-  // a single tile's adapters are in the first slots; of several tiles' some half are used
-  const int slots = row_tiles == 1 ? min(tiles.n_slots, bank.capacity) : tiles.n_slots;
-  const long long blocks = (long long)slots * parts * chunks * (row_tiles == 1 ? 2 : 1);
-  int ways = 1;
-  while (ways < 8 && ways * blocks <= FIRST_BLOCKS && K >= 64 * 2 * ways) ways *= 2;
-  // Where the product's blocks leave tensor memory for these, they run side by side; else these have the larger ring. Products read 128 rows, so that
-  // the last stage has them behind it.
-  const int stage = (first_rows(tiles) + first_ranks(bank)) * 128, behind = (128 - first_rows(tiles)) * 128;
-  const int stages = min(FIRST_STAGES, ((tiles.tile_rows > 128 ? FIRST_DEEP_BYTES : FIRST_BYTES) - behind) / stage);
-  const int bytes = 1024 + max(stages * stage + behind, 128 * FIRST_PITCH * 4);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(slots * ways, parts, chunks);
-  cfg.blockDim = dim3(FIRST_THREADS);
-  cfg.dynamicSmemBytes = bytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ways;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  static const bool plain = getenv("KRK_NO_PDL") != nullptr;
-  cfg.attrs = attr;
-  cfg.numAttrs = plain ? 1 : 2;
-  return (int)cudaLaunchKernelEx(&cfg, first_factor_tiles_kernel, t, done, n_done, map_x, map_a, K, bank, tiles, ways, stages, first_rows(tiles), first_ranks(bank), error);
-}
-
 template <bool GATED>
 int launch_gemm(const Maps& maps, bf16* out, float* shares, int* done, int shared, int most_shares, int aligned, int N, int K, const AdapterBank& bank, const AdapterTiles& tiles,
                 int pairs, int* error, cudaStream_t stream) {
   static unsigned long long allowed = 0;
   auto kern = adapted_gemm_kernel<GATED>;
-  const cudaError_t e = allow_shared(kern, BESIDE_BYTES + DEEP_RING_BYTES, &allowed);
+  const cudaError_t e = allow_shared(kern, BESIDE_BYTES + LARGE_RING_BYTES, &allowed);
   if (e != cudaSuccess) return (int)e;
-  const int ring = tiles.tile_rows <= 128 ? RING_BYTES : DEEP_RING_BYTES;
+  const int ring = tiles.tile_rows <= 128 ? RING_BYTES : LARGE_RING_BYTES;
   return (int)launch_pdl(kern, dim3(2 * pairs), dim3(THREADS), BESIDE_BYTES + ring, stream, maps, out, shares, done, shared, most_shares, aligned, ring, N, K, bank,
                          tiles, error);
 }
@@ -757,23 +543,19 @@ KRK_API int krk_adapted_gemm(void* out, const void* x, long long ldx, const void
     return -2;
   const AdapterTiles tiles = {row_adapter, info, slots, rows, tile_rows, n_slots};
   const long long all = (long long)((rows + tile_rows - 1) / tile_rows) * ((N + 255) / 256);
-  const int k_blocks = (K + BK - 1) / BK, per_adapter = bank->parts * bank->rank;
-  if (all * (k_blocks + n_slots) > 0x7fffffffLL || (long long)n_slots * tile_rows > 0x7fffffffLL || (long long)n_slots * 8 > 0x7fffffffLL ||
-      (long long)bank->capacity * per_adapter > 0x7fffffffLL)
+  const int k_blocks = (K + BK - 1) / BK;
+  if (all * (k_blocks + n_slots) > 0x7fffffffLL || (long long)n_slots * tile_rows > 0x7fffffffLL)
     return -3;
   if (shared < 0 || shared > all || (shared < all && (shared % PAIRS || !shares))) return -2;
   Maps maps;
-  CUtensorMap map_x, map_a;
   int rc = make_map_bf16(&maps.x, x, rows, K, ldx, tile_rows / 2);
   if (rc) return rc;
   rc = gated ? make_map_bf16_3d(&maps.w, w, K, 2, width, (long long)width * ldw, ldw, 2, 64) : make_map_bf16(&maps.w, w, N, K, ldw, 128);
   if (!rc) rc = make_map_bf16(&maps.t, t, (long long)n_slots * tile_rows, bank->parts * bank->wide, bank->parts * bank->wide, tile_rows / 2);
   for (int p = 0; p < bank->parts && !rc; ++p) rc = make_map_b(&maps.b[p], *bank, p, N, gated);
-  if (!rc) rc = make_map_bf16(&map_x, x, rows, K, ldx, first_rows(tiles));
-  if (!rc) rc = make_map_bf16(&map_a, bank->a, (long long)bank->capacity * per_adapter, K, K, first_ranks(*bank));
   const int rest = (int)(all - shared), most_shares = rest ? (PAIRS + rest - 1) / rest + 1 : 0;
   int* done = rest ? reinterpret_cast<int*>(shares + (size_t)rest * most_shares * tile_rows * 256) : nullptr;
-  if (!rc) rc = launch_first((bf16*)t, done, 2 * rest, map_x, map_a, K, *bank, tiles, error, stream);
+  if (!rc) rc = krk_first_factor(t, false, done, 2 * rest, x, ldx, K, *bank, tiles, error, stream);
   if (rc) return rc;
   const int pairs = rest || all > PAIRS ? PAIRS : (int)all;
   // as many pairs a tile, where that leaves few of them idle: fewer shares, and no pair has two

@@ -30,6 +30,7 @@ _ADAPT_SIGNATURES = {
     "krk_step_maps": [_P, _P, _P, _P, c_int, c_int, _P, c_int, c_int, _P, c_int, _P, _P, _P, _P, _P, POINTER(_P), POINTER(_P), POINTER(c_int), c_int, _P, _P],
     "krk_adapter_first": [_P, _P, c_longlong, c_int, c_int, _BANK, _P, _P, c_int, _P],
     "krk_adapted_gemm": [_P, _P, c_longlong, _P, c_longlong, c_int, c_int, c_int, _BANK, _P, _P, _P, c_int, c_int, _P, _P, c_int, c_int, _P, _P],
+    "krk_adapted_skinny": [_P, _P, _P, c_int, c_int, c_int, _BANK, _P, _P, _P, c_int, c_int, _P, c_int, _P, _P],
     "krk_adapter_second": [_P, _P, _P, c_int, c_int, _BANK, _P, c_int, c_int, _P],
 }
 
@@ -191,6 +192,13 @@ class AdapterOps:
         described, dtype, error = self._bank(bank), _code(w.dtype), self.error.data_ptr()
         ldx, ldw, x_at, w_at = x.stride(0) if M > 1 else K, w.stride(0) if N > 1 else K, x.data_ptr(), w.data_ptr()
         if w.dtype is torch.bfloat16 and K >= 64 and not (K | ldx | ldw | (gated or N)) & 7 and not (x_at | w_at) & 15:
+            if M <= self.SKINNY_MAX_ROWS and K % 32 == 0 and ldx == K and ldw == K and not os.environ.get("NOSK"):
+                t = self.error.new_empty(M * bank.parts * (-(-bank.rank // 16) * 8))
+                self.launches += 1
+                self._ok(self.adapt.krk_adapted_skinny(
+                    out.data_ptr(), x_at, w_at, M, N, K, described, rows.row_adapter.data_ptr(), rows.info[0], rows.slots[0], rows.n_slots[0], rows.heights[0],
+                    t.data_ptr(), int(gated > 0), error, self._stream()), what)
+                return out
             which, shared = self._tiling(rows, M, K, N)
             height = rows.heights[which]
             n_slots, tiles = rows.n_slots[which], -(-M // height) * -(-N // 256)

@@ -38,3 +38,8 @@ __device__ __forceinline__ int part_of(const AdapterBank& bank, int n) {
   for (int i = 1; i < KRK_MAX_PARTS; ++i) p += (i < bank.parts && n >= bank.begin[i]);
   return p;
 }
+
+// t = scale (x A^T) of every slot, or (compact) of every row that has an adapter (first_factor.cu); sets n_done words at `done` to zero. Lets the next kernel start
+// once what came before is over: that one may read what earlier kernels wrote before it waits, and waits before it reads t.
+int krk_first_factor(void* t, bool compact, int* done, int n_done, const void* x, long long ldx, int K, const AdapterBank& bank, const AdapterTiles& tiles, int* error,
+                     cudaStream_t stream);

@@ -40,14 +40,14 @@ SCAN_SOURCES = ["recurrent.cu", "recurrent_chunks.cu", "ssd.cu"]
 MEMORY_SOURCES = ["matrix_memory.cu", "matrix_memory_chunks.cu", "matrix_memory_step.cu"]
 MOE_SOURCES = ["routed.cu", "few_experts.cu", "grouped_gemm.cu"]
 CACHE_SOURCES = ["evict.cu"]
-ADAPT_SOURCES = ["adapters.cu", "adapted_gemm.cu"]
+ADAPT_SOURCES = ["adapters.cu", "first_factor.cu", "adapted_gemm.cu", "adapted_skinny.cu"]
 SMALL_LIBRARIES = {"mix": MIX_SOURCES, "scan": SCAN_SOURCES, "memory": MEMORY_SOURCES, "moe": MOE_SOURCES, "cache": CACHE_SOURCES,
                    "adapt": ADAPT_SOURCES}
 PARTS_SOURCES = ["partial_attention.cu", "few_rows_attention.cu", "many_rows_attention.cu", "prefix_tcgen05.cu", "key_weights_tcgen05.cu"]
 LATENT_SOURCES = ["latent_prefill.cu"]
 ATTN_SOURCES = ["attention_simple.cu", "attention_mma.cu", "attention_tcgen05.cu"]
 HEADERS = ["common.cuh", "mma.cuh", "tcgen05.cuh", "attention_noalloc.h", "attention_tiles.cuh", "partial_attention.cuh"]
-ADAPT_HEADERS = ["adapters.cuh"]
+OWN_HEADERS = {"core": ["skinny.cuh"], "adapt": ["skinny.cuh", "adapters.cuh", "warp_copies.cuh"]}
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
@@ -113,14 +113,13 @@ def library_path(kind: str, head_dim=None) -> tuple[Path, list, list]:
         sources, defines, stem = _existing(CORE_SOURCES), [], "libkrk_core"
     elif kind in SMALL_LIBRARIES:
         sources, defines, stem = _existing(SMALL_LIBRARIES[kind]), [], f"libkrk_{kind}"
-        headers = _existing(ADAPT_HEADERS) if kind == "adapt" else []
-        return build_dir() / f"{stem}_{_key(sources + headers, defines, [])}.so", sources, defines
+        return build_dir() / f"{stem}_{_key(sources + OWN_HEADERS.get(kind, []), defines, [])}.so", sources, defines
     elif kind == "parts":
         sources, defines = _existing(PARTS_SOURCES), [f"-DKRK_HEAD_DIM={int(head_dim)}"]
         return build_dir() / f"libkrk_parts_d{int(head_dim)}_{_key(sources, defines, [])}.so", sources, defines
     else:
         sources, defines, stem = _existing(ATTN_SOURCES), [f"-DKRK_HEAD_DIM={int(head_dim)}"], f"libkrk_attn_d{int(head_dim)}"
-    return build_dir() / f"{stem}_{_key(sources, defines)}.so", sources, defines
+    return build_dir() / f"{stem}_{_key(sources + OWN_HEADERS.get(kind, []), defines)}.so", sources, defines
 
 
 def _compile_one(nvcc: str, src: Path, obj: Path, defines) -> None:
