@@ -38,8 +38,8 @@ constexpr uint32_t W_BYTES = 128 * BK * 2;  // a block's half of the pair's weig
 constexpr int PATCH_PITCH = 36;             // words of two rows in a warp's patch for the transpose
 constexpr int PATCH_BYTES = 16 * PATCH_PITCH * 4;
 constexpr int MOST_STAGES = 7;
-constexpr int RING_BYTES = 96 * 1024, LARGE_RING_BYTES = 128 * 1024;  // an SM has room for a block of the first factor's beside it
-constexpr size_t BESIDE_BYTES = 1024 + READERS * PATCH_BYTES + (2 * MOST_STAGES + 8) * 8 + (MOST_STAGES + 6) * 4;
+constexpr int RING_BYTES = 128 * 1024;  // an SM has room for a block of the first factor's beside it
+constexpr size_t SMEM_BYTES = 1024 + RING_BYTES + READERS * PATCH_BYTES + (2 * MOST_STAGES + 8) * 8 + (MOST_STAGES + 6) * 4;
 
 struct Maps {
   CUtensorMap x, w, t, b[KRK_MAX_PARTS];
@@ -74,56 +74,67 @@ __device__ __forceinline__ void tmem_wait_ld_of(uint32_t (&r)[32]) {
                : "memory");
 }
 
-// The work of a pair: of the tiles before `shared`, tiles pair, pair + pairs, ... as a whole; of the tiles from there on a share. A tile's units are its blocks of k
-// and, where there is a single row tile, its adapters (else they go to who has the last k). With `aligned` a tile is dealt to so many pairs
-// in equal parts; else the units of all tiles, in order, to all pairs, `run` from pair * run on.
+// The work of a pair: of the tiles before `shared`, tiles pair, pair + pairs, ... as a whole; of the tiles from there on a share. A tile has its blocks of k
+// and, where there is a single row tile, its adapters (else they go to who has the last k). With `aligned` a tile is dealt to so many pairs, blocks and
+// adapters in equal parts; else the blocks and adapters of all tiles, in order, to all pairs, `run` from pair * run on.
 struct Walk {
-  int shared, units, run, aligned, at, end, whole, pairs;
-  __device__ Walk(int pair, int pairs_, int tiles, int shared_, int units_, int aligned_) : shared(shared_), units(units_), aligned(aligned_), whole(pair), pairs(pairs_) {
-    const int all = units * (tiles - shared);
-    if (aligned) {
-      run = (units + aligned - 1) / aligned;
-      const int t = pair / aligned, first = pair % aligned * run;
-      at = min(t * units + first, all);
-      end = t >= tiles - shared ? at : max(at, t * units + min(units, first + run));
+  int k_blocks, extra, shared, run, aligned, at, end, whole, pairs;
+  __device__ Walk(int pair, int pairs_, int tiles, int shared_, int k_blocks_, int extra_, int aligned_)
+      : k_blocks(k_blocks_), extra(extra_), shared(shared_), aligned(aligned_), whole(pair), pairs(pairs_) {
+    const int units = k_blocks + extra, all = units * (tiles - shared);
+    if (aligned) {  // tile and part
+      run = 1;
+      at = min(pair, (tiles - shared) * aligned);
+      end = min(pair + 1, (tiles - shared) * aligned);
     } else {
       run = max(1, (int)(((long long)all + pairs - 1) / pairs));
       at = (int)min((long long)pair * run, (long long)all);
       end = (int)min((long long)at + run, (long long)all);
     }
   }
-  // tile t, of which units u0 to u1
-  __device__ bool next(int& t, int& u0, int& u1) {
+  // tile t, of which blocks of k from k0 to k1, adapters from e0 to e1
+  __device__ bool next(int& t, int& k0, int& k1, int& e0, int& e1) {
     if (whole < shared) {
       t = whole;
       whole += pairs;
-      u0 = 0;
-      u1 = units;
+      k0 = e0 = 0;
+      k1 = k_blocks;
+      e1 = extra;
+      return true;
+    }
+    if (at >= end) return false;
+    if (aligned) {
+      const int part = at % aligned, ks = (k_blocks + aligned - 1) / aligned, es = (extra + aligned - 1) / aligned;
+      t = shared + at / aligned;
+      k0 = min(k_blocks, part * ks);
+      k1 = min(k_blocks, k0 + ks);
+      e0 = min(extra, part * es);
+      e1 = min(extra, e0 + es);
+      at = end;
       return true;
     }
     // from behind: a run begins with what it has of its last tile, whose t it does not need, and waits for t where nothing is left to load but that
-    if (at >= end) return false;
-    t = (end - 1) / units;
-    u1 = end - t * units;
-    u0 = max(0, at - t * units);
+    const int units = k_blocks + extra, of = (end - 1) / units, u1 = end - of * units, u0 = max(0, at - of * units);
+    t = shared + of;
+    k0 = min(k_blocks, u0);
+    k1 = min(k_blocks, u1);
+    e0 = max(0, u0 - k_blocks);
+    e1 = max(0, u1 - k_blocks);
     end -= u1 - u0;
-    t += shared;
     return true;
   }
-  __device__ int first_pair(int t) const { return aligned ? (t - shared) * aligned : (int)((long long)(t - shared) * units / run); }
-  __device__ int count(int t) const {
-    return aligned ? (units + run - 1) / run : (int)(((long long)(t - shared + 1) * units - 1) / run) - first_pair(t) + 1;
-  }
+  __device__ int first_pair(int t) const { return aligned ? (t - shared) * aligned : (int)((long long)(t - shared) * (k_blocks + extra) / run); }
+  __device__ int count(int t) const { return aligned ? aligned : (int)(((long long)(t - shared + 1) * (k_blocks + extra) - 1) / run) - first_pair(t) + 1; }
 };
 
 template <bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(512)  // (of 320: 128 registers a thread leave room for a block of the first factor's)
-adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, float* __restrict__ shares, int* __restrict__ done, int shared, int most_shares, int aligned, int ring_bytes, int N, int K, const __grid_constant__ AdapterBank bank,
+adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, float* __restrict__ shares, int* __restrict__ done, int shared, int most_shares, int aligned, int N, int K, const __grid_constant__ AdapterBank bank,
                     const __grid_constant__ AdapterTiles tiles, int* __restrict__ error) {
   constexpr int BC = GATED ? 64 : 128;  // columns of C a block makes of a tile; the pair twice as many
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  unsigned char* patches = ring + ring_bytes;
+  unsigned char* patches = ring + RING_BYTES;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(patches + READERS * PATCH_BYTES);  // the first block's: copies of both have landed
   uint64_t* empty_bar = full_bar + MOST_STAGES;   // either block's: the products have read a stage
   uint64_t* acc_full = empty_bar + MOST_STAGES;   // either block's
@@ -177,13 +188,13 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
   uint32_t tmem[2] = {warp >= 1 ? tmem_slot[0] : 0, 0};
   const int half = tiles.tile_rows / 2;  // rows that each block of the pair brings
   const uint32_t stage_bytes = W_BYTES + (uint32_t)half * BK * 2;
-  const int stages = min(MOST_STAGES, (int)(ring_bytes / stage_bytes));
+  const int stages = min(MOST_STAGES, (int)(RING_BYTES / stage_bytes));
   const int k_blocks = (K + BK - 1) / BK, row_tiles = (tiles.rows + tiles.tile_rows - 1) / tiles.tile_rows;
   const int all_tiles = row_tiles * ((N + 2 * BC - 1) / (2 * BC));
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const bool extras = row_tiles == 1;
-  Walk walk(pair, pairs, all_tiles, shared, k_blocks + (extras ? tiles.info[1] : 0), aligned);
-  int t, u0, u1;
+  Walk walk(pair, pairs, all_tiles, shared, k_blocks, extras ? tiles.info[1] : 0, aligned);
+  int t, k0, k1, e0, e1;
 
   if (warp == 0) {
     int s = 0, asked = 0;
@@ -213,7 +224,7 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
       else tma_load_2d_pair_warp(stage, &maps.w, bar, kb * BK, f0);
       tma_load_2d_pair_warp(stage + W_BYTES, &maps.x, bar, kb * BK, m0);
     };
-    while (ok && walk.next(t, u0, u1)) {
+    while (ok && walk.next(t, k0, k1, e0, e1)) {
       const int rt = t % row_tiles, wt = t / row_tiles, f0 = (wt * 2 + (int)rank) * BC, m0 = rt * tiles.tile_rows + (int)rank * half;
       const int first = tiles.info[2 * rt], count = tiles.info[2 * rt + 1];
       // which parts the pair's columns reach into (gated: both)
@@ -222,7 +233,7 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
         p0 = part_of(bank, wt * 2 * BC);
         p1 = part_of(bank, min(N, (wt + 1) * 2 * BC) - 1) + 1;
       }
-      const int e0 = extras ? max(0, u0 - k_blocks) : 0, e1 = extras ? u1 - k_blocks : u1 == k_blocks ? count : 0;  // of the tile's adapters
+      if (!extras) e1 = k1 == k_blocks ? count : 0;
       // a lane's adapter of the list, and its parts' ranks in steps of 16, a byte each
       int a = -1;
       uint32_t ranks = 0;
@@ -240,13 +251,12 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
         for (int p = p0; p < p1; ++p) n += ((ranks >> 8 * p & 255) + 3) / 4;
         left += __reduce_add_sync(0xffffffffu, n);
       }
-      const int k1 = min(k_blocks, u1);
-      for (int kb = u0; kb < k1; ++kb) {
+      for (int kb = k0; kb < k1; ++kb) {
         if (!enter(4 | (kb + 1 == k1 && left == 0 ? 256 : 0))) break;
         shared_block(kb, f0, m0);
       }
       // a share of adapters that leave these columns as they are: zeros from behind the last k
-      if (ok && u0 >= k1 && left == 0 && enter(1 | 256)) shared_block(k_blocks, f0, m0);
+      if (ok && k0 >= k1 && left == 0 && enter(1 | 256)) shared_block(k_blocks, f0, m0);
       for (int i = e0; i < e1 && ok; ++i) {
         if ((i - e0) % 32 == 0) look(i);
         grid_dependency_wait();  // t
@@ -291,7 +301,7 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
     };
     if (buf_cols <= 128) grow();
     const uint32_t idesc = umma_idesc(256, tiles.tile_rows);
-    while (ok && walk.next(t, u0, u1)) {
+    while (ok && walk.next(t, k0, k1, e0, e1)) {
       if (buf == 1) grow();
       if (!ok) break;
       const uint32_t acc = buf ? tmem[1] : tmem[0];
@@ -340,7 +350,7 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
     unsigned char* patch = patches + (warp - 2) * PATCH_BYTES;
     int buf = 0;
     uint32_t parity = 0;
-    while (walk.next(t, u0, u1)) {
+    while (walk.next(t, k0, k1, e0, e1)) {
       if (!__all_sync(0xffffffffu, mbar_wait(acc_full + buf, parity))) {
         if (lane == 0) atomicExch(error, 5);
         break;
@@ -521,10 +531,9 @@ int launch_gemm(const Maps& maps, bf16* out, float* shares, int* done, int share
                 int pairs, int* error, cudaStream_t stream) {
   static unsigned long long allowed = 0;
   auto kern = adapted_gemm_kernel<GATED>;
-  const cudaError_t e = allow_shared(kern, BESIDE_BYTES + LARGE_RING_BYTES, &allowed);
+  const cudaError_t e = allow_shared(kern, SMEM_BYTES, &allowed);
   if (e != cudaSuccess) return (int)e;
-  const int ring = tiles.tile_rows <= 128 ? RING_BYTES : LARGE_RING_BYTES;
-  return (int)launch_pdl(kern, dim3(2 * pairs), dim3(THREADS), BESIDE_BYTES + ring, stream, maps, out, shares, done, shared, most_shares, aligned, ring, N, K, bank,
+  return (int)launch_pdl(kern, dim3(2 * pairs), dim3(THREADS), SMEM_BYTES, stream, maps, out, shares, done, shared, most_shares, aligned, N, K, bank,
                          tiles, error);
 }
 
@@ -559,7 +568,7 @@ KRK_API int krk_adapted_gemm(void* out, const void* x, long long ldx, const void
   if (rc) return rc;
   const int pairs = rest || all > PAIRS ? PAIRS : (int)all;
   // as many pairs a tile, where that leaves few of them idle: fewer shares, and no pair has two
-  const int aligned = rest && rest * (PAIRS / rest) * 10 >= PAIRS * 9 ? PAIRS / rest : 0;
+  const int aligned = rest && rest * (PAIRS / rest) * 10 >= PAIRS * 9 ? min(PAIRS / rest, k_blocks) : 0;
   return gated ? launch_gemm<true>(maps, (bf16*)out, shares, done, shared, most_shares, aligned, width, K, *bank, tiles, pairs, error, stream)
                : launch_gemm<false>(maps, (bf16*)out, shares, done, shared, most_shares, aligned, width, K, *bank, tiles, pairs, error, stream);
 }

@@ -8,13 +8,13 @@ others, never share any.
 from __future__ import annotations
 
 import ctypes
-import os
-from ctypes import POINTER, Structure, byref, c_float, c_int, c_longlong, c_void_p
+from ctypes import POINTER, Structure, byref, c_int, c_longlong, c_void_p
+from functools import lru_cache
 
 import torch
 
 from .build import build_library
-from .cache_ops import PAGE, KernelError, _code, _current_device, _load, _ptr
+from .cache_ops import KernelError, _code, _current_device, _load, _ptr
 
 _P = c_void_p
 _I32 = torch.int32
@@ -27,7 +27,7 @@ class _Bank(Structure):
 
 _BANK = POINTER(_Bank)
 _ADAPT_SIGNATURES = {
-    "krk_step_maps": [_P, _P, _P, _P, c_int, c_int, _P, c_int, c_int, _P, c_int, _P, _P, _P, _P, _P, POINTER(_P), POINTER(_P), POINTER(c_int), c_int, _P, _P],
+    "krk_step_maps": [_P, _P, _P, _P, c_int, c_int, _P, c_int, c_int, _P, c_int, _P, c_int, _P, _P],
     "krk_adapter_first": [_P, _P, c_longlong, c_int, c_int, _BANK, _P, _P, c_int, _P],
     "krk_adapted_gemm": [_P, _P, c_longlong, _P, c_longlong, c_int, c_int, c_int, _BANK, _P, _P, _P, c_int, c_int, _P, _P, c_int, c_int, _P, _P],
     "krk_adapted_skinny": [_P, _P, _P, c_int, c_int, c_int, _BANK, _P, _P, _P, c_int, c_int, _P, c_int, _P, _P],
@@ -37,36 +37,66 @@ _ADAPT_SIGNATURES = {
 
 class AdapterRows:
     """Which adapter each row of a step has (``row_adapter``, int32 on the device, -1 for none), and for tiles of rows of
-    one height or three the adapters that occur in them. Made by ``Kernels.step_maps``."""
+    one height or three the adapters that occur in them. A part of ``StepMaps``."""
 
     HEIGHTS = (128, 192, 256)
 
-    def __init__(self, n_rows: int, n_seqs: int, device):
-        self.n_rows, self.n_seqs = n_rows, n_seqs
-        self.heights = self.HEIGHTS if n_rows > 256 else (max(32, -(-n_rows // 32) * 32),)
-        tiles = [-(-n_rows // h) for h in self.heights]
-        self.n_slots = [t + n_seqs for t in tiles]
-        at = n_rows + n_rows % 2  # pairs of words lie on boundaries of theirs
-        self.buffer = torch.empty(at + sum(2 * t + 2 * s for t, s in zip(tiles, self.n_slots)), dtype=_I32, device=device)
-        self.row_adapter = self.buffer[:n_rows]
-        address = self.buffer.data_ptr()
-        self.info, self.slots = [], []  # addresses
-        for t, s in zip(tiles, self.n_slots):
-            self.info.append(address + 4 * at)
-            self.slots.append(address + 4 * (at + 2 * t))
-            at += 2 * t + 2 * s
+    def __init__(self, maps: "StepMaps", at: int):
+        self.n_rows, self.n_seqs = maps.n_rows, maps.n_seqs
+        self.heights = self.HEIGHTS if self.n_rows > 256 else (max(32, -(-self.n_rows // 32) * 32),)
+        self.buffer, self._at = maps.buffer, at
+        self.row_adapter_at = maps.address + 4 * at
+
+    @property
+    def row_adapter(self):
+        return self.buffer[self._at:self._at + self.n_rows]
+
+    def tiles(self, which: int) -> tuple:
+        """(height, address of the tiles' first slots and counts, address of the slots, slots) for one of the heights."""
+        at = self.row_adapter_at + 4 * (self.n_rows + self.n_rows % 2)
+        for i, height in enumerate(self.heights):
+            tiles = -(-self.n_rows // height)
+            if i == which:
+                return height, at, at + 8 * tiles, tiles + self.n_seqs
+            at += 8 * (2 * tiles + self.n_seqs)
+        raise IndexError(which)
+
+    def words(self) -> int:
+        """Of the buffer: a row's adapter, then on a boundary of eight bytes the heights' tiles and slots, two words each."""
+        return self.n_rows + self.n_rows % 2 + sum(2 * (2 * -(-self.n_rows // h) + self.n_seqs) for h in self.heights)
 
 
 class StepMaps:
     """What ``Kernels.step_maps`` makes: ``cu_q`` [sequences + 1], the first row of every sequence; ``row_seq``, ``row_pos`` [rows], a row's sequence and
-    position; with a page table ``row_place`` [rows] (int64), its place in the cache, page * 64 + position in the page; ``adapters`` (AdapterRows or None)."""
+    position; with a page table ``row_place`` [rows] (int64), its place in the cache, page * 64 + position in the page; ``adapters`` (AdapterRows or None).
+    All are views of one buffer."""
 
     def __init__(self, n_rows: int, n_seqs: int, device, with_places: bool = True, with_adapters: bool = True):
-        self.n_rows, self.n_seqs = n_rows, n_seqs
-        self.buffer = torch.empty(n_seqs + 1 + 2 * n_rows, dtype=_I32, device=device)
-        self.cu_q, self.row_seq, self.row_pos = self.buffer[:n_seqs + 1], self.buffer[n_seqs + 1:n_seqs + 1 + n_rows], self.buffer[n_seqs + 1 + n_rows:]
-        self.row_place = torch.empty(n_rows, dtype=torch.int64, device=device) if with_places else None
-        self.adapters = AdapterRows(n_rows, n_seqs, device) if with_adapters else None
+        self.n_rows, self.n_seqs, self.with_places = n_rows, n_seqs, with_places
+        # places first; adapters on a boundary of eight bytes
+        self._first = 2 * n_rows if with_places else 0
+        at = self._first + n_seqs + 1 + 2 * n_rows
+        at += at % 2
+        extra = 0
+        if with_adapters:
+            tiles = sum(2 * (2 * -(-n_rows // h) + n_seqs) for h in AdapterRows.HEIGHTS) if n_rows > 256 else 2 * (2 * (n_rows > 0) + n_seqs)
+            extra = n_rows + n_rows % 2 + tiles
+        self.buffer = torch.empty(at + extra, dtype=_I32, device=device)
+        self.address = self.buffer.data_ptr()
+        self.adapters = AdapterRows(self, at) if with_adapters else None
+        self._views = None
+
+    def _split(self):
+        if self._views is None:
+            n, rows, words = self.n_seqs + 1, self.n_rows, self.buffer
+            parts = words.split_with_sizes((self._first, n, rows, rows, words.shape[0] - self._first - n - 2 * rows))
+            self._views = (parts[0].view(torch.int64) if self.with_places else None, parts[1], parts[2], parts[3])
+        return self._views
+
+    row_place = property(lambda self: self._split()[0])
+    cu_q = property(lambda self: self._split()[1])
+    row_seq = property(lambda self: self._split()[2])
+    row_pos = property(lambda self: self._split()[3])
 
 
 class AdapterOps:
@@ -94,52 +124,55 @@ class AdapterOps:
         what, n, n_rows = "maps of a step", lengths.shape[0], int(n_rows)
         if n_rows < 0 or n > self.MOST_SEQUENCES:
             raise KernelError(f"{what}: {n} sequences with {n_rows} rows (up to {self.MOST_SEQUENCES} sequences are taken)")
-        for name, t in (("slots", slots), ("starts", starts), ("lengths", lengths), ("adapters", adapters)):
-            if t is not None and (t.dtype is not _I32 or t.shape != (n,) or not t.is_contiguous()):
-                raise KernelError(f"{what}: {name} are contiguous int32, one for each of {n} sequences, got {t.dtype} {list(t.shape)}")
+        tensors = (slots, starts, lengths) if adapters is None else (slots, starts, lengths, adapters)
+        for t in tensors:
+            if t.dtype is not _I32 or t.shape != (n,) or not t.is_contiguous():
+                raise KernelError(f"{what}: slots, starts, lengths and adapters are contiguous int32, one for each of {n} sequences, got "
+                                  f"{', '.join(f'{t.dtype} {list(t.shape)}' for t in tensors)}")
         width = n_slots = n_pages = 0
         if table is not None:
             if table.dtype is not _I32 or table.dim() != 2 or not table.is_contiguous():
                 raise KernelError(f"{what}: the page table is contiguous int32 [slots, pages of a slot], got {table.dtype} {list(table.shape)}")
             n_slots, width = table.shape
+            tensors += (table,)
             if pages is not None:
                 if pages.dtype is not _I32 or pages.dim() != 1 or not pages.is_contiguous():
                     raise KernelError(f"{what}: pages are a contiguous int32 list, got {pages.dtype} {list(pages.shape)}")
                 n_pages = pages.shape[0]
+                tensors += (pages,)
         elif pages is not None:
             raise KernelError(f"{what}: pages are entered in a page table, and there is none")
-        self._check_device(what, slots, starts, lengths, *(t for t in (table, pages, adapters) if t is not None))
+        self._check_device(what, *tensors)
         if out is None:
             out = StepMaps(n_rows, n, lengths.device, table is not None, adapters is not None)
-        elif (out.n_rows, out.n_seqs) != (n_rows, n) or (table is not None and out.row_place is None) or (out.adapters is None) != (adapters is None):
+        elif (out.n_rows, out.n_seqs) != (n_rows, n) or (table is not None and not out.with_places) or (out.adapters is None) != (adapters is None):
             raise KernelError(f"{what}: maps made for {out.n_seqs} sequences with {out.n_rows} rows do not fit {n} with {n_rows}, or lack places or adapters")
-        rows = out.adapters
-        if rows is None:
-            info = lists = heights = None
-            count = 0
-        else:
-            count = len(rows.heights)
-            info, lists, heights = (_P * count)(*rows.info), (_P * count)(*rows.slots), (c_int * count)(*rows.heights)
+        elif out.buffer.get_device() != lengths.get_device():
+            raise KernelError(f"{what}: maps on {out.buffer.device} for lengths on {lengths.device}")
         self._ok(self.adapt.krk_step_maps(
             slots.data_ptr(), starts.data_ptr(), lengths.data_ptr(), _ptr(adapters), n, n_rows, _ptr(table), width, n_slots, _ptr(pages), n_pages,
-            out.cu_q.data_ptr(), out.row_seq.data_ptr(), out.row_pos.data_ptr(), None if rows is None else rows.row_adapter.data_ptr(),
-            None if table is None else out.row_place.data_ptr(), info, lists, heights, count, self.error.data_ptr(), self._stream()), what)
+            out.address, int(out.with_places), self.error.data_ptr(), self._stream()), what)
         return out
 
     # -- products ------------------------------------------------------------------------------
     def _check_adapted(self, what, x, w, bank, rows):
-        (M, K), (N, k) = x.shape, w.shape
+        """Raise unless the product can be taken; (rows, inputs, outputs, elements between rows of x and of w, their addresses)."""
+        (M, K), (N, k), (ldx, step_x), (ldw, step_w), dtype = x.shape, w.shape, x.stride(), w.stride(), w.dtype
         if k != K or bank.inputs != K or bank.outputs != N:
             raise KernelError(f"{what}: rows of {K} and weights {list(w.shape)} do not fit a bank from {bank.inputs} to {list(bank.outs)}")
-        if x.dtype is not w.dtype or bank.dtype is not w.dtype:
+        if x.dtype is not dtype or bank.dtype is not dtype:
             raise KernelError(f"{what}: rows, weights and adapters have one dtype, got {x.dtype}, {w.dtype} and {bank.dtype}")
         if rows.n_rows != M:
             raise KernelError(f"{what}: {M} rows, and adapters for {rows.n_rows}")
-        if x.stride(1) != 1 or w.stride(1) != 1 or (M > 1 and x.stride(0) < K) or (N > 1 and w.stride(0) < K):
+        if M <= 1:
+            ldx = K  # (a single row has no stride that means anything)
+        if N <= 1:
+            ldw = K
+        if step_x != 1 or step_w != 1 or ldx < K or ldw < K:
             raise KernelError(f"{what}: rows of elements side by side are asked for, got strides {x.stride()} and {w.stride()}")
-        here = self.error.get_device()
-        if not here == x.get_device() == w.get_device() == bank.a.get_device() == rows.buffer.get_device() == _current_device():
+        if not self.error.get_device() == x.get_device() == w.get_device() == bank.a.get_device() == rows.buffer.get_device() == _current_device():
             self._check_device(what, x, w, bank.a, rows.buffer)
+        return M, K, N, ldx, ldw, x.data_ptr(), w.data_ptr()
 
     @staticmethod
     def _bank(bank):
@@ -165,57 +198,52 @@ class AdapterOps:
 
     PAIRS = 74  # of SMs
 
-    def _tiling(self, rows, M: int, K: int, N: int) -> tuple[int, int]:
+    @staticmethod
+    @lru_cache(maxsize=4096)
+    def _tiling(heights, M: int, K: int, N: int) -> tuple[int, int]:
         """(which of the rows' tile heights, the first tile that the pairs share): by the time of whole rounds of the pairs, or of whole rounds
         and shares of what is left, in clocks."""
-        if len(rows.heights) == 1:
+        if len(heights) == 1:
             return 0, 0
-        if os.environ.get('TR'):
-            h = int(os.environ['TR']); i = rows.heights.index(h); tiles = -(-M // h) * -(-N // 256)
-            return i, (tiles if os.environ.get('NOSH') else tiles // 74 * 74)
         best = None
-        for i, h in enumerate(rows.heights):
+        for i, h in enumerate(heights):
             tiles = -(-M // h) * -(-N // 256)
             tile = -(-K // 64) * (176 + 1.3125 * h)
-            whole, rest = divmod(tiles, self.PAIRS)
-            for cost, shared in (((whole + (rest > 0)) * tile, tiles), (whole * tile + rest / self.PAIRS * tile + 6000 + (self.PAIRS + rest) * h / 2, tiles - rest)):
+            whole, rest = divmod(tiles, AdapterOps.PAIRS)
+            for cost, shared in (((whole + (rest > 0)) * tile, tiles), (whole * tile + rest / AdapterOps.PAIRS * tile + 6000 + (AdapterOps.PAIRS + rest) * h / 2, tiles - rest)):
                 if best is None or cost < best[0]:
                     best = cost, i, shared
         return best[1], best[2]
 
     def _adapted(self, what, x, w, bank, rows, gated):
-        self._check_adapted(what, x, w, bank, rows)
-        (M, K), N = x.shape, w.shape[0]
+        M, K, N, ldx, ldw, x_at, w_at = self._check_adapted(what, x, w, bank, rows)
         out = x.new_empty(M, gated or N)
         if M == 0:
             return out
-        described, dtype, error = self._bank(bank), _code(w.dtype), self.error.data_ptr()
-        ldx, ldw, x_at, w_at = x.stride(0) if M > 1 else K, w.stride(0) if N > 1 else K, x.data_ptr(), w.data_ptr()
-        if w.dtype is torch.bfloat16 and K >= 64 and not (K | ldx | ldw | (gated or N)) & 7 and not (x_at | w_at) & 15:
-            if M <= self.SKINNY_MAX_ROWS and K % 32 == 0 and ldx == K and ldw == K and not os.environ.get("NOSK"):
-                t = self.error.new_empty(M * bank.parts * (-(-bank.rank // 16) * 8))
-                self.launches += 1
-                self._ok(self.adapt.krk_adapted_skinny(
-                    out.data_ptr(), x_at, w_at, M, N, K, described, rows.row_adapter.data_ptr(), rows.info[0], rows.slots[0], rows.n_slots[0], rows.heights[0],
-                    t.data_ptr(), int(gated > 0), error, self._stream()), what)
+        described, error, stream, row_adapter = self._bank(bank), self.error.data_ptr(), self._stream(), rows.row_adapter_at
+        if bank.dtype is torch.bfloat16 and K >= 64 and not (K | ldx | ldw | (gated or N)) & 7 and not (x_at | w_at) & 15:
+            self.launches += 1
+            half_width = bank.parts * (-(-bank.rank // 16) * 8)
+            if M <= self.SKINNY_MAX_ROWS and not K & 31 and ldx == K and ldw == K:
+                height, info, slots, n_slots = rows.tiles(0)
+                t = self.error.new_empty(M * half_width)
+                self._ok(self.adapt.krk_adapted_skinny(out.data_ptr(), x_at, w_at, M, N, K, described, row_adapter, info, slots, n_slots, height, t.data_ptr(),
+                                                       int(gated > 0), error, stream), what)
                 return out
-            which, shared = self._tiling(rows, M, K, N)
-            height = rows.heights[which]
-            n_slots, tiles = rows.n_slots[which], -(-M // height) * -(-N // 256)
-            t_words = n_slots * height * bank.parts * (-(-bank.rank // 16) * 8)
-            rest = tiles - shared
+            which, shared = self._tiling(rows.heights, M, K, N)
+            height, info, slots, n_slots = rows.tiles(which)
+            rest = -(-M // height) * -(-N // 256) - shared
+            t_words = n_slots * height * half_width
             t = self.error.new_empty(t_words + (rest * ((-(-self.PAIRS // rest) + 1) * height * 256 + 2) if rest else 0))
             t_at = t.data_ptr()
-            self.launches += 1
-            self._ok(self.adapt.krk_adapted_gemm(
-                out.data_ptr(), x_at, ldx, w_at, ldw, M, N, K, described, rows.row_adapter.data_ptr(), rows.info[which], rows.slots[which], n_slots, height,
-                t_at, t_at + 4 * t_words if rest else None, shared, int(gated > 0), error, self._stream()), what)
+            self._ok(self.adapt.krk_adapted_gemm(out.data_ptr(), x_at, ldx, w_at, ldw, M, N, K, described, row_adapter, info, slots, n_slots, height, t_at,
+                                                 t_at + 4 * t_words if rest else None, shared, int(gated > 0), error, stream), what)
             return out
-        t = self.error.new_empty(M * bank.parts * (-(-bank.rank // 16) * 16))
+        # float32, and sizes, strides and addresses that the tensor cores' copies do not take
         if not x.is_contiguous():
             x = x.contiguous()
-        y = self.linear(x, w, out_float32=True)
-        stream, row_adapter = self._stream(), rows.row_adapter.data_ptr()
+        t = self.error.new_empty(M * bank.parts * (-(-bank.rank // 16) * 16))
+        y, dtype = self.linear(x, w, out_float32=True), _code(w.dtype)
         self._ok(self.adapt.krk_adapter_first(t.data_ptr(), x.data_ptr(), K, M, K, described, row_adapter, error, dtype, stream), what)
         self._ok(self.adapt.krk_adapter_second(out.data_ptr(), y.data_ptr(), t.data_ptr(), M, N, described, row_adapter, int(gated > 0), dtype, stream), what)
         return out

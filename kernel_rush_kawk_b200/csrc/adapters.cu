@@ -251,23 +251,41 @@ __global__ void __launch_bounds__(256) second_factor_kernel(T* __restrict__ out,
 
 }  // namespace
 
-// The maps of a step of n_seqs sequences and n_rows rows. Optional: adapters (with row_adapter and the lists of n_lists tile heights), table
-// (with slots and pages, of which n_pages are given). Heights are 128, 192 or 256, or one height of at least n_rows and at most 256.
-KRK_API int krk_step_maps(const int* slots, const int* starts, const int* lengths, const int* adapters, int n_seqs, int n_rows, int* table, int width,
-                          int n_slots, const int* pages, int n_pages, int* cu, int* row_seq, int* row_pos, int* row_adapter, long long* row_place,
-                          int* const* info, int* const* list, const int* tile_rows, int n_lists, int* error, cudaStream_t stream) {
+// The maps of a step of n_seqs sequences and n_rows rows. Optional: adapters, table (with slots and pages, of which n_pages are given). `words` takes, in order:
+// with `places` row_place (two words a row); cu [n_seqs + 1], row_seq and row_pos [n_rows]; with adapters, on a boundary of two words each, row_adapter [n_rows], and for
+// tiles of 128, 192 and 256 rows, or of all rows up to a multiple of 32 where there are no more than 256, a tile's first slot and number of adapters, and the
+// slots, one for each tile and sequence: an adapter and its tile.
+KRK_API int krk_step_maps(const int* slots, const int* starts, const int* lengths, const int* adapters, int n_seqs, int n_rows, int* table, int width, int n_slots,
+                          const int* pages, int n_pages, int* words, int places, int* error, cudaStream_t stream) {
   constexpr size_t MOST = 200 * 1024;
   const size_t smem = (size_t)(n_seqs + 1) * 8;
-  if (n_seqs < 0 || n_rows < 0 || n_lists < 0 || n_lists > 3 || smem > MOST) return -2;
-  Maps m = {slots, starts, lengths, adapters, n_seqs, n_rows, table, width, n_slots, pages, n_pages, cu, row_seq, row_pos, row_adapter, row_place};
-  m.n_lists = n_lists;
-  m.error = error;
-  for (int i = 0; i < n_lists; ++i) {
-    if (tile_rows[i] < 1 || tile_rows[i] > 256 || (n_rows > tile_rows[i] && MAP_ROWS % tile_rows[i])) return -2;
-    m.info[i] = info[i];
-    m.list[i] = list[i];
-    m.tile_rows[i] = tile_rows[i];
+  if (n_seqs < 0 || n_rows < 0 || smem > MOST || ((uintptr_t)words & 7) || (table && !places)) return -2;
+  Maps m = {slots, starts, lengths, adapters, n_seqs, n_rows, table, width, n_slots, pages, n_pages};
+  int* const first = words;
+  if (places) {
+    m.row_place = table ? reinterpret_cast<long long*>(words) : nullptr;
+    words += 2 * (size_t)n_rows;
   }
+  m.cu = words;
+  m.row_seq = m.cu + n_seqs + 1;
+  m.row_pos = m.row_seq + n_rows;
+  words = m.row_pos + n_rows;
+  if (adapters) {
+    words += (words - first) & 1;
+    m.row_adapter = words;
+    words += n_rows + (n_rows & 1);
+    const int all[3] = {128, 192, 256}, one = n_rows > 32 ? (n_rows + 31) / 32 * 32 : 32;
+    m.n_lists = n_rows > 256 ? 3 : 1;
+    for (int i = 0; i < m.n_lists; ++i) {
+      const int height = m.n_lists == 1 ? one : all[i];
+      const size_t tiles = ((size_t)n_rows + height - 1) / height;
+      m.tile_rows[i] = height;
+      m.info[i] = words;
+      m.list[i] = words + 2 * tiles;
+      words += 2 * (2 * tiles + n_seqs);
+    }
+  }
+  m.error = error;
   static unsigned long long allowed = 0;
   if (smem > 32 * 1024) {
     const cudaError_t e = allow_shared(step_maps_kernel, MOST, &allowed);

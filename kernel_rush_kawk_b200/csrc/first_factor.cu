@@ -17,12 +17,13 @@ using namespace tc;
 // The product's blocks come in while these run, once what came before is over, and wait for t where they need it; so a ring of few blocks of k is no
 // larger than fits beside theirs.
 constexpr int FIRST_RANKS = 128, FIRST_STAGES = 8, FIRST_THREADS = 192, FIRST_PITCH = FIRST_RANKS + 4;
-constexpr int FIRST_BYTES = 100 * 1024, FIRST_SMALL_BYTES = 72 * 1024;  // of the ring, beside the product's smaller and larger one
+constexpr int FIRST_BYTES = 72 * 1024;  // of the ring, beside the product's
 constexpr int FIRST_BLOCKS = 148;  // as many as are worth sharing k among
-static_assert(128 * FIRST_PITCH * 4 <= FIRST_SMALL_BYTES, "the sums take the ring's place");
+static_assert(128 * FIRST_PITCH * 4 <= FIRST_BYTES, "the sums take the ring's place");
 
 template <bool COMPACT>
-__global__ void __launch_bounds__(FIRST_THREADS) first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_done, const __grid_constant__ CUtensorMap map_x,
+__global__ void __launch_bounds__(FIRST_THREADS, 5)  // (of three that an SM's memory takes: in 64 registers they fit beside the product's)
+first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_done, const __grid_constant__ CUtensorMap map_x,
                                                                            const __grid_constant__ CUtensorMap map_a, int K,
                                                                            const __grid_constant__ AdapterBank bank, const __grid_constant__ AdapterTiles tiles,
                                                                            int ways, int stages, int box_rows, int box_ranks, int* __restrict__ error) {
@@ -141,11 +142,21 @@ __global__ void __launch_bounds__(FIRST_THREADS) first_factor_tiles_kernel(bf16*
       const int rank = bank.ranks[a * bank.parts + part];
       const float scale = bank.scale[a * bank.parts + part];
       float v[8] = {};
-      for (int w = 0; w < ways; ++w) {
-        const float* from = (ways > 1 ? cg::this_cluster().map_shared_rank(sums, w) : sums) + row * FIRST_PITCH + c;
-        const float4 lo = *reinterpret_cast<const float4*>(from), hi = *reinterpret_cast<const float4*>(from + 4);
-        v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
-        v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
+      for (int w0 = 0; w0 < ways; w0 += 4) {  // four blocks' on their way at once
+        float4 lo[4], hi[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          if (w0 + w < ways) {
+            const float* from = (ways > 1 ? cg::this_cluster().map_shared_rank(sums, w0 + w) : sums) + row * FIRST_PITCH + c;
+            lo[w] = *reinterpret_cast<const float4*>(from);
+            hi[w] = *reinterpret_cast<const float4*>(from + 4);
+          }
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          if (w0 + w < ways) {
+            v[0] += lo[w].x; v[1] += lo[w].y; v[2] += lo[w].z; v[3] += lo[w].w;
+            v[4] += hi[w].x; v[5] += hi[w].y; v[6] += hi[w].z; v[7] += hi[w].w;
+          }
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = j + i < rank ? v[i] * scale : 0.f;
@@ -186,7 +197,7 @@ int launch_first(bf16* t, int* done, int n_done, const CUtensorMap& map_x, const
   while (ways < 8 && 2 * ways * blocks <= FIRST_BLOCKS && K >= 64 * 2 * ways) ways *= 2;
   // Products read 128 rows, so that the last stage has them behind it.
   const int stage = (first_rows(tiles) + first_ranks(bank)) * 128, behind = (128 - first_rows(tiles)) * 128;
-  const int stages = min(FIRST_STAGES, ((tiles.tile_rows > 128 ? FIRST_SMALL_BYTES : FIRST_BYTES) - behind) / stage);
+  const int stages = min(FIRST_STAGES, (FIRST_BYTES - behind) / stage);
   const int bytes = 1024 + max(stages * stage + behind, 128 * FIRST_PITCH * 4);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(slots * ways, parts, chunks);

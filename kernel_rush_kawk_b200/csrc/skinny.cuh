@@ -280,7 +280,8 @@ int launch_warps(void* out, const void* x, const void* W, int M, int N, int K, f
   if (smem > 220 * 1024) return -2;
   auto kern = skinny_kernel<WARPS, NT, RT, SWIGLU, TOut, KSPLIT, RING, Extra>;
   if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static unsigned long long allowed = 0;
+    cudaError_t e = allow_shared(kern, smem, &allowed);
     if (e != cudaSuccess) return (int)e;
   }
   const int blocks = (N + 16 * RT - 1) / (16 * RT);

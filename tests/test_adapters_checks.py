@@ -5,7 +5,7 @@ import torch
 
 from adapter_helpers import gated64, make_adapters, make_bank, maps_by_hand, product64
 from kernel_rush_kawk_b200.csrc import adapter_ops, cache_ops
-from kernel_rush_kawk_b200.csrc.adapter_ops import AdapterOps, AdapterRows, StepMaps
+from kernel_rush_kawk_b200.csrc.adapter_ops import AdapterOps, StepMaps
 from kernel_rush_kawk_b200.csrc.cache_ops import CacheOps, KernelError
 from kernel_rush_kawk_b200.parts.adapters import AdapterBank, AdapterError
 
@@ -63,7 +63,7 @@ def product(x=None, w=None, bank=None, rows=None, gated=0):
     x = torch.randn(3, 16) if x is None else x
     w = torch.randn(12, 16) if w is None else w
     bank = AdapterBank(16, (8, 4), 2, 4, torch.float32, "cpu") if bank is None else bank
-    rows = AdapterRows(3, 3, "cpu") if rows is None else rows
+    rows = StepMaps(3, 3, "cpu").adapters if rows is None else rows
     if gated:
         return Checks().adapted_gate_up_swiglu(x, w, gated, bank, rows)
     return Checks()._check_adapted("adapted product", x, w, bank, rows)
@@ -75,7 +75,7 @@ def test_a_product_that_fits_is_taken():
 
 @pytest.mark.parametrize("change", [
     dict(x=torch.randn(3, 15)), dict(w=torch.randn(12, 15)), dict(w=torch.randn(11, 16)), dict(x=torch.randn(3, 16).bfloat16()),
-    dict(x=torch.randn(3, 16).bfloat16(), w=torch.randn(12, 16).bfloat16()), dict(x=torch.randn(4, 16)), dict(rows=AdapterRows(2, 2, "cpu")),
+    dict(x=torch.randn(3, 16).bfloat16(), w=torch.randn(12, 16).bfloat16()), dict(x=torch.randn(4, 16)), dict(rows=StepMaps(2, 2, "cpu").adapters),
     dict(x=torch.randn(16, 3).t()), dict(w=torch.randn(16, 12).t()), dict(x=torch.randn(1, 16).expand(3, 16)), dict(x=elsewhere(torch.randn(3, 16))),
     dict(w=elsewhere(torch.randn(12, 16))), dict(bank=AdapterBank(16, (8, 5), 2, 4, torch.float32, "cpu")),
     dict(bank=AdapterBank(15, (8, 4), 2, 4, torch.float32, "cpu")), dict(gated=8), dict(gated=6)])
@@ -106,15 +106,21 @@ def test_too_many_sequences():
 
 
 def test_lists_have_room_for_every_tile():
-    for n_rows, n_seqs in ((1, 1), (256, 256), (257, 3), (5000, 40)):
-        rows = AdapterRows(n_rows, n_seqs, "cpu")
-        at = rows.buffer.data_ptr() + 4 * (n_rows + n_rows % 2)
-        for h, info, slots, n_slots in zip(rows.heights, rows.info, rows.slots, rows.n_slots):
-            tiles = -(-n_rows // h)
-            assert info == at and slots == at + 8 * tiles and n_slots == tiles + n_seqs and info % 8 == 0
-            at = slots + 8 * n_slots
-        assert at == rows.buffer.data_ptr() + 4 * rows.buffer.numel()
-        assert n_rows > 256 or rows.heights[0] >= n_rows
+    for places in (False, True):
+        for n_rows, n_seqs in ((0, 3), (1, 1), (255, 8), (256, 256), (257, 3), (5000, 40), (777, 0)):
+            maps = StepMaps(n_rows, n_seqs, "cpu", with_places=places)
+            rows = maps.adapters
+            end = maps.address + 4 * maps.buffer.numel()
+            assert rows.row_adapter_at % 8 == 0 and rows.row_adapter_at >= maps.address + 4 * (2 * n_rows * places + n_seqs + 1 + 2 * n_rows)
+            at = rows.row_adapter_at + 4 * (n_rows + n_rows % 2)
+            for i, h in enumerate(rows.heights):
+                height, info, slots, n_slots = rows.tiles(i)
+                tiles = -(-n_rows // h)
+                assert height == h and info == at and slots == at + 8 * tiles and n_slots == tiles + n_seqs and info % 8 == 0
+                at = slots + 8 * n_slots
+            assert at == end == rows.row_adapter_at + 4 * rows.words()
+            assert n_rows > 256 or rows.heights[0] >= n_rows
+            assert (maps.row_place is None) != places and maps.row_pos.shape == (n_rows,) and maps.cu_q.shape == (n_seqs + 1,)
 
 
 def test_the_definition_itself():

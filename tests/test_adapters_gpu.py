@@ -232,7 +232,8 @@ def check_lists(rows, per_sequence, lengths):
     words = rows.buffer.cpu().tolist()
     of = per_row(lengths, per_sequence)
     base = rows.buffer.data_ptr()
-    for height, info, slots, n_slots in zip(rows.heights, rows.info, rows.slots, rows.n_slots):
+    for which in range(len(rows.heights)):
+        height, info, slots, n_slots = rows.tiles(which)
         at = (slots - base) // 4
         pairs = list(zip(words[at:at + 2 * n_slots:2], words[at + 1:at + 2 * n_slots:2]))
         used, last = set(), 0
