@@ -38,8 +38,8 @@ constexpr uint32_t W_BYTES = 128 * BK * 2;  // a block's half of the pair's weig
 constexpr int PATCH_PITCH = 36;             // words of two rows in a warp's patch for the transpose
 constexpr int PATCH_BYTES = 16 * PATCH_PITCH * 4;
 constexpr int MOST_STAGES = 7;
-constexpr int RING_BYTES = 128 * 1024;  // an SM has room for a block of the first factor's beside it
-constexpr size_t SMEM_BYTES = 1024 + RING_BYTES + READERS * PATCH_BYTES + (2 * MOST_STAGES + 8) * 8 + (MOST_STAGES + 6) * 4;
+constexpr int RING_BYTES = 128 * 1024, DEEP_RING_BYTES = 192 * 1024;  // beside the smaller an SM has room for a block of the first factor's
+constexpr size_t BESIDE_BYTES = 1024 + READERS * PATCH_BYTES + (2 * MOST_STAGES + 8) * 8 + (MOST_STAGES + 6) * 4;
 
 struct Maps {
   CUtensorMap x, w, t, b[KRK_MAX_PARTS];
@@ -52,6 +52,23 @@ __device__ __forceinline__ void umma_bf16_pair_warp(uint32_t tmem_d, uint64_t a_
       "setp.ne.b32 p, %4, 0;\n"
       "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}"
       ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// A stage's four products and its release at once.
+__device__ __forceinline__ void umma_stage_pair_warp(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate, uint64_t* release) {
+  asm volatile(
+      "{\n.reg .pred p, q, t;\n.reg .b64 a1, a2, a3, b1, b2, b3;\n"
+      "elect.sync _|q, 0xffffffff;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "setp.eq.b32 t, 0, 0;\n"
+      "add.u64 a1, %1, 2;\nadd.u64 a2, %1, 4;\nadd.u64 a3, %1, 6;\n"
+      "add.u64 b1, %2, 2;\nadd.u64 b2, %2, 4;\nadd.u64 b3, %2, 6;\n"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], a1, b1, %3, t;\n"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], a2, b2, %3, t;\n"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], a3, b3, %3, t;\n"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%5], %6;\n}"
+      ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(smem_u32(release)), "h"((uint16_t)3)
       : "memory");
 }
 __device__ __forceinline__ void umma_commit_pair_warp(uint64_t* bar) {
@@ -129,12 +146,12 @@ struct Walk {
 
 template <bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(512)  // (of 320: 128 registers a thread leave room for a block of the first factor's)
-adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, float* __restrict__ shares, int* __restrict__ done, int shared, int most_shares, int aligned, int N, int K, const __grid_constant__ AdapterBank bank,
+adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, float* __restrict__ shares, int* __restrict__ done, int shared, int most_shares, int aligned, int ring_bytes, int N, int K, const __grid_constant__ AdapterBank bank,
                     const __grid_constant__ AdapterTiles tiles, int* __restrict__ error) {
   constexpr int BC = GATED ? 64 : 128;  // columns of C a block makes of a tile; the pair twice as many
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  unsigned char* patches = ring + RING_BYTES;
+  unsigned char* patches = ring + ring_bytes;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(patches + READERS * PATCH_BYTES);  // the first block's: copies of both have landed
   uint64_t* empty_bar = full_bar + MOST_STAGES;   // either block's: the products have read a stage
   uint64_t* acc_full = empty_bar + MOST_STAGES;   // either block's
@@ -188,7 +205,7 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
   uint32_t tmem[2] = {warp >= 1 ? tmem_slot[0] : 0, 0};
   const int half = tiles.tile_rows / 2;  // rows that each block of the pair brings
   const uint32_t stage_bytes = W_BYTES + (uint32_t)half * BK * 2;
-  const int stages = min(MOST_STAGES, (int)(RING_BYTES / stage_bytes));
+  const int stages = min(MOST_STAGES, (int)(ring_bytes / stage_bytes));
   const int k_blocks = (K + BK - 1) / BK, row_tiles = (tiles.rows + tiles.tile_rows - 1) / tiles.tile_rows;
   const int all_tiles = row_tiles * ((N + 2 * BC - 1) / (2 * BC));
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -318,20 +335,15 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
         unsigned char* stage = ring + s * stage_bytes;
         const uint64_t w_desc = umma_desc(stage), r_desc = umma_desc(stage + W_BYTES);
         if ((what & 255) == 4) {
-#pragma unroll
-          for (int k = 0; k < BK / UMMA_K; ++k) {
-            const uint64_t adv = (uint64_t)((k * UMMA_K * 2) >> 4);
-            umma_bf16_pair_warp(acc, w_desc + adv, r_desc + adv, idesc, more);
-            more = 1;
-          }
+          umma_stage_pair_warp(acc, w_desc, r_desc, idesc, more, empty_bar + s);
         } else {
           for (int k = 0; k < (what & 255); ++k) {
             const uint64_t adv = (uint64_t)((k * UMMA_K * 2) >> 4);
-            umma_bf16_pair_warp(acc, w_desc + adv, r_desc + adv, idesc, more);
-            more = 1;
+            umma_bf16_pair_warp(acc, w_desc + adv, r_desc + adv, idesc, more || k > 0);
           }
+          umma_commit_pair_warp(empty_bar + s);
         }
-        umma_commit_pair_warp(empty_bar + s);
+        more = 1;
         if (++s == stages) { s = 0; parity ^= 1; }
       }
       if (ok) {
@@ -351,7 +363,7 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
     int buf = 0;
     uint32_t parity = 0;
     while (walk.next(t, k0, k1, e0, e1)) {
-      if (!__all_sync(0xffffffffu, mbar_wait(acc_full + buf, parity))) {
+      if (!__all_sync(0xffffffffu, mbar_wait_long(acc_full + buf, parity))) {
         if (lane == 0) atomicExch(error, 5);
         break;
       }
@@ -531,9 +543,11 @@ int launch_gemm(const Maps& maps, bf16* out, float* shares, int* done, int share
                 int pairs, int* error, cudaStream_t stream) {
   static unsigned long long allowed = 0;
   auto kern = adapted_gemm_kernel<GATED>;
-  const cudaError_t e = allow_shared(kern, SMEM_BYTES, &allowed);
+  const cudaError_t e = allow_shared(kern, BESIDE_BYTES + DEEP_RING_BYTES, &allowed);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(kern, dim3(2 * pairs), dim3(THREADS), SMEM_BYTES, stream, maps, out, shares, done, shared, most_shares, aligned, N, K, bank,
+  // tiles of many rows want stages ahead: a block of k of 256 rows takes 650 clocks with four, 590 with five, 575 with six, its products alone 512
+  const int ring = tiles.tile_rows <= 128 ? RING_BYTES : DEEP_RING_BYTES;
+  return (int)launch_pdl(kern, dim3(2 * pairs), dim3(THREADS), BESIDE_BYTES + ring, stream, maps, out, shares, done, shared, most_shares, aligned, ring, N, K, bank,
                          tiles, error);
 }
 

@@ -9,31 +9,30 @@ namespace {
 using namespace tc;
 
 // The first factor of many requests' adapters, t = scale (x A^T), sums in 32 bits on the tensor cores. rounded to bfloat16. Two forms of t: of every slot,
-// [slot][tile_rows][parts * wide], zeros where a row has another adapter than the slot's (COMPACT false); of every row, [rows][parts * wide], where it has an adapter. A cluster has 128 rows of a slot's tile (y), 128 of the
-// adapter's ranks, all parts' side by side (z), and its `ways` blocks share k. A block multiplies its part of k on the tensor cores (128 rows by 128
-// ranks, fed by TMA in blocks of 64 k); the blocks' sums meet in 32 bits through distributed shared memory, each block adding and writing its share of
-// the rows, in the blocks' order.
+// [slot][tile_rows][parts * wide], zeros where a row has another adapter than the slot's (COMPACT false); of every row, [rows][parts * wide], where it has an adapter. A cluster has 128 rows of a slot's tile (y), 64 or 128 of the
+// adapter's ranks, all parts' side by side (z), and its `ways` blocks share k. A block multiplies its part of k on the tensor cores (fed by TMA in blocks of 64 k); each block sends its sums of every block's share of the rows to that block's shared
+// memory, in 32 bits, which adds them in the blocks' order and writes its rows.
 //
 // The product's blocks come in while these run, once what came before is over, and wait for t where they need it; so a ring of few blocks of k is no
 // larger than fits beside theirs.
-constexpr int FIRST_RANKS = 128, FIRST_STAGES = 8, FIRST_THREADS = 192, FIRST_PITCH = FIRST_RANKS + 4;
-constexpr int FIRST_BYTES = 72 * 1024;  // of the ring, beside the product's
-constexpr int FIRST_BLOCKS = 148;  // as many as are worth sharing k among
-static_assert(128 * FIRST_PITCH * 4 <= FIRST_BYTES, "the sums take the ring's place");
+constexpr int FIRST_RANKS = 128, FIRST_STAGES = 8, FIRST_THREADS = 192;
+constexpr int FIRST_BYTES = 73 * 1024, FIRST_DEEP_BYTES = 160 * 1024;  // of shared memory, beside the product's blocks and alone
 
 template <bool COMPACT>
 __global__ void __launch_bounds__(FIRST_THREADS, 5)  // (of three that an SM's memory takes: in 64 registers they fit beside the product's)
 first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_done, const __grid_constant__ CUtensorMap map_x,
                                                                            const __grid_constant__ CUtensorMap map_a, int K,
                                                                            const __grid_constant__ AdapterBank bank, const __grid_constant__ AdapterTiles tiles,
-                                                                           int ways, int stages, int box_rows, int box_ranks, int* __restrict__ error) {
+                                                                           int ways, int stages, int ring_bytes, int box_rows, int box_ranks, int* __restrict__ error) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  float* sums = reinterpret_cast<float*>(ring);  // [128][FIRST_PITCH], when the ring has done its work
+  float* inbox = reinterpret_cast<float*>(ring + ring_bytes);  // [ways][this block's rows][pitch]
+  const int pitch = box_ranks + 4;
   __shared__ uint64_t full_bar[FIRST_STAGES], empty_bar[FIRST_STAGES], acc_bar;
   __shared__ uint32_t tmem_slot;
   __shared__ int asked_for;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = blockIdx.x % ways, slot = blockIdx.x / ways;
+  if (ways > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // "I have started"
   grid_dependency_wait();
   // Tensor memory is taken before the product's blocks are let in, which take what is left and wait for what these make. They are let in here, since
   // they read what earlier kernels wrote before they wait.
@@ -46,6 +45,7 @@ first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_do
   tc_fence_after();
   grid_launch_dependents();
   const uint32_t acc = tmem_slot;
+  if (ways > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every block of the cluster has started
   auto leave = [&] {
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(acc), "r"(FIRST_RANKS) : "memory");
   };
@@ -56,10 +56,12 @@ first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_do
   if (a < 0 || a >= bank.capacity) return leave();  // the whole cluster (the product says so)
   const int here = min(128, min(tiles.tile_rows - (int)blockIdx.y * 128, tiles.rows - r0));  // rows
   if (here <= 0) return leave();
+  namespace cg = cooperative_groups;
+  const int share = (here + ways - 1) / ways;  // of the rows
   bool has = false;
   for (int r = threadIdx.x; r < here; r += FIRST_THREADS) has |= tiles.row_adapter[r0 + r] == a;
   const int k_blocks = (K + 63) / 64, each = (k_blocks + ways - 1) / ways, b0 = min(way * each, k_blocks), b1 = min(b0 + each, k_blocks);
-  const int n0 = blockIdx.z * FIRST_RANKS, per_adapter = bank.parts * bank.rank;
+  const int n0 = blockIdx.z * box_ranks, per_adapter = bank.parts * bank.rank;
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(full_bar + s, 1);
@@ -83,9 +85,7 @@ first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_do
           break;
         }
         const uint32_t stage = smem_u32(ring) + s * bytes, bar = smem_u32(full_bar + s);
-        mbar_expect_tx_warp(bar, bytes);
-        tma_load_2d_warp(stage, &map_x, bar, b * 64, r0);
-        tma_load_2d_warp(stage + box_rows * 128, &map_a, bar, b * 64, a * per_adapter + n0);
+        two_loads_warp(stage, &map_x, b * 64, r0, stage + box_rows * 128, &map_a, b * 64, a * per_adapter + n0, bar, bytes);
       }
     } else if (warp == 1) {
       const uint32_t idesc = umma_idesc(128, box_ranks);  // (rows beyond the copies' give rows that nobody reads)
@@ -104,12 +104,9 @@ first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_do
       umma_commit_warp(&acc_bar);  // arrives even after a failed wait, so that all move on
     }
     if (!__all_sync(0xffffffffu, mbar_wait(&acc_bar, 0)) && lane == 0) atomicExch(error, 5);
-    __syncthreads();  // the ring has been read by the products that the barrier stands for
-    if (threadIdx.x == 0 && asked_for >= 0)  // copies on their way end before the ring is written
-      for (int i = max(0, asked_for - stages); i < asked_for; ++i) mbar_wait(full_bar + i % stages, (uint32_t)(i / stages) & 1u, WAIT_LIMIT_NS / 20);
-    __syncthreads();
     if (warp >= 2 && (warp & 3) * 32 < here) {
       const int row = (warp & 3) * 32 + lane;
+      float* to = (ways > 1 ? cg::this_cluster().map_shared_rank(inbox, row < here ? row / share : 0) : inbox) + (way * share + row % share) * pitch;
       tc_fence_after();
 #pragma unroll
       for (int c = 0; c < FIRST_RANKS; c += 32) {
@@ -117,46 +114,39 @@ first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_do
         uint32_t v[32];
         tmem_ld_32x32(acc + ((uint32_t)((warp & 3) * 32) << 16) + c, v);
         tmem_wait_ld();
+        if (row < here)
 #pragma unroll
-        for (int j = 0; j < 32; j += 4)
-          *reinterpret_cast<float4*>(sums + row * FIRST_PITCH + c + j) =
-              b1 > b0 ? make_float4(__uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])) : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int j = 0; j < 32; j += 4)
+            if (c + j < box_ranks)
+              *reinterpret_cast<float4*>(to + c + j) =
+                  b1 > b0 ? make_float4(__uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
       tc_fence_before();
     }
     __syncthreads();
     tc_fence_after();
+    if (threadIdx.x == 0 && asked_for >= 0)  // copies on their way end before shared memory is given up
+      for (int i = max(0, asked_for - stages); i < asked_for; ++i) mbar_wait(full_bar + i % stages, (uint32_t)(i / stages) & 1u, WAIT_LIMIT_NS / 20);
   }
-  leave();  // (nobody who holds tensor memory waits for another block)
+  leave();  // (nobody who holds tensor memory waits for another block's end)
   if (has && ways > 1) cluster_sync();
   if (COMPACT && !has) return;
   // eight ranks of a row a thread
-  namespace cg = cooperative_groups;
-  const int share = (here + ways - 1) / ways, first_row = way * share, rows = min(share, here - first_row);
+  const int first_row = way * share, rows = min(share, here - first_row), groups = box_ranks / 8;
   const int width = bank.parts * bank.wide;
-  for (int o = threadIdx.x; o < rows * (FIRST_RANKS / 8); o += FIRST_THREADS) {
-    const int row = first_row + o / (FIRST_RANKS / 8), c = o % (FIRST_RANKS / 8) * 8, part = (n0 + c) / bank.rank, j = (n0 + c) % bank.rank;
+  for (int o = threadIdx.x; o < rows * groups; o += FIRST_THREADS) {
+    const int mine = o / groups, row = first_row + mine, c = o % groups * 8, part = (n0 + c) / bank.rank, j = (n0 + c) % bank.rank;
     if (part >= bank.parts) continue;
     uint4 pack = make_uint4(0, 0, 0, 0);
     if (tiles.row_adapter[r0 + row] == a) {
       const int rank = bank.ranks[a * bank.parts + part];
       const float scale = bank.scale[a * bank.parts + part];
       float v[8] = {};
-      for (int w0 = 0; w0 < ways; w0 += 4) {  // four blocks' on their way at once
-        float4 lo[4], hi[4];
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          if (w0 + w < ways) {
-            const float* from = (ways > 1 ? cg::this_cluster().map_shared_rank(sums, w0 + w) : sums) + row * FIRST_PITCH + c;
-            lo[w] = *reinterpret_cast<const float4*>(from);
-            hi[w] = *reinterpret_cast<const float4*>(from + 4);
-          }
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          if (w0 + w < ways) {
-            v[0] += lo[w].x; v[1] += lo[w].y; v[2] += lo[w].z; v[3] += lo[w].w;
-            v[4] += hi[w].x; v[5] += hi[w].y; v[6] += hi[w].z; v[7] += hi[w].w;
-          }
+      for (int w = 0; w < ways; ++w) {
+        const float* from = inbox + (w * share + mine) * pitch + c;
+        const float4 lo = *reinterpret_cast<const float4*>(from), hi = *reinterpret_cast<const float4*>(from + 4);
+        v[0] += lo.x; v[1] += lo.y; v[2] += lo.z; v[3] += lo.w;
+        v[4] += hi.x; v[5] += hi.y; v[6] += hi.z; v[7] += hi.w;
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = j + i < rank ? v[i] * scale : 0.f;
@@ -167,12 +157,11 @@ first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_do
     *reinterpret_cast<uint4*>(to) = pack;
     if (j + 8 == bank.rank && bank.wide > bank.rank) *reinterpret_cast<uint4*>(to + 8) = make_uint4(0, 0, 0, 0);  // the product takes whole steps of sixteen
   }
-  if (has && ways > 1) cluster_sync();  // no block leaves while another reads its sums
 }
 
-// rows and ranks of a copy of the first factor's: as many as there are
+// rows and ranks of a copy of the first factor's: as many as there are (64 of the ranks where the rows are many: the sums of both have their place in shared memory)
 int first_rows(const AdapterTiles& tiles) { return min(128, (min(tiles.rows, tiles.tile_rows) + 7) / 8 * 8); }
-int first_ranks(const AdapterBank& bank) { return min(FIRST_RANKS, (bank.parts * bank.rank + 15) / 16 * 16); }
+int first_ranks(const AdapterBank& bank, const AdapterTiles& tiles) { return min(first_rows(tiles) > 64 ? 64 : FIRST_RANKS, (bank.parts * bank.rank + 15) / 16 * 16); }
 
 template <bool COMPACT>
 int launch_first(bf16* t, int* done, int n_done, const CUtensorMap& map_x, const CUtensorMap& map_a, int K, const AdapterBank& bank, const AdapterTiles& tiles, int* error,
@@ -186,19 +175,24 @@ int launch_first(bf16* t, int* done, int n_done, const CUtensorMap& map_x, const
     e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e == cudaSuccess) __atomic_fetch_or(&told, 1ull << (device & 63), __ATOMIC_RELAXED);
   }
-  if (e == cudaSuccess) e = allow_shared(kern, 1024 + FIRST_BYTES, &allowed);
+  if (e == cudaSuccess) e = allow_shared(kern, FIRST_DEEP_BYTES, &allowed);
   if (e != cudaSuccess) return (int)e;
   const int row_tiles = (tiles.rows + tiles.tile_rows - 1) / tiles.tile_rows, ranks = bank.parts * bank.rank;
-  const int parts = (min(tiles.tile_rows, tiles.rows) + 127) / 128, chunks = (ranks + FIRST_RANKS - 1) / FIRST_RANKS;
-  // a single tile's adapters are in the first slots
+  const int box_rows = first_rows(tiles), box_ranks = first_ranks(bank, tiles);
+  const int parts = (min(tiles.tile_rows, tiles.rows) + 127) / 128, chunks = (ranks + box_ranks - 1) / box_ranks;
+  // Blocks that share k: of a single tile, whose adapters are in the first slots, as many as half of the SMs have one of; of many tiles, of whose slots some third
+  // is not used, six at most (clusters of eight leave an eighth of the SMs without one).
   const int slots = row_tiles == 1 ? min(tiles.n_slots, bank.capacity) : tiles.n_slots;
   const long long blocks = (long long)slots * parts * chunks;
-  int ways = 1;
-  while (ways < 8 && 2 * ways * blocks <= FIRST_BLOCKS && K >= 64 * 2 * ways) ways *= 2;
-  // Products read 128 rows, so that the last stage has them behind it.
-  const int stage = (first_rows(tiles) + first_ranks(bank)) * 128, behind = (128 - first_rows(tiles)) * 128;
-  const int stages = min(FIRST_STAGES, (FIRST_BYTES - behind) / stage);
-  const int bytes = 1024 + max(stages * stage + behind, 128 * FIRST_PITCH * 4);
+  const int most = row_tiles == 1 ? 8 : 6;
+  int ways = (int)max(1ll, min((long long)most, (row_tiles == 1 ? 74 : 180) / blocks));
+  ways = max(1, min(ways, K / 128));
+  // Beside the product's blocks where these take tiles of few rows and wait for W's bytes; before them, on all of an SM's memory, where they would be slowed
+  // down. Products read 128 rows, so that the last stage has them behind it.
+  const int stage = (box_rows + box_ranks) * 128, behind = max(0, 128 - box_rows - box_ranks) * 128;
+  const int inbox = ways * ((box_rows + ways - 1) / ways) * (box_ranks + 4) * 4, room = (tiles.tile_rows > 128 ? FIRST_DEEP_BYTES : FIRST_BYTES) - 1024 - inbox;
+  const int stages = max(1, min(FIRST_STAGES, (room - behind) / stage)), ring = (stages * stage + behind + 1023) / 1024 * 1024;
+  const int bytes = 1024 + ring + inbox;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(slots * ways, parts, chunks);
   cfg.blockDim = dim3(FIRST_THREADS);
@@ -214,7 +208,7 @@ int launch_first(bf16* t, int* done, int n_done, const CUtensorMap& map_x, const
   static const bool plain = getenv("KRK_NO_PDL") != nullptr;
   cfg.attrs = attr;
   cfg.numAttrs = plain ? 1 : 2;
-  return (int)cudaLaunchKernelEx(&cfg, kern, t, done, n_done, map_x, map_a, K, bank, tiles, ways, stages, first_rows(tiles), first_ranks(bank), error);
+  return (int)cudaLaunchKernelEx(&cfg, kern, t, done, n_done, map_x, map_a, K, bank, tiles, ways, stages, ring, box_rows, box_ranks, error);
 }
 
 }  // namespace
@@ -225,7 +219,7 @@ int krk_first_factor(void* t, bool compact, int* done, int n_done, const void* x
   if (rows > 0x7fffffffLL || (long long)tiles.n_slots * 8 > 0x7fffffffLL) return -3;
   CUtensorMap map_x, map_a;
   int rc = make_map_bf16(&map_x, x, tiles.rows, K, ldx, first_rows(tiles));
-  if (!rc) rc = make_map_bf16(&map_a, bank.a, rows, K, K, first_ranks(bank));
+  if (!rc) rc = make_map_bf16(&map_a, bank.a, rows, K, K, first_ranks(bank, tiles));
   if (rc) return rc;
   return compact ? launch_first<true>((bf16*)t, done, n_done, map_x, map_a, K, bank, tiles, error, stream)
                  : launch_first<false>((bf16*)t, done, n_done, map_x, map_a, K, bank, tiles, error, stream);
