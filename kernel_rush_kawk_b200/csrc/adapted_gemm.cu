@@ -38,7 +38,7 @@ constexpr uint32_t W_BYTES = 128 * BK * 2;  // a block's half of the pair's weig
 constexpr int PATCH_PITCH = 36;             // words of two rows in a warp's patch for the transpose
 constexpr int PATCH_BYTES = 16 * PATCH_PITCH * 4;
 constexpr int MOST_STAGES = 7;
-constexpr int RING_BYTES = 128 * 1024, DEEP_RING_BYTES = 192 * 1024;  // beside the smaller an SM has room for a block of the first factor's
+constexpr int RING_BYTES = 104 * 1024, DEEP_RING_BYTES = 192 * 1024;  // beside the smaller an SM has room for a block of the first factor's
 constexpr size_t BESIDE_BYTES = 1024 + READERS * PATCH_BYTES + (2 * MOST_STAGES + 8) * 8 + (MOST_STAGES + 6) * 4;
 
 struct Maps {

@@ -16,7 +16,7 @@ using namespace tc;
 // The product's blocks come in while these run, once what came before is over, and wait for t where they need it; so a ring of few blocks of k is no
 // larger than fits beside theirs.
 constexpr int FIRST_RANKS = 128, FIRST_STAGES = 8, FIRST_THREADS = 192;
-constexpr int FIRST_BYTES = 73 * 1024, FIRST_DEEP_BYTES = 160 * 1024;  // of shared memory, beside the product's blocks and alone
+constexpr int FIRST_BYTES = 96 * 1024, FIRST_DEEP_BYTES = 160 * 1024;  // of shared memory, beside the product's blocks and alone
 
 template <bool COMPACT>
 __global__ void __launch_bounds__(FIRST_THREADS, 5)  // (of three that an SM's memory takes: in 64 registers they fit beside the product's)
@@ -26,7 +26,8 @@ first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_do
                                                                            int ways, int stages, int ring_bytes, int box_rows, int box_ranks, int* __restrict__ error) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  float* inbox = reinterpret_cast<float*>(ring + ring_bytes);  // [ways][this block's rows][pitch]
+  // [ways][this block's rows][pitch]; of a block by itself, in the ring's place when that has done its work
+  float* inbox = reinterpret_cast<float*>(ways > 1 ? ring + ring_bytes : ring);
   const int pitch = box_ranks + 4;
   __shared__ uint64_t full_bar[FIRST_STAGES], empty_bar[FIRST_STAGES], acc_bar;
   __shared__ uint32_t tmem_slot;
@@ -104,6 +105,10 @@ first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_do
       umma_commit_warp(&acc_bar);  // arrives even after a failed wait, so that all move on
     }
     if (!__all_sync(0xffffffffu, mbar_wait(&acc_bar, 0)) && lane == 0) atomicExch(error, 5);
+    __syncthreads();
+    if (threadIdx.x == 0 && asked_for >= 0)  // copies on their way end before their place is given up
+      for (int i = max(0, asked_for - stages); i < asked_for; ++i) mbar_wait(full_bar + i % stages, (uint32_t)(i / stages) & 1u, WAIT_LIMIT_NS / 20);
+    __syncthreads();
     if (warp >= 2 && (warp & 3) * 32 < here) {
       const int row = (warp & 3) * 32 + lane;
       float* to = (ways > 1 ? cg::this_cluster().map_shared_rank(inbox, row < here ? row / share : 0) : inbox) + (way * share + row % share) * pitch;
@@ -125,8 +130,6 @@ first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_do
     }
     __syncthreads();
     tc_fence_after();
-    if (threadIdx.x == 0 && asked_for >= 0)  // copies on their way end before shared memory is given up
-      for (int i = max(0, asked_for - stages); i < asked_for; ++i) mbar_wait(full_bar + i % stages, (uint32_t)(i / stages) & 1u, WAIT_LIMIT_NS / 20);
   }
   leave();  // (nobody who holds tensor memory waits for another block's end)
   if (has && ways > 1) cluster_sync();
@@ -180,18 +183,19 @@ int launch_first(bf16* t, int* done, int n_done, const CUtensorMap& map_x, const
   const int row_tiles = (tiles.rows + tiles.tile_rows - 1) / tiles.tile_rows, ranks = bank.parts * bank.rank;
   const int box_rows = first_rows(tiles), box_ranks = first_ranks(bank, tiles);
   const int parts = (min(tiles.tile_rows, tiles.rows) + 127) / 128, chunks = (ranks + box_ranks - 1) / box_ranks;
-  // Blocks that share k: of a single tile, whose adapters are in the first slots, as many as half of the SMs have one of; of many tiles, of whose slots some third
+  // Blocks that share k: of a single tile, whose adapters are in the first slots, as the SMs take one of; of many tiles, of whose slots some third
   // is not used, six at most (clusters of eight leave an eighth of the SMs without one).
   const int slots = row_tiles == 1 ? min(tiles.n_slots, bank.capacity) : tiles.n_slots;
   const long long blocks = (long long)slots * parts * chunks;
   const int most = row_tiles == 1 ? 8 : 6;
-  int ways = (int)max(1ll, min((long long)most, (row_tiles == 1 ? 74 : 180) / blocks));
+  int ways = (int)max(1ll, min((long long)most, (row_tiles == 1 ? 148 : 180) / blocks));
   ways = max(1, min(ways, K / 128));
   // Beside the product's blocks where these take tiles of few rows and wait for W's bytes; before them, on all of an SM's memory, where they would be slowed
   // down. Products read 128 rows, so that the last stage has them behind it.
   const int stage = (box_rows + box_ranks) * 128, behind = max(0, 128 - box_rows - box_ranks) * 128;
-  const int inbox = ways * ((box_rows + ways - 1) / ways) * (box_ranks + 4) * 4, room = (tiles.tile_rows > 128 ? FIRST_DEEP_BYTES : FIRST_BYTES) - 1024 - inbox;
-  const int stages = max(1, min(FIRST_STAGES, (room - behind) / stage)), ring = (stages * stage + behind + 1023) / 1024 * 1024;
+  const int sums = ways * ((box_rows + ways - 1) / ways) * (box_ranks + 4) * 4, inbox = ways > 1 ? sums : 0;
+  const int room = (tiles.tile_rows > 128 ? FIRST_DEEP_BYTES : FIRST_BYTES) - 1024 - inbox;
+  const int stages = max(1, min(FIRST_STAGES, (room - behind) / stage)), ring = (max(stages * stage + behind, sums - inbox) + 1023) / 1024 * 1024;
   const int bytes = 1024 + ring + inbox;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(slots * ways, parts, chunks);

@@ -72,7 +72,8 @@ class AdapterBank:
             raise AdapterError(f"an adapter of rank {r} in a bank of rank {self.rank}")
         self.a[index, part * self.rank:part * self.rank + r].copy_(a)
         self.b[index, self.begin[part]:self.begin[part] + n, :r].copy_(b)
-        self.b[index, self.begin[part]:self.begin[part] + n, r:].zero_()  # the kernels take whole steps of sixteen
+        if r < self.rank:
+            self.b[index, self.begin[part]:self.begin[part] + n, r:].zero_()  # the kernels take whole steps of sixteen
         self.scale[index, part] = float(scale)
         self.ranks[index, part] = r
 
