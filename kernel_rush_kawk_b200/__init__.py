@@ -15,10 +15,11 @@ replay. All arithmetic of the model runs in this package's own CUDA kernels.
 from .config import ConfigError, DisoraxConfig, FogizenConfig, GivizenConfig, Qwen3Config, TaredraConfig, ZadunexConfig, ZefapelConfig, read_config, register_architecture
 from .cache import KeyEviction
 from .engine import Engine, StepEntry
+from .parts.adapters import AdapterError, AdapterRoom
 from .sampling import SamplingParams
 from .weights import WeightError, write_model_folder
 
 __version__ = "0.1.0"
 __all__ = ["ConfigError", "DisoraxConfig", "FogizenConfig", "GivizenConfig", "Qwen3Config", "TaredraConfig", "ZadunexConfig", "ZefapelConfig", "read_config",
-           "register_architecture", "Engine", "KeyEviction", "StepEntry",
+           "register_architecture", "AdapterError", "AdapterRoom", "Engine", "KeyEviction", "StepEntry",
            "SamplingParams", "WeightError", "write_model_folder"]

@@ -137,6 +137,7 @@ class SequenceCache:
         self.width = max(1, -(-rows // PAGE))
         self.slots = FreeList(self.max_slots, "cache slot")
         self.length = [0] * self.max_slots  # rows held
+        self.adapter = [-1] * self.max_slots  # the low-rank adapter that a slot's sequence runs with, -1 for none
         self.evicted = [0] * self.max_slots  # rows given up: the next row's position is length + evicted
         self._family: list = [None] * self.max_slots  # (number, shared positions) of slots that share pages with others
         self._families = 0
@@ -185,8 +186,9 @@ class SequenceCache:
                 self._where[run] = src
 
     # -- slots --------------------------------------------------------------
-    def alloc(self) -> int:
+    def alloc(self, adapter: int = -1) -> int:
         slot = self.slots.take()
+        self.adapter[slot] = adapter
         self.length[slot] = self.evicted[slot] = 0
         self._family[slot] = None
         for g in self._state_groups:
@@ -199,6 +201,7 @@ class SequenceCache:
             g.ledger.release(slot)
         self.length[slot] = self.evicted[slot] = 0
         self._family[slot] = None
+        self.adapter[slot] = -1
 
     def can_share(self) -> bool:
         """Whether sequences can share pages: no run keeps a window of keys, whose pages are written again, and no keys are evicted."""
@@ -216,7 +219,7 @@ class SequenceCache:
             raise CacheError(f"a fork shares whole pages of {PAGE} positions that its source holds; got {length} of {self.length[slot]}")
         if self._state_groups and length != self.length[slot]:
             raise CacheError(f"the state behind position {length} is gone: the sequence is at {self.length[slot]}")
-        new = self.alloc()
+        new = self.alloc(self.adapter[slot])
         for g in self._kv_groups:
             for logical, page in g.ledger.share(slot, new, length // PAGE):
                 g.table_host[new, logical] = page
@@ -288,6 +291,28 @@ class SequenceCache:
             for logical, page in g.ledger.grow(slot, length):
                 g.table_host[slot, logical] = page
                 g.dirty.add(slot)
+
+    def reserve_pass(self, slots, lengths) -> list | None:
+        """``reserve`` for the sequences of a pass, in their order. Returns the new pages, one sequence's after the other's, where a kernel may enter them in the
+        device's table from the sequences' lengths alone (``entered`` says that it did); else None, and ``sync`` brings the table up to date."""
+        by_lengths = len(self._kv_groups) == 1 and self._kv_groups[0].ledger.ring is None and not self._kv_groups[0].dirty
+        group = self._kv_groups[0] if by_lengths else None
+        pages: list = []
+        for slot, length in zip(slots, lengths):
+            before = len(group.ledger.pages[slot]) if by_lengths else 0
+            by_lengths = by_lengths and before == -(-self.length[slot] // PAGE)
+            self.reserve(slot, length)
+            if group is not None:
+                pages += group.ledger.pages[slot][before:]
+        return pages if by_lengths else None
+
+    def entered(self, slots) -> None:
+        """The device's table holds these slots' pages."""
+        self._kv_groups[0].dirty.difference_update(slots)
+
+    def page_table(self) -> torch.Tensor:
+        """The device's table of the only storage group that keeps keys."""
+        return self._kv_groups[0].table
 
     def advance(self, slot: int, n: int) -> None:
         self.length[slot] += n

@@ -51,6 +51,10 @@ def build_parser() -> argparse.ArgumentParser:
                    help="hold about N keys a sequence: those that received least attention are given up")
     g.add_argument("--keep-recent", type=int, default=None, metavar="N", help="of the keys kept, the newest N whatever they received (default: a quarter)")
 
+    g.add_argument("--adapter", action="append", default=[], metavar="NAME=DIR", help="load a low-rank adapter from a folder; repeatable")
+    g.add_argument("--use-adapter", action="append", default=None, metavar="NAME",
+                   help="the adapter that the prompts run with; once for all of them, or once for each in order ('-': none)")
+
     w = sub.add_parser("write-random", help="write a model folder with random weights")
     w.add_argument("--preset", required=True)
     w.add_argument("--seed", type=int, default=0)
@@ -89,7 +93,7 @@ def main(argv=None) -> int:
         folder = write_model_folder(args.out, preset_config(args.preset), args.seed, args.std)
         print(folder)
         return 0
-    from . import Engine, KeyEviction
+    from . import AdapterError, AdapterRoom, Engine, KeyEviction
     from .cache import CacheError
     prompts = list(args.prompt_ids)
     if args.prompt_file:
@@ -108,13 +112,33 @@ def main(argv=None) -> int:
             options["eviction"] = KeyEviction(keep=args.keep_keys, recent=recent)
         except CacheError as e:
             parser.error(str(e))
+    adapters = None
+    if args.use_adapter is not None and not args.adapter:
+        parser.error("--use-adapter goes with --adapter")
+    if args.adapter:
+        from .weights.adapters import read_adapter
+        try:
+            loaded = {name: read_adapter(folder) for name, eq, folder in (a.partition("=") for a in args.adapter)}
+            options["adapters"] = AdapterRoom(len(loaded), max(a.shape[0] for factors in loaded.values() for a, _, _ in factors.values()))
+        except (AdapterError, ValueError) as e:
+            parser.error(str(e))
+        adapters = [None if name == "-" else name for name in args.use_adapter or ["-"]]
+        adapters = adapters * len(prompts) if len(adapters) == 1 else adapters
+        if len(adapters) != len(prompts) or any(name is not None and name not in loaded for name in adapters):
+            parser.error(f"--use-adapter names one of {', '.join(loaded)} or '-', once or for each of {len(prompts)} prompts")
     if args.model:
         engine = Engine(args.model, **options)
     else:
         engine = Engine.from_random(args.random, seed=args.weights_seed, **options)
+    if args.adapter:
+        try:
+            for name, factors in loaded.items():
+                engine.load_adapter(name, factors)
+        except AdapterError as e:
+            parser.error(str(e))
     outs = engine.generate_all(prompts, args.max_new_tokens, temperature=args.temperature, seed=args.seed,
                                stop_token_ids=args.stop_token_id or (), max_batch=args.max_batch,
-                               share_prefix=args.share_prefix)
+                               share_prefix=args.share_prefix, adapters=adapters)
     for prompt, out in zip(prompts, outs):
         print(json.dumps({"prompt": prompt, "tokens": out}))
     return 0

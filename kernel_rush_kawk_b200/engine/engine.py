@@ -10,7 +10,8 @@ options add what the reference lacks: unequal prompt lengths need no option;
 place then holds None); ``dtype`` picks the bfloat16 serving path or the true
 float32 path; ``share_prefix`` runs what prompts have in common once, in pages that their sequences share;
 ``eviction`` (a ``KeyEviction``, at construction) bounds the keys that a sequence holds by giving up those that received
-least attention. After a call ``Engine.last_stats`` holds the batch's times (the
+least attention; ``adapters`` (an ``AdapterRoom``, at construction) makes room for low-rank adapters, which ``load_adapter`` fills and a call
+names, one for each prompt. After a call ``Engine.last_stats`` holds the batch's times (the
 reference logs the like: engine/engine.py:206,378); a kernel that flagged bad
 input or gave up on a wait makes the call raise ``KernelError``.
 
@@ -31,8 +32,10 @@ import torch
 from ..cache.eviction import KeyEviction
 from ..cache.store import PAGE, SequenceCache
 from ..config.registry import get_architecture, preset_config, read_config
+from ..parts.adapters import AdapterError, AdapterRoom
 from ..parts.base import KVNeed
 from ..sampling.sampler import Sampler, SamplingParams
+from ..weights.adapters import read_adapter
 from ..weights.loader import checkpoint_shapes, read_checkpoint
 from ..weights.random_init import random_tensors
 from .generate import GenerationLoop, pages_needed, shared_pages
@@ -69,7 +72,8 @@ def _default_ops(device: torch.device, head_dims):
 class Engine:
     def __init__(self, model_path=None, *, dtype="bfloat16", max_tokens: int | None = None, max_slots: int = 64,
                  max_context: int | None = None, use_cuda_graphs: bool = True, max_step_rows: int = 16384,
-                 step_tokens: int = 2048, device="cuda:0", ops=None, eviction: KeyEviction | None = None, _config=None, _tensors=None):
+                 step_tokens: int = 2048, device="cuda:0", ops=None, eviction: KeyEviction | None = None,
+                 adapters: AdapterRoom | None = None, _config=None, _tensors=None):
         torch.backends.cuda.matmul.allow_tf32 = False
         torch.backends.cudnn.allow_tf32 = False
         torch.backends.cuda.matmul.allow_bf16_reduced_precision_reduction = False
@@ -112,6 +116,13 @@ class Engine:
         self.eviction = eviction
         if eviction is not None:
             self._check_eviction()
+        self.adapters: dict[str, int] = {}  # name -> its place in the banks
+        self.adapter_room, self._beside = adapters, {}
+        if adapters is not None:
+            self._beside = self.model.open_adapters(adapters)
+            if not self._beside:
+                raise ValueError("adapters cannot stand beside any weight of this model: " + ", ".join(sorted(
+                    {s.kind for layer in self.plan.layers for s in (layer.mixer, layer.feed_forward) if s is not None})) + " layers take none")
         self.cache = self.stepper = self.loop = None
         self.sampler = Sampler(self.ops, self.device)
         self.last_stats = None  # GenerationStats of the last batch that generate / generate_all ran
@@ -154,7 +165,7 @@ class Engine:
             torch.cuda.empty_cache()
         self.cache = SequenceCache(self.model.cache_needs(), max_tokens, max_slots, self.max_context, self.device,
                                    self.dtype, step_tokens=self.step_tokens, eviction=self.eviction, pass_tokens=self.max_step_rows)
-        self.stepper = Stepper(self.model, self.cache, self.ops, self.max_step_rows, self.use_cuda_graphs)
+        self.stepper = Stepper(self.model, self.cache, self.ops, self.max_step_rows, self.use_cuda_graphs, self.adapter_room is not None)
         self.loop = GenerationLoop(self.stepper, self.cache, self.sampler)
 
     def _ensure_cache(self, prompt_lens, max_new_tokens: int, pages: int | None = None) -> None:
@@ -168,14 +179,70 @@ class Engine:
             return
         self._build_cache(pages * PAGE, slots)
 
+    # -- adapters ----------------------------------------------------------------
+    def load_adapter(self, name: str, source, scale: float | None = None) -> None:
+        """Hold a low-rank adapter under a name (in the place of one of that name). ``source``: a folder (weights.adapters), or a mapping of checkpoint
+        names of weights to (a [r, inputs], b [outputs, r], scale). ``scale`` takes the place of theirs. Weights that it does not name stay as they are.
+        An adapter that a running generation uses cannot be replaced."""
+        if self.adapter_room is None:
+            raise AdapterError("this engine has no room for adapters (Engine(adapters=AdapterRoom(count, rank)))")
+        factors = dict(source) if hasattr(source, "keys") else read_adapter(source)
+        unknown = sorted(set(factors) - set(self._beside))
+        if unknown or not factors:
+            raise AdapterError(f"adapter '{name}' stands beside no weight of this model that takes one: {', '.join(unknown) or 'it is empty'}")
+        for weight, (a, b, _) in factors.items():  # before anything is written
+            bank, part = self._beside[weight]
+            if a.dim() != 2 or b.dim() != 2 or a.shape[1] != bank.inputs or b.shape != (bank.outs[part], a.shape[0]) or not 1 <= a.shape[0] <= bank.rank:
+                raise AdapterError(f"adapter '{name}' beside {weight}: [r, {bank.inputs}] and [{bank.outs[part]}, r] with r up to {bank.rank} are asked for, "
+                                   f"got {list(a.shape)} and {list(b.shape)}")
+        if name in self.adapters:
+            index = self.adapters[name]
+            self._check_unused(name, index)
+        else:
+            free = sorted(set(range(self.adapter_room.count)) - set(self.adapters.values()))
+            if not free:
+                raise AdapterError(f"no room for adapter '{name}': {self.adapter_room.count} are held ({', '.join(sorted(self.adapters))})")
+            index = free[0]
+        for bank in {id(bank): bank for bank, _ in self._beside.values()}.values():
+            bank.clear(index)
+        for weight, (a, b, s) in factors.items():
+            bank, part = self._beside[weight]
+            bank.put(index, part, a.to(self.device), b.to(self.device), s if scale is None else scale)
+        self.adapters[name] = index
+
+    def drop_adapter(self, name: str) -> None:
+        """Make room: the name is forgotten."""
+        if name not in self.adapters:
+            raise AdapterError(f"no adapter '{name}' is held")
+        self._check_unused(name, self.adapters[name])
+        del self.adapters[name]
+
+    def _check_unused(self, name: str, index: int) -> None:
+        if self.cache is not None and any(self.cache.slots.is_held(s) and self.cache.adapter[s] == index for s in range(self.cache.max_slots)):
+            raise AdapterError(f"adapter '{name}' is in use by a running generation")
+
+    def _adapters_of(self, names, n: int):
+        """Their places in the banks, for n prompts; None where none has one."""
+        if names is None:
+            return None
+        names = [names] * n if isinstance(names, str) else list(names)
+        if len(names) != n:
+            raise AdapterError(f"{len(names)} adapters for {n} prompts")
+        for name in names:
+            if name is not None and name not in self.adapters:
+                raise AdapterError(f"no adapter '{name}' is held ({', '.join(sorted(self.adapters)) or 'none is'})")
+        return [-1 if name is None else self.adapters[name] for name in names]
+
     # -- the reference's entry ------------------------------------------------
     def generate(self, input_ids, max_new_tokens: int, *, temperature: float = 0.0, seed: int = 0,
-                 stop_token_ids=(), share_prefix: bool = False):
+                 stop_token_ids=(), share_prefix: bool = False, adapters=None):
         """Yield, per step, one token id per sequence (None once a sequence has ended
         on a stop token). All sequences start together; their lengths may differ.
 
         ``share_prefix``: what prompts begin with in common (whole pages of 64 tokens; a prompt given n times draws n samples of
-        it) is run and held once, and read once a step for all of its sequences.
+        it) is run and held once, and read once a step for all of its sequences. Prompts with different adapters share nothing.
+
+        ``adapters``: the name of a loaded adapter for all prompts, or a list with one name or None for each.
 
         This is a generator: arguments are checked, and a cache without a fixed size is
         grown if the call needs more room, at the first ``next()``. One generation runs
@@ -188,29 +255,32 @@ class Engine:
             if len(row) + max_new_tokens - 1 > self.max_context:
                 raise ValueError(f"a prompt of {len(row)} tokens plus {max_new_tokens} new ones exceeds "
                                  f"the context of {self.max_context}")
+        of = self._adapters_of(adapters, len(prompts))
         self._ensure_cache([len(p) for p in prompts], max_new_tokens,
-                           shared_pages(prompts, max_new_tokens) if share_prefix else None)
+                           shared_pages(prompts, max_new_tokens, of) if share_prefix else None)
         try:
             yield from self.loop.run_batch(prompts, max_new_tokens, SamplingParams(temperature, seed), stop_token_ids,
-                                           share_prefix=share_prefix)
+                                           share_prefix=share_prefix, adapters=of)
         finally:
             self.last_stats = self.loop.stats
             log.info("generate: %s", self.last_stats.line())
 
     def generate_all(self, input_ids, max_new_tokens: int, *, temperature: float = 0.0, seed: int = 0,
-                     stop_token_ids=(), max_batch: int | None = None, share_prefix: bool = False) -> list:
+                     stop_token_ids=(), max_batch: int | None = None, share_prefix: bool = False,
+                     adapters=None) -> list:
         """Any number of requests, run as consecutive batches; returns each request's tokens."""
         prompts = [list(map(int, row)) for row in input_ids]
         if not prompts or max_new_tokens < 1:
             return [[] for _ in prompts]
+        of = self._adapters_of(adapters, len(prompts))
         if self.max_tokens is None:  # no fixed size: room for the largest batch these requests can form
             size = max_batch or self.max_slots
             lens = sorted((len(p) for p in prompts), reverse=True)[:size]
-            self._ensure_cache(lens, max_new_tokens, max(shared_pages(prompts[i:i + size], max_new_tokens)
+            self._ensure_cache(lens, max_new_tokens, max(shared_pages(prompts[i:i + size], max_new_tokens, of and of[i:i + size])
                                                          for i in range(0, len(prompts), size)) if share_prefix else None)
         try:
             return self.loop.run_requests(prompts, max_new_tokens, SamplingParams(temperature, seed), stop_token_ids,
-                                          max_batch, share_prefix)
+                                          max_batch, share_prefix, of)
         finally:
             self.last_stats = self.loop.stats
             log.info("generate_all, last batch: %s", self.last_stats.line())

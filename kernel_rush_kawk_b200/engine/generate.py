@@ -42,6 +42,7 @@ from .step import StepEntry
 class Sequence:
     request: int
     prompt: list
+    adapter: int = -1
     slot: int = -1
     produced: list = field(default_factory=list)
     finished: bool = False
@@ -95,11 +96,12 @@ def pages_needed(prompt_len: int, max_new_tokens: int, eviction: KeyEviction | N
     return -(-rows_held(prompt_len, max_new_tokens, eviction, pass_tokens) // PAGE)
 
 
-def shared_prefixes(prompts: list) -> list:
-    """Groups of prompts that begin alike: (request indices, tokens shared) with the shared tokens whole pages, at least one token of
+def shared_prefixes(prompts: list, adapters=None) -> list:
+    """Groups of prompts that begin alike, and run with the same adapter (``adapters``: theirs, -1 for none), whose keys are others: (request indices, tokens shared) with the shared tokens whole pages, at least one token of
     every prompt behind them, 0 for a prompt alone. Neighbours in the order of the prompts' tokens join a group while the pages that it
     saves, (members - 1) * shared pages, do not get fewer."""
-    order = sorted(range(len(prompts)), key=lambda i: prompts[i])
+    of = adapters or [-1] * len(prompts)
+    order = sorted(range(len(prompts)), key=lambda i: (of[i], prompts[i]))
     groups: list = []
     for i in order:
         p = prompts[i]
@@ -108,6 +110,8 @@ def shared_prefixes(prompts: list) -> list:
             other = prompts[members[0]]
             most = min(len(p) - 1, shared if len(members) > 1 else len(other) - 1)
             n = 0
+            if of[i] != of[members[0]]:
+                most = 0
             while n < most and p[n] == other[n]:
                 n += 1
             n -= n % PAGE
@@ -118,14 +122,14 @@ def shared_prefixes(prompts: list) -> list:
     return groups
 
 
-def shared_pages(prompts: list, max_new_tokens: int) -> int:
+def shared_pages(prompts: list, max_new_tokens: int, adapters=None) -> int:
     """Pages that a batch of prompts comes to hold which share what they begin with: a group's shared ones count once."""
     pages = sum(pages_needed(len(p), max_new_tokens) for p in prompts)
-    return pages - sum((len(members) - 1) * (shared // PAGE) for members, shared in shared_prefixes(prompts))
+    return pages - sum((len(members) - 1) * (shared // PAGE) for members, shared in shared_prefixes(prompts, adapters))
 
 
 def split_into_batches(prompt_lens: list, max_new_tokens: int, max_slots: int, max_pages: int, eviction: KeyEviction | None = None,
-                       pass_tokens: int | None = None, prompts: list | None = None) -> list:
+                       pass_tokens: int | None = None, prompts: list | None = None, adapters=None) -> list:
     """Consecutive requests are grouped while slots and pages last. Returns lists of
     request indices. A request that cannot fit even alone raises ValueError. ``prompts``: theirs, where a batch shares what they begin with."""
     needs = [pages_needed(n, max_new_tokens, eviction, pass_tokens) for n in prompt_lens]
@@ -143,7 +147,7 @@ def split_into_batches(prompt_lens: list, max_new_tokens: int, max_slots: int, m
             low, high = size, most + 1
             while high - low > 1:
                 middle = most if high > most else (low + high) // 2
-                fits = shared_pages(prompts[first:first + middle], max_new_tokens) <= max_pages
+                fits = shared_pages(prompts[first:first + middle], max_new_tokens, adapters and adapters[first:first + middle]) <= max_pages
                 low, high = (middle, high) if fits else (low, middle)
             size = low
         batches.append(list(range(first, first + size)))
@@ -162,16 +166,16 @@ class GenerationLoop:
         self.stats = GenerationStats()  # of the last batch
 
     def run_batch(self, prompts: list, max_new_tokens: int, sampling: SamplingParams = SamplingParams(),
-                  stop_token_ids=(), first_request: int = 0, share_prefix: bool = False):
+                  stop_token_ids=(), first_request: int = 0, share_prefix: bool = False, adapters=None):
         """Generator: yields, per step, a list with one entry per prompt: the new token
-        id, or None for a sequence that ended at an earlier step."""
+        id, or None for a sequence that ended at an earlier step. ``adapters``: the low-rank adapter of each prompt (-1: none)."""
         if max_new_tokens < 1 or not prompts:
             return
         for i, p in enumerate(prompts):
             if len(p) == 0:
                 raise ValueError(f"prompt {i} is empty")
         stops = frozenset(int(t) for t in stop_token_ids)
-        seqs = [Sequence(first_request + i, list(p)) for i, p in enumerate(prompts)]
+        seqs = [Sequence(first_request + i, list(p), -1 if adapters is None else adapters[i]) for i, p in enumerate(prompts)]
         stats = self.stats = GenerationStats(len(seqs), sum(len(p) for p in prompts))
         t_begin = time.perf_counter()
         t_first = None
@@ -208,7 +212,7 @@ class GenerationLoop:
                 live, begun, stats.shared_tokens = self._start_shared(seqs)
             else:
                 for s in seqs:
-                    s.slot = self.cache.alloc()
+                    s.slot = self.cache.alloc(s.adapter)
                 live, begun = list(seqs), [0] * len(seqs)
             logits = self.stepper.step([StepEntry(s.slot, s.prompt[n:], [len(s.prompt) - 1 - n]) for s, n in zip(live, begun)])
             tokens = self.sampler.select(logits, sampling, [s.request for s in live], 0)
@@ -262,9 +266,9 @@ class GenerationLoop:
         """Run what the prompts share, once; (the sequences in the order of their groups, the tokens that each has had, how many of these in all did
         not run again)."""
         order, begun, first = [], [], []
-        groups = [([seqs[i] for i in members], shared) for members, shared in shared_prefixes([s.prompt for s in seqs])]
+        groups = [([seqs[i] for i in members], shared) for members, shared in shared_prefixes([s.prompt for s in seqs], [s.adapter for s in seqs])]
         for members, shared in groups:
-            members[0].slot = self.cache.alloc()
+            members[0].slot = self.cache.alloc(members[0].adapter)
             if shared:
                 first.append(StepEntry(members[0].slot, members[0].prompt[:shared], []))
         if first:
@@ -277,16 +281,17 @@ class GenerationLoop:
         return order, begun, sum((len(members) - 1) * shared for members, shared in groups)
 
     def run_requests(self, prompts: list, max_new_tokens: int, sampling: SamplingParams = SamplingParams(),
-                     stop_token_ids=(), max_batch: int | None = None, share_prefix: bool = False) -> list:
+                     stop_token_ids=(), max_batch: int | None = None, share_prefix: bool = False, adapters=None) -> list:
         """Run every request, batch after batch; returns each request's generated tokens."""
         max_slots = min(self.cache.max_slots, max_batch or self.cache.max_slots)
         batches = split_into_batches([len(p) for p in prompts], max_new_tokens, max_slots, self.cache.n_pages, self.cache.eviction,
-                                     getattr(self.stepper, "max_step_rows", None), prompts if share_prefix else None)
+                                     getattr(self.stepper, "max_step_rows", None), prompts if share_prefix else None, adapters)
         results: list = [None] * len(prompts)
         for batch in batches:
             outs = [[] for _ in batch]
             for step_out in self.run_batch([prompts[i] for i in batch], max_new_tokens, sampling, stop_token_ids,
-                                           first_request=batch[0], share_prefix=share_prefix):
+                                           first_request=batch[0], share_prefix=share_prefix,
+                                           adapters=adapters and [adapters[i] for i in batch]):
                 for j, tok in enumerate(step_out):
                     if tok is not None:
                         outs[j].append(tok)

@@ -16,6 +16,7 @@ from dataclasses import dataclass
 import torch
 
 from ..parts import base as parts_base
+from ..parts.adapters import AdapterBank
 from ..parts.base import KVNeed, StateNeed, Stream, TensorSpec
 from ..parts.plan import ModelPlan, PartSpec
 
@@ -147,6 +148,20 @@ class Model:
                               if part is not None)
         if self.position is not None:
             self.graph_safe = self.graph_safe and getattr(self.position, "graph_safe", False)
+
+    def open_adapters(self, room) -> dict:
+        """Banks for the products that adapters may stand beside, one for each part and group. Returns the weights' checkpoint names -> (bank, part of it);
+        empty where no layer takes adapters."""
+        where: dict = {}
+        for built in self.tree.all_parts():
+            groups, specs = built.part.adapter_groups(), built.part.tensor_specs()
+            banks = {}
+            for group, keys in groups.items():
+                shapes = [specs[key].shape for key in keys]
+                bank = banks[group] = AdapterBank(shapes[0][1], [n for n, _ in shapes], room.count, room.rank, self.runtime.dtype, self.runtime.device)
+                where.update({built.spec.tensors[key]: (bank, part) for part, key in enumerate(keys)})
+            built.part.banks = banks
+        return where
 
     def cache_needs(self) -> list:
         return self.tree.cache_needs()

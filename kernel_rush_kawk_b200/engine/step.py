@@ -29,7 +29,7 @@ import numpy as np
 import torch
 
 from ..cache.prefix import PrefixGroups, single_tokens_share
-from ..cache.store import SequenceCache
+from ..cache.store import PAGE, SequenceCache
 
 
 @dataclass
@@ -46,26 +46,30 @@ class BatchMeta:
     tokens[r], row_seq[r] (which sequence of the pass row r belongs to), row_pos[r]
     (its position in the sequence); seq_slot[s], seq_start[s] (cached length before
     the pass), seq_qlen[s], cu_q[s] (first row of sequence s; cu_q[n_seqs] = rows);
-    want[w] (rows whose logits are asked for). Where keys are evicted (``shifts``), row_pos and seq_start count the rows
+    want[w] (rows whose logits are asked for). row_seq, row_pos and cu_q follow from the others: a longer pass may have them
+    made on the device (``make_maps``). Where keys are evicted (``shifts``), row_pos and seq_start count the rows
     held, and seq_shift[s] how much further these lie in the sequence.
 
-    ``prefix`` (a PrefixGroups, or None) says which neighbouring sequences share pages."""
+    ``prefix`` (a PrefixGroups, or None) says which neighbouring sequences share pages, ``adapters`` (an AdapterRows, or None) which rows have
+    which low-rank adapters."""
 
-    FIELDS = ("tokens", "row_seq", "row_pos", "seq_slot", "seq_start", "seq_qlen", "cu_q", "want")
+    FIELDS = ("tokens", "seq_slot", "seq_start", "seq_qlen", "want", "pages", "row_seq", "row_pos", "cu_q")
 
-    def __init__(self, n_rows: int, n_seqs: int, n_want: int, device, shifts: bool = False):
+    def __init__(self, n_rows: int, n_seqs: int, n_want: int, device, shifts: bool = False, adapters: bool = False):
         self.n_rows, self.n_seqs, self.n_want = n_rows, n_seqs, n_want
-        sizes = (n_rows, n_rows, n_rows, n_seqs, n_seqs, n_seqs, n_seqs + 1, n_want)
+        n_pages = n_rows // PAGE + n_seqs if n_rows != n_seqs else 0  # that the pass may need beyond those which its sequences have
+        sizes = (n_rows, n_seqs, n_seqs, n_seqs, n_want, n_pages, n_rows, n_rows, n_seqs + 1)
         fields = self.FIELDS
-        if shifts:
-            sizes, fields = sizes + (n_seqs,), fields + ("seq_shift",)
-        self.prefix = None
+        for name in ("seq_shift",) * shifts + ("seq_adapter",) * adapters:
+            sizes, fields = (n_seqs,) + sizes, (name,) + fields
+        self.prefix = self.adapters = self.maps = None
         # every array starts on a 16-byte boundary
         offsets, total = [], 0
         for s in sizes:
             offsets.append(total)
             total += -(-s // 4) * 4
         self.total = max(total, 4)
+        self.made_from = offsets[fields.index("row_seq")]  # what a longer pass may have made on the device comes last
         self.offsets, self.sizes = offsets, sizes
         self.buffer = torch.zeros(self.total, dtype=torch.int32, device=device)
         self.host = torch.zeros(self.total, dtype=torch.int32, pin_memory=self.buffer.is_cuda)
@@ -74,7 +78,9 @@ class BatchMeta:
         self._single_token_shape = False  # the pinned buffer holds the constant arrays of a one-token-each pass
         for name, off, size in zip(fields, offsets, sizes):
             setattr(self, name, self.buffer[off:off + size])
+        self._own = (self.row_seq, self.row_pos, self.cu_q)
         self.copied = torch.cuda.Event() if self.buffer.is_cuda else None
+        self.bytes = self.total * 4  # of the last upload
         # host-side facts, valid for the pass being built
         self.max_q_len = 1
         self.max_kv_len = 1
@@ -87,8 +93,10 @@ class BatchMeta:
     def host_field(self, name: str) -> np.ndarray:
         return self._host_views[name]
 
-    def fill(self, slots, starts, token_lists, want_rows, shifts=None) -> None:
-        """Write one pass into the pinned buffer and start its copy to the device."""
+    def fill(self, slots, starts, token_lists, want_rows, shifts=None, adapters=None, ops=None, pages=None, table=None) -> None:
+        """Write one pass into the pinned buffer and start its copy to the device. ``ops``: what follows from the sequences' lengths is made there, and
+        ``pages`` (a host list, the sequences' new ones in order) are entered in ``table``. ``adapters``: every sequence's low-rank adapter (-1: none), which
+        needs ``ops``."""
         if self.copied is not None:
             self.copied.synchronize()  # the previous copy out of this pinned buffer is over
         q_lens = [len(t) for t in token_lists]
@@ -104,6 +112,11 @@ class BatchMeta:
                 self._single_token_shape = True
             view["tokens"][:] = [t[0] for t in token_lists]
             view["row_pos"][:] = starts
+        elif ops is not None:
+            view["tokens"][:] = np.concatenate([np.asarray(t, dtype=np.int32) for t in token_lists])
+            view["seq_qlen"][:] = q_lens
+            if pages:
+                view["pages"][:len(pages)] = pages
         else:
             cu = np.zeros(len(q_lens) + 1, dtype=np.int32)
             np.cumsum(q_lens, out=cu[1:])
@@ -117,7 +130,15 @@ class BatchMeta:
         view["want"][:] = want_rows
         if "seq_shift" in view:
             view["seq_shift"][:] = 0 if shifts is None else shifts
-        self.upload()
+        made = ops is not None and self.n_rows != self.n_seqs
+        self.row_seq, self.row_pos, self.cu_q = self._own
+        if adapters is not None:
+            view["seq_adapter"][:] = adapters
+        self.upload(self.made_from if made else None)
+        if made or adapters is not None:
+            self.make_maps(ops, adapters is not None, len(pages or ()), table)
+        else:
+            self.adapters = None
         self.max_q_len = max(q_lens)
         self.max_kv_len = max(s + n for s, n in zip(starts, q_lens))
         self.is_decode = self.max_q_len == 1
@@ -126,15 +147,26 @@ class BatchMeta:
 
     uploaded = 0  # bytes of batch descriptions copied to the device so far, all instances together
 
-    def upload(self) -> None:
-        BatchMeta.uploaded += self.total * 4
-        self.buffer.copy_(self.host, non_blocking=True)
+    def make_maps(self, ops, adapters: bool, n_pages: int, table) -> None:
+        """Have the device work out what follows from the sequences' lengths, and the pages and adapters of their rows."""
+        if self.maps is None or (self.maps.adapters is None) == adapters or (table is not None and not self.maps.with_places):
+            self.maps = None
+        self.maps = ops.step_maps(self.seq_slot, self.seq_start, self.seq_qlen, self.n_rows, table=table, pages=self.pages[:n_pages] if table is not None else None,
+                                  adapters=self.seq_adapter if adapters else None, out=self.maps)
+        self.adapters = self.maps.adapters
+        if self.n_rows != self.n_seqs:
+            self.row_seq, self.row_pos, self.cu_q = self.maps.row_seq, self.maps.row_pos, self.maps.cu_q
+
+    def upload(self, words: int | None = None) -> None:
+        words = self.total if words is None else max(words, 4)
+        BatchMeta.uploaded += words * 4
+        self.bytes = words * 4
+        if words == self.total:
+            self.buffer.copy_(self.host, non_blocking=True)
+        else:
+            self.buffer[:words].copy_(self.host[:words], non_blocking=True)
         if self.copied is not None:
             self.copied.record()
-
-    @property
-    def bytes(self) -> int:
-        return self.total * 4
 
 
 class StepContext:
@@ -176,7 +208,7 @@ class DecodeRun:
         cache.sync()
         token_lists = [[t] for t in tokens]
         self.graph = stepper._graph(slots, starts, token_lists)
-        self.graph.meta.fill(slots, starts, token_lists, list(range(n)), stepper._shifts(slots))
+        stepper._fill_single(self.graph.meta, slots, starts, token_lists)
         stepper.h2d_bytes = self.graph.meta.bytes
         ring = stepper._run_rings.get((n, self.depth))
         if ring is None:
@@ -234,8 +266,9 @@ class Stepper:
     # used last stay (each holds its activations and logits, 40 MB and more for 64 sequences of the 4B shape)
     MAX_GROUP_GRAPHS = 64
 
-    def __init__(self, model, cache: SequenceCache, ops, max_step_rows: int = 16384, use_graphs: bool = True):
+    def __init__(self, model, cache: SequenceCache, ops, max_step_rows: int = 16384, use_graphs: bool = True, adapted: bool = False):
         self.model = model
+        self.adapted = bool(adapted)  # sequences may run with low-rank adapters
         self.cache = cache
         self.ops = ops
         self.max_step_rows = int(max_step_rows)
@@ -319,13 +352,20 @@ class Stepper:
         if ring is None:
             if len(self._metas) > 64:
                 self._metas.clear()
-            ring = self._metas[key] = [0, [BatchMeta(n_rows, n_seqs, n_want, self.device, self.cache.eviction is not None) for _ in range(2)]]
+            ring = self._metas[key] = [0, [BatchMeta(n_rows, n_seqs, n_want, self.device, self.cache.eviction is not None, self.adapted) for _ in range(2)]]
         ring[0] ^= 1
         return ring[1][ring[0]]
 
     def _shifts(self, slots):
         """How much further each sequence's rows lie in it than in the cache, where keys are evicted."""
         return [self.cache.evicted[s] for s in slots] if self.cache.eviction is not None else None
+
+    def _adapters(self, slots):
+        """Every sequence's low-rank adapter, or None where none has any."""
+        if not self.adapted:
+            return None
+        of = [self.cache.adapter[s] for s in slots]
+        return of if max(of) >= 0 else None
 
     def _prefix(self, slots, single: bool = True):
         """The groups of neighbours that share pages, or None where none do or where reading them once does not pay. Float32 steps read
@@ -347,7 +387,6 @@ class Stepper:
         for i, first, n in chosen:
             e = entries[i]
             start = cache.length[e.slot]
-            cache.reserve(e.slot, start + n)
             slots.append(e.slot)
             starts.append(start)
             token_lists.append(e.tokens[first:first + n])
@@ -356,14 +395,22 @@ class Stepper:
                     want_rows.append(row + w - first)
                     which.append((i, w))
             row += n
-        cache.sync()
+        pages = cache.reserve_pass(slots, [start + n for start, (_, _, n) in zip(starts, chosen)])
         n_rows, n_seqs = row, len(chosen)
         decode = all(n == 1 for _, _, n in chosen)
+        # the maps of a longer pass, and the pages that it needs, are worked out on the device
+        by_lengths = hasattr(self.ops, "step_maps") and n_rows != n_seqs
+        if not (by_lengths and pages is not None):
+            cache.sync()
         if decode and self.use_graphs:
             logits = self._replay(slots, starts, token_lists, want_rows, n_seqs)
         else:
             meta = self._meta(n_rows, n_seqs, len(want_rows))
-            meta.fill(slots, starts, token_lists, want_rows, self._shifts(slots))
+            adapters = self._adapters(slots)
+            meta.fill(slots, starts, token_lists, want_rows, self._shifts(slots), adapters, self.ops if by_lengths or adapters else None,
+                      pages, cache.page_table() if by_lengths and pages is not None else None)
+            if by_lengths and pages is not None:
+                cache.entered(slots)
             groups = self._prefix(slots, decode)
             meta.prefix = None if groups is None else PrefixGroups(*groups, self.device)
             self.h2d_bytes += meta.bytes
@@ -386,9 +433,10 @@ class Stepper:
         """The captured step of these sequences: by their number and, where neighbours share pages, the number and size of the groups."""
         n = len(slots)
         groups = self._prefix(slots)
+        adapted = self._adapters(slots) is not None
         if groups is None:
-            return self._graphs.get(n) or self._capture(n, slots, starts, token_lists)
-        key = (n, PrefixGroups.shape_of(*groups))
+            return self._graphs.get(self._key(n, None, adapted)) or self._capture(n, slots, starts, token_lists)
+        key = self._key(n, PrefixGroups.shape_of(*groups), adapted)
         g = self._graphs.pop(key, None)
         if g is None:
             self._drop_group_graphs(self.MAX_GROUP_GRAPHS - 1)
@@ -397,6 +445,17 @@ class Stepper:
         if (g.meta.prefix.sizes, g.meta.prefix.lengths) != tuple(map(tuple, groups)):
             g.meta.prefix.update(PrefixGroups(*groups, self.device))
         return g
+
+    @staticmethod
+    def _key(n: int, shape, adapted: bool):
+        if shape is None:
+            return f"{n} adapted" if adapted else n
+        return (n, shape, adapted) if adapted else (n, shape)
+
+    def _fill_single(self, meta, slots, starts, token_lists) -> None:
+        """A step of one token each, with all its rows wanted."""
+        adapters = self._adapters(slots)
+        meta.fill(slots, starts, token_lists, list(range(len(slots))), self._shifts(slots), adapters, self.ops if adapters else None)
 
     def _drop_group_graphs(self, keep: int) -> None:
         """Let go of all but the ``keep`` captured steps of groups that were used last."""
@@ -409,7 +468,7 @@ class Stepper:
 
     def _replay(self, slots, starts, token_lists, want_rows, n: int):
         g = self._graph(slots, starts, token_lists)
-        g.meta.fill(slots, starts, token_lists, list(range(n)), self._shifts(slots))
+        self._fill_single(g.meta, slots, starts, token_lists)
         self.h2d_bytes += g.meta.bytes
         g.graph.replay()
         if len(want_rows) == n:
@@ -442,7 +501,7 @@ class Stepper:
             g, meta = None, self._meta(n, n, n)
             groups = self._prefix(slots)
             meta.prefix = None if groups is None else PrefixGroups(*groups, self.device)
-        meta.fill(slots, starts, token_lists, list(range(n)), self._shifts(slots))
+        self._fill_single(meta, slots, starts, token_lists)
         self.h2d_bytes = meta.bytes
         req = torch.tensor(list(requests) if requests is not None else list(range(n)), dtype=torch.int32).to(self.device)
         out = torch.empty((n_steps, n), dtype=torch.int32, device=self.device)
@@ -476,10 +535,10 @@ class Stepper:
         return DecodeRun(self, list(slots), [int(t) for t in tokens], sampling, list(requests), int(first_step), int(depth))
 
     def _capture(self, n: int, slots, starts, token_lists, prefix: PrefixGroups | None = None) -> _DecodeGraph:
-        meta = BatchMeta(n, n, n, self.device, self.cache.eviction is not None)
-        meta.fill(slots, starts, token_lists, list(range(n)), self._shifts(slots))
+        meta = BatchMeta(n, n, n, self.device, self.cache.eviction is not None, self.adapted)
+        self._fill_single(meta, slots, starts, token_lists)
         meta.prefix = prefix
-        key = n if prefix is None else (n, prefix.shape)
+        key = self._key(n, None if prefix is None else prefix.shape, meta.adapters is not None)
         ctx = StepContext(self.ops, meta, self.cache)
         # Run once outside a capture: everything that allocates or initialises lazily
         # does so now. The pass writes this step's keys and values; the replay of the

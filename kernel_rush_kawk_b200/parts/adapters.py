@@ -8,6 +8,8 @@ queries, keys and values) in fixed storage, so that variants come and go while c
 
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
 
 MAX_PARTS = 4  # projections side by side in one product
@@ -16,6 +18,18 @@ MAX_RANK = 256
 
 class AdapterError(ValueError):
     pass
+
+
+@dataclass(frozen=True)
+class AdapterRoom:
+    """How many low-rank adapters an engine holds at a time, and of which rank at most."""
+
+    count: int
+    rank: int
+
+    def __post_init__(self):
+        if self.count < 1 or not 1 <= self.rank <= MAX_RANK:
+            raise AdapterError(f"an engine has room for one adapter at least, of ranks from 1 to {MAX_RANK}; got {self.count} of rank {self.rank}")
 
 
 class AdapterBank:

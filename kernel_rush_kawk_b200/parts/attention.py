@@ -11,7 +11,7 @@ softmax statistics in 32-bit, q head h reads kv head h // (heads / kv_heads)
 A run that reads another run's cache (``own_cache`` False) has no k/v
 projections: it projects, normalises and rotates queries only.
 
-Where neighbours of a step share pages, what they share is read once for all of them; where keys
+Low-rank adapters of the step's rows may stand beside the projections (parts/adapters.py). Where neighbours of a step share pages, what they share is read once for all of them; where keys
 are evicted, the attention counts the weight that each key receives.
 """
 
@@ -71,6 +71,9 @@ class GQAttention(Mixer):
     def attention_head_dims(self):
         return (self.head_dim,)
 
+    def adapter_groups(self):
+        return {"qkv": ("q_proj", "k_proj", "v_proj") if self.own_cache else ("q_proj",), "o": ("o_proj",)}
+
     def set_position(self, position) -> None:
         self.position = position
 
@@ -88,7 +91,7 @@ class GQAttention(Mixer):
     def forward(self, ctx, h, cache):
         ops = ctx.ops
         kv_in_row = self.kv_heads if self.own_cache else 0
-        qkv = ops.linear(h, self.w_qkv)
+        qkv = self.product(ctx, h, self.w_qkv, "qkv")
         tables = self.position.rotary_tables() if self.position is not None else None
         cos, sin = tables if tables is not None else (None, None)
         prefix = getattr(ctx.batch, "prefix", None)  # neighbours of the step that share pages
@@ -102,7 +105,7 @@ class GQAttention(Mixer):
         else:
             attn = ops.rope_attention(qkv, self.heads, kv_in_row, self.head_dim, self.q_gain, self.k_gain, self.eps,
                                       cos, sin, ctx.batch, cache, self.scale, self.window)
-        return ops.linear(attn, self.w_o)
+        return self.product(ctx, attn, self.w_o, "o")
 
 
 register_mixer("gqa_attention", GQAttention)

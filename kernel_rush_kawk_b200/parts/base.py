@@ -77,6 +77,21 @@ class Part:
     def tensor_specs(self) -> dict[str, TensorSpec]:
         return {}
 
+    #: low-rank adapters of this part's products (``adapter_groups``): group -> AdapterBank, where the engine has room for any
+    banks: dict = {}
+
+    def adapter_groups(self) -> dict[str, tuple[str, ...]]:
+        """Which of its products low-rank adapters may stand beside: a group's name -> the keys of its tensors ([outputs, inputs]) in the
+        order in which they are one product."""
+        return {}
+
+    def product(self, ctx, x, w, group: str):
+        """x W^T, with the adapters of the step's rows beside it where they have any."""
+        rows = getattr(ctx.batch, "adapters", None)
+        if rows is None or group not in self.banks:
+            return ctx.ops.linear(x, w)
+        return ctx.ops.adapted_linear(x, w, self.banks[group], rows)
+
     def bind(self, tensors: dict, runtime) -> None:
         """Take this part's tensors (keyed as in ``tensor_specs``). ``runtime`` gives
         ``device``, ``dtype`` (torch dtype of the path) and ``ops`` (the kernels)."""

@@ -3,7 +3,8 @@
 gu = h Wgu^T with Wgu = cat(Wgate, Wup) (engine/model.py:116,301 of
 willzeng274/kernel-rush-kawk); a = round(round(silu(g)) * u) with
 silu(g) = g / (1 + exp(-g)) in 32-bit (engine/kernels/swiglu.py:21-24,
-engine/kernels/gemm.py:108-113); d = a Wdown^T. No biases.
+engine/kernels/gemm.py:108-113); d = a Wdown^T. No biases. Low-rank adapters of the step's rows may
+stand beside all three (parts/adapters.py); gate and up are then not rounded before the activation.
 """
 
 from __future__ import annotations
@@ -33,9 +34,16 @@ class SwiGLU(FeedForward):
         self.w_gate_up = torch.cat([tensors["gate_proj"], tensors["up_proj"]], dim=0).contiguous()
         self.w_down = tensors["down_proj"].contiguous()
 
+    def adapter_groups(self):
+        return {"gate_up": ("gate_proj", "up_proj"), "down": ("down_proj",)}
+
     def forward(self, ctx, h):
-        act = ctx.ops.gate_up_swiglu(h, self.w_gate_up, self.intermediate)
-        return ctx.ops.linear(act, self.w_down)
+        rows = getattr(ctx.batch, "adapters", None)
+        if rows is None or "gate_up" not in self.banks:
+            act = ctx.ops.gate_up_swiglu(h, self.w_gate_up, self.intermediate)
+        else:
+            act = ctx.ops.adapted_gate_up_swiglu(h, self.w_gate_up, self.intermediate, self.banks["gate_up"], rows)
+        return self.product(ctx, act, self.w_down, "down")
 
 
 register_feed_forward("swiglu", SwiGLU)
