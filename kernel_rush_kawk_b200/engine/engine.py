@@ -192,8 +192,8 @@ class Engine:
             raise AdapterError(f"adapter '{name}' stands beside no weight of this model that takes one: {', '.join(unknown) or 'it is empty'}")
         for weight, (a, b, _) in factors.items():  # before anything is written
             bank, part = self._beside[weight]
-            if a.dim() != 2 or b.dim() != 2 or a.shape[1] != bank.inputs or b.shape != (bank.outs[part], a.shape[0]) or not 1 <= a.shape[0] <= bank.rank:
-                raise AdapterError(f"adapter '{name}' beside {weight}: [r, {bank.inputs}] and [{bank.outs[part]}, r] with r up to {bank.rank} are asked for, "
+            if a.dim() != 2 or b.dim() != 2 or a.shape[1] != bank.inputs or b.shape != (bank.outs[part], a.shape[0]) or not 1 <= a.shape[0] <= bank.most:
+                raise AdapterError(f"adapter '{name}' beside {weight}: [r, {bank.inputs}] and [{bank.outs[part]}, r] with r up to {bank.most} are asked for, "
                                    f"got {list(a.shape)} and {list(b.shape)}")
         if name in self.adapters:
             index = self.adapters[name]

@@ -50,6 +50,7 @@ class AdapterBank:
             raise AdapterError(f"adapters are float32 or bfloat16 like the projection beside them, got {dtype}")
         self.inputs, self.outs, self.capacity = int(inputs), outs, int(capacity)
         self.outputs = sum(outs)
+        self.most = int(rank)
         self.rank = -(-int(rank) // 8) * 8
         self.dtype = dtype
         self.begin = [sum(outs[:i]) for i in range(len(outs) + 1)]
@@ -82,8 +83,8 @@ class AdapterBank:
         if a.dim() != 2 or b.dim() != 2 or a.shape[1] != self.inputs or b.shape != (n, a.shape[0]):
             raise AdapterError(f"an adapter from {self.inputs} to {n} is [rank, {self.inputs}] and [{n}, rank], got {list(a.shape)} and {list(b.shape)}")
         r = a.shape[0]
-        if not 1 <= r <= self.rank:
-            raise AdapterError(f"an adapter of rank {r} in a bank of rank {self.rank}")
+        if not 1 <= r <= self.most:
+            raise AdapterError(f"an adapter of rank {r} in a bank of rank {self.most}")
         self.a[index, part * self.rank:part * self.rank + r].copy_(a)
         self.b[index, self.begin[part]:self.begin[part] + n, :r].copy_(b)
         if r < self.rank:

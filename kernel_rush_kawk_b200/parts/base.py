@@ -85,12 +85,16 @@ class Part:
         order in which they are one product."""
         return {}
 
+    def adapted(self, ctx, group: str):
+        """(bank, AdapterRows) of a group where the step's rows have adapters, else None."""
+        bank = self.banks.get(group)
+        rows = None if bank is None else getattr(ctx.batch, "adapters", None)
+        return None if rows is None else (bank, rows)
+
     def product(self, ctx, x, w, group: str):
         """x W^T, with the adapters of the step's rows beside it where they have any."""
-        rows = getattr(ctx.batch, "adapters", None)
-        if rows is None or group not in self.banks:
-            return ctx.ops.linear(x, w)
-        return ctx.ops.adapted_linear(x, w, self.banks[group], rows)
+        beside = self.adapted(ctx, group)
+        return ctx.ops.linear(x, w) if beside is None else ctx.ops.adapted_linear(x, w, *beside)
 
     def bind(self, tensors: dict, runtime) -> None:
         """Take this part's tensors (keyed as in ``tensor_specs``). ``runtime`` gives

@@ -38,11 +38,11 @@ class SwiGLU(FeedForward):
         return {"gate_up": ("gate_proj", "up_proj"), "down": ("down_proj",)}
 
     def forward(self, ctx, h):
-        rows = getattr(ctx.batch, "adapters", None)
-        if rows is None or "gate_up" not in self.banks:
+        beside = self.adapted(ctx, "gate_up")
+        if beside is None:
             act = ctx.ops.gate_up_swiglu(h, self.w_gate_up, self.intermediate)
         else:
-            act = ctx.ops.adapted_gate_up_swiglu(h, self.w_gate_up, self.intermediate, self.banks["gate_up"], rows)
+            act = ctx.ops.adapted_gate_up_swiglu(h, self.w_gate_up, self.intermediate, *beside)
         return self.product(ctx, act, self.w_down, "down")
 
 

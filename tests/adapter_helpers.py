@@ -98,3 +98,40 @@ def maps_by_hand(slots, starts, lengths, table, pages, adapters):
             of.append(adapters[s] if adapters is not None else None)
             place.append(table[slot][p // 64] * 64 + p % 64 if table is not None else None)
     return cu, seq, pos, place, of
+
+
+# -- engines ------------------------------------------------------------------------------------------------------------
+
+def random_factors(cfg, w, seed, rank, keys=("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj"), layers=None, std=0.25):
+    """{checkpoint name: (a, b, scale)} for the named projections of a plain model's layers, large enough to move the logits."""
+    g = torch.Generator().manual_seed(seed)
+    out = {}
+    for name, t in w.items():
+        if t.dim() == 2 and name.split(".")[-2] in keys and (layers is None or int(name.split(".")[2]) in layers):
+            r = max(1, rank - len(out) % 3)
+            out[name] = (torch.randn((r, t.shape[1]), generator=g) / t.shape[1] ** 0.5, torch.randn((t.shape[0], r), generator=g) * std / r ** 0.5, 0.75 + 0.25 * (seed % 3))
+    return out
+
+
+def merged(w, factors):
+    """The plain model's weights with an adapter's products added (None: as they are)."""
+    if factors is None:
+        return w
+    return {name: t if name not in factors else (t.double() + factors[name][2] * factors[name][1].double() @ factors[name][0].double()).to(t.dtype)
+            for name, t in w.items()}
+
+
+def write_adapter(folder, factors, alpha=8.0, prefix="base_model.model.", **config):
+    """An adapter's folder; the scales are alpha / r."""
+    import json
+
+    from safetensors.torch import save_file
+
+    folder.mkdir(parents=True)
+    (folder / "adapter_config.json").write_text(json.dumps({"r": 4, "lora_alpha": alpha, **config}))
+    tensors = {}
+    for name, (a, b, _) in factors.items():
+        module = prefix + name.removesuffix(".weight")
+        tensors[module + ".lora_A.weight"], tensors[module + ".lora_B.weight"] = a.contiguous(), b.contiguous()
+    save_file(tensors, str(folder / "adapter_model.safetensors"))
+    return folder
