@@ -31,6 +31,7 @@ _ADAPT_SIGNATURES = {
     "krk_adapter_first": [_P, _P, c_longlong, c_int, c_int, _BANK, _P, _P, c_int, _P],
     "krk_adapted_gemm": [_P, _P, c_longlong, _P, c_longlong, c_int, c_int, c_int, _BANK, _P, _P, _P, c_int, c_int, _P, _P, c_int, c_int, _P, _P],
     "krk_adapted_skinny": [_P, _P, _P, c_int, c_int, c_int, _BANK, _P, _P, _P, c_int, c_int, _P, c_int, _P, _P],
+    "krk_adapted_few_f32": [_P, _P, c_longlong, _P, c_longlong, c_int, c_int, c_int, _BANK, _P, _P, _P, _P],
     "krk_adapter_second": [_P, _P, _P, c_int, c_int, _BANK, _P, c_int, c_int, _P],
 }
 
@@ -239,7 +240,12 @@ class AdapterOps:
             self._ok(self.adapt.krk_adapted_gemm(out.data_ptr(), x_at, ldx, w_at, ldw, M, N, K, described, row_adapter, info, slots, n_slots, height, t_at,
                                                  t_at + 4 * t_words if rest else None, shared, int(gated > 0), error, stream), what)
             return out
-        # float32, and sizes, strides and addresses that the tensor cores' copies do not take
+        if w.dtype is torch.float32 and M <= self.SKINNY_MAX_ROWS and not gated and not (K | ldx | ldw) & 3 and not (x_at | w_at) & 15:
+            self.launches += 1
+            t = self.error.new_empty(M * bank.parts * (-(-bank.rank // 16) * 16))
+            self._ok(self.adapt.krk_adapted_few_f32(out.data_ptr(), x_at, ldx, w_at, ldw, M, N, K, described, row_adapter, t.data_ptr(), error, stream), what)
+            return out
+        # more rows of float32, and sizes, strides and addresses that the tensor cores' copies do not take
         if not x.is_contiguous():
             x = x.contiguous()
         t = self.error.new_empty(M * bank.parts * (-(-bank.rank // 16) * 16))

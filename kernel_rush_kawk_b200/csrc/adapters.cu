@@ -186,47 +186,124 @@ __global__ void __launch_bounds__(MAP_THREADS) step_maps_kernel(const Maps m) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Every type, any size: t[r, p * wide + j] = scale sum_k x[r, k] A[a, p * rank + j, k] in 32 bits, a warp a sum
+// Every type, any size: t[r, p * wide + j] = scale sum_k x[r, k] A[a, p * rank + j, k] in 32 bits
 // ---------------------------------------------------------------------------------------------------------------------
 //
-// A sum's order depends on K alone, so a row gives the same bits whatever stands beside it.
-template <typename T>
+// A block has four columns of t and the rows, of sixteen neighbours, that have one adapter: A's rows are read once for four of them. Its eight warps take pieces of
+// 128 k in turn, a lane four of a piece, whether or not addresses let it read them at once; lanes are added up, then warps in order. A sum's order so depends
+// on K alone, and a row gives the same bits whatever stands beside it. Bound by the way to L2 of A, of whose rows a warp has a few in flight. (A warp a sum over
+// all of K: sixteen rows, rank 64, K = 9,728: 130 us, and the product behind it waited.) Columns behind an adapter's rank, up to the next multiple of 16 of the
+// bank's, are zeros.
+constexpr int FIRST_COLS = 4, FIRST_WINDOW = 16;
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ void four_of(float (&v)[4], const T* p, int n) {
+  if constexpr (WIDE && sizeof(T) == 4) {
+    const float4 all = *reinterpret_cast<const float4*>(p);
+    v[0] = all.x; v[1] = all.y; v[2] = all.z; v[3] = all.w;
+  } else if constexpr (WIDE) {
+    const uint2 all = *reinterpret_cast<const uint2*>(p);
+    v[0] = __uint_as_float(all.x << 16); v[1] = __uint_as_float(all.x & 0xffff0000u);
+    v[2] = __uint_as_float(all.y << 16); v[3] = __uint_as_float(all.y & 0xffff0000u);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? to_float<T>(p[i]) : 0.f;
+  }
+}
+
+// R rows of one adapter; w: the first of the columns' rows of A
+template <typename T, bool WIDE, int R>
+__device__ __forceinline__ void first_sums(float* sums, const T* const (&x)[R], const T* w, int cols, int K, int lane, int warp) {
+  float sum[R][FIRST_COLS];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int c = 0; c < FIRST_COLS; ++c) sum[r][c] = 0.f;
+#pragma unroll 2
+  for (int k = 128 * warp + 4 * lane; k < K; k += 128 * 8) {
+    float u[R][4], v[FIRST_COLS][4];
+#pragma unroll
+    for (int c = 0; c < FIRST_COLS; ++c) four_of<T, WIDE>(v[c], w + (size_t)min(c, cols - 1) * K + k, K - k);
+#pragma unroll
+    for (int r = 0; r < R; ++r) four_of<T, WIDE>(u[r], x[r] + k, K - k);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int c = 0; c < FIRST_COLS; ++c) sum[r][c] = fmaf(u[r][i], v[c][i], sum[r][c]);
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int c = 0; c < FIRST_COLS; ++c) {
+      const float all = warp_sum(sum[r][c]);
+      if (lane == 0) sums[(r * FIRST_COLS + c) * 8 + warp] = all;
+    }
+}
+
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) first_factor_kernel(float* __restrict__ t, const T* __restrict__ x, long long ldx, int K, const __grid_constant__ AdapterBank bank,
-                                                           const int* __restrict__ row_adapter, int rows, int* __restrict__ error) {
-  grid_launch_dependents();
+                                                           const int* __restrict__ row_adapter, int rows, int early, int* __restrict__ error) {
+  __shared__ float sums[4 * FIRST_COLS * 8];
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per_row = bank.parts * bank.rank;
-  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-    const int a = row_adapter[r];
-    if (a < 0 || a >= bank.capacity) {
-      if (a >= bank.capacity && threadIdx.x == 0) atomicExch(error, KRK_ERROR_ADAPTER);
+  if (early) grid_launch_dependents();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int column = blockIdx.x * FIRST_COLS, p = column / bank.wide, j = column % bank.wide;  // (wide is a multiple of 16)
+  for (int r0 = blockIdx.y * FIRST_WINDOW; r0 < rows; r0 += gridDim.y * FIRST_WINDOW) {
+    const int r = r0 + blockIdx.z;
+    const int theirs = lane < FIRST_WINDOW && r0 + lane < rows ? row_adapter[r0 + lane] : -1;
+    const int a = __shfl_sync(0xffffffffu, theirs, blockIdx.z);
+    unsigned left = __ballot_sync(0xffffffffu, theirs == a);
+    const int before = __popc(left & ((1u << blockIdx.z) - 1));
+    if (r >= rows || a < 0 || before % 4) continue;  // (a row before this one has the adapter and takes this one along)
+    if (a >= bank.capacity) {
+      if (tid == 0) atomicExch(error, KRK_ERROR_ADAPTER);
       continue;
     }
-    for (int i = blockIdx.x * 8 + warp; i < per_row; i += gridDim.x * 8) {
-      const int p = i / bank.rank, j = i % bank.rank;
-      if (j >= bank.ranks[a * bank.parts + p]) continue;
-      const T* w = reinterpret_cast<const T*>(bank.a) + ((size_t)a * per_row + i) * K;
-      const T* xr = x + (size_t)r * ldx;
-      float sum = 0.f;
-      for (int k = lane; k < K; k += 32) sum += to_float<T>(xr[k]) * to_float<T>(w[k]);
-      sum = warp_sum(sum);
-      if (lane == 0) t[((size_t)r * bank.parts + p) * bank.wide + j] = sum * bank.scale[a * bank.parts + p];
+    left &= ~((1u << blockIdx.z) - 1);
+    const int cols = min(bank.ranks[a * bank.parts + p] - j, FIRST_COLS), n = min(__popc(left), 4);
+    const float scale = bank.scale[a * bank.parts + p];
+    const T* w = reinterpret_cast<const T*>(bank.a) + ((size_t)(a * bank.parts + p) * bank.rank + j) * K;
+    {
+      int at[4];
+      const T* from[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        at[i] = r0 + (left ? __ffs(left) - 1 : blockIdx.z);
+        left &= left - 1;
+        from[i] = x + (size_t)at[i] * ldx;
+      }
+      if (cols > 0) {
+        if (n == 1) {
+          const T* const one[1] = {from[0]};
+          first_sums<T, WIDE, 1>(sums, one, w, cols, K, lane, warp);
+        } else if (n == 2) {
+          const T* const two[2] = {from[0], from[1]};
+          first_sums<T, WIDE, 2>(sums, two, w, cols, K, lane, warp);
+        } else {
+          const T* const four[4] = {from[0], from[1], from[2], from[3]};
+          first_sums<T, WIDE, 4>(sums, four, w, cols, K, lane, warp);
+        }
+      }
+      __syncthreads();
+      grid_launch_dependents();
+      if (tid < n * FIRST_COLS) {
+        const int i = tid / FIRST_COLS, c = tid % FIRST_COLS;
+        float all = 0.f;
+        if (c < cols) {
+#pragma unroll
+          for (int s = 0; s < 8; ++s) all += sums[tid * 8 + s];
+          all *= scale;
+        }
+        t[(size_t)at[i] * bank.parts * bank.wide + column + c] = all;
+      }
+      __syncthreads();
     }
   }
 }
 
 // out[r, n] = y[r, n] + sum_j t[r, p of n, j] B[a, n, j], y in 32 bits, rounded once; gated: out = silu(gate) * up of the two halves.
-template <typename T>
-__device__ __forceinline__ float second_factor(const AdapterBank& bank, const float* t, int a, int r, int n, int N) {
-  const int p = part_of(bank, n), rank = bank.ranks[a * bank.parts + p];
-  const T* b = reinterpret_cast<const T*>(bank.b) + ((size_t)a * N + n) * bank.rank;
-  const float* tr = t + ((size_t)r * bank.parts + p) * bank.wide;
-  float sum = 0.f;
-  for (int j = 0; j < rank; ++j) sum += tr[j] * to_float<T>(b[j]);
-  return sum;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(256) second_factor_kernel(T* __restrict__ out, const float* __restrict__ y, const float* __restrict__ t, const __grid_constant__ AdapterBank bank,
                                                             const int* __restrict__ row_adapter, int rows, int N, int gated) {
@@ -238,12 +315,18 @@ __global__ void __launch_bounds__(256) second_factor_kernel(T* __restrict__ out,
   for (int r = blockIdx.y; r < rows; r += gridDim.y) {
     int a = row_adapter[r];
     if (a >= bank.capacity) a = -1;
-    float v = y[(size_t)r * N + n];
-    if (a >= 0) v += second_factor<T>(bank, t, a, r, n, N);
+    const int whose[1] = {a}, row[1] = {r};
+    float v;
     if (gated) {
-      float u = y[(size_t)r * N + width + n];
-      if (a >= 0) u += second_factor<T>(bank, t, a, r, width + n, N);
-      v = v / (1.0f + expf(-v)) * u;
+      float sums[1][2] = {{y[(size_t)r * N + n], y[(size_t)r * N + width + n]}};
+      const int at[2] = {n, width + n};
+      add_second_factor<T, 1, 2>(bank, t, whose, row, at, sums);
+      v = sums[0][0] / (1.0f + expf(-sums[0][0])) * sums[0][1];
+    } else {
+      float sums[1][1] = {{y[(size_t)r * N + n]}};
+      const int at[1] = {n};
+      add_second_factor<T, 1, 1>(bank, t, whose, row, at, sums);
+      v = sums[0][0];
     }
     out[(size_t)r * width + n] = from_float<T>(v);
   }
@@ -295,14 +378,25 @@ KRK_API int krk_step_maps(const int* slots, const int* starts, const int* length
   return (int)launch_pdl(step_maps_kernel, dim3(blocks), dim3(MAP_THREADS), smem, stream, m);
 }
 
+int krk_first_factor_f32(float* t, const void* x, long long ldx, int rows, int K, const AdapterBank& bank, const int* row_adapter, int* error, int dtype,
+                         cudaStream_t stream) {
+  const dim3 grid(bank.parts * bank.wide / FIRST_COLS, min((rows + FIRST_WINDOW - 1) / FIRST_WINDOW, 32768), min(rows, FIRST_WINDOW));
+  const bool wide = !((K | ldx) & 3) && !(((uintptr_t)x | (uintptr_t)bank.a) & 15);
+  // The next kernel's blocks go to the SMs that have none of these first, and many of them on few SMs cost more than what they would stream beside these (eight rows of
+  // K = 9,728, rank 64, 128 blocks here: 82 us and 63 behind them; four rows, 64 blocks: 47 and 51).
+  const int early = (long long)grid.x * grid.y * grid.z <= 74;
+  auto launch = [&](auto kernel, auto* typed) {
+    return (int)launch_pdl(kernel, grid, dim3(256), 0, stream, t, typed, ldx, K, bank, row_adapter, rows, early, error);
+  };
+  if (dtype == KRK_DTYPE_F32) return launch(wide ? first_factor_kernel<float, true> : first_factor_kernel<float, false>, (const float*)x);
+  if (dtype == KRK_DTYPE_BF16) return launch(wide ? first_factor_kernel<bf16, true> : first_factor_kernel<bf16, false>, (const bf16*)x);
+  return -4;
+}
+
 // t [rows, parts * wide] float32 of every row that has an adapter.
 KRK_API int krk_adapter_first(float* t, const void* x, long long ldx, int rows, int K, const AdapterBank* bank, const int* row_adapter, int* error, int dtype,
                               cudaStream_t stream) {
-  if (rows == 0) return 0;
-  const dim3 grid((bank->parts * bank->rank + 7) / 8, min(rows, 32768));
-  if (dtype == KRK_DTYPE_F32) return (int)launch_pdl(first_factor_kernel<float>, grid, dim3(256), 0, stream, t, (const float*)x, ldx, K, *bank, row_adapter, rows, error);
-  if (dtype == KRK_DTYPE_BF16) return (int)launch_pdl(first_factor_kernel<bf16>, grid, dim3(256), 0, stream, t, (const bf16*)x, ldx, K, *bank, row_adapter, rows, error);
-  return -4;
+  return rows == 0 ? 0 : krk_first_factor_f32(t, x, ldx, rows, K, *bank, row_adapter, error, dtype, stream);
 }
 
 // out [rows, N] (gated: [rows, N / 2]) from y [rows, N] float32 and t.

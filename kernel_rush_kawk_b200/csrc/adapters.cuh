@@ -39,7 +39,67 @@ __device__ __forceinline__ int part_of(const AdapterBank& bank, int n) {
   return p;
 }
 
+// sums[r][c] += sum_j t[r, p of n, j] B[a, n, j] in 32 bits for R rows and C columns at once (a[r] negative: nothing; n[c] negative: not there), the factors' sum one
+// chain over j, added to what is there at the end; t float32 [rows, parts * wide]. Sixteen j of all of them are read before they are multiplied: one output
+// after another took 13 us behind sixteen rows of rank 64.
+template <typename T, int R, int C>
+__device__ __forceinline__ void add_second_factor(const AdapterBank& bank, const float* t, const int (&a)[R], const int (&row)[R], const int (&n)[C], float (&sums)[R][C]) {
+  const T* b[R][C];
+  const float* tr[R][C];
+  int rank[R][C], most = 0;
+  float sum[R][C];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const bool there = a[r] >= 0 && n[c] >= 0;
+      const int p = there ? part_of(bank, n[c]) : 0;
+      rank[r][c] = there ? bank.ranks[a[r] * bank.parts + p] : 0;
+      b[r][c] = reinterpret_cast<const T*>(bank.b) + ((size_t)max(a[r], 0) * bank.begin[KRK_MAX_PARTS] + max(n[c], 0)) * bank.rank;
+      tr[r][c] = t + ((size_t)row[r] * bank.parts + p) * bank.wide;
+      most = max(most, rank[r][c]);
+      sum[r][c] = 0.f;
+    }
+  constexpr int AT_ONCE = R * C > 2 ? 8 : 16;
+#pragma unroll 1
+  for (int j = 0; j < most; j += AT_ONCE) {
+    __align__(16) float u[R][C][AT_ONCE], v[R][C][AT_ONCE];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; i += 4) {
+          const bool in = j + i < rank[r][c];  // (the bank's rank is a multiple of eight, and both factors are zeros behind the adapter's)
+          *reinterpret_cast<float4*>(&u[r][c][i]) = in ? __ldcg(reinterpret_cast<const float4*>(tr[r][c] + j + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4*>(&v[r][c][i]) = in ? *reinterpret_cast<const float4*>(b[r][c] + j + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+          } else {
+            const uint2 two = in ? *reinterpret_cast<const uint2*>(b[r][c] + j + i) : make_uint2(0, 0);
+            v[r][c][i] = __uint_as_float(two.x << 16);
+            v[r][c][i + 1] = __uint_as_float(two.x & 0xffff0000u);
+            v[r][c][i + 2] = __uint_as_float(two.y << 16);
+            v[r][c][i + 3] = __uint_as_float(two.y & 0xffff0000u);
+          }
+        }
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int c = 0; c < C; ++c) sum[r][c] = fmaf(u[r][c][i], v[r][c][i], sum[r][c]);
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (rank[r][c] > 0) sums[r][c] += sum[r][c];
+}
+
 // t = scale (x A^T) of every slot, or (compact) of every row that has an adapter (first_factor.cu); sets n_done words at `done` to zero. Lets the next kernel start
 // once what came before is over: that one may read what earlier kernels wrote before it waits, and waits before it reads t.
 int krk_first_factor(void* t, bool compact, int* done, int n_done, const void* x, long long ldx, int K, const AdapterBank& bank, const AdapterTiles& tiles, int* error,
                      cudaStream_t stream);
+// The same in 32 bits, for every type: t [rows, parts * wide] float32 of every row that has an adapter (adapters.cu). Lets the next kernel start as above.
+int krk_first_factor_f32(float* t, const void* x, long long ldx, int rows, int K, const AdapterBank& bank, const int* row_adapter, int* error, int dtype,
+                         cudaStream_t stream);

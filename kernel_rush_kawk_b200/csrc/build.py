@@ -40,14 +40,14 @@ SCAN_SOURCES = ["recurrent.cu", "recurrent_chunks.cu", "ssd.cu"]
 MEMORY_SOURCES = ["matrix_memory.cu", "matrix_memory_chunks.cu", "matrix_memory_step.cu"]
 MOE_SOURCES = ["routed.cu", "few_experts.cu", "grouped_gemm.cu"]
 CACHE_SOURCES = ["evict.cu"]
-ADAPT_SOURCES = ["adapters.cu", "first_factor.cu", "adapted_gemm.cu", "adapted_skinny.cu"]
+ADAPT_SOURCES = ["adapters.cu", "first_factor.cu", "adapted_gemm.cu", "adapted_skinny.cu", "adapted_few_f32.cu"]
 SMALL_LIBRARIES = {"mix": MIX_SOURCES, "scan": SCAN_SOURCES, "memory": MEMORY_SOURCES, "moe": MOE_SOURCES, "cache": CACHE_SOURCES,
                    "adapt": ADAPT_SOURCES}
 PARTS_SOURCES = ["partial_attention.cu", "few_rows_attention.cu", "many_rows_attention.cu", "prefix_tcgen05.cu", "key_weights_tcgen05.cu"]
 LATENT_SOURCES = ["latent_prefill.cu"]
 ATTN_SOURCES = ["attention_simple.cu", "attention_mma.cu", "attention_tcgen05.cu"]
 HEADERS = ["common.cuh", "mma.cuh", "tcgen05.cuh", "attention_noalloc.h", "attention_tiles.cuh", "partial_attention.cuh"]
-OWN_HEADERS = {"core": ["skinny.cuh"], "adapt": ["skinny.cuh", "adapters.cuh", "warp_copies.cuh"]}
+OWN_HEADERS = {"core": ["skinny.cuh", "few_f32.cuh"], "adapt": ["skinny.cuh", "few_f32.cuh", "adapters.cuh", "warp_copies.cuh"]}
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]

@@ -68,7 +68,7 @@ __host__ __device__ constexpr int ring_loads() {
 // previous kernel), so the memory system is busy from the
 // block's first instruction.
 template <int WARPS, int NT, int RT, int SWIGLU, typename TOut, int KSPLIT = 1, int RING = 0, typename Extra = NoExtra>
-__global__ void __launch_bounds__(WARPS * 32)
+__global__ void __launch_bounds__(WARPS * 32, Extra::ON && WARPS == 4 ? 5 : 0)  // (five of the small blocks share an SM, see launch)
 skinny_kernel(TOut* __restrict__ out, const bf16* __restrict__ x, const bf16* __restrict__ W,
               int M, int N, int K, float limit, const __grid_constant__ Extra extra) {
   extern __shared__ __align__(16) unsigned char smem_raw[];

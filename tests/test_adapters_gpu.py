@@ -137,6 +137,19 @@ def test_float32_rows_are_the_same_in_any_company(ops):
         assert torch.equal(alone[0], whole[r])
 
 
+@pytest.mark.parametrize("rows", [1, 2, 5, 9, 16])
+@pytest.mark.parametrize("outs,K,rank", [((96, 40, 7), 36, 3), ((300, 20), 516, 17), ((16400, 33), 64, 8), ((65, 64, 63, 2), 128, 128), ((12300,), 1028, 40)])
+def test_few_float32_rows(ops, rows, outs, K, rank):
+    """Up to sixteen rows in the product's own launch: every way that it splits rows and columns, borders of parts inside it, and the bits of many rows."""
+    lengths, of = [1] * rows, spread([1] * rows, 5)
+    x, w, adapters, bank = case(14, torch.float32, K, outs, lengths, of, rank, 5, skip={(1, len(outs) - 1)})
+    got = ops.adapted_linear(x, w, bank, rows_of_step(ops, lengths, of, DEV))
+    assert_within(got, *product64(x, w, adapters, outs, of, True))
+    more = torch.cat([x, torch.randn((30, K), device=DEV)])
+    many = ops.adapted_linear(more, w, bank, rows_of_step(ops, [1] * (rows + 30), of + [2] * 30, DEV))
+    assert torch.equal(got, many[:rows])
+
+
 @pytest.mark.parametrize("rows", [1, 9, 16, 40, 700])
 def test_the_same_call_gives_the_same_bits(ops, rows):
     lengths = [1] * rows if rows < 100 else [rows - 200, 150, 50]
