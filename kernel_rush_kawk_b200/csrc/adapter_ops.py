@@ -104,6 +104,7 @@ class AdapterOps:
     """Mixed into ``Kernels``."""
 
     MOST_SEQUENCES = 25000  # of one call of step_maps: every block holds their first rows and pages in shared memory
+    MOST_ROWS = 1 << 28
 
     @property
     def adapt(self) -> ctypes.CDLL:
@@ -123,8 +124,8 @@ class AdapterOps:
         Lengths that do not add up to ``n_rows``, slots that the table does not have, and sequences that outgrow it or the given pages are
         found on the device: the error word is set (``check`` raises), and the rows concerned have position or place -1."""
         what, n, n_rows = "maps of a step", lengths.shape[0], int(n_rows)
-        if n_rows < 0 or n > self.MOST_SEQUENCES:
-            raise KernelError(f"{what}: {n} sequences with {n_rows} rows (up to {self.MOST_SEQUENCES} sequences are taken)")
+        if not 0 <= n_rows <= self.MOST_ROWS or n > self.MOST_SEQUENCES:
+            raise KernelError(f"{what}: {n} sequences with {n_rows} rows (up to {self.MOST_SEQUENCES} sequences and {self.MOST_ROWS} rows are taken)")
         tensors = (slots, starts, lengths) if adapters is None else (slots, starts, lengths, adapters)
         for t in tensors:
             if t.dtype is not _I32 or t.shape != (n,) or not t.is_contiguous():

@@ -190,11 +190,12 @@ class Engine:
         unknown = sorted(set(factors) - set(self._beside))
         if unknown or not factors:
             raise AdapterError(f"adapter '{name}' stands beside no weight of this model that takes one: {', '.join(unknown) or 'it is empty'}")
-        for weight, (a, b, _) in factors.items():  # before anything is written
+        for weight, (a, b, s) in factors.items():  # before anything is written
             bank, part = self._beside[weight]
-            if a.dim() != 2 or b.dim() != 2 or a.shape[1] != bank.inputs or b.shape != (bank.outs[part], a.shape[0]) or not 1 <= a.shape[0] <= bank.most:
-                raise AdapterError(f"adapter '{name}' beside {weight}: [r, {bank.inputs}] and [{bank.outs[part]}, r] with r up to {bank.most} are asked for, "
-                                   f"got {list(a.shape)} and {list(b.shape)}")
+            try:
+                bank.check(part, a, b, s if scale is None else scale)
+            except AdapterError as e:
+                raise AdapterError(f"adapter '{name}' beside {weight}: {e}") from e
         if name in self.adapters:
             index = self.adapters[name]
             self._check_unused(name, index)

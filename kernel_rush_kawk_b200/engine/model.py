@@ -151,16 +151,21 @@ class Model:
 
     def open_adapters(self, room) -> dict:
         """Banks for the products that adapters may stand beside, one for each part and group. Returns the weights' checkpoint names -> (bank, part of it);
-        empty where no layer takes adapters."""
+        empty where no layer takes adapters. A weight that several parts have takes none."""
         where: dict = {}
+        twice = set()  # weights of several parts, each of which would need the adapter
         for built in self.tree.all_parts():
             groups, specs = built.part.adapter_groups(), built.part.tensor_specs()
             banks = {}
             for group, keys in groups.items():
                 shapes = [specs[key].shape for key in keys]
                 bank = banks[group] = AdapterBank(shapes[0][1], [n for n, _ in shapes], room.count, room.rank, self.runtime.dtype, self.runtime.device)
-                where.update({built.spec.tensors[key]: (bank, part) for part, key in enumerate(keys)})
+                names = [built.spec.tensors[key] for key in keys]
+                twice.update(name for i, name in enumerate(names) if name in where or name in names[:i])
+                where.update({name: (bank, part) for part, name in enumerate(names)})
             built.part.banks = banks
+        for name in twice:
+            del where[name]
         return where
 
     def cache_needs(self) -> list:

@@ -399,7 +399,7 @@ class Stepper:
         n_rows, n_seqs = row, len(chosen)
         decode = all(n == 1 for _, _, n in chosen)
         # the maps of a longer pass, and the pages that it needs, are worked out on the device
-        by_lengths = hasattr(self.ops, "step_maps") and n_rows != n_seqs
+        by_lengths = hasattr(self.ops, "step_maps") and n_rows != n_seqs and n_seqs <= getattr(self.ops, "MOST_SEQUENCES", n_seqs)
         if not (by_lengths and pages is not None):
             cache.sync()
         if decode and self.use_graphs:

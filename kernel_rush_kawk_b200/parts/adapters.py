@@ -8,6 +8,7 @@ queries, keys and values) in fixed storage, so that variants come and go while c
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import torch
@@ -38,7 +39,12 @@ class AdapterBank:
 
     ``a`` [capacity, parts * rank, inputs], ``b`` [capacity, outputs, rank] (the rank rounded up to a multiple of eight), ``scale`` (float32)
     and ``ranks`` (int32) [capacity, parts]; a part whose rank is 0 is left as it is by the adapter. What lies behind an adapter's rank is never read as
-    a number."""
+    a number. The tensors stay the bank's own: they are filled by ``put``."""
+
+    a = property(lambda self: self._a)
+    b = property(lambda self: self._b)
+    scale = property(lambda self: self._scale)
+    ranks = property(lambda self: self._ranks)
 
     def __init__(self, inputs: int, outs, capacity: int, rank: int, dtype: torch.dtype, device):
         outs = (int(outs),) if isinstance(outs, int) else tuple(int(n) for n in outs)
@@ -55,10 +61,10 @@ class AdapterBank:
         self.dtype = dtype
         self.begin = [sum(outs[:i]) for i in range(len(outs) + 1)]
         parts = len(outs)
-        self.a = torch.zeros((capacity, parts * self.rank, self.inputs), dtype=dtype, device=device)
-        self.b = torch.zeros((capacity, self.outputs, self.rank), dtype=dtype, device=device)
-        self.scale = torch.zeros((capacity, parts), dtype=torch.float32, device=device)
-        self.ranks = torch.zeros((capacity, parts), dtype=torch.int32, device=device)
+        self._a = torch.zeros((capacity, parts * self.rank, self.inputs), dtype=dtype, device=device)
+        self._b = torch.zeros((capacity, self.outputs, self.rank), dtype=dtype, device=device)
+        self._scale = torch.zeros((capacity, parts), dtype=torch.float32, device=device)
+        self._ranks = torch.zeros((capacity, parts), dtype=torch.int32, device=device)
         self._described = None  # how the kernels are told (Kernels keeps it here)
 
     @property
@@ -73,18 +79,26 @@ class AdapterBank:
             raise AdapterError(f"adapter {index} of a bank of {self.capacity}")
         return index
 
-    def put(self, index: int, part: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
-        """Adapter ``index`` of ``part``: a [r, inputs], b [the part's outputs, r]. The copies are queued on the current stream, behind the steps that
-        were queued on it before."""
-        self._index(index)
+    def check(self, part: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
+        """Raise unless ``put`` takes them."""
         if not 0 <= part < self.parts:
             raise AdapterError(f"part {part} of a bank of {self.parts}")
         n = self.outs[part]
         if a.dim() != 2 or b.dim() != 2 or a.shape[1] != self.inputs or b.shape != (n, a.shape[0]):
             raise AdapterError(f"an adapter from {self.inputs} to {n} is [rank, {self.inputs}] and [{n}, rank], got {list(a.shape)} and {list(b.shape)}")
-        r = a.shape[0]
-        if not 1 <= r <= self.most:
-            raise AdapterError(f"an adapter of rank {r} in a bank of rank {self.most}")
+        if not 1 <= a.shape[0] <= self.most:
+            raise AdapterError(f"an adapter of rank {a.shape[0]} in a bank of rank {self.most}")
+        # rows of other adapters are multiplied by these factors as well, as zeros, and are to stay numbers
+        if not math.isfinite(scale) or not all(torch.isfinite(t.detach().to(self.dtype)).all() for t in (a, b)):
+            raise AdapterError(f"an adapter's factors and scale are finite numbers ({self.dtype})")
+
+    @torch.no_grad()
+    def put(self, index: int, part: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
+        """Adapter ``index`` of ``part``: a [r, inputs], b [the part's outputs, r], of finite numbers (which the host waits to know). The copies are queued
+        on the current stream, behind the steps that were queued on it before."""
+        self._index(index)
+        self.check(part, a, b, scale)
+        n, r = self.outs[part], a.shape[0]
         self.a[index, part * self.rank:part * self.rank + r].copy_(a)
         self.b[index, self.begin[part]:self.begin[part] + n, :r].copy_(b)
         if r < self.rank:

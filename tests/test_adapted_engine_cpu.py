@@ -2,6 +2,7 @@
 adapters read from files."""
 
 import json
+from dataclasses import replace
 
 import pytest
 import torch
@@ -13,6 +14,7 @@ from helpers import prompts_for
 from kernel_rush_kawk_b200 import AdapterError, AdapterRoom, Engine, KeyEviction, StepEntry
 from kernel_rush_kawk_b200.csrc.adapter_ops import StepMaps
 from kernel_rush_kawk_b200.engine.generate import shared_pages, shared_prefixes
+from kernel_rush_kawk_b200.engine.model import Model, PartTree
 from kernel_rush_kawk_b200.weights.adapters import read_adapter
 
 
@@ -225,6 +227,12 @@ def test_refusals(folders):
         with pytest.raises(AdapterError):
             AdapterRoom(*room)
     engine.load_adapter("x", factors)
+    said = engine.generate_all([[1, 2, 3]], 3, adapters="x")
+    last = list(factors)[-1]
+    broken = dict(factors) | {last: (factors[last][0], torch.full_like(factors[last][1], float("nan")), 1.0)}
+    with pytest.raises(AdapterError, match="finite"):
+        engine.load_adapter("x", broken)  # and what the name had before is all there
+    assert engine.generate_all([[1, 2, 3]], 3, adapters="x") == said
     with pytest.raises(AdapterError, match="2 adapters for 1"):
         engine.generate_all([[1, 2]], 2, adapters=["x", None])
     with pytest.raises(AdapterError):
@@ -292,3 +300,17 @@ def test_command_line(folders, tmp_path, capsys):
         with pytest.raises(SystemExit):
             main(base + more)
     capsys.readouterr()
+
+
+def test_a_weight_of_two_layers_takes_none(folders):
+    """Two layers that have one checkpoint tensor between them: an adapter would have to stand beside both."""
+    engine = make(folders)
+    plan = engine.plan
+    layers = list(plan.layers)
+    layers[1] = replace(layers[1], feed_forward=replace(layers[1].feed_forward, tensors=layers[0].feed_forward.tensors))
+    plan = replace(plan, layers=tuple(layers))
+    tensors = {name: torch.zeros(spec.shape) for name, spec in PartTree(plan).expected_tensors().items()}
+    where = Model(plan, engine.model.runtime, tensors).open_adapters(AdapterRoom(1, 4))
+    gone = set(engine._beside) - set(where)
+    assert gone == set(layers[0].feed_forward.tensors.values()) | set(engine.plan.layers[1].feed_forward.tensors.values()) and where
+

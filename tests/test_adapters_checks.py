@@ -59,6 +59,38 @@ def test_what_a_bank_takes():
             bank.put(*args)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_bank_holds_numbers(dtype):
+    """Rows of other adapters are multiplied by an adapter's factors too, as zeros: an infinity would make them none."""
+    bank = AdapterBank(8, (4, 6), 2, 5, dtype, "cpu")
+    a, b = torch.randn(5, 8), torch.randn(6, 5)
+    bank.put(0, 1, a, b, 0.5)
+    held = [t.clone() for t in (bank.a, bank.b, bank.scale, bank.ranks)]
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        for which in range(3):
+            args = [a.clone(), b.clone(), 1.0]
+            if which == 2:
+                args[2] = bad
+            else:
+                args[which][2, 3] = bad
+            with pytest.raises(AdapterError, match="finite"):
+                bank.put(0, 1, *args)
+    if dtype is torch.bfloat16:  # finite in 32 bits, and not in 16
+        with pytest.raises(AdapterError, match="finite"):
+            bank.put(0, 1, a, torch.full((6, 5), torch.finfo(torch.float32).max))
+    assert all(torch.equal(t, was) for t, was in zip((bank.a, bank.b, bank.scale, bank.ranks), held))
+
+
+def test_a_bank_keeps_its_tensors():
+    bank = AdapterBank(8, 4, 1, 4, torch.float32, "cpu")
+    for name in ("a", "b", "scale", "ranks"):
+        with pytest.raises(AttributeError):
+            setattr(bank, name, getattr(bank, name).clone())
+    a = torch.randn(4, 8, requires_grad=True)
+    bank.put(0, 0, a, torch.randn(4, 4))
+    assert torch.equal(bank.a[0, :4], a) and not bank.a.requires_grad
+
+
 def product(x=None, w=None, bank=None, rows=None, gated=0):
     x = torch.randn(3, 16) if x is None else x
     w = torch.randn(12, 16) if w is None else w
@@ -103,6 +135,8 @@ def test_too_many_sequences():
     many = torch.zeros(AdapterOps.MOST_SEQUENCES + 1, dtype=torch.int32)
     with pytest.raises(KernelError):
         Checks().step_maps(many, many, many, 0)
+    with pytest.raises(KernelError):
+        Checks().step_maps(many[:1], many[:1], many[:1], AdapterOps.MOST_ROWS + 1)
 
 
 def test_lists_have_room_for_every_tile():

@@ -114,7 +114,9 @@ def test_what_lies_behind_a_rank_is_no_number(ops, lengths):
     x, w, adapters, bank = case(6, torch.bfloat16, 128, (64, 64), lengths, None, 24, 2, skip={(0, 1)})
     big = make_adapters(torch.Generator().manual_seed(9), 1, 128, (64, 64), 24, torch.bfloat16, DEV)[0]
     for p in range(2):
-        bank.put(0, p, big[p][0] * float("inf"), big[p][1] * float("nan"), 1.0)
+        bank.put(0, p, big[p][0], big[p][1], 1.0)
+    bank.a[0].fill_(float("inf"))
+    bank.b[0].fill_(float("nan"))
     bank.clear(0)
     small = (adapters[0][0][0][:3].contiguous(), adapters[0][0][1][:, :3].contiguous(), 1.5)
     bank.put(0, 0, *small)
@@ -345,4 +347,50 @@ def test_maps_in_a_captured_step(ops):
         assert maps.cu_q.tolist() == cu and maps.row_seq.tolist() == seq and maps.row_pos.tolist() == pos and maps.row_place.tolist() == place
         assert maps.adapters.row_adapter.tolist() == at and table.tolist() == host
         check_lists(maps.adapters, [0, 1, 2, 3], n)
+    ops.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lengths", [[1], [1] * 16, [1] * 33, [100, 1, 180]])
+@pytest.mark.parametrize("outs,rank", [((64, 40, 24, 8), 130), ((128, 64), 256), ((264,), 200), ((16, 16, 16, 16), 72)])
+def test_large_ranks_and_many_parts(ops, dtype, lengths, outs, rank):
+    of = spread(lengths, 3)
+    x, w, adapters, bank = case(15, dtype, 192, outs, lengths, of, rank, 3, skip={(0, len(outs) - 1)})
+    got = ops.adapted_linear(x, w, bank, rows_of_step(ops, lengths, of, DEV))
+    assert_within(got, *product64(x, w, adapters, outs, per_row(lengths, of), True))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("length", [1, 3])
+def test_a_thousand_sequences(ops, dtype, length):
+    lengths, of = [length] * 1000, spread([1] * 1000, 150, 7)
+    x, w, adapters, bank = case(16, dtype, 96, (72, 24), lengths, of, 8, 150)
+    got = ops.adapted_linear(x, w, bank, rows_of_step(ops, lengths, of, DEV))
+    assert_within(got, *product64(x, w, adapters, (72, 24), per_row(lengths, of), True))
+
+
+def test_two_streams_at_once(ops):
+    """Products of every kind on two streams, side by side: the bits of one after the other."""
+    calls = []
+    for seed, dtype, lengths, K, outs in [(17, torch.bfloat16, [700, 300], 2048, (1024, 512)), (18, torch.bfloat16, [1] * 64, 2048, (2048,)),
+                                          (19, torch.bfloat16, [1] * 8, 2048, (2048,)), (20, torch.float32, [1] * 6, 1024, (1024,)),
+                                          (21, torch.bfloat16, [513], 1024, (256,)), (22, torch.bfloat16, [1] * 200, 1024, (4096,))]:
+        of = spread(lengths, 4)
+        x, w, _, bank = case(seed, dtype, K, outs, lengths, of, 16, 4)
+        rows = rows_of_step(ops, lengths, of, DEV)
+        calls.append(lambda x=x, w=w, bank=bank, rows=rows: ops.adapted_linear(x, w, bank, rows))
+    expected = [call() for call in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for turn in range(12):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                for j in range(len(calls)):
+                    which = (j + 3 * i + turn) % len(calls)
+                    got[i].append((which, calls[which]()))
+    torch.cuda.synchronize()
+    for results in got:
+        for which, y in results:
+            assert torch.equal(y, expected[which])
     ops.check()
