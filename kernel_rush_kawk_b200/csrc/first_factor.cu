@@ -8,10 +8,39 @@ namespace {
 
 using namespace tc;
 
-// The first factor of many requests' adapters, t = scale (x A^T), sums in 32 bits on the tensor cores. rounded to bfloat16. Two forms of t: of every slot,
-// [slot][tile_rows][parts * wide], zeros where a row has another adapter than the slot's (COMPACT false); of every row, [rows][parts * wide], where it has an adapter. A cluster has 128 rows of a slot's tile (y), 64 or 128 of the
-// adapter's ranks, all parts' side by side (z), and its `ways` blocks share k. A block multiplies its part of k on the tensor cores (fed by TMA in blocks of 64 k); each block sends its sums of every block's share of the rows to that block's shared
-// memory, in 32 bits, which adds them in the blocks' order and writes its rows.
+// The four products of a block of 64 k, and its place's release, by a whole warp.
+__device__ __forceinline__ void umma_stage_warp(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate, uint64_t* release) {
+  asm volatile(
+      "{\n.reg .pred p, q, t;\n.reg .b64 a1, a2, a3, b1, b2, b3;\n"
+      "elect.sync _|q, 0xffffffff;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "setp.eq.b32 t, 0, 0;\n"
+      "add.u64 a1, %1, 2;\nadd.u64 a2, %1, 4;\nadd.u64 a3, %1, 6;\n"
+      "add.u64 b1, %2, 2;\nadd.u64 b2, %2, 4;\nadd.u64 b3, %2, 6;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n}"
+      ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(smem_u32(release))
+      : "memory");
+}
+
+// The first factor of many requests' adapters, t = scale (x A^T), sums in 32 bits on the tensor cores, rounded to bfloat16 (half a step of 2^-8 of a sum that is itself
+// a part of the result, which is rounded the same way). Two forms of t: of every slot, [slot][tile_rows][parts * wide], zeros where a row has another adapter
+// than the slot's (COMPACT false); of every row, [rows][parts * wide], where it has an adapter.
+//
+// A cluster has 128 rows of a slot's tile (y) and 64 or 128 of the adapter's ranks, all parts' side by side (z), and its `ways` blocks share k. A block multiplies
+// its part of k on the tensor cores, fed by TMA in blocks of 64; it sends its sums of every block's share of the rows to that block's shared memory, in 32
+// bits, which adds them in the blocks' order and writes its rows. So a sum's order depends on sizes and on the number of slots alone.
+//
+// What it costs. It has to read x and the used adapters' A: 2,001 rows of 4,096 are 16 MB, 2.5 us. One cold call of that, rank 16 of three parts, 108
+// blocks: 17,700 clocks (9 us) of which the blocks of k take 4,400, 400 each; before them come the wait, tensor memory, the slot and its rows' adapters (4,300) and the
+// first copies' way (3,000 with the products behind it), after them the sums' way to their block (2,300), the clusters' meeting (1,700) and the writing (1,800). Long
+// runs of k (9,728, 75 blocks): 343 clocks a block of k of four products, a stage's way round and not its bytes: neither copies of only the groups
+// of 32 rows that have the adapter (two a block of k: 125 -> 128 us of 2,268 rows with the product; one of 32 or 64 rows: no difference) nor eight places for five
+// changed it; places and parities counted instead of divided, and a block's four products asked for at once, took 2,400 rows of 60 requests from 152 to 137 us.
+// By single lanes a block of k took 700 clocks.
 //
 // The product's blocks come in while these run, once what came before is over, and wait for t where they need it; so a ring of few blocks of k is no
 // larger than fits beside theirs.
@@ -76,31 +105,40 @@ first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_do
   if (has) {  // the same for the whole cluster
     const uint32_t bytes = (uint32_t)(box_rows + box_ranks) * 128;
     if (warp == 0) {
+      int s = 0;
+      uint32_t parity = 1;  // (the first round's places are free)
       for (int b = b0; b < b1; ++b) {
-        const int i = b - b0, s = i % stages;
-        if (i >= stages && !__all_sync(0xffffffffu, mbar_wait(empty_bar + s, (i / stages - 1) & 1))) {
+        if (!__all_sync(0xffffffffu, mbar_wait(empty_bar + s, parity))) {
           if (lane == 0) {
             atomicExch(error, 3);
-            asked_for = i;
+            asked_for = b - b0;
           }
           break;
         }
         const uint32_t stage = smem_u32(ring) + s * bytes, bar = smem_u32(full_bar + s);
         two_loads_warp(stage, &map_x, b * 64, r0, stage + box_rows * 128, &map_a, b * 64, a * per_adapter + n0, bar, bytes);
+        if (++s == stages) {
+          s = 0;
+          parity ^= 1;
+        }
       }
     } else if (warp == 1) {
       const uint32_t idesc = umma_idesc(128, box_ranks);  // (rows beyond the copies' give rows that nobody reads)
+      const uint64_t x_desc = umma_desc(ring), a_desc = umma_desc(ring + box_rows * 128);
+      int s = 0;
+      uint32_t parity = 0;
       for (int b = b0; b < b1; ++b) {
-        const int i = b - b0, s = i % stages;
-        if (!__all_sync(0xffffffffu, mbar_wait(full_bar + s, (i / stages) & 1))) {
+        if (!__all_sync(0xffffffffu, mbar_wait(full_bar + s, parity))) {
           if (lane == 0) atomicExch(error, 4);
           break;
         }
         tc_fence_after();
-        const uint64_t x_desc = umma_desc(ring + s * bytes), a_desc = umma_desc(ring + s * bytes + box_rows * 128);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) umma_bf16_warp(acc, x_desc + k * 2, a_desc + k * 2, idesc, (b > b0 || k > 0) ? 1u : 0u);
-        umma_commit_warp(empty_bar + s);
+        const uint64_t at = s * (bytes >> 4);
+        umma_stage_warp(acc, x_desc + at, a_desc + at, idesc, b > b0, empty_bar + s);
+        if (++s == stages) {
+          s = 0;
+          parity ^= 1;
+        }
       }
       umma_commit_warp(&acc_bar);  // arrives even after a failed wait, so that all move on
     }
