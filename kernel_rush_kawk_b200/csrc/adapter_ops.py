@@ -203,18 +203,31 @@ class AdapterOps:
     @staticmethod
     @lru_cache(maxsize=4096)
     def _tiling(heights, M: int, K: int, N: int) -> tuple[int, int]:
-        """(which of the rows' tile heights, the first tile that the pairs share): by the time of whole rounds of the pairs, or of whole rounds
-        and shares of what is left, in clocks."""
-        if len(heights) == 1:
+        """(which of the rows' tile heights, the first tile that the pairs share): whole rounds of the pairs, or whole rounds and shares of what is left, by
+        their time in clocks. Up to 128 rows W's bytes are the cost, and all pairs share all tiles: 64 rows of 2,560 x 6,144 22.5 us, as whole tiles
+        24.6, of 9,728 x 2,560 26.6 and 53.2; 128 rows 25.9 and 27.3, 32.8 and 61.4.
+
+        Above, a round takes what a block of k takes of a pair, 380 clocks and half a clock a row, and shares take the way to memory and back, as many times as
+        a tile has pairs; a row tile takes its first factor. The constants come from six shapes (K and N of 2,560 to 9,728 and 19,456), 160 to 4,096 rows, every
+        height with shares and without: what this picks is 0.5 % behind the fastest on average, 8 % at worst. Cold, us, whole and shares: 256 rows of 2,560 x
+        6,144 27.3 and 32.8, of 9,728 x 2,560 57.3 and 45.1; 2,268 rows of that, tiles of 256, 124.9 and 110.6; 400 rows of 2,560 x 6,144 in tiles of 256 26.6 and
+        38.9, of 192 30.7, of 128 38.9; 512 rows of 2,560 x 19,456 61.4 and 86."""
+        if len(heights) == 1 and heights[0] <= 128:
             return 0, 0
         best = None
         for i, h in enumerate(heights):
-            tiles = -(-M // h) * -(-N // 256)
-            tile = -(-K // 64) * (176 + 1.3125 * h)
-            whole, rest = divmod(tiles, AdapterOps.PAIRS)
-            for cost, shared in (((whole + (rest > 0)) * tile, tiles), (whole * tile + rest / AdapterOps.PAIRS * tile + 6000 + (AdapterOps.PAIRS + rest) * h / 2, tiles - rest)):
+            row_tiles = -(-M // h)
+            tiles = row_tiles * -(-N // 256)
+            tile = -(-K // 64) * (380 + 0.516 * h)
+            shared = tiles // AdapterOps.PAIRS * AdapterOps.PAIRS if len(heights) > 1 else 0
+            rest = tiles - shared
+            options = [(-(-tiles // AdapterOps.PAIRS) * tile, tiles)]
+            if rest:
+                options.append(((shared + rest) / AdapterOps.PAIRS * tile + 8000 + 24 * h * (2 + AdapterOps.PAIRS / rest), shared))
+            for cost, first in options:
+                cost += 4000 * row_tiles
                 if best is None or cost < best[0]:
-                    best = cost, i, shared
+                    best = cost, i, first
         return best[1], best[2]
 
     def _adapted(self, what, x, w, bank, rows, gated):
