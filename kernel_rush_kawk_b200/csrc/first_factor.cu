@@ -27,8 +27,8 @@ __device__ __forceinline__ void umma_stage_warp(uint32_t tmem_d, uint64_t a_desc
 }
 
 // The first factor of many requests' adapters, t = scale (x A^T), sums in 32 bits on the tensor cores, rounded to bfloat16 (half a step of 2^-8 of a sum that is itself
-// a part of the result, which is rounded the same way). Two forms of t: of every slot, [slot][tile_rows][parts * wide], zeros where a row has another adapter
-// than the slot's (COMPACT false); of every row, [rows][parts * wide], where it has an adapter.
+// a part of the result, which is rounded the same way). t is of every slot,
+// [slot][tile_rows][parts * wide], zeros where a row has another adapter than the slot's.
 //
 // A cluster has 128 rows of a slot's tile (y) and 64 or 128 of the adapter's ranks, all parts' side by side (z), and its `ways` blocks share k. A block multiplies
 // its part of k on the tensor cores, fed by TMA in blocks of 64; it sends its sums of every block's share of the rows to that block's shared memory, in 32
@@ -47,7 +47,6 @@ __device__ __forceinline__ void umma_stage_warp(uint32_t tmem_d, uint64_t a_desc
 constexpr int FIRST_RANKS = 128, FIRST_STAGES = 8, FIRST_THREADS = 192;
 constexpr int FIRST_BYTES = 96 * 1024, FIRST_DEEP_BYTES = 160 * 1024;  // of shared memory, beside the product's blocks and alone
 
-template <bool COMPACT>
 __global__ void __launch_bounds__(FIRST_THREADS, 5)  // (of three that an SM's memory takes: in 64 registers they fit beside the product's)
 first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_done, const __grid_constant__ CUtensorMap map_x,
                                                                            const __grid_constant__ CUtensorMap map_a, int K,
@@ -171,7 +170,6 @@ first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_do
   }
   leave();  // (nobody who holds tensor memory waits for another block's end)
   if (has && ways > 1) cluster_sync();
-  if (COMPACT && !has) return;
   // eight ranks of a row a thread
   const int first_row = way * share, rows = min(share, here - first_row), groups = box_ranks / 8;
   const int width = bank.parts * bank.wide;
@@ -193,21 +191,114 @@ first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_do
       for (int i = 0; i < 8; ++i) v[i] = j + i < rank ? v[i] * scale : 0.f;
       pack = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
     }
-    else if (COMPACT) continue;
-    bf16* to = t + (COMPACT ? (size_t)(r0 + row) : (size_t)slot * tiles.tile_rows + blockIdx.y * 128 + row) * width + part * bank.wide + j;
+    bf16* to = t + ((size_t)slot * tiles.tile_rows + blockIdx.y * 128 + row) * width + part * bank.wide + j;
     *reinterpret_cast<uint4*>(to) = pack;
     if (j + 8 == bank.rank && bank.wide > bank.rank) *reinterpret_cast<uint4*>(to + 8) = make_uint4(0, 0, 0, 0);  // the product takes whole steps of sixteen
   }
+}
+
+// The same for adapters that few rows have each, of one tile: memory is what bounds it, and neither tensor memory nor clusters are worth their way. A block has 16 of a
+// slot's ranks and all of k, a warp a part of it, five blocks of 32 k on their way to registers at a time; the ranks are a product's M, up to 16 of the
+// adapter's rows, wherever they are, its N. The warps' sums are added in order: a sum's order depends on K alone.
+//
+// COMPACT: t of every row, for up to 16 rows (the tiles' form served these before: 16 rows with nine adapters of rank 16, the product with it, cold, 9,728 x 2,560 24.6 us
+// and 20.5 here, 4,096 x 2,560 18.4 and 16.4; one row of 2,560 x 6,144 14.3 and 14.3; sixteen adapters of rank 64 beside 4,096 x 24,576 61 and 65). By eight
+// warps a long k takes more rounds of loads: one row of 9,728 x 2,560 22.5, by sixteen 18.4.
+constexpr int FEW_DEEP = 5, FEW_RANKS = 16;
+
+template <bool COMPACT, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, 16 / WARPS)
+first_factor_few_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_done, const bf16* __restrict__ x, long long ldx, int K, const __grid_constant__ AdapterBank bank,
+                        const __grid_constant__ AdapterTiles tiles) {
+  __shared__ float sums[WARPS][FEW_RANKS][17];
+  __shared__ int list[256], listed;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  if (blockIdx.x + blockIdx.y == 0)
+    for (int i = tid; i < n_done; i += 32 * WARPS) done[i] = 0;
+  const int slot = blockIdx.y, a = tiles.slots[2 * slot], rows = min(tiles.rows, tiles.tile_rows);
+  if (a < 0 || a >= bank.capacity) return;  // (the product says so)
+  if (warp == 0) {
+    int n = 0;
+    for (int r = lane; r - lane < rows; r += 32) {
+      const bool has = r < rows && tiles.row_adapter[r] == a;
+      const unsigned all = __ballot_sync(0xffffffffu, has);
+      if (has) list[n + __popc(all & ((1u << lane) - 1))] = r;
+      n += __popc(all);
+    }
+    if (lane == 0) listed = n;
+  }
+  __syncthreads();
+  const int n = listed, i0 = blockIdx.x * FEW_RANKS, per = bank.parts * bank.rank, width = bank.parts * bank.wide;
+  const bf16* w = reinterpret_cast<const bf16*>(bank.a) + ((size_t)a * per + i0 + g) * K + 8 * q;
+  const bool w0_there = i0 + g < per, w1_there = i0 + g + 8 < per;
+  const int chunks = (K + 31) / 32, each = (chunks + WARPS - 1) / WARPS, c1 = min(chunks, (warp + 1) * each);
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  bf16* to = t + (COMPACT ? 0 : (size_t)slot * tiles.tile_rows * width);
+  for (int m0 = 0; m0 < n; m0 += 16) {
+    const int row[2] = {m0 + g < n ? list[m0 + g] : -1, m0 + 8 + g < n ? list[m0 + 8 + g] : -1};
+    const bf16* from[2] = {x + max(row[0], 0) * ldx + 8 * q, x + max(row[1], 0) * ldx + 8 * q};
+    float acc[2][4] = {};
+    for (int c = warp * each; c < c1; c += FEW_DEEP) {
+      uint4 w4[FEW_DEEP][2], x4[FEW_DEEP][2];
+#pragma unroll
+      for (int d = 0; d < FEW_DEEP; ++d) {
+        const int k = (c + d) * 32;
+        const bool in = c + d < c1 && k + 8 * q < K;
+        w4[d][0] = in && w0_there ? ld_stream_16(w + k) : zero;
+        w4[d][1] = in && w1_there ? ld_stream_16(w + (size_t)8 * K + k) : zero;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) x4[d][h] = in && row[h] >= 0 ? __ldcg(reinterpret_cast<const uint4*>(from[h] + k)) : zero;
+      }
+#pragma unroll
+      for (int d = 0; d < FEW_DEEP; ++d)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          mma_bf16_16816(acc[h], w4[d][0].x, w4[d][1].x, w4[d][0].y, w4[d][1].y, x4[d][h].x, x4[d][h].y);
+          mma_bf16_16816(acc[h], w4[d][0].z, w4[d][1].z, w4[d][0].w, w4[d][1].w, x4[d][h].z, x4[d][h].w);
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sums[warp][g + c / 2 * 8][8 * h + 2 * q + c % 2] = acc[h][c];
+    __syncthreads();
+    const int i = tid % FEW_RANKS, m = tid / FEW_RANKS;
+    if (m < 16 && m0 + m < n && i0 + i < per) {
+      float sum = 0.f;
+#pragma unroll
+      for (int s = 0; s < WARPS; ++s) sum += sums[s][i][m];
+      const int part = (i0 + i) / bank.rank, j = (i0 + i) % bank.rank;
+      bf16* at = to + (size_t)list[m0 + m] * width + part * bank.wide + j;
+      *at = __float2bfloat16_rn(j < bank.ranks[a * bank.parts + part] ? sum * bank.scale[a * bank.parts + part] : 0.f);
+      if (j + 8 >= bank.rank && bank.wide > bank.rank) at[8] = __float2bfloat16_rn(0.f);  // the product takes whole steps of sixteen
+    }
+    __syncthreads();
+  }
+  if constexpr (!COMPACT)
+    for (int o = tid; o < 2 * rows; o += 32 * WARPS) {
+      const int i = i0 + o % 2 * 8, r = o / 2;
+      if (i >= per || tiles.row_adapter[r] == a) continue;
+      bf16* at = to + (size_t)r * width + i / bank.rank * bank.wide + i % bank.rank;
+      *reinterpret_cast<uint4*>(at) = zero;
+      if (i % bank.rank + 8 == bank.rank && bank.wide > bank.rank) *reinterpret_cast<uint4*>(at + 8) = zero;
+    }
+}
+
+template <bool COMPACT, int WARPS>
+int launch_few(bf16* t, int* done, int n_done, const bf16* x, long long ldx, int K, const AdapterBank& bank, const AdapterTiles& tiles, cudaStream_t stream) {
+  const dim3 grid((bank.parts * bank.rank + FEW_RANKS - 1) / FEW_RANKS, min(tiles.n_slots, bank.capacity));
+  return (int)launch_pdl(first_factor_few_kernel<COMPACT, WARPS>, grid, dim3(32 * WARPS), 0, stream, t, done, n_done, x, ldx, K, bank, tiles);
 }
 
 // rows and ranks of a copy of the first factor's: as many as there are (64 of the ranks where the rows are many: the sums of both have their place in shared memory)
 int first_rows(const AdapterTiles& tiles) { return min(128, (min(tiles.rows, tiles.tile_rows) + 7) / 8 * 8); }
 int first_ranks(const AdapterBank& bank, const AdapterTiles& tiles) { return min(first_rows(tiles) > 64 ? 64 : FIRST_RANKS, (bank.parts * bank.rank + 15) / 16 * 16); }
 
-template <bool COMPACT>
 int launch_first(bf16* t, int* done, int n_done, const CUtensorMap& map_x, const CUtensorMap& map_a, int K, const AdapterBank& bank, const AdapterTiles& tiles, int* error,
                  cudaStream_t stream) {
-  auto kern = first_factor_tiles_kernel<COMPACT>;
+  auto kern = first_factor_tiles_kernel;
   // an SM gives its memory to L1 or to blocks anew only when it is empty: split as the product's blocks need it, they come in beside these
   static unsigned long long told = 0, allowed = 0;
   int device = 0;
@@ -259,10 +350,15 @@ int krk_first_factor(void* t, bool compact, int* done, int n_done, const void* x
                      cudaStream_t stream) {
   const long long rows = (long long)bank.capacity * bank.parts * bank.rank;
   if (rows > 0x7fffffffLL || (long long)tiles.n_slots * 8 > 0x7fffffffLL) return -3;
+  if (compact) return launch_few<true, 16>((bf16*)t, done, n_done, (const bf16*)x, ldx, K, bank, tiles, stream);
+  // A tile of more than 128 rows with many slots, which blocks of the other kernel would take all of an SM's memory for, the product's blocks behind them: 256 rows of
+  // 9,728 x 2,560 with 120 adapters of rank 16 105 us cold, 61 here; 32 adapters 57 and 55, of 2,560 x 6,144 45 and 37; 160 rows with 64 of rank 64 70 and
+  // 53, of 4,096 x 2,560 55 and 64; with eight adapters, of 9,728 x 2,560, 49 and 59.
+  if (tiles.rows <= tiles.tile_rows && tiles.tile_rows > 128 && min(tiles.n_slots, bank.capacity) >= 24)
+    return launch_few<false, 8>((bf16*)t, done, n_done, (const bf16*)x, ldx, K, bank, tiles, stream);
   CUtensorMap map_x, map_a;
   int rc = make_map_bf16(&map_x, x, tiles.rows, K, ldx, first_rows(tiles));
   if (!rc) rc = make_map_bf16(&map_a, bank.a, rows, K, K, first_ranks(bank, tiles));
   if (rc) return rc;
-  return compact ? launch_first<true>((bf16*)t, done, n_done, map_x, map_a, K, bank, tiles, error, stream)
-                 : launch_first<false>((bf16*)t, done, n_done, map_x, map_a, K, bank, tiles, error, stream);
+  return launch_first((bf16*)t, done, n_done, map_x, map_a, K, bank, tiles, error, stream);
 }
