@@ -6,6 +6,14 @@
 // The first factor's kernel (first_factor.cu) makes t, rounded to bfloat16 (half a step of 2^-8 of a sum that is itself a part of the result, which is
 // rounded the same way).
 //
+// Bound by the tensor cores for many rows and by W's bytes for few. Cold, with the first factor's kernel: 2,001 rows of one prompt, rank 16, 4,096 x 6,144 82 us
+// (101 GFLOP, 61 us at the measured peak; the library's product alone 79 at the power limit, this 94), 3,963 rows with gate and up of 2,560 x 19,456
+// 272 (239), nine prompts, 2,103 rows, of 9,728 x 2,560 with adapters of rank 64 96 (63). By counters the tensor pipe is busy for 80 to 86 % of the product's cycles; before it
+// comes the first factor, 9 to 17 us, which takes all of the SMs' memory there. 64 rows of 2,560 x 6,144: eight adapters 18.4 us, sixty of rank up to 32 26 (41 MB,
+// 6.2 us), all of rank 32 33 (84 MB, 12.9 us): an adapter is a stage of the ring whatever its rank, some 900 clocks of 256 rows, 400 of 64. (Sums left in 32 bits and the second factors by
+// mma.sync in a kernel behind, 16 columns of eight rows a warp: 256 rows with 120 adapters gained, 95 -> 67 us, most others lost, 64 rows
+// with eight 23.6 -> 28.7, since every eight rows read their adapters' B again.)
+//
 // adapted_gemm_kernel works in pairs of blocks (cta_group::2): 256 rows of W are the product's M, half of them in each block's shared memory, and a
 // tile's rows, 32 to 256, its N. So a product costs what it has rows, in steps of 32, and W passes once for up to 256 of them. Pairs stay
 // and walk the tiles; an accumulator is half of tensor memory, so that one tile is read back while the next is multiplied.

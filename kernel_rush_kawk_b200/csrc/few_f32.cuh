@@ -1,9 +1,8 @@
 // Up to 16 float32 rows times a matrix of float32 weights, every sum one chain of multiply-adds over k, on the CUDA cores.
 //
-// Bound by the weights' bytes: each is read once, by bulk copies a slice or two ahead; a
-// thread owns one or two output columns of one or two rows. One row of 151,936 x 2,560: 235 us, 6.6 TB/s; three rows 226,
-// of 2,560 x 9,728 35 us, where the chain of K multiply-adds is the bound (20 us at four clocks each; copies of 16 bytes by
-// all threads: 265 and 46; the general kernel: 1.9 ms and 570 us of 2,560 x 4,096).
+// Bound by the weights' bytes: each is read once, by bulk copies a slice or two ahead; a thread owns one or two output columns of one or two
+// rows. One row of 151,936 x 2,560: 235 us, 6.6 TB/s; three rows 226, of 2,560 x 9,728 35 us, where the chain of K multiply-adds is the bound
+// (20 us at four clocks each; copies of 16 bytes by all threads: 265 and 46; the general kernel: 1.9 ms and 570 us of 2,560 x 4,096).
 //
 // `More` is what a program puts behind the sums (nothing: NoMore): ask() at a block's beginning, wait() and add() at its end.
 #pragma once

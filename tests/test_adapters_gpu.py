@@ -394,3 +394,22 @@ def test_two_streams_at_once(ops):
         for which, y in results:
             assert torch.equal(y, expected[which])
     ops.check()
+
+
+@pytest.mark.parametrize("lengths", [[1] * 200, [9] * 28, [100] + [1] * 60, [1] * 129])
+@pytest.mark.parametrize("K,outs,rank", [(72, (64, 40), 24), (5000, (96,), 8), (640, (128, 128), 64)])
+def test_large_tiles_with_many_adapters(ops, lengths, K, outs, rank):
+    """One tile of 129 to 256 rows whose slots are many: adapters of one row and of a hundred, unequal parts of k."""
+    of = spread(lengths, 29, 5)
+    x, w, adapters, bank = case(23, torch.bfloat16, K, outs, lengths, of, rank, 29, skip={(2, 0)})
+    got = ops.adapted_linear(x, w, bank, rows_of_step(ops, lengths, of, DEV))
+    assert_within(got, *product64(x, w, adapters, outs, per_row(lengths, of), True))
+
+
+@pytest.mark.parametrize("rows", [1, 7, 16])
+@pytest.mark.parametrize("K,outs,rank", [(64, (48,), 8), (9728, (40, 24), 40), (2592, (64, 64, 64), 16)])
+def test_few_rows_and_every_length_of_k(ops, rows, K, outs, rank):
+    lengths, of = [1] * rows, spread([1] * rows, 4, 6)
+    x, w, adapters, bank = case(24, torch.bfloat16, K, outs, lengths, of, rank, 4, skip={(1, 0)})
+    step = rows_of_step(ops, lengths, of, DEV)
+    assert_within(ops.adapted_linear(x, w, bank, step), *product64(x, w, adapters, outs, of, True))
