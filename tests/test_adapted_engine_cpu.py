@@ -314,3 +314,14 @@ def test_a_weight_of_two_layers_takes_none(folders):
     gone = set(engine._beside) - set(where)
     assert gone == set(layers[0].feed_forward.tensors.values()) | set(engine.plan.layers[1].feed_forward.tensors.values()) and where
 
+
+def test_passes_of_more_sequences_than_the_maps_take(folders):
+    """Their rows are described by the host, as where there are no such maps."""
+    ops = AdapterTorchOps()
+    engine = make(folders, ops=ops)
+    prompts = prompts_for(NAME, [9, 70, 4], 8)
+    expected = engine.generate_all(prompts, 3)
+    made = ops.calls["maps"]
+    assert made > 0
+    ops.MOST_SEQUENCES = 2
+    assert engine.generate_all(prompts, 3) == expected and ops.calls["maps"] == made
