@@ -413,3 +413,28 @@ def test_few_rows_and_every_length_of_k(ops, rows, K, outs, rank):
     x, w, adapters, bank = case(24, torch.bfloat16, K, outs, lengths, of, rank, 4, skip={(1, 0)})
     step = rows_of_step(ops, lengths, of, DEV)
     assert_within(ops.adapted_linear(x, w, bank, step), *product64(x, w, adapters, outs, of, True))
+
+
+def test_two_graphs_side_by_side(ops):
+    """Captured products of many and of few rows over one bank, replayed on two streams at once: neither's scratch is the other's."""
+    graphs = []
+    for seed, lengths in ((25, [400, 330]), (26, [1] * 70), (27, [1] * 12), (28, [1] * 230)):
+        of = spread(lengths, 4)
+        x, w, _, bank = case(29, torch.bfloat16, 1024, (1024, 256), lengths, of, 16, 4)
+        rows = rows_of_step(ops, lengths, of, DEV)
+        expected = ops.adapted_linear(x, w, bank, rows)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = ops.adapted_linear(x, w, bank, rows)
+        graphs.append((graph, y, expected, x, w, bank, rows))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(20):
+        for stream, (graph, y, *_) in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                y.zero_()
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, y, expected, *_ in graphs:
+        assert torch.equal(y, expected)
+    ops.check()
