@@ -10,7 +10,8 @@
 // (101 GFLOP, 61 us at the measured peak; the library's product alone 79 at the power limit, this 94), 3,963 rows with gate and up of 2,560 x 19,456
 // 272 (239), nine prompts, 2,103 rows, of 9,728 x 2,560 with adapters of rank 64 96 (63). By counters the tensor pipe is busy for 80 to 86 % of the product's cycles; before it
 // comes the first factor, 9 to 17 us, which takes all of the SMs' memory there. 64 rows of 2,560 x 6,144: eight adapters 18.4 us, sixty of rank up to 32 26 (41 MB,
-// 6.2 us), all of rank 32 33 (84 MB, 12.9 us): an adapter is a stage of the ring whatever its rank, some 900 clocks of 256 rows, 400 of 64. (Sums left in 32 bits and the second factors by
+// 6.2 us), all of rank 32 33 (84 MB, 12.9 us): an adapter is a stage of the ring whatever its rank, some 600 clocks of its
+// producer, whatever it loads (boxes as narrow as the rank, swizzled within 32 or 64 bytes, changed nothing). (Sums left in 32 bits and the second factors by
 // mma.sync in a kernel behind, 16 columns of eight rows a warp: 256 rows with 120 adapters gained, 95 -> 67 us, most others lost, 64 rows
 // with eight 23.6 -> 28.7, since every eight rows read their adapters' B again.)
 //
@@ -225,11 +226,13 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
     int s = 0, asked = 0;
     uint32_t parity = 1;  // of the round before: a first round finds its stages empty
     bool ok = true;
-    const uint32_t bytes = 2 * stage_bytes, ring_at = smem_u32(ring), steps_at = smem_u32(const_cast<int*>(steps)), own_full = smem_u32(full_bar);
-    const uint32_t first_full = cluster_address(full_bar, 0);
-    uint32_t stage, bar;
+    const uint32_t ring_at = smem_u32(ring), steps_at = smem_u32(const_cast<int*>(steps)), own_full = smem_u32(full_bar), first_full = cluster_address(full_bar, 0);
+    uint32_t stage;
+    PairStage to;
+    to.bytes = 2 * stage_bytes;
+    to.expects = rank == 0;
     // a stage to fill
-    auto enter = [&](int what) {
+    auto enter = [&] {
       if (!__all_sync(0xffffffffu, mbar_wait(empty_bar + s, parity))) {
         if (lane == 0) {
           atomicExch(error, 3);
@@ -237,18 +240,19 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
         }
         return ok = false;
       }
-      if (rank == 0) expect_with_word_warp(own_full + 8 * s, bytes, steps_at + 4 * s, what);
       stage = ring_at + s * stage_bytes;
-      bar = first_full + 8 * s;
+      to.bar = first_full + 8 * s;
+      to.own_bar = own_full + 8 * s;
+      to.word_at = steps_at + 4 * s;
       ++asked;
       if (++s == stages) { s = 0; parity ^= 1; }
       return true;
     };
-    auto shared_block = [&](int kb, int f0, int m0) {
-      if (GATED) tma_load_3d_pair_warp(stage, &maps.w, bar, kb * BK, 0, f0);
-      else tma_load_2d_pair_warp(stage, &maps.w, bar, kb * BK, f0);
-      tma_load_2d_pair_warp(stage + W_BYTES, &maps.x, bar, kb * BK, m0);
+    auto shared_block = [&](int what, int kb, int f0, int m0) {
+      if (GATED) stage_3d_2d_warp(to, what, stage, &maps.w, kb * BK, 0, f0, stage + W_BYTES, &maps.x, kb * BK, m0);
+      else stage_2d_2d_warp(to, what, stage, &maps.w, kb * BK, f0, stage + W_BYTES, &maps.x, kb * BK, m0);
     };
+    bool waited = false;
     while (ok && walk.next(t, k0, k1, e0, e1)) {
       const int rt = t % row_tiles, wt = t / row_tiles, f0 = (wt * 2 + (int)rank) * BC, m0 = rt * tiles.tile_rows + (int)rank * half;
       const int first = tiles.info[2 * rt], count = tiles.info[2 * rt + 1];
@@ -277,23 +281,24 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
         left += __reduce_add_sync(0xffffffffu, n);
       }
       for (int kb = k0; kb < k1; ++kb) {
-        if (!enter(4 | (kb + 1 == k1 && left == 0 ? 256 : 0))) break;
-        shared_block(kb, f0, m0);
+        if (!enter()) break;
+        shared_block(4 | (kb + 1 == k1 && left == 0 ? 256 : 0), kb, f0, m0);
       }
       // a share of adapters that leave these columns as they are: zeros from behind the last k
-      if (ok && k0 >= k1 && left == 0 && enter(1 | 256)) shared_block(k_blocks, f0, m0);
+      if (ok && k0 >= k1 && left == 0 && enter()) shared_block(1 | 256, k_blocks, f0, m0);
       for (int i = e0; i < e1 && ok; ++i) {
         if ((i - e0) % 32 == 0) look(i);
-        grid_dependency_wait();  // t
+        if (!waited) grid_dependency_wait();  // t
+        waited = true;
         const int ai = __shfl_sync(0xffffffffu, a, (i - e0) % 32);
         const uint32_t of = __shfl_sync(0xffffffffu, ranks, (i - e0) % 32);
         for (int p = p0; p < p1 && ok; ++p)
           for (int r = of >> 8 * p & 255, kb = 0; r > 0; r -= 4, ++kb) {
             --left;
-            if (!enter(min(r, 4) | (left == 0 ? 256 : 0))) break;
-            if (GATED) tma_load_4d_pair_warp(stage, &maps.b[p], bar, kb * BK, -p, f0, ai);
-            else tma_load_3d_pair_warp(stage, &maps.b[p], bar, kb * BK, f0 - bank.begin[p], ai);
-            tma_load_2d_pair_warp(stage + W_BYTES, &maps.t, bar, p * bank.wide + kb * BK, (first + i) * tiles.tile_rows + (int)rank * half);
+            if (!enter()) break;
+            const int what = min(r, 4) | (left == 0 ? 256 : 0), column = p * bank.wide + kb * BK, row = (first + i) * tiles.tile_rows + (int)rank * half;
+            if (GATED) stage_4d_2d_warp(to, what, stage, &maps.b[p], kb * BK, -p, f0, ai, stage + W_BYTES, &maps.t, column, row);
+            else stage_3d_2d_warp(to, what, stage, &maps.b[p], kb * BK, f0 - bank.begin[p], ai, stage + W_BYTES, &maps.t, column, row);
           }
       }
     }
