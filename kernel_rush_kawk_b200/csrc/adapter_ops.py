@@ -254,11 +254,14 @@ class AdapterOps:
             self._ok(self.adapt.krk_adapted_gemm(out.data_ptr(), x_at, ldx, w_at, ldw, M, N, K, described, row_adapter, info, slots, n_slots, height, t_at,
                                                  t_at + 4 * t_words if rest else None, shared, int(gated > 0), error, stream), what)
             return out
-        if w.dtype is torch.float32 and M <= self.SKINNY_MAX_ROWS and not gated and not (K | ldx | ldw) & 3 and not (x_at | w_at) & 15:
+        # The second factor behind each sum, by the thread that holds it, up to 256 ranks times rows; more of them go over all SMs in a launch of their own. us,
+        # 2,560 x 6,144, 9,728 x 2,560 and gate and up of 2,560 x 19,456: one row of rank 16 18.5, 36.9 and 45.1 (a launch of its own 24.5, 43.0 and 47.1), eight rows
+        # with eight of rank 32 32.8, 55 and 68 (34.8, 61 and 64), sixteen with nine of rank 32 49, 98 and 121 (45, 98 and 109), of rank 64 64, 104 and 147 (51, 102 and 123).
+        if w.dtype is torch.float32 and M <= self.SKINNY_MAX_ROWS and M * bank.rank <= 256 and not (K | ldx | ldw) & 3 and not (x_at | w_at) & 15:
             self.launches += 1
-            t = self.error.new_empty(M * bank.parts * (-(-bank.rank // 16) * 16))
-            self._ok(self.adapt.krk_adapted_few_f32(out.data_ptr(), x_at, ldx, w_at, ldw, M, N, K, described, row_adapter, t.data_ptr(), error, stream), what)
-            return out
+            t, y = self.error.new_empty(M * bank.parts * (-(-bank.rank // 16) * 16)), x.new_empty(M, N) if gated else out
+            self._ok(self.adapt.krk_adapted_few_f32(y.data_ptr(), x_at, ldx, w_at, ldw, M, N, K, described, row_adapter, t.data_ptr(), error, stream), what)
+            return self.swiglu(y, gated) if gated else out
         # more rows of float32, and sizes, strides and addresses that the tensor cores' copies do not take
         if not x.is_contiguous():
             x = x.contiguous()

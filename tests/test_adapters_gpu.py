@@ -140,7 +140,7 @@ def test_float32_rows_are_the_same_in_any_company(ops):
 
 
 @pytest.mark.parametrize("rows", [1, 2, 5, 9, 16])
-@pytest.mark.parametrize("outs,K,rank", [((96, 40, 7), 36, 3), ((300, 20), 516, 17), ((16400, 33), 64, 8), ((65, 64, 63, 2), 128, 128), ((12300,), 1028, 40)])
+@pytest.mark.parametrize("outs,K,rank", [((96, 40, 7), 36, 3), ((300, 20), 516, 17), ((16400, 33), 64, 8), ((65, 64, 63, 2), 128, 128), ((12300,), 1028, 40), ((70, 41), 260, 16)])
 def test_few_float32_rows(ops, rows, outs, K, rank):
     """Up to sixteen rows in the product's own launch: every way that it splits rows and columns, borders of parts inside it, and the bits of many rows."""
     lengths, of = [1] * rows, spread([1] * rows, 5)
@@ -438,3 +438,16 @@ def test_two_graphs_side_by_side(ops):
     for _, y, expected, *_ in graphs:
         assert torch.equal(y, expected)
     ops.check()
+
+
+@pytest.mark.parametrize("rows", [1, 5, 16])
+@pytest.mark.parametrize("half,K,rank", [(100, 68, 5), (8200, 96, 16), (33, 1000, 64)])
+def test_few_float32_rows_with_gate_and_up(ops, rows, half, K, rank):
+    """And the bits that many rows give."""
+    lengths, of = [1] * rows, spread([1] * rows, 5, 4)
+    x, w, adapters, bank = case(30, torch.float32, K, (half, half), lengths, of, rank, 5, skip={(1, 1)})
+    got = ops.adapted_gate_up_swiglu(x, w, half, bank, rows_of_step(ops, lengths, of, DEV))
+    assert_within(got, *gated64(*product64(x, w, adapters, (half, half), of, True)))
+    more = torch.cat([x, torch.randn((20, K), device=DEV)])
+    many = ops.adapted_gate_up_swiglu(more, w, half, bank, rows_of_step(ops, [1] * (rows + 20), of + [2] * 20, DEV))
+    assert torch.equal(got, many[:rows])
