@@ -29,6 +29,7 @@
 // two sums. Every wait is bounded: one that runs out sets the error word, and the blocks leave after freeing their tensor memory.
 #include "adapters.cuh"
 #include "mma.cuh"
+#include "shares.cuh"
 #include "warp_copies.cuh"
 
 namespace {
@@ -40,7 +41,6 @@ using namespace tc;
 // ---------------------------------------------------------------------------------------------------------------------
 
 constexpr int BK = 64, UMMA_K = 16;
-constexpr int PAIRS = 74;  // of SMs
 constexpr int READERS = 8;  // warps that read accumulators: two to a quarter of tensor memory's lanes
 constexpr int THREADS = 64 + 32 * READERS;
 constexpr uint32_t W_BYTES = 128 * BK * 2;  // a block's half of the pair's weights
@@ -99,59 +99,6 @@ __device__ __forceinline__ void tmem_wait_ld_of(uint32_t (&r)[32]) {
                :
                : "memory");
 }
-
-// The work of a pair: of the tiles before `shared`, tiles pair, pair + pairs, ... as a whole; of the tiles from there on a share. A tile has its blocks of k
-// and, where there is a single row tile, its adapters (else they go to who has the last k). With `aligned` a tile is dealt to so many pairs, blocks and
-// adapters in equal parts; else the blocks and adapters of all tiles, in order, to all pairs, `run` from pair * run on.
-struct Walk {
-  int k_blocks, extra, shared, run, aligned, at, end, whole, pairs;
-  __device__ Walk(int pair, int pairs_, int tiles, int shared_, int k_blocks_, int extra_, int aligned_)
-      : k_blocks(k_blocks_), extra(extra_), shared(shared_), aligned(aligned_), whole(pair), pairs(pairs_) {
-    const int units = k_blocks + extra, all = units * (tiles - shared);
-    if (aligned) {  // tile and part
-      run = 1;
-      at = min(pair, (tiles - shared) * aligned);
-      end = min(pair + 1, (tiles - shared) * aligned);
-    } else {
-      run = max(1, (int)(((long long)all + pairs - 1) / pairs));
-      at = (int)min((long long)pair * run, (long long)all);
-      end = (int)min((long long)at + run, (long long)all);
-    }
-  }
-  // tile t, of which blocks of k from k0 to k1, adapters from e0 to e1
-  __device__ bool next(int& t, int& k0, int& k1, int& e0, int& e1) {
-    if (whole < shared) {
-      t = whole;
-      whole += pairs;
-      k0 = e0 = 0;
-      k1 = k_blocks;
-      e1 = extra;
-      return true;
-    }
-    if (at >= end) return false;
-    if (aligned) {
-      const int part = at % aligned, ks = (k_blocks + aligned - 1) / aligned, es = (extra + aligned - 1) / aligned;
-      t = shared + at / aligned;
-      k0 = min(k_blocks, part * ks);
-      k1 = min(k_blocks, k0 + ks);
-      e0 = min(extra, part * es);
-      e1 = min(extra, e0 + es);
-      at = end;
-      return true;
-    }
-    // from behind: a run begins with what it has of its last tile, whose t it does not need, and waits for t where nothing is left to load but that
-    const int units = k_blocks + extra, of = (end - 1) / units, u1 = end - of * units, u0 = max(0, at - of * units);
-    t = shared + of;
-    k0 = min(k_blocks, u0);
-    k1 = min(k_blocks, u1);
-    e0 = max(0, u0 - k_blocks);
-    e1 = max(0, u1 - k_blocks);
-    end -= u1 - u0;
-    return true;
-  }
-  __device__ int first_pair(int t) const { return aligned ? (t - shared) * aligned : (int)((long long)(t - shared) * (k_blocks + extra) / run); }
-  __device__ int count(int t) const { return aligned ? aligned : (int)(((long long)(t - shared + 1) * (k_blocks + extra) - 1) / run) - first_pair(t) + 1; }
-};
 
 template <bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(512)  // (of 320: 128 registers a thread leave room for a block of the first factor's)
@@ -262,7 +209,7 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
         p0 = part_of(bank, wt * 2 * BC);
         p1 = part_of(bank, min(N, (wt + 1) * 2 * BC) - 1) + 1;
       }
-      if (!extras) e1 = k1 == k_blocks ? count : 0;
+      if (!extras) e1 = walk.ends(k0, k1) ? count : 0;
       // a lane's adapter of the list, and its parts' ranks in steps of 16, a byte each
       int a = -1;
       uint32_t ranks = 0;
@@ -589,13 +536,12 @@ KRK_API int krk_adapted_gemm(void* out, const void* x, long long ldx, const void
   rc = gated ? make_map_bf16_3d(&maps.w, w, K, 2, width, (long long)width * ldw, ldw, 2, 64) : make_map_bf16(&maps.w, w, N, K, ldw, 128);
   if (!rc) rc = make_map_bf16(&maps.t, t, (long long)n_slots * tile_rows, bank->parts * bank->wide, bank->parts * bank->wide, tile_rows / 2);
   for (int p = 0; p < bank->parts && !rc; ++p) rc = make_map_b(&maps.b[p], *bank, p, N, gated);
-  const int rest = (int)(all - shared), most_shares = rest ? (PAIRS + rest - 1) / rest + 1 : 0;
+  const int rest = (int)(all - shared), most_shares = rest ? shares_of_a_tile(rest) : 0;
   int* done = rest ? reinterpret_cast<int*>(shares + (size_t)rest * most_shares * tile_rows * 256) : nullptr;
   if (!rc) rc = krk_first_factor(t, false, done, 2 * rest, x, ldx, K, *bank, tiles, error, stream);
   if (rc) return rc;
   const int pairs = rest || all > PAIRS ? PAIRS : (int)all;
-  // as many pairs a tile, where that leaves few of them idle: fewer shares, and no pair has two
-  const int aligned = rest && rest * (PAIRS / rest) * 10 >= PAIRS * 9 ? min(PAIRS / rest, k_blocks) : 0;
+  const int aligned = rest ? aligned_parts(rest, k_blocks) : 0;
   return gated ? launch_gemm<true>(maps, (bf16*)out, shares, done, shared, most_shares, aligned, width, K, *bank, tiles, pairs, error, stream)
                : launch_gemm<false>(maps, (bf16*)out, shares, done, shared, most_shares, aligned, width, K, *bank, tiles, pairs, error, stream);
 }

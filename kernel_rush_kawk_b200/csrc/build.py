@@ -47,7 +47,7 @@ PARTS_SOURCES = ["partial_attention.cu", "few_rows_attention.cu", "many_rows_att
 LATENT_SOURCES = ["latent_prefill.cu"]
 ATTN_SOURCES = ["attention_simple.cu", "attention_mma.cu", "attention_tcgen05.cu"]
 HEADERS = ["common.cuh", "mma.cuh", "tcgen05.cuh", "attention_noalloc.h", "attention_tiles.cuh", "partial_attention.cuh"]
-OWN_HEADERS = {"core": ["skinny.cuh", "few_f32.cuh"], "adapt": ["skinny.cuh", "few_f32.cuh", "adapters.cuh", "warp_copies.cuh"]}
+OWN_HEADERS = {"core": ["skinny.cuh", "few_f32.cuh"], "adapt": ["skinny.cuh", "few_f32.cuh", "adapters.cuh", "shares.cuh", "warp_copies.cuh"]}
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
