@@ -26,6 +26,27 @@ __device__ __forceinline__ void umma_stage_warp(uint32_t tmem_d, uint64_t a_desc
       : "memory");
 }
 
+// The slot of block `index` of n, and what it holds. Of a single tile there are as many blocks as the bank has adapters, which may be fewer than slots. Where the tile
+// has more adapters than that, some are none of the bank's and may stand before those that are: the blocks take the latter, in order.
+__device__ __forceinline__ int2 take_slot(const AdapterTiles& tiles, int capacity, int index, int n, int& slot) {
+  const int2* slots = reinterpret_cast<const int2*>(tiles.slots);
+  const int count = tiles.info[1];
+  slot = index;
+  int2 is = slots[index];
+  if (count > n) {
+    is.x = -1;
+    for (int s = 0; s < count; ++s) {
+      const int2 other = slots[s];
+      if ((unsigned)other.x < (unsigned)capacity && index-- == 0) {
+        slot = s;
+        is = other;
+        break;
+      }
+    }
+  }
+  return is;
+}
+
 // The first factor of many requests' adapters, t = scale (x A^T), sums in 32 bits on the tensor cores, rounded to bfloat16 (half a step of 2^-8 of a sum that is itself
 // a part of the result, which is rounded the same way). t is of every slot,
 // [slot][tile_rows][parts * wide], zeros where a row has another adapter than the slot's.
@@ -60,7 +81,7 @@ first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_do
   __shared__ uint64_t full_bar[FIRST_STAGES], empty_bar[FIRST_STAGES], acc_bar;
   __shared__ uint32_t tmem_slot;
   __shared__ int asked_for;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = blockIdx.x % ways, slot = blockIdx.x / ways;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = blockIdx.x % ways;
   if (ways > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // "I have started"
   grid_dependency_wait();
   // Tensor memory is taken before the product's blocks are let in, which take what is left and wait for what these make. They are let in here, since
@@ -80,7 +101,8 @@ first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_do
   };
   if (blockIdx.x + blockIdx.y + blockIdx.z == 0)
     for (int i = threadIdx.x; i < n_done; i += FIRST_THREADS) done[i] = 0;  // the product's counts of shares
-  const int2 is = *reinterpret_cast<const int2*>(tiles.slots + 2 * slot);
+  int slot;
+  const int2 is = take_slot(tiles, bank.capacity, blockIdx.x / ways, gridDim.x / ways, slot);
   const int a = is.x, r0 = is.y * tiles.tile_rows + blockIdx.y * 128;
   if (a < 0 || a >= bank.capacity) return leave();  // the whole cluster (the product says so)
   const int here = min(128, min(tiles.tile_rows - (int)blockIdx.y * 128, tiles.rows - r0));  // rows
@@ -217,7 +239,8 @@ first_factor_few_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_done
   grid_launch_dependents();
   if (blockIdx.x + blockIdx.y == 0)
     for (int i = tid; i < n_done; i += 32 * WARPS) done[i] = 0;
-  const int slot = blockIdx.y, a = tiles.slots[2 * slot], rows = min(tiles.rows, tiles.tile_rows);
+  int slot;
+  const int a = take_slot(tiles, bank.capacity, blockIdx.y, gridDim.y, slot).x, rows = min(tiles.rows, tiles.tile_rows);
   if (a < 0 || a >= bank.capacity) return;  // (the product says so)
   if (warp == 0) {
     int n = 0;
