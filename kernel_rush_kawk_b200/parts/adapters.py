@@ -8,7 +8,6 @@ queries, keys and values) in fixed storage, so that variants come and go while c
 
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass
 
 import torch
@@ -89,7 +88,8 @@ class AdapterBank:
         if not 1 <= a.shape[0] <= self.most:
             raise AdapterError(f"an adapter of rank {a.shape[0]} in a bank of rank {self.most}")
         # rows of other adapters are multiplied by these factors as well, as zeros, and are to stay numbers
-        if not math.isfinite(scale) or not all(torch.isfinite(t.detach().to(self.dtype)).all() for t in (a, b)):
+        # (the scale is held in 32 bits)
+        if not abs(scale) <= torch.finfo(torch.float32).max or not all(torch.isfinite(t.detach().to(self.dtype)).all() for t in (a, b)):
             raise AdapterError(f"an adapter's factors and scale are finite numbers ({self.dtype})")
 
     @torch.no_grad()
