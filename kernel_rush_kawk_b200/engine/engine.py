@@ -204,6 +204,7 @@ class Engine:
             if not free:
                 raise AdapterError(f"no room for adapter '{name}': {self.adapter_room.count} are held ({', '.join(sorted(self.adapters))})")
             index = free[0]
+        self.adapters.pop(name, None)  # until all of it is there
         for bank in {id(bank): bank for bank, _ in self._beside.values()}.values():
             bank.clear(index)
         for weight, (a, b, s) in factors.items():
