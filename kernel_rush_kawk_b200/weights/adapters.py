@@ -3,7 +3,7 @@
 A folder holds ``adapter_config.json`` (``r`` and ``lora_alpha``: the scale is alpha / r, or alpha / sqrt(r) with
 ``use_rslora``) and safetensors with two tensors for each weight: ``<module>.lora_A.weight`` [r, inputs] and
 ``<module>.lora_B.weight`` [outputs, r], where ``<module>.weight`` is the weight's name in the checkpoint (a leading
-``base_model.model.`` is dropped). An adapter's tensors may have ranks of their own; the scale then goes by each one's.
+``base_model.model.`` is dropped). Adapters that are more than these products, or beside weights changed for them, are refused. An adapter's tensors may have ranks of their own; the scale then goes by each one's.
 """
 
 from __future__ import annotations
@@ -27,9 +27,15 @@ def read_adapter(folder) -> dict[str, tuple[torch.Tensor, torch.Tensor, float]]:
         alpha = float(config["lora_alpha"])
     except (OSError, ValueError, KeyError, TypeError) as e:
         raise AdapterError(f"{folder}: adapter_config.json with a lora_alpha is asked for ({e})") from e
-    for key in ("alpha_pattern", "modules_to_save", "use_dora", "fan_in_fan_out"):
+    for key in ("alpha_pattern", "modules_to_save", "use_dora", "fan_in_fan_out", "use_qalora", "alora_invocation_tokens", "layer_replication", "lora_bias",
+                "trainable_token_indices"):
         if config.get(key):
             raise AdapterError(f"{folder}: adapters with {key} are not taken")
+    if config.get("peft_type", "LORA") != "LORA":
+        raise AdapterError(f"{folder}: adapters of the type {config['peft_type']} are not taken")
+    # beginnings that leave the weights as they are; others take a product out of them, and the factors then belong to what is left
+    if config.get("init_lora_weights") not in (None, True, False, "gaussian", "eva", "orthogonal"):
+        raise AdapterError(f"{folder}: adapters that began with '{config['init_lora_weights']}' belong to changed weights and are not taken")
     if config.get("bias", "none") != "none":
         raise AdapterError(f"{folder}: adapters with biases are not taken")
     shards = sorted(folder.glob("*.safetensors"))

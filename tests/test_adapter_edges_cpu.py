@@ -3,9 +3,10 @@
 import pytest
 import torch
 
-from adapter_helpers import random_factors
+from adapter_helpers import random_factors, write_adapter
 from helpers import prompts_for
 from kernel_rush_kawk_b200.parts.adapters import AdapterBank, AdapterError
+from kernel_rush_kawk_b200.weights.adapters import read_adapter
 from test_adapted_engine_cpu import NAME, make, plain_of
 
 
@@ -49,3 +50,17 @@ def test_an_adapter_that_is_not_all_there_has_no_name(folders, monkeypatch):
     other = make(folders)
     other.load_adapter("x", new)
     assert engine.generate_all(prompt, 4, adapters="a") == other.generate_all(prompt, 4, adapters="x")
+
+
+def test_files_of_more_than_products(tmp_path):
+    """Adapters whose weights are changed for them, or that do not run on every token, would be taken for others."""
+    factors = {"model.layers.0.mlp.down_proj.weight": (torch.randn(3, 8), torch.randn(6, 3), 1.0)}
+    refused = [dict(init_lora_weights=v) for v in ("pissa", "pissa_niter_16", "olora", "loftq", "corda")] + [
+        dict(alora_invocation_tokens=[7, 8]), dict(layer_replication=[[0, 2]]), dict(use_qalora=True), dict(lora_bias=True), dict(trainable_token_indices=[1]),
+        dict(peft_type="LOHA")]
+    for i, config in enumerate(refused):
+        with pytest.raises(AdapterError, match="not taken"):
+            read_adapter(write_adapter(tmp_path / f"r{i}", factors, **config))
+    for i, config in enumerate([dict(init_lora_weights=v) for v in (True, False, None, "gaussian", "eva", "orthogonal")] + [
+            dict(peft_type="LORA", use_qalora=False, alora_invocation_tokens=None, layer_replication=None, lora_bias=False, trainable_token_indices=None)]):
+        assert set(read_adapter(write_adapter(tmp_path / f"t{i}", factors, **config))) == set(factors)
