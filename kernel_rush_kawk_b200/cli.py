@@ -117,8 +117,12 @@ def main(argv=None) -> int:
         parser.error("--use-adapter goes with --adapter")
     if args.adapter:
         from .weights.adapters import read_adapter
+        given = [a.partition("=") for a in args.adapter]
+        names = [name for name, _, _ in given]
+        if not all(name and folder for name, _, folder in given) or "-" in names or len(set(names)) < len(names):
+            parser.error(f"--adapter is NAME=DIR, each with a name of its own other than '-'; got {', '.join(args.adapter)}")
         try:
-            loaded = {name: read_adapter(folder) for name, eq, folder in (a.partition("=") for a in args.adapter)}
+            loaded = {name: read_adapter(folder) for name, _, folder in given}
             options["adapters"] = AdapterRoom(len(loaded), max(a.shape[0] for factors in loaded.values() for a, _, _ in factors.values()))
         except (AdapterError, ValueError) as e:
             parser.error(str(e))

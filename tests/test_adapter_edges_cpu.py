@@ -64,3 +64,15 @@ def test_files_of_more_than_products(tmp_path):
     for i, config in enumerate([dict(init_lora_weights=v) for v in (True, False, None, "gaussian", "eva", "orthogonal")] + [
             dict(peft_type="LORA", use_qalora=False, alora_invocation_tokens=None, layer_replication=None, lora_bias=False, trainable_token_indices=None)]):
         assert set(read_adapter(write_adapter(tmp_path / f"t{i}", factors, **config))) == set(factors)
+
+
+@pytest.mark.parametrize("given", [["{0}"], ["{0}="], ["=x"], ["-={0}"], ["x={0}", "x={0}"], ["x={0}", "y"]])
+def test_command_line_adapters_have_a_name_and_a_folder(folders, tmp_path, capsys, monkeypatch, given):
+    """Without a folder the current one would be read; of one name given twice, or of '-', one adapter could not be asked for."""
+    from kernel_rush_kawk_b200.cli import main
+
+    folder = write_adapter(tmp_path / "a", {"model.layers.0.mlp.down_proj.weight": (torch.randn(3, 8), torch.randn(6, 3), 1.0)})
+    monkeypatch.chdir(folder)
+    with pytest.raises(SystemExit):
+        main(["generate", "--model", str(folders[NAME]), "--prompt-ids", "1,2"] + ["--adapter=" + a.format(folder) for a in given])
+    assert "NAME=DIR" in capsys.readouterr().err.splitlines()[-1]
