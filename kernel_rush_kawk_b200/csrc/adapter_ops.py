@@ -121,8 +121,8 @@ class AdapterOps:
         tokens need beyond are taken from ``pages`` (int32), in the order of the sequences, and entered. ``adapters`` (int32, one a
         sequence, -1 for none): its low-rank adapter. ``out``: a StepMaps to fill again (a captured step goes on reading it). No two sequences may have one slot.
 
-        Lengths that do not add up to ``n_rows``, slots that the table does not have, and sequences that outgrow it or the given pages are
-        found on the device: the error word is set (``check`` raises), and the rows concerned have position or place -1."""
+        Lengths that do not add up to ``n_rows``, slots that the table does not have, sequences that outgrow it or the given pages, and pages that a sequence
+        holds and the table lacks (entries below 0) are found on the device: the error word is set (``check`` raises), and the rows concerned have position or place -1."""
         what, n, n_rows = "maps of a step", lengths.shape[0], int(n_rows)
         if not 0 <= n_rows <= self.MOST_ROWS or n > self.MOST_SEQUENCES:
             raise KernelError(f"{what}: {n} sequences with {n_rows} rows (up to {self.MOST_SEQUENCES} sequences and {self.MOST_ROWS} rows are taken)")

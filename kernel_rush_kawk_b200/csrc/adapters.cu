@@ -131,6 +131,7 @@ __global__ void __launch_bounds__(MAP_THREADS) step_maps_kernel(const Maps m) {
           int at;
           if (b < have) {
             at = *entry;
+            bad |= at < 0;
           } else {
             const long long i = fresh[seq] + (b - have);
             at = i < m.n_pages ? m.pages[i] : -1;
