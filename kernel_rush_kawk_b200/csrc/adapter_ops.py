@@ -69,7 +69,7 @@ class AdapterRows:
 
 class StepMaps:
     """What ``Kernels.step_maps`` makes: ``cu_q`` [sequences + 1], the first row of every sequence; ``row_seq``, ``row_pos`` [rows], a row's sequence and
-    position; with a page table ``row_place`` [rows] (int64), its place in the cache, page * 64 + position in the page; ``adapters`` (AdapterRows or None).
+    position; with a page table ``row_place`` [rows] (int64), its place in the cache, page * 64 + position in the page (-1 where maps with room for places are filled without a table); ``adapters`` (AdapterRows or None).
     All are views of one buffer."""
 
     def __init__(self, n_rows: int, n_seqs: int, device, with_places: bool = True, with_adapters: bool = True):

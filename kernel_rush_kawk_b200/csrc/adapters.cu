@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(256) second_factor_kernel(T* __restrict__ out,
 }  // namespace
 
 // The maps of a step of n_seqs sequences and n_rows rows. Optional: adapters, table (with slots and pages, of which n_pages are given). `words` takes, in order:
-// with `places` row_place (two words a row); cu [n_seqs + 1], row_seq and row_pos [n_rows]; with adapters, on a boundary of two words each, row_adapter [n_rows], and for
+// with `places` row_place (two words a row, -1 without a table); cu [n_seqs + 1], row_seq and row_pos [n_rows]; with adapters, on a boundary of two words each, row_adapter [n_rows], and for
 // tiles of 128, 192 and 256 rows, or of all rows up to a multiple of 32 where there are no more than 256, a tile's first slot and number of adapters, and the
 // slots, one for each tile and sequence: an adapter and its tile.
 KRK_API int krk_step_maps(const int* slots, const int* starts, const int* lengths, const int* adapters, int n_seqs, int n_rows, int* table, int width, int n_slots,
@@ -351,7 +351,7 @@ KRK_API int krk_step_maps(const int* slots, const int* starts, const int* length
   Maps m = {slots, starts, lengths, adapters, n_seqs, n_rows, table, width, n_slots, pages, n_pages};
   int* const first = words;
   if (places) {
-    m.row_place = table ? reinterpret_cast<long long*>(words) : nullptr;
+    m.row_place = reinterpret_cast<long long*>(words);
     words += 2 * (size_t)n_rows;
   }
   m.cu = words;

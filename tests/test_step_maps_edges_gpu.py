@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from kernel_rush_kawk_b200.csrc import KernelError, load_kernels
+from kernel_rush_kawk_b200.csrc.adapter_ops import StepMaps
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -31,4 +32,18 @@ def test_a_held_page_that_the_table_lacks(ops, lengths):
     on_it = [p < 128 for p in range(70, 70 + lengths[0])]
     place = maps.row_place.tolist()
     assert all((place[r] == -1) == lost for r, lost in enumerate(on_it)) and all(v >= 0 for v in place[lengths[0]:])
+    ops.check()
+
+
+@pytest.mark.parametrize("n", [1, 900])
+def test_places_without_a_table(ops, n):
+    """Maps that are filled again without a table keep no places of the step before."""
+    maps = StepMaps(n + 2, 2, DEV, with_adapters=False)
+    maps.buffer.fill_(77)
+    args = ints([0, 1]), ints([64, 3]), ints([n, 2]), n + 2
+    table = torch.arange(40, dtype=torch.int32, device=DEV).view(2, 20).contiguous()
+    ops.step_maps(*args, table=table, pages=ints(list(range(50, 70))), out=maps)
+    assert maps.row_place.ge(0).all()
+    ops.step_maps(*args, out=maps)
+    assert maps.row_place.eq(-1).all() and maps.row_pos.tolist() == list(range(64, 64 + n)) + [3, 4]
     ops.check()
