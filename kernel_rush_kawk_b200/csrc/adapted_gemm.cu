@@ -525,9 +525,9 @@ KRK_API int krk_adapted_gemm(void* out, const void* x, long long ldx, const void
       (((uintptr_t)x | (uintptr_t)w | (uintptr_t)out | (uintptr_t)bank->a | (uintptr_t)bank->b | (uintptr_t)t | (uintptr_t)shares) & 15))
     return -2;
   const AdapterTiles tiles = {row_adapter, info, slots, rows, tile_rows, n_slots};
-  const long long all = (long long)((rows + tile_rows - 1) / tile_rows) * ((N + 255) / 256);
-  const int k_blocks = (K + BK - 1) / BK;
-  if (all * (k_blocks + n_slots) > 0x7fffffffLL || (long long)n_slots * tile_rows > 0x7fffffffLL)
+  const int k_blocks = (K + BK - 1) / BK, row_tiles = (rows + tile_rows - 1) / tile_rows;
+  const long long all = (long long)row_tiles * ((N + 255) / 256);
+  if (all * (k_blocks + (row_tiles == 1 ? n_slots : 0)) > 0x7fffffffLL || (long long)n_slots * tile_rows > 0x7fffffffLL)  // (adapters are dealt out of a single row tile alone)
     return -3;
   if (shared < 0 || shared > all || (shared < all && (shared % PAIRS || !shares))) return -2;
   Maps maps;
