@@ -26,15 +26,23 @@ struct Unit {
   int row0, n_tok, key_lo, key_hi, slot, start;
 };
 
-__device__ __forceinline__ Unit prefix_unit(const Segments& s, int group) {
+// A group's keys, which its prefix's earlier steps wrote and copies describe; and its rows, which a kernel of this step may have counted (cu_q).
+__device__ __forceinline__ Unit prefix_keys(const Segments& s, int group) {
   Unit u;
+  u.row0 = u.n_tok = u.key_lo = 0;
+  u.key_hi = min(s.group_len[group], s.width * KRK_PAGE);  // no page beyond a slot's
+  u.slot = s.seq_slot[s.group_cu[group]];
+  u.start = 0x3fffffff;  // every key of the prefix lies before every row
+  return u;
+}
+__device__ __forceinline__ void add_rows(Unit& u, const Segments& s, int group) {
   const int first = s.group_cu[group], last = s.group_cu[group + 1];
   u.row0 = s.cu_q[first];
   u.n_tok = s.cu_q[last] - u.row0;
-  u.key_lo = 0;
-  u.key_hi = min(s.group_len[group], s.width * KRK_PAGE);  // no page beyond a slot's
-  u.slot = s.seq_slot[first];
-  u.start = 0x3fffffff;  // every key of the prefix lies before every row
+}
+__device__ __forceinline__ Unit prefix_unit(const Segments& s, int group) {
+  Unit u = prefix_keys(s, group);
+  add_rows(u, s, group);
   return u;
 }
 

@@ -82,12 +82,11 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + 2 * TILE_BYTES);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
 
-  // Groups, slots and page tables are written by copies and by kernels that no later one overtakes: read before the wait for the kernel that
-  // writes the rows.
+  // Groups and slots are written by copies, the prefix's pages were entered in earlier steps, whose attention no later kernel overtook: read before the wait for
+  // the kernel that writes the rows. Where a sequence's rows begin may be worked out by a kernel of this very step that lets later ones start at once: behind it.
   const int kh = blockIdx.x % HKV, split = blockIdx.x / HKV % n_splits, pair = blockIdx.x / HKV / n_splits;
   const int G = HQ / HKV;
-  const Unit u = prefix_unit(seg, blockIdx.y);
-  const int n_rows = u.n_tok * G, pair_row = pair * 2 * rows;
+  Unit u = prefix_keys(seg, blockIdx.y);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (a number that the compiler knows to be the warp's)
   int p_lo, p_hi;
   split_pages(0, u.key_hi, split, n_splits, p_lo, p_hi);
@@ -99,6 +98,8 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     for (int p = 0; p < 4; ++p) first_pages[p] = page_row(p);
   grid_dependency_wait();
   grid_launch_dependents();  // in this order: the next kernel reads rows and keys before it waits for the parts
+  add_rows(u, seg, blockIdx.y);
+  const int n_rows = u.n_tok * G, pair_row = pair * 2 * rows;
   if (pair_row >= n_rows) return;
   const int tiles = halves || pair_row + rows < n_rows ? 2 : 1;
   // tile t's rows start at tile_row(t), its j-th step is block_of(t, j) of the share's n blocks of 128 keys, and it has steps(t) of them
