@@ -1,6 +1,6 @@
 // The float32 product of up to 16 rows (few_f32.cuh) with the rows' low-rank adapters: t is made by a launch that the weights' copies begin beside, and a thread
 // adds the second factor to the sum that it holds. The result has the bits of the three launches that more rows take (adapters.cu).
-// Bound as the product alone is, by its chains of multiply-adds and the weights' bytes: six rows of 2,560 x 6,144, four adapters of rank 8, cold and replayed 22.5 to 24.5
+// Bound as the product alone is, which takes twice its bytes' time there (its chains of 2,560 multiply-adds at four clocks are 5 us of it): six rows of 2,560 x 6,144, four adapters of rank 8, cold and replayed 22.5 to 24.5
 // us (the product alone 22.5; 64 MB, 9.8 us), a call 18.6 where three launches took 28.7.
 #include <climits>
 

@@ -429,6 +429,9 @@ adapted_gemm_kernel(const __grid_constant__ Maps maps, bf16* __restrict__ out, f
                 const float a = __uint_as_float(w[j + i]), b = __uint_as_float(w[j + 2 + i]);
                 const float got = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
                 const float gate = odd ? got : a, up = odd ? b : got;
+                // By the fast exponential and quotient, good to 2^-17 (of gates below -87, whose products are below 2^-119 of up, nothing is left); half a step of the
+                // result is 2^-8. By expf and a division, which shares have the time for: 3,963 rows of 2,560 x 19,456 278.6 -> 282.6 us cold, 512 rows 61.5 -> 64, 200
+                // rows 47 -> 53, 4,000 rows of 320 x 8,192 53 -> 73.
                 z[i] = __fdividef(gate, 1.0f + __expf(-gate)) * up;
               }
               words[(j / 2 + (odd ? 1 : 0)) * PATCH_PITCH + (lane >> 1)] = pack_bf16x2(z[0], z[1]);

@@ -188,7 +188,8 @@ class AdapterOps:
     def adapted_linear(self, x, w, bank, rows):
         """y = x W^T + s (x A^T) B^T, A, B and s those of each row's adapter: x [rows, inputs], w [outputs, inputs], ``bank`` (parts.adapters.AdapterBank)
         the adapters, ``rows`` (AdapterRows) which row has which. Any number of rows, float32 or bfloat16; sums are held in
-        32 bits and rounded once. A float32 row gives the same bits whatever stands beside it. Rows without an adapter give x W^T."""
+        32 bits and rounded once. Scratch of more than 16 bfloat16 rows: their tiles' height times tiles and sequences times parts times the rank, 16 bits each
+        (a thousand sequences of one token, rank 64, three parts: 99 MB; 25,000, rank 16: 0.6 GB). A float32 row gives the same bits whatever stands beside it. Rows without an adapter give x W^T."""
         return self._adapted("adapted product", self._resolve(x), w, bank, rows, 0)
 
     def adapted_gate_up_swiglu(self, x, w_gate_up, intermediate, bank, rows):
@@ -209,7 +210,7 @@ class AdapterOps:
 
         Above, a round takes what a block of k takes of a pair, 380 clocks and half a clock a row, and shares take the way to memory and back, as many times as
         a tile has pairs; a row tile takes its first factor. The constants come from six shapes (K and N of 2,560 to 9,728 and 19,456), 160 to 4,096 rows, every
-        height with shares and without: what this picks is 0.5 % behind the fastest on average, 8 % at worst. Cold, us, whole and shares: 256 rows of 2,560 x
+        height with shares and without: what this picks is 0.4 % behind the fastest on average, 8 % at worst. Cold, us, whole and shares: 256 rows of 2,560 x
         6,144 27.3 and 32.8, of 9,728 x 2,560 57.3 and 45.1; 2,268 rows of that, tiles of 256, 124.9 and 110.6; 400 rows of 2,560 x 6,144 in tiles of 256 26.6 and
         38.9, of 192 30.7, of 128 38.9; 512 rows of 2,560 x 19,456 61.4 and 86."""
         if len(heights) == 1 and heights[0] <= 128:

@@ -224,7 +224,7 @@ first_factor_tiles_kernel(bf16* __restrict__ t, int* __restrict__ done, int n_do
 // adapter's rows, wherever they are, its N. The warps' sums are added in order: a sum's order depends on K alone.
 //
 // COMPACT: t of every row, for up to 16 rows (the tiles' form served these before: 16 rows with nine adapters of rank 16, the product with it, cold, 9,728 x 2,560 24.6 us
-// and 20.5 here, 4,096 x 2,560 18.4 and 16.4; one row of 2,560 x 6,144 14.3 and 14.3; sixteen adapters of rank 64 beside 4,096 x 24,576 61 and 65). By eight
+// and 20.5 here, 4,096 x 2,560 18.4 and 16.4; one row of 2,560 x 6,144 14.3 and 12.3 to 14.4, the timer's steps being 2; sixteen adapters of rank 64 beside 4,096 x 24,576 61 and 65). By eight
 // warps a long k takes more rounds of loads: one row of 9,728 x 2,560 22.5, by sixteen 18.4.
 constexpr int FEW_DEEP = 5, FEW_RANKS = 16;
 
@@ -337,6 +337,7 @@ int launch_first(bf16* t, int* done, int n_done, const CUtensorMap& map_x, const
   const int parts = (min(tiles.tile_rows, tiles.rows) + 127) / 128, chunks = (ranks + box_ranks - 1) / box_ranks;
   // Blocks that share k: of a single tile, whose adapters are in the first slots, as the SMs take one of; of many tiles, of whose slots some third
   // is not used, six at most (clusters of eight leave an eighth of the SMs without one).
+  // (By the bank's room: 64 rows of one adapter, 9,728 x 2,560, 28.7 us in a bank of one, 30.8 of 24 and 41 of 64.)
   const int slots = row_tiles == 1 ? min(tiles.n_slots, bank.capacity) : tiles.n_slots;
   const long long blocks = (long long)slots * parts * chunks;
   const int most = row_tiles == 1 ? 8 : 6;
@@ -376,7 +377,9 @@ int krk_first_factor(void* t, bool compact, int* done, int n_done, const void* x
   if (compact) return launch_few<true, 16>((bf16*)t, done, n_done, (const bf16*)x, ldx, K, bank, tiles, stream);
   // A tile of more than 128 rows with many slots, which blocks of the other kernel would take all of an SM's memory for, the product's blocks behind them: 256 rows of
   // 9,728 x 2,560 with 120 adapters of rank 16 105 us cold, 61 here; 32 adapters 57 and 55, of 2,560 x 6,144 45 and 37; 160 rows with 64 of rank 64 70 and
-  // 53, of 4,096 x 2,560 55 and 64; with eight adapters, of 9,728 x 2,560, 49 and 59.
+  // 53, of 4,096 x 2,560 55 and 64; with eight adapters, of 9,728 x 2,560, 49 and 59. These banks held what the step used. The rule goes by the bank's room, since which
+  // adapters a step has is known on the device alone, and loses where few of them have many rows each: 200 rows of one adapter of 9,728 x 2,560 43 in a bank of one, 45 of
+  // 23, and 172 of 24 or more; of eight adapters 51 and 59.
   if (tiles.rows <= tiles.tile_rows && tiles.tile_rows > 128 && min(tiles.n_slots, bank.capacity) >= 24)
     return launch_few<false, 8>((bf16*)t, done, n_done, (const bf16*)x, ldx, K, bank, tiles, stream);
   CUtensorMap map_x, map_a;
