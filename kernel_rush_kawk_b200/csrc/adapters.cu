@@ -45,8 +45,7 @@ __global__ void __launch_bounds__(MAP_THREADS) step_maps_kernel(const Maps m) {
   __shared__ long long warp_rows[MAP_THREADS / 32], warp_pages[MAP_THREADS / 32];
   __shared__ int found[MAP_THREADS / 32][256];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  grid_launch_dependents();
-  grid_dependency_wait();
+  grid_dependency_wait();  // (and no later kernel is let in: some read a step's description and page table before they wait for the one before)
   // lengths and new pages of all sequences, added up: a thread's run of sequences, the threads' sums, the runs again
   const int each = (m.n_seqs + MAP_THREADS - 1) / MAP_THREADS, s0 = min(tid * each, m.n_seqs), s1 = min(s0 + each, m.n_seqs);
   long long rows = 0, pages = 0;

@@ -83,7 +83,7 @@ prefix_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
 
   // Groups and slots are written by copies, the prefix's pages were entered in earlier steps, whose attention no later kernel overtook: read before the wait for
-  // the kernel that writes the rows. Where a sequence's rows begin may be worked out by a kernel of this very step that lets later ones start at once: behind it.
+  // the kernel that writes the rows. Where a sequence's rows begin may be worked out by a kernel of this very step: behind it.
   const int kh = blockIdx.x % HKV, split = blockIdx.x / HKV % n_splits, pair = blockIdx.x / HKV / n_splits;
   const int G = HQ / HKV;
   Unit u = prefix_keys(seg, blockIdx.y);

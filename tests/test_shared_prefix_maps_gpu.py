@@ -67,3 +67,54 @@ def test_right_behind_the_maps(ops, heads, kv, dim, sizes, lengths, tokens, capt
             y = step()
         assert torch.equal(y, expected)
     ops.check()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [1, 5, 64])
+def test_single_tokens_right_behind_the_maps(ops, n, dim, captured):
+    """Attention of tokens whose pages the maps have just entered."""
+    heads, kv = 8, 2
+    held = [64 * (i % 5) if i % 2 == 0 else 17 * i % 300 for i in range(n)]
+    qkv, batch, cache = make_step(DEV, torch.bfloat16, heads, kv, dim, held, [1] * n, seed=4)
+    cache.k.nan_to_num_(0)
+    cache.v.nan_to_num_(0)
+    wanted = cache.table.clone()
+    table, k, v = cache.table, cache.k.clone(), cache.v.clone()
+    fresh = [(s, h // 64) for s, h in zip(batch.slots, held) if h % 64 == 0]
+    pages = torch.tensor([int(wanted[at]) for at in fresh], dtype=torch.int32, device=DEV)
+    stale = wanted.clone()
+    for at in fresh:
+        stale[at] = 0  # some page, for who reads too early
+    attend = lambda: ops.rope_attention(qkv, heads, kv, dim, None, None, 1e-6, None, None, batch, cache, dim ** -0.5, None)
+    expected = attend().clone()
+    after = cache.k.clone(), cache.v.clone()
+    maps = StepMaps(n, n, DEV, with_adapters=False)
+
+    def step():
+        ops.step_maps(batch.seq_slot, batch.seq_start, batch.seq_qlen, n, table=table, pages=pages, out=maps)
+        return attend()
+
+    def before():
+        table.copy_(stale)
+        cache.k.copy_(k)
+        cache.v.copy_(v)
+
+    if captured:
+        before()
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = step()
+    busy = torch.randn((8192, 8192), device=DEV, dtype=torch.bfloat16)
+    for _ in range(10):
+        before()
+        busy @ busy
+        if captured:
+            graph.replay()
+        else:
+            y = step()
+        assert torch.equal(y, expected) and torch.equal(table, wanted)
+        assert torch.equal(cache.k, after[0]) and torch.equal(cache.v, after[1])
+    ops.check()

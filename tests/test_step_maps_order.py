@@ -1,4 +1,4 @@
-"""What a step's maps are read for must wait for them: they are made by a kernel that lets the next ones start at once (no GPU)."""
+"""Kernels start beside the ones before them: what reads a step's maps must not do so before they are made (no GPU)."""
 
 import re
 
@@ -46,6 +46,15 @@ def test_the_first_factor_waits_before_it_lets_the_product_in(name):
     """The products read a step's maps and rows before they wait: by then all that was before the first factor is over."""
     (body,) = [body for _, n, body in ALL if n == name]
     assert body.index("grid_dependency_wait") < body.index("grid_launch_dependents")
+
+
+def test_no_kernel_overtakes_the_maps():
+    """The attention of single tokens reads positions, slots and the page table before it waits, as copies leave them: the kernel that makes maps and enters
+    pages lets none in, like those that select tokens and move a step on."""
+    (body,) = [body for _, n, body in ALL if n == "step_maps_kernel"]
+    assert "grid_launch_dependents" not in body
+    (select,) = [body for _, n, body in ALL if n == "select_finish_kernel"]
+    assert "grid_launch_dependents" not in select
 
 
 def test_there_are_kernels():
